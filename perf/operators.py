@@ -231,7 +231,7 @@ def _clip_plain(s):
 
 
 def _clip_own(s):
-    return [s["set"].clip(s["case"]["max_norm"], out=s["out_views"]), s["out"]]
+    return [s["set"].clip(s["case"]["max_norm"]), s["out"]]
 
 
 def _adam_plain(s):
@@ -282,7 +282,7 @@ def prepare(case, seed):
         if own:
             from oxibonsai_b200 import training
 
-            s["set"], s["out_views"] = training.GradientSet(_views(grads, places)), training.GradientSet(_views(out, places))
+            s["set"] = training.GradientSet(_views(grads, places), out=_views(out, places))
         return s
     places, grads, params, m, v = _adam_inputs(case, seed)
     s = dict(case=case, grads=grads, params=params, m=m, v=v, step=0)
