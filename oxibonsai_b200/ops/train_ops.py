@@ -1,0 +1,124 @@
+"""Torch-facing wrappers of the training kernels in ``libbonsai_cuda.so`` (csrc/cuda/multi_tensor.cu, linear_ce.cu).
+
+Every function launches on torch's current stream of the tensors' device.  As in :mod:`cuda_ops` there is no PyTorch fallback:
+CUDA tensors go through the kernels, and a missing library raises.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Sequence
+
+import torch
+
+from . import cuda_ops as K
+
+_vp, _i, _d, _ll = C.c_void_p, C.c_int, C.c_double, C.c_longlong
+_SIG = {
+    "bonsai_mt_partials": [_i],
+    "bonsai_mt_norm": [_i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "bonsai_mt_clip": [_i, _vp, _vp, _vp, _vp, _vp, _d, _vp, _vp, _vp],
+    "bonsai_ce_workspace": [_i, _i, _i, _i, _i, _i, _i],
+    "bonsai_ce_forward": [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _ll, _i, C.c_float, _vp, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_ce_backward": [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_mt_adam": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _d, _vp, _d, _d, _d, _d, _i, _vp, _d, _vp, _vp, _vp],
+}
+_declared = False
+TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _lib():
+    global _declared
+    l = K.lib()
+    if not _declared:
+        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_workspace": _ll})
+        _declared = True
+    return l
+
+
+# ---- many tensors ---------------------------------------------------------------------------------------------------------------
+class TensorTable:
+    """Addresses, sizes and types of dense CUDA tensors of one device, packed for the kernels.  Tensors without values are left out."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        live = [t for t in tensors if t.numel()]
+        self.n = len(live)
+        self.ptrs = (C.c_void_p * max(1, self.n))(*[t.data_ptr() for t in live])
+        self.numel = (C.c_longlong * max(1, self.n))(*[t.numel() for t in live])
+        self.types = (C.c_ubyte * max(1, self.n))(*[TYPE_CODES[t.dtype] for t in live])
+        self.partials = int(_lib().bonsai_mt_partials(self.n))
+
+
+def mt_norm(grads: TensorTable, device: torch.device) -> torch.Tensor:
+    """The 2-norm over all values of a table's tensors: a 0-dim f32 tensor."""
+    if grads.n == 0:
+        return torch.zeros((), dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        partial = torch.empty(grads.partials, dtype=torch.float64, device=device)
+        K.check(_lib().bonsai_mt_norm(grads.n, grads.ptrs, grads.numel, grads.types, partial.data_ptr(), norm.data_ptr(), K.stream()), "mt_norm")
+    return norm
+
+
+def mt_clip(grads: TensorTable, out: TensorTable, max_norm: float, device: torch.device) -> torch.Tensor:
+    """``out`` = ``grads`` scaled to a global norm of at most ``max_norm``; returns the norm before.  ``out`` may be ``grads``."""
+    if grads.n == 0:
+        return torch.zeros((), dtype=torch.float32, device=device)
+    with torch.cuda.device(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        partial = torch.empty(grads.partials, dtype=torch.float64, device=device)
+        K.check(_lib().bonsai_mt_clip(grads.n, grads.ptrs, out.ptrs, grads.numel, grads.types, out.types, max_norm, partial.data_ptr(),
+                                      norm.data_ptr(), K.stream()), "mt_clip")
+    return norm
+
+
+def mt_adam(params: TensorTable, grads: TensorTable, m: TensorTable, v: TensorTable, step: torch.Tensor, lr: float | torch.Tensor,
+            betas: tuple[float, float], eps: float, weight_decay: float, decoupled: bool, max_norm: float | None = None) -> torch.Tensor | None:
+    """One Adam step; ``step`` (int64 on the device) is raised by one.  With ``max_norm`` the gradients enter scaled to that global norm,
+    and the norm before comes back."""
+    device = step.device
+    with torch.cuda.device(device):
+        norm = partial = None
+        if max_norm is not None:
+            norm = torch.empty((), dtype=torch.float32, device=device)
+            partial = torch.empty(grads.partials, dtype=torch.float64, device=device)
+        lr_dev = lr if isinstance(lr, torch.Tensor) else None
+        K.check(_lib().bonsai_mt_adam(params.n, params.ptrs, grads.ptrs, m.ptrs, v.ptrs, params.numel, params.types, grads.types,
+                                      0.0 if lr_dev is not None else lr, K.ptr(lr_dev), betas[0], betas[1], eps, weight_decay, int(decoupled),
+                                      step.data_ptr(), 0.0 if max_norm is None else max_norm, K.ptr(partial), K.ptr(norm), K.stream()), "mt_adam")
+    return norm
+
+
+# ---- cross entropy of a linear head ------------------------------------------------------------------------------------------------
+REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+def linear_ce_forward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, reduction: str,
+                      label_smoothing: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """hidden [n, d], weight [v, d] (one type, unit stride along d), targets int64 [n] -> the loss (f32, 0-dim or [n]) and what the
+    backward pass takes: the list of live rows and their log-sum-exp."""
+    (n, d), v, device = hidden.shape, weight.shape[0], hidden.device
+    code = TYPE_CODES[hidden.dtype]
+    with torch.cuda.device(device):
+        loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=device)
+        live = torch.empty(4 + 2 * n, dtype=torch.int32, device=device)
+        lse = torch.empty(n, dtype=torch.float32, device=device)
+        ws = torch.empty(int(_lib().bonsai_ce_workspace(n, v, d, code, 0, 0, 0)), dtype=torch.uint8, device=device)
+        K.check(_lib().bonsai_ce_forward(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), targets.data_ptr(), n, v, d, code,
+                                         ignore_index, REDUCTIONS[reduction], label_smoothing, live.data_ptr(), lse.data_ptr(), loss.data_ptr(),
+                                         ws.data_ptr(), ws.numel(), K.stream()), "linear_ce_forward")
+    return loss, live, lse
+
+
+def linear_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, live: torch.Tensor, lse: torch.Tensor, up: torch.Tensor, reduction: str,
+                       label_smoothing: float, want_hidden: bool, want_weight: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of :func:`linear_ce_forward`; ``up`` is the loss's gradient (f32, contiguous)."""
+    (n, d), v, device = hidden.shape, weight.shape[0], hidden.device
+    code = TYPE_CODES[hidden.dtype]
+    with torch.cuda.device(device):
+        dh = torch.empty((n, d), dtype=hidden.dtype, device=device) if want_hidden else None
+        dw = torch.empty((v, d), dtype=weight.dtype, device=device) if want_weight else None
+        ws = torch.empty(int(_lib().bonsai_ce_workspace(n, v, d, code, 1, int(want_hidden), int(want_weight))), dtype=torch.uint8, device=device)
+        K.check(_lib().bonsai_ce_backward(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), n, v, d, code,
+                                          REDUCTIONS[reduction], label_smoothing, live.data_ptr(), lse.data_ptr(), up.data_ptr(), K.ptr(dh),
+                                          K.ptr(dw), ws.data_ptr(), ws.numel(), K.stream()), "linear_ce_backward")
+    return dh, dw

@@ -8,7 +8,8 @@ with momentum / Nesterov, Adam, AdamW, ``clip_grad_norm``, constant / warm-up / 
 (one-cycle, reduce-on-plateau, linear warm-up + cosine decay, polynomial decay, cyclic), gradient.rs (scalar-graph
 ``Tensor`` with backward rules), losses.rs (cross-entropy, label smoothing, focal, KL, distillation, MSE, Huber,
 contrastive, next-token loss) and gradient_checkpoint.rs (segments that keep only their input and recompute on demand).
-Everything is written over torch tensors so it runs on the GPU next to the inference engine.
+Everything is written over torch tensors so it runs on the GPU next to the inference engine.  ``linear_loss`` (the loss of a head
+without its logits) and ``multi_tensor`` (norm, clipping and Adam over all tensors at once) run kernels of their own there.
 """
 from __future__ import annotations
 
@@ -18,6 +19,9 @@ from typing import Callable, Iterable, Sequence
 
 import torch
 import torch.nn.functional as F
+
+from .linear_loss import linear_cross_entropy, linear_ntp_loss, linear_sequence_perplexity  # noqa: F401
+from .multi_tensor import FusedAdam, FusedAdamW, GradientSet, clip_global_norm, global_grad_norm  # noqa: F401
 
 
 # ---- LoRA -------------------------------------------------------------------------------------------------------------------
@@ -390,6 +394,7 @@ class LoraTrainingConfig:
     warmup_steps: int = 10
     weight_decay: float = 0.0
     max_grad_norm: float = 1.0
+    fused: bool = False           # clip and step all adapters in two launches (FusedAdamW) instead of tensor by tensor
 
 
 @dataclass
@@ -405,7 +410,8 @@ class LoraTrainer:
 
     def __init__(self, registry: LoraRegistry, config: LoraTrainingConfig | None = None):
         self.registry, self.config = registry, config or LoraTrainingConfig()
-        self.opt = AdamW(registry.parameters(), self.config.lr, weight_decay=self.config.weight_decay)
+        kind = FusedAdamW if self.config.fused else AdamW
+        self.opt = kind(registry.parameters(), self.config.lr, weight_decay=self.config.weight_decay)
         self.sched = LinearWarmupCosineDecay(self.config.lr, self.config.warmup_steps, self.config.total_steps)
         self.history: list[TrainingStep] = []
 
@@ -416,9 +422,12 @@ class LoraTrainer:
         self.opt.zero_grad()
         loss = loss_fn()
         loss.backward()
-        gn = clip_grad_norm(self.opt.params, self.config.max_grad_norm)
         lr = self.current_lr()
-        self.opt.step(lr)
+        if self.config.fused:
+            gn = float(self.opt.step(lr, max_norm=self.config.max_grad_norm))
+        else:
+            gn = clip_grad_norm(self.opt.params, self.config.max_grad_norm)
+            self.opt.step(lr)
         s = TrainingStep(len(self.history), float(loss.detach()), lr, gn)
         self.history.append(s)
         return s
