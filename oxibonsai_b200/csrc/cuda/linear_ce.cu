@@ -4,40 +4,90 @@
 //   loss_i = lse_i - sum_v q_iv z_iv
 //   dz_iv = u_i (exp(z_iv - lse_i) - q_iv),   dh = dz W,   dW = dz^T h
 //
-// Rows whose target is the ignored one are left out before anything is multiplied: the kernels work on the list of live rows, whose length
-// stays on the device.  A target outside the vocabulary makes its row's loss and gradients NaN.
+// Four products of 2 n V D operations: the logits for the loss, the logits again piece by piece for dz, and the two gradients.  One
+// kernel makes them all (ce_gemm_kernel), on pairs of SMs with tcgen05.mma cta_group::2 over tiles of 256 x up to 256, and differs
+// by where its operands lie and what happens to a finished tile:
+//   CE_LSE  h [n][D] x W [V][D]: a row's maximum and sum of exponentials over its half of the tile's columns; no logit leaves the SM
+//   CE_DZ   the same product; exp(z - lse) - q in 16 bits into the piece's buffer [n][piece]
+//   CE_DH   dz [n][piece] x W [piece][D], summed over the piece: W is read across its rows (MN-major operand), nothing is transposed
+//   CE_DW   dz^T [piece][n] x h [n][D]: both operands across their rows
+// The tensor cores bound all four where there are many tokens; with few, the head's bytes do.
+//
+// Rows whose target is the ignored one are left out before anything is multiplied: the live rows are copied side by side, and their number
+// stays on the device.  A target outside the vocabulary makes its row's loss and gradients NaN, and so does a wait that expires.
+//
+// dz is rounded to the inputs' 16-bit type before it is multiplied, as the operand of a tensor-core product has to be.  It is stored without the
+// upstream gradient's size (that factor enters with the products' sums), in f16 scaled by 2^15: probabilities down to 2^-29 stay normal.
+//
+// float32 inputs become three bfloat16 parts each (8 bits a part, exact down to 2^-24) and six products of parts: the parts that are left out
+// are below 2^-24 of the product.  The tensor cores' sums truncate, which over thousands of steps of one sign costs more than f32
+// rounding would; so every kCeSegment blocks the tile is added to registers with rounding.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace bonsai {
 
-constexpr int kCeTile = 64, kCeK = 16, kCeThreads = 256;
 enum CeType { CE_F32 = 0, CE_F16 = 1, CE_BF16 = 2 };
 enum CeReduce { CE_MEAN = 0, CE_SUM = 1, CE_NONE = 2 };
+enum CeMode { CE_LSE, CE_DZ, CE_DH, CE_DW };
+
+constexpr int kCeStages = 6;
+constexpr int kCeBlock = 64;                            // k per stage
+constexpr int kCeOperand = 128 * kCeBlock * 2;          // 16 KB: a CTA's half of one operand
+constexpr int kCeEpiWarps = 8;
+constexpr int kCeThreads = (kCeEpiWarps + 2) * 32;
+constexpr int kCeCols = 256;                            // TMEM columns of an accumulator, two of them
+constexpr int kCeGroup = 16;                            // row tiles that share the head's tiles while those are in L2
+constexpr int kCeSegment = 2;                           // f32: blocks of k between two additions to registers
+constexpr int kCeTerms = 6;
+constexpr float kCeLog2e = 1.4426950408889634f;
+__device__ const unsigned char kCeTermA[kCeTerms] = {2, 0, 1, 1, 0, 0}, kCeTermB[kCeTerms] = {0, 2, 1, 0, 1, 0};      // the small ones first
 
 struct CeRows {         // the live rows, in order: filled by ce_rows_kernel
-  int* count;           // [4]: live rows
+  int* count;
   int* index;           // [N] row of the hidden states
   int* target;          // [N] its target, -1 outside the vocabulary
-  float* lse;           // [N]
+  float* lse2;          // [N] log2 of the sum of exponentials
 };
 
-__device__ __forceinline__ float ce_f32(float x) { return x; }
-__device__ __forceinline__ float ce_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float ce_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void ce_put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void ce_put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void ce_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+struct CeGemm {
+  CeRows rows;
+  int columns;          // LSE, DZ: vocabulary rows of the piece; DH, DW: width
+  int depth;            // k: width (LSE, DZ), vocabulary rows of the piece (DH); DW: the live rows
+  int m;                // DW: vocabulary rows of the piece
+  int tile_n;           // columns of a tile, a multiple of 16
+  int a_rows;           // K-major A: rows of a copy
+  int c0;               // first vocabulary row of the piece; where the head's rows start in its tensor map: w_row
+  int w_row;
+  int vocab;
+  float smoothing;
+  // LSE
+  float *part_m, *part_s, *part_z, *at_target;
+  long long ldn;
+  int slot;             // first slot of this piece
+  // DZ
+  const float* factor;  // [N] u_i over the largest one
+  uint16_t* dz;
+  long long ldz, plane; // elements of a row, of a plane
+  // DH, DW
+  const float* scale;   // what the sums are multiplied by
+  int splits, first, last;
+  float* acc;           // DH: [splits][ldn][columns] sums of several pieces or parts
+  void* out;            // [..][columns] of the inputs' type
+};
 
-// One block walks the targets and lists the live rows in order.  `zero_loss`: where the loss of ignored rows goes (reduction "none").
-__global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* __restrict__ targets, int n, int vocab, long long ignore, CeRows r, float* zero_loss) {
+// ---- rows ---------------------------------------------------------------------------------------------------------------------------
+// One block walks the targets and lists the live rows in order.  `each`: the loss of ignored rows (reduction "none").
+__global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* __restrict__ targets, int n, int vocab, long long ignore, CeRows r, float* each) {
   __shared__ int warps[32];
-  __shared__ int base;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  if (t == 0) base = 0;
-  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int base = 0;
   for (int i0 = 0; i0 < n; i0 += 1024) {
     const int i = i0 + t;
     const long long tgt = i < n ? targets[i] : ignore;
@@ -45,193 +95,585 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* __restri
     const unsigned m = __ballot_sync(0xffffffffu, live);
     if (lane == 0) warps[warp] = __popc(m);
     __syncthreads();
-    int before = base, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      const int c = warps[w];
-      if (w < warp) before += c;
-      all += c;
+    const int c = warps[lane];
+    int before = lane < warp ? c : 0, all = c;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
     }
     if (live) {
-      const int at = before + __popc(m & ((1u << lane) - 1));
+      const int at = base + before + __popc(m & ((1u << lane) - 1));
       r.index[at] = i;
       r.target[at] = tgt >= 0 && tgt < vocab ? (int)tgt : -1;
-    } else if (i < n && zero_loss != nullptr) {
-      zero_loss[i] = 0.0f;
+    } else if (i < n && each != nullptr) {
+      each[i] = 0.0f;
     }
-    __syncthreads();
-    if (t == 0) base += all;
+    base += all;
     __syncthreads();
   }
   if (t == 0) *r.count = base;
 }
 
-template <typename LA, typename LB>
-__device__ __forceinline__ void ce_tile(LA a, LB b, int K, float (&acc)[4][4], float (*sa)[kCeTile + 4], float (*sb)[kCeTile + 4]) {
-  const int t = threadIdx.x, tx = t & 15, ty = t >> 4;
-  for (int k0 = 0; k0 < K; k0 += kCeK) {
-    for (int i = t; i < kCeTile * kCeK; i += kCeThreads) {
-      sa[i & 15][i >> 4] = k0 + (i & 15) < K ? a(i >> 4, k0 + (i & 15)) : 0.0f;
-      sb[i & 15][i >> 4] = k0 + (i & 15) < K ? b(i >> 4, k0 + (i & 15)) : 0.0f;
+__device__ __forceinline__ float ce_f32(float x) { return x; }
+__device__ __forceinline__ uint16_t ce_bits(__half x) { return __half_as_ushort(x); }
+__device__ __forceinline__ uint16_t ce_bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+
+// x as the sum of three bfloat16; what is not finite stays in the first
+__device__ __forceinline__ void ce_split(float x, uint16_t* p) {
+  const __nv_bfloat16 a = __float2bfloat16_rn(x);
+  const float fa = __bfloat162float(a), r = isfinite(fa) ? x - fa : 0.0f;
+  const __nv_bfloat16 b = __float2bfloat16_rn(r);
+  p[0] = ce_bits(a);
+  p[1] = ce_bits(b);
+  p[2] = ce_bits(__float2bfloat16_rn(r - __bfloat162float(b)));
+}
+
+// Rows of a matrix side by side with a row stride of whole 16-byte words: the live rows (count given; zeros up to the next 256) or all of
+// them, f32 as three planes.  A thread takes eight values.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_pack_kernel(const T* __restrict__ src, long long ld, long long row0, int rows, const int* count, const int* index,
+                                                      int width, uint16_t* dst, int ldd, long long plane) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = count != nullptr ? *count : rows, n_out = count != nullptr ? (n + 255) / 256 * 256 : rows, words = ldd >> 3;
+  const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(ld * sizeof(T))) & 15) == 0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n_out * words; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / words), k0 = (int)(i % words) * 8;
+    __align__(16) T v[8];
+    const T* s = src + (index != nullptr && r < n ? (long long)index[r] : row0 + r) * ld + k0;
+    if (r < n && wide && k0 + 8 <= width) {
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(s)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = r < n && k0 + j < width ? s[j] : T(0.0f);
     }
-    __syncthreads();
+    uint16_t* o = dst + (long long)r * ldd + k0;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
+    } else {
+      __align__(16) uint16_t p[3][8];
 #pragma unroll
-    for (int k = 0; k < kCeK; ++k)
+      for (int j = 0; j < 8; ++j) {
+        uint16_t q[3];
+        ce_split(ce_f32(v[j]), q);
+        p[0][j] = q[0]; p[1][j] = q[1]; p[2][j] = q[2];
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][4 * ty + i], sb[k][4 * tx + j], acc[i][j]);
-    __syncthreads();
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(o + k * plane) = *reinterpret_cast<const uint4*>(p[k]);
+    }
   }
 }
 
-template <typename T>
-struct CeHead {
-  const T* h;
-  const T* w;
-  long long ldh, ldw;
-  int vocab, hidden;
+// ---- the product ----------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t ce_map(uint32_t addr, uint32_t rank) {      // the same shared-memory place in CTA `rank` of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void ce_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void ce_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrives on the barrier at this place in both CTAs once the MMAs issued so far are done
+__device__ __forceinline__ void ce_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tc::smem_u32(bar)),
+               "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void ce_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void ce_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ce_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// An operand across its rows (MN-major): a tile of 64 columns x 64 k is 64 rows of 128 bytes, swizzled like the K-major tiles; the next 64 columns
+// begin 8 KB further (leading offset), the next eight k 1 KB (stride), sixteen k 2 KB.
+__device__ __forceinline__ uint64_t ce_desc_mn(uint32_t smem_addr) {
+  return (tc::smem_desc_sw128(smem_addr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(8192 >> 4) << 16);
+}
+
+template <int MODE>
+struct CeTiles {       // tiles of a launch, and which one has which number
+  int rt, ct, all;
+  __device__ __forceinline__ CeTiles(const CeGemm& p, int n) {
+    rt = ((MODE == CE_DW ? p.m : n) + 255) >> 8;
+    ct = (p.columns + p.tile_n - 1) / p.tile_n;
+    all = rt * ct * (MODE == CE_DH ? p.splits : 1);
+  }
+  __device__ __forceinline__ void at(int i, int* r, int* c, int* split) const {
+    *split = 0;
+    if (MODE == CE_LSE || MODE == CE_DZ) {      // groups of row tiles; in a group the row tiles of one column tile after another
+      const int g = i / (kCeGroup * ct), in = i - g * kCeGroup * ct, high = min(kCeGroup, rt - g * kCeGroup);
+      *c = in / high;
+      *r = g * kCeGroup + in % high;
+    } else {                                    // the column tiles of a row tile one after another
+      *c = i % ct;
+      *r = i / ct % rt;
+      *split = i / ct / rt;
+    }
+  }
 };
 
-// partial [slot][N] = (maximum, sum of exp below it, sum of z) of a row over 64 vocabulary rows; zt: z at the target
+template <typename T> __device__ __forceinline__ uint32_t ce_pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t ce_pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t ce_pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 32 neighbouring values of a row, `valid` of them inside
 template <typename T>
-__global__ void __launch_bounds__(kCeThreads) ce_lse_kernel(CeHead<T> p, CeRows r, float* part, float* zt, long long n_ld) {
-  __shared__ float sa[kCeK][kCeTile + 4], sb[kCeK][kCeTile + 4];
-  const int n = *r.count, r0 = blockIdx.y * kCeTile, v0 = blockIdx.x * kCeTile;
-  if (r0 >= n) return;
-  float acc[4][4] = {};
-  ce_tile([&](int m, int k) { return r0 + m < n ? ce_f32(p.h[(long long)r.index[r0 + m] * p.ldh + k]) : 0.0f; },
-          [&](int m, int k) { return v0 + m < p.vocab ? ce_f32(p.w[(long long)(v0 + m) * p.ldw + k]) : 0.0f; }, p.hidden, acc, sa, sb);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+__device__ __forceinline__ void ce_store32(T* dst, const float* v, int valid) {
+  if (valid >= 32 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
-    float m = -INFINITY, s = 0.0f, z = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (v0 + 4 * tx + j >= p.vocab) acc[i][j] = -INFINITY;
-      else z += acc[i][j];
-      m = fmaxf(m, acc[i][j]);
-    }
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s += __expf(acc[i][j] - m);
-    for (int o = 8; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      z += __shfl_xor_sync(0xffffffffu, z, o);
-    }
-    if (row < n) {
+      for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (v0 + 4 * tx + j == r.target[row]) zt[row] = acc[i][j];
-      if (tx == 0) {
-        float* o = part + (long long)blockIdx.x * 3 * n_ld + row;
-        o[0] = m;
-        o[n_ld] = s;
-        o[2 * n_ld] = z;
-      }
+        reinterpret_cast<uint4*>(dst)[j] = make_uint4(ce_pack2<T>(v[8 * j], v[8 * j + 1]), ce_pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                                                      ce_pack2<T>(v[8 * j + 4], v[8 * j + 5]), ce_pack2<T>(v[8 * j + 6], v[8 * j + 7]));
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < valid) dst[j] = T(v[j]);
   }
 }
 
-__global__ void __launch_bounds__(256) ce_merge_kernel(CeRows r, const float* part, const float* zt, long long n_ld, int slots, int vocab, float smoothing, float* row_loss,
-                                                       float* each) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= *r.count) return;
-  float m = -INFINITY, s = 0.0f, z = 0.0f;
-  for (int k = 0; k < slots; ++k) m = fmaxf(m, part[(long long)k * 3 * n_ld + i]);
-  for (int k = 0; k < slots; ++k) {
-    s += part[((long long)k * 3 + 1) * n_ld + i] * expf(part[(long long)k * 3 * n_ld + i] - m);
-    z += part[((long long)k * 3 + 2) * n_ld + i];
+// T: the inputs' type.  The operands in shared memory are T, or bfloat16 parts of f32.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_gemm_kernel(const __grid_constant__ CUtensorMap amap,
+                                                                                         const __grid_constant__ CUtensorMap bmap, const CeGemm p) {
+  constexpr bool kF32 = sizeof(T) == 4, kAcross = MODE == CE_DH || MODE == CE_DW;      // B is MN-major
+  constexpr int kTerms = kF32 ? kCeTerms : 1;
+  extern __shared__ uint8_t ce_smem[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)ce_smem + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = base;
+  uint8_t* sB = base + kCeStages * kCeOperand;
+  __shared__ uint64_t full[kCeStages], empty[kCeStages], accf[2], acce[2];
+  __shared__ uint32_t tmem_slot;
+  const int t = threadIdx.x, warp = __shfl_sync(0xffffffffu, t >> 5, 0), lane = t & 31;
+  const uint32_t rank = blockIdx.x & 1;
+  const int cid = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == kCeEpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(2 * kCeCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  const float lse = m + logf(s);
-  r.lse[i] = lse;
-  const float loss = r.target[i] < 0 ? NAN : lse - (1.0f - smoothing) * zt[i] - smoothing / vocab * z;
-  row_loss[i] = loss;
-  if (each != nullptr) each[r.index[i]] = loss;
-}
-
-__global__ void __launch_bounds__(256) ce_total_kernel(CeRows r, const float* row_loss, int reduce, float* loss) {
-  __shared__ double s[256];
-  double v = 0.0;
-  for (int i = threadIdx.x; i < *r.count; i += 256) v += (double)row_loss[i];
-  s[threadIdx.x] = v;
+  if (t == 0) {
+    for (int i = 0; i < kCeStages; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&accf[i], 1);
+      tc::mbar_init(&acce[i], 2 * kCeEpiWarps);
+    }
+    tc::mbar_fence_init();
+  }
+  tc::tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 256; ++i) v += s[i];
-    *loss = (float)(reduce == CE_MEAN ? v / (double)*r.count : v);
-  }
-}
+  ce_cluster_sync();                 // both CTAs' barriers exist and both have their TMEM
+  tc::tc_fence_after();
+  const uint32_t taddr = tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = *p.rows.count;
+  const CeTiles<MODE> tiles(p, n);
+  const int blocks_all = ((MODE == CE_DW ? n : p.depth) + kCeBlock - 1) / kCeBlock;
+  // blocks of k that a part of a split tile takes
+  auto part = [&](int split, int* b0, int* b1) {
+    *b0 = 0;
+    *b1 = blocks_all;
+    if (MODE == CE_DH) {
+      *b0 = (int)((long long)blocks_all * split / p.splits);
+      *b1 = (int)((long long)blocks_all * (split + 1) / p.splits);
+    }
+  };
 
-struct CeUp {           // u_i
-  const float* up;
-  int reduce;
-};
-__device__ __forceinline__ float ce_weight(const CeUp& u, const CeRows& r, int i) {
-  const float g = u.reduce == CE_NONE ? u.up[r.index[i]] : u.reduce == CE_MEAN ? u.up[0] / (float)*r.count : u.up[0];
-  return r.target[i] < 0 ? NAN : g;
-}
+  if (warp == kCeEpiWarps) {
+    if (tc::elect_one()) {
+      bool failed = false;
+      int s = 0, issued = 0;
+      uint32_t phase = 1;
+      for (int tile = cid; tile < tiles.all && !failed; tile += nclusters) {
+        int rt, ct, split, b0, b1;
+        tiles.at(tile, &rt, &ct, &split);
+        part(split, &b0, &b1);
+        const int row0 = rt * 256 + (int)rank * 128, col0 = ct * p.tile_n + (int)rank * (p.tile_n >> 1);
+        // rows behind the last live one are not copied: what lies in their place meets no other row
+        const bool has = MODE == CE_DW || row0 < n, other = MODE == CE_DW || rt * 256 + 128 < n;
+        const uint32_t abytes = MODE == CE_DW ? kCeOperand : (uint32_t)p.a_rows * kCeBlock * 2;
+        const uint32_t bytes = abytes * (1 + (other ? 1 : 0)) + 2 * (kAcross ? (uint32_t)kCeOperand : (uint32_t)p.tile_n * kCeBlock);
+        for (int kb = b0; kb < b1 && !failed; ++kb) {
+          const int k = kb * kCeBlock;
+          for (int term = 0; term < kTerms; ++term, ++issued) {
+            const int pa = kF32 ? kCeTermA[term] : 0, pb = kF32 ? kCeTermB[term] : 0;
+            if (!tc::mbar_wait(&empty[s], phase)) { failed = true; break; }
+            const uint32_t bar = ce_map(tc::smem_u32(&full[s]), 0), a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kCeOperand);
+            if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], bytes);
+            if (MODE == CE_DW) {
+              ce_load(a, &amap, row0, k, pa, bar);
+              ce_load(a + 8192, &amap, row0 + 64, k, pa, bar);
+            } else if (has) {
+              ce_load(a, &amap, k, row0, pa, bar);
+            }
+            if (kAcross) {
+              const int kw = MODE == CE_DH ? p.w_row + k : k;
+              ce_load(b, &bmap, col0, kw, pb, bar);
+              ce_load(b + 8192, &bmap, col0 + 64, kw, pb, bar);
+            } else {
+              ce_load(b, &bmap, k, p.w_row + col0, pb, bar);
+            }
+            if (++s == kCeStages) { s = 0; phase ^= 1; }
+          }
+        }
+      }
+      if (rank == 0) tc::mbar_drain(full, issued, kCeStages);      // both CTAs' copies; the other one waits at the barrier below
+    }
+  } else if (warp == kCeEpiWarps + 1) {
+    if (rank == 0 && tc::elect_one()) {
+      constexpr uint32_t fmt = sizeof(T) == 2 && __is_same(T, __half) ? tc::FMT_F16 : tc::FMT_BF16;
+      const uint32_t idesc = tc::idesc_f32acc(fmt, fmt, 256, (uint32_t)p.tile_n) | (MODE == CE_DW ? 1u << 15 : 0u) | (kAcross ? 1u << 16 : 0u);
+      bool failed = false;
+      int s = 0, seg = 0;
+      uint32_t phase = 0;
+      for (int tile = cid; tile < tiles.all && !failed; tile += nclusters) {
+        int rt, ct, split, b0, b1;
+        tiles.at(tile, &rt, &ct, &split);
+        part(split, &b0, &b1);
+        for (int k0 = b0; k0 < b1 && !failed; ++seg) {
+          const int ab = seg & 1, k1 = kF32 ? min(b1, k0 + kCeSegment) : b1;
+          if (!tc::mbar_wait(&acce[ab], ((seg >> 1) & 1) ^ 1)) { failed = true; break; }
+          tc::tc_fence_after();
+          for (int i = 0; i < (k1 - k0) * kTerms; ++i) {
+            if (!tc::mbar_wait(&full[s], phase)) { failed = true; break; }
+            tc::tc_fence_after();
+            const uint32_t a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kCeOperand);
+            const uint64_t da = MODE == CE_DW ? ce_desc_mn(a) : tc::smem_desc_sw128(a), db = kAcross ? ce_desc_mn(b) : tc::smem_desc_sw128(b);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+              ce_mma(taddr + ab * kCeCols, da + (MODE == CE_DW ? 128 : 2) * k, db + (kAcross ? 128 : 2) * k, idesc, i > 0 || k > 0);
+            ce_commit(&empty[s]);
+            if (++s == kCeStages) { s = 0; phase ^= 1; }
+          }
+          ce_commit(&accf[ab]);
+          k0 = k1;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t drained[2] = {ce_map(tc::smem_u32(&acce[0]), 0), ce_map(tc::smem_u32(&acce[1]), 0)};
+    bool failed = false;
+    int seg = 0;
+    for (int tile = cid; tile < tiles.all; tile += nclusters) {
+      int rt, ct, split, b0, b1;
+      tiles.at(tile, &rt, &ct, &split);
+      part(split, &b0, &b1);
+      const int row = rt * 256 + (int)rank * 128 + quarter * 32 + lane, col0 = ct * p.tile_n, cols = min(p.tile_n, p.columns - col0);
+      const bool live = row < (MODE == CE_DW ? p.m : n);
+      // what a row brings
+      float lse2 = 0.0f, f = 0.0f, scale = 0.0f;
+      int target = -1;
+      if (MODE == CE_LSE || MODE == CE_DZ) {
+        if (live) target = p.rows.target[row] - p.c0 - col0;
+        if (target >= cols) target = -1;                      // another tile's, though it may lie in this one's last 32 columns
+        if (MODE == CE_DZ && live) {
+          lse2 = p.rows.lse2[row];
+          f = p.factor[row];
+        }
+      } else {
+        scale = *p.scale;
+      }
+      float top = -INFINITY, sum = 0.0f, sum_z = 0.0f;
 
-template <typename T>
-__global__ void __launch_bounds__(kCeThreads) ce_dz_kernel(CeHead<T> p, CeRows r, CeUp u, float smoothing, int c0, int width, float* dz) {
-  __shared__ float sa[kCeK][kCeTile + 4], sb[kCeK][kCeTile + 4];
-  const int n = *r.count, r0 = blockIdx.y * kCeTile, v0 = c0 + blockIdx.x * kCeTile, end = min(p.vocab, c0 + width);
-  if (r0 >= n) return;
-  float acc[4][4] = {};
-  ce_tile([&](int m, int k) { return r0 + m < n ? ce_f32(p.h[(long long)r.index[r0 + m] * p.ldh + k]) : 0.0f; },
-          [&](int m, int k) { return v0 + m < end ? ce_f32(p.w[(long long)(v0 + m) * p.ldw + k]) : 0.0f; }, p.hidden, acc, sa, sb);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+      auto finish = [&](float* v, int c0) {      // columns c0 .. c0 + 31 of the tile
+        const int valid = cols - c0;
+        if (failed) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
-    if (row >= n) continue;
-    const float g = ce_weight(u, r, row), lse = r.lse[row];
+          for (int j = 0; j < 32; ++j) v[j] = NAN;
+        }
+        if constexpr (MODE == CE_LSE) {
+          if (valid < 32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int v = v0 + 4 * tx + j;
-      if (v < end) dz[(long long)row * width + v - c0] = g * (expf(acc[i][j] - lse) - (v == r.target[row] ? 1.0f - smoothing : 0.0f) - smoothing / p.vocab);
+            for (int j = 0; j < 32; ++j)
+              if (j >= valid) v[j] = -INFINITY;
+          }
+          float m = v[0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) m = fmaxf(m, v[j]);
+          if (p.smoothing != 0.0f) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum_z += j < valid ? v[j] : 0.0f;
+          }
+          if ((unsigned)(target - c0) < 32u) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z = j == target - c0 ? v[j] : z;
+            p.at_target[row] = z;
+          }
+          m = fmaxf(top, m * kCeLog2e);
+          float s0 = 0.0f, s1 = 0.0f;
+          const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            s0 += ce_exp2(fmaf(v[j], kCeLog2e, -ref));
+            s1 += ce_exp2(fmaf(v[j + 1], kCeLog2e, -ref));
+          }
+          sum = sum * ce_exp2(top - ref) + (s0 + s1);
+          top = m;
+        } else if constexpr (MODE == CE_DZ) {
+          const float even = p.smoothing / (float)p.vocab, up = kF32 || __is_same(T, __nv_bfloat16) ? f : f * 32768.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = up * (ce_exp2(fmaf(v[j], kCeLog2e, -lse2)) - even);
+          if ((unsigned)(target - c0) < 32u) {
+            const float q = up * (1.0f - p.smoothing);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] -= j == target - c0 ? q : 0.0f;
+          }
+          if (!live) {          // up to the end of the tile: rows are a product's k
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          }
+          uint16_t* o = p.dz + (long long)row * p.ldz + col0 + c0;
+          if constexpr (!kF32) {
+            ce_store32<T>(reinterpret_cast<T*>(o), v, valid);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              ce_store32<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16*>(o + k * p.plane), v, valid);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float a = __bfloat162float(__float2bfloat16_rn(v[j]));
+                v[j] = isfinite(a) ? v[j] - a : 0.0f;
+              }
+            }
+          }
+        } else if constexpr (MODE == CE_DH) {
+          if (live) {
+            float* acc = p.acc + ((long long)split * p.ldn + row) * p.columns + col0 + c0;
+            if (!p.first) {
+              if (valid >= 32 && (reinterpret_cast<uintptr_t>(acc) & 15) == 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float4 a = reinterpret_cast<const float4*>(acc)[j];
+                  v[4 * j] += a.x; v[4 * j + 1] += a.y; v[4 * j + 2] += a.z; v[4 * j + 3] += a.w;
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < valid) v[j] += acc[j];
+              }
+            }
+            if (p.splits == 1 && p.last) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= scale;
+              ce_store32<T>((T*)p.out + (long long)p.rows.index[row] * p.columns + col0 + c0, v, valid);
+            } else {
+              ce_store32<float>(acc, v, valid);
+            }
+          }
+        } else {
+          if (live) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= scale;
+            ce_store32<T>((T*)p.out + (long long)(p.c0 + row) * p.columns + col0 + c0, v, valid);
+          }
+        }
+      };
+
+      if constexpr (kF32) {
+        float acc[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
+#pragma unroll 1
+        for (int k0 = b0; k0 < b1; k0 += kCeSegment, ++seg) {
+          const int ab = seg & 1;
+          if (!failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg >> 1) & 1, lane)) failed = true;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t r[32];
+            tc::tmem_ld32(taddr + lane_base + ab * kCeCols + (half + 2 * i) * 32, r);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[i][j] += __uint_as_float(r[j]);
+          }
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ce_arrive_at(drained[ab]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((half + 2 * i) * 32 < cols) finish(acc[i], (half + 2 * i) * 32);
+      } else {
+        const bool none = b0 == b1;            // an empty sum: no live row
+        const int ab = seg & 1;
+        if (!none && !failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg >> 1) & 1, lane)) failed = true;
+        tc::tc_fence_after();
+#pragma unroll 1
+        for (int c0 = half * 32; c0 < cols; c0 += 64) {
+          uint32_t r[32];
+          float v[32];
+          tc::tmem_ld32(taddr + lane_base + ab * kCeCols + c0, r);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = none ? 0.0f : __uint_as_float(r[j]);
+          finish(v, c0);
+        }
+        if (!none) {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ce_arrive_at(drained[ab]);
+          ++seg;
+        }
+      }
+      if (MODE == CE_LSE && live) {
+        const long long at = (long long)(p.slot + 2 * ct + half) * p.ldn + row;
+        p.part_m[at] = top;
+        p.part_s[at] = sum;
+        if (p.smoothing != 0.0f) p.part_z[at] = sum_z;
+      }
     }
   }
+  tc::tc_fence_before();
+  __syncwarp();
+  ce_cluster_sync();                 // nobody leaves while the other CTA may still read its shared memory or TMEM, or signal it
+  tc::tc_fence_after();
+  if (warp == kCeEpiWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(2 * kCeCols) : "memory");
 }
 
-// dh [N][D] f32 += dz W of one piece (the list's order)
+// ---- joining ----------------------------------------------------------------------------------------------------------------------------
+// 32 rows a block, a warp for every 32nd slot of their maxima and sums; then the row's loss
+__global__ void __launch_bounds__(1024) ce_merge_kernel(CeRows r, const float* __restrict__ part_m, const float* __restrict__ part_s, const float* __restrict__ part_z,
+                                                        const float* at_target, long long ldn, int slots, int vocab, float smoothing, float* row_loss, float* each) {
+  __shared__ float sm[32][33];
+  __shared__ double ss[32][33], sz[32][33];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane, n = *r.count;
+  if (blockIdx.x * 32 >= n) return;
+  float top = -INFINITY;
+  double s = 0.0, z = 0.0;
+  bool bad = false;
+  if (row < n) {
+#pragma unroll 4
+    for (int k = warp; k < slots; k += 32) {
+      const float m = part_m[k * ldn + row];
+      bad |= m != m;
+      top = fmaxf(top, m);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+    for (int k = warp; k < slots; k += 32) {
+      s += (double)(part_s[k * ldn + row] * ce_exp2(part_m[k * ldn + row] - ref));
+      if (smoothing != 0.0f) z += (double)part_z[k * ldn + row];
+    }
+    if (bad) s = NAN;
+  }
+  sm[warp][lane] = top;
+  ss[warp][lane] = s;
+  sz[warp][lane] = z;
+  __syncthreads();
+  if (warp == 0 && row < n) {
+    for (int w = 1; w < 32; ++w) top = fmaxf(top, sm[w][lane]);
+    s = z = 0.0;
+    for (int w = 0; w < 32; ++w) {
+      s += ss[w][lane] * (double)(sm[w][lane] == -INFINITY ? 0.0f : ce_exp2(sm[w][lane] - top));
+      z += sz[w][lane];
+    }
+    const double lse2 = (double)top + log2(s);
+    r.lse2[row] = (float)lse2;
+    double loss = lse2 * 0.69314718055994530942 - (double)(1.0f - smoothing) * (double)at_target[row];
+    if (smoothing != 0.0f) loss -= (double)smoothing * z / vocab;
+    if (r.target[row] < 0) loss = NAN;
+    row_loss[row] = (float)loss;
+    if (each != nullptr) each[r.index[row]] = (float)loss;
+  }
+}
+
+__global__ void __launch_bounds__(1024) ce_total_kernel(const int* count, const float* __restrict__ row_loss, int reduce, float* loss) {
+  __shared__ double s[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = *count;
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) v += (double)row_loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    v = s[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (threadIdx.x == 0) *loss = (float)(reduce == CE_MEAN ? v / (double)n : v);
+  }
+}
+
+// factor_i = u_i / max |u|, scale = max |u| over what dz is stored with
+__global__ void __launch_bounds__(1024) ce_up_kernel(CeRows r, const float* __restrict__ up, int reduce, float dz_scale, float* factor, float* scale) {
+  __shared__ float s[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = *r.count;
+  float top = 0.0f;
+  if (reduce == CE_NONE) {
+    for (int i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, fabsf(up[r.index[i]]));
+  } else {
+    top = fabsf(up[0]);
+  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = warp_max(s[threadIdx.x & 31]);
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float u = reduce == CE_NONE ? up[r.index[i]] : up[0];
+    factor[i] = r.target[i] < 0 ? NAN : top > 0.0f ? u / top : u;      // u is 0 or NaN where no |u| is above 0
+  }
+  if (threadIdx.x == 0) *scale = n > 0 ? top / dz_scale / (reduce == CE_MEAN ? (float)n : 1.0f) : 0.0f;
+}
+
+// dh: the parts' sums, to the rows' places
 template <typename T>
-__global__ void __launch_bounds__(kCeThreads) ce_dh_kernel(CeHead<T> p, CeRows r, const float* dz, int c0, int width, int first, float* dh) {
-  __shared__ float sa[kCeK][kCeTile + 4], sb[kCeK][kCeTile + 4];
-  const int n = *r.count, r0 = blockIdx.y * kCeTile, d0 = blockIdx.x * kCeTile, k = min(width, p.vocab - c0);
-  if (r0 >= n) return;
-  float acc[4][4] = {};
-  ce_tile([&](int m, int v) { return r0 + m < n ? dz[(long long)(r0 + m) * width + v] : 0.0f; },
-          [&](int m, int v) { return d0 + m < p.hidden ? ce_f32(p.w[(long long)(c0 + v) * p.ldw + d0 + m]) : 0.0f; }, k, acc, sa, sb);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (r0 + 4 * ty + i < n && d0 + 4 * tx + j < p.hidden) {
-        float* o = dh + (long long)(r0 + 4 * ty + i) * p.hidden + d0 + 4 * tx + j;
-        *o = first ? acc[i][j] : *o + acc[i][j];
-      }
+__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, const float* __restrict__ acc, int splits, long long ldn, int width, const float* scale, T* out) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = *r.count;
+  const float f = *scale;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n * width; i += (long long)gridDim.x * 256) {
+    float v = 0.0f;
+    for (int k = 0; k < splits; ++k) v += acc[k * ldn * width + i];
+    out[(long long)r.index[i / width] * width + i % width] = T(v * f);
+  }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kCeThreads) ce_dw_kernel(CeHead<T> p, CeRows r, const float* dz, int c0, int width, T* dw) {
-  __shared__ float sa[kCeK][kCeTile + 4], sb[kCeK][kCeTile + 4];
-  const int n = *r.count, m0 = blockIdx.y * kCeTile, d0 = blockIdx.x * kCeTile, rows = min(width, p.vocab - c0);
-  float acc[4][4] = {};
-  ce_tile([&](int m, int i) { return m0 + m < rows ? dz[(long long)i * width + m0 + m] : 0.0f; },
-          [&](int m, int i) { return d0 + m < p.hidden ? ce_f32(p.h[(long long)r.index[i] * p.ldh + d0 + m]) : 0.0f; }, n, acc, sa, sb);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (m0 + 4 * ty + i < rows && d0 + 4 * tx + j < p.hidden) ce_put(dw + (long long)(c0 + m0 + 4 * ty + i) * p.hidden + d0 + 4 * tx + j, acc[i][j]);
-}
-
-// rows of dh to their places; the others are cleared before
-template <typename T>
-__global__ void __launch_bounds__(256) ce_scatter_kernel(CeRows r, const float* dh, int hidden, T* out) {
-  const int i = blockIdx.x;
-  if (i >= *r.count) return;
-  for (int k = threadIdx.x; k < hidden; k += 256) ce_put(out + (long long)r.index[i] * hidden + k, dh[(long long)i * hidden + k]);
-}
-
+// ---- host -----------------------------------------------------------------------------------------------------------------------------
 struct CeArgs {
   const void *hidden, *weight;
   const long long* targets;
@@ -246,90 +688,274 @@ struct CeArgs {
   long long ws_bytes;
 };
 
-static long long ce_piece(const CeArgs& a) {      // vocabulary rows of a piece of dz
-  const long long most = (1ll << 28) / a.rows / kCeTile * kCeTile;
-  return most < kCeTile ? kCeTile : most > a.vocab ? a.vocab : most;
+struct CePlan {
+  int planes, ldd, padded, tile_v, clusters;
+  bool packed;                 // the head is copied piece by piece: f32, or rows that TMA cannot take
+  int piece, pieces, splits;
+  long long x, w, parts, part, rows, dz, acc, bytes;      // places in the workspace, and its size
+};
+
+static long long ce_up_to(long long v, long long unit) { return (v + unit - 1) / unit * unit; }
+
+static int ce_sms() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
 }
-static int ce_slots(const CeArgs& a) { return (a.vocab + kCeTile - 1) / kCeTile; }
-static long long ce_forward_bytes(const CeArgs& a) { return 4ll * a.rows * (3ll * ce_slots(a) + 2); }
-static long long ce_backward_bytes(const CeArgs& a) { return 4ll * a.rows * (ce_piece(a) + a.width); }
+
+// Vocabulary rows of a tile: the fewest rounds of tiles times the cycles of a block of k, 2 per column on the tensor core or the copies at
+// some 70 bytes a cycle, whichever is longer.
+static int ce_tile_columns(int rows, int vocab, int clusters) {
+  const long long row_tiles = (rows + 255) / 256;
+  const long long a_bytes = (rows < 128 ? rows : 128) * 128;
+  int best = 256;
+  long long best_cost = -1;
+  for (int tn = 256; tn >= 128; tn -= 16) {
+    const long long tiles = row_tiles * ((vocab + tn - 1) / tn), rounds = (tiles + clusters - 1) / clusters;
+    const long long tensor = 2 * tn, copies = (a_bytes + 64 * tn) / 70, cost = rounds * ((tensor > copies ? tensor : copies) + 16);
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = tn;
+    }
+  }
+  return best;
+}
+
+// Parts of a row tile's sum over the piece: as many as even out the rounds of tiles over the clusters, each of at least 16 blocks of k.
+static int ce_splits(int rows, int width, int piece, int clusters) {
+  const long long tiles = (long long)((rows + 255) / 256) * ((width + 255) / 256), blocks = (piece + kCeBlock - 1) / kCeBlock;
+  int best = 1;
+  double best_cost = -1.0;
+  for (int s = 1; s <= 64 && (s == 1 || blocks / s >= 16); ++s) {
+    const long long rounds = (tiles * s + clusters - 1) / clusters;
+    const double cost = (double)rounds * ((double)blocks / s + 8.0);      // a part costs its blocks and an epilogue of some eight blocks' time
+    if (best_cost < 0 || cost < best_cost * 0.97) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+static CePlan ce_plan(const CeArgs& a, bool backward) {
+  CePlan p = {};
+  p.planes = a.type == CE_F32 ? 3 : 1;
+  p.ldd = (int)ce_up_to(a.width, 8);
+  p.padded = (int)ce_up_to(a.rows, 256);
+  p.clusters = ce_sms() / 2 < 1 ? 1 : ce_sms() / 2;
+  p.packed = p.planes == 3 || a.ldw % 8 != 0 || (reinterpret_cast<uintptr_t>(a.weight) & 15) != 0;
+  // pieces of the vocabulary: half a gigabyte of dz and of the copied head, at least 4096 rows
+  long long most = ce_up_to(a.vocab, 256);
+  const long long room = 1ll << 29;
+  if (backward && room / (2ll * p.planes * p.padded) < most) most = room / (2ll * p.planes * p.padded);
+  if (p.packed && room / (2ll * p.planes * p.ldd) < most) most = room / (2ll * p.planes * p.ldd);
+  if (most < 4096) most = 4096;
+  p.pieces = (int)((a.vocab + most - 1) / most);
+  p.piece = (int)ce_up_to((a.vocab + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (a.vocab + p.piece - 1) / p.piece;
+  p.tile_v = ce_tile_columns(a.rows, p.piece < a.vocab ? p.piece : a.vocab, p.clusters);
+  p.splits = ce_splits(a.rows, a.width, p.piece, p.clusters);
+  long long at = 0;
+  auto take = [&](long long bytes) {
+    const long long place = at;
+    at = ce_up_to(at + bytes, 1024);
+    return place;
+  };
+  p.x = take(2ll * p.planes * p.padded * p.ldd);
+  p.w = p.packed ? take(2ll * p.planes * p.piece * p.ldd) : 0;
+  p.rows = take(8ll * p.padded);                       // forward: z at the target, the rows' losses; backward: their factors, the scale
+  if (!backward) {
+    p.parts = 2ll * p.pieces * ((p.piece + p.tile_v - 1) / p.tile_v);
+    p.part = take((a.smoothing != 0.0f ? 12ll : 8ll) * p.parts * p.padded);
+  } else {
+    p.dz = take(2ll * p.planes * p.padded * p.piece);
+    if (a.dhidden != nullptr && (p.splits > 1 || p.pieces > 1)) p.acc = take(4ll * p.splits * p.padded * a.width);
+  }
+  p.bytes = at;
+  return p;
+}
+
+static bool ce_tensor_map(CUtensorMap* map, const void* base, int type, long long inner, long long rows, long long ld, int planes, long long plane, int box_x, int box_y) {
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(planes > 1 ? plane * 2 : ld * 2)};
+  cuuint32_t box[3] = {(cuuint32_t)box_x, (cuuint32_t)box_y, 1}, estr[3] = {1, 1, 1};
+  return cuTensorMapEncodeTiled(map, type == CE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                                strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int MODE>
+static cudaError_t ce_launch(const CUtensorMap& am, const CUtensorMap& bm, const CeGemm& g, long long tiles, int clusters, cudaStream_t st) {
+  const size_t smem = 1024 + (size_t)kCeStages * 2 * kCeOperand;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(ce_gemm_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch_pdl(ce_gemm_kernel<T, MODE>, dim3(2 * (unsigned)(tiles < clusters ? tiles : clusters)), dim3(kCeThreads), smem, st, am, bm, g);
+}
+
+template <typename T>
+static cudaError_t ce_pack(const void* src, long long ld, long long row0, int rows, const int* count, const int* index, int width, void* dst, int ldd,
+                           long long plane, cudaStream_t st) {
+  const long long words = ce_up_to(rows, count != nullptr ? 256 : 1) * (ldd >> 3), blocks = (words + 255) / 256;
+  return launch_pdl(ce_pack_kernel<T>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const T*)src, ld, row0, rows, count, index,
+                    width, (uint16_t*)dst, ldd, plane);
+}
+
+// What the logits' product takes: maps of the live rows and of a piece's rows of the head.
+struct CeLogits {
+  CUtensorMap x, w;
+  int w_row;             // the piece's first row in its map
+};
+
+template <typename T>
+static bool ce_head_piece(const CeArgs& a, const CePlan& p, int c0, int rows, int box_x, int box_y, CUtensorMap* map, int* w_row) {
+  if (p.packed) {
+    *w_row = 0;
+    return ce_tensor_map(map, a.ws + p.w, a.type, a.width, rows, p.ldd, p.planes, (long long)p.piece * p.ldd, box_x, box_y);
+  }
+  *w_row = c0;
+  return ce_tensor_map(map, a.weight, a.type, a.width, c0 + rows, a.ldw, 1, 0, box_x, box_y);
+}
 
 template <typename T>
 static int ce_forward(const CeArgs& a, cudaStream_t st) {
-  float *part = (float*)a.ws, *zt = part + 3ll * ce_slots(a) * a.rows, *row_loss = zt + a.rows;
-  const CeHead<T> p = {(const T*)a.hidden, (const T*)a.weight, a.ldh, a.ldw, a.vocab, a.width};
-  ce_rows_kernel<<<1, 1024, 0, st>>>(a.targets, a.rows, a.vocab, a.ignore, a.live, a.reduce == CE_NONE ? a.loss : nullptr);
-  ce_lse_kernel<T><<<dim3(ce_slots(a), (a.rows + kCeTile - 1) / kCeTile), kCeThreads, 0, st>>>(p, a.live, part, zt, a.rows);
-  ce_merge_kernel<<<(a.rows + 255) / 256, 256, 0, st>>>(a.live, part, zt, a.rows, ce_slots(a), a.vocab, a.smoothing, row_loss,
-                                                       a.reduce == CE_NONE ? a.loss : nullptr);
-  if (a.reduce != CE_NONE) ce_total_kernel<<<1, 256, 0, st>>>(a.live, row_loss, a.reduce, a.loss);
-  return launch_status();
+  const CePlan p = ce_plan(a, false);
+  float *at_target = (float*)(a.ws + p.rows), *row_loss = at_target + p.padded;
+  float* part = (float*)(a.ws + p.part);
+  float* each = a.reduce == CE_NONE ? a.loss : nullptr;
+  cudaError_t e = launch_pdl(ce_rows_kernel, dim3(1), dim3(1024), 0, st, a.targets, a.rows, a.vocab, a.ignore, a.live, each);
+  if (e == cudaSuccess)
+    e = ce_pack<T>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.ws + p.x, p.ldd, (long long)p.padded * p.ldd, st);
+  CeGemm g = {};
+  g.rows = a.live; g.depth = a.width; g.tile_n = p.tile_v; g.a_rows = a.rows < 128 ? (int)ce_up_to(a.rows, 8) : 128;
+  g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded;
+  g.part_m = part; g.part_s = part + p.parts * p.padded; g.part_z = part + 2 * p.parts * p.padded; g.at_target = at_target;
+  CUtensorMap xm, wm;
+  if (!ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, (long long)p.padded * p.ldd, kCeBlock, g.a_rows)) return BONSAI_CUDA_BAD_ARG;
+  for (int c0 = 0; c0 < a.vocab && e == cudaSuccess; c0 += p.piece) {
+    const int rows = a.vocab - c0 < p.piece ? a.vocab - c0 : p.piece;
+    if (p.packed) e = ce_pack<T>(a.weight, a.ldw, c0, rows, nullptr, nullptr, a.width, a.ws + p.w, p.ldd, (long long)p.piece * p.ldd, st);
+    if (e != cudaSuccess) break;
+    if (!ce_head_piece<T>(a, p, c0, rows, kCeBlock, p.tile_v / 2, &wm, &g.w_row)) return BONSAI_CUDA_BAD_ARG;
+    g.c0 = c0; g.columns = rows;
+    const int ct = (rows + p.tile_v - 1) / p.tile_v;
+    e = ce_launch<T, CE_LSE>(xm, wm, g, (long long)(p.padded / 256) * ct, p.clusters, st);
+    g.slot += 2 * ct;
+  }
+  if (e == cudaSuccess)
+    e = launch_pdl(ce_merge_kernel, dim3((a.rows + 31) / 32), dim3(1024), 0, st, a.live, (const float*)g.part_m, (const float*)g.part_s, (const float*)g.part_z,
+                   (const float*)at_target, (long long)p.padded, g.slot, a.vocab, a.smoothing, row_loss, each);
+  if (e == cudaSuccess && a.reduce != CE_NONE) e = launch_pdl(ce_total_kernel, dim3(1), dim3(1024), 0, st, (const int*)a.live.count, (const float*)row_loss, a.reduce, a.loss);
+  return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
 template <typename T>
 static int ce_backward(const CeArgs& a, cudaStream_t st) {
-  const int piece = (int)ce_piece(a), row_tiles = (a.rows + kCeTile - 1) / kCeTile, d_tiles = (a.width + kCeTile - 1) / kCeTile;
-  float *dz = (float*)a.ws, *dh = dz + (long long)a.rows * piece;
-  const CeHead<T> p = {(const T*)a.hidden, (const T*)a.weight, a.ldh, a.ldw, a.vocab, a.width};
-  const CeUp u = {a.up, a.reduce};
-  for (int c0 = 0; c0 < a.vocab; c0 += piece) {
-    const int tiles = (piece + kCeTile - 1) / kCeTile;
-    ce_dz_kernel<T><<<dim3(tiles, row_tiles), kCeThreads, 0, st>>>(p, a.live, u, a.smoothing, c0, piece, dz);
-    if (a.dhidden != nullptr) ce_dh_kernel<T><<<dim3(d_tiles, row_tiles), kCeThreads, 0, st>>>(p, a.live, dz, c0, piece, c0 == 0, dh);
-    if (a.dweight != nullptr) ce_dw_kernel<T><<<dim3(d_tiles, tiles), kCeThreads, 0, st>>>(p, a.live, dz, c0, piece, (T*)a.dweight);
+  const CePlan p = ce_plan(a, true);
+  float *factor = (float*)(a.ws + p.rows), *scale = factor + p.padded;
+  if (a.dhidden != nullptr && cudaMemsetAsync(a.dhidden, 0, (size_t)a.rows * a.width * sizeof(T), st) != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
+  cudaError_t e = launch_pdl(ce_up_kernel, dim3(1), dim3(1024), 0, st, a.live, a.up, a.reduce, a.type == CE_F16 ? 32768.0f : 1.0f, factor, scale);
+  if (e == cudaSuccess)
+    e = ce_pack<T>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.ws + p.x, p.ldd, (long long)p.padded * p.ldd, st);
+  const long long x_plane = (long long)p.padded * p.ldd, z_plane = (long long)p.padded * p.piece;
+  CeGemm g = {};
+  g.rows = a.live; g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded; g.factor = factor; g.scale = scale;
+  g.a_rows = a.rows < 128 ? (int)ce_up_to(a.rows, 8) : 128;
+  g.dz = (uint16_t*)(a.ws + p.dz); g.ldz = p.piece; g.plane = z_plane; g.splits = p.splits; g.acc = (float*)(a.ws + p.acc);
+  CUtensorMap xm, wm, zm;
+  for (int c0 = 0; c0 < a.vocab && e == cudaSuccess; c0 += p.piece) {
+    const int rows = a.vocab - c0 < p.piece ? a.vocab - c0 : p.piece;
+    if (p.packed) e = ce_pack<T>(a.weight, a.ldw, c0, rows, nullptr, nullptr, a.width, a.ws + p.w, p.ldd, (long long)p.piece * p.ldd, st);
+    if (e != cudaSuccess) break;
+    g.c0 = c0;
+    if (!ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, x_plane, kCeBlock, g.a_rows) ||
+        !ce_head_piece<T>(a, p, c0, rows, kCeBlock, p.tile_v / 2, &wm, &g.w_row))
+      return BONSAI_CUDA_BAD_ARG;
+    g.columns = rows; g.depth = a.width; g.tile_n = p.tile_v;
+    e = ce_launch<T, CE_DZ>(xm, wm, g, (long long)(p.padded / 256) * ((rows + p.tile_v - 1) / p.tile_v), p.clusters, st);
+    g.columns = a.width; g.tile_n = 256;
+    const long long ct = (a.width + 255) / 256;
+    if (e == cudaSuccess && a.dhidden != nullptr) {
+      if (!ce_tensor_map(&zm, a.ws + p.dz, a.type, rows, p.padded, p.piece, p.planes, z_plane, kCeBlock, g.a_rows) ||
+          !ce_head_piece<T>(a, p, c0, rows, 64, kCeBlock, &wm, &g.w_row))
+        return BONSAI_CUDA_BAD_ARG;
+      g.depth = rows; g.first = c0 == 0; g.last = c0 + rows == a.vocab; g.out = a.dhidden;
+      e = ce_launch<T, CE_DH>(zm, wm, g, (p.padded / 256) * ct * p.splits, p.clusters, st);
+    }
+    if (e == cudaSuccess && a.dweight != nullptr) {
+      if (!ce_tensor_map(&zm, a.ws + p.dz, a.type, rows, p.padded, p.piece, p.planes, z_plane, 64, kCeBlock) ||
+          !ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, x_plane, 64, kCeBlock))
+        return BONSAI_CUDA_BAD_ARG;
+      g.m = rows; g.out = a.dweight;
+      e = ce_launch<T, CE_DW>(zm, xm, g, (rows + 255) / 256 * ct, p.clusters, st);
+    }
   }
-  if (a.dhidden != nullptr) {
-    if (cudaMemsetAsync(a.dhidden, 0, (size_t)a.rows * a.width * sizeof(T), st) != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
-    ce_scatter_kernel<T><<<a.rows, 256, 0, st>>>(a.live, dh, a.width, (T*)a.dhidden);
+  if (e == cudaSuccess && a.dhidden != nullptr && p.splits > 1) {
+    const long long blocks = ((long long)a.rows * a.width + 255) / 256;
+    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st, a.live, (const float*)g.acc, p.splits, (long long)p.padded,
+                   a.width, (const float*)scale, (T*)a.dhidden);
   }
-  return launch_status();
+  return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
 static bool ce_good(const CeArgs& a) {
-  return a.rows >= 1 && a.vocab >= 1 && a.width >= 1 && a.type >= CE_F32 && a.type <= CE_BF16 && a.reduce >= CE_MEAN && a.reduce <= CE_NONE;
+  return a.hidden != nullptr && a.weight != nullptr && a.rows >= 1 && a.vocab >= 1 && a.width >= 1 && a.ldh >= a.width && a.ldw >= a.width &&
+         a.rows < 0x7fffe000 && a.vocab < 0x7fffe000 && a.width < 0x7fffe000 && a.type >= CE_F32 && a.type <= CE_BF16 && a.reduce >= CE_MEAN &&
+         a.reduce <= CE_NONE;
+}
+
+static CeArgs ce_args(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce,
+                      float smoothing, int* live, float* lse2, void* ws, long long ws_bytes) {
+  CeArgs a = {};
+  a.hidden = hidden; a.weight = weight; a.ldh = ldh; a.ldw = ldw;
+  a.rows = rows; a.vocab = vocab; a.width = width; a.type = type; a.reduce = reduce; a.smoothing = smoothing;
+  if (live != nullptr) a.live = CeRows{live, live + 4, live + 4 + rows, lse2};
+  a.ws = (uint8_t*)ws; a.ws_bytes = ws_bytes;
+  return a;
 }
 
 }  // namespace bonsai
 
 extern "C" {
 
-long long bonsai_ce_workspace(int rows, int vocab, int width, int type, int backward, int want_hidden, int want_weight) {
+// Bytes of workspace of the calls below, for these arguments (dhidden of the backward call: wanted or not); -1 for arguments that are refused.
+long long bonsai_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type,
+                              float smoothing, int backward, int want_hidden) {
   using namespace bonsai;
-  CeArgs a = {};
-  a.rows = rows; a.vocab = vocab; a.width = width; a.type = type;
-  (void)want_hidden; (void)want_weight;
-  return ce_good(a) ? (backward ? ce_backward_bytes(a) : ce_forward_bytes(a)) : -1;
+  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, CE_MEAN, smoothing, nullptr, nullptr, nullptr, 0);
+  a.dhidden = want_hidden ? const_cast<void*>(hidden) : nullptr;
+  return ce_good(a) ? ce_plan(a, backward != 0).bytes : -1;
 }
 
-// hidden [rows][ldh], weight [vocab][ldw] of one type (0 f32, 1 f16, 2 bf16), targets [rows].  live: 4 + 2 rows int32, lse: rows f32; both are
-// filled here and read by the backward call.  loss: one f32, or one for each row (reduce 2).
+// hidden [rows][ldh], weight [vocab][ldw] of one type (0 f32, 1 f16, 2 bf16), targets [rows].  live: 4 + 2 rows int32, lse2: rows f32; both are
+// filled here and read by the backward call.  loss: one f32, or one for each row (reduce 2).  ws: 1024-byte aligned.
 int bonsai_ce_forward(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* targets, int rows, int vocab, int width,
-                      int type, long long ignore, int reduce, float smoothing, int* live, float* lse, float* loss, void* ws, long long ws_bytes,
+                      int type, long long ignore, int reduce, float smoothing, int* live, float* lse2, float* loss, void* ws, long long ws_bytes,
                       cudaStream_t st) {
   using namespace bonsai;
-  CeArgs a = {};
-  a.hidden = hidden; a.weight = weight; a.targets = targets; a.ldh = ldh; a.ldw = ldw; a.ignore = ignore;
-  a.rows = rows; a.vocab = vocab; a.width = width; a.type = type; a.reduce = reduce; a.smoothing = smoothing;
-  a.live = CeRows{live, live + 4, live + 4 + rows, lse};
-  a.loss = loss; a.ws = (uint8_t*)ws; a.ws_bytes = ws_bytes;
-  if (!ce_good(a) || hidden == nullptr || weight == nullptr || targets == nullptr || live == nullptr || lse == nullptr || loss == nullptr ||
-      ldh < width || ldw < width || ws == nullptr || ws_bytes < ce_forward_bytes(a))
+  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, lse2, ws, ws_bytes);
+  a.targets = targets; a.ignore = ignore; a.loss = loss;
+  if (!ce_good(a) || targets == nullptr || live == nullptr || lse2 == nullptr || loss == nullptr || ws == nullptr ||
+      (reinterpret_cast<uintptr_t>(ws) & 15) != 0 || ws_bytes < ce_plan(a, false).bytes)
     return BONSAI_CUDA_BAD_ARG;
   return type == CE_F32 ? ce_forward<float>(a, st) : type == CE_F16 ? ce_forward<__half>(a, st) : ce_forward<__nv_bfloat16>(a, st);
 }
 
 // up: d loss, one f32 or one for each row.  dhidden [rows][width], dweight [vocab][width] of the inputs' type; null: not wanted.
 int bonsai_ce_backward(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce,
-                       float smoothing, int* live, float* lse, const float* up, void* dhidden, void* dweight, void* ws, long long ws_bytes,
+                       float smoothing, int* live, float* lse2, const float* up, void* dhidden, void* dweight, void* ws, long long ws_bytes,
                        cudaStream_t st) {
   using namespace bonsai;
-  CeArgs a = {};
-  a.hidden = hidden; a.weight = weight; a.ldh = ldh; a.ldw = ldw;
-  a.rows = rows; a.vocab = vocab; a.width = width; a.type = type; a.reduce = reduce; a.smoothing = smoothing;
-  a.live = CeRows{live, live + 4, live + 4 + rows, lse};
-  a.up = up; a.dhidden = dhidden; a.dweight = dweight; a.ws = (uint8_t*)ws; a.ws_bytes = ws_bytes;
-  if (!ce_good(a) || hidden == nullptr || weight == nullptr || live == nullptr || lse == nullptr || up == nullptr || ldh < width || ldw < width ||
-      ws == nullptr || ws_bytes < ce_backward_bytes(a))
+  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, lse2, ws, ws_bytes);
+  a.up = up; a.dhidden = dhidden; a.dweight = dweight;
+  if (!ce_good(a) || live == nullptr || lse2 == nullptr || up == nullptr || ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) != 0 ||
+      ws_bytes < ce_plan(a, true).bytes)
     return BONSAI_CUDA_BAD_ARG;
   return type == CE_F32 ? ce_backward<float>(a, st) : type == CE_F16 ? ce_backward<__half>(a, st) : ce_backward<__nv_bfloat16>(a, st);
 }
