@@ -8,7 +8,10 @@
 // kernel makes them all (ce_gemm_kernel), on pairs of SMs with tcgen05.mma cta_group::2 over tiles of 256 x up to 256, and differs
 // by where its operands lie and what happens to a finished tile:
 //   CE_LSE  h [n][D] x W [V][D]: a row's maximum and sum of exponentials over its half of the tile's columns; no logit leaves the SM
-//   CE_DZ   the same product; exp(z - lse) - q in 16 bits into the piece's buffer [n][piece]
+//   CE_FEW  the same for up to 128 tokens, W [V][D] x h: the head's rows fill the tile and its columns are the tokens.  The head's bytes bound it, if
+//           the tensor cores leave them the power: one token in a tile of 256 rows had the card at 1 GHz under its cap, 294 us for the
+//           8B head where its bytes take 190
+//   CE_DZ   the product again; exp(z - lse) - q in 16 bits into the piece's buffer [n][piece]
 //   CE_DH   dz [n][piece] x W [piece][D], summed over the piece: W is read across its rows (MN-major operand), nothing is transposed
 //   CE_DW   dz^T [piece][n] x h [n][D]: both operands across their rows
 // The tensor cores bound all four where there are many tokens; with few, the head's bytes do.
@@ -20,8 +23,11 @@
 // upstream gradient's size (that factor enters with the products' sums), in f16 scaled by 2^15: probabilities down to 2^-29 stay normal.
 //
 // float32 inputs become three bfloat16 parts each (8 bits a part, exact down to 2^-24) and six products of parts: the parts that are left out
-// are below 2^-24 of the product.  The tensor cores' sums truncate, which over thousands of steps of one sign costs more than f32
-// rounding would; so every kCeSegment blocks the tile is added to registers with rounding.
+// are below 2^-24 of the product.
+//
+// The tensor cores' sums truncate: over a few hundred steps a logit of 10 loses some 1e-5, always downwards, which an f32 loss shows.  Where the result is f32
+// (the loss of any type, all products of f32) a tile is therefore added to registers, with rounding, every few blocks of k.  Gradients in 16 bits
+// round a hundred times coarser and take the tensor cores' sum as it is.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -33,7 +39,7 @@ namespace bonsai {
 
 enum CeType { CE_F32 = 0, CE_F16 = 1, CE_BF16 = 2 };
 enum CeReduce { CE_MEAN = 0, CE_SUM = 1, CE_NONE = 2 };
-enum CeMode { CE_LSE, CE_DZ, CE_DH, CE_DW };
+enum CeMode { CE_LSE, CE_FEW, CE_DZ, CE_DH, CE_DW };
 
 constexpr int kCeStages = 6;
 constexpr int kCeBlock = 64;                            // k per stage
@@ -41,8 +47,10 @@ constexpr int kCeOperand = 128 * kCeBlock * 2;          // 16 KB: a CTA's half o
 constexpr int kCeEpiWarps = 8;
 constexpr int kCeThreads = (kCeEpiWarps + 2) * 32;
 constexpr int kCeCols = 256;                            // TMEM columns of an accumulator, two of them
+constexpr int kCeFew = 128;                             // tokens up to which the head's rows fill the tile
 constexpr int kCeGroup = 16;                            // row tiles that share the head's tiles while those are in L2
-constexpr int kCeSegment = 2;                           // f32: blocks of k between two additions to registers
+constexpr int kCeStage = 32 * 128;                      // shared memory of an epilogue warp: 32 rows of 128 bytes on their way out
+constexpr int kCeSegment32 = 2, kCeSegment16 = 16;       // blocks of k between two additions to registers: f32, the loss of 16-bit types
 constexpr int kCeTerms = 6;
 constexpr float kCeLog2e = 1.4426950408889634f;
 __device__ const unsigned char kCeTermA[kCeTerms] = {2, 0, 1, 1, 0, 0}, kCeTermB[kCeTerms] = {0, 2, 1, 0, 1, 0};      // the small ones first
@@ -60,7 +68,7 @@ struct CeGemm {
   int depth;            // k: width (LSE, DZ), vocabulary rows of the piece (DH); DW: the live rows
   int m;                // DW: vocabulary rows of the piece
   int tile_n;           // columns of a tile, a multiple of 16
-  int a_rows;           // K-major A: rows of a copy
+  int a_rows;           // K-major A: rows of a copy; FEW: rows of the head in a CTA's half of a tile
   int c0;               // first vocabulary row of the piece; where the head's rows start in its tensor map: w_row
   int w_row;
   int vocab;
@@ -75,8 +83,8 @@ struct CeGemm {
   long long ldz, plane; // elements of a row, of a plane
   // DH, DW
   const float* scale;   // what the sums are multiplied by
-  int splits, first, last;
-  float* acc;           // DH: [splits][ldn][columns] sums of several pieces or parts
+  int piece_blocks, clusters, acc_rows, first, last;
+  float* acc;           // DH: [splits][live rows up to 256][columns] sums of several pieces or parts
   void* out;            // [..][columns] of the inputs' type
 };
 
@@ -208,13 +216,33 @@ __device__ __forceinline__ uint64_t ce_desc_mn(uint32_t smem_addr) {
   return (tc::smem_desc_sw128(smem_addr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(8192 >> 4) << 16);
 }
 
+// DH: parts into which the sum over a piece is cut, from the number of live rows, which only the device knows: as many as even out the rounds of
+// tiles over the clusters.  Costs are in times of one block of k (0.27 us): a part costs its blocks and an epilogue of some eight, and its sums are
+// written and read again at some 200 000 values in that time.  1640 live rows x 4096 over 50 688 vocabulary rows: one part, two rounds
+// for one and a half, 658 us; three parts 560.
+__device__ __forceinline__ int ce_splits(int n, int width, int piece_blocks, int terms, int clusters, int acc_rows) {
+  const int rows = (n + 255) & ~255, tiles = (rows >> 8) * ((width + 255) >> 8);
+  int best = 1;
+  float best_cost = 0.0f;
+  for (int s = 1; s <= 16 && (s == 1 || ((long long)s * rows <= acc_rows && piece_blocks / s >= 8)); ++s) {
+    const int rounds = (tiles * s + clusters - 1) / clusters;
+    const float cost = (float)rounds * ((float)piece_blocks * terms / s + 8.0f) + (s > 1 ? (float)s * n * width * 5e-6f : 0.0f);
+    if (s == 1 || cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
 template <int MODE>
 struct CeTiles {       // tiles of a launch, and which one has which number
-  int rt, ct, all;
-  __device__ __forceinline__ CeTiles(const CeGemm& p, int n) {
-    rt = ((MODE == CE_DW ? p.m : n) + 255) >> 8;
-    ct = (p.columns + p.tile_n - 1) / p.tile_n;
-    all = rt * ct * (MODE == CE_DH ? p.splits : 1);
+  int rt, ct, all, splits;
+  __device__ __forceinline__ CeTiles(const CeGemm& p, int n, int terms) {
+    rt = MODE == CE_FEW ? (n > 0 ? (p.columns + 2 * p.a_rows - 1) / (2 * p.a_rows) : 0) : ((MODE == CE_DW ? p.m : n) + 255) >> 8;
+    ct = MODE == CE_FEW ? 1 : (p.columns + p.tile_n - 1) / p.tile_n;
+    splits = MODE == CE_DH ? ce_splits(n, p.columns, p.piece_blocks, terms, p.clusters, p.acc_rows) : 1;
+    all = rt * ct * splits;
   }
   __device__ __forceinline__ void at(int i, int* r, int* c, int* split) const {
     *split = 0;
@@ -240,24 +268,124 @@ template <> __device__ __forceinline__ uint32_t ce_pack2<__nv_bfloat16>(float a,
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 32 neighbouring values of a row, `valid` of them inside
+// A warp's 32 rows on their way out: every thread has a row's values, 32 columns at a time, and writes them to shared memory (128 bytes a row, 16-byte
+// chunks swizzled); then eight threads store a row's chunks side by side, four rows per instruction.  From the rows' own threads each
+// store met 32 different lines, and rows of odd widths went value by value: 777 x 32003 x 1001 took 300 us for dW, 64 MB.
 template <typename T>
-__device__ __forceinline__ void ce_store32(T* dst, const float* v, int valid) {
-  if (valid >= 32 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+__device__ __forceinline__ void ce_stage(uint8_t* stage, int lane, int chunk0, const float* v) {
+  uint8_t* row = stage + lane * 128;
+#pragma unroll
+  for (int j = 0; j < (int)sizeof(T) * 2; ++j) {
+    uint4 w;
     if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      w = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        reinterpret_cast<uint4*>(dst)[j] = make_uint4(ce_pack2<T>(v[8 * j], v[8 * j + 1]), ce_pack2<T>(v[8 * j + 2], v[8 * j + 3]),
-                                                      ce_pack2<T>(v[8 * j + 4], v[8 * j + 5]), ce_pack2<T>(v[8 * j + 6], v[8 * j + 7]));
+      w = make_uint4(ce_pack2<T>(v[8 * j], v[8 * j + 1]), ce_pack2<T>(v[8 * j + 2], v[8 * j + 3]), ce_pack2<T>(v[8 * j + 4], v[8 * j + 5]),
+                     ce_pack2<T>(v[8 * j + 6], v[8 * j + 7]));
     }
+    *reinterpret_cast<uint4*>(row + (((chunk0 + j) ^ (lane & 7)) << 4)) = w;
+  }
+}
+
+// A row's 32 columns from its own thread (f32's parts of dz, 64 bytes each on aligned rows: staged they took twice as long)
+__device__ __forceinline__ void ce_store32(__nv_bfloat16* dst, const float* v, int valid) {
+  if (valid >= 32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      reinterpret_cast<uint4*>(dst)[j] = make_uint4(ce_pack2<__nv_bfloat16>(v[8 * j], v[8 * j + 1]), ce_pack2<__nv_bfloat16>(v[8 * j + 2], v[8 * j + 3]),
+                                                    ce_pack2<__nv_bfloat16>(v[8 * j + 4], v[8 * j + 5]), ce_pack2<__nv_bfloat16>(v[8 * j + 6], v[8 * j + 7]));
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j < valid) dst[j] = T(v[j]);
+      if (j < valid) dst[j] = __float2bfloat16_rn(v[j]);
   }
+}
+
+// dst: this thread's row, at the block's first column; `valid` of the staged columns are inside, `add`: f32 sums that are there already
+template <typename T>
+__device__ __forceinline__ void ce_flush(const uint8_t* stage, int lane, T* dst, bool ok, int valid, bool add = false) {
+  constexpr int kPer = 16 / sizeof(T);
+  __syncwarp();
+  const unsigned rows = __ballot_sync(0xffffffffu, ok), odd = __ballot_sync(0xffffffffu, ok && (reinterpret_cast<uintptr_t>(dst) & 15) != 0);
+  const unsigned long long mine = reinterpret_cast<unsigned long long>(dst);
+  if (odd == 0) {
+    const int c = lane & 7, n = valid - c * kPer;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      T* o = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, mine, r)) + c * kPer;
+      if (((rows >> r) & 1) == 0 || n <= 0) continue;
+      const uint4* from = reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+      if (n >= kPer) {
+        uint4 w = *from;
+        if constexpr (sizeof(T) == 4) {
+          if (add) {
+            const float4 a = *reinterpret_cast<const float4*>(o);
+            w = make_uint4(__float_as_uint(__uint_as_float(w.x) + a.x), __float_as_uint(__uint_as_float(w.y) + a.y),
+                           __float_as_uint(__uint_as_float(w.z) + a.z), __float_as_uint(__uint_as_float(w.w) + a.w));
+          }
+        }
+        *reinterpret_cast<uint4*>(o) = w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (j < n) {
+            T x = reinterpret_cast<const T*>(from)[j];
+            if constexpr (sizeof(T) == 4) {
+              if (add) x += o[j];
+            }
+            o[j] = x;
+          }
+      }
+    }
+  } else {
+    for (int r = 0; r < 32; ++r) {
+      T* o = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, mine, r));
+      if (((rows >> r) & 1) == 0) continue;
+#pragma unroll
+      for (int j = lane; j < 128 / (int)sizeof(T); j += 32)
+        if (j < valid) {
+          T x = *reinterpret_cast<const T*>(stage + r * 128 + (((j / kPer) ^ (r & 7)) << 4) + (j % kPer) * sizeof(T));
+          if constexpr (sizeof(T) == 4) {
+            if (add) x += o[j];
+          }
+          o[j] = x;
+        }
+    }
+  }
+  __syncwarp();
+}
+
+// `valid` of 32 neighbouring logits of a row into its running maximum (of z log2 e) and sums; at: the target's place among them
+__device__ __forceinline__ void ce_lse_add(float* v, int valid, bool with_z, int at, float* at_target, float& top, float& sum, float& sum_z) {
+  if (valid < 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j >= valid) v[j] = -INFINITY;
+  }
+  float m = v[0];
+#pragma unroll
+  for (int j = 1; j < 32; ++j) m = fmaxf(m, v[j]);
+  if (with_z) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) sum_z += j < valid ? v[j] : 0.0f;
+  }
+  if ((unsigned)at < 32u && at < valid) {          // behind the end it is another half's or tile's
+    float z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z = j == at ? v[j] : z;
+    *at_target = z;
+  }
+  m = fmaxf(top, m * kCeLog2e);
+  float s0 = 0.0f, s1 = 0.0f;
+  const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    s0 += ce_exp2(fmaf(v[j], kCeLog2e, -ref));
+    s1 += ce_exp2(fmaf(v[j + 1], kCeLog2e, -ref));
+  }
+  sum = sum * ce_exp2(top - ref) + (s0 + s1);
+  top = m;
 }
 
 // T: the inputs' type.  The operands in shared memory are T, or bfloat16 parts of f32.
@@ -265,7 +393,9 @@ template <typename T, int MODE>
 __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_gemm_kernel(const __grid_constant__ CUtensorMap amap,
                                                                                          const __grid_constant__ CUtensorMap bmap, const CeGemm p) {
   constexpr bool kF32 = sizeof(T) == 4, kAcross = MODE == CE_DH || MODE == CE_DW;      // B is MN-major
-  constexpr int kTerms = kF32 ? kCeTerms : 1;
+  constexpr int kTerms = kF32 ? kCeTerms : 1, kSegment = kF32 ? kCeSegment32 : kCeSegment16;
+  constexpr bool kSums = kF32 || MODE == CE_LSE || MODE == CE_FEW;           // sums in registers
+  constexpr int kChunks = MODE == CE_FEW ? 2 : 4;          // of 32 columns, in a half of a tile
   extern __shared__ uint8_t ce_smem[];
   uint8_t* base = (uint8_t*)(((uintptr_t)ce_smem + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
@@ -276,6 +406,10 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
   const uint32_t rank = blockIdx.x & 1;
   const int cid = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (MODE != CE_DW && p.a_rows < 128) {          // rows that no copy fills: zeros draw less power than what an earlier kernel has left there
+    for (int i = t; i < kCeStages * kCeOperand / 16; i += kCeThreads) reinterpret_cast<uint4*>(sA)[i] = make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async();
+  }
   if (warp == kCeEpiWarps + 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(2 * kCeCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -298,15 +432,15 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
   const uint32_t taddr = tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = *p.rows.count;
-  const CeTiles<MODE> tiles(p, n);
+  const CeTiles<MODE> tiles(p, n, kTerms);
   const int blocks_all = ((MODE == CE_DW ? n : p.depth) + kCeBlock - 1) / kCeBlock;
   // blocks of k that a part of a split tile takes
   auto part = [&](int split, int* b0, int* b1) {
     *b0 = 0;
     *b1 = blocks_all;
     if (MODE == CE_DH) {
-      *b0 = (int)((long long)blocks_all * split / p.splits);
-      *b1 = (int)((long long)blocks_all * (split + 1) / p.splits);
+      *b0 = (int)((long long)blocks_all * split / tiles.splits);
+      *b1 = (int)((long long)blocks_all * (split + 1) / tiles.splits);
     }
   };
 
@@ -321,7 +455,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         part(split, &b0, &b1);
         const int row0 = rt * 256 + (int)rank * 128, col0 = ct * p.tile_n + (int)rank * (p.tile_n >> 1);
         // rows behind the last live one are not copied: what lies in their place meets no other row
-        const bool has = MODE == CE_DW || row0 < n, other = MODE == CE_DW || rt * 256 + 128 < n;
+        const bool has = MODE == CE_DW || MODE == CE_FEW || row0 < n, other = MODE == CE_DW || MODE == CE_FEW || rt * 256 + 128 < n;
         const uint32_t abytes = MODE == CE_DW ? kCeOperand : (uint32_t)p.a_rows * kCeBlock * 2;
         const uint32_t bytes = abytes * (1 + (other ? 1 : 0)) + 2 * (kAcross ? (uint32_t)kCeOperand : (uint32_t)p.tile_n * kCeBlock);
         for (int kb = b0; kb < b1 && !failed; ++kb) {
@@ -334,6 +468,8 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
             if (MODE == CE_DW) {
               ce_load(a, &amap, row0, k, pa, bar);
               ce_load(a + 8192, &amap, row0 + 64, k, pa, bar);
+            } else if (MODE == CE_FEW) {
+              ce_load(a, &amap, k, p.w_row + (rt * 2 + (int)rank) * p.a_rows, pa, bar);
             } else if (has) {
               ce_load(a, &amap, k, row0, pa, bar);
             }
@@ -342,7 +478,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
               ce_load(b, &bmap, col0, kw, pb, bar);
               ce_load(b + 8192, &bmap, col0 + 64, kw, pb, bar);
             } else {
-              ce_load(b, &bmap, k, p.w_row + col0, pb, bar);
+              ce_load(b, &bmap, k, MODE == CE_FEW ? col0 : p.w_row + col0, pb, bar);
             }
             if (++s == kCeStages) { s = 0; phase ^= 1; }
           }
@@ -362,7 +498,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         tiles.at(tile, &rt, &ct, &split);
         part(split, &b0, &b1);
         for (int k0 = b0; k0 < b1 && !failed; ++seg) {
-          const int ab = seg & 1, k1 = kF32 ? min(b1, k0 + kCeSegment) : b1;
+          const int ab = seg & 1, k1 = kSums ? min(b1, k0 + kSegment) : b1;
           if (!tc::mbar_wait(&acce[ab], ((seg >> 1) & 1) ^ 1)) { failed = true; break; }
           tc::tc_fence_after();
           for (int i = 0; i < (k1 - k0) * kTerms; ++i) {
@@ -383,67 +519,70 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = warp >> 2;
+    const int quarter = warp & 3, half = warp >> 2, middle = ((p.tile_n >> 1) + 31) & ~31;      // a half's columns: 0 .. middle, middle .. tile_n
+    uint8_t* stage = base + kCeStages * 2 * kCeOperand + warp * kCeStage;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t drained[2] = {ce_map(tc::smem_u32(&acce[0]), 0), ce_map(tc::smem_u32(&acce[1]), 0)};
     bool failed = false;
     int seg = 0;
+    float few_top[2], few_sum[2], few_z[2];          // FEW: a thread's tokens, over all tiles
+    int few_target[2];
+    if (MODE == CE_FEW) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int token = (half ? middle : 0) + 32 * i + lane;
+        few_top[i] = -INFINITY;
+        few_sum[i] = few_z[i] = 0.0f;
+        few_target[i] = token < n ? p.rows.target[token] : -1;
+        if (few_target[i] < 0) few_target[i] = -0x40000000;          // in no tile
+      }
+    }
     for (int tile = cid; tile < tiles.all; tile += nclusters) {
       int rt, ct, split, b0, b1;
       tiles.at(tile, &rt, &ct, &split);
       part(split, &b0, &b1);
-      const int row = rt * 256 + (int)rank * 128 + quarter * 32 + lane, col0 = ct * p.tile_n, cols = min(p.tile_n, p.columns - col0);
+      const int row = rt * 256 + (int)rank * 128 + quarter * 32 + lane, col0 = ct * p.tile_n, cols = MODE == CE_FEW ? p.tile_n : min(p.tile_n, p.columns - col0);
       const bool live = row < (MODE == CE_DW ? p.m : n);
       // what a row brings
       float lse2 = 0.0f, f = 0.0f, scale = 0.0f;
       int target = -1;
       if (MODE == CE_LSE || MODE == CE_DZ) {
         if (live) target = p.rows.target[row] - p.c0 - col0;
-        if (target >= cols) target = -1;                      // another tile's, though it may lie in this one's last 32 columns
         if (MODE == CE_DZ && live) {
           lse2 = p.rows.lse2[row];
           f = p.factor[row];
         }
-      } else {
+      } else if (MODE != CE_FEW) {
         scale = *p.scale;
       }
       float top = -INFINITY, sum = 0.0f, sum_z = 0.0f;
 
+      // 16-bit rows go out 64 columns at a time, the last 32 of a half alone
+      const int begin = half ? middle : 0, end = min(cols, half ? p.tile_n : middle);
+      auto put16 = [&](const float* v, int c0, T* o, bool ok) {
+        if constexpr (!kF32) {
+          const int odd = ((c0 - begin) >> 5) & 1, first = c0 - 32 * odd;
+          ce_stage<T>(stage, lane, 4 * odd, v);
+          if (odd || c0 + 32 >= end) ce_flush<T>(stage, lane, o + first, ok, min(32 + 32 * odd, end - first));
+        }
+      };
       auto finish = [&](float* v, int c0) {      // columns c0 .. c0 + 31 of the tile
-        const int valid = cols - c0;
+        const int valid = end - c0;
         if (failed) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = NAN;
         }
         if constexpr (MODE == CE_LSE) {
-          if (valid < 32) {
+          ce_lse_add(v, valid, p.smoothing != 0.0f, target - c0, p.at_target + row, top, sum, sum_z);
+        } else if constexpr (MODE == CE_FEW) {
+          // the tile's rows are the head's: transposed through shared memory, a thread has a token's logits of 32 rows
+          ce_stage<float>(stage, lane, 0, v);
+          __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j >= valid) v[j] = -INFINITY;
-          }
-          float m = v[0];
-#pragma unroll
-          for (int j = 1; j < 32; ++j) m = fmaxf(m, v[j]);
-          if (p.smoothing != 0.0f) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sum_z += j < valid ? v[j] : 0.0f;
-          }
-          if ((unsigned)(target - c0) < 32u) {
-            float z = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z = j == target - c0 ? v[j] : z;
-            p.at_target[row] = z;
-          }
-          m = fmaxf(top, m * kCeLog2e);
-          float s0 = 0.0f, s1 = 0.0f;
-          const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            s0 += ce_exp2(fmaf(v[j], kCeLog2e, -ref));
-            s1 += ce_exp2(fmaf(v[j + 1], kCeLog2e, -ref));
-          }
-          sum = sum * ce_exp2(top - ref) + (s0 + s1);
-          top = m;
+          for (int j = 0; j < 32; ++j) v[j] = *reinterpret_cast<const float*>(stage + j * 128 + (((lane >> 2) ^ (j & 7)) << 4) + (lane & 3) * 4);
+          __syncwarp();
+          const int i = (c0 - begin) >> 5, v0 = (rt * 2 + (int)rank) * p.a_rows + quarter * 32, inside = min(p.a_rows - quarter * 32, p.columns - v0);
+          if (inside > 0) ce_lse_add(v, inside, p.smoothing != 0.0f, few_target[i] - p.c0 - v0, p.at_target + begin + 32 * i + lane, few_top[i], few_sum[i], few_z[i]);
         } else if constexpr (MODE == CE_DZ) {
           const float even = p.smoothing / (float)p.vocab, up = kF32 || __is_same(T, __nv_bfloat16) ? f : f * 32768.0f;
 #pragma unroll
@@ -457,13 +596,13 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.0f;
           }
-          uint16_t* o = p.dz + (long long)row * p.ldz + col0 + c0;
+          uint16_t* o = p.dz + (long long)row * p.ldz + col0;
           if constexpr (!kF32) {
-            ce_store32<T>(reinterpret_cast<T*>(o), v, valid);
+            put16(v, c0, reinterpret_cast<T*>(o), true);
           } else {
 #pragma unroll
             for (int k = 0; k < 3; ++k) {
-              ce_store32<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16*>(o + k * p.plane), v, valid);
+              ce_store32(reinterpret_cast<__nv_bfloat16*>(o + c0 + k * p.plane), v, valid);
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const float a = __bfloat162float(__float2bfloat16_rn(v[j]));
@@ -472,9 +611,9 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
             }
           }
         } else if constexpr (MODE == CE_DH) {
-          if (live) {
-            float* acc = p.acc + ((long long)split * p.ldn + row) * p.columns + col0 + c0;
-            if (!p.first) {
+          float* acc = p.acc + ((long long)split * ((n + 255) & ~255) + row) * p.columns + col0 + c0;
+          if (tiles.splits == 1 && p.last) {
+            if (!p.first && live) {
               if (valid >= 32 && (reinterpret_cast<uintptr_t>(acc) & 15) == 0) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -487,56 +626,67 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
                   if (j < valid) v[j] += acc[j];
               }
             }
-            if (p.splits == 1 && p.last) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= scale;
-              ce_store32<T>((T*)p.out + (long long)p.rows.index[row] * p.columns + col0 + c0, v, valid);
-            } else {
-              ce_store32<float>(acc, v, valid);
-            }
-          }
-        } else {
-          if (live) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= scale;
-            ce_store32<T>((T*)p.out + (long long)(p.c0 + row) * p.columns + col0 + c0, v, valid);
+            T* o = (T*)p.out + (long long)(live ? p.rows.index[row] : 0) * p.columns + col0;
+            if constexpr (!kF32) {
+              put16(v, c0, o, live);
+            } else {
+              ce_stage<float>(stage, lane, 0, v);
+              ce_flush<float>(stage, lane, o + c0, live, min(32, valid));
+            }
+          } else {
+            ce_stage<float>(stage, lane, 0, v);
+            ce_flush<float>(stage, lane, acc, live, min(32, valid), !p.first);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= scale;
+          T* o = (T*)p.out + (long long)(p.c0 + row) * p.columns + col0;
+          if constexpr (!kF32) {
+            put16(v, c0, o, live);
+          } else {
+            ce_stage<float>(stage, lane, 0, v);
+            ce_flush<float>(stage, lane, o + c0, live, min(32, valid));
           }
         }
       };
 
-      if constexpr (kF32) {
-        float acc[4][32];
+      if constexpr (kSums) {
+        float acc[kChunks][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kChunks; ++i)
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
 #pragma unroll 1
-        for (int k0 = b0; k0 < b1; k0 += kCeSegment, ++seg) {
+        for (int k0 = b0; k0 < b1; k0 += kSegment, ++seg) {
           const int ab = seg & 1;
           if (!failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg >> 1) & 1, lane)) failed = true;
           tc::tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t r[32];
-            tc::tmem_ld32(taddr + lane_base + ab * kCeCols + (half + 2 * i) * 32, r);
-            tc::tmem_wait_ld();
+          for (int i = 0; i < kChunks; ++i) {
+            if (begin + 32 * i < end) {
+              uint32_t r[32];
+              tc::tmem_ld32(taddr + lane_base + ab * kCeCols + begin + 32 * i, r);
+              tc::tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[i][j] += __uint_as_float(r[j]);
+              for (int j = 0; j < 32; ++j) acc[i][j] += __uint_as_float(r[j]);
+            }
           }
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) ce_arrive_at(drained[ab]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((half + 2 * i) * 32 < cols) finish(acc[i], (half + 2 * i) * 32);
+        for (int i = 0; i < kChunks; ++i)
+          if (begin + 32 * i < end) finish(acc[i], begin + 32 * i);
       } else {
         const bool none = b0 == b1;            // an empty sum: no live row
         const int ab = seg & 1;
         if (!none && !failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg >> 1) & 1, lane)) failed = true;
         tc::tc_fence_after();
 #pragma unroll 1
-        for (int c0 = half * 32; c0 < cols; c0 += 64) {
+        for (int c0 = begin; c0 < end; c0 += 32) {
           uint32_t r[32];
           float v[32];
           tc::tmem_ld32(taddr + lane_base + ab * kCeCols + c0, r);
@@ -559,6 +709,18 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         if (p.smoothing != 0.0f) p.part_z[at] = sum_z;
       }
     }
+    if (MODE == CE_FEW) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int token = (half ? middle : 0) + 32 * i + lane;
+        const long long at = (long long)(p.slot + (cid * 2 + (int)rank) * 4 + quarter) * p.ldn + token;
+        if (token < n && token < (half ? p.tile_n : middle)) {
+          p.part_m[at] = few_top[i];
+          p.part_s[at] = few_sum[i];
+          if (p.smoothing != 0.0f) p.part_z[at] = few_z[i];
+        }
+      }
+    }
   }
   tc::tc_fence_before();
   __syncwarp();
@@ -569,48 +731,56 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------------------------
-// 32 rows a block, a warp for every 32nd slot of their maxima and sums; then the row's loss
-__global__ void __launch_bounds__(1024) ce_merge_kernel(CeRows r, const float* __restrict__ part_m, const float* __restrict__ part_s, const float* __restrict__ part_z,
-                                                        const float* at_target, long long ldn, int slots, int vocab, float smoothing, float* row_loss, float* each) {
-  __shared__ float sm[32][33];
-  __shared__ double ss[32][33], sz[32][33];
+// Eight rows a block (a 32-byte sector of every slot's line), 64 threads for a row's slots; then the row's loss
+constexpr int kCeMergeRows = 8, kCeMergeLanes = 64;
+__global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(CeRows r, const float* __restrict__ part_m, const float* __restrict__ part_s,
+                                                                               const float* __restrict__ part_z, const float* at_target, long long ldn, int slots,
+                                                                               int vocab, float smoothing, float* row_loss, float* each) {
+  __shared__ float sm[kCeMergeLanes][kCeMergeRows];
+  __shared__ double ss[kCeMergeLanes][kCeMergeRows], sz[kCeMergeLanes][kCeMergeRows];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane, n = *r.count;
-  if (blockIdx.x * 32 >= n) return;
+  const int i = threadIdx.x % kCeMergeRows, l = threadIdx.x / kCeMergeRows, row = blockIdx.x * kCeMergeRows + i, n = *r.count;
+  if (blockIdx.x * kCeMergeRows >= n) return;
   float top = -INFINITY;
   double s = 0.0, z = 0.0;
-  bool bad = false;
   if (row < n) {
-#pragma unroll 4
-    for (int k = warp; k < slots; k += 32) {
-      const float m = part_m[k * ldn + row];
-      bad |= m != m;
-      top = fmaxf(top, m);
+    constexpr int U = 8;
+    for (int k = l; k < slots; k += U * kCeMergeLanes) {
+      float m[U], e[U], m8 = top, s8 = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = k + u * kCeMergeLanes;
+        m[u] = q < slots ? part_m[q * ldn + row] : -INFINITY;
+        e[u] = q < slots ? part_s[q * ldn + row] : 0.0f;
+        if (smoothing != 0.0f && q < slots) z += (double)part_z[q * ldn + row];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) m8 = fmaxf(m8, m[u]);
+      const float ref = m8 == -INFINITY ? 0.0f : m8;
+#pragma unroll
+      for (int u = 0; u < U; ++u) s8 += e[u] * ce_exp2(m[u] - ref);
+      s = s * (double)ce_exp2(top - ref) + (double)s8;
+      top = m8;
     }
-    const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-    for (int k = warp; k < slots; k += 32) {
-      s += (double)(part_s[k * ldn + row] * ce_exp2(part_m[k * ldn + row] - ref));
-      if (smoothing != 0.0f) z += (double)part_z[k * ldn + row];
-    }
-    if (bad) s = NAN;
   }
-  sm[warp][lane] = top;
-  ss[warp][lane] = s;
-  sz[warp][lane] = z;
-  __syncthreads();
-  if (warp == 0 && row < n) {
-    for (int w = 1; w < 32; ++w) top = fmaxf(top, sm[w][lane]);
-    s = z = 0.0;
-    for (int w = 0; w < 32; ++w) {
-      s += ss[w][lane] * (double)(sm[w][lane] == -INFINITY ? 0.0f : ce_exp2(sm[w][lane] - top));
-      z += sz[w][lane];
+  sm[l][i] = top;
+  ss[l][i] = s;
+  sz[l][i] = z;
+  for (int o = kCeMergeLanes / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (l < o) {
+      const float a = sm[l][i], b = sm[l + o][i], m = fmaxf(a, b), ref = m == -INFINITY ? 0.0f : m;
+      ss[l][i] = ss[l][i] * (double)ce_exp2(a - ref) + ss[l + o][i] * (double)ce_exp2(b - ref);
+      sz[l][i] += sz[l + o][i];
+      sm[l][i] = m;
     }
-    const double lse2 = (double)top + log2(s);
+  }
+  if (l == 0 && row < n) {
+    const double lse2 = (double)sm[0][i] + log2(ss[0][i]);
     r.lse2[row] = (float)lse2;
     double loss = lse2 * 0.69314718055994530942 - (double)(1.0f - smoothing) * (double)at_target[row];
-    if (smoothing != 0.0f) loss -= (double)smoothing * z / vocab;
+    if (smoothing != 0.0f) loss -= (double)smoothing * sz[0][i] / vocab;
     if (r.target[row] < 0) loss = NAN;
     row_loss[row] = (float)loss;
     if (each != nullptr) each[r.index[row]] = (float)loss;
@@ -661,10 +831,13 @@ __global__ void __launch_bounds__(1024) ce_up_kernel(CeRows r, const float* __re
 
 // dh: the parts' sums, to the rows' places
 template <typename T>
-__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, const float* __restrict__ acc, int splits, long long ldn, int width, const float* scale, T* out) {
+__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, const float* __restrict__ acc, int piece_blocks, int terms, int clusters, int acc_rows, int width, const float* scale,
+                                                      T* out) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n = *r.count;
+  const int n = *r.count, splits = ce_splits(n, width, piece_blocks, terms, clusters, acc_rows);
+  const long long ldn = (n + 255) & ~255;
+  if (splits == 1) return;          // the product has stored its tiles itself
   const float f = *scale;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n * width; i += (long long)gridDim.x * 256) {
     float v = 0.0f;
@@ -690,8 +863,9 @@ struct CeArgs {
 
 struct CePlan {
   int planes, ldd, padded, tile_v, clusters;
+  bool few;                    // the loss by CE_FEW
   bool packed;                 // the head is copied piece by piece: f32, or rows that TMA cannot take
-  int piece, pieces, splits;
+  int piece, pieces, acc_rows;
   long long x, w, parts, part, rows, dz, acc, bytes;      // places in the workspace, and its size
 };
 
@@ -721,22 +895,6 @@ static int ce_tile_columns(int rows, int vocab, int clusters) {
   return best;
 }
 
-// Parts of a row tile's sum over the piece: as many as even out the rounds of tiles over the clusters, each of at least 16 blocks of k.
-static int ce_splits(int rows, int width, int piece, int clusters) {
-  const long long tiles = (long long)((rows + 255) / 256) * ((width + 255) / 256), blocks = (piece + kCeBlock - 1) / kCeBlock;
-  int best = 1;
-  double best_cost = -1.0;
-  for (int s = 1; s <= 64 && (s == 1 || blocks / s >= 16); ++s) {
-    const long long rounds = (tiles * s + clusters - 1) / clusters;
-    const double cost = (double)rounds * ((double)blocks / s + 8.0);      // a part costs its blocks and an epilogue of some eight blocks' time
-    if (best_cost < 0 || cost < best_cost * 0.97) {
-      best_cost = cost;
-      best = s;
-    }
-  }
-  return best;
-}
-
 static CePlan ce_plan(const CeArgs& a, bool backward) {
   CePlan p = {};
   p.planes = a.type == CE_F32 ? 3 : 1;
@@ -754,7 +912,7 @@ static CePlan ce_plan(const CeArgs& a, bool backward) {
   p.piece = (int)ce_up_to((a.vocab + p.pieces - 1) / p.pieces, 256);
   p.pieces = (a.vocab + p.piece - 1) / p.piece;
   p.tile_v = ce_tile_columns(a.rows, p.piece < a.vocab ? p.piece : a.vocab, p.clusters);
-  p.splits = ce_splits(a.rows, a.width, p.piece, p.clusters);
+  p.acc_rows = p.padded + 4096;
   long long at = 0;
   auto take = [&](long long bytes) {
     const long long place = at;
@@ -765,11 +923,12 @@ static CePlan ce_plan(const CeArgs& a, bool backward) {
   p.w = p.packed ? take(2ll * p.planes * p.piece * p.ldd) : 0;
   p.rows = take(8ll * p.padded);                       // forward: z at the target, the rows' losses; backward: their factors, the scale
   if (!backward) {
-    p.parts = 2ll * p.pieces * ((p.piece + p.tile_v - 1) / p.tile_v);
+    p.few = a.rows <= kCeFew;
+    p.parts = p.few ? 8ll * p.clusters * p.pieces : 2ll * p.pieces * ((p.piece + p.tile_v - 1) / p.tile_v);
     p.part = take((a.smoothing != 0.0f ? 12ll : 8ll) * p.parts * p.padded);
   } else {
     p.dz = take(2ll * p.planes * p.padded * p.piece);
-    if (a.dhidden != nullptr && (p.splits > 1 || p.pieces > 1)) p.acc = take(4ll * p.splits * p.padded * a.width);
+    if (a.dhidden != nullptr) p.acc = take(4ll * p.acc_rows * a.width);
   }
   p.bytes = at;
   return p;
@@ -786,7 +945,7 @@ static bool ce_tensor_map(CUtensorMap* map, const void* base, int type, long lon
 
 template <typename T, int MODE>
 static cudaError_t ce_launch(const CUtensorMap& am, const CUtensorMap& bm, const CeGemm& g, long long tiles, int clusters, cudaStream_t st) {
-  const size_t smem = 1024 + (size_t)kCeStages * 2 * kCeOperand;
+  const size_t smem = 1024 + (size_t)kCeStages * 2 * kCeOperand + kCeEpiWarps * kCeStage;
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -837,19 +996,30 @@ static int ce_forward(const CeArgs& a, cudaStream_t st) {
   g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded;
   g.part_m = part; g.part_s = part + p.parts * p.padded; g.part_z = part + 2 * p.parts * p.padded; g.at_target = at_target;
   CUtensorMap xm, wm;
-  if (!ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, (long long)p.padded * p.ldd, kCeBlock, g.a_rows)) return BONSAI_CUDA_BAD_ARG;
+  if (p.few) g.tile_n = (int)ce_up_to(a.rows, 16);
+  if (!ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, (long long)p.padded * p.ldd, kCeBlock, p.few ? g.tile_n / 2 : g.a_rows))
+    return BONSAI_CUDA_BAD_ARG;
   for (int c0 = 0; c0 < a.vocab && e == cudaSuccess; c0 += p.piece) {
     const int rows = a.vocab - c0 < p.piece ? a.vocab - c0 : p.piece;
     if (p.packed) e = ce_pack<T>(a.weight, a.ldw, c0, rows, nullptr, nullptr, a.width, a.ws + p.w, p.ldd, (long long)p.piece * p.ldd, st);
     if (e != cudaSuccess) break;
-    if (!ce_head_piece<T>(a, p, c0, rows, kCeBlock, p.tile_v / 2, &wm, &g.w_row)) return BONSAI_CUDA_BAD_ARG;
     g.c0 = c0; g.columns = rows;
+    if (p.few) {          // rows of the head in a tile: the clusters have whole rounds of them
+      const int rounds = (rows + 256 * p.clusters - 1) / (256 * p.clusters), tiles = rounds * p.clusters;
+      g.a_rows = (int)ce_up_to((rows + 2 * tiles - 1) / (2 * tiles), 8);
+      if (!ce_head_piece<T>(a, p, c0, rows, kCeBlock, g.a_rows, &wm, &g.w_row)) return BONSAI_CUDA_BAD_ARG;
+      const int launched = (rows + 2 * g.a_rows - 1) / (2 * g.a_rows) < p.clusters ? (rows + 2 * g.a_rows - 1) / (2 * g.a_rows) : p.clusters;
+      e = ce_launch<T, CE_FEW>(wm, xm, g, launched, p.clusters, st);
+      g.slot += 8 * launched;
+      continue;
+    }
+    if (!ce_head_piece<T>(a, p, c0, rows, kCeBlock, p.tile_v / 2, &wm, &g.w_row)) return BONSAI_CUDA_BAD_ARG;
     const int ct = (rows + p.tile_v - 1) / p.tile_v;
     e = ce_launch<T, CE_LSE>(xm, wm, g, (long long)(p.padded / 256) * ct, p.clusters, st);
     g.slot += 2 * ct;
   }
   if (e == cudaSuccess)
-    e = launch_pdl(ce_merge_kernel, dim3((a.rows + 31) / 32), dim3(1024), 0, st, a.live, (const float*)g.part_m, (const float*)g.part_s, (const float*)g.part_z,
+    e = launch_pdl(ce_merge_kernel, dim3((a.rows + kCeMergeRows - 1) / kCeMergeRows), dim3(kCeMergeRows * kCeMergeLanes), 0, st, a.live, (const float*)g.part_m, (const float*)g.part_s, (const float*)g.part_z,
                    (const float*)at_target, (long long)p.padded, g.slot, a.vocab, a.smoothing, row_loss, each);
   if (e == cudaSuccess && a.reduce != CE_NONE) e = launch_pdl(ce_total_kernel, dim3(1), dim3(1024), 0, st, (const int*)a.live.count, (const float*)row_loss, a.reduce, a.loss);
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
@@ -867,7 +1037,8 @@ static int ce_backward(const CeArgs& a, cudaStream_t st) {
   CeGemm g = {};
   g.rows = a.live; g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded; g.factor = factor; g.scale = scale;
   g.a_rows = a.rows < 128 ? (int)ce_up_to(a.rows, 8) : 128;
-  g.dz = (uint16_t*)(a.ws + p.dz); g.ldz = p.piece; g.plane = z_plane; g.splits = p.splits; g.acc = (float*)(a.ws + p.acc);
+  g.dz = (uint16_t*)(a.ws + p.dz); g.ldz = p.piece; g.plane = z_plane; g.piece_blocks = p.piece / kCeBlock; g.clusters = p.clusters;
+  g.acc_rows = p.acc_rows; g.acc = (float*)(a.ws + p.acc);
   CUtensorMap xm, wm, zm;
   for (int c0 = 0; c0 < a.vocab && e == cudaSuccess; c0 += p.piece) {
     const int rows = a.vocab - c0 < p.piece ? a.vocab - c0 : p.piece;
@@ -886,7 +1057,7 @@ static int ce_backward(const CeArgs& a, cudaStream_t st) {
           !ce_head_piece<T>(a, p, c0, rows, 64, kCeBlock, &wm, &g.w_row))
         return BONSAI_CUDA_BAD_ARG;
       g.depth = rows; g.first = c0 == 0; g.last = c0 + rows == a.vocab; g.out = a.dhidden;
-      e = ce_launch<T, CE_DH>(zm, wm, g, (p.padded / 256) * ct * p.splits, p.clusters, st);
+      e = ce_launch<T, CE_DH>(zm, wm, g, p.clusters, p.clusters, st);
     }
     if (e == cudaSuccess && a.dweight != nullptr) {
       if (!ce_tensor_map(&zm, a.ws + p.dz, a.type, rows, p.padded, p.piece, p.planes, z_plane, 64, kCeBlock) ||
@@ -896,10 +1067,10 @@ static int ce_backward(const CeArgs& a, cudaStream_t st) {
       e = ce_launch<T, CE_DW>(zm, xm, g, (rows + 255) / 256 * ct, p.clusters, st);
     }
   }
-  if (e == cudaSuccess && a.dhidden != nullptr && p.splits > 1) {
+  if (e == cudaSuccess && a.dhidden != nullptr) {
     const long long blocks = ((long long)a.rows * a.width + 255) / 256;
-    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st, a.live, (const float*)g.acc, p.splits, (long long)p.padded,
-                   a.width, (const float*)scale, (T*)a.dhidden);
+    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st, a.live, (const float*)g.acc, g.piece_blocks,
+                   p.planes == 3 ? kCeTerms : 1, p.clusters, p.acc_rows, a.width, (const float*)scale, (T*)a.dhidden);
   }
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
