@@ -1082,11 +1082,11 @@ static bool ce_good(const CeArgs& a) {
 }
 
 static CeArgs ce_args(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce,
-                      float smoothing, int* live, float* lse2, void* ws, long long ws_bytes) {
+                      float smoothing, int* live, void* ws, long long ws_bytes) {
   CeArgs a = {};
   a.hidden = hidden; a.weight = weight; a.ldh = ldh; a.ldw = ldw;
   a.rows = rows; a.vocab = vocab; a.width = width; a.type = type; a.reduce = reduce; a.smoothing = smoothing;
-  if (live != nullptr) a.live = CeRows{live, live + 4, live + 4 + rows, lse2};
+  if (live != nullptr) a.live = CeRows{live, live + 4, live + 4 + rows, reinterpret_cast<float*>(live + 4 + 2ll * rows)};
   a.ws = (uint8_t*)ws; a.ws_bytes = ws_bytes;
   return a;
 }
@@ -1099,20 +1099,20 @@ extern "C" {
 long long bonsai_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type,
                               float smoothing, int backward, int want_hidden) {
   using namespace bonsai;
-  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, CE_MEAN, smoothing, nullptr, nullptr, nullptr, 0);
+  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, CE_MEAN, smoothing, nullptr, nullptr, 0);
   a.dhidden = want_hidden ? const_cast<void*>(hidden) : nullptr;
   return ce_good(a) ? ce_plan(a, backward != 0).bytes : -1;
 }
 
-// hidden [rows][ldh], weight [vocab][ldw] of one type (0 f32, 1 f16, 2 bf16), targets [rows].  live: 4 + 2 rows int32, lse2: rows f32; both are
+// hidden [rows][ldh], weight [vocab][ldw] of one type (0 f32, 1 f16, 2 bf16), targets [rows].  live: 4 + 3 rows words,
 // filled here and read by the backward call.  loss: one f32, or one for each row (reduce 2).  ws: 1024-byte aligned.
 int bonsai_ce_forward(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* targets, int rows, int vocab, int width,
-                      int type, long long ignore, int reduce, float smoothing, int* live, float* lse2, float* loss, void* ws, long long ws_bytes,
+                      int type, long long ignore, int reduce, float smoothing, int* live, float* loss, void* ws, long long ws_bytes,
                       cudaStream_t st) {
   using namespace bonsai;
-  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, lse2, ws, ws_bytes);
+  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, ws, ws_bytes);
   a.targets = targets; a.ignore = ignore; a.loss = loss;
-  if (!ce_good(a) || targets == nullptr || live == nullptr || lse2 == nullptr || loss == nullptr || ws == nullptr ||
+  if (!ce_good(a) || targets == nullptr || live == nullptr || loss == nullptr || ws == nullptr ||
       (reinterpret_cast<uintptr_t>(ws) & 15) != 0 || ws_bytes < ce_plan(a, false).bytes)
     return BONSAI_CUDA_BAD_ARG;
   return type == CE_F32 ? ce_forward<float>(a, st) : type == CE_F16 ? ce_forward<__half>(a, st) : ce_forward<__nv_bfloat16>(a, st);
@@ -1120,12 +1120,12 @@ int bonsai_ce_forward(const void* hidden, long long ldh, const void* weight, lon
 
 // up: d loss, one f32 or one for each row.  dhidden [rows][width], dweight [vocab][width] of the inputs' type; null: not wanted.
 int bonsai_ce_backward(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce,
-                       float smoothing, int* live, float* lse2, const float* up, void* dhidden, void* dweight, void* ws, long long ws_bytes,
+                       float smoothing, int* live, const float* up, void* dhidden, void* dweight, void* ws, long long ws_bytes,
                        cudaStream_t st) {
   using namespace bonsai;
-  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, lse2, ws, ws_bytes);
+  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, ws, ws_bytes);
   a.up = up; a.dhidden = dhidden; a.dweight = dweight;
-  if (!ce_good(a) || live == nullptr || lse2 == nullptr || up == nullptr || ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) != 0 ||
+  if (!ce_good(a) || live == nullptr || up == nullptr || ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) != 0 ||
       ws_bytes < ce_plan(a, true).bytes)
     return BONSAI_CUDA_BAD_ARG;
   return type == CE_F32 ? ce_backward<float>(a, st) : type == CE_F16 ? ce_backward<__half>(a, st) : ce_backward<__nv_bfloat16>(a, st);

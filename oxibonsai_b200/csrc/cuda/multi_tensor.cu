@@ -13,6 +13,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace bonsai {
@@ -41,9 +43,12 @@ template <> __device__ __forceinline__ void mt_store<float>(void* p, long long i
 template <> __device__ __forceinline__ void mt_store<__half>(void* p, long long i, float v) { ((__half*)p)[i] = __float2half_rn(v); }
 template <> __device__ __forceinline__ void mt_store<__nv_bfloat16>(void* p, long long i, float v) { ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v); }
 
+// eight neighbouring values as one access of 16 (16-bit types) or 32 bytes
 __device__ __forceinline__ void mt_load8(const float* p, float* v) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p)
+               : "memory");
 }
 __device__ __forceinline__ void mt_load8(const __half* p, float* v) {
   const uint4 u = *reinterpret_cast<const uint4*>(p);
@@ -61,8 +66,9 @@ __device__ __forceinline__ void mt_load8(const __nv_bfloat16* p, float* v) {
   for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
 __device__ __forceinline__ void mt_store8(float* p, const float* v) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]),
+               "f"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void mt_store8(__half* p, const float* v) {
   __half2 h[4];
@@ -77,20 +83,23 @@ __device__ __forceinline__ void mt_store8(__nv_bfloat16* p, const float* v) {
   *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
 }
 
-__device__ __forceinline__ bool mt_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+template <typename T>
+__device__ __forceinline__ bool mt_aligned(const T* p) { return (reinterpret_cast<uintptr_t>(p) & (8 * sizeof(T) - 1)) == 0; }
 
-// Runs one(i) for the values before the first place where every pointer is 16-byte aligned and behind the last whole eight, and
-// eight(i) for the eights between; pointers that never line up go value by value.
-template <typename Lined, typename One, typename Eight>
-__device__ __forceinline__ void mt_walk(long long lo, long long hi, Lined lined, One one, Eight eight) {
+// Runs one(i) for the values before the first place where every pointer is aligned for eight and behind the last whole eight, and
+// eights<n>(i, stride) for n eights at a time between; pointers that never line up go value by value.
+template <int U, typename Lined, typename One, typename Eights>
+__device__ __forceinline__ void mt_walk(long long lo, long long hi, Lined lined, One one, Eights eights) {
   const int t = threadIdx.x;
   int head = 0;
   while (head < 8 && !lined(lo + head)) ++head;
   const long long n8 = head < 8 && hi - lo > head ? (hi - lo - head) >> 3 : 0;
   if (n8 > 0) {
     if (t < head) one(lo + t);
-    for (long long i = t; i < n8; i += kMtThreads) eight(lo + head + 8 * i);
-    for (long long i = lo + head + 8 * n8 + t; i < hi; i += kMtThreads) one(i);
+    long long i = t;
+    for (; i + (U - 1) * kMtThreads < n8; i += U * kMtThreads) eights(std::integral_constant<int, U>(), lo + head + 8 * i);
+    for (; i < n8; i += kMtThreads) eights(std::integral_constant<int, 1>(), lo + head + 8 * i);
+    for (long long k = lo + head + 8 * n8 + t; k < hi; k += kMtThreads) one(k);
   } else {
     for (long long i = lo + t; i < hi; i += kMtThreads) one(i);
   }
@@ -124,20 +133,25 @@ template <typename T>
 __device__ __forceinline__ double mt_squares(const void* g, long long lo, long long hi) {
   double acc = 0.0;
   const T* p = (const T*)g;
-  mt_walk(
+  mt_walk<4>(
       lo, hi, [&](long long i) { return mt_aligned(p + i); },
       [&](long long i) { const double x = (double)mt_load<T>(p, i); acc += x * x; },
-      [&](long long i) {
-        float x[8];
-        mt_load8(p + i, x);
-        float s = 0.0f;
+      [&](auto count, long long i) {
+        constexpr int N = decltype(count)::value;
+        float x[N][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s = fmaf(x[k], x[k], s);
-        if (s > 1e-30f && s < 1e37f) {
-          acc += (double)s;
-        } else {                    // squares that leave the range of f32, zeros and NaN
+        for (int u = 0; u < N; ++u) mt_load8(p + i + u * 8ll * kMtThreads, x[u]);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) acc += (double)x[k] * (double)x[k];
+        for (int u = 0; u < N; ++u) {
+          float s = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s = fmaf(x[u][k], x[u][k], s);
+          if (s > 1e-30f && s < 1e37f) {
+            acc += (double)s;
+          } else {                    // squares that leave the range of f32, zeros and NaN
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc += (double)x[u][k] * (double)x[u][k];
+          }
         }
       });
   return acc;
@@ -195,15 +209,20 @@ template <typename T, typename O>
 __device__ __forceinline__ void mt_scale(const void* g, void* out, long long lo, long long hi, float share) {
   const T* p = (const T*)g;
   O* o = (O*)out;
-  mt_walk(
+  mt_walk<2>(
       lo, hi, [&](long long i) { return mt_aligned(p + i) && mt_aligned(o + i); },
       [&](long long i) { mt_store<O>(o, i, mt_load<T>(p, i) * share); },
-      [&](long long i) {
-        float x[8];
-        mt_load8(p + i, x);
+      [&](auto count, long long i) {
+        constexpr int N = decltype(count)::value;
+        float x[N][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] *= share;
-        mt_store8(o + i, x);
+        for (int u = 0; u < N; ++u) mt_load8(p + i + u * 8ll * kMtThreads, x[u]);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[u][k] *= share;
+          mt_store8(o + i + u * 8ll * kMtThreads, x[u]);
+        }
       });
 }
 
@@ -256,7 +275,7 @@ template <typename P, typename G>
 __device__ __forceinline__ void mt_adam(const MtAdamNow& a, void* pp, const void* gg, float* m, float* v, long long lo, long long hi) {
   P* p = (P*)pp;
   const G* g = (const G*)gg;
-  mt_walk(
+  mt_walk<1>(
       lo, hi, [&](long long i) { return mt_aligned(p + i) && mt_aligned(g + i) && mt_aligned(m + i) && mt_aligned(v + i); },
       [&](long long i) {
         float x = mt_load<P>(p, i), mi = m[i], vi = v[i];
@@ -265,7 +284,7 @@ __device__ __forceinline__ void mt_adam(const MtAdamNow& a, void* pp, const void
         m[i] = mi;
         v[i] = vi;
       },
-      [&](long long i) {
+      [&](auto, long long i) {
         float x[8], y[8], mi[8], vi[8];
         mt_load8(p + i, x);
         mt_load8(g + i, y);

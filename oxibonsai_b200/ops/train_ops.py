@@ -5,6 +5,7 @@ CUDA tensors go through the kernels, and a missing library raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Sequence
 
@@ -18,11 +19,12 @@ _SIG = {
     "bonsai_mt_norm": [_i, _vp, _vp, _vp, _vp, _vp, _vp],
     "bonsai_mt_clip": [_i, _vp, _vp, _vp, _vp, _vp, _d, _vp, _vp, _vp],
     "bonsai_ce_workspace": [_vp, _ll, _vp, _ll, _i, _i, _i, _i, C.c_float, _i, _i],
-    "bonsai_ce_forward": [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _ll, _i, C.c_float, _vp, _vp, _vp, _vp, _ll, _vp],
-    "bonsai_ce_backward": [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_ce_forward": [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _ll, _i, C.c_float, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_ce_backward": [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
     "bonsai_mt_adam": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _d, _vp, _d, _d, _d, _d, _i, _vp, _d, _vp, _vp, _vp],
 }
 _declared = False
+_HERE = contextlib.nullcontext()
 TYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -35,27 +37,43 @@ def _lib():
     return l
 
 
+def _on(device: torch.device):
+    """A context in which ``device`` is the current one."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    """The current stream's handle, without a stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 # ---- many tensors ---------------------------------------------------------------------------------------------------------------
 class TensorTable:
     """Addresses, sizes and types of dense CUDA tensors of one device, packed for the kernels.  Tensors without values are left out."""
 
     def __init__(self, tensors: Sequence[torch.Tensor]):
-        live = [t for t in tensors if t.numel()]
-        self.n = len(live)
-        self.ptrs = (C.c_void_p * max(1, self.n))(*[t.data_ptr() for t in live])
-        self.numel = (C.c_longlong * max(1, self.n))(*[t.numel() for t in live])
-        self.types = (C.c_ubyte * max(1, self.n))(*[TYPE_CODES[t.dtype] for t in live])
+        numel = [t.numel() for t in tensors]
+        if 0 in numel:
+            tensors = [t for t, n in zip(tensors, numel) if n]
+            numel = [n for n in numel if n]
+        self.n = len(numel)
+        self.ptrs = (C.c_void_p * max(1, self.n))(*[t.data_ptr() for t in tensors])
+        self.numel = (C.c_longlong * max(1, self.n))(*numel)
+        self.types = (C.c_ubyte * max(1, self.n))(*[TYPE_CODES[t.dtype] for t in tensors])
         self.partials = int(_lib().bonsai_mt_partials(self.n))
+
+
+def _norm_room(grads: TensorTable, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    return torch.empty((), dtype=torch.float32, device=device), torch.empty(grads.partials, dtype=torch.float64, device=device)
 
 
 def mt_norm(grads: TensorTable, device: torch.device) -> torch.Tensor:
     """The 2-norm over all values of a table's tensors: a 0-dim f32 tensor."""
     if grads.n == 0:
         return torch.zeros((), dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        partial = torch.empty(grads.partials, dtype=torch.float64, device=device)
-        K.check(_lib().bonsai_mt_norm(grads.n, grads.ptrs, grads.numel, grads.types, partial.data_ptr(), norm.data_ptr(), K.stream()), "mt_norm")
+    with _on(device):
+        norm, partial = _norm_room(grads, device)
+        K.check(_lib().bonsai_mt_norm(grads.n, grads.ptrs, grads.numel, grads.types, partial.data_ptr(), norm.data_ptr(), _stream(device)), "mt_norm")
     return norm
 
 
@@ -63,11 +81,10 @@ def mt_clip(grads: TensorTable, out: TensorTable, max_norm: float, device: torch
     """``out`` = ``grads`` scaled to a global norm of at most ``max_norm``; returns the norm before.  ``out`` may be ``grads``."""
     if grads.n == 0:
         return torch.zeros((), dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        partial = torch.empty(grads.partials, dtype=torch.float64, device=device)
+    with _on(device):
+        norm, partial = _norm_room(grads, device)
         K.check(_lib().bonsai_mt_clip(grads.n, grads.ptrs, out.ptrs, grads.numel, grads.types, out.types, max_norm, partial.data_ptr(),
-                                      norm.data_ptr(), K.stream()), "mt_clip")
+                                      norm.data_ptr(), _stream(device)), "mt_clip")
     return norm
 
 
@@ -76,15 +93,14 @@ def mt_adam(params: TensorTable, grads: TensorTable, m: TensorTable, v: TensorTa
     """One Adam step; ``step`` (int64 on the device) is raised by one.  With ``max_norm`` the gradients enter scaled to that global norm,
     and the norm before comes back."""
     device = step.device
-    with torch.cuda.device(device):
+    with _on(device):
         norm = partial = None
         if max_norm is not None:
-            norm = torch.empty((), dtype=torch.float32, device=device)
-            partial = torch.empty(grads.partials, dtype=torch.float64, device=device)
+            norm, partial = _norm_room(grads, device)
         lr_dev = lr if isinstance(lr, torch.Tensor) else None
         K.check(_lib().bonsai_mt_adam(params.n, params.ptrs, grads.ptrs, m.ptrs, v.ptrs, params.numel, params.types, grads.types,
                                       0.0 if lr_dev is not None else lr, K.ptr(lr_dev), betas[0], betas[1], eps, weight_decay, int(decoupled),
-                                      step.data_ptr(), 0.0 if max_norm is None else max_norm, K.ptr(partial), K.ptr(norm), K.stream()), "mt_adam")
+                                      step.data_ptr(), 0.0 if max_norm is None else max_norm, K.ptr(partial), K.ptr(norm), _stream(device)), "mt_adam")
     return norm
 
 
@@ -93,20 +109,19 @@ REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
 def linear_ce_forward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, reduction: str,
-                      label_smoothing: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                      label_smoothing: float) -> tuple[torch.Tensor, torch.Tensor]:
     """hidden [n, d], weight [v, d] (one type, unit stride along d), targets int64 [n] -> the loss (f32, 0-dim or [n]) and what the
     backward pass takes: the list of live rows and their log2 of the sum of exponentials."""
     (n, d), v, device = hidden.shape, weight.shape[0], hidden.device
     args = (hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0))
     code = TYPE_CODES[hidden.dtype]
-    with torch.cuda.device(device):
+    with _on(device):
         loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=device)
-        live = torch.empty(4 + 2 * n, dtype=torch.int32, device=device)
-        lse2 = torch.empty(n, dtype=torch.float32, device=device)
+        live = torch.empty(4 + 3 * n, dtype=torch.int32, device=device)          # their number, rows, targets, and lse2 as f32
         ws = _ce_workspace(args, n, v, d, code, label_smoothing, 0, 0, device)
         K.check(_lib().bonsai_ce_forward(*args, targets.data_ptr(), n, v, d, code, ignore_index, REDUCTIONS[reduction], label_smoothing, live.data_ptr(),
-                                         lse2.data_ptr(), loss.data_ptr(), ws.data_ptr(), ws.numel(), K.stream()), "linear_ce_forward")
-    return loss, live, lse2
+                                         loss.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device)), "linear_ce_forward")
+    return loss, live
 
 
 def _ce_workspace(args, n: int, v: int, d: int, code: int, label_smoothing: float, backward: int, want_hidden: int, device) -> torch.Tensor:
@@ -115,16 +130,16 @@ def _ce_workspace(args, n: int, v: int, d: int, code: int, label_smoothing: floa
     return torch.empty(size, dtype=torch.uint8, device=device)
 
 
-def linear_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, live: torch.Tensor, lse2: torch.Tensor, up: torch.Tensor, reduction: str,
+def linear_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, live: torch.Tensor, up: torch.Tensor, reduction: str,
                        label_smoothing: float, want_hidden: bool, want_weight: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """Gradients of :func:`linear_ce_forward`; ``up`` is the loss's gradient (f32, contiguous)."""
     (n, d), v, device = hidden.shape, weight.shape[0], hidden.device
     args = (hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0))
     code = TYPE_CODES[hidden.dtype]
-    with torch.cuda.device(device):
+    with _on(device):
         dh = torch.empty((n, d), dtype=hidden.dtype, device=device) if want_hidden else None
         dw = torch.empty((v, d), dtype=weight.dtype, device=device) if want_weight else None
         ws = _ce_workspace(args, n, v, d, code, label_smoothing, 1, int(want_hidden), device)
-        K.check(_lib().bonsai_ce_backward(*args, n, v, d, code, REDUCTIONS[reduction], label_smoothing, live.data_ptr(), lse2.data_ptr(), up.data_ptr(),
-                                          K.ptr(dh), K.ptr(dw), ws.data_ptr(), ws.numel(), K.stream()), "linear_ce_backward")
+        K.check(_lib().bonsai_ce_backward(*args, n, v, d, code, REDUCTIONS[reduction], label_smoothing, live.data_ptr(), up.data_ptr(),
+                                          K.ptr(dh), K.ptr(dw), ws.data_ptr(), ws.numel(), _stream(device)), "linear_ce_backward")
     return dh, dw

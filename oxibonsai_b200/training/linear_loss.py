@@ -63,21 +63,24 @@ def _cpu_backward(hidden, weight, targets, live, lse, up, reduction, smoothing, 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction, smoothing):
-        run = train_ops.linear_ce_forward if hidden.is_cuda else _cpu_forward
-        loss, live, lse = run(hidden, weight, targets, ignore_index, reduction, smoothing)
-        ctx.save_for_backward(hidden, weight, targets, live, lse)
+        if hidden.is_cuda:
+            loss, live = train_ops.linear_ce_forward(hidden, weight, targets, ignore_index, reduction, smoothing)
+            ctx.save_for_backward(hidden, weight, live)
+        else:
+            loss, live, lse = _cpu_forward(hidden, weight, targets, ignore_index, reduction, smoothing)
+            ctx.save_for_backward(hidden, weight, live, targets, lse)
         ctx.reduction, ctx.smoothing = reduction, smoothing
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, up):
-        hidden, weight, targets, live, lse = ctx.saved_tensors
+        hidden, weight, live, *cpu = ctx.saved_tensors
         want = ctx.needs_input_grad[:2]
-        up = up.to(lse.dtype).contiguous()
         if hidden.is_cuda:
-            dh, dw = train_ops.linear_ce_backward(hidden, weight, live, lse, up, ctx.reduction, ctx.smoothing, *want)
+            dh, dw = train_ops.linear_ce_backward(hidden, weight, live, up.contiguous(), ctx.reduction, ctx.smoothing, *want)
         else:
+            targets, lse = cpu
             dh, dw = _cpu_backward(hidden, weight, targets, live, lse, up, ctx.reduction, ctx.smoothing, *want)
         return dh, dw, None, None, None, None
 

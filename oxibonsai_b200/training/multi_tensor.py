@@ -20,6 +20,8 @@ _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 def _dense(t: torch.Tensor) -> bool:
     """Whether the values fill one stretch of memory, in whatever order of the axes."""
+    if t.is_contiguous():
+        return True
     want = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
         if stride != want:
@@ -29,19 +31,20 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.shape == b.shape and all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
+    return a.shape == b.shape and (a.stride() == b.stride() or all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1))
 
 
 def _check(tensors: Sequence[torch.Tensor], what: str) -> torch.device:
     device = None
     for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _TYPES:
+        if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES or t.layout != torch.strided:
             raise TypeError(f"{what}: dense float32, float16 or bfloat16 tensors are wanted, got "
                             f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
-        if device is not None and t.device != device:
+        if device is None:
+            device = t.device
+        elif t.device != device:
             raise ValueError(f"{what}: tensors of one device are wanted, got {device} and {t.device}")
-        device = t.device
-        if t.numel() and not _dense(t):
+        if not _dense(t) and t.numel():
             raise ValueError(f"{what}: a tensor of shape {tuple(t.shape)} has gaps or repeats in memory (strides {t.stride()})")
     if device is not None and device.type not in ("cuda", "cpu"):
         raise ValueError(f"{what}: CUDA or CPU tensors are wanted, got {device}")
@@ -50,10 +53,16 @@ def _check(tensors: Sequence[torch.Tensor], what: str) -> torch.device:
 
 def _check_apart(tensors: Iterable[torch.Tensor], what: str) -> None:
     """Tensors that are written must not share memory: two blocks would scale or step the same values."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
-    for (_, end), (begin, _) in zip(spans, spans[1:]):
-        if begin < end:
+    last = 0
+    for begin, size in sorted([(t.data_ptr(), t.nbytes) for t in tensors]):
+        if size and begin < last:
             raise ValueError(f"{what}: two of the tensors share memory")
+        last = max(last, begin + size)
+
+
+def _counters(tensors: Sequence[torch.Tensor]) -> list[torch.Tensor]:
+    """Tensors that have the version counters of all of these: views of one tensor share its counter."""
+    return list({id(t if t._base is None else t._base): t for t in tensors}.values())
 
 
 class GradientSet:
@@ -76,6 +85,7 @@ class GradientSet:
                 raise ValueError(f"GradientSet: out is on {self.out[0].device}, the gradients on {self.device}")
         # a tensor may be clipped onto itself and onto nothing else that the set holds
         _check_apart([g for g, o in zip(self.tensors, self.out) if g.data_ptr() != o.data_ptr() or g.dtype != o.dtype] + self.out, "GradientSet")
+        self._written = _counters(self.out)
         self._table = self._out_table = None
         if self.device.type == "cuda":
             self._table = train_ops.TensorTable(self.tensors)
@@ -84,14 +94,12 @@ class GradientSet:
     def __len__(self) -> int:
         return len(self.tensors)
 
-    @torch.no_grad()
     def norm(self) -> torch.Tensor:
         """sqrt(sum of all squares) as a 0-dim float32 tensor."""
         if self._table is not None:
             return train_ops.mt_norm(self._table, self.device)
         return _norm(self.tensors).float()
 
-    @torch.no_grad()
     def clip(self, max_norm: float) -> torch.Tensor:
         """Scales by ``max_norm / (norm + 1e-6)`` where the norm is above ``max_norm > 0`` (by 1 otherwise, as ``clip_grad_norm`` does)
         and returns the norm before.  A norm that is NaN scales nothing; an infinite one scales by 0."""
@@ -100,13 +108,15 @@ class GradientSet:
         else:
             n = _norm(self.tensors)
             share, norm = _share(float(n), max_norm), n.float()
-            for g, o in zip(self.tensors, self.out):
-                if share != 1.0 or g is not o:
-                    o.copy_(g.float() * share)
-        increment_version(self.out)
+            with torch.no_grad():
+                for g, o in zip(self.tensors, self.out):
+                    if share != 1.0 or g is not o:
+                        o.copy_(g.float() * share)
+        increment_version(self._written)
         return norm
 
 
+@torch.no_grad()
 def _norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     return sum((t.double().square().sum() for t in tensors), torch.zeros((), dtype=torch.float64)).sqrt()
 
@@ -117,12 +127,12 @@ def _share(norm: float, max_norm: float) -> float:
 
 def global_grad_norm(params: Iterable[torch.Tensor]) -> torch.Tensor:
     """``grad_norm`` as a 0-dim tensor on the gradients' device, in two launches."""
-    return GradientSet([p.grad.detach() for p in params if p.grad is not None]).norm()
+    return GradientSet([g for g in [p.grad for p in params] if g is not None]).norm()
 
 
 def clip_global_norm(params: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
     """``clip_grad_norm`` as a 0-dim tensor on the gradients' device, in two launches."""
-    return GradientSet([p.grad.detach() for p in params if p.grad is not None]).clip(max_norm)
+    return GradientSet([g for g in [p.grad for p in params] if g is not None]).clip(max_norm)
 
 
 class FusedAdam:
@@ -158,7 +168,10 @@ class FusedAdam:
         _check_apart(self.params + self.m + self.v, name)
         self.steps = torch.full((), steps, dtype=torch.int64, device=self.device)
         self.grads = None if grads is None else list(grads)
+        self._written = _counters(self.params)
         self._tables = None
+        if self.device.type == "cuda":
+            self._fixed = [train_ops.TensorTable(x) for x in (self.params, self.m, self.v)]
         if self.grads is not None:
             if len(self.grads) != len(self.params):
                 raise ValueError(f"{name}: {len(self.grads)} gradients for {len(self.params)} parameters")
@@ -166,14 +179,17 @@ class FusedAdam:
             if any(not _same_order(p, g) for p, g in zip(self.params, self.grads)):
                 raise ValueError(f"{name}: fixed gradients need their parameters' shapes and strides")
             if self.device.type == "cuda":
-                self._tables = [train_ops.TensorTable(x) for x in (self.params, self.grads, self.m, self.v)]
+                self._tables = self._with(self.grads)
+
+    def _with(self, grads: Sequence[torch.Tensor]) -> list[train_ops.TensorTable]:
+        return [self._fixed[0], train_ops.TensorTable(grads), *self._fixed[1:]]
 
     def _check_grads(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor]) -> None:
         name = type(self).__name__
         for p, g in zip(params, grads):
-            if g.layout != torch.strided or g.dtype not in _TYPES:
+            if g.dtype not in _TYPES or g.layout != torch.strided:
                 raise TypeError(f"{name}: dense float32, float16 or bfloat16 gradients are wanted, got {g.dtype} ({g.layout})")
-            if g.device != self.device or g.shape != p.shape:
+            if g.shape != p.shape or g.device != self.device:
                 raise ValueError(f"{name}: a gradient of shape {tuple(g.shape)} on {g.device} for a parameter of shape {tuple(p.shape)} on {p.device}")
 
     @property
@@ -181,7 +197,6 @@ class FusedAdam:
         """Steps done (waits for the GPU)."""
         return int(self.steps)
 
-    @torch.no_grad()
     def step(self, lr: float | torch.Tensor | None = None, max_norm: float | None = None) -> torch.Tensor | None:
         lr = self.lr if lr is None else lr
         if isinstance(lr, torch.Tensor) and (lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != self.device):
@@ -190,23 +205,27 @@ class FusedAdam:
             tables = self._tables
         else:
             grads = self.grads if self.grads is not None else [p.grad for p in self.params]
-            live = [i for i, g in enumerate(grads) if g is not None]
-            params, m, v = ([part[i] for i in live] for part in (self.params, self.m, self.v))
-            grads = [grads[i].detach() for i in live]
+            params, m, v, every = self.params, self.m, self.v, True
+            if any(g is None for g in grads):
+                live = [i for i, g in enumerate(grads) if g is not None]
+                params, grads, m, v = ([part[i] for i in live] for part in (params, grads, m, v))
+                every = False
             self._check_grads(params, grads)
             if self.device.type == "cpu":
                 return self._step_cpu(params, grads, m, v, float(lr), max_norm)
             # the kernel walks memory: a gradient that autograd laid out in another order than its parameter is copied into it
-            grads = [g if _same_order(p, g) else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
-            tables = [train_ops.TensorTable(x) for x in (params, grads, m, v)]
+            with torch.no_grad():
+                grads = [g if _same_order(p, g) else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
+            tables = self._with(grads) if every else [train_ops.TensorTable(x) for x in (params, grads, m, v)]
         if tables[0].n == 0:
             self.steps += 1
             return None if max_norm is None else torch.zeros((), dtype=torch.float32, device=self.device)
         norm = train_ops.mt_adam(*tables, self.steps, lr if isinstance(lr, torch.Tensor) else float(lr), self.betas, self.eps, self.wd, self.decoupled,
                                  None if max_norm is None else float(max_norm))
-        increment_version(self.params)
+        increment_version(self._written)
         return norm
 
+    @torch.no_grad()
     def _step_cpu(self, params, grads, m, v, lr: float, max_norm: float | None) -> torch.Tensor | None:
         self.steps += 1
         t, (b1, b2), norm, share = int(self.steps), self.betas, None, 1.0
