@@ -46,21 +46,37 @@ constexpr int kCeBlock = 64;                            // k per stage
 constexpr int kCeOperand = 128 * kCeBlock * 2;          // 16 KB: a CTA's half of one operand
 constexpr int kCeEpiWarps = 8;
 constexpr int kCeThreads = (kCeEpiWarps + 2) * 32;
-constexpr int kCeCols = 256;                            // TMEM columns of an accumulator, two of them
+constexpr int kCeCols = 512;                            // TMEM columns, for two accumulators of 256 or, with few tokens, four of 128
 constexpr int kCeFew = 128;                             // tokens up to which the head's rows fill the tile
 constexpr int kCeGroup = 16;                            // row tiles that share the head's tiles while those are in L2
 constexpr int kCeStage = 32 * 128;                      // shared memory of an epilogue warp: 32 rows of 128 bytes on their way out
-constexpr int kCeSegment32 = 2, kCeSegment16 = 16;       // blocks of k between two additions to registers: f32, the loss of 16-bit types
+constexpr int kCeSegment32 = 2, kCeSegment16 = 16, kCeSegmentFew = 4;          // blocks of k between two additions to registers
 constexpr int kCeTerms = 6;
 constexpr float kCeLog2e = 1.4426950408889634f;
 __device__ const unsigned char kCeTermA[kCeTerms] = {2, 0, 1, 1, 0, 0}, kCeTermB[kCeTerms] = {0, 2, 1, 0, 1, 0};      // the small ones first
 
 struct CeRows {         // the live rows, in order: filled by ce_rows_kernel
-  int* count;
+  int* count;           // [2]: how many; blocks of ce_merge_kernel that are done
   int* index;           // [N] row of the hidden states
   int* target;          // [N] its target, -1 outside the vocabulary
+  int* place;           // [N] the other way: place of a row in this list, -1 for ignored ones
   float* lse2;          // [N] log2 of the sum of exponentials
 };
+
+struct CeUp {           // the upstream gradient u: one value, or one for each row ("none")
+  const float* up;
+  const float* top;     // "none": max |u|
+  int reduce;
+  float dz_scale;       // what dz is stored with
+};
+__device__ __forceinline__ float ce_up_top(const CeUp& u) { return u.reduce == CE_NONE ? *u.top : fabsf(*u.up); }
+// u_i over the largest |u|; u is 0 or NaN where none is above 0
+__device__ __forceinline__ float ce_up_factor(const CeUp& u, const CeRows& r, int row) {
+  const float top = ce_up_top(u), x = u.up[u.reduce == CE_NONE ? r.index[row] : 0];
+  return r.target[row] < 0 ? NAN : top > 0.0f ? x / top : x;
+}
+// what the products' sums are multiplied by
+__device__ __forceinline__ float ce_up_scale(const CeUp& u, int n) { return n > 0 ? ce_up_top(u) / u.dz_scale / (u.reduce == CE_MEAN ? (float)n : 1.0f) : 0.0f; }
 
 struct CeGemm {
   CeRows rows;
@@ -78,11 +94,10 @@ struct CeGemm {
   long long ldn;
   int slot;             // first slot of this piece
   // DZ
-  const float* factor;  // [N] u_i over the largest one
+  CeUp up;
   uint16_t* dz;
   long long ldz, plane; // elements of a row, of a plane
   // DH, DW
-  const float* scale;   // what the sums are multiplied by
   int piece_blocks, clusters, acc_rows, first, last;
   float* acc;           // DH: [splits][live rows up to 256][columns] sums of several pieces or parts
   void* out;            // [..][columns] of the inputs' type
@@ -110,9 +125,11 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* __restri
       before += __shfl_xor_sync(0xffffffffu, before, o);
       all += __shfl_xor_sync(0xffffffffu, all, o);
     }
+    if (i < n && !live) r.place[i] = -1;
     if (live) {
       const int at = base + before + __popc(m & ((1u << lane) - 1));
       r.index[at] = i;
+      r.place[i] = at;
       r.target[at] = tgt >= 0 && tgt < vocab ? (int)tgt : -1;
     } else if (i < n && each != nullptr) {
       each[i] = 0.0f;
@@ -120,7 +137,10 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* __restri
     base += all;
     __syncthreads();
   }
-  if (t == 0) *r.count = base;
+  if (t == 0) {
+    r.count[0] = base;
+    r.count[1] = 0;
+  }
 }
 
 __device__ __forceinline__ float ce_f32(float x) { return x; }
@@ -393,14 +413,15 @@ template <typename T, int MODE>
 __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_gemm_kernel(const __grid_constant__ CUtensorMap amap,
                                                                                          const __grid_constant__ CUtensorMap bmap, const CeGemm p) {
   constexpr bool kF32 = sizeof(T) == 4, kAcross = MODE == CE_DH || MODE == CE_DW;      // B is MN-major
-  constexpr int kTerms = kF32 ? kCeTerms : 1, kSegment = kF32 ? kCeSegment32 : kCeSegment16;
+  constexpr int kTerms = kF32 ? kCeTerms : 1, kSegment = kF32 ? kCeSegment32 : MODE == CE_FEW ? kCeSegmentFew : kCeSegment16;
   constexpr bool kSums = kF32 || MODE == CE_LSE || MODE == CE_FEW;           // sums in registers
+  constexpr int kBufs = MODE == CE_FEW ? 4 : 2, kCols = kCeCols / kBufs;
   constexpr int kChunks = MODE == CE_FEW ? 2 : 4;          // of 32 columns, in a half of a tile
   extern __shared__ uint8_t ce_smem[];
   uint8_t* base = (uint8_t*)(((uintptr_t)ce_smem + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
   uint8_t* sB = base + kCeStages * kCeOperand;
-  __shared__ uint64_t full[kCeStages], empty[kCeStages], accf[2], acce[2];
+  __shared__ uint64_t full[kCeStages], empty[kCeStages], accf[kBufs], acce[kBufs];
   __shared__ uint32_t tmem_slot;
   const int t = threadIdx.x, warp = __shfl_sync(0xffffffffu, t >> 5, 0), lane = t & 31;
   const uint32_t rank = blockIdx.x & 1;
@@ -411,7 +432,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
     tc::fence_proxy_async();
   }
   if (warp == kCeEpiWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(2 * kCeCols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(kCeCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (t == 0) {
@@ -419,7 +440,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBufs; ++i) {
       tc::mbar_init(&accf[i], 1);
       tc::mbar_init(&acce[i], 2 * kCeEpiWarps);
     }
@@ -498,8 +519,8 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         tiles.at(tile, &rt, &ct, &split);
         part(split, &b0, &b1);
         for (int k0 = b0; k0 < b1 && !failed; ++seg) {
-          const int ab = seg & 1, k1 = kSums ? min(b1, k0 + kSegment) : b1;
-          if (!tc::mbar_wait(&acce[ab], ((seg >> 1) & 1) ^ 1)) { failed = true; break; }
+          const int ab = seg % kBufs, k1 = kSums ? min(b1, k0 + kSegment) : b1;
+          if (!tc::mbar_wait(&acce[ab], ((seg / kBufs) & 1) ^ 1)) { failed = true; break; }
           tc::tc_fence_after();
           for (int i = 0; i < (k1 - k0) * kTerms; ++i) {
             if (!tc::mbar_wait(&full[s], phase)) { failed = true; break; }
@@ -508,7 +529,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
             const uint64_t da = MODE == CE_DW ? ce_desc_mn(a) : tc::smem_desc_sw128(a), db = kAcross ? ce_desc_mn(b) : tc::smem_desc_sw128(b);
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k)
-              ce_mma(taddr + ab * kCeCols, da + (MODE == CE_DW ? 128 : 2) * k, db + (kAcross ? 128 : 2) * k, idesc, i > 0 || k > 0);
+              ce_mma(taddr + ab * kCols, da + (MODE == CE_DW ? 128 : 2) * k, db + (kAcross ? 128 : 2) * k, idesc, i > 0 || k > 0);
             ce_commit(&empty[s]);
             if (++s == kCeStages) { s = 0; phase ^= 1; }
           }
@@ -522,7 +543,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
     const int quarter = warp & 3, half = warp >> 2, middle = ((p.tile_n >> 1) + 31) & ~31;      // a half's columns: 0 .. middle, middle .. tile_n
     uint8_t* stage = base + kCeStages * 2 * kCeOperand + warp * kCeStage;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t drained[2] = {ce_map(tc::smem_u32(&acce[0]), 0), ce_map(tc::smem_u32(&acce[1]), 0)};
+    const uint32_t drained = ce_map(tc::smem_u32(&acce[0]), 0);
     bool failed = false;
     int seg = 0;
     float few_top[2], few_sum[2], few_z[2];          // FEW: a thread's tokens, over all tiles
@@ -550,10 +571,10 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         if (live) target = p.rows.target[row] - p.c0 - col0;
         if (MODE == CE_DZ && live) {
           lse2 = p.rows.lse2[row];
-          f = p.factor[row];
+          f = ce_up_factor(p.up, p.rows, row);
         }
       } else if (MODE != CE_FEW) {
-        scale = *p.scale;
+        scale = ce_up_scale(p.up, n);
       }
       float top = -INFINITY, sum = 0.0f, sum_z = 0.0f;
 
@@ -584,7 +605,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
           const int i = (c0 - begin) >> 5, v0 = (rt * 2 + (int)rank) * p.a_rows + quarter * 32, inside = min(p.a_rows - quarter * 32, p.columns - v0);
           if (inside > 0) ce_lse_add(v, inside, p.smoothing != 0.0f, few_target[i] - p.c0 - v0, p.at_target + begin + 32 * i + lane, few_top[i], few_sum[i], few_z[i]);
         } else if constexpr (MODE == CE_DZ) {
-          const float even = p.smoothing / (float)p.vocab, up = kF32 || __is_same(T, __nv_bfloat16) ? f : f * 32768.0f;
+          const float even = p.smoothing / (float)p.vocab, up = f * p.up.dz_scale;
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = up * (ce_exp2(fmaf(v[j], kCeLog2e, -lse2)) - even);
           if ((unsigned)(target - c0) < 32u) {
@@ -660,14 +681,14 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
           for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
 #pragma unroll 1
         for (int k0 = b0; k0 < b1; k0 += kSegment, ++seg) {
-          const int ab = seg & 1;
-          if (!failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg >> 1) & 1, lane)) failed = true;
+          const int ab = seg % kBufs;
+          if (!failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg / kBufs) & 1, lane)) failed = true;
           tc::tc_fence_after();
 #pragma unroll
           for (int i = 0; i < kChunks; ++i) {
             if (begin + 32 * i < end) {
               uint32_t r[32];
-              tc::tmem_ld32(taddr + lane_base + ab * kCeCols + begin + 32 * i, r);
+              tc::tmem_ld32(taddr + lane_base + ab * kCols + begin + 32 * i, r);
               tc::tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; ++j) acc[i][j] += __uint_as_float(r[j]);
@@ -675,21 +696,21 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
           }
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ce_arrive_at(drained[ab]);
+          if (lane == 0) ce_arrive_at(drained + ab * 8);
         }
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
           if (begin + 32 * i < end) finish(acc[i], begin + 32 * i);
       } else {
         const bool none = b0 == b1;            // an empty sum: no live row
-        const int ab = seg & 1;
-        if (!none && !failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg >> 1) & 1, lane)) failed = true;
+        const int ab = seg % kBufs;
+        if (!none && !failed && !tc::mbar_wait_warp<64>(&accf[ab], (seg / kBufs) & 1, lane)) failed = true;
         tc::tc_fence_after();
 #pragma unroll 1
         for (int c0 = begin; c0 < end; c0 += 32) {
           uint32_t r[32];
           float v[32];
-          tc::tmem_ld32(taddr + lane_base + ab * kCeCols + c0, r);
+          tc::tmem_ld32(taddr + lane_base + ab * kCols + c0, r);
           tc::tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = none ? 0.0f : __uint_as_float(r[j]);
@@ -698,7 +719,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         if (!none) {
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ce_arrive_at(drained[ab]);
+          if (lane == 0) ce_arrive_at(drained + ab * 8);
           ++seg;
         }
       }
@@ -727,21 +748,23 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
   ce_cluster_sync();                 // nobody leaves while the other CTA may still read its shared memory or TMEM, or signal it
   tc::tc_fence_after();
   if (warp == kCeEpiWarps + 1)
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(2 * kCeCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(kCeCols) : "memory");
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------------------------
-// Eight rows a block (a 32-byte sector of every slot's line), 64 threads for a row's slots; then the row's loss
+// Eight rows a block (a 32-byte sector of every slot's line), 64 threads for a row's slots; then the row's loss.  The last block to finish
+// adds up the rows, in their order.
 constexpr int kCeMergeRows = 8, kCeMergeLanes = 64;
 __global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(CeRows r, const float* __restrict__ part_m, const float* __restrict__ part_s,
                                                                                const float* __restrict__ part_z, const float* at_target, long long ldn, int slots,
-                                                                               int vocab, float smoothing, float* row_loss, float* each) {
+                                                                               int vocab, float smoothing, int reduce, float* row_loss, float* loss) {
   __shared__ float sm[kCeMergeLanes][kCeMergeRows];
   __shared__ double ss[kCeMergeLanes][kCeMergeRows], sz[kCeMergeLanes][kCeMergeRows];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int i = threadIdx.x % kCeMergeRows, l = threadIdx.x / kCeMergeRows, row = blockIdx.x * kCeMergeRows + i, n = *r.count;
-  if (blockIdx.x * kCeMergeRows >= n) return;
+  const int blocks = n > 0 ? (n + kCeMergeRows - 1) / kCeMergeRows : 1;
+  if (blockIdx.x >= blocks) return;
   float top = -INFINITY;
   double s = 0.0, z = 0.0;
   if (row < n) {
@@ -779,70 +802,67 @@ __global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(
   if (l == 0 && row < n) {
     const double lse2 = (double)sm[0][i] + log2(ss[0][i]);
     r.lse2[row] = (float)lse2;
-    double loss = lse2 * 0.69314718055994530942 - (double)(1.0f - smoothing) * (double)at_target[row];
-    if (smoothing != 0.0f) loss -= (double)smoothing * sz[0][i] / vocab;
-    if (r.target[row] < 0) loss = NAN;
-    row_loss[row] = (float)loss;
-    if (each != nullptr) each[r.index[row]] = (float)loss;
+    double x = lse2 * 0.69314718055994530942 - (double)(1.0f - smoothing) * (double)at_target[row];
+    if (smoothing != 0.0f) x -= (double)smoothing * sz[0][i] / vocab;
+    if (r.target[row] < 0) x = NAN;
+    if (reduce == CE_NONE)
+      loss[r.index[row]] = (float)x;
+    else
+      row_loss[row] = (float)x;
   }
-}
-
-__global__ void __launch_bounds__(1024) ce_total_kernel(const int* count, const float* __restrict__ row_loss, int reduce, float* loss) {
-  __shared__ double s[32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n = *count;
-  double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) v += (double)row_loss[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  if (reduce == CE_NONE) return;
+  __shared__ int last;
+  __threadfence();
   __syncthreads();
-  if (threadIdx.x < 32) {
-    v = s[threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (threadIdx.x == 0) *loss = (float)(reduce == CE_MEAN ? v / (double)n : v);
+  if (threadIdx.x == 0) last = atomicAdd(r.count + 1, 1) == blocks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double v = 0.0;
+  for (int k = threadIdx.x; k < n; k += kCeMergeRows * kCeMergeLanes) v += (double)__ldcg(row_loss + k);
+  double* sums = &ss[0][0];
+  sums[threadIdx.x] = v;
+  for (int o = kCeMergeRows * kCeMergeLanes / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
   }
+  if (threadIdx.x == 0) *loss = (float)(reduce == CE_MEAN ? sums[0] / (double)n : sums[0]);
 }
 
-// factor_i = u_i / max |u|, scale = max |u| over what dz is stored with
-__global__ void __launch_bounds__(1024) ce_up_kernel(CeRows r, const float* __restrict__ up, int reduce, float dz_scale, float* factor, float* scale) {
+// max |u| over the live rows
+__global__ void __launch_bounds__(1024) ce_top_kernel(CeRows r, const float* __restrict__ up, float* out) {
   __shared__ float s[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = *r.count;
   float top = 0.0f;
-  if (reduce == CE_NONE) {
-    for (int i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, fabsf(up[r.index[i]]));
-  } else {
-    top = fabsf(up[0]);
-  }
+  for (int i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, fabsf(up[r.index[i]]));
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = top;
   __syncthreads();
   top = warp_max(s[threadIdx.x & 31]);
-  for (int i = threadIdx.x; i < n; i += 1024) {
-    const float u = reduce == CE_NONE ? up[r.index[i]] : up[0];
-    factor[i] = r.target[i] < 0 ? NAN : top > 0.0f ? u / top : u;      // u is 0 or NaN where no |u| is above 0
-  }
-  if (threadIdx.x == 0) *scale = n > 0 ? top / dz_scale / (reduce == CE_MEAN ? (float)n : 1.0f) : 0.0f;
+  if (threadIdx.x == 0) *out = top;
 }
 
-// dh: the parts' sums, to the rows' places
+// dh: zeros for ignored rows, and the parts' sums where there are several
 template <typename T>
-__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, const float* __restrict__ acc, int piece_blocks, int terms, int clusters, int acc_rows, int width, const float* scale,
-                                                      T* out) {
+__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, CeUp u, const float* __restrict__ acc, int rows, int piece_blocks, int terms, int clusters, int acc_rows,
+                                                      int width, T* out) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = *r.count, splits = ce_splits(n, width, piece_blocks, terms, clusters, acc_rows);
+  if (splits == 1 && n == rows) return;          // the product has stored its tiles itself
   const long long ldn = (n + 255) & ~255;
-  if (splits == 1) return;          // the product has stored its tiles itself
-  const float f = *scale;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n * width; i += (long long)gridDim.x * 256) {
-    float v = 0.0f;
-    for (int k = 0; k < splits; ++k) v += acc[k * ldn * width + i];
-    out[(long long)r.index[i / width] * width + i % width] = T(v * f);
+  const float f = ce_up_scale(u, n);
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int at = r.place[row];
+    if (at >= 0 && splits == 1) continue;
+    for (int d = threadIdx.x; d < width; d += 256) {
+      float v = 0.0f;
+      if (at >= 0)
+        for (int k = 0; k < splits; ++k) v += acc[(k * ldn + at) * width + d];
+      out[(long long)row * width + d] = T(v * f);
+    }
   }
 }
 
@@ -854,11 +874,11 @@ struct CeArgs {
   int rows, vocab, width, type, reduce;
   float smoothing;
   CeRows live;
+  uint16_t* x;          // the live rows side by side, kept between the calls
   float* loss;
   const float* up;
   void *dhidden, *dweight;
   uint8_t* ws;
-  long long ws_bytes;
 };
 
 struct CePlan {
@@ -866,14 +886,16 @@ struct CePlan {
   bool few;                    // the loss by CE_FEW
   bool packed;                 // the head is copied piece by piece: f32, or rows that TMA cannot take
   int piece, pieces, acc_rows;
-  long long x, w, parts, part, rows, dz, acc, bytes;      // places in the workspace, and its size
+  long long lists, kept;       // bytes of one of the live rows' lists, and of all that the forward call keeps for the backward one
+  long long w, parts, part, rows, dz, acc, bytes;      // places in the workspace, and its size
 };
 
 static long long ce_up_to(long long v, long long unit) { return (v + unit - 1) / unit * unit; }
 
 static int ce_sms() {
   int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // the driver encodes tensor maps in the calling thread's context, and a thread that has launched nothing yet (autograd's) has none
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
 }
 
@@ -919,9 +941,10 @@ static CePlan ce_plan(const CeArgs& a, bool backward) {
     at = ce_up_to(at + bytes, 1024);
     return place;
   };
-  p.x = take(2ll * p.planes * p.padded * p.ldd);
+  p.lists = ce_up_to(4ll * a.rows, 256);
+  p.kept = 256 + 4 * p.lists + 2ll * p.planes * p.padded * p.ldd;
   p.w = p.packed ? take(2ll * p.planes * p.piece * p.ldd) : 0;
-  p.rows = take(8ll * p.padded);                       // forward: z at the target, the rows' losses; backward: their factors, the scale
+  p.rows = take(8ll * p.padded);                       // forward: z at the target, the rows' losses; backward: max |u|
   if (!backward) {
     p.few = a.rows <= kCeFew;
     p.parts = p.few ? 8ll * p.clusters * p.pieces : 2ll * p.pieces * ((p.piece + p.tile_v - 1) / p.tile_v);
@@ -983,21 +1006,20 @@ static bool ce_head_piece(const CeArgs& a, const CePlan& p, int c0, int rows, in
 }
 
 template <typename T>
-static int ce_forward(const CeArgs& a, cudaStream_t st) {
-  const CePlan p = ce_plan(a, false);
+static int ce_forward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
   float *at_target = (float*)(a.ws + p.rows), *row_loss = at_target + p.padded;
   float* part = (float*)(a.ws + p.part);
   float* each = a.reduce == CE_NONE ? a.loss : nullptr;
   cudaError_t e = launch_pdl(ce_rows_kernel, dim3(1), dim3(1024), 0, st, a.targets, a.rows, a.vocab, a.ignore, a.live, each);
   if (e == cudaSuccess)
-    e = ce_pack<T>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.ws + p.x, p.ldd, (long long)p.padded * p.ldd, st);
+    e = ce_pack<T>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.x, p.ldd, (long long)p.padded * p.ldd, st);
   CeGemm g = {};
   g.rows = a.live; g.depth = a.width; g.tile_n = p.tile_v; g.a_rows = a.rows < 128 ? (int)ce_up_to(a.rows, 8) : 128;
   g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded;
   g.part_m = part; g.part_s = part + p.parts * p.padded; g.part_z = part + 2 * p.parts * p.padded; g.at_target = at_target;
   CUtensorMap xm, wm;
   if (p.few) g.tile_n = (int)ce_up_to(a.rows, 16);
-  if (!ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, (long long)p.padded * p.ldd, kCeBlock, p.few ? g.tile_n / 2 : g.a_rows))
+  if (!ce_tensor_map(&xm, a.x, a.type, a.width, p.padded, p.ldd, p.planes, (long long)p.padded * p.ldd, kCeBlock, p.few ? g.tile_n / 2 : g.a_rows))
     return BONSAI_CUDA_BAD_ARG;
   for (int c0 = 0; c0 < a.vocab && e == cudaSuccess; c0 += p.piece) {
     const int rows = a.vocab - c0 < p.piece ? a.vocab - c0 : p.piece;
@@ -1020,22 +1042,19 @@ static int ce_forward(const CeArgs& a, cudaStream_t st) {
   }
   if (e == cudaSuccess)
     e = launch_pdl(ce_merge_kernel, dim3((a.rows + kCeMergeRows - 1) / kCeMergeRows), dim3(kCeMergeRows * kCeMergeLanes), 0, st, a.live, (const float*)g.part_m, (const float*)g.part_s, (const float*)g.part_z,
-                   (const float*)at_target, (long long)p.padded, g.slot, a.vocab, a.smoothing, row_loss, each);
-  if (e == cudaSuccess && a.reduce != CE_NONE) e = launch_pdl(ce_total_kernel, dim3(1), dim3(1024), 0, st, (const int*)a.live.count, (const float*)row_loss, a.reduce, a.loss);
+                   (const float*)at_target, (long long)p.padded, g.slot, a.vocab, a.smoothing, a.reduce, row_loss, a.loss);
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
 template <typename T>
-static int ce_backward(const CeArgs& a, cudaStream_t st) {
-  const CePlan p = ce_plan(a, true);
-  float *factor = (float*)(a.ws + p.rows), *scale = factor + p.padded;
-  if (a.dhidden != nullptr && cudaMemsetAsync(a.dhidden, 0, (size_t)a.rows * a.width * sizeof(T), st) != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
-  cudaError_t e = launch_pdl(ce_up_kernel, dim3(1), dim3(1024), 0, st, a.live, a.up, a.reduce, a.type == CE_F16 ? 32768.0f : 1.0f, factor, scale);
-  if (e == cudaSuccess)
-    e = ce_pack<T>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.ws + p.x, p.ldd, (long long)p.padded * p.ldd, st);
+static int ce_backward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
+  float* top = (float*)(a.ws + p.rows);
+  const CeUp up = {a.up, top, a.reduce, a.type == CE_F16 ? 32768.0f : 1.0f};
+  cudaError_t e = cudaSuccess;
+  if (a.reduce == CE_NONE) e = launch_pdl(ce_top_kernel, dim3(1), dim3(1024), 0, st, a.live, a.up, top);
   const long long x_plane = (long long)p.padded * p.ldd, z_plane = (long long)p.padded * p.piece;
   CeGemm g = {};
-  g.rows = a.live; g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded; g.factor = factor; g.scale = scale;
+  g.rows = a.live; g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded; g.up = up;
   g.a_rows = a.rows < 128 ? (int)ce_up_to(a.rows, 8) : 128;
   g.dz = (uint16_t*)(a.ws + p.dz); g.ldz = p.piece; g.plane = z_plane; g.piece_blocks = p.piece / kCeBlock; g.clusters = p.clusters;
   g.acc_rows = p.acc_rows; g.acc = (float*)(a.ws + p.acc);
@@ -1045,7 +1064,7 @@ static int ce_backward(const CeArgs& a, cudaStream_t st) {
     if (p.packed) e = ce_pack<T>(a.weight, a.ldw, c0, rows, nullptr, nullptr, a.width, a.ws + p.w, p.ldd, (long long)p.piece * p.ldd, st);
     if (e != cudaSuccess) break;
     g.c0 = c0;
-    if (!ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, x_plane, kCeBlock, g.a_rows) ||
+    if (!ce_tensor_map(&xm, a.x, a.type, a.width, p.padded, p.ldd, p.planes, x_plane, kCeBlock, g.a_rows) ||
         !ce_head_piece<T>(a, p, c0, rows, kCeBlock, p.tile_v / 2, &wm, &g.w_row))
       return BONSAI_CUDA_BAD_ARG;
     g.columns = rows; g.depth = a.width; g.tile_n = p.tile_v;
@@ -1061,33 +1080,35 @@ static int ce_backward(const CeArgs& a, cudaStream_t st) {
     }
     if (e == cudaSuccess && a.dweight != nullptr) {
       if (!ce_tensor_map(&zm, a.ws + p.dz, a.type, rows, p.padded, p.piece, p.planes, z_plane, 64, kCeBlock) ||
-          !ce_tensor_map(&xm, a.ws + p.x, a.type, a.width, p.padded, p.ldd, p.planes, x_plane, 64, kCeBlock))
+          !ce_tensor_map(&xm, a.x, a.type, a.width, p.padded, p.ldd, p.planes, x_plane, 64, kCeBlock))
         return BONSAI_CUDA_BAD_ARG;
       g.m = rows; g.out = a.dweight;
       e = ce_launch<T, CE_DW>(zm, xm, g, (rows + 255) / 256 * ct, p.clusters, st);
     }
   }
   if (e == cudaSuccess && a.dhidden != nullptr) {
-    const long long blocks = ((long long)a.rows * a.width + 255) / 256;
-    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st, a.live, (const float*)g.acc, g.piece_blocks,
-                   p.planes == 3 ? kCeTerms : 1, p.clusters, p.acc_rows, a.width, (const float*)scale, (T*)a.dhidden);
+    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(a.rows < 148 * 8 ? a.rows : 148 * 8)), dim3(256), 0, st, a.live, up, (const float*)g.acc, a.rows, g.piece_blocks,
+                   p.planes == 3 ? kCeTerms : 1, p.clusters, p.acc_rows, a.width, (T*)a.dhidden);
   }
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
 static bool ce_good(const CeArgs& a) {
-  return a.hidden != nullptr && a.weight != nullptr && a.rows >= 1 && a.vocab >= 1 && a.width >= 1 && a.ldh >= a.width && a.ldw >= a.width &&
-         a.rows < 0x7fffe000 && a.vocab < 0x7fffe000 && a.width < 0x7fffe000 && a.type >= CE_F32 && a.type <= CE_BF16 && a.reduce >= CE_MEAN &&
-         a.reduce <= CE_NONE;
+  return a.weight != nullptr && a.rows >= 1 && a.vocab >= 1 && a.width >= 1 && a.ldw >= a.width && a.rows < 0x7fffe000 && a.vocab < 0x7fffe000 &&
+         a.width < 0x7fffe000 && a.type >= CE_F32 && a.type <= CE_BF16 && a.reduce >= CE_MEAN && a.reduce <= CE_NONE;
 }
 
-static CeArgs ce_args(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce,
-                      float smoothing, int* live, void* ws, long long ws_bytes) {
+static CeArgs ce_args(const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce, float smoothing, void* kept, void* ws) {
   CeArgs a = {};
-  a.hidden = hidden; a.weight = weight; a.ldh = ldh; a.ldw = ldw;
+  a.weight = weight; a.ldw = ldw;
   a.rows = rows; a.vocab = vocab; a.width = width; a.type = type; a.reduce = reduce; a.smoothing = smoothing;
-  if (live != nullptr) a.live = CeRows{live, live + 4, live + 4 + rows, reinterpret_cast<float*>(live + 4 + 2ll * rows)};
-  a.ws = (uint8_t*)ws; a.ws_bytes = ws_bytes;
+  a.ws = (uint8_t*)ws;
+  if (kept != nullptr && rows > 0) {
+    uint8_t* at = (uint8_t*)kept + 256;
+    const long long lists = ce_up_to(4ll * rows, 256);
+    a.live = CeRows{(int*)kept, (int*)at, (int*)(at + lists), (int*)(at + 2 * lists), (float*)(at + 3 * lists)};
+    a.x = (uint16_t*)(at + 4 * lists);
+  }
   return a;
 }
 
@@ -1095,40 +1116,45 @@ static CeArgs ce_args(const void* hidden, long long ldh, const void* weight, lon
 
 extern "C" {
 
-// Bytes of workspace of the calls below, for these arguments (dhidden of the backward call: wanted or not); -1 for arguments that are refused.
-long long bonsai_ce_workspace(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type,
-                              float smoothing, int backward, int want_hidden) {
+// Bytes for the calls below with these arguments: of what the forward call keeps for the backward one (what 0), of the forward call's workspace (1),
+// of the backward call's without and with dhidden (2, 3); -1 for arguments that are refused.
+long long bonsai_ce_bytes(const void* weight, long long ldw, int rows, int vocab, int width, int type, float smoothing, int what) {
   using namespace bonsai;
-  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, CE_MEAN, smoothing, nullptr, nullptr, 0);
-  a.dhidden = want_hidden ? const_cast<void*>(hidden) : nullptr;
-  return ce_good(a) ? ce_plan(a, backward != 0).bytes : -1;
+  CeArgs a = ce_args(weight, ldw, rows, vocab, width, type, CE_MEAN, smoothing, nullptr, nullptr);
+  a.dhidden = what == 3 ? const_cast<void*>(weight) : nullptr;
+  if (!ce_good(a) || what < 0 || what > 3) return -1;
+  const CePlan p = ce_plan(a, what >= 2);
+  return what == 0 ? p.kept : p.bytes;
 }
 
-// hidden [rows][ldh], weight [vocab][ldw] of one type (0 f32, 1 f16, 2 bf16), targets [rows].  live: 4 + 3 rows words,
-// filled here and read by the backward call.  loss: one f32, or one for each row (reduce 2).  ws: 1024-byte aligned.
+// hidden [rows][ldh], weight [vocab][ldw] of one type (0 f32, 1 f16, 2 bf16), targets [rows].  loss: one f32, or one for each row (reduce 2).
+// kept, ws: 256-byte aligned.
 int bonsai_ce_forward(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* targets, int rows, int vocab, int width,
-                      int type, long long ignore, int reduce, float smoothing, int* live, float* loss, void* ws, long long ws_bytes,
+                      int type, long long ignore, int reduce, float smoothing, void* kept, long long kept_bytes, float* loss, void* ws, long long ws_bytes,
                       cudaStream_t st) {
   using namespace bonsai;
-  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, ws, ws_bytes);
-  a.targets = targets; a.ignore = ignore; a.loss = loss;
-  if (!ce_good(a) || targets == nullptr || live == nullptr || loss == nullptr || ws == nullptr ||
-      (reinterpret_cast<uintptr_t>(ws) & 15) != 0 || ws_bytes < ce_plan(a, false).bytes)
+  CeArgs a = ce_args(weight, ldw, rows, vocab, width, type, reduce, smoothing, kept, ws);
+  a.hidden = hidden; a.ldh = ldh; a.targets = targets; a.ignore = ignore; a.loss = loss;
+  if (!ce_good(a) || hidden == nullptr || ldh < width || targets == nullptr || loss == nullptr || kept == nullptr || ws == nullptr ||
+      ((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(kept)) & 255) != 0)
     return BONSAI_CUDA_BAD_ARG;
-  return type == CE_F32 ? ce_forward<float>(a, st) : type == CE_F16 ? ce_forward<__half>(a, st) : ce_forward<__nv_bfloat16>(a, st);
+  const CePlan p = ce_plan(a, false);
+  if (kept_bytes < p.kept || ws_bytes < p.bytes) return BONSAI_CUDA_BAD_ARG;
+  return type == CE_F32 ? ce_forward<float>(a, p, st) : type == CE_F16 ? ce_forward<__half>(a, p, st) : ce_forward<__nv_bfloat16>(a, p, st);
 }
 
-// up: d loss, one f32 or one for each row.  dhidden [rows][width], dweight [vocab][width] of the inputs' type; null: not wanted.
-int bonsai_ce_backward(const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce,
-                       float smoothing, int* live, const float* up, void* dhidden, void* dweight, void* ws, long long ws_bytes,
-                       cudaStream_t st) {
+// kept: from the forward call.  up: d loss, one f32 or one for each row.  dhidden [rows][width], dweight [vocab][width] of the inputs' type; null: not
+// wanted.
+int bonsai_ce_backward(const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce, float smoothing, void* kept,
+                       long long kept_bytes, const float* up, void* dhidden, void* dweight, void* ws, long long ws_bytes, cudaStream_t st) {
   using namespace bonsai;
-  CeArgs a = ce_args(hidden, ldh, weight, ldw, rows, vocab, width, type, reduce, smoothing, live, ws, ws_bytes);
+  CeArgs a = ce_args(weight, ldw, rows, vocab, width, type, reduce, smoothing, kept, ws);
   a.up = up; a.dhidden = dhidden; a.dweight = dweight;
-  if (!ce_good(a) || live == nullptr || up == nullptr || ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) != 0 ||
-      ws_bytes < ce_plan(a, true).bytes)
+  if (!ce_good(a) || kept == nullptr || up == nullptr || ws == nullptr || ((reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(kept)) & 255) != 0)
     return BONSAI_CUDA_BAD_ARG;
-  return type == CE_F32 ? ce_backward<float>(a, st) : type == CE_F16 ? ce_backward<__half>(a, st) : ce_backward<__nv_bfloat16>(a, st);
+  const CePlan p = ce_plan(a, true);
+  if (kept_bytes < p.kept || ws_bytes < p.bytes) return BONSAI_CUDA_BAD_ARG;
+  return type == CE_F32 ? ce_backward<float>(a, p, st) : type == CE_F16 ? ce_backward<__half>(a, p, st) : ce_backward<__nv_bfloat16>(a, p, st);
 }
 
 }  // extern "C"

@@ -18,9 +18,9 @@ _SIG = {
     "bonsai_mt_partials": [_i],
     "bonsai_mt_norm": [_i, _vp, _vp, _vp, _vp, _vp, _vp],
     "bonsai_mt_clip": [_i, _vp, _vp, _vp, _vp, _vp, _d, _vp, _vp, _vp],
-    "bonsai_ce_workspace": [_vp, _ll, _vp, _ll, _i, _i, _i, _i, C.c_float, _i, _i],
-    "bonsai_ce_forward": [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _ll, _i, C.c_float, _vp, _vp, _vp, _ll, _vp],
-    "bonsai_ce_backward": [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_ce_bytes": [_vp, _ll, _i, _i, _i, _i, C.c_float, _i],
+    "bonsai_ce_forward": [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _ll, _i, C.c_float, _vp, _ll, _vp, _vp, _ll, _vp],
+    "bonsai_ce_backward": [_vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp],
     "bonsai_mt_adam": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _d, _vp, _d, _d, _d, _d, _i, _vp, _d, _vp, _vp, _vp],
 }
 _declared = False
@@ -32,7 +32,7 @@ def _lib():
     global _declared
     l = K.lib()
     if not _declared:
-        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_workspace": _ll})
+        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_bytes": _ll})
         _declared = True
     return l
 
@@ -108,38 +108,36 @@ def mt_adam(params: TensorTable, grads: TensorTable, m: TensorTable, v: TensorTa
 REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
+def _ce_bytes(weight: torch.Tensor, n: int, label_smoothing: float, what: int) -> int:
+    size = int(_lib().bonsai_ce_bytes(weight.data_ptr(), weight.stride(0), n, *weight.shape, TYPE_CODES[weight.dtype], label_smoothing, what))
+    K.check(min(0, size), "linear_ce_bytes")
+    return size
+
+
 def linear_ce_forward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, reduction: str,
                       label_smoothing: float) -> tuple[torch.Tensor, torch.Tensor]:
     """hidden [n, d], weight [v, d] (one type, unit stride along d), targets int64 [n] -> the loss (f32, 0-dim or [n]) and what the
-    backward pass takes: the list of live rows and their log2 of the sum of exponentials."""
+    backward pass takes: the live rows side by side, their list and their log-sum-exp."""
     (n, d), v, device = hidden.shape, weight.shape[0], hidden.device
-    args = (hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0))
-    code = TYPE_CODES[hidden.dtype]
     with _on(device):
         loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=device)
-        live = torch.empty(4 + 3 * n, dtype=torch.int32, device=device)          # their number, rows, targets, and lse2 as f32
-        ws = _ce_workspace(args, n, v, d, code, label_smoothing, 0, 0, device)
-        K.check(_lib().bonsai_ce_forward(*args, targets.data_ptr(), n, v, d, code, ignore_index, REDUCTIONS[reduction], label_smoothing, live.data_ptr(),
+        kept = torch.empty(_ce_bytes(weight, n, label_smoothing, 0), dtype=torch.uint8, device=device)
+        ws = torch.empty(_ce_bytes(weight, n, label_smoothing, 1), dtype=torch.uint8, device=device)
+        K.check(_lib().bonsai_ce_forward(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), targets.data_ptr(), n, v, d,
+                                         TYPE_CODES[hidden.dtype], ignore_index, REDUCTIONS[reduction], label_smoothing, kept.data_ptr(), kept.numel(),
                                          loss.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device)), "linear_ce_forward")
-    return loss, live
+    return loss, kept
 
 
-def _ce_workspace(args, n: int, v: int, d: int, code: int, label_smoothing: float, backward: int, want_hidden: int, device) -> torch.Tensor:
-    size = int(_lib().bonsai_ce_workspace(*args, n, v, d, code, label_smoothing, backward, want_hidden))
-    K.check(min(0, size), "linear_ce_workspace")
-    return torch.empty(size, dtype=torch.uint8, device=device)
-
-
-def linear_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, live: torch.Tensor, up: torch.Tensor, reduction: str,
-                       label_smoothing: float, want_hidden: bool, want_weight: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """Gradients of :func:`linear_ce_forward`; ``up`` is the loss's gradient (f32, contiguous)."""
-    (n, d), v, device = hidden.shape, weight.shape[0], hidden.device
-    args = (hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0))
-    code = TYPE_CODES[hidden.dtype]
+def linear_ce_backward(weight: torch.Tensor, kept: torch.Tensor, n: int, up: torch.Tensor, reduction: str, label_smoothing: float, want_hidden: bool,
+                       want_weight: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of :func:`linear_ce_forward` over n rows; ``up`` is the loss's gradient (f32, contiguous)."""
+    (v, d), device = weight.shape, weight.device
     with _on(device):
-        dh = torch.empty((n, d), dtype=hidden.dtype, device=device) if want_hidden else None
+        dh = torch.empty((n, d), dtype=weight.dtype, device=device) if want_hidden else None
         dw = torch.empty((v, d), dtype=weight.dtype, device=device) if want_weight else None
-        ws = _ce_workspace(args, n, v, d, code, label_smoothing, 1, int(want_hidden), device)
-        K.check(_lib().bonsai_ce_backward(*args, n, v, d, code, REDUCTIONS[reduction], label_smoothing, live.data_ptr(), up.data_ptr(),
-                                          K.ptr(dh), K.ptr(dw), ws.data_ptr(), ws.numel(), _stream(device)), "linear_ce_backward")
+        ws = torch.empty(_ce_bytes(weight, n, label_smoothing, 3 if want_hidden else 2), dtype=torch.uint8, device=device)
+        K.check(_lib().bonsai_ce_backward(weight.data_ptr(), weight.stride(0), n, v, d, TYPE_CODES[weight.dtype], REDUCTIONS[reduction], label_smoothing,
+                                          kept.data_ptr(), kept.numel(), up.data_ptr(), K.ptr(dh), K.ptr(dw), ws.data_ptr(), ws.numel(),
+                                          _stream(device)), "linear_ce_backward")
     return dh, dw

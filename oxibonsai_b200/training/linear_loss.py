@@ -64,23 +64,24 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction, smoothing):
         if hidden.is_cuda:
-            loss, live = train_ops.linear_ce_forward(hidden, weight, targets, ignore_index, reduction, smoothing)
-            ctx.save_for_backward(hidden, weight, live)
+            loss, kept = train_ops.linear_ce_forward(hidden, weight, targets, ignore_index, reduction, smoothing)
+            ctx.save_for_backward(weight, kept)
         else:
             loss, live, lse = _cpu_forward(hidden, weight, targets, ignore_index, reduction, smoothing)
-            ctx.save_for_backward(hidden, weight, live, targets, lse)
+            ctx.save_for_backward(weight, hidden, live, targets, lse)
+        ctx.rows = len(hidden)
         ctx.reduction, ctx.smoothing = reduction, smoothing
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, up):
-        hidden, weight, live, *cpu = ctx.saved_tensors
+        weight, *rest = ctx.saved_tensors
         want = ctx.needs_input_grad[:2]
-        if hidden.is_cuda:
-            dh, dw = train_ops.linear_ce_backward(hidden, weight, live, up.contiguous(), ctx.reduction, ctx.smoothing, *want)
+        if weight.is_cuda:
+            dh, dw = train_ops.linear_ce_backward(weight, rest[0], ctx.rows, up.contiguous(), ctx.reduction, ctx.smoothing, *want)
         else:
-            targets, lse = cpu
+            hidden, live, targets, lse = rest
             dh, dw = _cpu_backward(hidden, weight, targets, live, lse, up, ctx.reduction, ctx.smoothing, *want)
         return dh, dw, None, None, None, None
 
@@ -114,7 +115,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise TypeError(f"linear_cross_entropy: hidden and weight of one type (float32, float16, bfloat16) are wanted, got {hidden.dtype} and {weight.dtype}")
     if min(weight.shape) < 1 or max(*weight.shape, targets.numel()) >= 2 ** 31 - 4096:
         raise ValueError(f"linear_cross_entropy: a vocabulary and a width of 1 to 2^31 are wanted, got {tuple(weight.shape)} and {targets.numel()} targets")
-    flat = hidden.reshape(-1, hidden.shape[-1])
+    flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     if targets.numel() == 0:
         loss = flat.float().sum() * 0.0 + weight[:0].float().sum() * 0.0       # zero gradients
         return loss * float("nan") if reduction == "mean" else loss if reduction == "sum" else flat.float().sum(-1).reshape(targets.shape)
@@ -122,7 +123,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         flat = flat if flat.stride(1) == 1 and flat.stride(0) >= flat.shape[1] else flat.contiguous()
         weight = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
     loss = _LinearCrossEntropy.apply(flat, weight, targets.reshape(-1).long(), ignore_index, reduction, float(label_smoothing))
-    return loss.reshape(targets.shape) if reduction == "none" else loss
+    return loss.reshape(targets.shape) if reduction == "none" and targets.dim() != 1 else loss
 
 
 def linear_ntp_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:

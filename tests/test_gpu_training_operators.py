@@ -173,6 +173,31 @@ def test_loss_on_another_stream_and_in_a_graph():
             assert torch.equal(loss, want[0]) and torch.equal(grads[0], want[1]) and torch.equal(grads[1], want[2])
 
 
+def test_loss_from_threads():
+    """Each pass as the first thing that a thread does on the GPU, and two threads at once."""
+    import threading
+
+    from oxibonsai_b200.ops import train_ops
+
+    h, w, t = loss_inputs(40, 500, 64, torch.bfloat16, DEV, seed=15)
+    want = run_loss(h, w, t)
+    got = {}
+
+    def go(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            loss, kept = train_ops.linear_ce_forward(h, w, t, -100, "mean", 0.0)
+            torch.cuda.current_stream().synchronize()
+            second = threading.Thread(target=lambda: got.__setitem__((i, "back"), train_ops.linear_ce_backward(w, kept, 40, torch.ones((), device=DEV), "mean", 0.0, True, True)))
+            second.start(), second.join()
+            got[i, "loss"] = loss
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(2)]
+    torch.cuda.synchronize()
+    [x.start() for x in threads], [x.join() for x in threads]
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i, "loss"], want[0]) and torch.equal(got[i, "back"][0], want[1]) and torch.equal(got[i, "back"][1], want[2])
+
+
 def test_loss_in_several_pieces():
     """Enough rows that the gradient of the logits goes through several pieces of the vocabulary."""
     h, w, t = loss_inputs(6000, 70000, 64, torch.bfloat16, DEV, seed=21, masked=0.1)
