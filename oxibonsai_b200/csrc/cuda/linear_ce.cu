@@ -29,16 +29,12 @@
 // (the loss of any type, all products of f32) a tile is therefore added to registers, with rounding, every few blocks of k.  Gradients in 16 bits
 // round a hundred times coarser and take the tensor cores' sum as it is.
 #include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "linear_ce.cuh"
 #include "tcgen05.cuh"
 
 namespace bonsai {
 
-enum CeType { CE_F32 = 0, CE_F16 = 1, CE_BF16 = 2 };
-enum CeReduce { CE_MEAN = 0, CE_SUM = 1, CE_NONE = 2 };
 enum CeMode { CE_LSE, CE_FEW, CE_DZ, CE_DH, CE_DW };
 
 constexpr int kCeStages = 6;
@@ -50,33 +46,9 @@ constexpr int kCeCols = 512;                            // TMEM columns, for two
 constexpr int kCeFew = 128;                             // tokens up to which the head's rows fill the tile
 constexpr int kCeGroup = 16;                            // row tiles that share the head's tiles while those are in L2
 constexpr int kCeStage = 32 * 128;                      // shared memory of an epilogue warp: 32 rows of 128 bytes on their way out
-constexpr int kCeSegment32 = 2, kCeSegment16 = 16, kCeSegmentFew = 4;          // blocks of k between two additions to registers
+constexpr int kCeSegment32 = 2, kCeSegment16 = 16, kCeSegmentFew = 8;          // blocks of k between two additions to registers
 constexpr int kCeTerms = 6;
-constexpr float kCeLog2e = 1.4426950408889634f;
 __device__ const unsigned char kCeTermA[kCeTerms] = {2, 0, 1, 1, 0, 0}, kCeTermB[kCeTerms] = {0, 2, 1, 0, 1, 0};      // the small ones first
-
-struct CeRows {         // the live rows, in order: filled by ce_rows_kernel
-  int* count;           // [2]: how many; blocks of ce_merge_kernel that are done
-  int* index;           // [N] row of the hidden states
-  int* target;          // [N] its target, -1 outside the vocabulary
-  int* place;           // [N] the other way: place of a row in this list, -1 for ignored ones
-  float* lse2;          // [N] log2 of the sum of exponentials
-};
-
-struct CeUp {           // the upstream gradient u: one value, or one for each row ("none")
-  const float* up;
-  const float* top;     // "none": max |u|
-  int reduce;
-  float dz_scale;       // what dz is stored with
-};
-__device__ __forceinline__ float ce_up_top(const CeUp& u) { return u.reduce == CE_NONE ? *u.top : fabsf(*u.up); }
-// u_i over the largest |u|; u is 0 or NaN where none is above 0
-__device__ __forceinline__ float ce_up_factor(const CeUp& u, const CeRows& r, int row) {
-  const float top = ce_up_top(u), x = u.up[u.reduce == CE_NONE ? r.index[row] : 0];
-  return r.target[row] < 0 ? NAN : top > 0.0f ? x / top : x;
-}
-// what the products' sums are multiplied by
-__device__ __forceinline__ float ce_up_scale(const CeUp& u, int n) { return n > 0 ? ce_up_top(u) / u.dz_scale / (u.reduce == CE_MEAN ? (float)n : 1.0f) : 0.0f; }
 
 struct CeGemm {
   CeRows rows;
@@ -158,8 +130,8 @@ __device__ __forceinline__ void ce_split(float x, uint16_t* p) {
 }
 
 // Rows of a matrix side by side with a row stride of whole 16-byte words: the live rows (count given; zeros up to the next 256) or all of
-// them, f32 as three planes.  A thread takes eight values.  Bound by memory.
-template <typename T>
+// them; f32 as three planes, or as it is for the few-rows kernels.  A thread takes eight values.  Bound by memory.
+template <typename T, bool kPlain = false>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const T* __restrict__ src, long long ld, long long row0, int rows, const int* count, const int* index,
                                                       int width, uint16_t* dst, int ldd, long long plane) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -178,7 +150,11 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T* __restrict__ src,
       for (int j = 0; j < 8; ++j) v[j] = r < n && k0 + j < width ? s[j] : T(0.0f);
     }
     uint16_t* o = dst + (long long)r * ldd + k0;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (kPlain) {
+      uint4* w = reinterpret_cast<uint4*>(reinterpret_cast<T*>(dst) + (long long)r * ldd + k0);
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) w[j] = reinterpret_cast<const uint4*>(v)[j];
+    } else if constexpr (sizeof(T) == 2) {
       *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
     } else {
       __align__(16) uint16_t p[3][8];
@@ -224,12 +200,6 @@ __device__ __forceinline__ void ce_arrive_at(uint32_t bar) {
 __device__ __forceinline__ void ce_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ce_exp2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // An operand across its rows (MN-major): a tile of 64 columns x 64 k is 64 rows of 128 bytes, swizzled like the K-major tiles; the next 64 columns
 // begin 8 KB further (leading offset), the next eight k 1 KB (stride), sixteen k 2 KB.
 __device__ __forceinline__ uint64_t ce_desc_mn(uint32_t smem_addr) {
@@ -884,6 +854,7 @@ struct CeArgs {
 struct CePlan {
   int planes, ldd, padded, tile_v, clusters;
   bool few;                    // the loss by CE_FEW
+  bool rows32;                 // f32 by the few-rows kernels
   bool packed;                 // the head is copied piece by piece: f32, or rows that TMA cannot take
   int piece, pieces, acc_rows;
   long long lists, kept;       // bytes of one of the live rows' lists, and of all that the forward call keeps for the backward one
@@ -923,7 +894,8 @@ static CePlan ce_plan(const CeArgs& a, bool backward) {
   p.ldd = (int)ce_up_to(a.width, 8);
   p.padded = (int)ce_up_to(a.rows, 256);
   p.clusters = ce_sms() / 2 < 1 ? 1 : ce_sms() / 2;
-  p.packed = p.planes == 3 || a.ldw % 8 != 0 || (reinterpret_cast<uintptr_t>(a.weight) & 15) != 0;
+  p.rows32 = a.type == CE_F32 && a.rows <= kCeFew32;
+  p.packed = (p.planes == 3 && !p.rows32) || a.ldw % 8 != 0 || (reinterpret_cast<uintptr_t>(a.weight) & 15) != 0;
   // pieces of the vocabulary: half a gigabyte of dz and of the copied head, at least 4096 rows
   long long most = ce_up_to(a.vocab, 256);
   const long long room = 1ll << 29;
@@ -935,6 +907,7 @@ static CePlan ce_plan(const CeArgs& a, bool backward) {
   p.pieces = (a.vocab + p.piece - 1) / p.piece;
   p.tile_v = ce_tile_columns(a.rows, p.piece < a.vocab ? p.piece : a.vocab, p.clusters);
   p.acc_rows = p.padded + 4096;
+  const long long planes = p.rows32 ? 2 : p.planes;      // 16-bit words of a kept value
   long long at = 0;
   auto take = [&](long long bytes) {
     const long long place = at;
@@ -942,7 +915,19 @@ static CePlan ce_plan(const CeArgs& a, bool backward) {
     return place;
   };
   p.lists = ce_up_to(4ll * a.rows, 256);
-  p.kept = 256 + 4 * p.lists + 2ll * p.planes * p.padded * p.ldd;
+  p.kept = 256 + 4 * p.lists + 2 * planes * p.padded * p.ldd;
+  if (p.rows32) {
+    p.rows = take(8ll * p.padded);
+    if (!backward) {
+      p.parts = ce_few_loss_slots();
+      p.part = take(12ll * p.parts * p.padded);
+    } else {
+      p.dz = take(4ll * a.rows * ce_up_to(a.vocab, 4));
+      if (a.dhidden != nullptr) p.acc = take(4ll * ce_few_slots(a.width) * a.rows * a.width);
+    }
+    p.bytes = at;
+    return p;
+  }
   p.w = p.packed ? take(2ll * p.planes * p.piece * p.ldd) : 0;
   p.rows = take(8ll * p.padded);                       // forward: z at the target, the rows' losses; backward: max |u|
   if (!backward) {
@@ -981,11 +966,11 @@ static cudaError_t ce_launch(const CUtensorMap& am, const CUtensorMap& bm, const
   return launch_pdl(ce_gemm_kernel<T, MODE>, dim3(2 * (unsigned)(tiles < clusters ? tiles : clusters)), dim3(kCeThreads), smem, st, am, bm, g);
 }
 
-template <typename T>
+template <typename T, bool kPlain = false>
 static cudaError_t ce_pack(const void* src, long long ld, long long row0, int rows, const int* count, const int* index, int width, void* dst, int ldd,
                            long long plane, cudaStream_t st) {
   const long long words = ce_up_to(rows, count != nullptr ? 256 : 1) * (ldd >> 3), blocks = (words + 255) / 256;
-  return launch_pdl(ce_pack_kernel<T>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const T*)src, ld, row0, rows, count, index,
+  return launch_pdl(ce_pack_kernel<T, kPlain>, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const T*)src, ld, row0, rows, count, index,
                     width, (uint16_t*)dst, ldd, plane);
 }
 
@@ -1005,12 +990,33 @@ static bool ce_head_piece(const CeArgs& a, const CePlan& p, int c0, int rows, in
   return ce_tensor_map(map, a.weight, a.type, a.width, c0 + rows, a.ldw, 1, 0, box_x, box_y);
 }
 
+static cudaError_t ce_merge(const CeArgs& a, const CePlan& p, const float* part_m, const float* part_s, const float* part_z, int slots, const float* at_target,
+                            float* row_loss, cudaStream_t st) {
+  return launch_pdl(ce_merge_kernel, dim3((a.rows + kCeMergeRows - 1) / kCeMergeRows), dim3(kCeMergeRows * kCeMergeLanes), 0, st, a.live, part_m, part_s, part_z,
+                    at_target, (long long)p.padded, slots, a.vocab, a.smoothing, a.reduce, row_loss, a.loss);
+}
+
+static CeFewArgs ce_few_args(const CeArgs& a, const CePlan& p) {
+  CeFewArgs f = {};
+  f.rows = a.live; f.weight = a.weight; f.x = a.x; f.ldw = a.ldw; f.ldx = p.ldd;
+  f.vocab = a.vocab; f.width = a.width; f.tokens = a.rows; f.smoothing = a.smoothing; f.row_count = a.rows;
+  return f;
+}
+
 template <typename T>
 static int ce_forward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
   float *at_target = (float*)(a.ws + p.rows), *row_loss = at_target + p.padded;
   float* part = (float*)(a.ws + p.part);
   float* each = a.reduce == CE_NONE ? a.loss : nullptr;
   cudaError_t e = launch_pdl(ce_rows_kernel, dim3(1), dim3(1024), 0, st, a.targets, a.rows, a.vocab, a.ignore, a.live, each);
+  if (p.rows32) {
+    if (e == cudaSuccess) e = ce_pack<T, true>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.x, p.ldd, 0, st);
+    CeFewArgs f = ce_few_args(a, p);
+    f.part_m = part; f.part_s = part + p.parts * p.padded; f.part_z = part + 2 * p.parts * p.padded; f.at_target = at_target; f.ldn = p.padded;
+    if (e == cudaSuccess) e = ce_few_loss(f, st);
+    if (e == cudaSuccess) e = ce_merge(a, p, f.part_m, f.part_s, f.part_z, (int)p.parts, at_target, row_loss, st);
+    return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
+  }
   if (e == cudaSuccess)
     e = ce_pack<T>(a.hidden, a.ldh, 0, a.rows, a.live.count, a.live.index, a.width, a.x, p.ldd, (long long)p.padded * p.ldd, st);
   CeGemm g = {};
@@ -1040,9 +1046,7 @@ static int ce_forward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
     e = ce_launch<T, CE_LSE>(xm, wm, g, (long long)(p.padded / 256) * ct, p.clusters, st);
     g.slot += 2 * ct;
   }
-  if (e == cudaSuccess)
-    e = launch_pdl(ce_merge_kernel, dim3((a.rows + kCeMergeRows - 1) / kCeMergeRows), dim3(kCeMergeRows * kCeMergeLanes), 0, st, a.live, (const float*)g.part_m, (const float*)g.part_s, (const float*)g.part_z,
-                   (const float*)at_target, (long long)p.padded, g.slot, a.vocab, a.smoothing, a.reduce, row_loss, a.loss);
+  if (e == cudaSuccess) e = ce_merge(a, p, g.part_m, g.part_s, g.part_z, g.slot, at_target, row_loss, st);
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
@@ -1052,6 +1056,13 @@ static int ce_backward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
   const CeUp up = {a.up, top, a.reduce, a.type == CE_F16 ? 32768.0f : 1.0f};
   cudaError_t e = cudaSuccess;
   if (a.reduce == CE_NONE) e = launch_pdl(ce_top_kernel, dim3(1), dim3(1024), 0, st, a.live, a.up, top);
+  if (p.rows32) {
+    CeFewArgs f = ce_few_args(a, p);
+    f.up = CeUp{a.up, top, a.reduce, 1.0f};
+    f.dz = (float*)(a.ws + p.dz); f.ldz = ce_up_to(a.vocab, 4); f.part = (float*)(a.ws + p.acc); f.dhidden = a.dhidden; f.dweight = a.dweight;
+    if (e == cudaSuccess) e = ce_few_gradients(f, st);
+    return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
+  }
   const long long x_plane = (long long)p.padded * p.ldd, z_plane = (long long)p.padded * p.piece;
   CeGemm g = {};
   g.rows = a.live; g.vocab = a.vocab; g.smoothing = a.smoothing; g.ldn = p.padded; g.up = up;

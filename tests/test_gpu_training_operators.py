@@ -29,7 +29,8 @@ def compare(h, w, t, up=None, reduction="mean", smoothing=0.0, ignore_index=-100
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n, v, d", [(1, 1, 1), (1, 2, 8), (3, 257, 63), (129, 1000, 64), (256, 256, 128), (257, 513, 200), (300, 5000, 1001), (64, 40000, 136),
-                                     (5, 151936, 64), (1000, 31, 72), (2, 300, 2056), (700, 3000, 520)])
+                                     (5, 151936, 64), (1000, 31, 72), (2, 300, 2056), (700, 3000, 520),
+                                     (8, 5001, 63), (9, 700, 264), (16, 3001, 520), (17, 90, 31), (32, 20000, 100), (33, 20000, 100), (8, 257, 4100), (128, 600, 72)])
 def test_loss_sizes(n, v, d, dtype):
     h, w, t = loss_inputs(n, v, d, dtype, DEV, seed=n + v + d, masked=0.0 if n < 4 else 0.2)
     compare(h, w, t, torch.tensor(UP.get(dtype, 1.0), device=DEV))
@@ -43,6 +44,26 @@ def test_loss_reductions(reduction, smoothing, dtype):
     if reduction == "none":
         up[7], up[11] = 0.0, -3.0
     compare(h, w, t, up * UP.get(dtype, 1.0), reduction, smoothing)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 8, 20])
+def test_loss_few_rows(n, dtype):
+    """The forms of a few rows: masks, each gradient alone, sums over rows, rows of the head with gaps between them."""
+    h, w, t = loss_inputs(n, 900, 136, dtype, DEV, seed=40 + n)
+    up = torch.rand(n, device=DEV) * UP.get(dtype, 1.0)
+    if n > 1:
+        t[1], t[n - 1] = -100, 899
+        h[1] = float("inf")
+    wide = torch.zeros(900, 144, dtype=dtype, device=DEV)
+    wide[:, 8:] = w
+    clean = torch.where((t == -100)[:, None], 0.0, h)
+    want, bound = loss_by_formula(clean, w, t, up, reduction="none", smoothing=0.2)
+    for head in (w, wide[:, 8:], wide[:, 8:].T.contiguous().T):
+        got = run_loss(h, head, t, up, "none", 0.2)
+        for g, x, b, what in zip(got, want, bound, ("loss", "dh", "dw")):
+            within(g, x, b, what)
+        assert torch.equal(run_loss(h, head, t, up, "none", 0.2, want="w")[1], got[2]) and torch.equal(run_loss(h, head, t, up, "none", 0.2, want="h")[1], got[1])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
