@@ -329,12 +329,13 @@ __device__ __forceinline__ void ce_flush(const uint8_t* stage, int lane, T* dst,
       }
     }
   } else {
+#pragma unroll 8
     for (int r = 0; r < 32; ++r) {
       T* o = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, mine, r));
-      if (((rows >> r) & 1) == 0) continue;
+      const int n = (rows >> r) & 1 ? valid : 0;
 #pragma unroll
       for (int j = lane; j < 128 / (int)sizeof(T); j += 32)
-        if (j < valid) {
+        if (j < n) {
           T x = *reinterpret_cast<const T*>(stage + r * 128 + (((j / kPer) ^ (r & 7)) << 4) + (j % kPer) * sizeof(T));
           if constexpr (sizeof(T) == 4) {
             if (add) x += o[j];
@@ -722,9 +723,9 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------------------------
-// Eight rows a block (a 32-byte sector of every slot's line), 64 threads for a row's slots; then the row's loss.  The last block to finish
+// Sixteen rows a block (64 bytes of every slot's line), 32 threads for a row's slots; then the row's loss.  The last block to finish
 // adds up the rows, in their order.
-constexpr int kCeMergeRows = 8, kCeMergeLanes = 64;
+constexpr int kCeMergeRows = 16, kCeMergeLanes = 32;
 __global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(CeRows r, const float* __restrict__ part_m, const float* __restrict__ part_s,
                                                                                const float* __restrict__ part_z, const float* at_target, long long ldn, int slots,
                                                                                int vocab, float smoothing, int reduce, float* row_loss, float* loss) {
@@ -827,10 +828,13 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, CeUp u, const fl
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const int at = r.place[row];
     if (at >= 0 && splits == 1) continue;
-    for (int d = threadIdx.x; d < width; d += 256) {
+    const int d = blockIdx.y * 256 + threadIdx.x;
+    if (d < width) {
       float v = 0.0f;
-      if (at >= 0)
+      if (at >= 0) {
+#pragma unroll 4
         for (int k = 0; k < splits; ++k) v += acc[(k * ldn + at) * width + d];
+      }
       out[(long long)row * width + d] = T(v * f);
     }
   }
@@ -1098,7 +1102,9 @@ static int ce_backward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
     }
   }
   if (e == cudaSuccess && a.dhidden != nullptr) {
-    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(a.rows < 148 * 8 ? a.rows : 148 * 8)), dim3(256), 0, st, a.live, up, (const float*)g.acc, a.rows, g.piece_blocks,
+    const int across = (a.width + 255) / 256, most = 148 * 16 / across > 0 ? 148 * 16 / across : 1;
+    if (across > 65535) return BONSAI_CUDA_BAD_ARG;
+    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most), (unsigned)across), dim3(256), 0, st, a.live, up, (const float*)g.acc, a.rows, g.piece_blocks,
                    p.planes == 3 ? kCeTerms : 1, p.clusters, p.acc_rows, a.width, (T*)a.dhidden);
   }
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;

@@ -108,8 +108,13 @@ def mt_adam(params: TensorTable, grads: TensorTable, m: TensorTable, v: TensorTa
 REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
+def _ld(t: torch.Tensor) -> int:
+    """Row stride; that of a single row may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
 def _ce_bytes(weight: torch.Tensor, n: int, label_smoothing: float, what: int) -> int:
-    size = int(_lib().bonsai_ce_bytes(weight.data_ptr(), weight.stride(0), n, *weight.shape, TYPE_CODES[weight.dtype], label_smoothing, what))
+    size = int(_lib().bonsai_ce_bytes(weight.data_ptr(), _ld(weight), n, *weight.shape, TYPE_CODES[weight.dtype], label_smoothing, what))
     K.check(min(0, size), "linear_ce_bytes")
     return size
 
@@ -123,7 +128,7 @@ def linear_ce_forward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch
         loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=device)
         kept = torch.empty(_ce_bytes(weight, n, label_smoothing, 0), dtype=torch.uint8, device=device)
         ws = torch.empty(_ce_bytes(weight, n, label_smoothing, 1), dtype=torch.uint8, device=device)
-        K.check(_lib().bonsai_ce_forward(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), targets.data_ptr(), n, v, d,
+        K.check(_lib().bonsai_ce_forward(hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight), targets.data_ptr(), n, v, d,
                                          TYPE_CODES[hidden.dtype], ignore_index, REDUCTIONS[reduction], label_smoothing, kept.data_ptr(), kept.numel(),
                                          loss.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device)), "linear_ce_forward")
     return loss, kept
@@ -137,7 +142,7 @@ def linear_ce_backward(weight: torch.Tensor, kept: torch.Tensor, n: int, up: tor
         dh = torch.empty((n, d), dtype=weight.dtype, device=device) if want_hidden else None
         dw = torch.empty((v, d), dtype=weight.dtype, device=device) if want_weight else None
         ws = torch.empty(_ce_bytes(weight, n, label_smoothing, 3 if want_hidden else 2), dtype=torch.uint8, device=device)
-        K.check(_lib().bonsai_ce_backward(weight.data_ptr(), weight.stride(0), n, v, d, TYPE_CODES[weight.dtype], REDUCTIONS[reduction], label_smoothing,
+        K.check(_lib().bonsai_ce_backward(weight.data_ptr(), _ld(weight), n, v, d, TYPE_CODES[weight.dtype], REDUCTIONS[reduction], label_smoothing,
                                           kept.data_ptr(), kept.numel(), up.data_ptr(), K.ptr(dh), K.ptr(dw), ws.data_ptr(), ws.numel(),
                                           _stream(device)), "linear_ce_backward")
     return dh, dw

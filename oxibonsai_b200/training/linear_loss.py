@@ -97,7 +97,12 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     type; logits, sums and products are float32 whatever the inputs, and on the GPU the gradient of the logits is rounded to the
     inputs' type before it is multiplied, as a product of that type does.  A target outside the vocabulary raises on the CPU; on the GPU,
     where nothing waits for the result, its loss and the gradients that it enters are NaN.  float16 gradients underflow as everywhere:
-    scale the loss."""
+    scale the loss.
+
+    On the GPU nothing is read back and all memory comes from torch's allocator, so that a pass and its gradients can be captured into a
+    CUDA graph; as with every operator of torch, capture them through ``torch.autograd.grad``, or while no eager graph of the same leaves
+    is alive.  Between the passes the live rows of ``hidden`` are kept (a copy) with 16 bytes per token; changing ``weight`` in between is an
+    error that autograd reports."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_cross_entropy: hidden [..., d] and weight [vocab, d] are wanted, got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if targets.shape != hidden.shape[:-1]:
@@ -110,18 +115,23 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"linear_cross_entropy: label_smoothing is between 0 and 1, got {label_smoothing}")
     if not hidden.device == weight.device == targets.device:
         raise ValueError(f"linear_cross_entropy: tensors of one device are wanted, got {hidden.device}, {weight.device} and {targets.device}")
+    if hidden.device.type not in ("cuda", "cpu"):
+        raise ValueError(f"linear_cross_entropy: CUDA or CPU tensors are wanted, got {hidden.device}")
     types = (torch.float32, torch.float16, torch.bfloat16) + (() if hidden.is_cuda else (torch.float64,))
     if hidden.dtype != weight.dtype or hidden.dtype not in types:
         raise TypeError(f"linear_cross_entropy: hidden and weight of one type (float32, float16, bfloat16) are wanted, got {hidden.dtype} and {weight.dtype}")
     if min(weight.shape) < 1 or max(*weight.shape, targets.numel()) >= 2 ** 31 - 4096:
-        raise ValueError(f"linear_cross_entropy: a vocabulary and a width of 1 to 2^31 are wanted, got {tuple(weight.shape)} and {targets.numel()} targets")
+        raise ValueError(f"linear_cross_entropy: a vocabulary and a width of at least 1 and less than 2^31 are wanted, got {tuple(weight.shape)} and "
+                         f"{targets.numel()} targets")
+    if weight.shape[1] > 2 ** 24:
+        raise ValueError(f"linear_cross_entropy: rows of at most 2^24 values are wanted, got {weight.shape[1]}")
     flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     if targets.numel() == 0:
         loss = flat.float().sum() * 0.0 + weight[:0].float().sum() * 0.0       # zero gradients
         return loss * float("nan") if reduction == "mean" else loss if reduction == "sum" else flat.float().sum(-1).reshape(targets.shape)
     if flat.is_cuda:
-        flat = flat if flat.stride(1) == 1 and flat.stride(0) >= flat.shape[1] else flat.contiguous()
-        weight = weight if weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
+        flat = flat if flat.is_contiguous() or (flat.stride(1) == 1 and flat.stride(0) >= flat.shape[1]) else flat.contiguous()
+        weight = weight if weight.is_contiguous() or (weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1]) else weight.contiguous()
     loss = _LinearCrossEntropy.apply(flat, weight, targets.reshape(-1).long(), ignore_index, reduction, float(label_smoothing))
     return loss.reshape(targets.shape) if reduction == "none" and targets.dim() != 1 else loss
 

@@ -187,8 +187,8 @@ class FusedAdam:
     def _check_grads(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor]) -> None:
         name = type(self).__name__
         for p, g in zip(params, grads):
-            if g.dtype not in _TYPES or g.layout != torch.strided:
-                raise TypeError(f"{name}: dense float32, float16 or bfloat16 gradients are wanted, got {g.dtype} ({g.layout})")
+            if not isinstance(g, torch.Tensor) or g.dtype not in _TYPES or g.layout != torch.strided:
+                raise TypeError(f"{name}: dense float32, float16 or bfloat16 gradients are wanted, got {getattr(g, 'dtype', type(g).__name__)}")
             if g.shape != p.shape or g.device != self.device:
                 raise ValueError(f"{name}: a gradient of shape {tuple(g.shape)} on {g.device} for a parameter of shape {tuple(p.shape)} on {p.device}")
 

@@ -97,6 +97,9 @@ def test_loss_strides_and_orders(dtype):
     a = run_loss(h.view(7, 10, 48), w, t.view(7, 10), reduction="none")
     b = run_loss(h, w, t, reduction="none")
     assert a[0].shape == (7, 10) and torch.equal(a[0].flatten(), b[0]) and torch.equal(a[1].flatten(0, 1), b[1]) and torch.equal(a[2], b[2])
+    compare(h[:1].T.contiguous().T, w, t[:1])                     # a single row may have any stride
+    compare(h[:, :1], w[:1, :1], torch.zeros_like(t))
+    compare(h[:, 5:6], w[:, 7:8], t)
     one = run_loss(h[0], w, t[0])
     assert one[0].shape == () and one[1].shape == (48,)
 

@@ -61,7 +61,8 @@ def test_linear_cross_entropy_refusals():
                        (lambda: TR.linear_cross_entropy(h, w, t[:3]), ValueError), (lambda: TR.linear_cross_entropy(h, w, t.float()), TypeError),
                        (lambda: TR.linear_cross_entropy(h, w, t, reduction="batch"), ValueError), (lambda: TR.linear_cross_entropy(h.half(), w, t), TypeError),
                        (lambda: TR.linear_cross_entropy(h, w, t, label_smoothing=1.5), ValueError), (lambda: TR.linear_cross_entropy(h.int(), w.int(), t), TypeError),
-                       (lambda: TR.linear_cross_entropy(h, w[:0], t), ValueError), (lambda: TR.linear_cross_entropy(h, w, t + 10), IndexError),
+                       (lambda: TR.linear_cross_entropy(h, w[:0], t), ValueError),
+                       (lambda: TR.linear_cross_entropy(h.to("meta"), w.to("meta"), t.to("meta")), ValueError), (lambda: TR.linear_cross_entropy(h, w, t + 10), IndexError),
                        (lambda: TR.linear_cross_entropy(h, w, t - 20), IndexError)):
         with pytest.raises(error):
             bad()
@@ -140,7 +141,7 @@ def test_fused_adam_state_and_refusals():
                        (lambda: TR.FusedAdam([x], grads=[torch.zeros(3)]), ValueError), (lambda: TR.FusedAdam([x], grads=[torch.zeros(4).double()]), TypeError),
                        (lambda: TR.FusedAdam([x], state=([torch.zeros(4)], [torch.zeros(3)])), ValueError), (lambda: TR.FusedAdam([x], state=([x], [x])), ValueError),
                        (lambda: TR.FusedAdam([torch.zeros(2, 3)], grads=[torch.zeros(3, 2).T]), ValueError),
-                       (lambda: TR.FusedAdam([x]).step(lr=torch.zeros(2)), ValueError)):
+                       (lambda: TR.FusedAdam([x]).step(lr=torch.zeros(2)), ValueError), (lambda: TR.FusedAdam([x], grads=[None]), TypeError)):
         with pytest.raises(error):
             bad()
 
