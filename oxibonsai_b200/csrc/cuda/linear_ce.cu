@@ -46,7 +46,7 @@ constexpr int kCeCols = 512;                            // TMEM columns, for two
 constexpr int kCeFew = 128;                             // tokens up to which the head's rows fill the tile
 constexpr int kCeGroup = 16;                            // row tiles that share the head's tiles while those are in L2
 constexpr int kCeStage = 32 * 128;                      // shared memory of an epilogue warp: 32 rows of 128 bytes on their way out
-constexpr int kCeSegment32 = 2, kCeSegment16 = 16, kCeSegmentFew = 8;          // blocks of k between two additions to registers
+constexpr int kCeSegment32 = 2, kCeSegment16 = 16, kCeSegmentFew = 4;          // blocks of k between two additions to registers: f32; the loss; of few tokens
 constexpr int kCeTerms = 6;
 __device__ const unsigned char kCeTermA[kCeTerms] = {2, 0, 1, 1, 0, 0}, kCeTermB[kCeTerms] = {0, 2, 1, 0, 1, 0};      // the small ones first
 
@@ -77,7 +77,7 @@ struct CeGemm {
 
 // ---- rows ---------------------------------------------------------------------------------------------------------------------------
 // One block walks the targets and lists the live rows in order.  `each`: the loss of ignored rows (reduction "none").
-__global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* __restrict__ targets, int n, int vocab, long long ignore, CeRows r, float* each) {
+__global__ void __launch_bounds__(1024) ce_rows_kernel(const long long* targets, int n, int vocab, long long ignore, CeRows r, float* each) {
   __shared__ int warps[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -132,7 +132,7 @@ __device__ __forceinline__ void ce_split(float x, uint16_t* p) {
 // Rows of a matrix side by side with a row stride of whole 16-byte words: the live rows (count given; zeros up to the next 256) or all of
 // them; f32 as three planes, or as it is for the few-rows kernels.  A thread takes eight values.  Bound by memory.
 template <typename T, bool kPlain = false>
-__global__ void __launch_bounds__(256) ce_pack_kernel(const T* __restrict__ src, long long ld, long long row0, int rows, const int* count, const int* index,
+__global__ void __launch_bounds__(256) ce_pack_kernel(const T* src, long long ld, long long row0, int rows, const int* count, const int* index,
                                                       int width, uint16_t* dst, int ldd, long long plane) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -194,8 +194,11 @@ __device__ __forceinline__ void ce_commit(uint64_t* bar) {
                "h"((uint16_t)3)
                : "memory");
 }
+// Says that this warp has read an accumulator (its tcgen05.ld have come back, and the tensor-memory fence is behind them).  Nothing in memory is handed over,
+// so the arrive releases nothing at cluster scope: that cost some 1.4 us each time, the stores before it included, and one token of the 8B head
+// took 250 us with sums in registers every 4 blocks instead of 217.
 __device__ __forceinline__ void ce_arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void ce_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -386,20 +389,22 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
   constexpr bool kF32 = sizeof(T) == 4, kAcross = MODE == CE_DH || MODE == CE_DW;      // B is MN-major
   constexpr int kTerms = kF32 ? kCeTerms : 1, kSegment = kF32 ? kCeSegment32 : MODE == CE_FEW ? kCeSegmentFew : kCeSegment16;
   constexpr bool kSums = kF32 || MODE == CE_LSE || MODE == CE_FEW;           // sums in registers
+  // few tokens: the second operand is half as long, which makes room for eight stages of the head's bytes
+  constexpr int kStages = MODE == CE_FEW ? 8 : kCeStages, kOperandB = MODE == CE_FEW ? kCeOperand / 2 : kCeOperand;
   constexpr int kBufs = MODE == CE_FEW ? 4 : 2, kCols = kCeCols / kBufs;
   constexpr int kChunks = MODE == CE_FEW ? 2 : 4;          // of 32 columns, in a half of a tile
   extern __shared__ uint8_t ce_smem[];
   uint8_t* base = (uint8_t*)(((uintptr_t)ce_smem + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = base;
-  uint8_t* sB = base + kCeStages * kCeOperand;
-  __shared__ uint64_t full[kCeStages], empty[kCeStages], accf[kBufs], acce[kBufs];
+  uint8_t* sB = base + kStages * kCeOperand;
+  __shared__ uint64_t full[kStages], empty[kStages], accf[kBufs], acce[kBufs];
   __shared__ uint32_t tmem_slot;
   const int t = threadIdx.x, warp = __shfl_sync(0xffffffffu, t >> 5, 0), lane = t & 31;
   const uint32_t rank = blockIdx.x & 1;
   const int cid = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (MODE != CE_DW && p.a_rows < 128) {          // rows that no copy fills: zeros draw less power than what an earlier kernel has left there
-    for (int i = t; i < kCeStages * kCeOperand / 16; i += kCeThreads) reinterpret_cast<uint4*>(sA)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = t; i < kStages * kCeOperand / 16; i += kCeThreads) reinterpret_cast<uint4*>(sA)[i] = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
   }
   if (warp == kCeEpiWarps + 1) {
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (t == 0) {
-    for (int i = 0; i < kCeStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
           for (int term = 0; term < kTerms; ++term, ++issued) {
             const int pa = kF32 ? kCeTermA[term] : 0, pb = kF32 ? kCeTermB[term] : 0;
             if (!tc::mbar_wait(&empty[s], phase)) { failed = true; break; }
-            const uint32_t bar = ce_map(tc::smem_u32(&full[s]), 0), a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kCeOperand);
+            const uint32_t bar = ce_map(tc::smem_u32(&full[s]), 0), a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kOperandB);
             if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], bytes);
             if (MODE == CE_DW) {
               ce_load(a, &amap, row0, k, pa, bar);
@@ -472,11 +477,11 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
             } else {
               ce_load(b, &bmap, k, MODE == CE_FEW ? col0 : p.w_row + col0, pb, bar);
             }
-            if (++s == kCeStages) { s = 0; phase ^= 1; }
+            if (++s == kStages) { s = 0; phase ^= 1; }
           }
         }
       }
-      if (rank == 0) tc::mbar_drain(full, issued, kCeStages);      // both CTAs' copies; the other one waits at the barrier below
+      if (rank == 0) tc::mbar_drain(full, issued, kStages);      // both CTAs' copies; the other one waits at the barrier below
     }
   } else if (warp == kCeEpiWarps + 1) {
     if (rank == 0 && tc::elect_one()) {
@@ -496,13 +501,13 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
           for (int i = 0; i < (k1 - k0) * kTerms; ++i) {
             if (!tc::mbar_wait(&full[s], phase)) { failed = true; break; }
             tc::tc_fence_after();
-            const uint32_t a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kCeOperand);
+            const uint32_t a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kOperandB);
             const uint64_t da = MODE == CE_DW ? ce_desc_mn(a) : tc::smem_desc_sw128(a), db = kAcross ? ce_desc_mn(b) : tc::smem_desc_sw128(b);
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k)
               ce_mma(taddr + ab * kCols, da + (MODE == CE_DW ? 128 : 2) * k, db + (kAcross ? 128 : 2) * k, idesc, i > 0 || k > 0);
             ce_commit(&empty[s]);
-            if (++s == kCeStages) { s = 0; phase ^= 1; }
+            if (++s == kStages) { s = 0; phase ^= 1; }
           }
           ce_commit(&accf[ab]);
           k0 = k1;
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
     __syncwarp();
   } else {
     const int quarter = warp & 3, half = warp >> 2, middle = ((p.tile_n >> 1) + 31) & ~31;      // a half's columns: 0 .. middle, middle .. tile_n
-    uint8_t* stage = base + kCeStages * 2 * kCeOperand + warp * kCeStage;
+    uint8_t* stage = base + kStages * (kCeOperand + kOperandB) + warp * kCeStage;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t drained = ce_map(tc::smem_u32(&acce[0]), 0);
     bool failed = false;
@@ -726,8 +731,8 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
 // Sixteen rows a block (64 bytes of every slot's line), 32 threads for a row's slots; then the row's loss.  The last block to finish
 // adds up the rows, in their order.
 constexpr int kCeMergeRows = 16, kCeMergeLanes = 32;
-__global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(CeRows r, const float* __restrict__ part_m, const float* __restrict__ part_s,
-                                                                               const float* __restrict__ part_z, const float* at_target, long long ldn, int slots,
+__global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(CeRows r, const float* part_m, const float* part_s,
+                                                                               const float* part_z, const float* at_target, long long ldn, int slots,
                                                                                int vocab, float smoothing, int reduce, float* row_loss, float* loss) {
   __shared__ float sm[kCeMergeLanes][kCeMergeRows];
   __shared__ double ss[kCeMergeLanes][kCeMergeRows], sz[kCeMergeLanes][kCeMergeRows];
@@ -801,7 +806,7 @@ __global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(
 }
 
 // max |u| over the live rows
-__global__ void __launch_bounds__(1024) ce_top_kernel(CeRows r, const float* __restrict__ up, float* out) {
+__global__ void __launch_bounds__(1024) ce_top_kernel(CeRows r, const float* up, float* out) {
   __shared__ float s[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -817,7 +822,7 @@ __global__ void __launch_bounds__(1024) ce_top_kernel(CeRows r, const float* __r
 
 // dh: zeros for ignored rows, and the parts' sums where there are several
 template <typename T>
-__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, CeUp u, const float* __restrict__ acc, int rows, int piece_blocks, int terms, int clusters, int acc_rows,
+__global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, CeUp u, const float* acc, int rows, int piece_blocks, int terms, int clusters, int acc_rows,
                                                       int width, T* out) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -835,7 +840,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, CeUp u, const fl
 #pragma unroll 4
         for (int k = 0; k < splits; ++k) v += acc[(k * ldn + at) * width + d];
       }
-      out[(long long)row * width + d] = T(v * f);
+      out[(long long)row * width + d] = T(at >= 0 ? v * f : 0.0f);
     }
   }
 }

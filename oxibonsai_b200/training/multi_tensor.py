@@ -243,6 +243,11 @@ class FusedAdam:
             p.copy_(x - (lr / (1 - b1 ** t)) * mi / (vi.sqrt() / (1 - b2 ** t) ** 0.5 + self.eps))
         return norm
 
+    @torch.no_grad()
+    def reset(self) -> None:
+        for part in (*self.m, *self.v, self.steps):
+            part.zero_()
+
     def zero_grad(self) -> None:
         """Drops ``p.grad``; with fixed gradients fills those with zeros."""
         if self.grads is not None:

@@ -149,6 +149,24 @@ def test_loss_wrong_targets(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [9, 300])
+def test_loss_upstream_gradients(n, dtype):
+    """Ignored rows have no gradient whatever comes from above; rows with an upstream gradient of 0 have none; sizes far apart keep their rows exact."""
+    h, w, t = loss_inputs(n, 400, 72, dtype, DEV, seed=50)
+    t[2] = -100
+    for bad in (float("inf"), float("nan")):
+        _, dh, dw = run_loss(h, w, t, torch.tensor(bad, device=DEV))
+        assert not dh[2].any() and dh[0].isnan().all() and dw.isnan().all()
+    up = torch.ones(n, device=DEV)
+    up[0], up[1] = 0.0, float("nan")
+    _, dh, _ = run_loss(h, w, t, up, "none")
+    assert not dh[0].any() and not dh[2].any() and dh[1].isnan().all() and dh[3:].isfinite().all()
+    up = torch.logspace(0, -4, n, device=DEV)
+    compare(h, w, t, up * UP.get(dtype, 1.0), "none")
+    assert not run_loss(h, w, t, torch.zeros((), device=DEV))[1].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_loss_far_logits(dtype):
     """Logits of hundreds: the largest carries the softmax, the others vanish; equal logits share it."""
     v, d = 600, 64

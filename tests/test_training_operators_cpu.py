@@ -135,6 +135,8 @@ def test_fused_adam_state_and_refusals():
     assert p[0][0] == want[0][0][0].to(torch.bfloat16) and torch.allclose(m[0].double(), want[1][0]) and torch.allclose(v[0].double(), want[2][0])
     opt.zero_grad()
     assert not g[0].any()
+    opt.reset()
+    assert opt.t == 0 and not m[0].any() and not v[0].any()
     x = torch.zeros(4)
     for bad, error in ((lambda: TR.FusedAdam([]), ValueError), (lambda: TR.FusedAdam([x, x]), ValueError), (lambda: TR.FusedAdam([x.long()]), TypeError),
                        (lambda: TR.FusedAdam([x], betas=(1.0, 0.9)), ValueError), (lambda: TR.FusedAdam([x], grads=[]), ValueError),
