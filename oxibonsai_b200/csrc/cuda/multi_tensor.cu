@@ -20,7 +20,10 @@
 namespace bonsai {
 
 constexpr int kMtTensors = 512;        // tensors of one launch; larger sets take several
-constexpr int kMtBlocksMax = 148 * 4;
+// Blocks of a launch: sets that take some tens of microseconds go in one wave (three blocks an SM, two of the Adam step), larger ones in pieces that
+// even the SMs out (13 M f32, clipped: 29.7 us in one wave, 31.2 in 888 pieces; 705 M bf16 into f32: 948 and 932).
+constexpr int kMtBlocksMax = 148 * 6, kMtWave = 148 * 3, kMtWaveAdam = 148 * 2;
+constexpr long long kMtSmall = 1ll << 24;
 constexpr int kMtThreads = 512;
 enum MtType : unsigned char { MT_F32 = 0, MT_F16 = 1, MT_BF16 = 2 };
 
@@ -158,7 +161,7 @@ __device__ __forceinline__ double mt_squares(const void* g, long long lo, long l
 }
 
 // `step`, where given, counts this optimizer step before the kernel that reads it.
-__global__ void __launch_bounds__(kMtThreads) mt_norm_kernel(const __grid_constant__ MtTable<1> tb, double* partial, long long* step) {
+__global__ void __launch_bounds__(kMtThreads, 3) mt_norm_kernel(const __grid_constant__ MtTable<1> tb, double* partial, long long* step) {
   __shared__ double s[kMtThreads / 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -235,7 +238,7 @@ __device__ __forceinline__ void mt_scale_to(int type, const void* g, void* out, 
   }
 }
 
-__global__ void __launch_bounds__(kMtThreads) mt_scale_kernel(const __grid_constant__ MtTable<2> tb, MtClip c) {
+__global__ void __launch_bounds__(kMtThreads, 3) mt_scale_kernel(const __grid_constant__ MtTable<2> tb, MtClip c) {
   __shared__ double s[kMtThreads / 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -307,7 +310,7 @@ __device__ __forceinline__ void mt_adam_by(int type, const MtAdamNow& a, void* p
   }
 }
 
-__global__ void __launch_bounds__(kMtThreads) mt_adam_kernel(const __grid_constant__ MtTable<4> tb, MtClip c, MtAdam h) {
+__global__ void __launch_bounds__(kMtThreads, 2) mt_adam_kernel(const __grid_constant__ MtTable<4> tb, MtClip c, MtAdam h) {
   __shared__ double s[kMtThreads / 32];
   __shared__ MtAdamNow now;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(kMtThreads) mt_adam_kernel(const __grid_consta
 
 // Tensors [at, at + n) of the set as one launch's table; returns its blocks.
 template <int NP>
-static int mt_table(MtTable<NP>* tb, void* const* const* ptrs, const long long* numel, const unsigned char* const* types, int at, int n) {
+static int mt_table(MtTable<NP>* tb, int wave, void* const* const* ptrs, const long long* numel, const unsigned char* const* types, int at, int n) {
   tb->tensors = n;
   tb->start[0] = 0;
   for (int i = 0; i < n; ++i) {
@@ -351,7 +354,8 @@ static int mt_table(MtTable<NP>* tb, void* const* const* ptrs, const long long* 
     tb->start[i + 1] = tb->start[i] + numel[at + i];
   }
   const long long total = tb->start[n], least = 8 * kMtThreads;      // eight values for every thread
-  long long per = (total + kMtBlocksMax - 1) / kMtBlocksMax;
+  const int most = total < kMtSmall ? wave : kMtBlocksMax;
+  long long per = (total + most - 1) / most;
   per = (per + 1023) / 1024 * 1024;
   tb->per_block = per < least ? least : per;
   const int blocks = (int)((total + tb->per_block - 1) / tb->per_block);
@@ -375,7 +379,7 @@ static cudaError_t mt_norm(int n, void* const* g, const long long* numel, const 
   cudaError_t e = cudaSuccess;
   *partials = 0;
   for (int at = 0; at < n && e == cudaSuccess; at += kMtTensors) {
-    const int blocks = mt_table<1>(&tb, &g, numel, &type, at, n - at < kMtTensors ? n - at : kMtTensors);
+    const int blocks = mt_table<1>(&tb, kMtWave, &g, numel, &type, at, n - at < kMtTensors ? n - at : kMtTensors);
     e = launch_pdl(mt_norm_kernel, dim3(blocks), dim3(kMtThreads), 0, st, tb, partial + *partials, at == 0 ? step : (long long*)nullptr);
     *partials += blocks;
   }
@@ -411,7 +415,7 @@ int bonsai_mt_clip(int n, void* const* g, void* const* out, const long long* num
   void* const* ptrs[2] = {g, out};
   const unsigned char* types[2] = {type, otype};
   for (int at = 0; at < n && e == cudaSuccess; at += kMtTensors) {
-    const int blocks = mt_table<2>(&tb, ptrs, numel, types, at, n - at < kMtTensors ? n - at : kMtTensors);
+    const int blocks = mt_table<2>(&tb, kMtWave, ptrs, numel, types, at, n - at < kMtTensors ? n - at : kMtTensors);
     e = launch_pdl(mt_scale_kernel, dim3(blocks), dim3(kMtThreads), 0, st, tb, MtClip{partial, partials, norm, max_norm});
   }
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
@@ -434,7 +438,7 @@ int bonsai_mt_adam(int n, void* const* p, void* const* g, void* const* m, void* 
   const unsigned char* types[2] = {ptype, gtype};
   const MtAdam h = {lr_dev, step, lr, beta1, beta2, eps, decay, decoupled};
   for (int at = 0; at < n && e == cudaSuccess; at += kMtTensors) {
-    const int blocks = mt_table<4>(&tb, ptrs, numel, types, at, n - at < kMtTensors ? n - at : kMtTensors);
+    const int blocks = mt_table<4>(&tb, kMtWaveAdam, ptrs, numel, types, at, n - at < kMtTensors ? n - at : kMtTensors);
     e = launch_pdl(mt_adam_kernel, dim3(blocks), dim3(kMtThreads), 0, st, tb, MtClip{partial, partials, norm, max_norm}, h);
   }
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
