@@ -432,3 +432,51 @@ def test_a_training_step_together():
     while not tr.is_complete():
         s = tr.step(lambda: TR.linear_cross_entropy(reg.apply_adapter("lin", h, h), head, t))
         assert s.grad_norm > 0 and s.loss > 0
+
+
+# ---- places past 32 bits ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n, v, d", [(530_000, 300, 4096), (24, 530_000, 4096), (600_000, 8192, 64)])
+def test_loss_far_places(n, v, d):
+    """Hidden states, a head and a piece of the logits' gradient of more than 2^31 values: rows at both ends against the formula."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    h = torch.empty(n, d, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    w = torch.empty(v, d, dtype=torch.bfloat16, device=DEV).normal_(0, 1.28 / d ** 0.5, generator=g)
+    t = torch.randint(0, v, (n,), generator=g, device=DEV)
+    t[n // 2] = -100
+    up = torch.rand(n, generator=g, device=DEV)
+    loss, dh, dw = run_loss(h, w, t, up, "none")
+    ends = torch.tensor(sorted({0, 1, n // 2, n - 2, n - 1}), device=DEV)
+    want, bound = loss_by_formula(h[ends], w, t[ends], up[ends], reduction="none")
+    within(loss[ends], want[0], bound[0], "loss")
+    within(dh[ends], want[1], bound[1], "dh")
+    for rows in (slice(0, 2), slice(v - 2, v)):
+        total = torch.zeros(2, d, dtype=torch.float64, device=DEV)
+        size = torch.zeros(2, d, dtype=torch.float64, device=DEV)
+        for a in range(0, n, 20_000):
+            x = h[a:a + 20_000].double()
+            lse = loss[a:a + 20_000].double() + (x * w[t[a:a + 20_000].clamp_min(0)].double()).sum(1)          # the loss is within its bound above
+            q = (t[a:a + 20_000, None] == torch.arange(v, device=DEV)[rows]).double()
+            dz = ((x @ w[rows].double().T - lse[:, None]).exp() - q) * torch.where(t[a:a + 20_000] == -100, 0.0, up[a:a + 20_000].double())[:, None]
+            total += dz.T @ x
+            size += dz.abs().T @ x.abs()
+        # dz is rounded by half a step, its exponent is off by less than another, the sums truncate by 2^-23 for each token
+        within(dw[rows], total, size * (2.0 ** -7 + n * 2.0 ** -23) + total.abs() * 2.0 ** -8, "dw")
+
+
+def test_many_values():
+    n = 2 ** 31 + 4099
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.empty(n, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    small = torch.ones(5, device=DEV)
+    want = sum(float(part.double().square().sum()) for part in x.split(1 << 28)) + 5
+    s = TR.GradientSet([x, small])
+    tail = x[-4099:].clone()
+    norm = s.clip(1.0)
+    assert float(norm) == pytest.approx(want ** 0.5, rel=2.0 ** -20)
+    assert torch.equal(x[-4099:], (tail.float() * (1.0 / (want ** 0.5 + 1e-6))).to(torch.bfloat16)) or torch.allclose(
+        x[-4099:].float(), tail.float() / want ** 0.5, rtol=2.0 ** -7)
+    p = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    TR.FusedAdam([p], lr=1.0, grads=[x], state=([m], [v]), eps=0.0).step()
+    live = x[-4099:] != 0
+    assert torch.equal(p[-4099:][live], -x[-4099:][live].sign()) and torch.allclose(m[-4099:], 0.1 * x[-4099:].float(), rtol=2.0 ** -22)
