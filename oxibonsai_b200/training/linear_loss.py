@@ -10,7 +10,6 @@ Reference: crates/oxibonsai-model/src/losses.rs (cross-entropy, label smoothing,
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..ops import train_ops
 
@@ -74,8 +73,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, up):
+        if torch.is_grad_enabled():
+            raise RuntimeError("linear_cross_entropy: its gradients cannot be differentiated again (create_graph=True)")
         weight, *rest = ctx.saved_tensors
         want = ctx.needs_input_grad[:2]
         if weight.is_cuda:
@@ -100,8 +100,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     scale the loss.
 
     On the GPU nothing is read back and all memory comes from torch's allocator, so that a pass and its gradients can be captured into a
-    CUDA graph; as with every operator of torch, capture them through ``torch.autograd.grad``, or while no eager graph of the same leaves
-    is alive.  Between the passes the live rows of ``hidden`` are kept (a copy) with 16 bytes per token; changing ``weight`` in between is an
+    CUDA graph; as with every operator of torch, no eager graph of the same leaves may be alive while a backward pass is captured.
+    Second derivatives are refused.  Between the passes the live rows of ``hidden`` are kept (a copy) with 16 bytes per token; changing ``weight`` in between is an
     error that autograd reports."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_cross_entropy: hidden [..., d] and weight [vocab, d] are wanted, got {tuple(hidden.shape)} and {tuple(weight.shape)}")

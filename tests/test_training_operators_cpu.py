@@ -49,6 +49,13 @@ def test_linear_cross_entropy_masked_rows():
     assert empty == 0 and TR.linear_cross_entropy(h[:0], w, t[:0]).isnan() and TR.linear_cross_entropy(h[:0], w, t[:0], reduction="none").shape == (0,)
 
 
+def test_linear_cross_entropy_has_no_second_derivative():
+    h, w, t = loss_inputs(5, 12, 6, torch.float64, "cpu")
+    h.requires_grad_(), w.requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(TR.linear_cross_entropy(h, w, t), [h, w], create_graph=True)
+
+
 def test_next_token_forms():
     h, w, t = loss_inputs(12, 30, 16, torch.float32, "cpu")
     assert torch.allclose(TR.linear_ntp_loss(h, w, t), TR.ntp_loss(h @ w.T, t), rtol=1e-5)
