@@ -828,19 +828,38 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeRows r, CeUp u, const fl
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = *r.count, splits = ce_splits(n, width, piece_blocks, terms, clusters, acc_rows);
   if (splits == 1 && n == rows) return;          // the product has stored its tiles itself
-  const long long ldn = (n + 255) & ~255;
   const float f = ce_up_scale(u, n);
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int at = r.place[row];
+  const int fours = (width + 3) >> 2;
+  const bool wide = (width & 3) == 0;
+  const long long ldn = (n + 255) & ~255, all = (long long)rows * fours;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+    const int row = (int)(i / fours), d = (int)(i % fours) * 4, at = r.place[row];
     if (at >= 0 && splits == 1) continue;
-    const int d = blockIdx.y * 256 + threadIdx.x;
-    if (d < width) {
-      float v = 0.0f;
-      if (at >= 0) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (at >= 0) {
 #pragma unroll 4
-        for (int k = 0; k < splits; ++k) v += acc[(k * ldn + at) * width + d];
+      for (int k = 0; k < splits; ++k) {
+        const float* a = acc + (k * ldn + at) * width + d;
+        if (wide) {
+          const float4 q = *reinterpret_cast<const float4*>(a);
+          v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (d + j < width) v[j] += a[j];
+        }
       }
-      out[(long long)row * width + d] = T(at >= 0 ? v * f : 0.0f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] *= f;
+    }
+    T* o = out + (long long)row * width + d;
+    if (wide && sizeof(T) == 2) {
+      __align__(8) T w[4] = {T(v[0]), T(v[1]), T(v[2]), T(v[3])};
+      *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (d + j < width) o[j] = T(v[j]);
     }
   }
 }
@@ -1107,9 +1126,8 @@ static int ce_backward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
     }
   }
   if (e == cudaSuccess && a.dhidden != nullptr) {
-    const int across = (a.width + 255) / 256, most = 148 * 16 / across > 0 ? 148 * 16 / across : 1;
-    if (across > 65535) return BONSAI_CUDA_BAD_ARG;
-    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most), (unsigned)across), dim3(256), 0, st, a.live, up, (const float*)g.acc, a.rows, g.piece_blocks,
+    const long long blocks = ((long long)a.rows * ((a.width + 3) / 4) + 255) / 256;
+    e = launch_pdl(ce_join_kernel<T>, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st, a.live, up, (const float*)g.acc, a.rows, g.piece_blocks,
                    p.planes == 3 ? kCeTerms : 1, p.clusters, p.acc_rows, a.width, (T*)a.dhidden);
   }
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
