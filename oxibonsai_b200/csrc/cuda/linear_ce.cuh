@@ -48,6 +48,7 @@ struct CeFewArgs {
   const void* x;             // [tokens of a launch][ldx] f32, zeros behind the last live row
   long long ldw, ldx;
   int vocab, width, tokens;  // tokens: the most there can be
+  int first, tokens_left;    // a launch's first token, and how many there can be from it on (set here)
   float smoothing;
   CeUp up;
   // the loss
@@ -61,7 +62,7 @@ struct CeFewArgs {
   int row_count;             // rows of dhidden
 };
 
-constexpr int kCeFew32 = 16;          // rows up to which these kernels run
+constexpr int kCeFew32 = 24;          // rows up to which these kernels run
 int ce_few_slots(int width);          // parts of dh
 int ce_few_loss_slots();              // parts of the loss
 cudaError_t ce_few_loss(const CeFewArgs& a, cudaStream_t st);

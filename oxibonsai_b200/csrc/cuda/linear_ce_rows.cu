@@ -1,10 +1,10 @@
-// The loss of an f32 head and its gradients for up to 16 live rows, on the CUDA cores.
+// The loss of an f32 head and its gradients for up to 24 live rows, on the CUDA cores.
 //
 // Here the head's bytes are all there is to it, and the tensor-core path has to copy them into three bfloat16 parts first: 4 + 6 bytes moved for each value
 // before the first product reads 6.  These kernels read the head as it lies, in any alignment, and multiply in f32; a value's multiplications, one
-// for each row, take less time than its bytes.  One row of 4096 x 151 936: 418 us here (6.0 TB/s), 2200 by parts.  From 17 rows on, two groups of
-// tokens go over the same rows of the head and the parts are faster (24 rows of 1734 x 99 135: 0.64 ms by parts, 1.38 here); with 16-bit types
-// the tensor cores need no copies and are faster from one row on.
+// for each row, take less time than its bytes.  One row of 4096 x 151 936: 418 us here (6.0 TB/s), 2200 by parts.  From 17 rows on the tokens come in two
+// launches of 16, which read the head twice: 24 rows of 4096 x 151 936 1.39 ms, 2.22 by parts, 17 rows of 2048 x 50 000 with both gradients 1.08 and
+// 1.32; with 32 rows the two are even.  With 16-bit types the tensor cores need no copies and are faster from one row on.
 //   ce_few_z_kernel   z = h W^T: a warp takes 64 / TN rows of the head against TN tokens, its lanes share the width; then the loss's running
 //                     maxima and sums (in registers, over all rows a warp takes) or dz = u (exp(z - lse) - q), f32
 //   ce_few_h_kernel   dh = dz W: a thread has four columns of dh in registers and walks down the head's rows; ce_few_join_kernel adds the parts
@@ -56,8 +56,8 @@ __global__ void __launch_bounds__(few_threads(TN), 1) ce_few_z_kernel(const CeFe
   __shared__ float block[3][DZ ? 1 : kFewWarps][TN];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = blockIdx.x * kFewWarps + (threadIdx.x >> 5), warps = gridDim.x * kFewWarps, n = *p.rows.count;
-  if (n == 0) return;
+  const int lane = threadIdx.x & 31, warp = blockIdx.x * kFewWarps + (threadIdx.x >> 5), warps = gridDim.x * kFewWarps, all = *p.rows.count, n = all - p.first;
+  if (n <= 0) return;
   // this lane's sums after the reduction: row (J lane + j) / TN, token (J lane + j) % TN
   const int t0 = (J * lane) % TN, r0 = J * lane / TN;
   int target[J];
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(few_threads(TN), 1) ce_few_z_kernel(const CeFe
     top[j] = -INFINITY;
     sum[j] = sum_z[j] = 0.0f;
     lse2[j] = DZ && ok ? p.rows.lse2[t] : 0.0f;
-    f[j] = DZ && ok ? ce_up_factor(p.up, p.rows, t) * ce_up_scale(p.up, n) : 0.0f;
+    f[j] = DZ && ok ? ce_up_factor(p.up, p.rows, t) * ce_up_scale(p.up, all) : 0.0f;
   }
   const float even = p.smoothing / (float)p.vocab;
   const int begin = (int)((long long)p.vocab * warp / warps), end = (int)((long long)p.vocab * (warp + 1) / warps);
@@ -190,9 +190,9 @@ __global__ void __launch_bounds__(kGradThreads, 2) ce_few_h_kernel(const CeFewAr
   constexpr int U = 4;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n = *p.rows.count, across = few_across(p.width), down = kGradThreads / across, x = threadIdx.x % across, y = threadIdx.x / across;
+  const int n = *p.rows.count - p.first, across = few_across(p.width), down = kGradThreads / across, x = threadIdx.x % across, y = threadIdx.x / across;
   const int c = blockIdx.x * across * 4 + (WIDE ? 4 * x : x);
-  if (n == 0) return;
+  if (n <= 0) return;
   float acc[TN][4];
 #pragma unroll
   for (int t = 0; t < TN; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
@@ -226,8 +226,9 @@ template <bool WIDE, int TN>
 __global__ void __launch_bounds__(kGradThreads, 2) ce_few_w_kernel(const CeFewArgs p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n = *p.rows.count, across = few_across(p.width), down = kGradThreads / across, x = threadIdx.x % across, y = threadIdx.x / across;
+  const int n = *p.rows.count - p.first, across = few_across(p.width), down = kGradThreads / across, x = threadIdx.x % across, y = threadIdx.x / across;
   const int c = blockIdx.x * across * 4 + (WIDE ? 4 * x : x);
+  if (p.first > 0 && n <= 0) return;
   float h[TN][4];
 #pragma unroll
   for (int t = 0; t < TN; ++t) {
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) ce_few_w_kernel(const CeFewAr
     for (int v = y; v < rows; v += down) {
       float* o = (float*)p.dweight + (long long)(v0 + v) * p.width;
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.first > 0) few_load<WIDE, false>(o, c, across, p.width, s);          // the earlier tokens' sums
 #pragma unroll
       for (int t = 0; t < TN; t += 4) {
         const float4 q = *reinterpret_cast<const float4*>(&dz[v][t]);
@@ -283,30 +285,54 @@ static int few_blocks(int width) {
 int ce_few_slots(int width) { return few_blocks(width) * (kGradThreads / few_across(width)); }
 int ce_few_loss_slots() { return kFewBlocks; }
 
+// The arguments for tokens `first` and on: every list and matrix of tokens moved up.
+static CeFewArgs few_from(CeFewArgs a, int first) {
+  a.first = first;
+  a.tokens_left = a.tokens - first;
+  a.rows.index += first; a.rows.target += first; a.rows.lse2 += first;
+  a.x = (const float*)a.x + first * a.ldx;
+  if (a.part_m != nullptr) { a.part_m += first; a.part_s += first; a.part_z += first; a.at_target += first; }
+  if (a.dz != nullptr) { a.dz += first * a.ldz; a.part += (long long)first * a.width; }
+  return a;
+}
+
 template <bool WIDE, bool DZ>
 static cudaError_t few_z(const CeFewArgs& a, cudaStream_t st) {
   const dim3 grid(kFewBlocks);
-  if (a.tokens <= 4) return launch_pdl(ce_few_z_kernel<WIDE, 4, DZ>, grid, dim3(few_threads(4)), 0, st, a);
-  if (a.tokens <= 8) return launch_pdl(ce_few_z_kernel<WIDE, 8, DZ>, grid, dim3(few_threads(8)), 0, st, a);
+  if (a.tokens_left <= 4) return launch_pdl(ce_few_z_kernel<WIDE, 4, DZ>, grid, dim3(few_threads(4)), 0, st, a);
+  if (a.tokens_left <= 8) return launch_pdl(ce_few_z_kernel<WIDE, 8, DZ>, grid, dim3(few_threads(8)), 0, st, a);
   return launch_pdl(ce_few_z_kernel<WIDE, 16, DZ>, grid, dim3(few_threads(16)), 0, st, a);
 }
 
 template <bool WIDE, int TN>
-static cudaError_t few_gradients(const CeFewArgs& a, cudaStream_t st) {
+static cudaError_t few_g(const CeFewArgs& a, cudaStream_t st) {
   const int across = few_across(a.width);
   const dim3 grid((a.width + across * 4 - 1) / (across * 4), few_blocks(a.width)), block(kGradThreads);
-  cudaError_t e = few_z<WIDE, true>(a, st);
-  if (e == cudaSuccess && a.dhidden != nullptr) e = launch_pdl(ce_few_h_kernel<WIDE, TN>, grid, block, 0, st, a);
-  if (e == cudaSuccess && a.dhidden != nullptr) e = launch_pdl(ce_few_join_kernel, dim3((a.width + 31) / 32, a.row_count), dim3(256), 0, st, a, ce_few_slots(a.width));
+  cudaError_t e = cudaSuccess;
+  if (a.dhidden != nullptr) e = launch_pdl(ce_few_h_kernel<WIDE, TN>, grid, block, 0, st, a);
   if (e == cudaSuccess && a.dweight != nullptr) e = launch_pdl(ce_few_w_kernel<WIDE, TN>, grid, block, 0, st, a);
   return e;
 }
 
-cudaError_t ce_few_loss(const CeFewArgs& a, cudaStream_t st) { return few_wide(a) ? few_z<true, false>(a, st) : few_z<false, false>(a, st); }
-
-cudaError_t ce_few_gradients(const CeFewArgs& a, cudaStream_t st) {
-  if (a.tokens <= 8) return few_wide(a) ? few_gradients<true, 8>(a, st) : few_gradients<false, 8>(a, st);
-  return few_wide(a) ? few_gradients<true, 16>(a, st) : few_gradients<false, 16>(a, st);
+template <bool WIDE>
+static cudaError_t few_gradients(const CeFewArgs& a, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  for (int first = 0; first < a.tokens && e == cudaSuccess; first += 16) {
+    const CeFewArgs b = few_from(a, first);
+    e = few_z<WIDE, true>(b, st);
+    if (e == cudaSuccess) e = b.tokens_left <= 8 ? few_g<WIDE, 8>(b, st) : few_g<WIDE, 16>(b, st);
+  }
+  if (e == cudaSuccess && a.dhidden != nullptr) e = launch_pdl(ce_few_join_kernel, dim3((a.width + 31) / 32, a.row_count), dim3(256), 0, st, a, ce_few_slots(a.width));
+  return e;
 }
+
+cudaError_t ce_few_loss(const CeFewArgs& a, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  for (int first = 0; first < a.tokens && e == cudaSuccess; first += 16)
+    e = few_wide(a) ? few_z<true, false>(few_from(a, first), st) : few_z<false, false>(few_from(a, first), st);
+  return e;
+}
+
+cudaError_t ce_few_gradients(const CeFewArgs& a, cudaStream_t st) { return few_wide(a) ? few_gradients<true>(a, st) : few_gradients<false>(a, st); }
 
 }  // namespace bonsai
