@@ -62,7 +62,9 @@ def _check_apart(tensors: Iterable[torch.Tensor], what: str) -> None:
 
 def _counters(tensors: Sequence[torch.Tensor]) -> list[torch.Tensor]:
     """Tensors that have the version counters of all of these: views of one tensor share its counter."""
-    return list({id(t if t._base is None else t._base): t for t in tensors}.values())
+    tensors = [t for t in tensors if not t.is_inference()]          # those have none
+    owners = [t if t._base is None else t._base for t in tensors]
+    return list({id(o): t for o, t in zip(owners, tensors)}.values())
 
 
 class GradientSet:

@@ -93,6 +93,22 @@ def test_gradient_set():
     assert TR.global_grad_norm([p, q]) == 5.0 and TR.clip_global_norm([p, q], 1.0) == 5.0 and TR.grad_norm([p]) == pytest.approx(1.0, rel=1e-5)
 
 
+def test_written_tensors_count_a_version():
+    flat, single = torch.ones(10), torch.ones(3)
+    views = [flat[:4], flat[5:]]
+    was = [t._version for t in (flat, single)]
+    TR.GradientSet(views + [single]).clip(1.0)
+    assert flat._version > was[0] and single._version > was[1]
+    p = torch.ones(3, requires_grad=True)
+    y = (p * p).sum()
+    opt = TR.FusedAdam([p], grads=[torch.ones(3)])
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        TR.GradientSet([torch.ones(3)]).clip(1.0)
+
+
 def test_gradient_set_refusals():
     a = torch.zeros(8)
     for bad, error in ((lambda: TR.GradientSet([a, a]), ValueError), (lambda: TR.GradientSet([a[:5], a[4:]]), ValueError),
