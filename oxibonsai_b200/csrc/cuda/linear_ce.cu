@@ -531,7 +531,6 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
         few_top[i] = -INFINITY;
         few_sum[i] = few_z[i] = 0.0f;
         few_target[i] = token < n ? p.rows.target[token] : -1;
-        if (few_target[i] < 0) few_target[i] = -0x40000000;          // in no tile
       }
     }
     for (int tile = cid; tile < tiles.all; tile += nclusters) {
