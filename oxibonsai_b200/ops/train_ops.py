@@ -49,9 +49,17 @@ def _stream(device: torch.device) -> int:
 
 # ---- many tensors ---------------------------------------------------------------------------------------------------------------
 class TensorTable:
-    """Addresses, sizes and types of dense CUDA tensors of one device, packed for the kernels.  Tensors without values are left out."""
+    """Addresses, sizes and types of dense CUDA tensors of one device, packed for the kernels.  Tensors without values are left out.
+    ``like``: the table of tensors of the same sizes.  ``keep``: the memory stays allocated as long as the table is there, whatever becomes
+    of the tensors."""
 
-    def __init__(self, tensors: Sequence[torch.Tensor]):
+    def __init__(self, tensors: Sequence[torch.Tensor], like: "TensorTable | None" = None, keep: bool = False):
+        self.memory = [t.untyped_storage() for t in tensors] if keep else None
+        if like is not None and like.n == len(tensors):
+            self.n, self.numel, self.partials = like.n, like.numel, like.partials
+            self.ptrs = (C.c_void_p * max(1, self.n))(*[t.data_ptr() for t in tensors])
+            self.types = (C.c_ubyte * max(1, self.n))(*[TYPE_CODES[t.dtype] for t in tensors])
+            return
         numel = [t.numel() for t in tensors]
         if 0 in numel:
             tensors = [t for t, n in zip(tensors, numel) if n]

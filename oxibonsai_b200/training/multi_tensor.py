@@ -90,8 +90,8 @@ class GradientSet:
         self._written = _counters(self.out)
         self._table = self._out_table = None
         if self.device.type == "cuda":
-            self._table = train_ops.TensorTable(self.tensors)
-            self._out_table = self._table if out is None else train_ops.TensorTable(self.out)
+            self._table = train_ops.TensorTable(self.tensors, keep=True)
+            self._out_table = self._table if out is None else train_ops.TensorTable(self.out, keep=True)
 
     def __len__(self) -> int:
         return len(self.tensors)
@@ -142,7 +142,8 @@ class FusedAdam:
     (``p.grad`` itself stays as it is) and returns their norm as a 0-dim tensor.
 
     Parameters are float32, float16 or bfloat16, the moments float32.  ``grads``: fixed gradient tensors, one for each parameter, whose
-    table is made once; without them every step looks up ``p.grad`` (parameters without one are skipped).  ``state``: lists of first and
+    table is made once (neither they nor the parameters may change their memory then); without them every step looks up ``p.grad``
+    (parameters without one are skipped) and where the parameters are.  ``state``: lists of first and
     second moments to go on from, updated in place.  The step count is on the device: with ``grads`` a step can be captured into a
     CUDA graph, ``lr`` then as a 0-dim float32 CUDA tensor where it changes."""
 
@@ -170,10 +171,8 @@ class FusedAdam:
         _check_apart(self.params + self.m + self.v, name)
         self.steps = torch.full((), steps, dtype=torch.int64, device=self.device)
         self.grads = None if grads is None else list(grads)
-        self._written = _counters(self.params)
         self._tables = None
-        if self.device.type == "cuda":
-            self._fixed = [train_ops.TensorTable(x) for x in (self.params, self.m, self.v)]
+        self._place()
         if self.grads is not None:
             if len(self.grads) != len(self.params):
                 raise ValueError(f"{name}: {len(self.grads)} gradients for {len(self.params)} parameters")
@@ -181,10 +180,28 @@ class FusedAdam:
             if any(not _same_order(p, g) for p, g in zip(self.params, self.grads)):
                 raise ValueError(f"{name}: fixed gradients need their parameters' shapes and strides")
             if self.device.type == "cuda":
-                self._tables = self._with(self.grads)
+                self._tables = self._with(self.grads, keep=True)
 
-    def _with(self, grads: Sequence[torch.Tensor]) -> list[train_ops.TensorTable]:
-        return [self._fixed[0], train_ops.TensorTable(grads), *self._fixed[1:]]
+    def _place(self) -> None:
+        """Notes where the parameters and moments are."""
+        self._written = _counters(self.params)
+        self._layout = [(p.shape, p.stride()) for p in self.params]
+        if self.device.type == "cuda":
+            self._at = [p.data_ptr() for p in self.params]
+            self._fixed = [train_ops.TensorTable(x, keep=True) for x in (self.params, self.m, self.v)]
+
+    def _follow(self) -> None:
+        """Parameters whose memory was replaced since (``p.data = ...``) are found at their new places."""
+        if [p.data_ptr() for p in self.params] == self._at:
+            return
+        name = type(self).__name__
+        if _check(self.params, name) != self.device or not all(_same_order(p, m) for p, m in zip(self.params, self.m)):
+            raise ValueError(f"{name}: a parameter has moved to another device or changed its shape since the optimizer was made")
+        _check_apart(self.params + self.m + self.v, name)
+        self._place()
+
+    def _with(self, grads: Sequence[torch.Tensor], keep: bool = False) -> list[train_ops.TensorTable]:
+        return [self._fixed[0], train_ops.TensorTable(grads, like=self._fixed[0], keep=keep), *self._fixed[1:]]
 
     def _check_grads(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor]) -> None:
         name = type(self).__name__
@@ -206,8 +223,13 @@ class FusedAdam:
         if self._tables is not None:
             tables = self._tables
         else:
+            if self.device.type == "cuda":
+                self._follow()
             grads = self.grads if self.grads is not None else [p.grad for p in self.params]
             params, m, v, every = self.params, self.m, self.v, True
+            if self.device.type == "cuda" and all(g is not None and g.layout is torch.strided and g.shape == shape and g.stride() == stride
+                                                  and g.dtype in _TYPES and g.device == self.device for g, (shape, stride) in zip(grads, self._layout)):
+                return self._run(self._with(grads), lr, max_norm)
             if any(g is None for g in grads):
                 live = [i for i, g in enumerate(grads) if g is not None]
                 params, grads, m, v = ([part[i] for i in live] for part in (params, grads, m, v))
@@ -219,6 +241,9 @@ class FusedAdam:
             with torch.no_grad():
                 grads = [g if _same_order(p, g) else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
             tables = self._with(grads) if every else [train_ops.TensorTable(x) for x in (params, grads, m, v)]
+        return self._run(tables, lr, max_norm)
+
+    def _run(self, tables: list[train_ops.TensorTable], lr: float | torch.Tensor, max_norm: float | None) -> torch.Tensor | None:
         if tables[0].n == 0:
             self.steps += 1
             return None if max_norm is None else torch.zeros((), dtype=torch.float32, device=self.device)

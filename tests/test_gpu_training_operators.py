@@ -389,6 +389,25 @@ def test_adam_without_fixed_gradients():
     assert fa.step(max_norm=1.0) == 0 and fa.t == 5
 
 
+def test_adam_follows_replaced_parameters():
+    p = torch.ones(1000, device=DEV, requires_grad=True)
+    p.grad = torch.ones(1000, device=DEV)
+    opt = TR.FusedAdam([p], lr=0.1)
+    opt.step()
+    old = p.data
+    p.data = p.data.clone()
+    opt.step()
+    assert float(p[0].detach()) < float(old[0]) - 0.05                   # the new memory was stepped, the old one not
+    p.data = torch.ones(500, 2, device=DEV)
+    p.grad = torch.ones(500, 2, device=DEV)
+    with pytest.raises(ValueError):
+        opt.step()
+    x = torch.full((64,), 3.0, device=DEV)
+    s = TR.GradientSet([x])
+    x.data = torch.zeros(64, device=DEV)
+    assert float(s.norm()) == 24.0                                        # a set keeps the memory that it was made with
+
+
 def test_adam_in_a_graph():
     p, g = [torch.ones(1000, device=DEV)], [torch.ones(1000, device=DEV)]
     q, lr = [torch.ones(1000, device=DEV)], torch.tensor(0.1, device=DEV)
