@@ -5,6 +5,7 @@ CUDA tensors go through the kernels, and a missing library raises.
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes as C
 from typing import Sequence
@@ -50,25 +51,25 @@ def _stream(device: torch.device) -> int:
 # ---- many tensors ---------------------------------------------------------------------------------------------------------------
 class TensorTable:
     """Addresses, sizes and types of dense CUDA tensors of one device, packed for the kernels.  Tensors without values are left out.
-    ``like``: the table of tensors of the same sizes.  ``keep``: the memory stays allocated as long as the table is there, whatever becomes
-    of the tensors."""
+    ``like``: the table of as many tensors of the same sizes (others are refused).  ``keep``: the memory stays allocated as long as the
+    table is there, whatever becomes of the tensors."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], like: "TensorTable | None" = None, keep: bool = False):
         self.memory = [t.untyped_storage() for t in tensors] if keep else None
-        if like is not None and like.n == len(tensors):
-            self.n, self.numel, self.partials = like.n, like.numel, like.partials
-            self.ptrs = (C.c_void_p * max(1, self.n))(*[t.data_ptr() for t in tensors])
-            self.types = (C.c_ubyte * max(1, self.n))(*[TYPE_CODES[t.dtype] for t in tensors])
-            return
-        numel = [t.numel() for t in tensors]
-        if 0 in numel:
-            tensors = [t for t, n in zip(tensors, numel) if n]
-            numel = [n for n in numel if n]
-        self.n = len(numel)
-        self.ptrs = (C.c_void_p * max(1, self.n))(*[t.data_ptr() for t in tensors])
-        self.numel = (C.c_longlong * max(1, self.n))(*numel)
-        self.types = (C.c_ubyte * max(1, self.n))(*[TYPE_CODES[t.dtype] for t in tensors])
-        self.partials = int(_lib().bonsai_mt_partials(self.n))
+        self.sizes = [t.numel() for t in tensors]
+        if like is not None and self.sizes != like.sizes:
+            raise ValueError("TensorTable: tensors of the sizes of the other table are wanted")
+        if 0 in self.sizes:
+            tensors = [t for t, n in zip(tensors, self.sizes) if n]
+        self.n = len(tensors)
+        # an optimizer makes a table for each of its steps: arrays from buffers, not element by element
+        self.ptrs = (C.c_void_p * max(1, self.n)).from_buffer(array.array("Q", [t.data_ptr() for t in tensors] or [0]))
+        self.types = (C.c_ubyte * max(1, self.n)).from_buffer_copy(bytes([TYPE_CODES[t.dtype] for t in tensors] or [0]))
+        if like is not None:
+            self.numel, self.partials = like.numel, like.partials
+        else:
+            self.numel = (C.c_longlong * max(1, self.n))(*[n for n in self.sizes if n])
+            self.partials = int(_lib().bonsai_mt_partials(self.n))
 
 
 def _norm_room(grads: TensorTable, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:

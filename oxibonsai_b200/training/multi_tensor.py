@@ -34,6 +34,10 @@ def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.shape == b.shape and (a.stride() == b.stride() or all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1))
 
 
+def _layout(tensors: Sequence[torch.Tensor]) -> tuple[list, list, list]:
+    return [t.shape for t in tensors], [t.stride() for t in tensors], [t.dtype for t in tensors]
+
+
 def _check(tensors: Sequence[torch.Tensor], what: str) -> torch.device:
     device = None
     for t in tensors:
@@ -185,20 +189,29 @@ class FusedAdam:
     def _place(self) -> None:
         """Notes where the parameters and moments are."""
         self._written = _counters(self.params)
-        self._layout = [(p.shape, p.stride()) for p in self.params]
+        self._at, self._layout = [p.data_ptr() for p in self.params], _layout(self.params)
         if self.device.type == "cuda":
-            self._at = [p.data_ptr() for p in self.params]
             self._fixed = [train_ops.TensorTable(x, keep=True) for x in (self.params, self.m, self.v)]
 
     def _follow(self) -> None:
-        """Parameters whose memory was replaced since (``p.data = ...``) are found at their new places."""
-        if [p.data_ptr() for p in self.params] == self._at:
+        """Parameters whose memory was replaced since (``p.data = ...``) are found at their new places.  ``p.data[:n]`` has the old address: the
+        tables hold for the noted sizes, orders and types only."""
+        if [p.data_ptr() for p in self.params] == self._at and _layout(self.params) == self._layout:
             return
         name = type(self).__name__
         if _check(self.params, name) != self.device or not all(_same_order(p, m) for p, m in zip(self.params, self.m)):
             raise ValueError(f"{name}: a parameter has moved to another device or changed its shape since the optimizer was made")
         _check_apart(self.params + self.m + self.v, name)
         self._place()
+
+    def _lie_like_params(self, grads: Sequence[torch.Tensor | None]) -> bool:
+        """Whether every parameter has a gradient that the kernel can walk as it is (list by list: some 0.1 us for each tensor and property)."""
+        if type(None) in set(map(type, grads)) or set([g.get_device() for g in grads]) != {self.device.index} or not set([g.dtype for g in grads]) <= set(_TYPES):
+            return False
+        try:
+            return [g.shape for g in grads] == self._layout[0] and [g.stride() for g in grads] == self._layout[1]
+        except RuntimeError:          # a sparse tensor has no strides
+            return False
 
     def _with(self, grads: Sequence[torch.Tensor], keep: bool = False) -> list[train_ops.TensorTable]:
         return [self._fixed[0], train_ops.TensorTable(grads, like=self._fixed[0], keep=keep), *self._fixed[1:]]
@@ -223,12 +236,10 @@ class FusedAdam:
         if self._tables is not None:
             tables = self._tables
         else:
-            if self.device.type == "cuda":
-                self._follow()
+            self._follow()
             grads = self.grads if self.grads is not None else [p.grad for p in self.params]
             params, m, v, every = self.params, self.m, self.v, True
-            if self.device.type == "cuda" and all(g is not None and g.layout is torch.strided and g.shape == shape and g.stride() == stride
-                                                  and g.dtype in _TYPES and g.device == self.device for g, (shape, stride) in zip(grads, self._layout)):
+            if self.device.type == "cuda" and self._lie_like_params(grads):
                 return self._run(self._with(grads), lr, max_norm)
             if any(g is None for g in grads):
                 live = [i for i, g in enumerate(grads) if g is not None]
