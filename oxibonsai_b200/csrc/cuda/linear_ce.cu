@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include "linear_ce.cuh"
+#include "linear_ce_issue.h"
 #include "tcgen05.cuh"
 
 namespace bonsai {
@@ -487,31 +488,39 @@ __global__ void __launch_bounds__(kCeThreads, 1) __cluster_dims__(2, 1, 1) ce_ge
     if (rank == 0 && tc::elect_one()) {
       constexpr uint32_t fmt = sizeof(T) == 2 && __is_same(T, __half) ? tc::FMT_F16 : tc::FMT_BF16;
       const uint32_t idesc = tc::idesc_f32acc(fmt, fmt, 256, (uint32_t)p.tile_n) | (MODE == CE_DW ? 1u << 15 : 0u) | (kAcross ? 1u << 16 : 0u);
-      bool failed = false;
-      int s = 0, seg = 0;
-      uint32_t phase = 0;
-      for (int tile = cid; tile < tiles.all && !failed; tile += nclusters) {
+      struct Issue {
+        uint8_t *sA, *sB;
+        uint64_t *full, *empty, *accf, *acce;
+        uint32_t taddr, idesc, phase;
+        int s;
+        __device__ __forceinline__ bool wait_acc(int ab, uint32_t parity) {
+          const bool ok = tc::mbar_wait(&acce[ab], parity);
+          tc::tc_fence_after();
+          return ok;
+        }
+        __device__ __forceinline__ bool wait_full() {
+          const bool ok = tc::mbar_wait(&full[s], phase);
+          tc::tc_fence_after();
+          return ok;
+        }
+        __device__ __forceinline__ void product(int ab, bool first) {
+          const uint32_t a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kOperandB);
+          const uint64_t da = MODE == CE_DW ? ce_desc_mn(a) : tc::smem_desc_sw128(a), db = kAcross ? ce_desc_mn(b) : tc::smem_desc_sw128(b);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)
+            ce_mma(taddr + ab * kCols, da + (MODE == CE_DW ? 128 : 2) * k, db + (kAcross ? 128 : 2) * k, idesc, !first || k > 0);
+          ce_commit(&empty[s]);
+          if (++s == kStages) { s = 0; phase ^= 1; }
+        }
+        __device__ __forceinline__ void commit_acc(int ab) { ce_commit(&accf[ab]); }
+      } issue = {sA, sB, full, empty, accf, acce, taddr, idesc, 0, 0};
+      bool ok = true;
+      int seg = 0;
+      for (int tile = cid; tile < tiles.all && ok; tile += nclusters) {
         int rt, ct, split, b0, b1;
         tiles.at(tile, &rt, &ct, &split);
         part(split, &b0, &b1);
-        for (int k0 = b0; k0 < b1 && !failed; ++seg) {
-          const int ab = seg % kBufs, k1 = kSums ? min(b1, k0 + kSegment) : b1;
-          if (!tc::mbar_wait(&acce[ab], ((seg / kBufs) & 1) ^ 1)) { failed = true; break; }
-          tc::tc_fence_after();
-          for (int i = 0; i < (k1 - k0) * kTerms; ++i) {
-            if (!tc::mbar_wait(&full[s], phase)) { failed = true; break; }
-            tc::tc_fence_after();
-            const uint32_t a = tc::smem_u32(sA + s * kCeOperand), b = tc::smem_u32(sB + s * kOperandB);
-            const uint64_t da = MODE == CE_DW ? ce_desc_mn(a) : tc::smem_desc_sw128(a), db = kAcross ? ce_desc_mn(b) : tc::smem_desc_sw128(b);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-              ce_mma(taddr + ab * kCols, da + (MODE == CE_DW ? 128 : 2) * k, db + (kAcross ? 128 : 2) * k, idesc, i > 0 || k > 0);
-            ce_commit(&empty[s]);
-            if (++s == kStages) { s = 0; phase ^= 1; }
-          }
-          ce_commit(&accf[ab]);
-          k0 = k1;
-        }
+        ok = ce_issue<kBufs, kSums ? kSegment : 0>(issue, b0, b1, kTerms, &seg);
       }
     }
     __syncwarp();
