@@ -19,8 +19,9 @@
 // Rows whose target is the ignored one are left out before anything is multiplied: the live rows are copied side by side, and their number
 // stays on the device.  A target outside the vocabulary makes its row's loss and gradients NaN, and so does a wait that expires.
 //
-// dz is rounded to the inputs' 16-bit type before it is multiplied, as the operand of a tensor-core product has to be.  It is stored without the
-// upstream gradient's size (that factor enters with the products' sums), in f16 scaled by 2^15: probabilities down to 2^-29 stay normal.
+// dz is rounded to the inputs' 16-bit type before it is multiplied, as the operand of a tensor-core product has to be.  It is stored over the largest
+// finite upstream gradient (that factor enters with the products' sums), in f16 times 2^15: in a row that has it probabilities down to 2^-29 stay normal. Where
+// rows bring gradients of their own (reduction "none"), dz of a row 2^k below the largest is held in steps of 2^(k-39) of its own.
 //
 // float32 inputs become three bfloat16 parts each (8 bits a part, exact down to 2^-24) and six products of parts: the parts that are left out
 // are below 2^-24 of the product.
@@ -813,14 +814,17 @@ __global__ void __launch_bounds__(kCeMergeRows * kCeMergeLanes) ce_merge_kernel(
   if (threadIdx.x == 0) *loss = (float)(reduce == CE_MEAN ? sums[0] / (double)n : sums[0]);
 }
 
-// max |u| over the live rows
+// max |u| over the live rows whose u is finite: an infinite one, as a NaN, is for its own row alone
 __global__ void __launch_bounds__(1024) ce_top_kernel(CeRows r, const float* up, float* out) {
   __shared__ float s[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = *r.count;
   float top = 0.0f;
-  for (int i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, fabsf(up[r.index[i]]));
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float u = fabsf(up[r.index[i]]);
+    if (u < INFINITY) top = fmaxf(top, u);
+  }
   top = warp_max(top);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = top;
   __syncthreads();

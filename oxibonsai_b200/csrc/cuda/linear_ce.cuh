@@ -20,12 +20,12 @@ struct CeRows {         // the live rows, in order: filled by ce_rows_kernel
 
 struct CeUp {           // the upstream gradient u: one value, or one for each row ("none")
   const float* up;
-  const float* top;     // "none": max |u|
+  const float* top;     // "none": max |u| of the finite ones
   int reduce;
   float dz_scale;       // what dz is stored with
 };
 __device__ __forceinline__ float ce_up_top(const CeUp& u) { return u.reduce == CE_NONE ? *u.top : fabsf(*u.up); }
-// u_i over the largest |u|; u is 0 or NaN where none is above 0
+// u_i over the largest finite |u|; where none is above 0, u_i itself: 0 or not finite
 __device__ __forceinline__ float ce_up_factor(const CeUp& u, const CeRows& r, int row) {
   const float top = ce_up_top(u), x = u.up[u.reduce == CE_NONE ? r.index[row] : 0];
   return r.target[row] < 0 ? NAN : top > 0.0f ? x / top : x;

@@ -97,7 +97,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     type; logits, sums and products are float32 whatever the inputs, and on the GPU the gradient of the logits is rounded to the
     inputs' type before it is multiplied, as a product of that type does.  A target outside the vocabulary raises on the CPU; on the GPU,
     where nothing waits for the result, its loss and the gradients that it enters are NaN.  float16 gradients underflow as everywhere:
-    scale the loss.
+    scale the loss; with "none" the GPU holds the gradient of the logits in steps of 2^-39 of the largest finite upstream gradient of the
+    call.  A token whose upstream gradient is not finite has no finite gradient, and neither has the head; other tokens' are as without it.
 
     On the GPU nothing is read back and all memory comes from torch's allocator, so that a pass and its gradients can be captured into a
     CUDA graph; as with every operator of torch, no eager graph of the same leaves may be alive while a backward pass is captured.
