@@ -128,8 +128,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"linear_cross_entropy: rows of at most 2^24 values are wanted, got {weight.shape[1]}")
     flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     if targets.numel() == 0:
-        loss = flat.float().sum() * 0.0 + weight[:0].float().sum() * 0.0       # zero gradients
-        return loss * float("nan") if reduction == "mean" else loss if reduction == "sum" else flat.float().sum(-1).reshape(targets.shape)
+        kind = torch.float64 if flat.dtype == torch.float64 else torch.float32
+        loss = flat.to(kind).sum(1) + weight[:0].to(kind).sum()                # zero gradients of both
+        return loss.sum() * float("nan") if reduction == "mean" else loss.sum() if reduction == "sum" else loss.reshape(targets.shape)
     if flat.is_cuda:
         flat = flat if flat.is_contiguous() or (flat.stride(1) == 1 and flat.stride(0) >= flat.shape[1]) else flat.contiguous()
         weight = weight if weight.is_contiguous() or (weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1]) else weight.contiguous()
