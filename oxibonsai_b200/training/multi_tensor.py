@@ -251,16 +251,20 @@ class FusedAdam:
             # the kernel walks memory: a gradient that autograd laid out in another order than its parameter is copied into it
             with torch.no_grad():
                 grads = [g if _same_order(p, g) else torch.empty_like(p, dtype=g.dtype).copy_(g) for p, g in zip(params, grads)]
-            tables = self._with(grads) if every else [train_ops.TensorTable(x) for x in (params, grads, m, v)]
+            if not every:
+                return self._run([train_ops.TensorTable(x) for x in (params, grads, m, v)], lr, max_norm, _counters(params))
+            tables = self._with(grads)
         return self._run(tables, lr, max_norm)
 
-    def _run(self, tables: list[train_ops.TensorTable], lr: float | torch.Tensor, max_norm: float | None) -> torch.Tensor | None:
+    def _run(self, tables: list[train_ops.TensorTable], lr: float | torch.Tensor, max_norm: float | None,
+             written: list[torch.Tensor] | None = None) -> torch.Tensor | None:
+        """``written``: tensors with the version counters of the parameters that are stepped, where those are not all."""
         if tables[0].n == 0:
             self.steps += 1
             return None if max_norm is None else torch.zeros((), dtype=torch.float32, device=self.device)
         norm = train_ops.mt_adam(*tables, self.steps, lr if isinstance(lr, torch.Tensor) else float(lr), self.betas, self.eps, self.wd, self.decoupled,
                                  None if max_norm is None else float(max_norm))
-        increment_version(self._written)
+        increment_version(self._written if written is None else written)
         return norm
 
     @torch.no_grad()

@@ -114,3 +114,20 @@ def test_adam_refuses_gradients_that_no_kernel_walks(launches):
     with pytest.raises(TypeError):
         opt.step()
     assert not launches
+
+
+@pytest.mark.parametrize("cpu", [False, True])
+def test_adam_counts_versions_of_the_parameters_that_it_steps(cpu, launches):
+    a, b = _parameter(5), _parameter(7)
+    opt = TR.FusedAdam([a, b]) if cpu else _optimizer([a, b])
+    loss = (b * b).sum()                                # keeps b for its backward pass
+    b.grad = None
+    was = a._version
+    opt.step(max_norm=1.0)
+    assert a._version > was
+    loss.backward()                                     # b has not been written
+    opt.step()
+    loss = (b * b).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
