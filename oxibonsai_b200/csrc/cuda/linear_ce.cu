@@ -1145,9 +1145,11 @@ static int ce_backward(const CeArgs& a, const CePlan& p, cudaStream_t st) {
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
+// Below 2^30 the sum of a row's number and a piece's or a tile's rows fits an int.
 static bool ce_good(const CeArgs& a) {
-  return a.weight != nullptr && a.rows >= 1 && a.vocab >= 1 && a.width >= 1 && a.ldw >= a.width && a.rows < 0x7fffe000 && a.vocab < 0x7fffe000 &&
-         a.width < 0x7fffe000 && a.type >= CE_F32 && a.type <= CE_BF16 && a.reduce >= CE_MEAN && a.reduce <= CE_NONE;
+  constexpr int most = 1 << 30;
+  return a.weight != nullptr && a.rows >= 1 && a.vocab >= 1 && a.width >= 1 && a.ldw >= a.width && a.rows < most && a.vocab < most && a.width < most &&
+         a.type >= CE_F32 && a.type <= CE_BF16 && a.reduce >= CE_MEAN && a.reduce <= CE_NONE;
 }
 
 static CeArgs ce_args(const void* weight, long long ldw, int rows, int vocab, int width, int type, int reduce, float smoothing, void* kept, void* ws) {

@@ -91,7 +91,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     """Cross entropy of the logits ``hidden @ weight.T`` against ``targets``, differentiable in ``hidden`` and ``weight``.
 
     ``hidden`` [..., d] and ``weight`` [vocab, d] have one type (float32, float16 or bfloat16; on the CPU float64 too), ``targets`` [...]
-    are int64 or int32.  Tokens with ``ignore_index`` have loss 0 and no gradient, whatever their hidden row holds; ``reduction`` is
+    are int64 or int32; each of the three sizes is below 2^30.  Tokens with ``ignore_index`` have loss 0 and no gradient, whatever their hidden row holds; ``reduction`` is
     "mean" over the others (NaN where there are none), "sum" or "none" (a loss of the shape of ``targets``).  The target distribution is
     ``(1 - label_smoothing)`` at the target plus ``label_smoothing / vocab`` everywhere.  The loss is float32, gradients have the inputs'
     type; logits, sums and products are float32 whatever the inputs, and on the GPU the gradient of the logits is rounded to the
@@ -121,8 +121,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     types = (torch.float32, torch.float16, torch.bfloat16) + (() if hidden.is_cuda else (torch.float64,))
     if hidden.dtype != weight.dtype or hidden.dtype not in types:
         raise TypeError(f"linear_cross_entropy: hidden and weight of one type (float32, float16, bfloat16) are wanted, got {hidden.dtype} and {weight.dtype}")
-    if min(weight.shape) < 1 or max(*weight.shape, targets.numel()) >= 2 ** 31 - 4096:
-        raise ValueError(f"linear_cross_entropy: a vocabulary and a width of at least 1 and less than 2^31 are wanted, got {tuple(weight.shape)} and "
+    if min(weight.shape) < 1 or max(*weight.shape, targets.numel()) >= 2 ** 30:
+        raise ValueError(f"linear_cross_entropy: a vocabulary and a width of at least 1 and less than 2^30 are wanted, got {tuple(weight.shape)} and "
                          f"{targets.numel()} targets")
     if weight.shape[1] > 2 ** 24:
         raise ValueError(f"linear_cross_entropy: rows of at most 2^24 values are wanted, got {weight.shape[1]}")
