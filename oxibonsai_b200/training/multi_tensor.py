@@ -55,13 +55,15 @@ def _check(tensors: Sequence[torch.Tensor], what: str) -> torch.device:
     return device or torch.device("cpu")
 
 
-def _check_apart(tensors: Iterable[torch.Tensor], what: str) -> None:
-    """Tensors that are written must not share memory: two blocks would scale or step the same values."""
-    last = 0
-    for begin, size in sorted([(t.data_ptr(), t.nbytes) for t in tensors]):
-        if size and begin < last:
+def _check_apart(tensors: Iterable[torch.Tensor], what: str, read: Iterable[torch.Tensor] = ()) -> None:
+    """Tensors that are written must not share memory, with one another or with those that are only ``read``: two blocks would scale or
+    step the same values, or one would read what another has written."""
+    last = last_written = 0
+    for begin, size, written in sorted([(t.data_ptr(), t.nbytes, True) for t in tensors] + [(t.data_ptr(), t.nbytes, False) for t in read]):
+        if size and begin < (last if written else last_written):
             raise ValueError(f"{what}: two of the tensors share memory")
         last = max(last, begin + size)
+        last_written = max(last_written, begin + size if written else 0)
 
 
 def _counters(tensors: Sequence[torch.Tensor]) -> list[torch.Tensor]:
@@ -183,6 +185,7 @@ class FusedAdam:
             self._check_grads(self.params, self.grads)
             if any(not _same_order(p, g) for p, g in zip(self.params, self.grads)):
                 raise ValueError(f"{name}: fixed gradients need their parameters' shapes and strides")
+            _check_apart(self.params + self.m + self.v, name, read=self.grads)
             if self.device.type == "cuda":
                 self._tables = self._with(self.grads, keep=True)
 
