@@ -134,12 +134,15 @@ def _share(norm: float, max_norm: float) -> float:
 
 
 def global_grad_norm(params: Iterable[torch.Tensor]) -> torch.Tensor:
-    """``grad_norm`` as a 0-dim tensor on the gradients' device, in two launches."""
-    return GradientSet([g for g in [p.grad for p in params] if g is not None]).norm()
+    """``grad_norm`` as a 0-dim tensor on the gradients' device, in two launches.  Nothing is written: a parameter may be listed twice, and
+    counts twice."""
+    grads = [g for g in [p.grad for p in params] if g is not None]
+    device = _check(grads, "global_grad_norm")
+    return train_ops.mt_norm(train_ops.TensorTable(grads), device) if device.type == "cuda" else _norm(grads).float()
 
 
 def clip_global_norm(params: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
-    """``clip_grad_norm`` as a 0-dim tensor on the gradients' device, in two launches."""
+    """``clip_grad_norm`` as a 0-dim tensor on the gradients' device, in two launches.  Gradients that share memory are refused."""
     return GradientSet([g for g in [p.grad for p in params] if g is not None]).clip(max_norm)
 
 
