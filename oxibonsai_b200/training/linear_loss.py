@@ -134,7 +134,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if flat.is_cuda:
         flat = flat if flat.is_contiguous() or (flat.stride(1) == 1 and flat.stride(0) >= flat.shape[1]) else flat.contiguous()
         weight = weight if weight.is_contiguous() or (weight.stride(1) == 1 and weight.stride(0) >= weight.shape[1]) else weight.contiguous()
-    loss = _LinearCrossEntropy.apply(flat, weight, targets.reshape(-1).long(), ignore_index, reduction, float(label_smoothing))
+    loss = _LinearCrossEntropy.apply(flat, weight, targets.reshape(-1).long().contiguous(), ignore_index, reduction, float(label_smoothing))
     return loss.reshape(targets.shape) if reduction == "none" and targets.dim() != 1 else loss
 
 
