@@ -2,9 +2,9 @@
 //
 // Here the head's bytes are all there is to it, and the tensor-core path has to copy them into three bfloat16 parts first: 4 + 6 bytes moved for each value
 // before the first product reads 6.  These kernels read the head as it lies, in any alignment, and multiply in f32; a value's multiplications, one
-// for each row, take less time than its bytes.  One row of 4096 x 151 936: 418 us here (6.0 TB/s), 2200 by parts.  From 17 rows on the tokens come in two
-// launches of 16, which read the head twice: 24 rows of 4096 x 151 936 1.39 ms, 2.22 by parts, 17 rows of 2048 x 50 000 with both gradients 1.08 and
-// 1.32; with 32 rows the two are even.  With 16-bit types the tensor cores need no copies and are faster from one row on.
+// for each row, take less time than its bytes.  One row of 4096 x 151 936: 429 us for the whole call (5.8 TB/s), 2200 by parts.  From 17 rows on the tokens
+// come in two launches of 16, which read the head twice: 24 rows of 4096 x 151 936 1.42 ms (its bytes: 0.38), 2.25 by parts, 17 rows of 2048 x 50 000
+// with both gradients 1.11 and 1.32; with 32 rows the two are even.  With 16-bit types the tensor cores need no copies and are faster from one row on.
 //   ce_few_z_kernel   z = h W^T: a warp takes 64 / TN rows of the head against TN tokens, its lanes share the width; then the loss's running
 //                     maxima and sums (in registers, over all rows a warp takes) or dz = u (exp(z - lse) - q), f32
 //   ce_few_h_kernel   dh = dz W: a thread has four columns of dh in registers and walks down the head's rows; ce_few_join_kernel adds the parts

@@ -10,7 +10,7 @@
 // copied to the device, and a captured launch carries its own table.  Squares are added in f32 over eight neighbours and in f64 from
 // there on; the partial sums of the blocks are added in one order by every block that needs the norm, so that there is no atomic, no
 // counter to reset, and the same values give the same bits.  All three are bound by memory: a clipped AdamW step of 705 M bf16 parameters with f32
-// moments moves 16.9 GB in 2.74 ms (6.2 TB/s), clipping 705 M bf16 gradients into f32 ones 5.6 GB in 0.93 ms (6.0 TB/s).
+// moments moves 16.9 GB in 2.73 to 2.79 ms (6.1 TB/s), clipping 705 M bf16 gradients into f32 ones 5.6 GB in 0.94 ms (6.0 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
