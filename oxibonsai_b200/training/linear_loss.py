@@ -91,10 +91,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     """Cross entropy of the logits ``hidden @ weight.T`` against ``targets``, differentiable in ``hidden`` and ``weight``.
 
     ``hidden`` [..., d] and ``weight`` [vocab, d] have one type (float32, float16 or bfloat16; on the CPU float64 too), ``targets`` [...]
-    are int64 or int32; each of the three sizes is below 2^30.  Tokens with ``ignore_index`` have loss 0 and no gradient, whatever their hidden row holds; ``reduction`` is
-    "mean" over the others (NaN where there are none), "sum" or "none" (a loss of the shape of ``targets``).  The target distribution is
-    ``(1 - label_smoothing)`` at the target plus ``label_smoothing / vocab`` everywhere.  The loss is float32, gradients have the inputs'
-    type; logits, sums and products are float32 whatever the inputs, and on the GPU the gradient of the logits is rounded to the
+    are int64 or int32; there are less than 2^30 tokens and vocabulary rows, of at most 2^24 values.  Tokens with ``ignore_index`` have
+    loss 0 and no gradient, whatever their hidden row holds; ``reduction`` is "mean" over the others (NaN where there are none), "sum" or
+    "none" (a loss of the shape of ``targets``).  The target distribution is ``(1 - label_smoothing)`` at the target plus
+    ``label_smoothing / vocab`` everywhere.  The loss is float32 (float64 of float64), gradients have the inputs' type; logits, sums and products are float32 whatever the inputs, and on the GPU the gradient of the logits is rounded to the
     inputs' type before it is multiplied, as a product of that type does.  A target outside the vocabulary raises on the CPU; on the GPU,
     where nothing waits for the result, its loss and the gradients that it enters are NaN.  float16 gradients underflow as everywhere:
     scale the loss; with "none" the GPU holds the gradient of the logits in steps of 2^-39 of the largest finite upstream gradient of the
@@ -102,8 +102,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 
     On the GPU nothing is read back and all memory comes from torch's allocator, so that a pass and its gradients can be captured into a
     CUDA graph; as with every operator of torch, no eager graph of the same leaves may be alive while a backward pass is captured.
-    Second derivatives are refused.  Between the passes the live rows of ``hidden`` are kept (a copy) with 16 bytes per token; changing ``weight`` in between is an
-    error that autograd reports."""
+    Second derivatives are refused.  Between the passes the live rows of ``hidden`` are kept (a copy) with 16 bytes per token; changing
+    ``weight`` in between is an error that autograd reports."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear_cross_entropy: hidden [..., d] and weight [vocab, d] are wanted, got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if targets.shape != hidden.shape[:-1]:
