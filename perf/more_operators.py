@@ -414,23 +414,23 @@ def run(state):
 
 
 def work(case):
+    size = BYTES[case["dtype"]]
     if case["do"] == "update":
-        n, d, out, r, size = case["rows"], case["d"], case["out"], case["rank"], BYTES[case["dtype"]]
+        n, d, out, r = case["rows"], case["d"], case["out"], case["rank"]
         weights = max(1, min(n, case["adapters"])) * r * (d + out) * size
         moved, flops = n * (d + 2 * out) * size + weights + 4 * n * (case["adapters"] > 0), 2.0 * n * r * (d + out)
-        if case["train"]:          # dy, x and the factors again, the three gradients
-            moved, flops = moved + n * (2 * d + out) * size + 2 * weights, 3 * flops
+        if case["train"]:          # the gradient of the output comes in, those of the rows and of both factors go out
+            moved, flops = moved + n * (d + out) * size + weights, 3 * flops
         return {"bytes": moved, "flops": flops}
-    size = BYTES[case["dtype"]]
     if case["do"] == "dropout":
         n = case["rows"] * case["d"]
         return {"bytes": 4 * n * size, "flops": 2.0 * n}
-    if case["do"] == "preference":         # two log-probabilities and a mask, the mask again and the gradient
+    if case["do"] == "preference":         # two log-probabilities and a mask; the gradient
         n = 2 * case["pairs"] * case["length"]
-        return {"bytes": n * (3 * size + 2) + 8 * case["pairs"], "flops": 3.0 * n}
-    n = case["rows"] * case["length"]      # three log-probabilities, gains and a mask, twice; the gradient
+        return {"bytes": n * (3 * size + 1) + 8 * case["pairs"], "flops": 3.0 * n}
+    n = case["rows"] * case["length"]      # three log-probabilities, gains and a mask; the gradient
     gains = n if case["per_token"] else case["rows"]
-    return {"bytes": 2 * (n * (3 * size + 1) + 4 * gains) + n * size + 8 * n * (case["reduction"] == "none"), "flops": 30.0 * n}
+    return {"bytes": n * (4 * size + 1) + 4 * gains + 8 * n * (case["reduction"] == "none"), "flops": 30.0 * n}
 
 
 def exact(case, seed):
