@@ -1,0 +1,808 @@
+// Low-rank updates of many adapters, and their gradients.  A row i of x has the adapter e = ids[i] with factors A_e [rank][in] and B_e [out][rank]:
+//
+//   forward    h_i = A_e x~_i;   y_i = base_i + s_e B_e h_i                   x~: x, or what dropout leaves of it (philox.cuh)
+//   backward   g_i = B_e^T dy_i; dx_i = s_e A_e^T g_i (dropped again);  dA_e = s_e sum_i g_i x~_i^T;  dB_e = s_e sum_i dy_i h_i^T
+//
+// Both directions of the rows are the same kernel (lr_rows_kernel): a product over a long axis that leaves `rank` values a row, and one from these to a long
+// axis.  A cluster of blocks takes one tile of rows of one adapter: each block multiplies its part of the long axis, the parts meet over
+// distributed shared memory in one order, and each block writes its part of the columns.  One launch, no workspace, no atomics; rank values never
+// leave the chip unless a backward pass wants them.  The factors' gradients are a second kernel (lr_outer_kernel): sums over an adapter's rows,
+// split over a cluster and joined the same way.
+//
+// All are bound by memory: 2 rank operations for each value that is read.  So the matrix instructions are mma.sync, whose operands are gathered rows
+// from shared memory; tcgen05 would want tiles of 128 rows and does not pay at one operation a byte.  The long product of 16-bit types multiplies them as they are
+// (f32 sums); everything that meets the rank values keeps these in two TF32 parts, 22 bits, beside 16-bit operands that TF32 holds exactly.  f32 operands are
+// two TF32 parts too, three products of them, added to f32 registers every few steps because the matrix instructions' own sums truncate.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "philox.cuh"
+
+namespace bonsai {
+
+constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
+constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
+enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
+
+struct LrGroups {            // which rows have which adapter
+  int mode;
+  const void* ids;           // LR_SELF
+  int ids_wide;              // int64, else int32
+  const int* order;          // LR_PLAN: rows by adapter; behind them those without one, and those whose id names none
+  const int* start;          // [adapters + 3]: where each adapter's rows begin in it
+  int n, adapters;
+};
+
+struct LrRowsArgs {
+  LrGroups groups;
+  const void* x; long long ldx;          // [n][k]
+  const void *w1, *w2;                   // forward: A, B; backward: B, A
+  const void* base; long long ld_base;   // [n][cols], may be null
+  void* y; long long ldy;                // null: the rank values alone are wanted
+  float* kept;                           // [n][padded rank] by place in the order, may be null
+  const float* scales;                   // of the adapters, or null: scale
+  float scale;
+  int k, cols, rank;
+  int stages;
+  int vec_x, vec_w1, vec_w2, vec_y;      // rows that 16-byte (w2 of the forward pass: 4-byte) accesses may take
+  DropoutRule drop;
+  int drop_x, drop_y;                    // forward: the rows of x; backward: those of dx
+};
+
+struct LrOuterArgs {
+  LrGroups groups;
+  // two products of one launch: 0: dA [rank][k] from x (dropped) and g, 1: dB [cols][rank] from dy and h
+  const void* q[2]; long long ldq[2];
+  const float* p[2];
+  void* out[2];
+  int width[2], blocks[2], vec[2];       // columns, blocks of columns
+  int rank;
+  const float* scales;
+  float scale;
+  DropoutRule drop;
+  int drop_x;
+};
+
+// ---- values ------------------------------------------------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ float lr_float(T v);
+template <> __device__ __forceinline__ float lr_float(float v) { return v; }
+template <> __device__ __forceinline__ float lr_float(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float lr_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T lr_round(float v);
+template <> __device__ __forceinline__ float lr_round(float v) { return v; }
+template <> __device__ __forceinline__ __half lr_round(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 lr_round(float v) { return __float2bfloat16_rn(v); }
+// the two halves of a word of 16-bit values
+template <typename T> __device__ __forceinline__ float2 lr_pair(uint32_t w);
+template <> __device__ __forceinline__ float2 lr_pair<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 lr_pair<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 lr_pair<float>(uint32_t w) { return make_float2(__uint_as_float(w), 0.0f); }     // not used
+
+// eight neighbouring values
+template <typename T, bool VEC>
+__device__ __forceinline__ void lr_load8(const T* p, int n, float* v) {
+  if (VEC) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = lr_pair<T>(w[i]);
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? lr_float<T>(p[i]) : 0.0f;
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void lr_store8(T* p, int n, const float* v) {
+  if (VEC) {
+    __align__(16) T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = lr_round<T>(v[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = lr_round<T>(v[i]);
+  }
+}
+
+// ---- shared memory, matrix instructions --------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t lr_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void lr_copy16(void* dst, const void* src, bool there) {       // zeros where it is not there
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(lr_smem(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void lr_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void lr_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// waits until at most `left` of the latest groups are in flight
+__device__ __forceinline__ void lr_wait_left(int left) {
+  if (left <= 0) lr_wait<0>();
+  else if (left == 1) lr_wait<1>();
+  else if (left == 2) lr_wait<2>();
+  else lr_wait<3>();
+}
+__device__ __forceinline__ void lr_ldm4(uint32_t* r, const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(lr_smem(p)) : "memory");
+}
+__device__ __forceinline__ void lr_ldm4t(uint32_t* r, const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(lr_smem(p)) : "memory");
+}
+template <typename T> __device__ __forceinline__ void lr_mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void lr_mma16<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void lr_mma16<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void lr_mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t lr_tf32(float v) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return r;
+}
+// v = hi + lo to 2^-23; an infinity has no second part
+__device__ __forceinline__ void lr_split(float v, uint32_t& hi, uint32_t& lo) {
+  hi = lr_tf32(v);
+  const float h = __uint_as_float(hi);
+  lo = fabsf(h) <= 3.4028234e38f ? lr_tf32(v - h) : 0u;
+}
+
+// ---- clusters ------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t lr_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t lr_ranks() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void lr_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void lr_meet() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 lr_remote4(const float* p, uint32_t rank) {
+  uint32_t at;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(lr_smem(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// ---- groups of rows ----------------------------------------------------------------------------------------------------------------------
+// adapters: group `adapters` are the rows without one, adapters + 1 those whose id names none
+__device__ __forceinline__ int lr_group(const LrGroups& g, int row) {
+  const long long id = g.ids_wide ? ((const long long*)g.ids)[row] : (long long)((const int*)g.ids)[row];
+  return id < 0 ? g.adapters : id < g.adapters ? (int)id : g.adapters + 1;
+}
+
+struct LrTile {
+  int group, count, place;   // rows in it, place of its first one in the order
+};
+
+// The tile of rows of slot `slot`; rows[i]: its row numbers, -1 behind the last.  Every block of a cluster finds the same one.
+template <int M>
+__device__ __forceinline__ LrTile lr_tile(const LrGroups& g, int slot, int* rows, int* s) {
+  const int t = threadIdx.x;
+  LrTile tile = {0, 0, 0};
+  if (g.mode == LR_ONE) {
+    tile.place = slot * M;
+    tile.count = g.n - tile.place < M ? g.n - tile.place : M;
+    if (t < M) rows[t] = t < tile.count ? tile.place + t : -1;
+  } else if (g.mode == LR_SELF) {
+    // Row `slot` leads a tile where the rows of its adapter before it fill whole tiles: it and the next ones are the tile.
+    const int mine = lr_group(g, slot), of = t < g.n ? lr_group(g, t) : -1;
+    const int before = __syncthreads_count(of == mine && t < slot);
+    if (before % M != 0) return tile;
+    if (t < M) rows[t] = -1;
+    const bool in = of == mine && t >= slot;
+    const unsigned b = __ballot_sync(0xffffffffu, in);
+    if ((t & 31) == 0) s[t >> 5] = __popc(b);
+    __syncthreads();
+    int at = __popc(b & ((1u << (t & 31)) - 1u)), all = 0;
+    for (int w = 0; w < kLrWarps; ++w) {
+      at += w < (t >> 5) ? s[w] : 0;
+      all += s[w];
+    }
+    if (in && at < M) rows[at] = t;
+    tile.group = mine;
+    tile.count = all < M ? all : M;
+  } else {
+    for (int e = t; e < g.adapters + 2; e += kLrThreads) {
+      const int lo = g.start[e], hi = g.start[e + 1], first = lo / M + e;
+      if (slot >= first && slot <= hi / M + e) { s[0] = e; s[1] = lo + (slot - first) * M; s[2] = hi; }
+    }
+    __syncthreads();
+    tile.group = s[0];
+    tile.place = s[1];
+    const int left = s[2] - tile.place;
+    if (left <= 0) return tile;
+    tile.count = left < M ? left : M;
+    if (t < M) rows[t] = t < tile.count ? g.order[tile.place + t] : -1;
+  }
+  __syncthreads();
+  return tile;
+}
+
+// Eight values of a row in shared memory, those without a bit set to 0; what stays is scaled behind the sums.  The thread that copied them calls it.
+template <typename T>
+__device__ __forceinline__ void lr_drop8(T* p, unsigned bits) {
+  if constexpr (sizeof(T) == 4) {
+    float4* v = reinterpret_cast<float4*>(p);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float4 f = v[h];
+      f.x = bits >> (4 * h) & 1u ? f.x : 0.0f; f.y = bits >> (4 * h + 1) & 1u ? f.y : 0.0f;
+      f.z = bits >> (4 * h + 2) & 1u ? f.z : 0.0f; f.w = bits >> (4 * h + 3) & 1u ? f.w : 0.0f;
+      v[h] = f;
+    }
+  } else {
+    uint4 w = *reinterpret_cast<uint4*>(p);
+    auto both = [&](int i) { return (bits >> i & 1u ? 0xffffu : 0u) | (bits >> (i + 1) & 1u ? 0xffff0000u : 0u); };
+    w.x &= both(0); w.y &= both(2); w.z &= both(4); w.w &= both(6);
+    *reinterpret_cast<uint4*>(p) = w;
+  }
+}
+
+// Eights of rows into shared memory: rows r < nrows of `from(r)` (null: zeros), columns c0 .. c0 + C - 1 of `width`; to: rows of `pitch` values.  any: a
+// readable address for copies of nothing.
+template <typename T, int C, typename From>
+__device__ __forceinline__ void lr_fill(T* to, int pitch, int nrows, int c0, int width, bool vec, const T* any, From from) {
+  for (int u = threadIdx.x; u < nrows * (C / 8); u += kLrThreads) {
+    const int r = u / (C / 8), c = u % (C / 8) * 8;
+    const T* src = from(r);
+    T* dst = to + r * pitch + c;
+    const int left = src != nullptr ? width - c0 - c : 0;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(dst + i * (16 / sizeof(T)), left > 0 ? src + c0 + c + i * (16 / sizeof(T)) : any, left > 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dst[i] = i < left ? src[c0 + c + i] : lr_round<T>(0.0f);
+    }
+  }
+}
+
+// ---- the rows ------------------------------------------------------------------------------------------------------------------------------
+template <int M> struct LrShape {
+  static constexpr int kM16 = M / 16, kParts = kLrWarps / kM16;       // warps over rows, and over the long axis
+  static constexpr int kChunk = M == 64 ? 64 : 128, kWarpK = kChunk / kParts;
+  static constexpr int kMw = M == 64 ? 2 : 1, kAcross = kLrWarps / (kM16 / kMw);      // of the second product: 16-row tiles of a warp, warps over columns
+};
+
+template <typename T, int R, int M, bool BACK> struct LrSmem {
+  static constexpr int kPad = 16 / sizeof(T);
+  static constexpr int kChunk = LrShape<M>::kChunk;
+  static constexpr int kPitchX = kChunk + kPad, kPitchW = BACK ? R + 8 : kChunk + kPad, kRowsW = BACK ? kChunk : R;
+  static constexpr int kStage = (M * kPitchX + kRowsW * kPitchW) * (int)sizeof(T);
+  static constexpr int kJoin = LrShape<M>::kParts * M * R * 4;         // the warps' parts, over the stages
+  static constexpr int kPart = M * R * 4, kPitchH = R + 4, kH = M * kPitchH * 4;
+  static constexpr int bytes(int stages) { return (stages * kStage > kJoin ? stages * kStage : kJoin) + kPart + kH; }
+};
+
+template <typename T, int R, int M, bool BACK>
+__global__ void __launch_bounds__(kLrThreads) lr_rows_kernel(const __grid_constant__ LrRowsArgs a) {
+  using S = LrShape<M>;
+  using L = LrSmem<T, R, M, BACK>;
+  constexpr bool F32 = sizeof(T) == 4;
+  extern __shared__ __align__(16) unsigned char lr_dynamic[];
+  __shared__ int rows[M];
+  __shared__ int scratch[kLrWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int ring = a.stages * L::kStage > L::kJoin ? a.stages * L::kStage : L::kJoin;
+  float* join = reinterpret_cast<float*>(lr_dynamic);
+  float* part = reinterpret_cast<float*>(lr_dynamic + ring);
+  float* hs = part + M * R;
+  const uint32_t rank = lr_rank(), ranks = lr_ranks();
+  const LrTile tile = lr_tile<M>(a.groups, blockIdx.x / ranks, rows, scratch);
+  if (tile.count == 0) return;                        // the whole cluster
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const bool has = tile.group < a.groups.adapters;
+  const uint2 key = a.drop_x || a.drop_y ? philox_key(a.drop) : make_uint2(0, 0);
+
+  if (has) {
+    const T* w1 = (const T*)a.w1 + (long long)tile.group * a.k * a.rank;
+    const int chunks = (a.k + S::kChunk - 1) / S::kChunk;
+    const int c0 = (int)((long long)chunks * rank / ranks), c1 = (int)((long long)chunks * (rank + 1) / ranks);
+    auto stage = [&](int i) { return reinterpret_cast<T*>(lr_dynamic + i * L::kStage); };
+    auto fetch = [&](int c, int slot) {
+      T* xs = stage(slot);
+      const int k0 = c * S::kChunk;
+      lr_fill<T, S::kChunk>(xs, L::kPitchX, M, k0, a.k, a.vec_x, (const T*)a.x, [&](int r) { return rows[r] < 0 ? (const T*)nullptr : (const T*)a.x + rows[r] * a.ldx; });
+      if (BACK)
+        lr_fill<T, R>(xs + M * L::kPitchX, L::kPitchW, S::kChunk, 0, a.rank, a.vec_w1, w1,
+                      [&](int r) { return k0 + r < a.k ? w1 + (long long)(k0 + r) * a.rank : (const T*)nullptr; });
+      else
+        lr_fill<T, S::kChunk>(xs + M * L::kPitchX, L::kPitchW, R, k0, a.k, a.vec_w1, w1,
+                              [&](int r) { return r < a.rank ? w1 + (long long)r * a.k : (const T*)nullptr; });
+    };
+    float acc[R / 8][4];
+#pragma unroll
+    for (int j = 0; j < R / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+    const int m0 = warp % S::kM16 * 16, kp = warp / S::kM16 * S::kWarpK;
+    for (int i = 0; i < a.stages - 1; ++i) {
+      if (c0 + i < c1) fetch(c0 + i, i);
+      lr_commit();
+    }
+    int slot = 0;
+    for (int c = c0; c < c1; ++c) {
+      lr_wait_left(a.stages - 2);
+      T* xs = stage(slot);
+      if (a.drop_x) {
+        for (int u = threadIdx.x; u < M * (S::kChunk / 8); u += kLrThreads) {       // the eights that this thread copied
+          const int r = u / (S::kChunk / 8), col = u % (S::kChunk / 8) * 8;
+          if (rows[r] >= 0) lr_drop8<T>(xs + r * L::kPitchX + col, dropout_bits((unsigned)(c * S::kChunk + col) >> 3, rows[r], key, a.drop.steps));
+        }
+      }
+      __syncthreads();
+      if (c + a.stages - 1 < c1) fetch(c + a.stages - 1, slot == 0 ? a.stages - 1 : slot - 1);
+      lr_commit();
+      const T* ws = xs + M * L::kPitchX;
+      if constexpr (!F32) {
+#pragma unroll
+        for (int k = 0; k < S::kWarpK; k += 16) {
+          uint32_t x[4];
+          lr_ldm4(x, xs + (m0 + (lane & 15)) * L::kPitchX + kp + k + (lane >> 4) * 8);
+#pragma unroll
+          for (int j = 0; j < R / 16; ++j) {
+            uint32_t w[4];
+            if (BACK) lr_ldm4t(w, ws + (kp + k + (lane & 15)) * L::kPitchW + j * 16 + (lane >> 4) * 8);
+            else lr_ldm4(w, ws + (j * 16 + (lane & 7) + (lane >> 4) * 8) * L::kPitchW + kp + k + (lane >> 3 & 1) * 8);
+            lr_mma16<T>(acc[2 * j], x, w[0], w[1]);
+            lr_mma16<T>(acc[2 * j + 1], x, w[2], w[3]);
+          }
+        }
+      } else {
+        float sum[R / 8][4];
+#pragma unroll
+        for (int j = 0; j < R / 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[j][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < S::kWarpK; k += 8) {
+          uint32_t hi[4], lo[4];
+          const float* xp = (const float*)xs + (m0 + g) * L::kPitchX + kp + k + t;
+          lr_split(xp[0], hi[0], lo[0]);
+          lr_split(xp[8 * L::kPitchX], hi[1], lo[1]);
+          lr_split(xp[4], hi[2], lo[2]);
+          lr_split(xp[8 * L::kPitchX + 4], hi[3], lo[3]);
+#pragma unroll
+          for (int j = 0; j < R / 8; ++j) {
+            const float* wp = BACK ? (const float*)ws + (kp + k + t) * L::kPitchW + j * 8 + g : (const float*)ws + (j * 8 + g) * L::kPitchW + kp + k + t;
+            uint32_t h0, l0, h1, l1;
+            lr_split(wp[0], h0, l0);
+            lr_split(wp[BACK ? 4 * L::kPitchW : 4], h1, l1);
+            lr_mma8(sum[j], lo, h0, h1);
+            lr_mma8(sum[j], hi, l0, l1);
+            lr_mma8(sum[j], hi, h0, h1);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < R / 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][i] += sum[j][i];
+      }
+      slot = slot + 1 == a.stages ? 0 : slot + 1;
+    }
+    lr_wait<0>();
+    __syncthreads();                                   // the stages are read: the warps' parts go over them
+    float* mine = join + (warp / S::kM16 * M + m0) * R;
+#pragma unroll
+    for (int j = 0; j < R / 8; ++j) {
+      *reinterpret_cast<float2*>(mine + g * R + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * R + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < M * R / 4; u += kLrThreads) {
+      float4 v = reinterpret_cast<const float4*>(join)[u];
+#pragma unroll
+      for (int p = 1; p < S::kParts; ++p) {
+        const float4 w = reinterpret_cast<const float4*>(join)[p * (M * R / 4) + u];
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
+      reinterpret_cast<float4*>(part)[u] = v;
+    }
+    lr_arrive();
+    lr_meet();
+    const float share = a.drop_x ? a.drop.share : 1.0f;
+    for (int u = threadIdx.x; u < M * R / 4; u += kLrThreads) {
+      float4 v = lr_remote4(part + 4 * u, 0);
+      for (uint32_t r = 1; r < ranks; ++r) {
+        const float4 w = lr_remote4(part + 4 * u, r);
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
+      const int row = u / (R / 4), col = u % (R / 4) * 4;
+      // behind the rank there is nothing, also beside an infinity, whose product with the zeros there is none
+      v.x = col < a.rank ? v.x * share : 0.0f; v.y = col + 1 < a.rank ? v.y * share : 0.0f;
+      v.z = col + 2 < a.rank ? v.z * share : 0.0f; v.w = col + 3 < a.rank ? v.w * share : 0.0f;
+      *reinterpret_cast<float4*>(hs + row * L::kPitchH + col) = v;
+      if (a.kept != nullptr && rank == 0 && row < tile.count) *reinterpret_cast<float4*>(a.kept + (long long)(tile.place + row) * R + col) = v;
+    }
+    lr_arrive();                                       // this block has read the others' parts; it leaves when they have read its own
+    __syncthreads();
+  }
+
+  // y = base + s W2 h: a warp takes 32 columns at a time.  Column 8 (c / 2) + 2 j + c % 2 is column c of its j-th product, so that the eight values that a
+  // thread has of a row lie side by side.
+  const float by = a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale;
+  const T* w2 = (const T*)a.w2 + (has ? (long long)tile.group * a.cols * a.rank : 0);
+  const int all = (a.cols + 31) / 32;
+  const int b0 = (int)((long long)all * rank / ranks), b1 = a.y != nullptr ? (int)((long long)all * (rank + 1) / ranks) : b0;
+  const int m0 = warp / S::kAcross * S::kMw * 16;
+  for (int b = b0 + warp % S::kAcross; b < b1; b += S::kAcross) {
+    const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
+    float from[S::kMw][2][8];
+#pragma unroll
+    for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = rows[m0 + m * 16 + h * 8 + g];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) from[m][h][i] = 0.0f;
+        if (a.base != nullptr && row >= 0 && left > 0) {
+          const T* p = (const T*)a.base + row * a.ld_base + col;
+          if (a.vec_y) lr_load8<T, true>(p, 8, from[m][h]);
+          else lr_load8<T, false>(p, left, from[m][h]);
+        }
+      }
+    float acc[S::kMw][4][4];
+#pragma unroll
+    for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.0f;
+    if (has) {
+      const int wc = b * 32 + 8 * (g >> 1);                      // eight columns, of which this thread takes every second
+#pragma unroll 2
+      for (int k = 0; k < R; k += 8) {
+        if (k >= a.rank) break;
+        float w[4][2];                                           // of product j: k + t, k + t + 4
+        const int k0 = k + t, k1 = k + t + 4;
+        if (BACK) {
+          float v[8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int kk = h ? k1 : k0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+            if (kk < a.rank && wc < a.cols) {
+              const T* p = w2 + (long long)kk * a.cols + wc;
+              if (a.vec_w2) lr_load8<T, true>(p, 8, v);
+              else lr_load8<T, false>(p, a.cols - wc, v);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j][h] = g & 1 ? v[2 * j + 1] : v[2 * j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int cc = wc + 2 * j + (g & 1);
+            const T* p = w2 + (long long)cc * a.rank;
+            w[j][0] = cc < a.cols && k0 < a.rank ? lr_float<T>(p[k0]) : 0.0f;
+            w[j][1] = cc < a.cols && k1 < a.rank ? lr_float<T>(p[k1]) : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < S::kMw; ++m) {
+          uint32_t hi[4], lo[4];
+          const float* hp = hs + (m0 + m * 16 + g) * L::kPitchH + k + t;
+          lr_split(hp[0], hi[0], lo[0]);
+          lr_split(hp[8 * L::kPitchH], hi[1], lo[1]);
+          lr_split(hp[4], hi[2], lo[2]);
+          lr_split(hp[8 * L::kPitchH + 4], hi[3], lo[3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (F32) {
+              uint32_t h0, l0, h1, l1;
+              lr_split(w[j][0], h0, l0);
+              lr_split(w[j][1], h1, l1);
+              lr_mma8(acc[m][j], lo, h0, h1);
+              lr_mma8(acc[m][j], hi, l0, l1);
+              lr_mma8(acc[m][j], hi, h0, h1);
+            } else {
+              lr_mma8(acc[m][j], lo, __float_as_uint(w[j][0]), __float_as_uint(w[j][1]));
+              lr_mma8(acc[m][j], hi, __float_as_uint(w[j][0]), __float_as_uint(w[j][1]));
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = rows[m0 + m * 16 + h * 8 + g];
+        if (row < 0 || left <= 0) continue;
+        float v[8];
+        const unsigned keep = a.drop_y ? dropout_bits((unsigned)col >> 3, row, key, a.drop.steps) : 0xffu;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = acc[m][i >> 1][2 * h + (i & 1)] * by;
+          v[i] = tile.group > a.groups.adapters ? __uint_as_float(0x7fc00000u) : !has ? from[m][h][i]
+                 : a.drop_y ? (keep >> i & 1u ? d * a.drop.share : 0.0f) : from[m][h][i] + d;
+        }
+        T* p = (T*)a.y + row * a.ldy + col;
+        if (a.vec_y) lr_store8<T, true>(p, 8, v);
+        else lr_store8<T, false>(p, left, v);
+      }
+  }
+  __syncwarp();
+  if (has) lr_meet();
+}
+
+// ---- the factors' gradients --------------------------------------------------------------------------------------------------------------
+// out[r][c] (or [c][r]) = s sum over the adapter's rows of p[row][r] q[row][c].  A cluster takes 128 columns of one adapter and one product, its blocks
+// split the rows.  The two rows 2 t and 2 t + 1 of every eight are what a thread has of a matrix instruction's axis of eight, which is how ldmatrix hands
+// out 16-bit values of q; p follows.
+template <typename T, int R> struct LrOuterSmem {
+  static constexpr int kPitchQ = kLrOuterCols + (sizeof(T) == 4 ? 4 : 8), kPitchP = R + 4;
+  static constexpr int kStage = kLrOuterRows * (kPitchQ * (int)sizeof(T) + kPitchP * 4);
+  static constexpr int kSum = R * kLrOuterCols * 4;
+  static constexpr int bytes(int stages) { return stages * kStage > kSum ? stages * kStage : kSum; }
+};
+
+template <typename T, int R>
+__global__ void __launch_bounds__(kLrThreads) lr_outer_kernel(const __grid_constant__ LrOuterArgs a) {
+  using L = LrOuterSmem<T, R>;
+  constexpr bool F32 = sizeof(T) == 4;
+  extern __shared__ __align__(16) unsigned char lr_dynamic[];
+  __shared__ int rows[3][kLrOuterRows];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t rank = lr_rank(), ranks = lr_ranks();
+  const int cluster = blockIdx.x / ranks, per = a.blocks[0] + a.blocks[1], adapter = cluster / per, within = cluster % per;
+  const int which = within < a.blocks[0] ? 0 : 1, width = a.width[which], col0 = (within - (which ? a.blocks[0] : 0)) * kLrOuterCols;
+  int first = 0, last = a.groups.n;
+  if (a.groups.mode == LR_PLAN) { first = a.groups.start[adapter]; last = a.groups.start[adapter + 1]; }
+  const int steps = (last - first + kLrOuterRows - 1) / kLrOuterRows;
+  const int s0 = (int)((long long)steps * rank / ranks), s1 = (int)((long long)steps * (rank + 1) / ranks);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const T* q = (const T*)a.q[which];
+  const bool drop = which == 0 && a.drop_x;
+  const uint2 key = drop ? philox_key(a.drop) : make_uint2(0, 0);
+  auto list = [&](int s) {          // row numbers of a step, three steps side by side
+    if (threadIdx.x < kLrOuterRows) {
+      const int place = first + s * kLrOuterRows + threadIdx.x;
+      rows[s % 3][threadIdx.x] = place < last ? (a.groups.mode == LR_PLAN ? a.groups.order[place] : place) : -1;
+    }
+  };
+  auto qs = [&](int i) { return reinterpret_cast<T*>(lr_dynamic + i * L::kStage); };
+  auto ps = [&](int i) { return reinterpret_cast<float*>(lr_dynamic + i * L::kStage + kLrOuterRows * L::kPitchQ * sizeof(T)); };
+  auto fetch = [&](int s, int slot) {
+    const int* list = rows[s % 3];
+    lr_fill<T, kLrOuterCols>(qs(slot), L::kPitchQ, kLrOuterRows, col0, width, a.vec[which], q, [&](int r) { return list[r] < 0 ? (const T*)nullptr : q + list[r] * a.ldq[which]; });
+    lr_fill<float, R>(ps(slot), L::kPitchP, kLrOuterRows, 0, R, true, a.p[which], [&](int r) {
+      const int place = first + s * kLrOuterRows + r;
+      return place < last ? a.p[which] + (long long)place * R : (const float*)nullptr;
+    });
+  };
+  float acc[R / 16][2][4];
+#pragma unroll
+  for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.0f;
+  // two stages: the rows of step s + 2 are listed while s is multiplied
+  if (s0 < s1) list(s0);
+  if (s0 + 1 < s1) list(s0 + 1);
+  __syncthreads();
+  if (s0 < s1) fetch(s0, 0);
+  lr_commit();
+  for (int s = s0; s < s1; ++s) {
+    const int slot = (s - s0) & 1;
+    if (s + 1 < s1) fetch(s + 1, slot ^ 1);
+    lr_commit();
+    if (s + 2 < s1) list(s + 2);
+    lr_wait<1>();
+    if (drop) {
+      const int* list = rows[s % 3];
+      for (int u = threadIdx.x; u < kLrOuterRows * (kLrOuterCols / 8); u += kLrThreads) {
+        const int r = u / (kLrOuterCols / 8), c = u % (kLrOuterCols / 8) * 8;
+        if (list[r] >= 0) lr_drop8<T>(qs(slot) + r * L::kPitchQ + c, dropout_bits((unsigned)(col0 + c) >> 3, list[r], key, a.drop.steps));
+      }
+    }
+    __syncthreads();
+    const T* qp = qs(slot) + warp * 16;
+    const float* pp = ps(slot);
+    float sum[R / 16][2][4];
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[i][j][k] = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < kLrOuterRows; k += 16) {
+      float v[2][2][2];             // of the first and the second eight rows: product j, rows 2 t and 2 t + 1
+      if constexpr (F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[h][j][i] = ((const float*)qp)[(k + 8 * h + 2 * t + i) * L::kPitchQ + j * 8 + g];
+      } else {
+        uint32_t w[4];
+        lr_ldm4t(w, qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 f = lr_pair<T>(w[2 * j + h]);
+            v[h][j][0] = f.x; v[h][j][1] = f.y;
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t vh[2][2], vl[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if constexpr (F32) lr_split(v[h][j][i], vh[j][i], vl[j][i]);
+            else vh[j][i] = __float_as_uint(v[h][j][i]);
+          }
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i) {
+          uint32_t hi[4], lo[4];
+          const float* p = pp + (k + 8 * h + 2 * t) * L::kPitchP + i * 16 + g;
+          lr_split(p[0], hi[0], lo[0]);
+          lr_split(p[8], hi[1], lo[1]);
+          lr_split(p[L::kPitchP], hi[2], lo[2]);
+          lr_split(p[L::kPitchP + 8], hi[3], lo[3]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float* d = F32 ? sum[i][j] : acc[i][j];
+            lr_mma8(d, lo, vh[j][0], vh[j][1]);
+            if constexpr (F32) lr_mma8(d, hi, vl[j][0], vl[j][1]);
+            lr_mma8(d, hi, vh[j][0], vh[j][1]);
+          }
+        }
+      }
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[i][j][k];
+    }
+    __syncthreads();
+  }
+  lr_wait<0>();
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(lr_dynamic);            // [R][128]
+#pragma unroll
+  for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float* p = part + (i * 16 + g) * kLrOuterCols + warp * 16 + j * 8 + 2 * t;
+      *reinterpret_cast<float2*>(p) = make_float2(acc[i][j][0], acc[i][j][1]);
+      *reinterpret_cast<float2*>(p + 8 * kLrOuterCols) = make_float2(acc[i][j][2], acc[i][j][3]);
+    }
+  lr_arrive();
+  lr_meet();
+  const float by = (a.scales != nullptr ? a.scales[adapter] : a.scale) * (drop ? a.drop.share : 1.0f);
+  T* out = (T*)a.out[which] + (long long)adapter * a.rank * width;
+  // each block adds and writes its share of the tile: along the rank for dB, whose rank values lie side by side
+  for (int u = threadIdx.x + rank * kLrThreads; u < R * kLrOuterCols / 4; u += kLrThreads * ranks) {
+    const int r = u / (kLrOuterCols / 4), c = u % (kLrOuterCols / 4) * 4;
+    if (r >= a.rank || col0 + c >= width) continue;
+    float4 v = lr_remote4(part + 4 * u, 0);
+    for (uint32_t k = 1; k < ranks; ++k) {
+      const float4 w = lr_remote4(part + 4 * u, k);
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
+    const float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col0 + c + i < width) out[which ? (long long)(col0 + c + i) * a.rank + r : (long long)r * width + col0 + c + i] = lr_round<T>(f[i]);
+  }
+  __syncwarp();
+  lr_arrive();
+  lr_meet();
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------------------------
+template <typename Kern, typename Args>
+static cudaError_t lr_launch(Kern kernel, int clusters, int ranks, int smem, cudaStream_t st, const Args& args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)clusters * ranks);
+  cfg.blockDim = dim3(kLrThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ranks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+// Blocks of a cluster: as many, in powers of two, as bring the grid near two blocks an SM, and no more than `most` have work.
+inline int lr_ranks_for(long long clusters, long long most) {
+  int ranks = 1;
+  while (ranks < 8 && 2 * ranks <= most && clusters * ranks < 148 * 2) ranks *= 2;
+  return ranks;
+}
+
+constexpr int kLrSmemMost = 227 * 1024 - 1024;
+
+template <typename T, int R, int M, bool BACK>
+static cudaError_t lr_rows_as(LrRowsArgs a, cudaStream_t st) {
+  using L = LrSmem<T, R, M, BACK>;
+  const LrGroups& g = a.groups;
+  const long long slots = g.mode == LR_ONE ? (g.n + M - 1) / M : g.mode == LR_SELF ? g.n : g.n / M + g.adapters + 2;
+  const long long busy = g.mode == LR_ONE ? slots : g.n / M + (g.n < g.adapters ? g.n : g.adapters);
+  const int chunks = (a.k + L::kChunk - 1) / L::kChunk;
+  const int ranks = lr_ranks_for(busy < 1 ? 1 : busy, chunks > 1 ? chunks : 1);
+  int stages = 4;
+  while (stages > 2 && L::bytes(stages) > (R <= 32 ? 72 * 1024 : kLrSmemMost)) --stages;
+  a.stages = stages;
+  if (slots * ranks >= 1ll << 31) return cudaErrorInvalidValue;
+  return lr_launch(lr_rows_kernel<T, R, M, BACK>, (int)slots, ranks, L::bytes(stages), st, a);
+}
+
+template <typename T, int R, bool BACK>
+static cudaError_t lr_rows_r(const LrRowsArgs& a, cudaStream_t st) {
+  const LrGroups& g = a.groups;
+  // Tiles of 64 rows where adapters fill them; 16 rows keep more clusters busy and waste less of the tiles
+  const long long each = g.mode == LR_ONE ? g.n : g.n / (g.adapters > 0 ? g.adapters : 1);
+  if (g.mode != LR_SELF && each >= 48 && g.n >= 1024) return lr_rows_as<T, R, 64, BACK>(a, st);
+  return lr_rows_as<T, R, 16, BACK>(a, st);
+}
+
+template <typename T, int R>
+static cudaError_t lr_outer_r(const LrOuterArgs& a, cudaStream_t st) {
+  using L = LrOuterSmem<T, R>;
+  const long long clusters = (long long)(a.blocks[0] + a.blocks[1]) * a.groups.adapters;
+  const long long steps = (a.groups.n / a.groups.adapters + kLrOuterRows - 1) / kLrOuterRows;
+  const int ranks = lr_ranks_for(clusters / 2, steps > 1 ? steps : 1);          // four blocks an SM: they are short
+  if (clusters * ranks >= 1ll << 31) return cudaErrorInvalidValue;
+  return lr_launch(lr_outer_kernel<T, R>, (int)clusters, ranks, L::bytes(2), st, a);
+}
+
+inline int lr_padded(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+
+// Instances by type, each in a file of its own.
+template <typename T> cudaError_t lr_rows(const LrRowsArgs& a, bool back, cudaStream_t st);
+template <typename T> cudaError_t lr_outer(const LrOuterArgs& a, cudaStream_t st);
+
+template <typename T>
+cudaError_t lr_rows_of(const LrRowsArgs& a, bool back, cudaStream_t st) {
+  switch (lr_padded(a.rank)) {
+    case 16: return back ? lr_rows_r<T, 16, true>(a, st) : lr_rows_r<T, 16, false>(a, st);
+    case 32: return back ? lr_rows_r<T, 32, true>(a, st) : lr_rows_r<T, 32, false>(a, st);
+    case 64: return back ? lr_rows_r<T, 64, true>(a, st) : lr_rows_r<T, 64, false>(a, st);
+    default: return back ? lr_rows_r<T, 128, true>(a, st) : lr_rows_r<T, 128, false>(a, st);
+  }
+}
+template <typename T>
+cudaError_t lr_outer_of(const LrOuterArgs& a, cudaStream_t st) {
+  switch (lr_padded(a.rank)) {
+    case 16: return lr_outer_r<T, 16>(a, st);
+    case 32: return lr_outer_r<T, 32>(a, st);
+    case 64: return lr_outer_r<T, 64>(a, st);
+    default: return lr_outer_r<T, 128>(a, st);
+  }
+}
+
+}  // namespace bonsai

@@ -1,0 +1,477 @@
+// Losses over log-probabilities of tokens, rows of `length` tokens of which a mask says which count:
+//
+//   preference  s_r = sum over the row's tokens of (l - ref) [over their number];  z = s_chosen - s_rejected, rows p and pairs + p;  m = beta z
+//               sigmoid  (1 - e) log(1 + exp(-m)) + e log(1 + exp(m))        hinge  max(0, 1 - m)        ipo  (z - 1 / (2 beta))^2
+//   policy      q = exp(l - old);  each = -min(q g, clip(q, 1 - lo, 1 + hi) g) + w (exp(ref - l) - (ref - l) - 1),  summed or averaged
+//
+// Both are bound by memory when they are large and by launches when they are small.  A block takes a chunk of one row and leaves its sums in
+// f64, one block adds them in one order: no atomics, the same values give the same bits.  The forward pass of the policy loss leaves each token's
+// slope in f32, which the backward pass scales (4 bytes written and read for a token instead of the 13 to 17 that it is made from); the
+// preference loss has one slope for a row.  Whether a ratio is clipped is decided in f64 on l - old, which is exact there, so that a token next to
+// a border falls on the same side whatever exp rounds.  Masked places reach nothing, whatever they hold.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace bonsai {
+
+constexpr int kTuneThreads = 256, kTuneQuads = 2, kTuneFinish = 512;
+
+template <typename T> __device__ __forceinline__ float tune_float(T v);
+template <> __device__ __forceinline__ float tune_float(float v) { return v; }
+template <> __device__ __forceinline__ float tune_float(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float tune_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Four neighbouring tokens from `p` on; WIDE: aligned, so that they are one access.  `n`: how many there are; the others are 0.
+template <bool WIDE>
+__device__ __forceinline__ void tune_load4(const float* p, int n, float* v) {
+  if (WIDE && n >= 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.0f;
+  }
+}
+template <bool WIDE, typename T>
+__device__ __forceinline__ void tune_load4(const T* p, int n, float* v) {
+  if (WIDE && n >= 4) {
+    __align__(8) T t[4];
+    *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = tune_float<T>(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? tune_float<T>(p[i]) : 0.0f;
+  }
+}
+// bit i: token i counts
+template <bool WIDE>
+__device__ __forceinline__ unsigned tune_mask4(const unsigned char* p, int n) {
+  if (p == nullptr) return n >= 4 ? 15u : (1u << n) - 1u;
+  unsigned m = 0;
+  if (WIDE && n >= 4) {
+    const uchar4 u = *reinterpret_cast<const uchar4*>(p);
+    m = (u.x != 0) | (u.y != 0) << 1 | (u.z != 0) << 2 | (u.w != 0) << 3;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m |= (i < n && p[i] != 0 ? 1u : 0u) << i;
+  }
+  return m;
+}
+__device__ __forceinline__ void tune_put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void tune_put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void tune_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <bool WIDE>
+__device__ __forceinline__ void tune_store4(float* p, int n, const float* v) {
+  if (WIDE && n >= 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = v[i];
+  }
+}
+template <bool WIDE, typename T>
+__device__ __forceinline__ void tune_store4(T* p, int n, const float* v) {
+  if (WIDE && n >= 4) {
+    __align__(8) T t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tune_put(&t[i], v[i]);
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) tune_put(p + i, v[i]);
+  }
+}
+
+// Sum over a block of `blockDim.x` threads (whole warps), in thread 0, in one order.
+template <typename S>
+__device__ __forceinline__ S tune_block_sum(S v, S* s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  S t = S(0);
+  if (threadIdx.x == 0)
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += s[i];
+  return t;
+}
+
+struct TuneRows {            // rows of tokens: an address and the distance of rows
+  const void* p;
+  long long ld;
+};
+struct TunePart {            // of one chunk
+  double loss, kl;           // preference: loss is the sum of l - ref
+  int live, clipped;
+};
+struct TuneShape {
+  long long rows;
+  int length, chunks;        // tokens of a row, blocks of a row
+};
+
+// The tokens of this block's chunk of its row, four at a time: body(place, number of tokens there).
+template <typename Body>
+__device__ __forceinline__ void tune_quads(const TuneShape& sh, int chunk, Body body) {
+  const int first = chunk * (int)blockDim.x * 4 * kTuneQuads + (int)threadIdx.x * 4;
+#pragma unroll
+  for (int q = 0; q < kTuneQuads; ++q) {
+    const int at = first + q * (int)blockDim.x * 4;
+    if (at < sh.length) body(at, sh.length - at);
+  }
+}
+
+struct PolicyArgs {
+  TuneShape shape;
+  TuneRows logps, old, ref, mask;       // old, ref and mask may be absent
+  const float* gain;
+  long long gain_ld;
+  int gain_per_token;
+  double log_low, log_high;             // of the borders 1 - lo and 1 + hi
+  float low, high, kl_weight;
+  float* slope;                         // [rows][length], absent where no gradient is wanted
+  float* each;                          // [rows][length], absent where the loss is added up
+  TunePart* part;                       // [rows][chunks]
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kTuneThreads) policy_kernel(PolicyArgs a) {
+  __shared__ double sd[kTuneThreads / 32];
+  __shared__ int si[kTuneThreads / 32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long row = blockIdx.x / a.shape.chunks;
+  const int chunk = (int)(blockIdx.x % a.shape.chunks);
+  const T* logps = (const T*)a.logps.p + row * a.logps.ld;
+  const T* old = a.old.p != nullptr ? (const T*)a.old.p + row * a.old.ld : nullptr;
+  const T* ref = a.ref.p != nullptr ? (const T*)a.ref.p + row * a.ref.ld : nullptr;
+  const unsigned char* mask = a.mask.p != nullptr ? (const unsigned char*)a.mask.p + row * a.mask.ld : nullptr;
+  const float* gain = a.gain + row * a.gain_ld;
+  const float row_gain = a.gain_per_token ? 0.0f : *gain;
+  double loss = 0.0, kls = 0.0;
+  int live = 0, cut = 0;
+  tune_quads(a.shape, chunk, [&](int at, int n) {
+    float l[4], o[4], r[4], g[4] = {row_gain, row_gain, row_gain, row_gain}, e[4], s[4];
+    const unsigned m = tune_mask4<WIDE>(mask == nullptr ? nullptr : mask + at, n);
+    tune_load4<WIDE>(logps + at, n, l);
+    if (old != nullptr) tune_load4<WIDE>(old + at, n, o);
+    if (ref != nullptr) tune_load4<WIDE>(ref + at, n, r);
+    if (a.gain_per_token) tune_load4<WIDE>(gain + at, n, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double step = old != nullptr ? (double)l[i] - (double)o[i] : (double)l[i] - (double)l[i];
+      const bool clipped = (g[i] > 0.0f && step > a.log_high) || (g[i] < 0.0f && step < a.log_low);
+      const float q = expf((float)step);
+      // a gain of 0 leaves 0, also where the ratio is infinite
+      const float gained = g[i] == 0.0f ? 0.0f : q * g[i];
+      float v = clipped ? -(g[i] > 0.0f ? a.high : a.low) * g[i] : -gained, d = clipped ? 0.0f : -gained, kl = 0.0f;
+      if (ref != nullptr) {
+        const float back = r[i] - l[i], grown = expm1f(back);
+        kl = grown - back;
+        if (a.kl_weight != 0.0f) {
+          v = fmaf(a.kl_weight, kl, v);
+          d = fmaf(-a.kl_weight, grown, d);
+        }
+      }
+      const bool on = m >> i & 1u;
+      e[i] = on ? v : 0.0f;
+      s[i] = on ? d : 0.0f;
+      loss += (double)e[i];
+      kls += on ? (double)kl : 0.0;
+      live += on;
+      cut += on && clipped;
+    }
+    if (a.slope != nullptr) tune_store4<WIDE>(a.slope + row * a.shape.length + at, n, s);
+    if (a.each != nullptr) tune_store4<WIDE>(a.each + row * a.shape.length + at, n, e);
+  });
+  loss = tune_block_sum(loss, sd);
+  kls = tune_block_sum(kls, sd);
+  live = tune_block_sum(live, si);
+  cut = tune_block_sum(cut, si);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = {loss, kls, live, cut};
+}
+
+enum TuneReduction { TUNE_TOKENS = 0, TUNE_SEQUENCES = 1, TUNE_SUM = 2, TUNE_NONE = 3 };
+
+// Adds the chunks up; weight[row] is what a token's loss counts in the whole.  One block.
+__global__ void __launch_bounds__(kTuneFinish) policy_finish_kernel(TuneShape sh, const TunePart* part, int reduction, float* loss, float* kl, float* clipped,
+                                                                    float* weight) {
+  __shared__ double sd[kTuneFinish / 32];
+  __shared__ long long sl[kTuneFinish / 32];
+  __shared__ long long counts[2];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  double sum = 0.0, kls = 0.0, means = 0.0;
+  long long live = 0, cut = 0, filled = 0;
+  for (long long row = threadIdx.x; row < sh.rows; row += kTuneFinish) {
+    double s = 0.0;
+    long long n = 0;
+    for (int c = 0; c < sh.chunks; ++c) {
+      const TunePart p = part[row * sh.chunks + c];
+      s += p.loss;
+      kls += p.kl;
+      n += p.live;
+      cut += p.clipped;
+    }
+    sum += s;
+    live += n;
+    filled += n > 0;
+    means += n > 0 ? s / (double)n : 0.0;
+  }
+  sum = tune_block_sum(sum, sd);
+  kls = tune_block_sum(kls, sd);
+  means = tune_block_sum(means, sd);
+  live = tune_block_sum(live, sl);
+  cut = tune_block_sum(cut, sl);
+  filled = tune_block_sum(filled, sl);
+  if (threadIdx.x == 0) {
+    const double n = (double)live;              // 0 / 0 is NaN: the mean of no tokens
+    if (loss != nullptr) *loss = (float)(reduction == TUNE_TOKENS ? sum / n : reduction == TUNE_SEQUENCES ? means / (double)filled : sum);
+    *kl = (float)(kls / n);
+    *clipped = (float)((double)cut / n);
+    counts[0] = live;
+    counts[1] = filled;
+  }
+  if (weight == nullptr) return;
+  __syncthreads();
+  for (long long row = threadIdx.x; row < sh.rows; row += kTuneFinish) {
+    long long n = 1;
+    if (reduction == TUNE_TOKENS) {
+      n = counts[0];
+    } else if (reduction == TUNE_SEQUENCES) {
+      n = 0;
+      for (int c = 0; c < sh.chunks; ++c) n += part[row * sh.chunks + c].live;
+      n *= counts[1];
+    }
+    weight[row] = n > 0 ? (float)(1.0 / (double)n) : 0.0f;
+  }
+}
+
+struct ScaleArgs {
+  TuneShape shape;
+  const float* slope;        // [rows][length], or one for a row
+  int slope_per_token;
+  const float* weight;       // for a row, absent: 1
+  const float* up;           // one, one for every `up_rows`-th row, or [rows][length]
+  int up_kind;               // 0, 1, 2
+  long long up_rows;
+  TuneRows mask;
+};
+
+// The gradient of the log-probabilities: slope * weight * the loss's gradient where the mask is set, else 0.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kTuneThreads) tune_scale_kernel(ScaleArgs a, T* __restrict__ out) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long row = blockIdx.x / a.shape.chunks, base = row * a.shape.length;
+  const int chunk = (int)(blockIdx.x % a.shape.chunks);
+  const unsigned char* mask = a.mask.p != nullptr ? (const unsigned char*)a.mask.p + row * a.mask.ld : nullptr;
+  float by = a.weight != nullptr ? a.weight[row] : 1.0f;
+  if (a.up_kind < 2) by *= a.up[a.up_kind == 0 ? 0 : row % a.up_rows];
+  if (!a.slope_per_token) by *= a.slope[row];
+  tune_quads(a.shape, chunk, [&](int at, int n) {
+    float s[4] = {1.0f, 1.0f, 1.0f, 1.0f}, u[4] = {1.0f, 1.0f, 1.0f, 1.0f}, g[4];
+    const unsigned m = tune_mask4<WIDE>(mask == nullptr ? nullptr : mask + at, n);
+    if (a.slope_per_token) tune_load4<WIDE>(a.slope + base + at, n, s);
+    if (a.up_kind == 2) tune_load4<WIDE>(a.up + base + at, n, u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = (m >> i & 1u) && s[i] != 0.0f ? s[i] * by * u[i] : 0.0f;        // masked tokens have slopes of 0
+    tune_store4<WIDE>(out + base + at, n, g);
+  });
+}
+
+struct PreferenceArgs {
+  TuneShape shape;           // 2 * pairs rows: the chosen ones, then the rejected ones
+  TuneRows logps, ref, mask;
+  TunePart* part;
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kTuneThreads) preference_kernel(PreferenceArgs a) {
+  __shared__ double sd[kTuneThreads / 32];
+  __shared__ int si[kTuneThreads / 32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long row = blockIdx.x / a.shape.chunks;
+  const int chunk = (int)(blockIdx.x % a.shape.chunks);
+  const T* logps = (const T*)a.logps.p + row * a.logps.ld;
+  const T* ref = a.ref.p != nullptr ? (const T*)a.ref.p + row * a.ref.ld : nullptr;
+  const unsigned char* mask = a.mask.p != nullptr ? (const unsigned char*)a.mask.p + row * a.mask.ld : nullptr;
+  double sum = 0.0;
+  int live = 0;
+  tune_quads(a.shape, chunk, [&](int at, int n) {
+    float l[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const unsigned m = tune_mask4<WIDE>(mask == nullptr ? nullptr : mask + at, n);
+    tune_load4<WIDE>(logps + at, n, l);
+    if (ref != nullptr) tune_load4<WIDE>(ref + at, n, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool on = m >> i & 1u;
+      sum += on ? (double)(l[i] - r[i]) : 0.0;
+      live += on;
+    }
+  });
+  sum = tune_block_sum(sum, sd);
+  live = tune_block_sum(live, si);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = {sum, 0.0, live, 0};
+}
+
+enum PreferenceKind { PREF_SIGMOID = 0, PREF_HINGE = 1, PREF_IPO = 2 };
+struct PreferenceRule {
+  int kind, average, reduction;      // reduction: 0 mean, 1 sum, 2 none
+  double beta, smoothing;
+};
+
+// Of one row: the sum over its chunks, and what a token counts in it (1, or one over their number).
+__device__ __forceinline__ double preference_row(const TunePart* part, int chunks, int average, double* token) {
+  double s = 0.0;
+  long long n = 0;
+  for (int c = 0; c < chunks; ++c) { s += part[c].loss; n += part[c].live; }
+  *token = average ? (n > 0 ? 1.0 / (double)n : 0.0) : 1.0;
+  return n > 0 ? s * *token : 0.0;
+}
+
+__global__ void __launch_bounds__(kTuneFinish) preference_finish_kernel(long long pairs, int chunks, const TunePart* part, PreferenceRule rule, float* loss,
+                                                                        float* chosen, float* rejected, float* slope) {
+  __shared__ double sd[kTuneFinish / 32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  double sum = 0.0;
+  for (long long p = threadIdx.x; p < pairs; p += kTuneFinish) {
+    double tc, tr;
+    const double sc = preference_row(part + p * chunks, chunks, rule.average, &tc), sr = preference_row(part + (pairs + p) * chunks, chunks, rule.average, &tr);
+    const double z = sc - sr, m = rule.beta * z;
+    double v, d;                                  // the pair's loss and its derivative by z
+    if (rule.kind == PREF_SIGMOID) {
+      const double fall = exp(-fabs(m)), soft = log1p(fall), on = (m < 0.0 ? fall : 1.0) / (1.0 + fall);        // on = 1 / (1 + exp(-m))
+      const double off = (m < 0.0 ? 1.0 : fall) / (1.0 + fall);
+      const double minus = soft + fmax(-m, 0.0), plus = soft + fmax(m, 0.0);     // log(1 + exp(-m)), log(1 + exp(m))
+      v = m != m ? m : rule.smoothing == 0.0 ? minus : (1.0 - rule.smoothing) * minus + rule.smoothing * plus;
+      d = rule.beta * (rule.smoothing * on - (1.0 - rule.smoothing) * off);
+    } else if (rule.kind == PREF_HINGE) {
+      v = m < 1.0 ? 1.0 - m : m != m ? m : 0.0;
+      d = m < 1.0 ? -rule.beta : m != m ? m : 0.0;
+    } else {
+      const double t = z - 0.5 / rule.beta;
+      v = t * t;
+      d = 2.0 * t;
+    }
+    if (rule.reduction == 2) loss[p] = (float)v;
+    sum += v;
+    chosen[p] = (float)(rule.beta * sc);
+    rejected[p] = (float)(rule.beta * sr);
+    if (slope != nullptr) {
+      if (rule.reduction == 0) d /= (double)pairs;
+      slope[p] = (float)(d * tc);
+      slope[pairs + p] = (float)(-d * tr);
+    }
+  }
+  sum = tune_block_sum(sum, sd);
+  if (threadIdx.x == 0 && rule.reduction != 2) *loss = (float)(rule.reduction == 0 ? sum / (double)pairs : sum);
+}
+
+// Threads of a block: rows that fit a few warps take no more.
+static int tune_threads(long long length) { return length <= 128 ? 32 : length <= 256 ? 64 : length <= 512 ? 128 : kTuneThreads; }
+static int tune_chunks(long long length) {
+  const int tokens = tune_threads(length) * 4 * kTuneQuads;
+  return (int)((length + tokens - 1) / tokens);
+}
+static bool tune_good(long long rows, long long length) {
+  return rows >= 1 && length >= 1 && length < 1ll << 30 && rows < 1ll << 31 && rows * tune_chunks(length) < 1ll << 31;
+}
+static TuneShape tune_shape(long long rows, long long length) { return {rows, (int)length, tune_chunks(length)}; }
+
+// Whether four neighbouring tokens of every row are one aligned access; an absent array does not matter.
+static bool tune_wide(const void* p, long long ld, int size) { return p == nullptr || (((uintptr_t)p | (uintptr_t)(ld * size)) % (4 * size) == 0); }
+
+
+}  // namespace bonsai
+
+extern "C" {
+
+// Bytes of workspace that both losses need for rows of `length` tokens; negative for sizes that are refused.
+long long bonsai_tune_bytes(long long rows, long long length) {
+  using namespace bonsai;
+  return tune_good(rows, length) ? rows * tune_chunks(length) * (long long)sizeof(TunePart) : BONSAI_CUDA_BAD_ARG;
+}
+
+// logps, old, ref: rows of tokens at distances of their ld (type 0 f32, 1 f16, 2 bf16), mask: bytes; old, ref and mask may be null.  gain: f32, for a
+// row or for a token.  reduction: TuneReduction.  Out: loss (f32, or [rows][length]), kl, clipped (f32), and where a gradient is wanted slope
+// [rows][length] and weight [rows].
+int bonsai_policy_loss(const void* logps, long long ld_logps, const void* old, long long ld_old, const void* ref, long long ld_ref, const void* mask,
+                       long long ld_mask, const float* gain, long long ld_gain, int gain_per_token, long long rows, long long length, int type, double low,
+                       double high, double kl_weight, int reduction, float* loss, float* kl, float* clipped, float* slope, float* weight, void* ws,
+                       long long ws_bytes, cudaStream_t st) {
+  using namespace bonsai;
+  if (logps == nullptr || gain == nullptr || loss == nullptr || kl == nullptr || clipped == nullptr || ws == nullptr || !tune_good(rows, length) || type < 0 ||
+      type > 2 || reduction < 0 || reduction > 3 || (slope == nullptr) != (weight == nullptr) || ws_bytes < bonsai_tune_bytes(rows, length) || !(low >= 0.0) ||
+      !(low <= 1.0) || !(high >= 0.0))
+    return BONSAI_CUDA_BAD_ARG;
+  const TuneShape sh = tune_shape(rows, length);
+  const int size = type == 0 ? 4 : 2, threads = tune_threads(length);
+  PolicyArgs a = {sh, {logps, ld_logps}, {old, ld_old}, {ref, ld_ref}, {mask, ld_mask}, gain, ld_gain, gain_per_token, log1p(-low), log1p(high),
+                  (float)(1.0 - low), (float)(1.0 + high), (float)kl_weight, slope, reduction == TUNE_NONE ? loss : nullptr, (TunePart*)ws};
+  const bool wide = length % 4 == 0 && tune_wide(logps, ld_logps, size) && tune_wide(old, ld_old, size) && tune_wide(ref, ld_ref, size) &&
+                    tune_wide(mask, ld_mask, 1) && (!gain_per_token || tune_wide(gain, ld_gain, 4)) && tune_wide(slope, length, 4) &&
+                    tune_wide(a.each, length, 4);
+  const dim3 grid((unsigned)(rows * sh.chunks)), block(threads);
+  cudaError_t e;
+  if (type == 0) e = wide ? launch_pdl(policy_kernel<float, true>, grid, block, 0, st, a) : launch_pdl(policy_kernel<float, false>, grid, block, 0, st, a);
+  else if (type == 1) e = wide ? launch_pdl(policy_kernel<__half, true>, grid, block, 0, st, a) : launch_pdl(policy_kernel<__half, false>, grid, block, 0, st, a);
+  else e = wide ? launch_pdl(policy_kernel<__nv_bfloat16, true>, grid, block, 0, st, a) : launch_pdl(policy_kernel<__nv_bfloat16, false>, grid, block, 0, st, a);
+  if (e == cudaSuccess)
+    e = launch_pdl(policy_finish_kernel, dim3(1), dim3(kTuneFinish), 0, st, sh, (const TunePart*)ws, reduction, reduction == TUNE_NONE ? (float*)nullptr : loss,
+                   kl, clipped, weight);
+  return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
+}
+
+// Rows 0 .. pairs - 1 are the chosen answers, the next `pairs` the rejected ones; ref and mask may be null.  kind: PreferenceKind; reduction 0 mean, 1 sum,
+// 2 none.  Out: loss (f32, or [pairs]), rewards [pairs], and where a gradient is wanted slope [2 * pairs].
+int bonsai_preference_loss(const void* logps, long long ld_logps, const void* ref, long long ld_ref, const void* mask, long long ld_mask, long long pairs,
+                           long long length, int type, int kind, int average, int reduction, double beta, double smoothing, float* loss, float* chosen,
+                           float* rejected, float* slope, void* ws, long long ws_bytes, cudaStream_t st) {
+  using namespace bonsai;
+  if (logps == nullptr || loss == nullptr || chosen == nullptr || rejected == nullptr || ws == nullptr || pairs < 1 || !tune_good(2 * pairs, length) ||
+      type < 0 || type > 2 || kind < 0 || kind > 2 || reduction < 0 || reduction > 2 || ws_bytes < bonsai_tune_bytes(2 * pairs, length) || !(beta > 0.0))
+    return BONSAI_CUDA_BAD_ARG;
+  const TuneShape sh = tune_shape(2 * pairs, length);
+  const int size = type == 0 ? 4 : 2, threads = tune_threads(length);
+  const PreferenceArgs a = {sh, {logps, ld_logps}, {ref, ld_ref}, {mask, ld_mask}, (TunePart*)ws};
+  const bool wide = length % 4 == 0 && tune_wide(logps, ld_logps, size) && tune_wide(ref, ld_ref, size) && tune_wide(mask, ld_mask, 1);
+  const dim3 grid((unsigned)(sh.rows * sh.chunks)), block(threads);
+  cudaError_t e;
+  if (type == 0) e = wide ? launch_pdl(preference_kernel<float, true>, grid, block, 0, st, a) : launch_pdl(preference_kernel<float, false>, grid, block, 0, st, a);
+  else if (type == 1) e = wide ? launch_pdl(preference_kernel<__half, true>, grid, block, 0, st, a) : launch_pdl(preference_kernel<__half, false>, grid, block, 0, st, a);
+  else
+    e = wide ? launch_pdl(preference_kernel<__nv_bfloat16, true>, grid, block, 0, st, a) : launch_pdl(preference_kernel<__nv_bfloat16, false>, grid, block, 0, st, a);
+  if (e == cudaSuccess)
+    e = launch_pdl(preference_finish_kernel, dim3(1), dim3(kTuneFinish), 0, st, pairs, sh.chunks, (const TunePart*)ws, PreferenceRule{kind, average, reduction, beta, smoothing},
+                   loss, chosen, rejected, slope);
+  return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
+}
+
+// out [rows][length] = slope * weight * up where the mask (may be null) is set.  slope: f32, for a token or for a row; weight: for a row, may be null;
+// up: one value (up_kind 0), that of row % up_rows (1), or one for a token (2).
+int bonsai_tune_scale(const float* slope, int slope_per_token, const float* weight, const float* up, int up_kind, long long up_rows, const void* mask,
+                      long long ld_mask, long long rows, long long length, int type, void* out, cudaStream_t st) {
+  using namespace bonsai;
+  if (slope == nullptr || up == nullptr || out == nullptr || !tune_good(rows, length) || type < 0 || type > 2 || up_kind < 0 || up_kind > 2 || up_rows < 1)
+    return BONSAI_CUDA_BAD_ARG;
+  const TuneShape sh = tune_shape(rows, length);
+  const int size = type == 0 ? 4 : 2;
+  const ScaleArgs a = {sh, slope, slope_per_token, weight, up, up_kind, up_rows, {mask, ld_mask}};
+  const bool wide = length % 4 == 0 && (!slope_per_token || tune_wide(slope, length, 4)) && (up_kind < 2 || tune_wide(up, length, 4)) &&
+                    tune_wide(mask, ld_mask, 1) && tune_wide(out, length, size);
+  const dim3 grid((unsigned)(rows * sh.chunks)), block(tune_threads(length));
+  cudaError_t e;
+  if (type == 0) e = wide ? launch_pdl(tune_scale_kernel<float, true>, grid, block, 0, st, a, (float*)out) : launch_pdl(tune_scale_kernel<float, false>, grid, block, 0, st, a, (float*)out);
+  else if (type == 1) e = wide ? launch_pdl(tune_scale_kernel<__half, true>, grid, block, 0, st, a, (__half*)out) : launch_pdl(tune_scale_kernel<__half, false>, grid, block, 0, st, a, (__half*)out);
+  else e = wide ? launch_pdl(tune_scale_kernel<__nv_bfloat16, true>, grid, block, 0, st, a, (__nv_bfloat16*)out) : launch_pdl(tune_scale_kernel<__nv_bfloat16, false>, grid, block, 0, st, a, (__nv_bfloat16*)out);
+  return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
+}
+
+}  // extern "C"

@@ -1,4 +1,5 @@
-"""Torch-facing wrappers of the training kernels in ``libbonsai_cuda.so`` (csrc/cuda/multi_tensor.cu, linear_ce.cu).
+"""Torch-facing wrappers of the training kernels in ``libbonsai_cuda.so`` (csrc/cuda/multi_tensor.cu, linear_ce.cu, dropout.cu,
+low_rank.cu, tuning_loss.cu).
 
 Every function launches on torch's current stream of the tensors' device.  As in :mod:`cuda_ops` there is no PyTorch fallback:
 CUDA tensors go through the kernels, and a missing library raises.
@@ -14,7 +15,7 @@ import torch
 
 from . import cuda_ops as K
 
-_vp, _i, _d, _ll = C.c_void_p, C.c_int, C.c_double, C.c_longlong
+_vp, _i, _d, _ll, _u64, _f = C.c_void_p, C.c_int, C.c_double, C.c_longlong, C.c_uint64, C.c_float
 _SIG = {
     "bonsai_mt_partials": [_i],
     "bonsai_mt_norm": [_i, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -23,6 +24,16 @@ _SIG = {
     "bonsai_ce_forward": [_vp, _ll, _vp, _ll, _vp, _i, _i, _i, _i, _ll, _i, C.c_float, _vp, _ll, _vp, _vp, _ll, _vp],
     "bonsai_ce_backward": [_vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp],
     "bonsai_mt_adam": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _d, _vp, _d, _d, _d, _d, _i, _vp, _d, _vp, _vp, _vp],
+    "bonsai_dropout": [_vp, _ll, _vp, _ll, _ll, _i, _u64, _vp, _i, _vp],
+    "bonsai_lr_padded": [_i],
+    "bonsai_lr_self_rows": [],
+    "bonsai_lr_plan": [_vp, _i, _i, _i, _vp, _vp, _vp],
+    "bonsai_lr_rows": [_vp, _ll, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _u64, _vp, _i, _vp],
+    "bonsai_lr_outer": [_vp, _ll, _vp, _vp, _i, _vp, _ll, _vp, _vp, _i, _vp, _f, _i, _i, _i, _i, _i, _vp, _vp, _u64, _vp, _i, _vp],
+    "bonsai_tune_bytes": [_ll, _ll],
+    "bonsai_policy_loss": [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _i, _ll, _ll, _i, _d, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_preference_loss": [_vp, _ll, _vp, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _i, _d, _d, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "bonsai_tune_scale": [_vp, _i, _vp, _vp, _i, _ll, _vp, _ll, _ll, _ll, _i, _vp, _vp],
 }
 _declared = False
 _HERE = contextlib.nullcontext()
@@ -33,7 +44,7 @@ def _lib():
     global _declared
     l = K.lib()
     if not _declared:
-        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_bytes": _ll})
+        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_bytes": _ll, "bonsai_tune_bytes": _ll})
         _declared = True
     return l
 
@@ -155,3 +166,132 @@ def linear_ce_backward(weight: torch.Tensor, kept: torch.Tensor, n: int, up: tor
                                           kept.data_ptr(), kept.numel(), up.data_ptr(), K.ptr(dh), K.ptr(dw), ws.data_ptr(), ws.numel(),
                                           _stream(device)), "linear_ce_backward")
     return dh, dw
+
+
+# ---- dropout ---------------------------------------------------------------------------------------------------------------------------
+Seed = int | torch.Tensor          # a tensor (int64, on the device) is read when the kernel runs
+
+
+def _seed(seed: Seed) -> tuple[int, int | None]:
+    return (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
+
+
+def dropout(x: torch.Tensor, steps: int, seed: Seed) -> torch.Tensor:
+    """Rows x [n, d] (unit stride along d): each value stays, over steps / 65536, where its 16 random bits are below ``steps``."""
+    with _on(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        K.check(_lib().bonsai_dropout(x.data_ptr(), _ld(x), y.data_ptr(), *x.shape, TYPE_CODES[x.dtype], *_seed(seed), steps, _stream(x.device)), "dropout")
+    return y
+
+
+# ---- low-rank updates --------------------------------------------------------------------------------------------------------------------
+class RowGroups:
+    """Which rows have which adapter, as the kernels take it.  ``ids`` None: one adapter; ``planned``: the order of rows by adapter is made
+    (backward passes need it; more rows than a block groups by itself have it in any case)."""
+
+    def __init__(self, ids: torch.Tensor | None, n: int, adapters: int, planned: bool):
+        self.ids, self.n, self.adapters = ids, n, adapters
+        self.order = self.start = None
+        self.mode = 0 if ids is None else 1
+        if ids is not None and (planned or n > _lib().bonsai_lr_self_rows()):
+            self.mode = 2
+            with _on(ids.device):
+                self.order = torch.empty(n, dtype=torch.int32, device=ids.device)
+                self.start = torch.empty(adapters + 3, dtype=torch.int32, device=ids.device)
+                K.check(_lib().bonsai_lr_plan(ids.data_ptr(), ids.dtype == torch.int64, n, adapters, self.order.data_ptr(), self.start.data_ptr(),
+                                              _stream(ids.device)), "low_rank_plan")
+
+
+def _scale(scale: float | torch.Tensor) -> tuple[int | None, float]:
+    return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
+
+
+def low_rank_rows(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, groups: RowGroups, back: bool, scale: float | torch.Tensor, steps: int, seed: Seed,
+                  base: torch.Tensor | None = None, out: torch.Tensor | None = None, keep: bool = False,
+                  only_kept: bool = False) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """x [n, k] -> (y [n, cols], the rank values by place or None): ``base + scale w2 (w1 x)`` with w1 [e, r, k] and w2 [e, cols, r], or, ``back``,
+    ``scale w2^T (w1^T x)`` with w1 [e, k, r] and w2 [e, r, cols].  Unit strides along rows, w1 and w2 dense.  ``steps`` of 65536 values stay: of x, or
+    of the result where ``back``."""
+    n, k = x.shape
+    rank, cols = (w1.shape[2], w2.shape[2]) if back else (w1.shape[1], w2.shape[1])
+    device = x.device
+    with _on(device):
+        y = None if only_kept else torch.empty((n, cols), dtype=x.dtype, device=device) if out is None else out
+        kept = torch.empty((n, _lib().bonsai_lr_padded(rank)), dtype=torch.float32, device=device) if keep else None
+        K.check(_lib().bonsai_lr_rows(x.data_ptr(), _ld(x), w1.data_ptr(), w2.data_ptr(), K.ptr(base), 0 if base is None else _ld(base), K.ptr(y),
+                                      0 if y is None else _ld(y), K.ptr(kept), *_scale(scale), n, k, cols, rank, groups.adapters, TYPE_CODES[x.dtype],
+                                      int(back), groups.mode, K.ptr(groups.ids), groups.ids is not None and groups.ids.dtype == torch.int64,
+                                      K.ptr(groups.order), K.ptr(groups.start), *_seed(seed), steps, _stream(device)), "low_rank_rows")
+    return y, kept
+
+
+def low_rank_outer(x: torch.Tensor | None, g: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor | None, d: int, rank: int, groups: RowGroups,
+                   scale: float | torch.Tensor, steps: int, seed: Seed) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Sums over each adapter's rows: (da [e, r, d] from x and g, db [e, out, r] from dy and h); what has no rank values is left out."""
+    n, out = dy.shape
+    device, e = dy.device, groups.adapters
+    with _on(device):
+        da = None if g is None else torch.empty((e, rank, d), dtype=dy.dtype, device=device)
+        db = None if h is None else torch.empty((e, out, rank), dtype=dy.dtype, device=device)
+        K.check(_lib().bonsai_lr_outer(K.ptr(x), 0 if x is None else _ld(x), K.ptr(g), K.ptr(da), d, dy.data_ptr(), _ld(dy), K.ptr(h), K.ptr(db), out,
+                                       *_scale(scale), n, rank, e, TYPE_CODES[dy.dtype], groups.mode, K.ptr(groups.order), K.ptr(groups.start),
+                                       *_seed(seed), steps, _stream(device)), "low_rank_outer")
+    return da, db
+
+
+# ---- losses over log-probabilities ---------------------------------------------------------------------------------------------------------
+POLICY_REDUCTIONS = {"tokens": 0, "sequences": 1, "sum": 2, "none": 3}
+PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+
+
+def _tune_room(rows: int, length: int, device: torch.device) -> torch.Tensor:
+    size = int(_lib().bonsai_tune_bytes(rows, length))
+    K.check(min(0, size), "tune_bytes")
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _rows(t: torch.Tensor | None) -> tuple[int | None, int]:
+    return (None, 0) if t is None else (t.data_ptr(), _ld(t))
+
+
+def policy_forward(logps, old, ref, mask, gain, clip: tuple[float, float], kl_weight: float, reduction: str, keep: bool) -> tuple:
+    """Rows [n, t] (unit stride along t), gain f32 [n] or [n, t] -> (loss, kl, clipped share, slopes [n, t] or None, weights [n] or None)."""
+    n, t = logps.shape
+    device = logps.device
+    with _on(device):
+        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
+        loss, kl, clipped = new(n, t) if reduction == "none" else new(), new(), new()
+        slope, weight = (new(n, t), new(n)) if keep else (None, None)
+        ws = _tune_room(n, t, device)
+        K.check(_lib().bonsai_policy_loss(*_rows(logps), *_rows(old), *_rows(ref), *_rows(mask), gain.data_ptr(), _ld(gain) if gain.dim() == 2 else gain.stride(0),
+                                          int(gain.dim() == 2), n, t, TYPE_CODES[logps.dtype], *clip, kl_weight, POLICY_REDUCTIONS[reduction], loss.data_ptr(),
+                                          kl.data_ptr(), clipped.data_ptr(), K.ptr(slope), K.ptr(weight), ws.data_ptr(), ws.numel(), _stream(device)), "policy_loss")
+    return loss, kl, clipped, slope, weight
+
+
+def preference_forward(logps, ref, mask, beta: float, kind: str, smoothing: float, average: bool, reduction: str, keep: bool) -> tuple:
+    """Rows [2 pairs, t] -> (loss, rewards of the chosen and of the rejected rows, slopes [2 pairs] or None)."""
+    n, t = logps.shape
+    device = logps.device
+    with _on(device):
+        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
+        loss, chosen, rejected = new(n // 2) if reduction == "none" else new(), new(n // 2), new(n // 2)
+        slope = new(n) if keep else None
+        ws = _tune_room(n, t, device)
+        K.check(_lib().bonsai_preference_loss(*_rows(logps), *_rows(ref), *_rows(mask), n // 2, t, TYPE_CODES[logps.dtype], PREFERENCE_KINDS[kind], int(average),
+                                              REDUCTIONS[reduction], beta, smoothing, loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), K.ptr(slope),
+                                              ws.data_ptr(), ws.numel(), _stream(device)), "preference_loss")
+    return loss, chosen, rejected, slope
+
+
+def tune_scale(slope: torch.Tensor, weight: torch.Tensor | None, up: torch.Tensor, mask: torch.Tensor | None, shape: tuple[int, int],
+               dtype: torch.dtype) -> torch.Tensor:
+    """Gradient [n, t] from slopes ([n, t] or [n]), weights of rows and the loss's gradient (0-dim, [n, t], or one for every row modulo its length)."""
+    n, t = shape
+    device = slope.device
+    with _on(device):
+        out = torch.empty((n, t), dtype=dtype, device=device)
+        kind = 0 if up.dim() == 0 else 2 if up.dim() == 2 else 1
+        K.check(_lib().bonsai_tune_scale(slope.data_ptr(), int(slope.dim() == 2), K.ptr(weight), up.data_ptr(), kind, max(1, up.numel()) if kind == 1 else 1,
+                                         *_rows(mask), n, t, TYPE_CODES[dtype], out.data_ptr(), _stream(device)), "tune_scale")
+    return out

@@ -9,7 +9,9 @@ with momentum / Nesterov, Adam, AdamW, ``clip_grad_norm``, constant / warm-up / 
 ``Tensor`` with backward rules), losses.rs (cross-entropy, label smoothing, focal, KL, distillation, MSE, Huber,
 contrastive, next-token loss) and gradient_checkpoint.rs (segments that keep only their input and recompute on demand).
 Everything is written over torch tensors so it runs on the GPU next to the inference engine.  ``linear_loss`` (the loss of a head
-without its logits) and ``multi_tensor`` (norm, clipping and Adam over all tensors at once) run kernels of their own there.
+without its logits), ``multi_tensor`` (norm, clipping and Adam over all tensors at once), ``low_rank`` (the updates of one or many
+adapters in one kernel), ``counter_dropout`` (dropout without a stored mask) and ``tuning_loss`` (preference pairs, clipped policy
+ratios) run kernels of their own there.
 """
 from __future__ import annotations
 
@@ -20,8 +22,11 @@ from typing import Callable, Iterable, Sequence
 import torch
 import torch.nn.functional as F
 
+from .counter_dropout import dropout  # noqa: F401
 from .linear_loss import linear_cross_entropy, linear_ntp_loss, linear_sequence_perplexity  # noqa: F401
+from .low_rank import AdapterBank, low_rank_update  # noqa: F401
 from .multi_tensor import FusedAdam, FusedAdamW, GradientSet, clip_global_norm, global_grad_norm  # noqa: F401
+from .tuning_loss import PolicyLoss, PreferenceLoss, policy_loss, preference_loss  # noqa: F401
 
 
 # ---- LoRA -------------------------------------------------------------------------------------------------------------------
@@ -31,6 +36,7 @@ class LoraConfig:
     alpha: float = 16.0
     dropout: float = 0.0
     target_modules: tuple[str, ...] = ("attn_q", "attn_v")
+    fused: bool = False           # the update, its dropout and the addition to the projection's result in one kernel (low_rank_update)
 
     @property
     def scale(self) -> float:
@@ -47,13 +53,18 @@ class LoraAdapter(torch.nn.Module):
         self.A = torch.nn.Parameter(torch.randn(config.rank, in_features, generator=g) / math.sqrt(config.rank))
         self.B = torch.nn.Parameter(torch.zeros(out_features, config.rank))
 
+    def _fused(self, x: torch.Tensor, base_out: torch.Tensor | None) -> torch.Tensor:
+        return low_rank_update(x, self.A, self.B, base=base_out, scale=self.config.scale, dropout=self.config.dropout if self.training else 0.0)
+
     def apply_delta(self, x: torch.Tensor) -> torch.Tensor:
+        if self.config.fused:
+            return self._fused(x, None)
         if self.training and self.config.dropout > 0:
             x = F.dropout(x, self.config.dropout)
         return (x @ self.A.T) @ self.B.T * self.config.scale
 
     def forward(self, x: torch.Tensor, base_out: torch.Tensor) -> torch.Tensor:
-        return base_out + self.apply_delta(x)
+        return self._fused(x, base_out) if self.config.fused else base_out + self.apply_delta(x)
 
     def param_count(self) -> int:
         return self.A.numel() + self.B.numel()

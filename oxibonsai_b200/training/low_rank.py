@@ -1,0 +1,246 @@
+"""Low-rank updates of one or many adapters beside a shared projection, with their gradients.
+
+``LoraAdapter`` applies one adapter to all rows in two matrix products, which write the rank values to memory and the update once more than it
+is needed.  Here the rows of a batch name their adapters, and one kernel makes the whole update: for serving many requests whose
+adapters differ beside one packed projection, and for training one or several adapters, with dropout on the way in.  CUDA tensors
+run csrc/cuda/low_rank.cu, CPU tensors the same steps in torch.
+
+Reference: crates/oxibonsai-model/src/lora.rs (``LoraAdapter::apply`` = ``(alpha / r) * B(A x)``, one adapter for all rows).
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.graph import increment_version
+
+from ..ops import train_ops
+from .counter_dropout import check_p, check_seed, keep_steps, kept, rows_of
+
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+MAX_RANK = 128
+
+
+def _cpu_parts(x, a, ids, scale, steps, seed):
+    """What both passes on the CPU need: the type of the sums, rows as they enter the adapters, a row's scale, its adapter's rows."""
+    kind = torch.float64 if x.dtype == torch.float64 else torch.float32
+    keep = kept(*x.shape, steps, seed) if steps < 65536 else None
+    share = 1.0 if keep is None else 65536.0 / steps if steps else 0.0
+    scales = scale.to(kind) if isinstance(scale, torch.Tensor) else torch.full((len(a),), scale, dtype=kind)
+    rows = [torch.arange(len(x))] if ids is None else [(ids == e).nonzero().flatten() for e in range(len(a))]
+    return kind, keep, share, scales, rows
+
+
+def _cpu_forward(x, a, b, base, ids, scale, steps, seed):
+    kind, keep, share, scales, rows = _cpu_parts(x, a, ids, scale, steps, seed)
+    xs = x.to(kind) if keep is None else torch.where(keep, x.to(kind) * share, 0.0)
+    y = torch.zeros(len(x), b.shape[1], dtype=kind) if base is None else base.to(kind).clone()
+    for e, at in enumerate(rows):
+        if len(at):
+            y[at] += (xs[at] @ a[e].to(kind).T) @ b[e].to(kind).T * scales[e]
+    return y.to(x.dtype)
+
+
+def _cpu_backward(x, a, b, ids, scale, steps, seed, up):
+    kind, keep, share, scales, rows = _cpu_parts(x, a, ids, scale, steps, seed)
+    xs = x.to(kind) if keep is None else torch.where(keep, x.to(kind) * share, 0.0)
+    dx, da, db = torch.zeros_like(xs), torch.zeros(a.shape, dtype=kind), torch.zeros(b.shape, dtype=kind)
+    for e, at in enumerate(rows):
+        if len(at):
+            u, ae, be = up[at].to(kind) * scales[e], a[e].to(kind), b[e].to(kind)
+            g = u @ be
+            dx[at], da[e], db[e] = g @ ae, g.T @ xs[at], u.T @ (xs[at] @ ae.T)
+    if keep is not None:
+        dx = torch.where(keep, dx * share, 0.0)
+    return dx.to(x.dtype), da.to(a.dtype), db.to(b.dtype)
+
+
+class _LowRankUpdate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, a, b, base, ids, scale, steps, seed):
+        ctx.scale, ctx.steps, ctx.seed = (None if isinstance(v, torch.Tensor) else v for v in (scale, steps, seed))
+        held = [v for v in (scale, seed) if isinstance(v, torch.Tensor)]
+        if not x.is_cuda:
+            ctx.save_for_backward(x, a, b, ids, *held)
+            return _cpu_forward(x, a, b, base, ids, scale, steps, seed)
+        groups = train_ops.RowGroups(ids, len(x), len(a), planned=True)
+        y, h = train_ops.low_rank_rows(x, a, b, groups, False, scale, steps, seed, base=base, keep=ctx.needs_input_grad[2])
+        # x is for the gradient of a, a for that of x
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, a if ctx.needs_input_grad[0] else None, b, h, *held)
+        ctx.groups, ctx.a_shape = groups, a.shape
+        return y
+
+    @staticmethod
+    def backward(ctx, up):
+        if torch.is_grad_enabled():
+            raise RuntimeError("low_rank_update: its gradients cannot be differentiated again (create_graph=True)")
+        x, a, b, more, *held = ctx.saved_tensors
+        scale = held.pop(0) if ctx.scale is None else ctx.scale
+        seed = held.pop(0) if ctx.seed is None else ctx.seed
+        want_x, want_a, want_b, want_base = ctx.needs_input_grad[:4]
+        dx = da = db = None
+        if not up.is_cuda:
+            dx, da, db = _cpu_backward(x, a, b, more, scale, ctx.steps, seed, up)
+        elif want_x or want_a or want_b:
+            rows, g, (_, rank, d) = rows_of(up), None, ctx.a_shape
+            if want_x or want_a:
+                second = a if want_x else b          # not read without want_x
+                dx, g = train_ops.low_rank_rows(rows, b, second.view(len(b), rank, -1), ctx.groups, True, scale, ctx.steps, seed, keep=want_a, only_kept=not want_x)
+            if want_a or want_b:
+                da, db = train_ops.low_rank_outer(x, g, rows, more, d, rank, ctx.groups, scale, ctx.steps, seed)
+        return dx if want_x else None, da if want_a else None, db if want_b else None, up if want_base else None, None, None, None, None
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of a tensor's values and the one behind the last."""
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _check_out(out, shape, x, others, base, wants_grad) -> None:
+    if wants_grad:
+        raise ValueError("low_rank_update: out is for calls without gradients")
+    if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"low_rank_update: out is {tuple(shape)} of {x.dtype} on {x.device}, got {tuple(out.shape)} of {out.dtype} on {out.device}")
+    if out.numel() == 0:
+        return
+    rows = out.view(-1, shape[-1]) if out.is_contiguous() else out if out.dim() == 2 else None
+    if rows is None or (rows.stride(1) != 1 and shape[-1] > 1) or (len(rows) > 1 and rows.stride(0) < shape[-1]):
+        raise ValueError(f"low_rank_update: out is dense, or a matrix of rows that do not overlap, got strides {out.stride()}")
+    same = base is not None and base.data_ptr() == out.data_ptr() and base.stride() == out.stride()
+    begin, end = _span(out)
+    for t in others + ([] if base is None or same else [base]):
+        lo, hi = _span(t) if t.numel() else (0, 0)
+        if lo < end and begin < hi:
+            raise ValueError("low_rank_update: out shares memory with an input that it is not itself")
+
+
+def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: torch.Tensor | None = None, ids: torch.Tensor | None = None,
+                    scale: float | torch.Tensor = 1.0, dropout: float = 0.0, seed: int | torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """``base + scale * b[e] (a[e] x)`` for every row of ``x``, where ``e`` is the row's adapter; differentiable in ``x``, ``a``, ``b`` and ``base``.
+
+    ``x`` [..., in], ``base`` [..., out] (what the shared projection gave; None: 0).  One adapter: ``a`` [rank, in] and ``b`` [out, rank]; many:
+    ``a`` [count, rank, in], ``b`` [count, out, rank] and ``ids`` [...] (int32 or int64) with each row's adapter, in any order.  A negative id
+    is a row without one, whose result is ``base`` as it is.  An id of ``count`` or more raises IndexError on the CPU; on the GPU, where nothing waits,
+    the results of that row and the gradient of its ``x`` are NaN, and no adapter's gradient has it.  ``scale``: a number, or float32 [count].  All
+    tensors have one type (float32, float16 or bfloat16; float64 on the CPU); ranks go up to 128, adapters to 65536, all sizes stay below 2^30.  ``dropout``
+    zeroes values of ``x`` on their way in, as :func:`dropout` of ``x`` (as rows) with the same ``seed`` does.
+
+    Sums are float32 whatever the inputs, the rank values keep 22 bits or more, results and gradients are rounded once.  ``out`` takes the result of a call
+    without gradients; it may be ``base`` itself.  Between the passes the rank values are kept (4 bytes each, the rank rounded up to 16, 32, 64 or 128), and
+    ``x``, ``a`` and ``b`` as every product keeps them.  On the GPU nothing is read back and all memory comes from torch's allocator; a pass and its
+    gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives are refused."""
+    what = "low_rank_update"
+    if x.dim() < 1 or a.dim() not in (2, 3) or b.dim() != a.dim() or x.shape[-1] != a.shape[-1] or a.shape[-2] != b.shape[-1] or a.shape[:-2] != b.shape[:-2]:
+        raise ValueError(f"{what}: x [..., in], a [count, rank, in] and b [count, out, rank] (or one adapter without count) are wanted, got "
+                         f"{tuple(x.shape)}, {tuple(a.shape)} and {tuple(b.shape)}")
+    single = a.dim() == 2
+    count, (rank, d), cols = 1 if single else a.shape[0], a.shape[-2:], b.shape[-2]
+    shape = x.shape[:-1] + (cols,)
+    n = math.prod(x.shape[:-1])
+    if not 1 <= rank <= MAX_RANK or not 1 <= count <= 65536 or min(d, cols) < 1 or max(d, cols, n) >= 2 ** 30:
+        raise ValueError(f"{what}: 1 to 65536 adapters of rank 1 to {MAX_RANK}, widths of at least 1 and sizes below 2^30 are wanted, got {count} of rank {rank}, "
+                         f"widths {d} and {cols}, {n} rows")
+    if base is not None and base.shape != shape:
+        raise ValueError(f"{what}: base of shape {tuple(shape)} is wanted, got {tuple(base.shape)}")
+    if ids is None and count != 1:
+        raise ValueError(f"{what}: with {count} adapters ids of shape {tuple(x.shape[:-1])} are wanted")
+    if ids is not None and ids.shape != x.shape[:-1]:
+        raise ValueError(f"{what}: ids of shape {tuple(x.shape[:-1])} are wanted, got {tuple(ids.shape)}")
+    if ids is not None and ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: ids are int32 or int64, got {ids.dtype}")
+    if isinstance(scale, torch.Tensor):
+        if scale.dtype != torch.float32 or scale.numel() != count or scale.dim() > 1:
+            raise ValueError(f"{what}: a scale for each adapter is float32 [{count}], got {scale.dtype} of shape {tuple(scale.shape)}")
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: the scale has no gradient")
+        scale = scale.detach().reshape(-1).contiguous()
+    else:
+        scale = float(scale)
+    given = [x, a, b] + [t for t in (base, ids, scale) if isinstance(t, torch.Tensor)]
+    if any(t.device != x.device for t in given) or x.device.type not in ("cuda", "cpu"):
+        raise ValueError(f"{what}: CUDA or CPU tensors of one device are wanted, got {', '.join(str(t.device) for t in given)}")
+    types = _TYPES if x.is_cuda else _TYPES + (torch.float64,)
+    if x.dtype not in types or any(t.dtype != x.dtype for t in (a, b) + (() if base is None else (base,))):
+        raise TypeError(f"{what}: x, a, b and base of one type (float32, float16, bfloat16) are wanted, got "
+                        f"{', '.join(str(t.dtype) for t in (x, a, b) + (() if base is None else (base,)))}")
+    steps = keep_steps(check_p(dropout, what))
+    seed = check_seed(seed, x.device, what) if seed is not None or steps < 65536 else 0
+    wants_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, a, b, base))
+    if out is not None:
+        _check_out(out, shape, x, [t for t in given if t is not base] + ([seed] if isinstance(seed, torch.Tensor) else []), base, wants_grad)
+    if single:
+        a, b = a[None], b[None]
+    if n == 0:
+        y = x @ a[0].T @ b[0].T                     # zero gradients
+        return out if out is not None else y if base is None else base + y
+    flat, base2 = rows_of(x), None if base is None else rows_of(base)
+    a, b = a.contiguous(), b.contiguous()
+    if ids is not None:
+        ids = ids.reshape(-1).contiguous()
+        if not x.is_cuda and bool((ids >= count).any()):
+            raise IndexError(f"{what}: an id names none of {count} adapters")
+    if wants_grad:
+        return _LowRankUpdate.apply(flat, a, b, base2, ids, scale, steps, seed).reshape(shape)
+    if not x.is_cuda:
+        y = _cpu_forward(flat, a, b, base2, ids, scale, steps, seed).reshape(shape)
+        return y if out is None else out.copy_(y)
+    groups = train_ops.RowGroups(ids, n, count, planned=False)
+    to = None if out is None else out if out.dim() == 2 else out.view(-1, cols)
+    y, _ = train_ops.low_rank_rows(flat, a, b, groups, False, scale, steps, seed, base=base2, out=to)
+    if out is None:
+        return y.reshape(shape)
+    if not out.is_inference():
+        increment_version(out)
+    return out
+
+
+class AdapterBank:
+    """The adapters of one projection that requests may name: factors side by side, as :func:`low_rank_update` takes them.  Adapters of a lower rank
+    than the bank's are filled up with zeros, which costs their bytes and changes no result.
+
+    >>> bank = AdapterBank(4096, 4096, rank=16, count=64, dtype=torch.bfloat16, device="cuda")
+    >>> bank.set(3, adapter)                        # a LoraAdapter
+    >>> y = bank(x, base, ids)                      # ids: each row's adapter, -1 without one
+    """
+
+    def __init__(self, in_features: int, out_features: int, rank: int, count: int, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if not 1 <= rank <= MAX_RANK or not 1 <= count <= 65536 or min(in_features, out_features) < 1:
+            raise ValueError(f"AdapterBank: 1 to 65536 adapters of rank 1 to {MAX_RANK} are wanted, got {count} of rank {rank}, {in_features} to {out_features}")
+        self.a = torch.zeros(count, rank, in_features, dtype=dtype, device=device)
+        self.b = torch.zeros(count, out_features, rank, dtype=dtype, device=device)
+        self.scales = torch.zeros(count, dtype=torch.float32, device=device)
+
+    @property
+    def count(self) -> int:
+        return len(self.a)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.a, self.b, self.scales))
+
+    @torch.no_grad()
+    def set(self, index: int, adapter) -> None:
+        """Copies a ``LoraAdapter`` into place ``index``."""
+        if not 0 <= index < self.count:
+            raise IndexError(f"AdapterBank: place {index} of {self.count}")
+        r, d = adapter.A.shape
+        if r > self.a.shape[1] or d != self.a.shape[2] or adapter.B.shape != (self.b.shape[1], r):
+            raise ValueError(f"AdapterBank: an adapter of rank up to {self.a.shape[1]} from {self.a.shape[2]} to {self.b.shape[1]} is wanted, got "
+                             f"{tuple(adapter.A.shape)} and {tuple(adapter.B.shape)}")
+        self.clear(index)
+        self.a[index, :r] = adapter.A
+        self.b[index, :, :r] = adapter.B
+        self.scales[index] = adapter.config.scale
+
+    @torch.no_grad()
+    def clear(self, index: int) -> None:
+        """Leaves place ``index`` without effect."""
+        if not 0 <= index < self.count:
+            raise IndexError(f"AdapterBank: place {index} of {self.count}")
+        for t in (self.a, self.b, self.scales):
+            t[index] = 0
+
+    @torch.no_grad()
+    def __call__(self, x: torch.Tensor, base: torch.Tensor | None, ids: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        return low_rank_update(x, self.a, self.b, base=base, ids=ids, scale=self.scales, out=out)
