@@ -88,9 +88,9 @@ int bonsai_lr_plan(const void* ids, int wide, int n, int adapters, int* order, i
 // back = 0: y [n][cols] = base + s w2 (w1 x), w1 [adapters][rank][k], w2 [adapters][cols][rank], x dropped by `steps` of 65536.
 // back = 1: y [n][cols] = s w2^T (w1^T x) dropped, w1 [adapters][k][rank], w2 [adapters][rank][cols].
 // mode: 0 one adapter, 1 ids of at most bonsai_lr_self_rows() rows, 2 order and start of bonsai_lr_plan.  kept (may be null; not with mode 1): the rank
-// values, f32 [n][bonsai_lr_padded(rank)] by place in the order.  base may be null, or y itself;
+// values, [n][bonsai_lr_padded(rank)] of 4 bytes by place in the order, for bonsai_lr_outer.  base may be null, or y itself;
 // y may be null where the rank values alone are wanted.
-int bonsai_lr_rows(const void* x, long long ldx, const void* w1, const void* w2, const void* base, long long ld_base, void* y, long long ldy, float* kept,
+int bonsai_lr_rows(const void* x, long long ldx, const void* w1, const void* w2, const void* base, long long ld_base, void* y, long long ldy, void* kept,
                    const float* scales, float scale, int n, int k, int cols, int rank, int adapters, int type, int back, int mode, const void* ids, int ids_wide,
                    const int* order, const int* start, unsigned long long seed, const long long* seed_dev, int steps, cudaStream_t st) {
   using namespace bonsai;
@@ -102,7 +102,8 @@ int bonsai_lr_rows(const void* x, long long ldx, const void* w1, const void* w2,
   LrRowsArgs a = {g, x, ldx, w1, w2, base, ld_base, y, ldy, kept, scales, scale, k, cols, rank, 0};
   a.vec_x = lr_vec(x, ldx, k, size);
   a.vec_w1 = back ? lr_vec(w1, rank, rank, size) : lr_vec(w1, k, k, size);
-  a.vec_w2 = back ? lr_vec(w2, cols, cols, size) : 0;
+  // forward: rank values of a column as words of 8 bytes
+  a.vec_w2 = back ? lr_vec(w2, cols, cols, size) : rank % (8 / size) == 0 && (uintptr_t)w2 % 8 == 0;
   a.vec_y = lr_vec(y, ldy, cols, size) && (base == nullptr || lr_vec(base, ld_base, cols, size));
   a.drop = lr_rule(seed, seed_dev, steps);
   a.drop_x = drop && !back;
@@ -113,7 +114,7 @@ int bonsai_lr_rows(const void* x, long long ldx, const void* w1, const void* w2,
 
 // da [adapters][rank][d] = s sum g x^T (x dropped), db [adapters][out][rank] = s sum dy h^T over each adapter's rows; either may be null.  g, h: `kept`
 // of the two directions.  Adapters without rows get zeros.
-int bonsai_lr_outer(const void* x, long long ldx, const float* g, void* da, int d, const void* dy, long long lddy, const float* h, void* db, int out,
+int bonsai_lr_outer(const void* x, long long ldx, const void* g, void* da, int d, const void* dy, long long lddy, const void* h, void* db, int out,
                     const float* scales, float scale, int n, int rank, int adapters, int type, int mode, const int* order, const int* start,
                     unsigned long long seed, const long long* seed_dev, int steps, cudaStream_t st) {
   using namespace bonsai;

@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "philox.cuh"
 
@@ -41,7 +43,7 @@ struct LrRowsArgs {
   const void *w1, *w2;                   // forward: A, B; backward: B, A
   const void* base; long long ld_base;   // [n][cols], may be null
   void* y; long long ldy;                // null: the rank values alone are wanted
-  float* kept;                           // [n][padded rank] by place in the order, may be null
+  void* kept;                            // [n][padded rank] by place in the order, may be null: f32, of bf16 the two parts [2][n][padded rank]
   const float* scales;                   // of the adapters, or null: scale
   float scale;
   int k, cols, rank;
@@ -55,7 +57,7 @@ struct LrOuterArgs {
   LrGroups groups;
   // two products of one launch: 0: dA [rank][k] from x (dropped) and g, 1: dB [cols][rank] from dy and h
   const void* q[2]; long long ldq[2];
-  const float* p[2];
+  const void* p[2];                      // `kept` of the rows
   void* out[2];
   int width[2], blocks[2], vec[2];       // columns, blocks of columns
   int rank;
@@ -249,22 +251,26 @@ __device__ __forceinline__ void lr_drop8(T* p, unsigned bits) {
   }
 }
 
+// Eight values at column `c` of a row of `width` (null: none) into shared memory, zeros behind the row's end.
+template <typename T>
+__device__ __forceinline__ void lr_copy8(T* dst, const T* src, int c, int width, bool vec, const T* any) {
+  const int left = src != nullptr ? width - c : 0;
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(dst + i * (16 / sizeof(T)), left > 0 ? src + c + i * (16 / sizeof(T)) : any, left > 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[i] = i < left ? src[c + i] : lr_round<T>(0.0f);
+  }
+}
+
 // Eights of rows into shared memory: rows r < nrows of `from(r)` (null: zeros), columns c0 .. c0 + C - 1 of `width`; to: rows of `pitch` values.  any: a
 // readable address for copies of nothing.
 template <typename T, int C, typename From>
 __device__ __forceinline__ void lr_fill(T* to, int pitch, int nrows, int c0, int width, bool vec, const T* any, From from) {
   for (int u = threadIdx.x; u < nrows * (C / 8); u += kLrThreads) {
     const int r = u / (C / 8), c = u % (C / 8) * 8;
-    const T* src = from(r);
-    T* dst = to + r * pitch + c;
-    const int left = src != nullptr ? width - c0 - c : 0;
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(dst + i * (16 / sizeof(T)), left > 0 ? src + c0 + c + i * (16 / sizeof(T)) : any, left > 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dst[i] = i < left ? src[c0 + c + i] : lr_round<T>(0.0f);
-    }
+    lr_copy8<T>(to + r * pitch + c, from(r), c0 + c, width, vec, any);
   }
 }
 
@@ -275,30 +281,37 @@ template <int M> struct LrShape {
   static constexpr int kMw = M == 64 ? 2 : 1, kAcross = kLrWarps / (kM16 / kMw);      // of the second product: 16-row tiles of a warp, warps over columns
 };
 
+// The rank values wait for the second product in two parts, each of the inputs' 16-bit type (f16 over a power of two for each row, so that neither large nor
+// small ones are lost) or TF32.
 template <typename T, int R, int M, bool BACK> struct LrSmem {
   static constexpr int kPad = 16 / sizeof(T);
   static constexpr int kChunk = LrShape<M>::kChunk;
   static constexpr int kPitchX = kChunk + kPad, kPitchW = BACK ? R + 8 : kChunk + kPad, kRowsW = BACK ? kChunk : R;
   static constexpr int kStage = (M * kPitchX + kRowsW * kPitchW) * (int)sizeof(T);
   static constexpr int kJoin = LrShape<M>::kParts * M * R * 4;         // the warps' parts, over the stages
-  static constexpr int kPart = M * R * 4, kPitchH = R + 4, kH = M * kPitchH * 4;
-  static constexpr int bytes(int stages) { return (stages * kStage > kJoin ? stages * kStage : kJoin) + kPart + kH; }
+  static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = 2 * M * kPitchH * (int)sizeof(T);
+  // what of base is on its way: each lane's own 16 bytes, `kDepth` steps of a warp
+  static constexpr int kDepth = sizeof(T) == 4 ? 2 : M == 16 ? 4 : 3, kPieces = LrShape<M>::kMw * 2 * (int)sizeof(T) / 2;
+  static constexpr int kBase = BACK ? 0 : kLrWarps * kDepth * kPieces * 512;
+  static constexpr int ring(int stages) { return stages * kStage > kJoin ? stages * kStage : kJoin; }
+  static constexpr int bytes(int stages) { return ring(stages) + kPart + kH + kBase; }
 };
 
 template <typename T, int R, int M, bool BACK>
-__global__ void __launch_bounds__(kLrThreads) lr_rows_kernel(const __grid_constant__ LrRowsArgs a) {
+__global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(const __grid_constant__ LrRowsArgs a) {
   using S = LrShape<M>;
   using L = LrSmem<T, R, M, BACK>;
   constexpr bool F32 = sizeof(T) == 4;
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
   __shared__ int rows[M];
+  __shared__ float factors[M];
   __shared__ int scratch[kLrWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int ring = a.stages * L::kStage > L::kJoin ? a.stages * L::kStage : L::kJoin;
+  unsigned char* behind = lr_dynamic + L::ring(a.stages);
   float* join = reinterpret_cast<float*>(lr_dynamic);
-  float* part = reinterpret_cast<float*>(lr_dynamic + ring);
-  float* hs = part + M * R;
+  float* part = reinterpret_cast<float*>(behind);
+  T* hs = reinterpret_cast<T*>(behind + L::kPart);                   // first parts, then second parts
   const uint32_t rank = lr_rank(), ranks = lr_ranks();
   const LrTile tile = lr_tile<M>(a.groups, blockIdx.x / ranks, rows, scratch);
   if (tile.count == 0) return;                        // the whole cluster
@@ -306,21 +319,70 @@ __global__ void __launch_bounds__(kLrThreads) lr_rows_kernel(const __grid_consta
   const bool has = tile.group < a.groups.adapters;
   const uint2 key = a.drop_x || a.drop_y ? philox_key(a.drop) : make_uint2(0, 0);
 
+  // The second product: a warp takes 32 columns at a time.  Column 8 (c / 2) + 2 j + c % 2 is column c of its j-th product, so that the eight values that
+  // a thread has of a row lie side by side.
+  const T* w2 = (const T*)a.w2 + (has ? (long long)tile.group * a.cols * a.rank : 0);
+  const int all = (a.cols + 31) / 32, me = warp / S::kAcross * S::kMw * 16;
+  const int b0 = (int)((long long)all * rank / ranks), b1 = a.y != nullptr ? (int)((long long)all * (rank + 1) / ranks) : b0;
+  long long at_base[S::kMw][2], at_y[S::kMw][2];
+  bool live[S::kMw][2];
+#pragma unroll
+  for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = rows[me + m * 16 + h * 8 + g];
+      live[m][h] = row >= 0;
+      at_base[m][h] = (long long)(row < 0 ? 0 : row) * a.ld_base;
+      at_y[m][h] = (long long)(row < 0 ? 0 : row) * a.ldy;
+    }
+  uint4* ahead = reinterpret_cast<uint4*>(behind + L::kPart + L::kH) + warp * L::kDepth * L::kPieces * 32 + lane;
+  const bool fetched = !BACK && a.base != nullptr && a.vec_y;
+  auto request = [&](int i) {           // base of this warp's i-th step
+    if constexpr (!BACK) {
+      const int b = b0 + warp % S::kAcross + i * S::kAcross, col = b * 32 + 8 * t;
+      if (fetched && b < b1 && col < a.cols) {
+        uint4* to = ahead + i % L::kDepth * L::kPieces * 32;
+#pragma unroll
+        for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int v = 0; v < (int)sizeof(T) / 2; ++v)
+              if (live[m][h]) lr_copy16(to + ((m * 2 + h) * ((int)sizeof(T) / 2) + v) * 32, (const T*)a.base + at_base[m][h] + col + v * (16 / (int)sizeof(T)), true);
+      }
+    }
+  };
+
   if (has) {
     const T* w1 = (const T*)a.w1 + (long long)tile.group * a.k * a.rank;
     const int chunks = (a.k + S::kChunk - 1) / S::kChunk;
     const int c0 = (int)((long long)chunks * rank / ranks), c1 = (int)((long long)chunks * (rank + 1) / ranks);
     auto stage = [&](int i) { return reinterpret_cast<T*>(lr_dynamic + i * L::kStage); };
+    // The eights that this thread copies of every chunk: their rows and columns stay the same.
+    constexpr int kAcrossX = S::kChunk / 8, kX = M * kAcrossX / kLrThreads, kRowStep = kLrThreads / kAcrossX;
+    constexpr int kAcrossW = BACK ? R / 8 : kAcrossX, kUnitsW = L::kRowsW * kAcrossW, kW = (kUnitsW + kLrThreads - 1) / kLrThreads, kStepW = kLrThreads / kAcrossW;
+    static_assert(M * kAcrossX % kLrThreads == 0 && kLrThreads % kAcrossX == 0 && kLrThreads % kAcrossW == 0, "whole rows of threads");
+    const int xr = threadIdx.x / kAcrossX, xc = threadIdx.x % kAcrossX * 8, wr = threadIdx.x / kAcrossW, wc = threadIdx.x % kAcrossW * 8;
+    const T* from[kX];
+    int from_row[kX];
+#pragma unroll
+    for (int i = 0; i < kX; ++i) {
+      from_row[i] = rows[xr + i * kRowStep];
+      from[i] = from_row[i] < 0 ? (const T*)nullptr : (const T*)a.x + from_row[i] * a.ldx;
+    }
     auto fetch = [&](int c, int slot) {
       T* xs = stage(slot);
+      T* ws = xs + M * L::kPitchX;
       const int k0 = c * S::kChunk;
-      lr_fill<T, S::kChunk>(xs, L::kPitchX, M, k0, a.k, a.vec_x, (const T*)a.x, [&](int r) { return rows[r] < 0 ? (const T*)nullptr : (const T*)a.x + rows[r] * a.ldx; });
-      if (BACK)
-        lr_fill<T, R>(xs + M * L::kPitchX, L::kPitchW, S::kChunk, 0, a.rank, a.vec_w1, w1,
-                      [&](int r) { return k0 + r < a.k ? w1 + (long long)(k0 + r) * a.rank : (const T*)nullptr; });
-      else
-        lr_fill<T, S::kChunk>(xs + M * L::kPitchX, L::kPitchW, R, k0, a.k, a.vec_w1, w1,
-                              [&](int r) { return r < a.rank ? w1 + (long long)r * a.k : (const T*)nullptr; });
+#pragma unroll
+      for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i], k0 + xc, a.k, a.vec_x, (const T*)a.x);
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        const int r = wr + i * kStepW;
+        if (kUnitsW % kLrThreads != 0 && r >= L::kRowsW) break;
+        if (BACK) lr_copy8<T>(ws + r * L::kPitchW + wc, k0 + r < a.k ? w1 + (long long)(k0 + r) * a.rank : (const T*)nullptr, wc, a.rank, a.vec_w1, w1);
+        else lr_copy8<T>(ws + r * L::kPitchW + wc, r < a.rank ? w1 + (long long)r * a.k : (const T*)nullptr, k0 + wc, a.k, a.vec_w1, w1);
+      }
     };
     float acc[R / 8][4];
 #pragma unroll
@@ -330,6 +392,10 @@ __global__ void __launch_bounds__(kLrThreads) lr_rows_kernel(const __grid_consta
     const int m0 = warp % S::kM16 * 16, kp = warp / S::kM16 * S::kWarpK;
     for (int i = 0; i < a.stages - 1; ++i) {
       if (c0 + i < c1) fetch(c0 + i, i);
+      if (i == a.stages - 2) {
+#pragma unroll
+        for (int d = 0; d < L::kDepth; ++d) request(d);
+      }
       lr_commit();
     }
     int slot = 0;
@@ -337,10 +403,10 @@ __global__ void __launch_bounds__(kLrThreads) lr_rows_kernel(const __grid_consta
       lr_wait_left(a.stages - 2);
       T* xs = stage(slot);
       if (a.drop_x) {
-        for (int u = threadIdx.x; u < M * (S::kChunk / 8); u += kLrThreads) {       // the eights that this thread copied
-          const int r = u / (S::kChunk / 8), col = u % (S::kChunk / 8) * 8;
-          if (rows[r] >= 0) lr_drop8<T>(xs + r * L::kPitchX + col, dropout_bits((unsigned)(c * S::kChunk + col) >> 3, rows[r], key, a.drop.steps));
-        }
+#pragma unroll
+        for (int i = 0; i < kX; ++i)
+          if (from_row[i] >= 0)
+            lr_drop8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, dropout_bits((unsigned)(c * S::kChunk + xc) >> 3, from_row[i], key, a.drop.steps));
       }
       __syncthreads();
       if (c + a.stages - 1 < c1) fetch(c + a.stages - 1, slot == 0 ? a.stages - 1 : slot - 1);
@@ -413,147 +479,261 @@ __global__ void __launch_bounds__(kLrThreads) lr_rows_kernel(const __grid_consta
     lr_arrive();
     lr_meet();
     const float share = a.drop_x ? a.drop.share : 1.0f;
-    for (int u = threadIdx.x; u < M * R / 4; u += kLrThreads) {
+    constexpr int kUnits = M * R / 4, kLanes = R / 4;              // of a row: neighbouring lanes
+#pragma unroll 1
+    for (int u = threadIdx.x; u < kUnits; u += kLrThreads) {       // a multiple of 32: whole warps
       float4 v = lr_remote4(part + 4 * u, 0);
       for (uint32_t r = 1; r < ranks; ++r) {
         const float4 w = lr_remote4(part + 4 * u, r);
         v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
       }
-      const int row = u / (R / 4), col = u % (R / 4) * 4;
+      const int row = u / kLanes, col = u % kLanes * 4;
       // behind the rank there is nothing, also beside an infinity, whose product with the zeros there is none
-      v.x = col < a.rank ? v.x * share : 0.0f; v.y = col + 1 < a.rank ? v.y * share : 0.0f;
-      v.z = col + 2 < a.rank ? v.z * share : 0.0f; v.w = col + 3 < a.rank ? v.w * share : 0.0f;
-      *reinterpret_cast<float4*>(hs + row * L::kPitchH + col) = v;
-      if (a.kept != nullptr && rank == 0 && row < tile.count) *reinterpret_cast<float4*>(a.kept + (long long)(tile.place + row) * R + col) = v;
-    }
-    lr_arrive();                                       // this block has read the others' parts; it leaves when they have read its own
-    __syncthreads();
-  }
-
-  // y = base + s W2 h: a warp takes 32 columns at a time.  Column 8 (c / 2) + 2 j + c % 2 is column c of its j-th product, so that the eight values that a
-  // thread has of a row lie side by side.
-  const float by = a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale;
-  const T* w2 = (const T*)a.w2 + (has ? (long long)tile.group * a.cols * a.rank : 0);
-  const int all = (a.cols + 31) / 32;
-  const int b0 = (int)((long long)all * rank / ranks), b1 = a.y != nullptr ? (int)((long long)all * (rank + 1) / ranks) : b0;
-  const int m0 = warp / S::kAcross * S::kMw * 16;
-  for (int b = b0 + warp % S::kAcross; b < b1; b += S::kAcross) {
-    const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
-    float from[S::kMw][2][8];
+      float f[4] = {col < a.rank ? v.x * share : 0.0f, col + 1 < a.rank ? v.y * share : 0.0f, col + 2 < a.rank ? v.z * share : 0.0f, col + 3 < a.rank ? v.w * share : 0.0f};
+      const bool keeps = a.kept != nullptr && rank == 0 && row < tile.count;
+      const long long place = (long long)(tile.place + row) * R + col;
+      if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
+        if (keeps) *reinterpret_cast<float4*>((float*)a.kept + place) = make_float4(f[0], f[1], f[2], f[3]);
+        float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
 #pragma unroll
-    for (int m = 0; m < S::kMw; ++m)
+        for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // the row's largest value between 2^13 and 2^14; zeros, infinities and what is next to them stay as they are
+        const int e = (int)(__float_as_uint(top) >> 23 & 255u) - 127 - 13;
+        const bool scaled = top > 1e-30f && top < 1e30f;
+        const float down = scaled ? __uint_as_float((unsigned)(127 - e) << 23) : 1.0f;
+        if (col == 0) factors[row] = scaled ? __uint_as_float((unsigned)(127 + e) << 23) : 1.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = rows[m0 + m * 16 + h * 8 + g];
+        for (int i = 0; i < 4; ++i) f[i] *= down;
+      }
+      if constexpr (F32) {
+        if (keeps) *reinterpret_cast<float4*>((float*)a.kept + place) = make_float4(f[0], f[1], f[2], f[3]);
+        uint4 hi, lo;
+        lr_split(f[0], hi.x, lo.x);
+        lr_split(f[1], hi.y, lo.y);
+        lr_split(f[2], hi.z, lo.z);
+        lr_split(f[3], hi.w, lo.w);
+        *reinterpret_cast<uint4*>(hs + row * L::kPitchH + col) = hi;
+        *reinterpret_cast<uint4*>(hs + (M + row) * L::kPitchH + col) = lo;
+      } else {
+        __align__(8) T hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) from[m][h][i] = 0.0f;
-        if (a.base != nullptr && row >= 0 && left > 0) {
-          const T* p = (const T*)a.base + row * a.ld_base + col;
-          if (a.vec_y) lr_load8<T, true>(p, 8, from[m][h]);
-          else lr_load8<T, false>(p, left, from[m][h]);
+        for (int i = 0; i < 4; ++i) {
+          hi[i] = lr_round<T>(f[i]);
+          const float h = lr_float<T>(hi[i]);
+          lo[i] = lr_round<T>(fabsf(h) <= 3.4028234e38f ? f[i] - h : 0.0f);
+        }
+        *reinterpret_cast<uint2*>(hs + row * L::kPitchH + col) = *reinterpret_cast<const uint2*>(hi);
+        *reinterpret_cast<uint2*>(hs + (M + row) * L::kPitchH + col) = *reinterpret_cast<const uint2*>(lo);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          if (keeps) {
+            *reinterpret_cast<uint2*>((T*)a.kept + place) = *reinterpret_cast<const uint2*>(hi);
+            *reinterpret_cast<uint2*>((T*)a.kept + (long long)a.groups.n * R + place) = *reinterpret_cast<const uint2*>(lo);
+          }
         }
       }
+    }
+    __syncwarp();
+    lr_arrive();                                       // this block has read the others' parts; it leaves when they have read its own
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int d = 0; d < L::kDepth; ++d) request(d);
+    lr_commit();
+    lr_wait<0>();
+  }
+
+  // Of the rank values the thread has 4 t .. 4 t + 3 of every sixteen (f32: 2 t and 2 t + 1 of every eight): the axis of a product may be taken in any order, and
+  // so its factors lie side by side.
+  constexpr int kStep = F32 ? 8 : 16, kEach = kStep / 4;
+  auto load_w = [&](int b, int k, uint32_t (*w)[2]) {
+    const int wc = b * 32 + 8 * (g >> 1), kk = k + kEach * t;      // eight columns, of which this thread takes every second
+    if (BACK) {
+      uint32_t v[kEach][F32 ? 8 : 4];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const T* p = w2 + (long long)(kk + i) * a.cols + wc;
+        const bool there = kk + i < a.rank && wc < a.cols;
+        if (a.vec_w2) {
+#pragma unroll
+          for (int q = 0; q < (int)sizeof(T) / 2; ++q) {
+            const uint4 u = there ? reinterpret_cast<const uint4*>(p)[q] : make_uint4(0, 0, 0, 0);
+            v[i][4 * q] = u.x; v[i][4 * q + 1] = u.y; v[i][4 * q + 2] = u.z; v[i][4 * q + 3] = u.w;
+          }
+        } else {
+          __align__(16) T e[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) e[q] = there && wc + q < a.cols ? p[q] : lr_round<T>(0.0f);
+#pragma unroll
+          for (int q = 0; q < (F32 ? 8 : 4); ++q) v[i][q] = reinterpret_cast<const uint32_t*>(e)[q];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (F32) {
+          w[j][0] = g & 1 ? v[0][2 * j + 1] : v[0][2 * j];
+          w[j][1] = g & 1 ? v[1][2 * j + 1] : v[1][2 * j];
+        } else {
+          const unsigned pick = g & 1 ? 0x7632u : 0x5410u;        // the upper or the lower halves of two words
+          w[j][0] = __byte_perm(v[0][j], v[1][j], pick);
+          w[j][1] = __byte_perm(v[kEach - 2][j], v[kEach - 1][j], pick);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int cc = wc + 2 * j + (g & 1);
+        const T* p = w2 + (long long)cc * a.rank + kk;
+        if (a.vec_w2) {
+          const uint2 u = cc < a.cols && kk < a.rank ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+          w[j][0] = u.x; w[j][1] = u.y;
+        } else {
+          __align__(8) T e[kEach];
+#pragma unroll
+          for (int q = 0; q < kEach; ++q) e[q] = cc < a.cols && kk + q < a.rank ? p[q] : lr_round<T>(0.0f);
+          w[j][0] = reinterpret_cast<const uint32_t*>(e)[0];
+          w[j][1] = reinterpret_cast<const uint32_t*>(e)[1];
+        }
+      }
+    }
+  };
+  auto load_h = [&](int m, int k, int part, uint32_t* h) {
+    const T* p = hs + (part * M + me + m * 16 + g) * L::kPitchH + k + kEach * t;
+    const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(p + 8 * L::kPitchH);
+    h[0] = u.x; h[1] = v.x; h[2] = u.y; h[3] = v.y;
+  };
+  const float by = a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale;
+  float scaled[S::kMw][2];
+#pragma unroll
+  for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) scaled[m][h] = has && sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? by * factors[me + m * 16 + h * 8 + g] : by;
+  constexpr bool kHold = R == 16;                                  // the rank values and the next factors stay in registers
+  uint32_t held[kHold ? R / kStep : 1][S::kMw][2][4], next[kHold ? R / kStep : 1][4][2];
+  int b = b0 + warp % S::kAcross;
+  if (kHold && has) {
+#pragma unroll
+    for (int k = 0; k < R / kStep; ++k) {
+#pragma unroll
+      for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) load_h(m, k * kStep, p, held[k][m][p]);
+      if (b < b1) load_w(b, k * kStep, next[k]);
+    }
+  }
+  for (int i = 0; b < b1; b += S::kAcross, ++i) {
+    const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
     float acc[S::kMw][4][4];
 #pragma unroll
     for (int m = 0; m < S::kMw; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.0f;
+        for (int q = 0; q < 4; ++q) acc[m][j][q] = 0.0f;
     if (has) {
-      const int wc = b * 32 + 8 * (g >> 1);                      // eight columns, of which this thread takes every second
-#pragma unroll 2
-      for (int k = 0; k < R; k += 8) {
-        if (k >= a.rank) break;
-        float w[4][2];                                           // of product j: k + t, k + t + 4
-        const int k0 = k + t, k1 = k + t + 4;
-        if (BACK) {
-          float v[8];
+      auto multiply = [&](uint32_t (*w)[2], auto h) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int kk = h ? k1 : k0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-            if (kk < a.rank && wc < a.cols) {
-              const T* p = w2 + (long long)kk * a.cols + wc;
-              if (a.vec_w2) lr_load8<T, true>(p, 8, v);
-              else lr_load8<T, false>(p, a.cols - wc, v);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j][h] = g & 1 ? v[2 * j + 1] : v[2 * j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int cc = wc + 2 * j + (g & 1);
-            const T* p = w2 + (long long)cc * a.rank;
-            w[j][0] = cc < a.cols && k0 < a.rank ? lr_float<T>(p[k0]) : 0.0f;
-            w[j][1] = cc < a.cols && k1 < a.rank ? lr_float<T>(p[k1]) : 0.0f;
-          }
-        }
-#pragma unroll
-        for (int m = 0; m < S::kMw; ++m) {
-          uint32_t hi[4], lo[4];
-          const float* hp = hs + (m0 + m * 16 + g) * L::kPitchH + k + t;
-          lr_split(hp[0], hi[0], lo[0]);
-          lr_split(hp[8 * L::kPitchH], hi[1], lo[1]);
-          lr_split(hp[4], hi[2], lo[2]);
-          lr_split(hp[8 * L::kPitchH + 4], hi[3], lo[3]);
+        for (int m = 0; m < S::kMw; ++m)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if constexpr (F32) {
               uint32_t h0, l0, h1, l1;
-              lr_split(w[j][0], h0, l0);
-              lr_split(w[j][1], h1, l1);
-              lr_mma8(acc[m][j], lo, h0, h1);
-              lr_mma8(acc[m][j], hi, l0, l1);
-              lr_mma8(acc[m][j], hi, h0, h1);
+              lr_split(__uint_as_float(w[j][0]), h0, l0);
+              lr_split(__uint_as_float(w[j][1]), h1, l1);
+              lr_mma8(acc[m][j], h(m, 1), h0, h1);
+              lr_mma8(acc[m][j], h(m, 0), l0, l1);
+              lr_mma8(acc[m][j], h(m, 0), h0, h1);
             } else {
-              lr_mma8(acc[m][j], lo, __float_as_uint(w[j][0]), __float_as_uint(w[j][1]));
-              lr_mma8(acc[m][j], hi, __float_as_uint(w[j][0]), __float_as_uint(w[j][1]));
+              lr_mma16<T>(acc[m][j], h(m, 1), w[j][0], w[j][1]);
+              lr_mma16<T>(acc[m][j], h(m, 0), w[j][0], w[j][1]);
             }
           }
+      };
+      if constexpr (kHold) {
+        uint32_t w[R / kStep][4][2];
+#pragma unroll
+        for (int k = 0; k < R / kStep; ++k) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { w[k][j][0] = next[k][j][0]; w[k][j][1] = next[k][j][1]; }
+          if (b + S::kAcross < b1) load_w(b + S::kAcross, k * kStep, next[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < R / kStep; ++k) multiply(w[k], [&](int m, int p) -> const uint32_t* { return held[k][m][p]; });
+      } else {
+#pragma unroll 2
+        for (int k = 0; k < R; k += kStep) {
+          if (k >= a.rank) break;
+          uint32_t w[4][2], hv[S::kMw][2][4];
+          load_w(b, k, w);
+#pragma unroll
+          for (int m = 0; m < S::kMw; ++m)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) load_h(m, k, p, hv[m][p]);
+          multiply(w, [&](int m, int p) -> const uint32_t* { return hv[m][p]; });
         }
       }
     }
+    if (!BACK) lr_wait<L::kDepth - 1>();
+    const uint4* here = ahead + i % L::kDepth * L::kPieces * 32;
 #pragma unroll
     for (int m = 0; m < S::kMw; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = rows[m0 + m * 16 + h * 8 + g];
-        if (row < 0 || left <= 0) continue;
+        if (!live[m][h] || left <= 0) continue;
         float v[8];
-        const unsigned keep = a.drop_y ? dropout_bits((unsigned)col >> 3, row, key, a.drop.steps) : 0xffu;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = acc[m][i >> 1][2 * h + (i & 1)] * by;
-          v[i] = tile.group > a.groups.adapters ? __uint_as_float(0x7fc00000u) : !has ? from[m][h][i]
-                 : a.drop_y ? (keep >> i & 1u ? d * a.drop.share : 0.0f) : from[m][h][i] + d;
+        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+        if (!BACK && a.base != nullptr) {
+          if (a.vec_y) {
+            __align__(16) T e[8];
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(e)[q] = here[((m * 2 + h) * ((int)sizeof(T) / 2) + q) * 32];
+            lr_load8<T, true>(e, 8, v);
+          } else {
+            lr_load8<T, false>((const T*)a.base + at_base[m][h] + col, left, v);
+          }
         }
-        T* p = (T*)a.y + row * a.ldy + col;
+        if (has) {
+          const unsigned keep = BACK && a.drop_y ? dropout_bits((unsigned)col >> 3, rows[me + m * 16 + h * 8 + g], key, a.drop.steps) : 0xffu;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float d = acc[m][q >> 1][2 * h + (q & 1)] * scaled[m][h];
+            if (BACK) v[q] = a.drop_y ? (keep >> q & 1u ? d * a.drop.share : 0.0f) : d;
+            else v[q] += d;
+          }
+        } else if (tile.group > a.groups.adapters) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = __uint_as_float(0x7fc00000u);
+        }
+        T* p = (T*)a.y + at_y[m][h] + col;
         if (a.vec_y) lr_store8<T, true>(p, 8, v);
         else lr_store8<T, false>(p, left, v);
       }
+    request(i + L::kDepth);
+    if (!BACK) lr_commit();
   }
+  lr_wait<0>();
   __syncwarp();
   if (has) lr_meet();
 }
 
 // ---- the factors' gradients --------------------------------------------------------------------------------------------------------------
 // out[r][c] (or [c][r]) = s sum over the adapter's rows of p[row][r] q[row][c].  A cluster takes 128 columns of one adapter and one product, its blocks
-// split the rows.  The two rows 2 t and 2 t + 1 of every eight are what a thread has of a matrix instruction's axis of eight, which is how ldmatrix hands
-// out 16-bit values of q; p follows.
+// split the rows.  bf16: the rank values' two parts times q, both as ldmatrix turns them.  f16 and f32: TF32, where f16 is exact (its range would lose small rank
+// values); the two rows 2 t and 2 t + 1 of every eight are then what a thread has of a matrix instruction's axis of eight, which is how
+// ldmatrix hands out 16-bit values of q; p follows.
 template <typename T, int R> struct LrOuterSmem {
-  static constexpr int kPitchQ = kLrOuterCols + (sizeof(T) == 4 ? 4 : 8), kPitchP = R + 4;
-  static constexpr int kStage = kLrOuterRows * (kPitchQ * (int)sizeof(T) + kPitchP * 4);
+  static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int kPitchQ = kLrOuterCols + (sizeof(T) == 4 ? 4 : 8), kPitchP = kBf16 ? R + 8 : R + 4;
+  static constexpr int kSizeP = kBf16 ? 2 : 4, kP = kLrOuterRows * kPitchP * kSizeP;            // one part
+  static constexpr int kStage = kLrOuterRows * kPitchQ * (int)sizeof(T) + 2 * kP;
   static constexpr int kSum = R * kLrOuterCols * 4;
   static constexpr int bytes(int stages) { return stages * kStage > kSum ? stages * kStage : kSum; }
 };
 
 template <typename T, int R>
-__global__ void __launch_bounds__(kLrThreads) lr_outer_kernel(const __grid_constant__ LrOuterArgs a) {
+__global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(const __grid_constant__ LrOuterArgs a) {
   using L = LrOuterSmem<T, R>;
-  constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool F32 = sizeof(T) == 4, BF16 = L::kBf16;
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
   __shared__ int rows[3][kLrOuterRows];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -576,14 +756,21 @@ __global__ void __launch_bounds__(kLrThreads) lr_outer_kernel(const __grid_const
     }
   };
   auto qs = [&](int i) { return reinterpret_cast<T*>(lr_dynamic + i * L::kStage); };
-  auto ps = [&](int i) { return reinterpret_cast<float*>(lr_dynamic + i * L::kStage + kLrOuterRows * L::kPitchQ * sizeof(T)); };
+  auto ps = [&](int i) { return lr_dynamic + i * L::kStage + kLrOuterRows * L::kPitchQ * sizeof(T); };
   auto fetch = [&](int s, int slot) {
     const int* list = rows[s % 3];
+    const int from = first + s * kLrOuterRows;
     lr_fill<T, kLrOuterCols>(qs(slot), L::kPitchQ, kLrOuterRows, col0, width, a.vec[which], q, [&](int r) { return list[r] < 0 ? (const T*)nullptr : q + list[r] * a.ldq[which]; });
-    lr_fill<float, R>(ps(slot), L::kPitchP, kLrOuterRows, 0, R, true, a.p[which], [&](int r) {
-      const int place = first + s * kLrOuterRows + r;
-      return place < last ? a.p[which] + (long long)place * R : (const float*)nullptr;
-    });
+    if constexpr (BF16) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const T* p = (const T*)a.p[which] + part * (long long)a.groups.n * R;
+        lr_fill<T, R>((T*)(ps(slot) + part * L::kP), L::kPitchP, kLrOuterRows, 0, R, true, p, [&](int r) { return from + r < last ? p + (long long)(from + r) * R : (const T*)nullptr; });
+      }
+    } else {
+      const float* p = (const float*)a.p[which];
+      lr_fill<float, R>((float*)ps(slot), L::kPitchP, kLrOuterRows, 0, R, true, p, [&](int r) { return from + r < last ? p + (long long)(from + r) * R : (const float*)nullptr; });
+    }
   };
   float acc[R / 16][2][4];
 #pragma unroll
@@ -604,81 +791,117 @@ __global__ void __launch_bounds__(kLrThreads) lr_outer_kernel(const __grid_const
     lr_commit();
     if (s + 2 < s1) list(s + 2);
     lr_wait<1>();
-    if (drop) {
+    if (drop) {                     // the eights that this thread copied
       const int* list = rows[s % 3];
       for (int u = threadIdx.x; u < kLrOuterRows * (kLrOuterCols / 8); u += kLrThreads) {
         const int r = u / (kLrOuterCols / 8), c = u % (kLrOuterCols / 8) * 8;
         if (list[r] >= 0) lr_drop8<T>(qs(slot) + r * L::kPitchQ + c, dropout_bits((unsigned)(col0 + c) >> 3, list[r], key, a.drop.steps));
       }
     }
-    __syncthreads();
-    const T* qp = qs(slot) + warp * 16;
-    const float* pp = ps(slot);
-    float sum[R / 16][2][4];
-    if constexpr (F32) {
+    if constexpr (!BF16) {          // and its rank values into two parts
+      for (int u = threadIdx.x; u < kLrOuterRows * (R / 8); u += kLrThreads) {
+        uint4* hi = reinterpret_cast<uint4*>(ps(slot) + (u / (R / 8) * L::kPitchP + u % (R / 8) * 8) * 4);
+        uint4* lo = reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(hi) + L::kP);
 #pragma unroll
-      for (int i = 0; i < R / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) sum[i][j][k] = 0.0f;
-    }
-#pragma unroll
-    for (int k = 0; k < kLrOuterRows; k += 16) {
-      float v[2][2][2];             // of the first and the second eight rows: product j, rows 2 t and 2 t + 1
-      if constexpr (F32) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) v[h][j][i] = ((const float*)qp)[(k + 8 * h + 2 * t + i) * L::kPitchQ + j * 8 + g];
-      } else {
-        uint32_t w[4];
-        lr_ldm4t(w, qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float2 f = lr_pair<T>(w[2 * j + h]);
-            v[h][j][0] = f.x; v[h][j][1] = f.y;
-          }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t vh[2][2], vl[2][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if constexpr (F32) lr_split(v[h][j][i], vh[j][i], vl[j][i]);
-            else vh[j][i] = __float_as_uint(v[h][j][i]);
-          }
-#pragma unroll
-        for (int i = 0; i < R / 16; ++i) {
-          uint32_t hi[4], lo[4];
-          const float* p = pp + (k + 8 * h + 2 * t) * L::kPitchP + i * 16 + g;
-          lr_split(p[0], hi[0], lo[0]);
-          lr_split(p[8], hi[1], lo[1]);
-          lr_split(p[L::kPitchP], hi[2], lo[2]);
-          lr_split(p[L::kPitchP + 8], hi[3], lo[3]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float* d = F32 ? sum[i][j] : acc[i][j];
-            lr_mma8(d, lo, vh[j][0], vh[j][1]);
-            if constexpr (F32) lr_mma8(d, hi, vl[j][0], vl[j][1]);
-            lr_mma8(d, hi, vh[j][0], vh[j][1]);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const float4 f = reinterpret_cast<const float4*>(hi)[h];
+          uint4 x, y;
+          lr_split(f.x, x.x, y.x);
+          lr_split(f.y, x.y, y.y);
+          lr_split(f.z, x.z, y.z);
+          lr_split(f.w, x.w, y.w);
+          hi[h] = x;
+          lo[h] = y;
         }
       }
     }
-    if constexpr (F32) {
+    __syncthreads();
+    const T* qp = qs(slot) + warp * 16;
+    if constexpr (BF16) {
+      const T* pp = (const T*)ps(slot);
 #pragma unroll
-      for (int i = 0; i < R / 16; ++i)
+      for (int k = 0; k < kLrOuterRows; k += 16) {
+        uint32_t w[4];
+        lr_ldm4t(w, qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < R / 16; ++i) {
+          uint32_t hi[4], lo[4];
+          const T* p = pp + (k + (lane & 7) + (lane >> 4) * 8) * L::kPitchP + i * 16 + (lane >> 3 & 1) * 8;
+          lr_ldm4t(lo, p + L::kP / 2);
+          lr_ldm4t(hi, p);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[i][j][k];
+          for (int j = 0; j < 2; ++j) {
+            lr_mma16<T>(acc[i][j], lo, w[2 * j], w[2 * j + 1]);
+            lr_mma16<T>(acc[i][j], hi, w[2 * j], w[2 * j + 1]);
+          }
+        }
+      }
+    } else {
+      const uint32_t* pp = (const uint32_t*)ps(slot);
+      float sum[R / 16][2][4];
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[i][j][k] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < kLrOuterRows; k += 16) {
+        float v[2][2][2];             // of the first and the second eight rows: product j, rows 2 t and 2 t + 1
+        if constexpr (F32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) v[h][j][i] = ((const float*)qp)[(k + 8 * h + 2 * t + i) * L::kPitchQ + j * 8 + g];
+        } else {
+          uint32_t w[4];
+          lr_ldm4t(w, qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float2 f = lr_pair<T>(w[2 * j + h]);
+              v[h][j][0] = f.x; v[h][j][1] = f.y;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t vh[2][2], vl[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if constexpr (F32) lr_split(v[h][j][i], vh[j][i], vl[j][i]);
+              else vh[j][i] = __float_as_uint(v[h][j][i]);
+            }
+#pragma unroll
+          for (int i = 0; i < R / 16; ++i) {
+            const uint32_t* p = pp + (k + 8 * h + 2 * t) * L::kPitchP + i * 16 + g;
+            const uint32_t hi[4] = {p[0], p[8], p[L::kPitchP], p[L::kPitchP + 8]};
+            p += L::kP / 4;
+            const uint32_t lo[4] = {p[0], p[8], p[L::kPitchP], p[L::kPitchP + 8]};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float* d = F32 ? sum[i][j] : acc[i][j];
+              lr_mma8(d, lo, vh[j][0], vh[j][1]);
+              if constexpr (F32) lr_mma8(d, hi, vl[j][0], vl[j][1]);
+              lr_mma8(d, hi, vh[j][0], vh[j][1]);
+            }
+          }
+        }
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < R / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[i][j][k];
+      }
     }
     __syncthreads();
   }
@@ -766,7 +989,10 @@ static cudaError_t lr_rows_r(const LrRowsArgs& a, cudaStream_t st) {
   const LrGroups& g = a.groups;
   // Tiles of 64 rows where adapters fill them; 16 rows keep more clusters busy and waste less of the tiles
   const long long each = g.mode == LR_ONE ? g.n : g.n / (g.adapters > 0 ? g.adapters : 1);
-  if (g.mode != LR_SELF && each >= 48 && g.n >= 1024) return lr_rows_as<T, R, 64, BACK>(a, st);
+  static_assert(LrSmem<T, R, 16, BACK>::bytes(2) <= kLrSmemMost, "shared memory");
+  if constexpr (LrSmem<T, R, 64, BACK>::bytes(2) <= kLrSmemMost) {       // f32 of rank above 64 has too large ones
+    if (g.mode != LR_SELF && each >= 48 && g.n >= 1024) return lr_rows_as<T, R, 64, BACK>(a, st);
+  }
   return lr_rows_as<T, R, 16, BACK>(a, st);
 }
 

@@ -259,9 +259,17 @@ def test_update_places_past_32_bits():
     want = (x[-3:].double() @ a.double().T) @ b.double().T
     want[-1] += 1
     assert float((y[-3:].double() - want).abs().max()) <= float(want.abs().max()) * 2.0 ** -8
-    _, g = TR.low_rank.train_ops.low_rank_rows(y, b[None], a[None], TR.low_rank.train_ops.RowGroups(None, n, 1, True), True, 1.0, 65536, 0, keep=True)
-    want = y[-3:].double() @ b.double()
-    assert float((g[-3:, :8].double() - want).abs().max()) <= float(y[-3:].double().abs().sum(1).max()) * float(b.abs().max()) * cols * 2.0 ** -23
+    dy = torch.zeros(n, 8, dtype=torch.bfloat16, device=DEV)
+    dy[-3:] = torch.randn(3, 8, device=DEV)
+    down, up = b.T.contiguous().requires_grad_(), a.requires_grad_()         # cols to 8
+    y.requires_grad_()
+    z = TR.low_rank_update(y, down, up)
+    dx, da, db = torch.autograd.grad(z, (y, down, up), dy)
+    args = y.detach()[-3:], None, dy[-3:], down.detach()[None], up.detach()[None], torch.ones(1, device=DEV), None
+    want, bound = update_by_formula(*args)
+    for got, w, e, what in zip((z.detach()[-3:], dx[-3:], da[None], db[None]), want, bound, NAMES):
+        within(got, w, e, what)
+    assert not dx[:-3].any()
 
 
 def test_update_refusals_on_the_gpu():
