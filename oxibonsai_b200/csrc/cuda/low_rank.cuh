@@ -25,6 +25,7 @@
 namespace bonsai {
 
 constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
+constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024;        // dynamic shared memory of a block, of each of two on an SM
 constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
 enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
 
@@ -291,7 +292,7 @@ template <typename T, int R, int M, bool BACK> struct LrSmem {
   static constexpr int kJoin = LrShape<M>::kParts * M * R * 4;         // the warps' parts, over the stages
   static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = 2 * M * kPitchH * (int)sizeof(T);
   // what of base is on its way: each lane's own 16 bytes, `kDepth` steps of a warp
-  static constexpr int kDepth = sizeof(T) == 4 ? 2 : M == 16 ? 4 : 3, kPieces = LrShape<M>::kMw * 2 * (int)sizeof(T) / 2;
+  static constexpr int kDepth = sizeof(T) == 4 ? (M == 16 ? 2 : 1) : M == 16 ? 4 : 3, kPieces = LrShape<M>::kMw * 2 * (int)sizeof(T) / 2;
   static constexpr int kBase = BACK ? 0 : kLrWarps * kDepth * kPieces * 512;
   static constexpr int ring(int stages) { return stages * kStage > kJoin ? stages * kStage : kJoin; }
   static constexpr int bytes(int stages) { return ring(stages) + kPart + kH + kBase; }
@@ -727,7 +728,9 @@ template <typename T, int R> struct LrOuterSmem {
   static constexpr int kSizeP = kBf16 ? 2 : 4, kP = kLrOuterRows * kPitchP * kSizeP;            // one part
   static constexpr int kStage = kLrOuterRows * kPitchQ * (int)sizeof(T) + 2 * kP;
   static constexpr int kSum = R * kLrOuterCols * 4;
-  static constexpr int bytes(int stages) { return stages * kStage > kSum ? stages * kStage : kSum; }
+  static constexpr int kStages = 3 * kStage <= kLrSmemMost ? 3 : 2;
+  static constexpr int kBytes = kStages * kStage > kSum ? kStages * kStage : kSum;
+  static_assert(kBytes <= kLrSmemMost, "shared memory");
 };
 
 template <typename T, int R>
@@ -735,7 +738,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
   using L = LrOuterSmem<T, R>;
   constexpr bool F32 = sizeof(T) == 4, BF16 = L::kBf16;
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
-  __shared__ int rows[3][kLrOuterRows];
+  __shared__ int rows[4][kLrOuterRows];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t rank = lr_rank(), ranks = lr_ranks();
@@ -749,16 +752,16 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
   const T* q = (const T*)a.q[which];
   const bool drop = which == 0 && a.drop_x;
   const uint2 key = drop ? philox_key(a.drop) : make_uint2(0, 0);
-  auto list = [&](int s) {          // row numbers of a step, three steps side by side
+  auto list = [&](int s) {          // row numbers of a step, four steps side by side
     if (threadIdx.x < kLrOuterRows) {
       const int place = first + s * kLrOuterRows + threadIdx.x;
-      rows[s % 3][threadIdx.x] = place < last ? (a.groups.mode == LR_PLAN ? a.groups.order[place] : place) : -1;
+      rows[s % 4][threadIdx.x] = place < last ? (a.groups.mode == LR_PLAN ? a.groups.order[place] : place) : -1;
     }
   };
   auto qs = [&](int i) { return reinterpret_cast<T*>(lr_dynamic + i * L::kStage); };
   auto ps = [&](int i) { return lr_dynamic + i * L::kStage + kLrOuterRows * L::kPitchQ * sizeof(T); };
   auto fetch = [&](int s, int slot) {
-    const int* list = rows[s % 3];
+    const int* list = rows[s % 4];
     const int from = first + s * kLrOuterRows;
     lr_fill<T, kLrOuterCols>(qs(slot), L::kPitchQ, kLrOuterRows, col0, width, a.vec[which], q, [&](int r) { return list[r] < 0 ? (const T*)nullptr : q + list[r] * a.ldq[which]; });
     if constexpr (BF16) {
@@ -779,20 +782,19 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.0f;
-  // two stages: the rows of step s + 2 are listed while s is multiplied
-  if (s0 < s1) list(s0);
-  if (s0 + 1 < s1) list(s0 + 1);
+  // a ring of stages that is full but for the one that is multiplied; the rows of the step behind it are listed meanwhile
+  constexpr int kAhead = L::kStages - 1;
+  for (int s = s0; s <= s0 + kAhead && s < s1; ++s) list(s);
   __syncthreads();
-  if (s0 < s1) fetch(s0, 0);
-  lr_commit();
-  for (int s = s0; s < s1; ++s) {
-    const int slot = (s - s0) & 1;
-    if (s + 1 < s1) fetch(s + 1, slot ^ 1);
+  for (int s = s0; s < s0 + kAhead; ++s) {
+    if (s < s1) fetch(s, s - s0);
     lr_commit();
-    if (s + 2 < s1) list(s + 2);
-    lr_wait<1>();
+  }
+  int slot = 0;
+  for (int s = s0; s < s1; ++s, slot = slot == kAhead ? 0 : slot + 1) {
+    lr_wait<kAhead - 1>();
     if (drop) {                     // the eights that this thread copied
-      const int* list = rows[s % 3];
+      const int* list = rows[s % 4];
       for (int u = threadIdx.x; u < kLrOuterRows * (kLrOuterCols / 8); u += kLrThreads) {
         const int r = u / (kLrOuterCols / 8), c = u % (kLrOuterCols / 8) * 8;
         if (list[r] >= 0) lr_drop8<T>(qs(slot) + r * L::kPitchQ + c, dropout_bits((unsigned)(col0 + c) >> 3, list[r], key, a.drop.steps));
@@ -816,6 +818,9 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
       }
     }
     __syncthreads();
+    if (s + kAhead < s1) fetch(s + kAhead, slot == 0 ? kAhead : slot - 1);
+    lr_commit();
+    if (s + kAhead + 1 < s1) list(s + kAhead + 1);
     const T* qp = qs(slot) + warp * 16;
     if constexpr (BF16) {
       const T* pp = (const T*)ps(slot);
@@ -903,7 +908,6 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
             for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[i][j][k];
       }
     }
-    __syncthreads();
   }
   lr_wait<0>();
   __syncthreads();
@@ -967,7 +971,6 @@ inline int lr_ranks_for(long long clusters, long long most) {
   return ranks;
 }
 
-constexpr int kLrSmemMost = 227 * 1024 - 1024;
 
 template <typename T, int R, int M, bool BACK>
 static cudaError_t lr_rows_as(LrRowsArgs a, cudaStream_t st) {
@@ -978,7 +981,7 @@ static cudaError_t lr_rows_as(LrRowsArgs a, cudaStream_t st) {
   const int chunks = (a.k + L::kChunk - 1) / L::kChunk;
   const int ranks = lr_ranks_for(busy < 1 ? 1 : busy, chunks > 1 ? chunks : 1);
   int stages = 4;
-  while (stages > 2 && L::bytes(stages) > (R <= 32 ? 72 * 1024 : kLrSmemMost)) --stages;
+  while (stages > 2 && L::bytes(stages) > (R <= 32 ? kLrSmemHalf : kLrSmemMost)) --stages;
   a.stages = stages;
   if (slots * ranks >= 1ll << 31) return cudaErrorInvalidValue;
   return lr_launch(lr_rows_kernel<T, R, M, BACK>, (int)slots, ranks, L::bytes(stages), st, a);
@@ -1003,7 +1006,7 @@ static cudaError_t lr_outer_r(const LrOuterArgs& a, cudaStream_t st) {
   const long long steps = (a.groups.n / a.groups.adapters + kLrOuterRows - 1) / kLrOuterRows;
   const int ranks = lr_ranks_for(clusters / 2, steps > 1 ? steps : 1);          // four blocks an SM: they are short
   if (clusters * ranks >= 1ll << 31) return cudaErrorInvalidValue;
-  return lr_launch(lr_outer_kernel<T, R>, (int)clusters, ranks, L::bytes(2), st, a);
+  return lr_launch(lr_outer_kernel<T, R>, (int)clusters, ranks, L::kBytes, st, a);
 }
 
 inline int lr_padded(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
