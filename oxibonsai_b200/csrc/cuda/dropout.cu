@@ -49,6 +49,18 @@ __device__ __forceinline__ void pack(Eight<__nv_bfloat16>& v, const float* f) {
   v.a = *reinterpret_cast<const uint4*>(h);
 }
 
+__device__ __forceinline__ void mask(Eight<float>& v, const uint4& words, unsigned limit) {
+  v.a.x = dropout_keeps(words, 0, limit) ? v.a.x : 0.0f; v.a.y = dropout_keeps(words, 1, limit) ? v.a.y : 0.0f;
+  v.a.z = dropout_keeps(words, 2, limit) ? v.a.z : 0.0f; v.a.w = dropout_keeps(words, 3, limit) ? v.a.w : 0.0f;
+  v.b.x = dropout_keeps(words, 4, limit) ? v.b.x : 0.0f; v.b.y = dropout_keeps(words, 5, limit) ? v.b.y : 0.0f;
+  v.b.z = dropout_keeps(words, 6, limit) ? v.b.z : 0.0f; v.b.w = dropout_keeps(words, 7, limit) ? v.b.w : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ void mask(Eight<T>& v, const uint4& words, unsigned limit) {
+  v.a.x = dropout_pair(v.a.x, words.x, limit); v.a.y = dropout_pair(v.a.y, words.y, limit);
+  v.a.z = dropout_pair(v.a.z, words.z, limit); v.a.w = dropout_pair(v.a.w, words.w, limit);
+}
+
 template <typename T> __device__ __forceinline__ float one_of(T v);
 template <> __device__ __forceinline__ float one_of(float v) { return v; }
 template <> __device__ __forceinline__ float one_of(__half v) { return __half2float(v); }
@@ -89,13 +101,14 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* __restri
         if (p[u].row < rows) v[u] = *reinterpret_cast<const Eight<T>*>(x + p[u].row * ldx + 8ll * p[u].group);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const unsigned keep = dropout_bits(p[u].group, p[u].row, key, rule.steps);
+        const uint4 words = dropout_words(p[u].group, p[u].row, key);
         if (p[u].row < rows) {
           float f[8];
           unpack(v[u], f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = (keep >> j & 1u) ? f[j] * rule.share : 0.0f;
+          for (int j = 0; j < 8; ++j) f[j] = f[j] * rule.share;
           pack(v[u], f);
+          mask(v[u], words, rule.limit);
           *reinterpret_cast<Eight<T>*>(y + p[u].row * (long long)d + 8ll * p[u].group) = v[u];
         }
       }
@@ -103,12 +116,13 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* __restri
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (p[u].row >= rows) continue;
-        const unsigned keep = dropout_bits(p[u].group, p[u].row, key, rule.steps), c = 8u * p[u].group, n = d - c < 8u ? d - c : 8u;
+        const uint4 words = dropout_words(p[u].group, p[u].row, key);
+        const unsigned c = 8u * p[u].group, n = d - c < 8u ? d - c : 8u;
         const T* from = x + p[u].row * ldx + c;
         T* to = y + p[u].row * (long long)d + c;
 #pragma unroll
         for (unsigned j = 0; j < 8; ++j)
-          if (j < n) put(to + j, (keep >> j & 1u) ? one_of<T>(from[j]) * rule.share : 0.0f);
+          if (j < n) put(to + j, dropout_keeps(words, j, rule.limit) ? one_of<T>(from[j]) * rule.share : 0.0f);
       }
     }
   }
@@ -132,14 +146,15 @@ static cudaError_t dropout_launch(const T* x, long long ldx, T* y, long long row
 
 extern "C" {
 
-// x: rows of d values (type 0 f32, 1 f16, 2 bf16) at distances of ldx; y: the same rows side by side.  seed_dev, where given, holds the seed.
+// x: rows of d values (type 0 f32, 1 f16, 2 bf16) at distances of ldx; y: the same rows side by side.  steps: of 65536 values that many
+// stay, less than all.  seed_dev, where given, holds the seed.
 int bonsai_dropout(const void* x, long long ldx, void* y, long long rows, long long d, int type, unsigned long long seed, const long long* seed_dev,
                    int steps, cudaStream_t st) {
   using namespace bonsai;
   if (x == nullptr || y == nullptr || rows < 1 || d < 1 || d >= 1ll << 31 || rows >= 1ll << 40 || rows > (1ll << 62) / d || type < 0 || type > 2 ||
-      steps < 0 || steps > 65536)
+      steps < 0 || steps > 65535)
     return BONSAI_CUDA_BAD_ARG;
-  const DropoutRule rule = {seed, seed_dev, (unsigned)steps, steps > 0 ? 65536.0f / (float)steps : 0.0f};
+  const DropoutRule rule = dropout_rule(seed, seed_dev, steps);
   cudaError_t e;
   if (type == 0) e = dropout_launch((const float*)x, ldx, (float*)y, rows, (unsigned)d, rule, st);
   else if (type == 1) e = dropout_launch((const __half*)x, ldx, (__half*)y, rows, (unsigned)d, rule, st);

@@ -62,10 +62,6 @@ static bool lr_groups_good(const LrGroups& g) {
 }
 // rows of `width` values at distances of ld that begin at multiples of 16 bytes and hold whole eights
 static int lr_vec(const void* p, long long ld, long long width, int size) { return width % 8 == 0 && ((uintptr_t)p | (uintptr_t)(ld * size)) % 16 == 0; }
-static DropoutRule lr_rule(unsigned long long seed, const long long* seed_dev, int steps) {
-  return {seed, seed_dev, (unsigned)steps, steps > 0 ? 65536.0f / (float)steps : 0.0f};
-}
-
 }  // namespace bonsai
 
 extern "C" {
@@ -105,7 +101,7 @@ int bonsai_lr_rows(const void* x, long long ldx, const void* w1, const void* w2,
   // forward: rank values of a column as words of 8 bytes
   a.vec_w2 = back ? lr_vec(w2, cols, cols, size) : rank % (8 / size) == 0 && (uintptr_t)w2 % 8 == 0;
   a.vec_y = lr_vec(y, ldy, cols, size) && (base == nullptr || lr_vec(base, ld_base, cols, size));
-  a.drop = lr_rule(seed, seed_dev, steps);
+  a.drop = dropout_rule(seed, seed_dev, steps);
   a.drop_x = drop && !back;
   a.drop_y = drop && back;
   const cudaError_t e = type == 0 ? lr_rows<float>(a, back, st) : type == 1 ? lr_rows<__half>(a, back, st) : lr_rows<__nv_bfloat16>(a, back, st);
@@ -131,7 +127,7 @@ int bonsai_lr_outer(const void* x, long long ldx, const void* g, void* da, int d
   a.rank = rank;
   a.scales = scales;
   a.scale = scale;
-  a.drop = lr_rule(seed, seed_dev, steps);
+  a.drop = dropout_rule(seed, seed_dev, steps);
   a.drop_x = steps < 65536;
   const cudaError_t e = type == 0 ? lr_outer<float>(a, st) : type == 1 ? lr_outer<__half>(a, st) : lr_outer<__nv_bfloat16>(a, st);
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;

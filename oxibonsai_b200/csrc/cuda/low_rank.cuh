@@ -48,7 +48,6 @@ struct LrRowsArgs {
   const float* scales;                   // of the adapters, or null: scale
   float scale;
   int k, cols, rank;
-  int stages;
   int vec_x, vec_w1, vec_w2, vec_y;      // rows that 16-byte (w2 of the forward pass: 4-byte) accesses may take
   DropoutRule drop;
   int drop_x, drop_y;                    // forward: the rows of x; backward: those of dx
@@ -83,6 +82,23 @@ template <> __device__ __forceinline__ float2 lr_pair<__half>(uint32_t w) { retu
 template <> __device__ __forceinline__ float2 lr_pair<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 lr_pair<float>(uint32_t w) { return make_float2(__uint_as_float(w), 0.0f); }     // not used
 
+// two values rounded into a word
+template <typename T> __device__ __forceinline__ uint32_t lr_two(float a, float b);
+template <> __device__ __forceinline__ uint32_t lr_two<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t lr_two<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// a * s + c of two values at once
+__device__ __forceinline__ void lr_fma2(float* a, float s, const float* c) {
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %2};\nmov.b64 z, {%3, %4};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "+f"(a[0]), "+f"(a[1])
+      : "f"(s), "f"(c[0]), "f"(c[1]));
+}
+
 // eight neighbouring values
 template <typename T, bool VEC>
 __device__ __forceinline__ void lr_load8(const T* p, int n, float* v) {
@@ -107,11 +123,12 @@ __device__ __forceinline__ void lr_load8(const T* p, int n, float* v) {
 template <typename T, bool VEC>
 __device__ __forceinline__ void lr_store8(T* p, int n, const float* v) {
   if (VEC) {
-    __align__(16) T t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = lr_round<T>(v[i]);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(lr_two<T>(v[0], v[1]), lr_two<T>(v[2], v[3]), lr_two<T>(v[4], v[5]), lr_two<T>(v[6], v[7]));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -124,34 +141,33 @@ __device__ __forceinline__ uint32_t lr_smem(const void* p) { return (uint32_t)__
 __device__ __forceinline__ void lr_copy16(void* dst, const void* src, bool there) {       // zeros where it is not there
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(lr_smem(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void lr_copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(lr_smem(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void lr_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void lr_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// waits until at most `left` of the latest groups are in flight
-__device__ __forceinline__ void lr_wait_left(int left) {
-  if (left <= 0) lr_wait<0>();
-  else if (left == 1) lr_wait<1>();
-  else if (left == 2) lr_wait<2>();
-  else lr_wait<3>();
-}
 __device__ __forceinline__ void lr_ldm4(uint32_t* r, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(lr_smem(p)) : "memory");
 }
 __device__ __forceinline__ void lr_ldm4t(uint32_t* r, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(lr_smem(p)) : "memory");
 }
-template <typename T> __device__ __forceinline__ void lr_mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void lr_mma16<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + d, or a b
+#define LR_MMA(name, shape, types)                                                                                                     \
+  __device__ __forceinline__ void name(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool start) {                                  \
+    const float c0 = start ? 0.0f : d[0], c1 = start ? 0.0f : d[1], c2 = start ? 0.0f : d[2], c3 = start ? 0.0f : d[3];                      \
+    asm volatile("mma.sync.aligned." shape ".row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"            \
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                                            \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));                        \
+  }
+LR_MMA(lr_mma_f16, "m16n8k16", "f16.f16")
+LR_MMA(lr_mma_bf16, "m16n8k16", "bf16.bf16")
+LR_MMA(lr_mma_tf32, "m16n8k8", "tf32.tf32")
+#undef LR_MMA
+template <typename T>
+__device__ __forceinline__ void lr_mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool start = false) {
+  if constexpr (std::is_same<T, __half>::value) lr_mma_f16(d, a, b0, b1, start);
+  else lr_mma_bf16(d, a, b0, b1, start);
 }
-template <> __device__ __forceinline__ void lr_mma16<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void lr_mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
+__device__ __forceinline__ void lr_mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool start = false) { lr_mma_tf32(d, a, b0, b1, start); }
 __device__ __forceinline__ uint32_t lr_tf32(float v) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
@@ -232,36 +248,35 @@ __device__ __forceinline__ LrTile lr_tile(const LrGroups& g, int slot, int* rows
   return tile;
 }
 
-// Eight values of a row in shared memory, those without a bit set to 0; what stays is scaled behind the sums.  The thread that copied them calls it.
+// Eight values of a row in shared memory, those that dropout takes set to 0; what stays is scaled behind the sums.  The thread that copied them calls it.
 template <typename T>
-__device__ __forceinline__ void lr_drop8(T* p, unsigned bits) {
+__device__ __forceinline__ void lr_drop8(T* p, const uint4& words, unsigned limit) {
   if constexpr (sizeof(T) == 4) {
-    float4* v = reinterpret_cast<float4*>(p);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float4 f = v[h];
-      f.x = bits >> (4 * h) & 1u ? f.x : 0.0f; f.y = bits >> (4 * h + 1) & 1u ? f.y : 0.0f;
-      f.z = bits >> (4 * h + 2) & 1u ? f.z : 0.0f; f.w = bits >> (4 * h + 3) & 1u ? f.w : 0.0f;
-      v[h] = f;
+      float4 f = reinterpret_cast<float4*>(p)[h];
+      f.x = dropout_keeps(words, 4 * h, limit) ? f.x : 0.0f; f.y = dropout_keeps(words, 4 * h + 1, limit) ? f.y : 0.0f;
+      f.z = dropout_keeps(words, 4 * h + 2, limit) ? f.z : 0.0f; f.w = dropout_keeps(words, 4 * h + 3, limit) ? f.w : 0.0f;
+      reinterpret_cast<float4*>(p)[h] = f;
     }
   } else {
     uint4 w = *reinterpret_cast<uint4*>(p);
-    auto both = [&](int i) { return (bits >> i & 1u ? 0xffffu : 0u) | (bits >> (i + 1) & 1u ? 0xffff0000u : 0u); };
-    w.x &= both(0); w.y &= both(2); w.z &= both(4); w.w &= both(6);
+    w.x = dropout_pair(w.x, words.x, limit); w.y = dropout_pair(w.y, words.y, limit);
+    w.z = dropout_pair(w.z, words.z, limit); w.w = dropout_pair(w.w, words.w, limit);
     *reinterpret_cast<uint4*>(p) = w;
   }
 }
 
-// Eight values at column `c` of a row of `width` (null: none) into shared memory, zeros behind the row's end.
+// Eight values into shared memory, of which `left` are there, zeros for the others (all of them or none where `vec`).  any: a readable address.
 template <typename T>
-__device__ __forceinline__ void lr_copy8(T* dst, const T* src, int c, int width, bool vec, const T* any) {
-  const int left = src != nullptr ? width - c : 0;
+__device__ __forceinline__ void lr_copy8(T* dst, const T* src, int left, bool vec, const T* any) {
   if (vec) {
+    if (left <= 0) src = any;
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(dst + i * (16 / sizeof(T)), left > 0 ? src + c + i * (16 / sizeof(T)) : any, left > 0);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(dst + i * (16 / sizeof(T)), src + (left > 0 ? i * (16 / (int)sizeof(T)) : 0), left > 0);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dst[i] = i < left ? src[c + i] : lr_round<T>(0.0f);
+    for (int i = 0; i < 8; ++i) dst[i] = i < left ? src[i] : lr_round<T>(0.0f);
   }
 }
 
@@ -271,7 +286,8 @@ template <typename T, int C, typename From>
 __device__ __forceinline__ void lr_fill(T* to, int pitch, int nrows, int c0, int width, bool vec, const T* any, From from) {
   for (int u = threadIdx.x; u < nrows * (C / 8); u += kLrThreads) {
     const int r = u / (C / 8), c = u % (C / 8) * 8;
-    lr_copy8<T>(to + r * pitch + c, from(r), c0 + c, width, vec, any);
+    const T* src = from(r);
+    lr_copy8<T>(to + r * pitch + c, src + c0 + c, src != nullptr ? width - c0 - c : 0, vec, any);
   }
 }
 
@@ -294,8 +310,11 @@ template <typename T, int R, int M, bool BACK> struct LrSmem {
   // what of base is on its way: each lane's own 16 bytes, `kDepth` steps of a warp
   static constexpr int kDepth = sizeof(T) == 4 ? (M == 16 ? 2 : 1) : M == 16 ? 4 : 3, kPieces = LrShape<M>::kMw * 2 * (int)sizeof(T) / 2;
   static constexpr int kBase = BACK ? 0 : kLrWarps * kDepth * kPieces * 512;
+  // as many stages as leave room for two blocks on an SM, or one where the rank is large
+  static constexpr int kMost = R <= 32 ? kLrSmemHalf : kLrSmemMost;
   static constexpr int ring(int stages) { return stages * kStage > kJoin ? stages * kStage : kJoin; }
   static constexpr int bytes(int stages) { return ring(stages) + kPart + kH + kBase; }
+  static constexpr int kStages = bytes(4) <= kMost ? 4 : bytes(3) <= kMost ? 3 : 2, kRing = ring(kStages), kBytes = bytes(kStages);
 };
 
 template <typename T, int R, int M, bool BACK>
@@ -309,7 +328,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
   __shared__ int scratch[kLrWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  unsigned char* behind = lr_dynamic + L::ring(a.stages);
+  unsigned char* behind = lr_dynamic + L::kRing;
   float* join = reinterpret_cast<float*>(lr_dynamic);
   float* part = reinterpret_cast<float*>(behind);
   T* hs = reinterpret_cast<T*>(behind + L::kPart);                   // first parts, then second parts
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int v = 0; v < (int)sizeof(T) / 2; ++v)
-              if (live[m][h]) lr_copy16(to + ((m * 2 + h) * ((int)sizeof(T) / 2) + v) * 32, (const T*)a.base + at_base[m][h] + col + v * (16 / (int)sizeof(T)), true);
+              if (live[m][h]) lr_copy16(to + ((m * 2 + h) * ((int)sizeof(T) / 2) + v) * 32, (const T*)a.base + at_base[m][h] + col + v * (16 / (int)sizeof(T)));
       }
     }
   };
@@ -369,20 +388,20 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
 #pragma unroll
     for (int i = 0; i < kX; ++i) {
       from_row[i] = rows[xr + i * kRowStep];
-      from[i] = from_row[i] < 0 ? (const T*)nullptr : (const T*)a.x + from_row[i] * a.ldx;
+      from[i] = (const T*)a.x + (from_row[i] < 0 ? rows[0] : from_row[i]) * a.ldx + xc;        // rows behind the last: any, their results go nowhere
     }
     auto fetch = [&](int c, int slot) {
       T* xs = stage(slot);
       T* ws = xs + M * L::kPitchX;
       const int k0 = c * S::kChunk;
 #pragma unroll
-      for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i], k0 + xc, a.k, a.vec_x, (const T*)a.x);
+      for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i] + k0, a.k - k0 - xc, a.vec_x, (const T*)a.x);
 #pragma unroll
       for (int i = 0; i < kW; ++i) {
         const int r = wr + i * kStepW;
         if (kUnitsW % kLrThreads != 0 && r >= L::kRowsW) break;
-        if (BACK) lr_copy8<T>(ws + r * L::kPitchW + wc, k0 + r < a.k ? w1 + (long long)(k0 + r) * a.rank : (const T*)nullptr, wc, a.rank, a.vec_w1, w1);
-        else lr_copy8<T>(ws + r * L::kPitchW + wc, r < a.rank ? w1 + (long long)r * a.k : (const T*)nullptr, k0 + wc, a.k, a.vec_w1, w1);
+        if (BACK) lr_copy8<T>(ws + r * L::kPitchW + wc, w1 + (long long)(k0 + r) * a.rank + wc, k0 + r < a.k ? a.rank - wc : 0, a.vec_w1, w1);
+        else lr_copy8<T>(ws + r * L::kPitchW + wc, w1 + (long long)r * a.k + k0 + wc, r < a.rank ? a.k - k0 - wc : 0, a.vec_w1, w1);
       }
     };
     float acc[R / 8][4];
@@ -391,9 +410,9 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
     const int m0 = warp % S::kM16 * 16, kp = warp / S::kM16 * S::kWarpK;
-    for (int i = 0; i < a.stages - 1; ++i) {
+    for (int i = 0; i < L::kStages - 1; ++i) {
       if (c0 + i < c1) fetch(c0 + i, i);
-      if (i == a.stages - 2) {
+      if (i == L::kStages - 2) {
 #pragma unroll
         for (int d = 0; d < L::kDepth; ++d) request(d);
       }
@@ -401,16 +420,16 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
     }
     int slot = 0;
     for (int c = c0; c < c1; ++c) {
-      lr_wait_left(a.stages - 2);
+      lr_wait<L::kStages - 2>();
       T* xs = stage(slot);
       if (a.drop_x) {
 #pragma unroll
         for (int i = 0; i < kX; ++i)
           if (from_row[i] >= 0)
-            lr_drop8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, dropout_bits((unsigned)(c * S::kChunk + xc) >> 3, from_row[i], key, a.drop.steps));
+            lr_drop8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, dropout_words((unsigned)(c * S::kChunk + xc) >> 3, from_row[i], key), a.drop.limit);
       }
       __syncthreads();
-      if (c + a.stages - 1 < c1) fetch(c + a.stages - 1, slot == 0 ? a.stages - 1 : slot - 1);
+      if (c + L::kStages - 1 < c1) fetch(c + L::kStages - 1, slot == 0 ? L::kStages - 1 : slot - 1);
       lr_commit();
       const T* ws = xs + M * L::kPitchX;
       if constexpr (!F32) {
@@ -457,7 +476,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[j][i] += sum[j][i];
       }
-      slot = slot + 1 == a.stages ? 0 : slot + 1;
+      slot = slot + 1 == L::kStages ? 0 : slot + 1;
     }
     lr_wait<0>();
     __syncthreads();                                   // the stages are read: the warps' parts go over them
@@ -546,13 +565,14 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
   // Of the rank values the thread has 4 t .. 4 t + 3 of every sixteen (f32: 2 t and 2 t + 1 of every eight): the axis of a product may be taken in any order, and
   // so its factors lie side by side.
   constexpr int kStep = F32 ? 8 : 16, kEach = kStep / 4;
+  const T* w2t = BACK ? w2 + (long long)(kEach * t) * a.cols + 8 * (g >> 1) : w2 + (long long)(8 * (g >> 1) + (g & 1)) * a.rank + kEach * t;
   auto load_w = [&](int b, int k, uint32_t (*w)[2]) {
     const int wc = b * 32 + 8 * (g >> 1), kk = k + kEach * t;      // eight columns, of which this thread takes every second
     if (BACK) {
       uint32_t v[kEach][F32 ? 8 : 4];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const T* p = w2 + (long long)(kk + i) * a.cols + wc;
+        const T* p = w2t + (long long)(k + i) * a.cols + b * 32;
         const bool there = kk + i < a.rank && wc < a.cols;
         if (a.vec_w2) {
 #pragma unroll
@@ -580,10 +600,11 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
         }
       }
     } else {
+      const T* first = w2t + (long long)b * 32 * a.rank + k;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int cc = wc + 2 * j + (g & 1);
-        const T* p = w2 + (long long)cc * a.rank + kk;
+        const T* p = first + 2 * j * a.rank;
         if (a.vec_w2) {
           const uint2 u = cc < a.cols && kk < a.rank ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
           w[j][0] = u.x; w[j][1] = u.y;
@@ -602,7 +623,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
     const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(p + 8 * L::kPitchH);
     h[0] = u.x; h[1] = v.x; h[2] = u.y; h[3] = v.y;
   };
-  const float by = a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale;
+  const float by = (a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale) * (a.drop_y ? a.drop.share : 1.0f);
   float scaled[S::kMw][2];
 #pragma unroll
   for (int m = 0; m < S::kMw; ++m)
@@ -624,14 +645,8 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
   for (int i = 0; b < b1; b += S::kAcross, ++i) {
     const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
     float acc[S::kMw][4][4];
-#pragma unroll
-    for (int m = 0; m < S::kMw; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][j][q] = 0.0f;
     if (has) {
-      auto multiply = [&](uint32_t (*w)[2], auto h) {
+      auto multiply = [&](uint32_t (*w)[2], auto h, bool start) {
 #pragma unroll
         for (int m = 0; m < S::kMw; ++m)
 #pragma unroll
@@ -640,11 +655,11 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
               uint32_t h0, l0, h1, l1;
               lr_split(__uint_as_float(w[j][0]), h0, l0);
               lr_split(__uint_as_float(w[j][1]), h1, l1);
-              lr_mma8(acc[m][j], h(m, 1), h0, h1);
+              lr_mma8(acc[m][j], h(m, 1), h0, h1, start);
               lr_mma8(acc[m][j], h(m, 0), l0, l1);
               lr_mma8(acc[m][j], h(m, 0), h0, h1);
             } else {
-              lr_mma16<T>(acc[m][j], h(m, 1), w[j][0], w[j][1]);
+              lr_mma16<T>(acc[m][j], h(m, 1), w[j][0], w[j][1], start);
               lr_mma16<T>(acc[m][j], h(m, 0), w[j][0], w[j][1]);
             }
           }
@@ -658,7 +673,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
           if (b + S::kAcross < b1) load_w(b + S::kAcross, k * kStep, next[k]);
         }
 #pragma unroll
-        for (int k = 0; k < R / kStep; ++k) multiply(w[k], [&](int m, int p) -> const uint32_t* { return held[k][m][p]; });
+        for (int k = 0; k < R / kStep; ++k) multiply(w[k], [&](int m, int p) -> const uint32_t* { return held[k][m][p]; }, k == 0);
       } else {
 #pragma unroll 2
         for (int k = 0; k < R; k += kStep) {
@@ -669,7 +684,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
           for (int m = 0; m < S::kMw; ++m)
 #pragma unroll
             for (int p = 0; p < 2; ++p) load_h(m, k, p, hv[m][p]);
-          multiply(w, [&](int m, int p) -> const uint32_t* { return hv[m][p]; });
+          multiply(w, [&](int m, int p) -> const uint32_t* { return hv[m][p]; }, k == 0);
         }
       }
     }
@@ -694,12 +709,16 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
           }
         }
         if (has) {
-          const unsigned keep = BACK && a.drop_y ? dropout_bits((unsigned)col >> 3, rows[me + m * 16 + h * 8 + g], key, a.drop.steps) : 0xffu;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float d = acc[m][q >> 1][2 * h + (q & 1)] * scaled[m][h];
-            if (BACK) v[q] = a.drop_y ? (keep >> q & 1u ? d * a.drop.share : 0.0f) : d;
-            else v[q] += d;
+          for (int q = 0; q < 8; q += 2) {
+            float* d = &acc[m][q >> 1][2 * h];
+            lr_fma2(d, scaled[m][h], v + q);
+            v[q] = d[0]; v[q + 1] = d[1];
+          }
+          if (BACK && a.drop_y) {
+            const uint4 words = dropout_words((unsigned)col >> 3, rows[me + m * 16 + h * 8 + g], key);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = dropout_keeps(words, q, a.drop.limit) ? v[q] : 0.0f;
           }
         } else if (tile.group > a.groups.adapters) {
 #pragma unroll
@@ -797,7 +816,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
       const int* list = rows[s % 4];
       for (int u = threadIdx.x; u < kLrOuterRows * (kLrOuterCols / 8); u += kLrThreads) {
         const int r = u / (kLrOuterCols / 8), c = u % (kLrOuterCols / 8) * 8;
-        if (list[r] >= 0) lr_drop8<T>(qs(slot) + r * L::kPitchQ + c, dropout_bits((unsigned)(col0 + c) >> 3, list[r], key, a.drop.steps));
+        if (list[r] >= 0) lr_drop8<T>(qs(slot) + r * L::kPitchQ + c, dropout_words((unsigned)(col0 + c) >> 3, list[r], key), a.drop.limit);
       }
     }
     if constexpr (!BF16) {          // and its rank values into two parts
@@ -980,11 +999,8 @@ static cudaError_t lr_rows_as(LrRowsArgs a, cudaStream_t st) {
   const long long busy = g.mode == LR_ONE ? slots : g.n / M + (g.n < g.adapters ? g.n : g.adapters);
   const int chunks = (a.k + L::kChunk - 1) / L::kChunk;
   const int ranks = lr_ranks_for(busy < 1 ? 1 : busy, chunks > 1 ? chunks : 1);
-  int stages = 4;
-  while (stages > 2 && L::bytes(stages) > (R <= 32 ? kLrSmemHalf : kLrSmemMost)) --stages;
-  a.stages = stages;
   if (slots * ranks >= 1ll << 31) return cudaErrorInvalidValue;
-  return lr_launch(lr_rows_kernel<T, R, M, BACK>, (int)slots, ranks, L::bytes(stages), st, a);
+  return lr_launch(lr_rows_kernel<T, R, M, BACK>, (int)slots, ranks, L::kBytes, st, a);
 }
 
 template <typename T, int R, bool BACK>
@@ -992,8 +1008,8 @@ static cudaError_t lr_rows_r(const LrRowsArgs& a, cudaStream_t st) {
   const LrGroups& g = a.groups;
   // Tiles of 64 rows where adapters fill them; 16 rows keep more clusters busy and waste less of the tiles
   const long long each = g.mode == LR_ONE ? g.n : g.n / (g.adapters > 0 ? g.adapters : 1);
-  static_assert(LrSmem<T, R, 16, BACK>::bytes(2) <= kLrSmemMost, "shared memory");
-  if constexpr (LrSmem<T, R, 64, BACK>::bytes(2) <= kLrSmemMost) {       // f32 of rank above 64 has too large ones
+  static_assert(LrSmem<T, R, 16, BACK>::kBytes <= kLrSmemMost, "shared memory");
+  if constexpr (LrSmem<T, R, 64, BACK>::kBytes <= kLrSmemMost) {       // f32 of rank above 64 has too large ones
     if (g.mode != LR_SELF && each >= 48 && g.n >= 1024) return lr_rows_as<T, R, 64, BACK>(a, st);
   }
   return lr_rows_as<T, R, 16, BACK>(a, st);

@@ -3,7 +3,7 @@
 // Dropout over rows of d values takes its bits from the counter (column / 8, 0, row, row >> 32) under the seed as key: 128 bits for eight
 // neighbouring values, 16 for each (value j of the eight has bits 16 (j % 2) of word j / 2).  A value stays where its 16 bits are below
 // `steps` of 65536, so that the probability has steps of 2^-16, and what stays is multiplied by 65536 / steps: the mean is kept exactly.  32
-// bits for a value would take twice the multiplications, which are what bounds the kernels that make masks (see dropout.cu).
+// bits for a value would take twice the instructions, which are what bounds the kernels that make masks (see dropout.cu).
 #pragma once
 #include <stdint.h>
 
@@ -12,9 +12,13 @@ namespace bonsai {
 struct DropoutRule {
   unsigned long long seed;
   const long long* seed_dev;     // given: read in place of `seed` when the kernel runs
-  unsigned steps;                // of 65536; 65536 keeps everything
+  unsigned limit;                // steps of 65536, below 65536, in the upper half
   float share;                   // 65536 / steps, 0 where nothing stays
 };
+
+inline DropoutRule dropout_rule(unsigned long long seed, const long long* seed_dev, int steps) {
+  return {seed, seed_dev, steps < 65536 ? (unsigned)steps << 16 : 0u, steps > 0 ? 65536.0f / (float)steps : 0.0f};
+}
 
 __device__ __forceinline__ uint2 philox_key(const DropoutRule& rule) {
   const unsigned long long s = rule.seed_dev != nullptr ? (unsigned long long)*rule.seed_dev : rule.seed;
@@ -32,14 +36,18 @@ __device__ __forceinline__ uint4 philox(uint4 c, uint2 k) {
   return c;
 }
 
-// Bit j: whether value 8 * group + j of a row stays.
-__device__ __forceinline__ unsigned dropout_bits(unsigned group, unsigned long long row, uint2 key, unsigned steps) {
-  const uint4 r = philox(make_uint4(group, 0u, (unsigned)row, (unsigned)(row >> 32)), key);
-  const unsigned w[4] = {r.x, r.y, r.z, r.w};
-  unsigned bits = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) bits |= (((j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu) < steps ? 1u : 0u) << j;
-  return bits;
+// The random words of values 8 * group .. 8 * group + 7 of a row, and whether value j of them stays.
+__device__ __forceinline__ uint4 dropout_words(unsigned group, unsigned long long row, uint2 key) {
+  return philox(make_uint4(group, 0u, (unsigned)row, (unsigned)(row >> 32)), key);
+}
+__device__ __forceinline__ bool dropout_keeps(const uint4& words, int j, unsigned limit) {
+  const unsigned w = j < 2 ? words.x : j < 4 ? words.y : j < 6 ? words.z : words.w;
+  return (j & 1 ? w : w << 16) < limit;
+}
+// Two 16-bit values in a word, those that do not stay set to 0; `random`: their 32 bits.
+__device__ __forceinline__ unsigned dropout_pair(unsigned two, unsigned random, unsigned limit) {
+  two = random << 16 < limit ? two : two & 0xffff0000u;
+  return random < limit ? two : two & 0xffffu;
 }
 
 }  // namespace bonsai

@@ -81,7 +81,7 @@ class _Dropout(torch.autograd.Function):
 
 def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = None, training: bool = True) -> torch.Tensor:
     """``x`` [..., d] with each value set to 0 with probability ``p`` and the others scaled by ``1 / (1 - p)``.  ``p`` is taken in steps of
-    2^-16, and so is the scale that goes with it.  A value that is dropped is 0 whatever it holds, and so is its gradient.
+    2^-16, and so is the scale that goes with it; where it is 0 then, ``x`` itself comes back.  A value that is dropped is 0 whatever it holds, and so is its gradient.
 
     ``seed``: an integer, or an int64 tensor on the device of ``x``, which is read when the kernel runs: a captured graph takes a new mask
     in each replay if the program changes the tensor in between (not between a pass and its backward pass, where autograd reports the change).
@@ -98,6 +98,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = N
     if x.shape[-1] >= 2 ** 31:
         raise ValueError(f"dropout: rows of less than 2^31 values are wanted, got {x.shape[-1]}")
     seed = check_seed(seed, x.device, "dropout") if seed is not None or (training and p > 0.0) else 0
-    if not training or p == 0.0 or x.numel() == 0:
+    steps = keep_steps(p)
+    if not training or steps == 65536 or x.numel() == 0:
         return x
-    return _Dropout.apply(x, keep_steps(p), seed)
+    return _Dropout.apply(x, steps, seed)
