@@ -198,8 +198,7 @@ __global__ void __launch_bounds__(kTuneThreads) policy_kernel(PolicyArgs a) {
 enum TuneReduction { TUNE_TOKENS = 0, TUNE_SEQUENCES = 1, TUNE_SUM = 2, TUNE_NONE = 3 };
 
 // Adds the chunks up; weight[row] is what a token's loss counts in the whole.  One block.
-__global__ void __launch_bounds__(kTuneFinish) policy_finish_kernel(TuneShape sh, const TunePart* part, int reduction, float* loss, float* kl, float* clipped,
-                                                                    float* weight) {
+__global__ void __launch_bounds__(kTuneFinish) policy_finish_kernel(TuneShape sh, const TunePart* part, int reduction, float* loss, float* stats, float* weight) {
   __shared__ double sd[kTuneFinish / 32];
   __shared__ long long sl[kTuneFinish / 32];
   __shared__ long long counts[2];
@@ -231,8 +230,8 @@ __global__ void __launch_bounds__(kTuneFinish) policy_finish_kernel(TuneShape sh
   if (threadIdx.x == 0) {
     const double n = (double)live;              // 0 / 0 is NaN: the mean of no tokens
     if (loss != nullptr) *loss = (float)(reduction == TUNE_TOKENS ? sum / n : reduction == TUNE_SEQUENCES ? means / (double)filled : sum);
-    *kl = (float)(kls / n);
-    *clipped = (float)((double)cut / n);
+    stats[0] = (float)(kls / n);
+    stats[1] = (float)((double)cut / n);
     counts[0] = live;
     counts[1] = filled;
   }
@@ -385,6 +384,18 @@ static bool tune_good(long long rows, long long length) {
 }
 static TuneShape tune_shape(long long rows, long long length) { return {rows, (int)length, tune_chunks(length)}; }
 
+// What a forward pass keeps: the chunks' sums, then where a gradient is wanted the weights of rows and the slopes (1: of rows, without weights; 2: of tokens).
+struct TuneKept {
+  long long weight, slope, bytes;
+};
+static TuneKept tune_kept(long long rows, long long length, int slopes) {
+  TuneKept k;
+  k.weight = (rows * tune_chunks(length) * (long long)sizeof(TunePart) + 15) / 16 * 16;
+  k.slope = k.weight + (slopes == 2 ? (rows * 4 + 15) / 16 * 16 : 0);
+  k.bytes = k.slope + (slopes == 2 ? rows * length * 4 : slopes == 1 ? rows * 4 : 0);
+  return k;
+}
+
 // Whether four neighbouring tokens of every row are one aligned access; an absent array does not matter.
 static bool tune_wide(const void* p, long long ld, int size) { return p == nullptr || (((uintptr_t)p | (uintptr_t)(ld * size)) % (4 * size) == 0); }
 
@@ -393,28 +404,30 @@ static bool tune_wide(const void* p, long long ld, int size) { return p == nullp
 
 extern "C" {
 
-// Bytes of workspace that both losses need for rows of `length` tokens; negative for sizes that are refused.
-long long bonsai_tune_bytes(long long rows, long long length) {
+// Bytes that a forward pass over rows of `length` tokens keeps; slopes: 0 where no gradient is wanted, 1 preference, 2 policy.  Negative for sizes that are
+// refused.
+long long bonsai_tune_bytes(long long rows, long long length, int slopes) {
   using namespace bonsai;
-  return tune_good(rows, length) ? rows * tune_chunks(length) * (long long)sizeof(TunePart) : BONSAI_CUDA_BAD_ARG;
+  return tune_good(rows, length) ? tune_kept(rows, length, slopes).bytes : BONSAI_CUDA_BAD_ARG;
 }
 
 // logps, old, ref: rows of tokens at distances of their ld (type 0 f32, 1 f16, 2 bf16), mask: bytes; old, ref and mask may be null.  gain: f32, for a
-// row or for a token.  reduction: TuneReduction.  Out: loss (f32, or [rows][length]), kl, clipped (f32), and where a gradient is wanted slope
-// [rows][length] and weight [rows].
+// row or for a token.  reduction: TuneReduction.  Out: loss (f32, or [rows][length]), stats (f32: the mean divergence, the share of clipped tokens), kept:
+// bonsai_tune_bytes(rows, length, 2 where a gradient is wanted, else 0).
 int bonsai_policy_loss(const void* logps, long long ld_logps, const void* old, long long ld_old, const void* ref, long long ld_ref, const void* mask,
                        long long ld_mask, const float* gain, long long ld_gain, int gain_per_token, long long rows, long long length, int type, double low,
-                       double high, double kl_weight, int reduction, float* loss, float* kl, float* clipped, float* slope, float* weight, void* ws,
-                       long long ws_bytes, cudaStream_t st) {
+                       double high, double kl_weight, int reduction, float* loss, float* stats, void* kept, long long kept_bytes, int gradient, cudaStream_t st) {
   using namespace bonsai;
-  if (logps == nullptr || gain == nullptr || loss == nullptr || kl == nullptr || clipped == nullptr || ws == nullptr || !tune_good(rows, length) || type < 0 ||
-      type > 2 || reduction < 0 || reduction > 3 || (slope == nullptr) != (weight == nullptr) || ws_bytes < bonsai_tune_bytes(rows, length) || !(low >= 0.0) ||
-      !(low <= 1.0) || !(high >= 0.0))
+  if (logps == nullptr || gain == nullptr || loss == nullptr || stats == nullptr || kept == nullptr || !tune_good(rows, length) || type < 0 || type > 2 ||
+      reduction < 0 || reduction > 3 || kept_bytes < tune_kept(rows, length, gradient ? 2 : 0).bytes || !(low >= 0.0) || !(low <= 1.0) || !(high >= 0.0))
     return BONSAI_CUDA_BAD_ARG;
+  const TuneKept at = tune_kept(rows, length, gradient ? 2 : 0);
+  float* slope = gradient ? (float*)((char*)kept + at.slope) : nullptr;
+  float* weight = gradient ? (float*)((char*)kept + at.weight) : nullptr;
   const TuneShape sh = tune_shape(rows, length);
   const int size = type == 0 ? 4 : 2, threads = tune_threads(length);
   PolicyArgs a = {sh, {logps, ld_logps}, {old, ld_old}, {ref, ld_ref}, {mask, ld_mask}, gain, ld_gain, gain_per_token, log1p(-low), log1p(high),
-                  (float)(1.0 - low), (float)(1.0 + high), (float)kl_weight, slope, reduction == TUNE_NONE ? loss : nullptr, (TunePart*)ws};
+                  (float)(1.0 - low), (float)(1.0 + high), (float)kl_weight, slope, reduction == TUNE_NONE ? loss : nullptr, (TunePart*)kept};
   const bool wide = length % 4 == 0 && tune_wide(logps, ld_logps, size) && tune_wide(old, ld_old, size) && tune_wide(ref, ld_ref, size) &&
                     tune_wide(mask, ld_mask, 1) && (!gain_per_token || tune_wide(gain, ld_gain, 4)) && tune_wide(slope, length, 4) &&
                     tune_wide(a.each, length, 4);
@@ -424,23 +437,24 @@ int bonsai_policy_loss(const void* logps, long long ld_logps, const void* old, l
   else if (type == 1) e = wide ? launch_pdl(policy_kernel<__half, true>, grid, block, 0, st, a) : launch_pdl(policy_kernel<__half, false>, grid, block, 0, st, a);
   else e = wide ? launch_pdl(policy_kernel<__nv_bfloat16, true>, grid, block, 0, st, a) : launch_pdl(policy_kernel<__nv_bfloat16, false>, grid, block, 0, st, a);
   if (e == cudaSuccess)
-    e = launch_pdl(policy_finish_kernel, dim3(1), dim3(kTuneFinish), 0, st, sh, (const TunePart*)ws, reduction, reduction == TUNE_NONE ? (float*)nullptr : loss,
-                   kl, clipped, weight);
+    e = launch_pdl(policy_finish_kernel, dim3(1), dim3(kTuneFinish), 0, st, sh, (const TunePart*)kept, reduction, reduction == TUNE_NONE ? (float*)nullptr : loss, stats,
+                   weight);
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
 // Rows 0 .. pairs - 1 are the chosen answers, the next `pairs` the rejected ones; ref and mask may be null.  kind: PreferenceKind; reduction 0 mean, 1 sum,
-// 2 none.  Out: loss (f32, or [pairs]), rewards [pairs], and where a gradient is wanted slope [2 * pairs].
+// 2 none.  Out: loss (f32, or [pairs]), rewards [2 * pairs], kept: bonsai_tune_bytes(2 * pairs, length, 1 where a gradient is wanted, else 0).
 int bonsai_preference_loss(const void* logps, long long ld_logps, const void* ref, long long ld_ref, const void* mask, long long ld_mask, long long pairs,
-                           long long length, int type, int kind, int average, int reduction, double beta, double smoothing, float* loss, float* chosen,
-                           float* rejected, float* slope, void* ws, long long ws_bytes, cudaStream_t st) {
+                           long long length, int type, int kind, int average, int reduction, double beta, double smoothing, float* loss, float* rewards,
+                           void* kept, long long kept_bytes, int gradient, cudaStream_t st) {
   using namespace bonsai;
-  if (logps == nullptr || loss == nullptr || chosen == nullptr || rejected == nullptr || ws == nullptr || pairs < 1 || !tune_good(2 * pairs, length) ||
-      type < 0 || type > 2 || kind < 0 || kind > 2 || reduction < 0 || reduction > 2 || ws_bytes < bonsai_tune_bytes(2 * pairs, length) || !(beta > 0.0))
+  if (logps == nullptr || loss == nullptr || rewards == nullptr || kept == nullptr || pairs < 1 || !tune_good(2 * pairs, length) || type < 0 || type > 2 ||
+      kind < 0 || kind > 2 || reduction < 0 || reduction > 2 || kept_bytes < tune_kept(2 * pairs, length, gradient ? 1 : 0).bytes || !(beta > 0.0))
     return BONSAI_CUDA_BAD_ARG;
+  float* slope = gradient ? (float*)((char*)kept + tune_kept(2 * pairs, length, 1).slope) : nullptr;
   const TuneShape sh = tune_shape(2 * pairs, length);
   const int size = type == 0 ? 4 : 2, threads = tune_threads(length);
-  const PreferenceArgs a = {sh, {logps, ld_logps}, {ref, ld_ref}, {mask, ld_mask}, (TunePart*)ws};
+  const PreferenceArgs a = {sh, {logps, ld_logps}, {ref, ld_ref}, {mask, ld_mask}, (TunePart*)kept};
   const bool wide = length % 4 == 0 && tune_wide(logps, ld_logps, size) && tune_wide(ref, ld_ref, size) && tune_wide(mask, ld_mask, 1);
   const dim3 grid((unsigned)(sh.rows * sh.chunks)), block(threads);
   cudaError_t e;
@@ -449,18 +463,22 @@ int bonsai_preference_loss(const void* logps, long long ld_logps, const void* re
   else
     e = wide ? launch_pdl(preference_kernel<__nv_bfloat16, true>, grid, block, 0, st, a) : launch_pdl(preference_kernel<__nv_bfloat16, false>, grid, block, 0, st, a);
   if (e == cudaSuccess)
-    e = launch_pdl(preference_finish_kernel, dim3(1), dim3(kTuneFinish), 0, st, pairs, sh.chunks, (const TunePart*)ws, PreferenceRule{kind, average, reduction, beta, smoothing},
-                   loss, chosen, rejected, slope);
+    e = launch_pdl(preference_finish_kernel, dim3(1), dim3(kTuneFinish), 0, st, pairs, sh.chunks, (const TunePart*)kept,
+                   PreferenceRule{kind, average, reduction, beta, smoothing}, loss, rewards, rewards + pairs, slope);
   return e == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
 }
 
-// out [rows][length] = slope * weight * up where the mask (may be null) is set.  slope: f32, for a token or for a row; weight: for a row, may be null;
-// up: one value (up_kind 0), that of row % up_rows (1), or one for a token (2).
-int bonsai_tune_scale(const float* slope, int slope_per_token, const float* weight, const float* up, int up_kind, long long up_rows, const void* mask,
-                      long long ld_mask, long long rows, long long length, int type, void* out, cudaStream_t st) {
+// Gradient out [rows][length] of a forward pass from what it kept (slopes: 1 preference, 2 policy): slope * weight * up, 0 where the mask (may be null) is
+// not set.  up: one value (up_kind 0), that of row % up_rows (1), or one for a token (2).
+int bonsai_tune_scale(const void* kept, long long kept_bytes, int slopes, const float* up, int up_kind, long long up_rows, const void* mask, long long ld_mask,
+                      long long rows, long long length, int type, void* out, cudaStream_t st) {
   using namespace bonsai;
-  if (slope == nullptr || up == nullptr || out == nullptr || !tune_good(rows, length) || type < 0 || type > 2 || up_kind < 0 || up_kind > 2 || up_rows < 1)
+  if (kept == nullptr || up == nullptr || out == nullptr || !tune_good(rows, length) || type < 0 || type > 2 || up_kind < 0 || up_kind > 2 || up_rows < 1 ||
+      slopes < 1 || slopes > 2 || kept_bytes < tune_kept(rows, length, slopes).bytes)
     return BONSAI_CUDA_BAD_ARG;
+  const TuneKept at = tune_kept(rows, length, slopes);
+  const int slope_per_token = slopes == 2;
+  const float *slope = (const float*)((const char*)kept + at.slope), *weight = slope_per_token ? (const float*)((const char*)kept + at.weight) : nullptr;
   const TuneShape sh = tune_shape(rows, length);
   const int size = type == 0 ? 4 : 2;
   const ScaleArgs a = {sh, slope, slope_per_token, weight, up, up_kind, up_rows, {mask, ld_mask}};

@@ -25,15 +25,14 @@ _SIG = {
     "bonsai_ce_backward": [_vp, _ll, _i, _i, _i, _i, _i, C.c_float, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp],
     "bonsai_mt_adam": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _d, _vp, _d, _d, _d, _d, _i, _vp, _d, _vp, _vp, _vp],
     "bonsai_dropout": [_vp, _ll, _vp, _ll, _ll, _i, _u64, _vp, _i, _vp],
-    "bonsai_lr_padded": [_i],
     "bonsai_lr_self_rows": [],
-    "bonsai_lr_plan": [_vp, _i, _i, _i, _vp, _vp, _vp],
-    "bonsai_lr_rows": [_vp, _ll, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _u64, _vp, _i, _vp],
-    "bonsai_lr_outer": [_vp, _ll, _vp, _vp, _i, _vp, _ll, _vp, _vp, _i, _vp, _f, _i, _i, _i, _i, _i, _vp, _vp, _u64, _vp, _i, _vp],
-    "bonsai_tune_bytes": [_ll, _ll],
-    "bonsai_policy_loss": [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _i, _ll, _ll, _i, _d, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
-    "bonsai_preference_loss": [_vp, _ll, _vp, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _i, _d, _d, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
-    "bonsai_tune_scale": [_vp, _i, _vp, _vp, _i, _ll, _vp, _ll, _ll, _ll, _i, _vp, _vp],
+    "bonsai_lr_bytes": [_i, _i, _i, _i, _i],
+    "bonsai_lr_forward": [_vp, _ll, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _f, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _ll, _i, _u64, _vp, _i, _vp],
+    "bonsai_lr_backward": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _vp, _ll, _i, _vp, _ll, _u64, _vp, _i, _vp],
+    "bonsai_tune_bytes": [_ll, _ll, _i],
+    "bonsai_policy_loss": [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _i, _ll, _ll, _i, _d, _d, _d, _i, _vp, _vp, _vp, _ll, _i, _vp],
+    "bonsai_preference_loss": [_vp, _ll, _vp, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _i, _d, _d, _vp, _vp, _vp, _ll, _i, _vp],
+    "bonsai_tune_scale": [_vp, _ll, _i, _vp, _i, _ll, _vp, _ll, _ll, _ll, _i, _vp, _vp],
 }
 _declared = False
 _HERE = contextlib.nullcontext()
@@ -44,7 +43,7 @@ def _lib():
     global _declared
     l = K.lib()
     if not _declared:
-        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_bytes": _ll, "bonsai_tune_bytes": _ll})
+        K.declare(_SIG, {"bonsai_mt_partials": _ll, "bonsai_ce_bytes": _ll, "bonsai_tune_bytes": _ll, "bonsai_lr_bytes": _ll})
         _declared = True
     return l
 
@@ -177,66 +176,57 @@ def _seed(seed: Seed) -> tuple[int, int | None]:
 
 
 def dropout(x: torch.Tensor, steps: int, seed: Seed) -> torch.Tensor:
-    """Rows x [n, d] (unit stride along d): each value stays, over steps / 65536, where its 16 random bits are below ``steps``."""
-    with _on(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        K.check(_lib().bonsai_dropout(x.data_ptr(), _ld(x), y.data_ptr(), *x.shape, TYPE_CODES[x.dtype], *_seed(seed), steps, _stream(x.device)), "dropout")
+    """Rows x [n, d] (unit stride along d): each value stays, over steps / 65536, where its 16 random bits are below ``steps`` (< 65536)."""
+    device = x.device
+    with _on(device):
+        y = x.new_empty(x.shape)
+        K.check(_lib().bonsai_dropout(x.data_ptr(), _ld(x), y.data_ptr(), *x.shape, TYPE_CODES[x.dtype], *_seed(seed), steps, _stream(device)), "dropout")
     return y
 
 
 # ---- low-rank updates --------------------------------------------------------------------------------------------------------------------
-class RowGroups:
-    """Which rows have which adapter, as the kernels take it.  ``ids`` None: one adapter; ``planned``: the order of rows by adapter is made
-    (backward passes need it; more rows than a block groups by itself have it in any case)."""
-
-    def __init__(self, ids: torch.Tensor | None, n: int, adapters: int, planned: bool):
-        self.ids, self.n, self.adapters = ids, n, adapters
-        self.order = self.start = None
-        self.mode = 0 if ids is None else 1
-        if ids is not None and (planned or n > _lib().bonsai_lr_self_rows()):
-            self.mode = 2
-            with _on(ids.device):
-                self.order = torch.empty(n, dtype=torch.int32, device=ids.device)
-                self.start = torch.empty(adapters + 3, dtype=torch.int32, device=ids.device)
-                K.check(_lib().bonsai_lr_plan(ids.data_ptr(), ids.dtype == torch.int64, n, adapters, self.order.data_ptr(), self.start.data_ptr(),
-                                              _stream(ids.device)), "low_rank_plan")
-
-
 def _scale(scale: float | torch.Tensor) -> tuple[int | None, float]:
     return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
 
 
-def low_rank_rows(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, groups: RowGroups, back: bool, scale: float | torch.Tensor, steps: int, seed: Seed,
-                  base: torch.Tensor | None = None, out: torch.Tensor | None = None, keep: bool = False,
-                  only_kept: bool = False) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """x [n, k] -> (y [n, cols], the rank values by place or None): ``base + scale w2 (w1 x)`` with w1 [e, r, k] and w2 [e, cols, r], or, ``back``,
-    ``scale w2^T (w1^T x)`` with w1 [e, k, r] and w2 [e, r, cols].  Unit strides along rows, w1 and w2 dense.  ``steps`` of 65536 values stay: of x, or
-    of the result where ``back``."""
-    n, k = x.shape
-    rank, cols = (w1.shape[2], w2.shape[2]) if back else (w1.shape[1], w2.shape[1])
-    device = x.device
+def _lr_room(n: int, rank: int, adapters: int, grouped: bool, values: bool, like: torch.Tensor) -> torch.Tensor:
+    size = int(_lib().bonsai_lr_bytes(n, rank, adapters, grouped, values))
+    K.check(min(0, size), "low_rank_bytes")
+    return like.new_empty(size, dtype=torch.uint8)
+
+
+def low_rank_forward(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: torch.Tensor | None, ids: torch.Tensor | None, scale: float | torch.Tensor,
+                     steps: int, seed: Seed, out: torch.Tensor | None = None, train: bool = False,
+                     values: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """x [n, d], a [e, r, d], b [e, out, r] (dense), base [n, out] or None (unit strides along rows), ids [n] or None -> the result [n, out] and what a
+    backward pass takes (``train``; ``values``: that of ``b`` too)."""
+    (n, d), (e, r, _), cols, device = x.shape, a.shape, b.shape[1], x.device
     with _on(device):
-        y = None if only_kept else torch.empty((n, cols), dtype=x.dtype, device=device) if out is None else out
-        kept = torch.empty((n, _lib().bonsai_lr_padded(rank)), dtype=torch.float32, device=device) if keep else None
-        K.check(_lib().bonsai_lr_rows(x.data_ptr(), _ld(x), w1.data_ptr(), w2.data_ptr(), K.ptr(base), 0 if base is None else _ld(base), K.ptr(y),
-                                      0 if y is None else _ld(y), K.ptr(kept), *_scale(scale), n, k, cols, rank, groups.adapters, TYPE_CODES[x.dtype],
-                                      int(back), groups.mode, K.ptr(groups.ids), groups.ids is not None and groups.ids.dtype == torch.int64,
-                                      K.ptr(groups.order), K.ptr(groups.start), *_seed(seed), steps, _stream(device)), "low_rank_rows")
+        y = x.new_empty((n, cols)) if out is None else out
+        grouped = ids is not None
+        kept = None
+        if values or grouped and (train or n > _lib().bonsai_lr_self_rows()):
+            kept = _lr_room(n, r, e, grouped, values, x)
+        K.check(_lib().bonsai_lr_forward(x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), K.ptr(base), 0 if base is None else _ld(base), y.data_ptr(), _ld(y),
+                                         *_scale(scale), n, d, cols, r, e, TYPE_CODES[x.dtype], K.ptr(ids), grouped and ids.dtype == torch.int64,
+                                         K.ptr(kept), 0 if kept is None else kept.numel(), values, *_seed(seed), steps, _stream(device)), "low_rank_forward")
     return y, kept
 
 
-def low_rank_outer(x: torch.Tensor | None, g: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor | None, d: int, rank: int, groups: RowGroups,
-                   scale: float | torch.Tensor, steps: int, seed: Seed) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """Sums over each adapter's rows: (da [e, r, d] from x and g, db [e, out, r] from dy and h); what has no rank values is left out."""
-    n, out = dy.shape
-    device, e = dy.device, groups.adapters
+def low_rank_backward(x: torch.Tensor | None, dy: torch.Tensor, a: torch.Tensor | None, b: torch.Tensor, d: int, kept: torch.Tensor | None, grouped: bool,
+                      values: bool, scale: float | torch.Tensor, steps: int, seed: Seed, want_x: bool, want_a: bool,
+                      want_b: bool) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of :func:`low_rank_forward` by x (needs ``a``), a (needs ``x``) and b (needs a pass with ``values``)."""
+    (n, cols), (e, _, r), device, dtype = dy.shape, b.shape, dy.device, dy.dtype
     with _on(device):
-        da = None if g is None else torch.empty((e, rank, d), dtype=dy.dtype, device=device)
-        db = None if h is None else torch.empty((e, out, rank), dtype=dy.dtype, device=device)
-        K.check(_lib().bonsai_lr_outer(K.ptr(x), 0 if x is None else _ld(x), K.ptr(g), K.ptr(da), d, dy.data_ptr(), _ld(dy), K.ptr(h), K.ptr(db), out,
-                                       *_scale(scale), n, rank, e, TYPE_CODES[dy.dtype], groups.mode, K.ptr(groups.order), K.ptr(groups.start),
-                                       *_seed(seed), steps, _stream(device)), "low_rank_outer")
-    return da, db
+        dx = dy.new_empty((n, d)) if want_x else None
+        da = dy.new_empty((e, r, d)) if want_a else None
+        db = dy.new_empty((e, cols, r)) if want_b else None
+        ws = _lr_room(n, r, e, False, True, dy) if want_a else None
+        K.check(_lib().bonsai_lr_backward(K.ptr(x), 0 if x is None else _ld(x), dy.data_ptr(), _ld(dy), K.ptr(a), b.data_ptr(), K.ptr(dx), K.ptr(da), K.ptr(db),
+                                          *_scale(scale), n, d, cols, r, e, TYPE_CODES[dtype], grouped, K.ptr(kept), 0 if kept is None else kept.numel(), values,
+                                          K.ptr(ws), 0 if ws is None else ws.numel(), *_seed(seed), steps, _stream(device)), "low_rank_backward")
+    return dx, da, db
 
 
 # ---- losses over log-probabilities ---------------------------------------------------------------------------------------------------------
@@ -244,10 +234,10 @@ POLICY_REDUCTIONS = {"tokens": 0, "sequences": 1, "sum": 2, "none": 3}
 PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
 
 
-def _tune_room(rows: int, length: int, device: torch.device) -> torch.Tensor:
-    size = int(_lib().bonsai_tune_bytes(rows, length))
+def _tune_room(rows: int, length: int, slopes: int, like: torch.Tensor) -> torch.Tensor:
+    size = int(_lib().bonsai_tune_bytes(rows, length, slopes))
     K.check(min(0, size), "tune_bytes")
-    return torch.empty(size, dtype=torch.uint8, device=device)
+    return like.new_empty(size, dtype=torch.uint8)
 
 
 def _rows(t: torch.Tensor | None) -> tuple[int | None, int]:
@@ -255,43 +245,39 @@ def _rows(t: torch.Tensor | None) -> tuple[int | None, int]:
 
 
 def policy_forward(logps, old, ref, mask, gain, clip: tuple[float, float], kl_weight: float, reduction: str, keep: bool) -> tuple:
-    """Rows [n, t] (unit stride along t), gain f32 [n] or [n, t] -> (loss, kl, clipped share, slopes [n, t] or None, weights [n] or None)."""
+    """Rows [n, t] (unit stride along t), gain f32 [n] or [n, t] -> (loss, [mean divergence, clipped share], what :func:`tune_scale` takes)."""
     n, t = logps.shape
     device = logps.device
     with _on(device):
-        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
-        loss, kl, clipped = new(n, t) if reduction == "none" else new(), new(), new()
-        slope, weight = (new(n, t), new(n)) if keep else (None, None)
-        ws = _tune_room(n, t, device)
+        loss = logps.new_empty((n, t) if reduction == "none" else (), dtype=torch.float32)
+        stats, kept = logps.new_empty(2, dtype=torch.float32), _tune_room(n, t, 2 * keep, logps)
         K.check(_lib().bonsai_policy_loss(*_rows(logps), *_rows(old), *_rows(ref), *_rows(mask), gain.data_ptr(), _ld(gain) if gain.dim() == 2 else gain.stride(0),
-                                          int(gain.dim() == 2), n, t, TYPE_CODES[logps.dtype], *clip, kl_weight, POLICY_REDUCTIONS[reduction], loss.data_ptr(),
-                                          kl.data_ptr(), clipped.data_ptr(), K.ptr(slope), K.ptr(weight), ws.data_ptr(), ws.numel(), _stream(device)), "policy_loss")
-    return loss, kl, clipped, slope, weight
+                                          gain.dim() == 2, n, t, TYPE_CODES[logps.dtype], *clip, kl_weight, POLICY_REDUCTIONS[reduction], loss.data_ptr(),
+                                          stats.data_ptr(), kept.data_ptr(), kept.numel(), keep, _stream(device)), "policy_loss")
+    return loss, stats, kept
 
 
 def preference_forward(logps, ref, mask, beta: float, kind: str, smoothing: float, average: bool, reduction: str, keep: bool) -> tuple:
-    """Rows [2 pairs, t] -> (loss, rewards of the chosen and of the rejected rows, slopes [2 pairs] or None)."""
+    """Rows [2 pairs, t] -> (loss, rewards [2 pairs], what :func:`tune_scale` takes)."""
     n, t = logps.shape
     device = logps.device
     with _on(device):
-        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=device)  # noqa: E731
-        loss, chosen, rejected = new(n // 2) if reduction == "none" else new(), new(n // 2), new(n // 2)
-        slope = new(n) if keep else None
-        ws = _tune_room(n, t, device)
-        K.check(_lib().bonsai_preference_loss(*_rows(logps), *_rows(ref), *_rows(mask), n // 2, t, TYPE_CODES[logps.dtype], PREFERENCE_KINDS[kind], int(average),
-                                              REDUCTIONS[reduction], beta, smoothing, loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), K.ptr(slope),
-                                              ws.data_ptr(), ws.numel(), _stream(device)), "preference_loss")
-    return loss, chosen, rejected, slope
+        loss = logps.new_empty(n // 2 if reduction == "none" else (), dtype=torch.float32)
+        rewards, kept = logps.new_empty(n, dtype=torch.float32), _tune_room(n, t, keep, logps)
+        K.check(_lib().bonsai_preference_loss(*_rows(logps), *_rows(ref), *_rows(mask), n // 2, t, TYPE_CODES[logps.dtype], PREFERENCE_KINDS[kind], average,
+                                              REDUCTIONS[reduction], beta, smoothing, loss.data_ptr(), rewards.data_ptr(), kept.data_ptr(), kept.numel(), keep,
+                                              _stream(device)), "preference_loss")
+    return loss, rewards, kept
 
 
-def tune_scale(slope: torch.Tensor, weight: torch.Tensor | None, up: torch.Tensor, mask: torch.Tensor | None, shape: tuple[int, int],
-               dtype: torch.dtype) -> torch.Tensor:
-    """Gradient [n, t] from slopes ([n, t] or [n]), weights of rows and the loss's gradient (0-dim, [n, t], or one for every row modulo its length)."""
+def tune_scale(kept: torch.Tensor, tokens: bool, up: torch.Tensor, mask: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype) -> torch.Tensor:
+    """Gradient [n, t] from what a loss kept (``tokens``: a slope for each) and the loss's own gradient (0-dim, [n, t], or one for every row modulo its
+    length)."""
     n, t = shape
-    device = slope.device
+    device = kept.device
     with _on(device):
-        out = torch.empty((n, t), dtype=dtype, device=device)
+        out = kept.new_empty((n, t), dtype=dtype)
         kind = 0 if up.dim() == 0 else 2 if up.dim() == 2 else 1
-        K.check(_lib().bonsai_tune_scale(slope.data_ptr(), int(slope.dim() == 2), K.ptr(weight), up.data_ptr(), kind, max(1, up.numel()) if kind == 1 else 1,
-                                         *_rows(mask), n, t, TYPE_CODES[dtype], out.data_ptr(), _stream(device)), "tune_scale")
+        K.check(_lib().bonsai_tune_scale(kept.data_ptr(), kept.numel(), 1 + tokens, up.data_ptr(), kind, up.numel() if kind == 1 else 1, *_rows(mask), n, t,
+                                         TYPE_CODES[dtype], out.data_ptr(), _stream(device)), "tune_scale")
     return out

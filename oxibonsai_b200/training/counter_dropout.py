@@ -76,7 +76,10 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, up):
-        return _Dropout.apply(up, ctx.steps, ctx.saved_tensors[0] if ctx.seed is None else ctx.seed), None, None
+        seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
+        if up.is_cuda and not torch.is_grad_enabled():
+            return train_ops.dropout(rows_of(up), ctx.steps, seed).view(up.shape), None, None
+        return _Dropout.apply(up, ctx.steps, seed), None, None
 
 
 def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = None, training: bool = True) -> torch.Tensor:

@@ -18,6 +18,7 @@ from ..ops import train_ops
 from .counter_dropout import check_p, check_seed, keep_steps, kept, rows_of
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
+_CPU_TYPES = _TYPES + (torch.float64,)
 MAX_RANK = 128
 
 
@@ -61,13 +62,14 @@ class _LowRankUpdate(torch.autograd.Function):
         ctx.scale, ctx.steps, ctx.seed = (None if isinstance(v, torch.Tensor) else v for v in (scale, steps, seed))
         held = [v for v in (scale, seed) if isinstance(v, torch.Tensor)]
         if not x.is_cuda:
+            ids = None if ids is None else ids.reshape(-1)
             ctx.save_for_backward(x, a, b, ids, *held)
             return _cpu_forward(x, a, b, base, ids, scale, steps, seed)
-        groups = train_ops.RowGroups(ids, len(x), len(a), planned=True)
-        y, h = train_ops.low_rank_rows(x, a, b, groups, False, scale, steps, seed, base=base, keep=ctx.needs_input_grad[2])
+        want_x, want_a, want_b = ctx.needs_input_grad[:3]
+        y, kept = train_ops.low_rank_forward(x, a, b, base, ids, scale, steps, seed, train=True, values=want_b)
         # x is for the gradient of a, a for that of x
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, a if ctx.needs_input_grad[0] else None, b, h, *held)
-        ctx.groups, ctx.a_shape = groups, a.shape
+        ctx.save_for_backward(x if want_a else None, a if want_x else None, b, kept, *held)
+        ctx.width, ctx.grouped = x.shape[1], ids is not None
         return y
 
     @staticmethod
@@ -82,12 +84,7 @@ class _LowRankUpdate(torch.autograd.Function):
         if not up.is_cuda:
             dx, da, db = _cpu_backward(x, a, b, more, scale, ctx.steps, seed, up)
         elif want_x or want_a or want_b:
-            rows, g, (_, rank, d) = rows_of(up), None, ctx.a_shape
-            if want_x or want_a:
-                second = a if want_x else b          # not read without want_x
-                dx, g = train_ops.low_rank_rows(rows, b, second.view(len(b), rank, -1), ctx.groups, True, scale, ctx.steps, seed, keep=want_a, only_kept=not want_x)
-            if want_a or want_b:
-                da, db = train_ops.low_rank_outer(x, g, rows, more, d, rank, ctx.groups, scale, ctx.steps, seed)
+            dx, da, db = train_ops.low_rank_backward(x, rows_of(up), a, b, ctx.width, more, ctx.grouped, want_b, scale, ctx.steps, seed, want_x, want_a, want_b)
         return dx if want_x else None, da if want_a else None, db if want_b else None, up if want_base else None, None, None, None, None
 
 
@@ -131,44 +128,50 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     ``x``, ``a`` and ``b`` as every product keeps them.  On the GPU nothing is read back and all memory comes from torch's allocator; a pass and its
     gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives are refused."""
     what = "low_rank_update"
-    if x.dim() < 1 or a.dim() not in (2, 3) or b.dim() != a.dim() or x.shape[-1] != a.shape[-1] or a.shape[-2] != b.shape[-1] or a.shape[:-2] != b.shape[:-2]:
+    xs, sa, sb, device, dtype = x.shape, a.shape, b.shape, x.device, x.dtype
+    single = len(sa) == 2
+    if len(xs) < 1 or len(sa) not in (2, 3) or len(sb) != len(sa) or xs[-1] != sa[-1] or sa[-2] != sb[-1] or sa[:-2] != sb[:-2]:
         raise ValueError(f"{what}: x [..., in], a [count, rank, in] and b [count, out, rank] (or one adapter without count) are wanted, got "
-                         f"{tuple(x.shape)}, {tuple(a.shape)} and {tuple(b.shape)}")
-    single = a.dim() == 2
-    count, (rank, d), cols = 1 if single else a.shape[0], a.shape[-2:], b.shape[-2]
-    shape = x.shape[:-1] + (cols,)
-    n = math.prod(x.shape[:-1])
-    if not 1 <= rank <= MAX_RANK or not 1 <= count <= 65536 or min(d, cols) < 1 or max(d, cols, n) >= 2 ** 30:
+                         f"{tuple(xs)}, {tuple(sa)} and {tuple(sb)}")
+    rows, d, rank, cols, count = xs[:-1], sa[-1], sa[-2], sb[-2], 1 if single else sa[0]
+    n = math.prod(rows)
+    if not 1 <= rank <= MAX_RANK or not 1 <= count <= 65536 or d < 1 or cols < 1 or max(d, cols, n) >= 2 ** 30:
         raise ValueError(f"{what}: 1 to 65536 adapters of rank 1 to {MAX_RANK}, widths of at least 1 and sizes below 2^30 are wanted, got {count} of rank {rank}, "
                          f"widths {d} and {cols}, {n} rows")
-    if base is not None and base.shape != shape:
-        raise ValueError(f"{what}: base of shape {tuple(shape)} is wanted, got {tuple(base.shape)}")
-    if ids is None and count != 1:
-        raise ValueError(f"{what}: with {count} adapters ids of shape {tuple(x.shape[:-1])} are wanted")
-    if ids is not None and ids.shape != x.shape[:-1]:
-        raise ValueError(f"{what}: ids of shape {tuple(x.shape[:-1])} are wanted, got {tuple(ids.shape)}")
-    if ids is not None and ids.dtype not in (torch.int32, torch.int64):
+    if base is not None:
+        if base.shape[:-1] != rows or base.shape[-1] != cols or base.dim() != len(xs):
+            raise ValueError(f"{what}: base of shape {(*rows, cols)} is wanted, got {tuple(base.shape)}")
+        if base.dtype != dtype:
+            raise TypeError(f"{what}: base has the type of x, {dtype}, got {base.dtype}")
+    if ids is None:
+        if count != 1:
+            raise ValueError(f"{what}: with {count} adapters ids of shape {tuple(rows)} are wanted")
+    elif ids.shape != rows:
+        raise ValueError(f"{what}: ids of shape {tuple(rows)} are wanted, got {tuple(ids.shape)}")
+    elif ids.dtype != torch.int32 and ids.dtype != torch.int64:
         raise TypeError(f"{what}: ids are int32 or int64, got {ids.dtype}")
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32 or scale.numel() != count or scale.dim() > 1:
             raise ValueError(f"{what}: a scale for each adapter is float32 [{count}], got {scale.dtype} of shape {tuple(scale.shape)}")
         if scale.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what}: the scale has no gradient")
-        scale = scale.detach().reshape(-1).contiguous()
+        if scale.device != device:
+            raise ValueError(f"{what}: tensors of one device are wanted, got a scale on {scale.device} and x on {device}")
+        if scale.requires_grad or not scale.is_contiguous():
+            scale = scale.detach().contiguous()
     else:
         scale = float(scale)
-    given = [x, a, b] + [t for t in (base, ids, scale) if isinstance(t, torch.Tensor)]
-    if any(t.device != x.device for t in given) or x.device.type not in ("cuda", "cpu"):
-        raise ValueError(f"{what}: CUDA or CPU tensors of one device are wanted, got {', '.join(str(t.device) for t in given)}")
-    types = _TYPES if x.is_cuda else _TYPES + (torch.float64,)
-    if x.dtype not in types or any(t.dtype != x.dtype for t in (a, b) + (() if base is None else (base,))):
-        raise TypeError(f"{what}: x, a, b and base of one type (float32, float16, bfloat16) are wanted, got "
-                        f"{', '.join(str(t.dtype) for t in (x, a, b) + (() if base is None else (base,)))}")
-    steps = keep_steps(check_p(dropout, what))
-    seed = check_seed(seed, x.device, what) if seed is not None or steps < 65536 else 0
-    wants_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, a, b, base))
+    if a.device != device or b.device != device or (base is not None and base.device != device) or (ids is not None and ids.device != device):
+        raise ValueError(f"{what}: tensors of one device are wanted, got {', '.join(str(t.device) for t in (x, a, b, base, ids) if t is not None)}")
+    if device.type not in ("cuda", "cpu"):
+        raise ValueError(f"{what}: CUDA or CPU tensors are wanted, got {device}")
+    if a.dtype != dtype or b.dtype != dtype or dtype not in (_TYPES if device.type == "cuda" else _CPU_TYPES):
+        raise TypeError(f"{what}: x, a and b of one type (float32, float16, bfloat16) are wanted, got {dtype}, {a.dtype} and {b.dtype}")
+    steps = 65536 if dropout == 0.0 else keep_steps(check_p(dropout, what))
+    seed = 0 if seed is None and steps == 65536 else check_seed(seed, device, what)
+    wants_grad = torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or (base is not None and base.requires_grad))
     if out is not None:
-        _check_out(out, shape, x, [t for t in given if t is not base] + ([seed] if isinstance(seed, torch.Tensor) else []), base, wants_grad)
+        _check_out(out, (*rows, cols), x, [t for t in (x, a, b, ids, scale, seed) if isinstance(t, torch.Tensor)], base, wants_grad)
     if single:
         a, b = a[None], b[None]
     if n == 0:
@@ -177,19 +180,18 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     flat, base2 = rows_of(x), None if base is None else rows_of(base)
     a, b = a.contiguous(), b.contiguous()
     if ids is not None:
-        ids = ids.reshape(-1).contiguous()
+        ids = ids.contiguous()
         if not x.is_cuda and bool((ids >= count).any()):
             raise IndexError(f"{what}: an id names none of {count} adapters")
     if wants_grad:
-        return _LowRankUpdate.apply(flat, a, b, base2, ids, scale, steps, seed).reshape(shape)
+        y = _LowRankUpdate.apply(flat, a, b, base2, ids, scale, steps, seed)
+        return y if len(xs) == 2 else y.reshape((*rows, cols))
     if not x.is_cuda:
-        y = _cpu_forward(flat, a, b, base2, ids, scale, steps, seed).reshape(shape)
+        y = _cpu_forward(flat, a, b, base2, None if ids is None else ids.reshape(-1), scale, steps, seed).reshape((*rows, cols))
         return y if out is None else out.copy_(y)
-    groups = train_ops.RowGroups(ids, n, count, planned=False)
-    to = None if out is None else out if out.dim() == 2 else out.view(-1, cols)
-    y, _ = train_ops.low_rank_rows(flat, a, b, groups, False, scale, steps, seed, base=base2, out=to)
+    y, _ = train_ops.low_rank_forward(flat, a, b, base2, ids, scale, steps, seed, out=None if out is None else out if out.dim() == 2 else out.view(-1, cols))
     if out is None:
-        return y.reshape(shape)
+        return y if len(xs) == 2 else y.reshape((*rows, cols))
     if not out.is_inference():
         increment_version(out)
     return out

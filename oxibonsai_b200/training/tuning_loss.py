@@ -51,29 +51,29 @@ def _check(what, logps, others, mask) -> None:
 
 
 def _rows(t):
-    return None if t is None else rows_of(t.detach())
+    return None if t is None else rows_of(t.detach() if t.requires_grad else t)
 
 
 # ---- preference pairs --------------------------------------------------------------------------------------------------------------------
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, ref, mask, beta, kind, smoothing, average, reduction, keep):
-        loss, chosen, rejected, slope = train_ops.preference_forward(logps, ref, mask, beta, kind, smoothing, average, reduction, keep)
+        loss, rewards, kept = train_ops.preference_forward(logps, ref, mask, beta, kind, smoothing, average, reduction, keep)
         if keep:
-            ctx.save_for_backward(slope, mask)
+            ctx.save_for_backward(kept, mask)
             ctx.shape, ctx.dtype = logps.shape, logps.dtype
-        ctx.mark_non_differentiable(chosen, rejected)
+        ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
-        return loss, chosen, rejected
+        return loss, rewards
 
     @staticmethod
-    def backward(ctx, up, *_):
+    def backward(ctx, up, _):
         if torch.is_grad_enabled():
             raise RuntimeError("preference_loss: its gradients cannot be differentiated again (create_graph=True)")
         if up is None:
             return (None,) * 9
-        slope, mask = ctx.saved_tensors
-        return (train_ops.tune_scale(slope, None, up.contiguous(), mask, ctx.shape, ctx.dtype),) + (None,) * 8
+        kept, mask = ctx.saved_tensors
+        return (train_ops.tune_scale(kept, False, up.contiguous(), mask, ctx.shape, ctx.dtype),) + (None,) * 8
 
 
 def _preference_cpu(logps, ref, mask, beta, kind, smoothing, average, reduction):
@@ -127,29 +127,29 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
     if not logps.is_cuda or logps.numel() == 0:
         return _preference_cpu(logps, ref_logps, mask, float(beta), kind, float(label_smoothing), average, reduction)
     keep = torch.is_grad_enabled() and logps.requires_grad
-    return PreferenceLoss(*_Preference.apply(rows_of(logps), _rows(ref_logps), _rows(mask), float(beta), kind, float(label_smoothing), bool(average), reduction, keep))
+    loss, rewards = _Preference.apply(rows_of(logps), _rows(ref_logps), _rows(mask), float(beta), kind, float(label_smoothing), bool(average), reduction, keep)
+    return PreferenceLoss(loss, *rewards.chunk(2))
 
 
 # ---- clipped policy ratio ----------------------------------------------------------------------------------------------------------------
 class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, old, ref, mask, gain, clip, kl_weight, reduction, keep):
-        loss, kl, clipped, slope, weight = train_ops.policy_forward(logps, old, ref, mask, gain, clip, kl_weight, reduction, keep)
+        loss, stats, kept = train_ops.policy_forward(logps, old, ref, mask, gain, clip, kl_weight, reduction, keep)
         if keep:
-            ctx.save_for_backward(slope, weight)
-            ctx.dtype = logps.dtype
-        ctx.mark_non_differentiable(kl, clipped)
+            ctx.save_for_backward(kept)
+            ctx.shape, ctx.dtype = logps.shape, logps.dtype
+        ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
-        return loss, kl, clipped
+        return loss, stats
 
     @staticmethod
-    def backward(ctx, up, *_):
+    def backward(ctx, up, _):
         if torch.is_grad_enabled():
             raise RuntimeError("policy_loss: its gradients cannot be differentiated again (create_graph=True)")
         if up is None:
             return (None,) * 9
-        slope, weight = ctx.saved_tensors
-        return (train_ops.tune_scale(slope, weight, up.contiguous(), None, slope.shape, ctx.dtype),) + (None,) * 8
+        return (train_ops.tune_scale(ctx.saved_tensors[0], True, up.contiguous(), None, ctx.shape, ctx.dtype),) + (None,) * 8
 
 
 def _policy_cpu(logps, old, ref, mask, gain, clip, kl_weight, reduction):
@@ -213,7 +213,7 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     clip = float(clip[0]), float(clip[1])
     if not logps.is_cuda or logps.numel() == 0:
         return _policy_cpu(logps, old_logps, ref_logps, mask, advantages, clip, float(kl_weight), reduction)
-    gain = advantages.detach().float()
-    gain = rows_of(gain) if gain.dim() == 2 else gain
+    gain = _rows(advantages.float()) if advantages.dim() == 2 else advantages.detach().float()
     keep = torch.is_grad_enabled() and logps.requires_grad
-    return PolicyLoss(*_Policy.apply(rows_of(logps), _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction, keep))
+    loss, stats = _Policy.apply(rows_of(logps), _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction, keep)
+    return PolicyLoss(loss, *stats.unbind())
