@@ -7,7 +7,8 @@ constexpr int kPlanThreads = 512, kPlanEach = 8;
 
 // order: the rows by adapter, in their own order within each; start[e]: where adapter e's begin.  A block makes one adapter's list on its own: it counts
 // the ids below its own, which is where the list begins, and goes through the ids once more.  Nothing is shared between blocks, no atomics.
-__global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* order, int* start) {
+// tiles (may be null): of 16 rows, those of adapter e in places start[e] / 16 + e to start[e + 1] / 16 + e, which are enough for all and lie apart.
+__global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* order, int* start, int4* tiles) {
   __shared__ int warps[kPlanThreads / 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -39,6 +40,7 @@ __global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* 
     start[e] = place;
     if (e == g.adapters + 1) start[e + 1] = g.n;
   }
+  const int begin = place;
   for (long long first = 0; first < g.n; first += per) {
     const long long row = first + (long long)t * kPlanEach;
     unsigned mine = 0;
@@ -50,6 +52,11 @@ __global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* 
     for (unsigned m = mine; m != 0; m &= m - 1) order[at++] = (int)row + __ffs(m) - 1;
     place += all;
   }
+  if (tiles != nullptr)
+    for (int i = t; i <= place / 16 - begin / 16; i += kPlanThreads) {
+      const int at = begin + 16 * i, left = place - at;
+      tiles[begin / 16 + e + i] = left > 0 ? make_int4(e, at, left < 16 ? left : 16, 0) : make_int4(-1, 0, 0, 0);
+    }
 }
 
 static bool lr_good(int n, int k, int cols, int rank, int adapters, int type) {
@@ -60,16 +67,38 @@ static bool lr_good(int n, int k, int cols, int rank, int adapters, int type) {
 // rows of `width` values at distances of ld that begin at multiples of 16 bytes and hold whole eights
 static int lr_vec(const void* p, long long ld, long long width, int size) { return width % 8 == 0 && ((uintptr_t)p | (uintptr_t)(ld * size)) % 16 == 0; }
 
-// What a forward pass leaves for the backward one: the rank values, the order of rows and where each adapter's rows begin in it.
-struct LrKept {
-  long long order, start, bytes;
+// What a forward pass leaves for the backward one, and what the backward pass works with: the rank values (and their two f16 parts where the second product is a
+// kernel of its own), the order of rows, where each adapter's rows begin in it, the tiles of 16 rows.
+struct LrRoom {
+  bool values, grouped, split;
+  long long parts, factors, order, start, tiles, bytes;
 };
-static LrKept lr_kept(int n, int rank, int adapters, bool grouped, bool values) {
-  LrKept k;
-  k.order = values ? 4ll * n * lr_padded(rank) : 0;
-  k.start = k.order + (grouped ? (4ll * n + 15) / 16 * 16 : 0);
-  k.bytes = k.start + (grouped ? 4ll * (adapters + 3) : 0);
+static LrRoom lr_room(int n, int rank, int adapters, int type, bool grouped, bool values) {
+  LrRoom k;
+  k.split = n >= kLrSplit;
+  k.values = values || k.split;
+  k.grouped = grouped;
+  auto up = [](long long b) { return (b + 15) / 16 * 16; };
+  const long long all = 4ll * n * lr_padded(rank);
+  k.parts = k.values ? all : 0;
+  k.factors = k.parts + (k.split && type == 1 ? all : 0);
+  k.order = k.factors + (k.split && type == 1 ? up(4ll * n) : 0);
+  k.start = k.order + (grouped ? up(4ll * n) : 0);
+  k.tiles = k.start + (grouped ? up(4ll * (adapters + 3)) : 0);
+  k.bytes = k.tiles + (grouped && k.split ? 16ll * (n / 16 + adapters + 2) : 0);
   return k;
+}
+static LrValues lr_values(void* room, const LrRoom& k) {
+  char* p = (char*)room;
+  const bool parts = k.factors > k.parts;
+  return {k.values ? p : nullptr, parts ? (__half*)(p + k.parts) : nullptr, parts ? (float*)(p + k.factors) : nullptr};
+}
+static void lr_grouped(LrGroups& g, void* room, const LrRoom& k) {
+  char* p = (char*)room;
+  g.mode = LR_PLAN;
+  g.order = (const int*)(p + k.order);
+  g.start = (const int*)(p + k.start);
+  g.tiles = k.split ? (const int4*)(p + k.tiles) : nullptr;
 }
 
 template <typename Args>
@@ -85,38 +114,37 @@ extern "C" {
 int bonsai_lr_self_rows() { return bonsai::kLrSelf; }
 
 // Bytes of `kept` for a forward pass (values: the rank values are wanted behind it; grouped: ids are given), and of the workspace of the backward pass
-// (values alone).  Negative for sizes that are refused.
-long long bonsai_lr_bytes(int n, int rank, int adapters, int grouped, int values) {
+// (values, not grouped).  0: none is needed.  Negative for sizes that are refused.
+long long bonsai_lr_bytes(int n, int rank, int adapters, int type, int grouped, int values) {
   using namespace bonsai;
-  return lr_good(n, 1, 1, rank, adapters, 0) ? lr_kept(n, rank, adapters, grouped, values).bytes : BONSAI_CUDA_BAD_ARG;
+  return lr_good(n, 1, 1, rank, adapters, type) ? lr_room(n, rank, adapters, type, grouped, values).bytes : BONSAI_CUDA_BAD_ARG;
 }
 
 // y [n][out] = base + s b (a x) by rows: a [adapters][rank][d], b [adapters][out][rank], rows of x, base and y at distances of their ld; base may be null, or y
 // itself.  ids (int32, or int64 where wide; negative: a row without an adapter) may be null with one adapter.  scales [adapters], or scale.  x is dropped
-// where steps < 65536.  kept: bonsai_lr_bytes of this call, null where nothing is kept and ids are absent or at most bonsai_lr_self_rows.
+// where steps < 65536.  kept: bonsai_lr_bytes of this call; null where nothing is kept and there are at most bonsai_lr_self_rows ids.
 int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b, const void* base, long long ld_base, void* y, long long ldy,
                       const float* scales, float scale, int n, int d, int out, int rank, int adapters, int type, const void* ids, int ids_wide, void* kept,
                       long long kept_bytes, int values, unsigned long long seed, const long long* seed_dev, int steps, cudaStream_t st) {
   using namespace bonsai;
   if (x == nullptr || a == nullptr || b == nullptr || y == nullptr || !lr_good(n, d, out, rank, adapters, type) || steps < 0 || steps > 65536 ||
-      (ids == nullptr && adapters != 1) || (values && kept == nullptr) || (ids != nullptr && kept == nullptr && n > kLrSelf))
+      (ids == nullptr && adapters != 1))
     return BONSAI_CUDA_BAD_ARG;
-  const LrKept at = lr_kept(n, rank, adapters, ids != nullptr, values);
-  if (kept != nullptr && kept_bytes < at.bytes) return BONSAI_CUDA_BAD_ARG;
-  char* room = (char*)kept;
-  LrGroups g = {LR_ONE, ids, ids_wide, nullptr, nullptr, n, adapters};
+  const bool self = ids != nullptr && kept == nullptr && !values && n <= kLrSelf;
+  const LrRoom at = lr_room(n, rank, adapters, type, ids != nullptr, values);
+  if (!self && at.bytes > 0 && (kept == nullptr || kept_bytes < at.bytes)) return BONSAI_CUDA_BAD_ARG;
+  LrGroups g = {LR_ONE, ids, ids_wide, nullptr, nullptr, nullptr, n, adapters};
   cudaError_t e = cudaSuccess;
   if (ids != nullptr) {
-    g.mode = kept == nullptr ? LR_SELF : LR_PLAN;
-    if (g.mode == LR_PLAN) {
-      g.order = (const int*)(room + at.order);
-      g.start = (const int*)(room + at.start);
-      e = launch_pdl(lr_plan_kernel, dim3(adapters + 2), dim3(kPlanThreads), 0, st, g, (int*)(room + at.order), (int*)(room + at.start));
+    g.mode = LR_SELF;
+    if (!self) {
+      lr_grouped(g, kept, at);
+      e = launch_pdl(lr_plan_kernel, dim3(adapters + 2), dim3(kPlanThreads), 0, st, g, (int*)g.order, (int*)g.start, (int4*)g.tiles);
     }
   }
   if (e != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
   const int size = type == 0 ? 4 : 2;
-  LrRowsArgs r = {g, x, ldx, a, b, base, ld_base, y, ldy, values ? kept : nullptr, scales, scale, d, out, rank};
+  LrRowsArgs r = {g, x, ldx, a, b, base, ld_base, y, ldy, self ? LrValues{} : lr_values(kept, at), scales, scale, d, out, rank};
   r.vec_x = lr_vec(x, ldx, d, size);
   r.vec_w1 = lr_vec(a, d, d, size);
   r.vec_w2 = rank % (8 / size) == 0 && (uintptr_t)b % 8 == 0;         // rank values of a column as words of 8 bytes
@@ -127,29 +155,25 @@ int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b
 }
 
 // Gradients of bonsai_lr_forward: dx [n][d], da, db (like a and b; zeros of adapters without rows), each may be null.  kept: of the forward pass, with the
-// values where db is wanted (values: whether it has them).  ws: bonsai_lr_bytes(n, rank, adapters, 0, 1) where da is wanted.
+// values where db is wanted (values, grouped: as there).  ws: bonsai_lr_bytes(n, rank, adapters, type, 0, 1) where dx or da is wanted.
 int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long lddy, const void* a, const void* b, void* dx, void* da, void* db,
                        const float* scales, float scale, int n, int d, int out, int rank, int adapters, int type, int grouped, const void* kept,
                        long long kept_bytes, int values, void* ws, long long ws_bytes, unsigned long long seed, const long long* seed_dev, int steps,
                        cudaStream_t st) {
   using namespace bonsai;
   if (dy == nullptr || b == nullptr || !lr_good(n, d, out, rank, adapters, type) || steps < 0 || steps > 65536 || (!grouped && adapters != 1) ||
-      (dx != nullptr && a == nullptr) || (da != nullptr && (x == nullptr || ws == nullptr)) || (db != nullptr && !values) || ((grouped || db != nullptr) && kept == nullptr))
+      (dx != nullptr && a == nullptr) || (da != nullptr && x == nullptr) || (db != nullptr && !values))
     return BONSAI_CUDA_BAD_ARG;
-  const LrKept at = lr_kept(n, rank, adapters, grouped, values);
-  if ((kept != nullptr && kept_bytes < at.bytes) || (da != nullptr && ws_bytes < lr_kept(n, rank, adapters, false, true).bytes)) return BONSAI_CUDA_BAD_ARG;
-  const char* room = (const char*)kept;
-  LrGroups g = {LR_ONE, nullptr, 0, nullptr, nullptr, n, adapters};
-  if (grouped) {
-    g.mode = LR_PLAN;
-    g.order = (const int*)(room + at.order);
-    g.start = (const int*)(room + at.start);
-  }
+  const bool rows = dx != nullptr || da != nullptr;
+  const LrRoom at = lr_room(n, rank, adapters, type, grouped, values), of = lr_room(n, rank, adapters, type, false, true);
+  if ((at.bytes > 0 && (kept == nullptr || kept_bytes < at.bytes)) || (rows && (ws == nullptr || ws_bytes < of.bytes))) return BONSAI_CUDA_BAD_ARG;
+  LrGroups g = {LR_ONE, nullptr, 0, nullptr, nullptr, nullptr, n, adapters};
+  if (grouped) lr_grouped(g, (void*)kept, at);
   const int size = type == 0 ? 4 : 2;
   const DropoutRule rule = dropout_rule(seed, seed_dev, steps);
   cudaError_t e = cudaSuccess;
-  if (dx != nullptr || da != nullptr) {
-    LrRowsArgs r = {g, dy, lddy, b, a, nullptr, 0, dx, d, da != nullptr ? ws : nullptr, scales, scale, out, d, rank};
+  if (rows) {
+    LrRowsArgs r = {g, dy, lddy, b, a, nullptr, 0, dx, d, lr_values(ws, of), scales, scale, out, d, rank};
     r.vec_x = lr_vec(dy, lddy, out, size);
     r.vec_w1 = lr_vec(b, rank, rank, size);
     r.vec_w2 = lr_vec(a, d, d, size);

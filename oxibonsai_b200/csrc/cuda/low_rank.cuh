@@ -3,11 +3,11 @@
 //   forward    h_i = A_e x~_i;   y_i = base_i + s_e B_e h_i                   x~: x, or what dropout leaves of it (philox.cuh)
 //   backward   g_i = B_e^T dy_i; dx_i = s_e A_e^T g_i (dropped again);  dA_e = s_e sum_i g_i x~_i^T;  dB_e = s_e sum_i dy_i h_i^T
 //
-// Both directions of the rows are the same kernel (lr_rows_kernel): a product over a long axis that leaves `rank` values a row, and one from these to a long
-// axis.  A cluster of blocks takes one tile of rows of one adapter: each block multiplies its part of the long axis, the parts meet over
-// distributed shared memory in one order, and each block writes its part of the columns.  One launch, no workspace, no atomics; rank values never
-// leave the chip unless a backward pass wants them.  The factors' gradients are a second kernel (lr_outer_kernel): sums over an adapter's rows,
-// split over a cluster and joined the same way.
+// Both directions of the rows are the same two products: one over a long axis that leaves `rank` values a row, and one from these to a long axis.  Few rows
+// (lr_rows_kernel): a cluster of blocks takes one tile of rows of one adapter; each block multiplies its part of the long axis, the parts meet
+// over distributed shared memory in one order, and each block writes its part of the columns.  One launch, no atomics; rank values leave the chip only
+// where a backward pass wants them.  Many rows: the same kernel stops at the rank values and lr_expand_kernel makes the second product.  The factors'
+// gradients (lr_outer_kernel) are sums over an adapter's rows, split over a cluster and joined the same way.
 //
 // All are bound by memory: 2 rank operations for each value that is read.  So the matrix instructions are mma.sync, whose operands are gathered rows
 // from shared memory; tcgen05 would want tiles of 128 rows and does not pay at one operation a byte.  The long product of 16-bit types multiplies them as they are
@@ -25,6 +25,8 @@
 namespace bonsai {
 
 constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
+// From so many rows on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.
+constexpr int kLrSplit = 1024;
 constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024;        // dynamic shared memory of a block, of each of two on an SM
 constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
 enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
@@ -35,7 +37,16 @@ struct LrGroups {            // which rows have which adapter
   int ids_wide;              // int64, else int32
   const int* order;          // LR_PLAN: rows by adapter; behind them those without one, and those whose id names none
   const int* start;          // [adapters + 3]: where each adapter's rows begin in it
+  const int4* tiles;         // LR_PLAN of kLrSplit rows and more: tiles of 16 rows: group (-1: none), place, rows
   int n, adapters;
+};
+
+// The rank values of a forward or a backward pass, by place in the order: f32 [n][R] (R: the padded rank), of bf16 two parts [2][n][R].  f16 for the second
+// product: two parts over a power of two for each row, and that power.
+struct LrValues {
+  void* values;
+  __half* parts;
+  float* factors;
 };
 
 struct LrRowsArgs {
@@ -44,11 +55,11 @@ struct LrRowsArgs {
   const void *w1, *w2;                   // forward: A, B; backward: B, A
   const void* base; long long ld_base;   // [n][cols], may be null
   void* y; long long ldy;                // null: the rank values alone are wanted
-  void* kept;                            // [n][padded rank] by place in the order, may be null: f32, of bf16 the two parts [2][n][padded rank]
+  LrValues kept;                         // null where nothing is kept
   const float* scales;                   // of the adapters, or null: scale
   float scale;
   int k, cols, rank;
-  int vec_x, vec_w1, vec_w2, vec_y;      // rows that 16-byte (w2 of the forward pass: 4-byte) accesses may take
+  int vec_x, vec_w1, vec_w2, vec_y;      // rows that 16-byte (w2 of the forward pass: 8-byte) accesses may take
   DropoutRule drop;
   int drop_x, drop_y;                    // forward: the rows of x; backward: those of dx
 };
@@ -291,25 +302,146 @@ __device__ __forceinline__ void lr_fill(T* to, int pitch, int nrows, int c0, int
   }
 }
 
+// ---- the second product ------------------------------------------------------------------------------------------------------------------------
+// A warp takes 16 rows and 32 columns at a time, four matrix instructions wide.  Column 8 (c / 2) + 2 j + c % 2 is column c of the j-th, so that the eight
+// values that a thread has of a row lie side by side.  Of the rank values a thread has 4 t .. 4 t + 3 of every sixteen (f32: 2 t and 2 t + 1 of
+// every eight): the axis of a product may be taken in any order, and so its factors lie side by side too.
+template <typename T> struct LrStep {
+  static constexpr int kStep = sizeof(T) == 4 ? 8 : 16, kEach = kStep / 4;
+};
+
+template <typename T, bool BACK>
+struct LrFactor {              // w2 of one adapter: forward [cols][rank], backward [rank][cols]
+  const T* p;                  // this thread's first value
+  int cols, rank, vec, g, t;
+  __device__ __forceinline__ LrFactor(const T* w2, int cols, int rank, int vec, int g, int t)
+      : p(BACK ? w2 + (long long)(LrStep<T>::kEach * t) * cols + 8 * (g >> 1) : w2 + (long long)(8 * (g >> 1) + (g & 1)) * rank + LrStep<T>::kEach * t),
+        cols(cols), rank(rank), vec(vec), g(g), t(t) {}
+  // columns 32 b and on, rank values k and on
+  __device__ __forceinline__ void load(int b, int k, uint32_t (*w)[2]) const {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int kEach = LrStep<T>::kEach;
+    const int wc = b * 32 + 8 * (g >> 1), kk = k + kEach * t;      // eight columns, of which this thread takes every second
+    if (BACK) {
+      uint32_t v[kEach][F32 ? 8 : 4];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const T* q = p + (long long)(k + i) * cols + b * 32;
+        const bool there = kk + i < rank && wc < cols;
+        if (vec) {
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+            const uint4 u = there ? reinterpret_cast<const uint4*>(q)[h] : make_uint4(0, 0, 0, 0);
+            v[i][4 * h] = u.x; v[i][4 * h + 1] = u.y; v[i][4 * h + 2] = u.z; v[i][4 * h + 3] = u.w;
+          }
+        } else {
+          __align__(16) T e[8];
+#pragma unroll
+          for (int h = 0; h < 8; ++h) e[h] = there && wc + h < cols ? q[h] : lr_round<T>(0.0f);
+#pragma unroll
+          for (int h = 0; h < (F32 ? 8 : 4); ++h) v[i][h] = reinterpret_cast<const uint32_t*>(e)[h];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (F32) {
+          w[j][0] = g & 1 ? v[0][2 * j + 1] : v[0][2 * j];
+          w[j][1] = g & 1 ? v[1][2 * j + 1] : v[1][2 * j];
+        } else {
+          const unsigned pick = g & 1 ? 0x7632u : 0x5410u;        // the upper or the lower halves of two words
+          w[j][0] = __byte_perm(v[0][j], v[1][j], pick);
+          w[j][1] = __byte_perm(v[kEach - 2][j], v[kEach - 1][j], pick);
+        }
+      }
+    } else {
+      const T* first = p + (long long)b * 32 * rank + k;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int cc = wc + 2 * j + (g & 1);
+        const T* q = first + 2 * j * rank;
+        if (vec) {
+          const uint2 u = cc < cols && kk < rank ? *reinterpret_cast<const uint2*>(q) : make_uint2(0, 0);
+          w[j][0] = u.x; w[j][1] = u.y;
+        } else {
+          __align__(8) T e[kEach];
+#pragma unroll
+          for (int h = 0; h < kEach; ++h) e[h] = cc < cols && kk + h < rank ? q[h] : lr_round<T>(0.0f);
+          w[j][0] = reinterpret_cast<const uint32_t*>(e)[0];
+          w[j][1] = reinterpret_cast<const uint32_t*>(e)[1];
+        }
+      }
+    }
+  }
+};
+
+// acc += the rank values of 16 rows (two parts) times the factors of 32 columns
+template <typename T>
+__device__ __forceinline__ void lr_multiply(float (*acc)[4], const uint32_t* hi, const uint32_t* lo, const uint32_t (*w)[2], bool start) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t h0, l0, h1, l1;
+      lr_split(__uint_as_float(w[j][0]), h0, l0);
+      lr_split(__uint_as_float(w[j][1]), h1, l1);
+      lr_mma8(acc[j], lo, h0, h1, start);
+      lr_mma8(acc[j], hi, l0, l1);
+      lr_mma8(acc[j], hi, h0, h1);
+    } else {
+      lr_mma16<T>(acc[j], lo, w[j][0], w[j][1], start);
+      lr_mma16<T>(acc[j], hi, w[j][0], w[j][1]);
+    }
+  }
+}
+
+// v (base, or zeros) + the eight sums of row g + 8 h, dropped where asked
+__device__ __forceinline__ void lr_finish(float* v, float (*acc)[4], int h, float scale, const uint4* words, unsigned limit) {
+#pragma unroll
+  for (int q = 0; q < 8; q += 2) {
+    float* d = &acc[q >> 1][2 * h];
+    lr_fma2(d, scale, v + q);
+    v[q] = d[0]; v[q + 1] = d[1];
+  }
+  if (words != nullptr) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = dropout_keeps(*words, q, limit) ? v[q] : 0.0f;
+  }
+}
+
+// f16: the power of two that brings a row's largest rank value between 2^13 and 2^14, and one over it; 1 for zeros, infinities and what is next to them
+__device__ __forceinline__ float lr_power(float top, float& down) {
+  const int e = (int)(__float_as_uint(top) >> 23 & 255u) - 127 - 13;
+  const bool scaled = top > 1e-30f && top < 1e30f;
+  down = scaled ? __uint_as_float((unsigned)(127 - e) << 23) : 1.0f;
+  return scaled ? __uint_as_float((unsigned)(127 + e) << 23) : 1.0f;
+}
+template <typename T>
+__device__ __forceinline__ void lr_parts(const float* f, T* hi, T* lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = lr_round<T>(f[i]);
+    const float h = lr_float<T>(hi[i]);
+    lo[i] = lr_round<T>(fabsf(h) <= 3.4028234e38f ? f[i] - h : 0.0f);
+  }
+}
+
 // ---- the rows ------------------------------------------------------------------------------------------------------------------------------
 template <int M> struct LrShape {
   static constexpr int kM16 = M / 16, kParts = kLrWarps / kM16;       // warps over rows, and over the long axis
   static constexpr int kChunk = M == 64 ? 64 : 128, kWarpK = kChunk / kParts;
-  static constexpr int kMw = M == 64 ? 2 : 1, kAcross = kLrWarps / (kM16 / kMw);      // of the second product: 16-row tiles of a warp, warps over columns
 };
 
-// The rank values wait for the second product in two parts, each of the inputs' 16-bit type (f16 over a power of two for each row, so that neither large nor
-// small ones are lost) or TF32.
-template <typename T, int R, int M, bool BACK> struct LrSmem {
+// SPLIT: the rank values are all that is made.  Else they wait for the second product in two parts, each of the inputs' 16-bit type (f16 over a power of two for
+// each row, so that neither large nor small ones are lost) or TF32, and tiles have 16 rows.
+template <typename T, int R, int M, bool BACK, bool SPLIT> struct LrSmem {
   static constexpr int kPad = 16 / sizeof(T);
   static constexpr int kChunk = LrShape<M>::kChunk;
   static constexpr int kPitchX = kChunk + kPad, kPitchW = BACK ? R + 8 : kChunk + kPad, kRowsW = BACK ? kChunk : R;
   static constexpr int kStage = (M * kPitchX + kRowsW * kPitchW) * (int)sizeof(T);
   static constexpr int kJoin = LrShape<M>::kParts * M * R * 4;         // the warps' parts, over the stages
-  static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = 2 * M * kPitchH * (int)sizeof(T);
+  static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = SPLIT ? 0 : 2 * M * kPitchH * (int)sizeof(T);
   // what of base is on its way: each lane's own 16 bytes, `kDepth` steps of a warp
-  static constexpr int kDepth = sizeof(T) == 4 ? (M == 16 ? 2 : 1) : M == 16 ? 4 : 3, kPieces = LrShape<M>::kMw * 2 * (int)sizeof(T) / 2;
-  static constexpr int kBase = BACK ? 0 : kLrWarps * kDepth * kPieces * 512;
+  static constexpr int kDepth = sizeof(T) == 4 ? 2 : 4, kPieces = (int)sizeof(T);
+  static constexpr int kBase = BACK || SPLIT ? 0 : kLrWarps * kDepth * kPieces * 512;
   // as many stages as leave room for two blocks on an SM, or one where the rank is large
   static constexpr int kMost = R <= 32 ? kLrSmemHalf : kLrSmemMost;
   static constexpr int ring(int stages) { return stages * kStage > kJoin ? stages * kStage : kJoin; }
@@ -317,11 +449,13 @@ template <typename T, int R, int M, bool BACK> struct LrSmem {
   static constexpr int kStages = bytes(4) <= kMost ? 4 : bytes(3) <= kMost ? 3 : 2, kRing = ring(kStages), kBytes = bytes(kStages);
 };
 
-template <typename T, int R, int M, bool BACK>
-__global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(const __grid_constant__ LrRowsArgs a) {
+template <typename T, int R, int M, bool BACK, bool SPLIT>
+__global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2 ? 3 : R <= 32 ? 2 : 1) lr_rows_kernel(const __grid_constant__ LrRowsArgs a) {
   using S = LrShape<M>;
-  using L = LrSmem<T, R, M, BACK>;
-  constexpr bool F32 = sizeof(T) == 4;
+  using L = LrSmem<T, R, M, BACK, SPLIT>;
+  static_assert(SPLIT || M == 16, "tiles of 16 rows");
+  constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value, BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kStep = LrStep<T>::kStep, kEach = LrStep<T>::kEach;
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
   __shared__ int rows[M];
   __shared__ float factors[M];
@@ -337,38 +471,24 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
   if (tile.count == 0) return;                        // the whole cluster
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const bool has = tile.group < a.groups.adapters;
+  if (SPLIT && !has) return;
   const uint2 key = a.drop_x || a.drop_y ? philox_key(a.drop) : make_uint2(0, 0);
 
-  // The second product: a warp takes 32 columns at a time.  Column 8 (c / 2) + 2 j + c % 2 is column c of its j-th product, so that the eight values that
-  // a thread has of a row lie side by side.
-  const T* w2 = (const T*)a.w2 + (has ? (long long)tile.group * a.cols * a.rank : 0);
-  const int all = (a.cols + 31) / 32, me = warp / S::kAcross * S::kMw * 16;
-  const int b0 = (int)((long long)all * rank / ranks), b1 = a.y != nullptr ? (int)((long long)all * (rank + 1) / ranks) : b0;
-  long long at_base[S::kMw][2], at_y[S::kMw][2];
-  bool live[S::kMw][2];
-#pragma unroll
-  for (int m = 0; m < S::kMw; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = rows[me + m * 16 + h * 8 + g];
-      live[m][h] = row >= 0;
-      at_base[m][h] = (long long)(row < 0 ? 0 : row) * a.ld_base;
-      at_y[m][h] = (long long)(row < 0 ? 0 : row) * a.ldy;
-    }
+  const int all = (a.cols + 31) / 32;
+  const int b0 = (int)((long long)all * rank / ranks), b1 = !SPLIT && a.y != nullptr ? (int)((long long)all * (rank + 1) / ranks) : b0;
+  const int row_of[2] = {SPLIT ? -1 : rows[g], SPLIT ? -1 : rows[g + 8]};
   uint4* ahead = reinterpret_cast<uint4*>(behind + L::kPart + L::kH) + warp * L::kDepth * L::kPieces * 32 + lane;
-  const bool fetched = !BACK && a.base != nullptr && a.vec_y;
+  const bool fetched = !BACK && !SPLIT && a.base != nullptr && a.vec_y;
   auto request = [&](int i) {           // base of this warp's i-th step
-    if constexpr (!BACK) {
-      const int b = b0 + warp % S::kAcross + i * S::kAcross, col = b * 32 + 8 * t;
+    if constexpr (!BACK && !SPLIT) {
+      const int b = b0 + warp + i * kLrWarps, col = b * 32 + 8 * t;
       if (fetched && b < b1 && col < a.cols) {
         uint4* to = ahead + i % L::kDepth * L::kPieces * 32;
 #pragma unroll
-        for (int m = 0; m < S::kMw; ++m)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int v = 0; v < (int)sizeof(T) / 2; ++v)
-              if (live[m][h]) lr_copy16(to + ((m * 2 + h) * ((int)sizeof(T) / 2) + v) * 32, (const T*)a.base + at_base[m][h] + col + v * (16 / (int)sizeof(T)));
+          for (int v = 0; v < (int)sizeof(T) / 2; ++v)
+            if (row_of[h] >= 0) lr_copy16(to + (h * ((int)sizeof(T) / 2) + v) * 32, (const T*)a.base + row_of[h] * a.ld_base + col + v * (16 / (int)sizeof(T)));
       }
     }
   };
@@ -510,45 +630,42 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
       const int row = u / kLanes, col = u % kLanes * 4;
       // behind the rank there is nothing, also beside an infinity, whose product with the zeros there is none
       float f[4] = {col < a.rank ? v.x * share : 0.0f, col + 1 < a.rank ? v.y * share : 0.0f, col + 2 < a.rank ? v.z * share : 0.0f, col + 3 < a.rank ? v.w * share : 0.0f};
-      const bool keeps = a.kept != nullptr && rank == 0 && row < tile.count;
-      const long long place = (long long)(tile.place + row) * R + col;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
-        if (keeps) *reinterpret_cast<float4*>((float*)a.kept + place) = make_float4(f[0], f[1], f[2], f[3]);
-        float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+      const bool keeps = a.kept.values != nullptr && rank == 0 && row < tile.count;
+      const long long place = (long long)(tile.place + row) * R + col, second = (long long)a.groups.n * R;
+      if (!BF16 && keeps) *reinterpret_cast<float4*>((float*)a.kept.values + place) = make_float4(f[0], f[1], f[2], f[3]);
+      if constexpr (F16) {
+        float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))), down;
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // the row's largest value between 2^13 and 2^14; zeros, infinities and what is next to them stay as they are
-        const int e = (int)(__float_as_uint(top) >> 23 & 255u) - 127 - 13;
-        const bool scaled = top > 1e-30f && top < 1e30f;
-        const float down = scaled ? __uint_as_float((unsigned)(127 - e) << 23) : 1.0f;
-        if (col == 0) factors[row] = scaled ? __uint_as_float((unsigned)(127 + e) << 23) : 1.0f;
+        const float up = lr_power(top, down);
+        if (col == 0) {
+          factors[row] = up;
+          if (keeps && a.kept.factors != nullptr) a.kept.factors[tile.place + row] = up;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] *= down;
       }
       if constexpr (F32) {
-        if (keeps) *reinterpret_cast<float4*>((float*)a.kept + place) = make_float4(f[0], f[1], f[2], f[3]);
-        uint4 hi, lo;
-        lr_split(f[0], hi.x, lo.x);
-        lr_split(f[1], hi.y, lo.y);
-        lr_split(f[2], hi.z, lo.z);
-        lr_split(f[3], hi.w, lo.w);
-        *reinterpret_cast<uint4*>(hs + row * L::kPitchH + col) = hi;
-        *reinterpret_cast<uint4*>(hs + (M + row) * L::kPitchH + col) = lo;
+        if constexpr (!SPLIT) {
+          uint4 hi, lo;
+          lr_split(f[0], hi.x, lo.x);
+          lr_split(f[1], hi.y, lo.y);
+          lr_split(f[2], hi.z, lo.z);
+          lr_split(f[3], hi.w, lo.w);
+          *reinterpret_cast<uint4*>(hs + row * L::kPitchH + col) = hi;
+          *reinterpret_cast<uint4*>(hs + (M + row) * L::kPitchH + col) = lo;
+        }
       } else {
         __align__(8) T hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          hi[i] = lr_round<T>(f[i]);
-          const float h = lr_float<T>(hi[i]);
-          lo[i] = lr_round<T>(fabsf(h) <= 3.4028234e38f ? f[i] - h : 0.0f);
+        lr_parts<T>(f, hi, lo);
+        if constexpr (!SPLIT) {
+          *reinterpret_cast<uint2*>(hs + row * L::kPitchH + col) = *reinterpret_cast<const uint2*>(hi);
+          *reinterpret_cast<uint2*>(hs + (M + row) * L::kPitchH + col) = *reinterpret_cast<const uint2*>(lo);
         }
-        *reinterpret_cast<uint2*>(hs + row * L::kPitchH + col) = *reinterpret_cast<const uint2*>(hi);
-        *reinterpret_cast<uint2*>(hs + (M + row) * L::kPitchH + col) = *reinterpret_cast<const uint2*>(lo);
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          if (keeps) {
-            *reinterpret_cast<uint2*>((T*)a.kept + place) = *reinterpret_cast<const uint2*>(hi);
-            *reinterpret_cast<uint2*>((T*)a.kept + (long long)a.groups.n * R + place) = *reinterpret_cast<const uint2*>(lo);
-          }
+        T* to = BF16 ? (T*)a.kept.values : (T*)a.kept.parts;
+        if (keeps && to != nullptr) {
+          *reinterpret_cast<uint2*>(to + place) = *reinterpret_cast<const uint2*>(hi);
+          *reinterpret_cast<uint2*>(to + second + place) = *reinterpret_cast<const uint2*>(lo);
         }
       }
     }
@@ -562,139 +679,58 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
     lr_wait<0>();
   }
 
-  // Of the rank values the thread has 4 t .. 4 t + 3 of every sixteen (f32: 2 t and 2 t + 1 of every eight): the axis of a product may be taken in any order, and
-  // so its factors lie side by side.
-  constexpr int kStep = F32 ? 8 : 16, kEach = kStep / 4;
-  const T* w2t = BACK ? w2 + (long long)(kEach * t) * a.cols + 8 * (g >> 1) : w2 + (long long)(8 * (g >> 1) + (g & 1)) * a.rank + kEach * t;
-  auto load_w = [&](int b, int k, uint32_t (*w)[2]) {
-    const int wc = b * 32 + 8 * (g >> 1), kk = k + kEach * t;      // eight columns, of which this thread takes every second
-    if (BACK) {
-      uint32_t v[kEach][F32 ? 8 : 4];
+  if constexpr (!SPLIT) {              // y = base + s W2 h
+    const LrFactor<T, BACK> w2((const T*)a.w2 + (has ? (long long)tile.group * a.cols * a.rank : 0), a.cols, a.rank, a.vec_w2, g, t);
+    auto load_h = [&](int k, int part, uint32_t* h) {
+      const T* p = hs + (part * M + g) * L::kPitchH + k + kEach * t;
+      const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(p + 8 * L::kPitchH);
+      h[0] = u.x; h[1] = v.x; h[2] = u.y; h[3] = v.y;
+    };
+    const float by = (a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale) * (a.drop_y ? a.drop.share : 1.0f);
+    const float scaled[2] = {F16 && has ? by * factors[g] : by, F16 && has ? by * factors[g + 8] : by};
+    constexpr bool kHold = R == 16;                                  // the rank values and the next factors stay in registers
+    constexpr int kSteps = kHold ? R / kStep : 1;
+    uint32_t held[kSteps][2][4], next[kSteps][4][2];
+    int b = b0 + warp;
+    if (kHold && has) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const T* p = w2t + (long long)(k + i) * a.cols + b * 32;
-        const bool there = kk + i < a.rank && wc < a.cols;
-        if (a.vec_w2) {
-#pragma unroll
-          for (int q = 0; q < (int)sizeof(T) / 2; ++q) {
-            const uint4 u = there ? reinterpret_cast<const uint4*>(p)[q] : make_uint4(0, 0, 0, 0);
-            v[i][4 * q] = u.x; v[i][4 * q + 1] = u.y; v[i][4 * q + 2] = u.z; v[i][4 * q + 3] = u.w;
-          }
-        } else {
-          __align__(16) T e[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) e[q] = there && wc + q < a.cols ? p[q] : lr_round<T>(0.0f);
-#pragma unroll
-          for (int q = 0; q < (F32 ? 8 : 4); ++q) v[i][q] = reinterpret_cast<const uint32_t*>(e)[q];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (F32) {
-          w[j][0] = g & 1 ? v[0][2 * j + 1] : v[0][2 * j];
-          w[j][1] = g & 1 ? v[1][2 * j + 1] : v[1][2 * j];
-        } else {
-          const unsigned pick = g & 1 ? 0x7632u : 0x5410u;        // the upper or the lower halves of two words
-          w[j][0] = __byte_perm(v[0][j], v[1][j], pick);
-          w[j][1] = __byte_perm(v[kEach - 2][j], v[kEach - 1][j], pick);
-        }
-      }
-    } else {
-      const T* first = w2t + (long long)b * 32 * a.rank + k;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int cc = wc + 2 * j + (g & 1);
-        const T* p = first + 2 * j * a.rank;
-        if (a.vec_w2) {
-          const uint2 u = cc < a.cols && kk < a.rank ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
-          w[j][0] = u.x; w[j][1] = u.y;
-        } else {
-          __align__(8) T e[kEach];
-#pragma unroll
-          for (int q = 0; q < kEach; ++q) e[q] = cc < a.cols && kk + q < a.rank ? p[q] : lr_round<T>(0.0f);
-          w[j][0] = reinterpret_cast<const uint32_t*>(e)[0];
-          w[j][1] = reinterpret_cast<const uint32_t*>(e)[1];
-        }
+      for (int k = 0; k < kSteps; ++k) {
+        load_h(k * kStep, 0, held[k][0]);
+        load_h(k * kStep, 1, held[k][1]);
+        if (b < b1) w2.load(b, k * kStep, next[k]);
       }
     }
-  };
-  auto load_h = [&](int m, int k, int part, uint32_t* h) {
-    const T* p = hs + (part * M + me + m * 16 + g) * L::kPitchH + k + kEach * t;
-    const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(p + 8 * L::kPitchH);
-    h[0] = u.x; h[1] = v.x; h[2] = u.y; h[3] = v.y;
-  };
-  const float by = (a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale) * (a.drop_y ? a.drop.share : 1.0f);
-  float scaled[S::kMw][2];
+    for (int i = 0; b < b1; b += kLrWarps, ++i) {
+      const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
+      float acc[4][4];
+      if (has) {
+        if constexpr (kHold) {
+          uint32_t w[kSteps][4][2];
 #pragma unroll
-  for (int m = 0; m < S::kMw; ++m)
+          for (int k = 0; k < kSteps; ++k) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) scaled[m][h] = has && sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? by * factors[me + m * 16 + h * 8 + g] : by;
-  constexpr bool kHold = R == 16;                                  // the rank values and the next factors stay in registers
-  uint32_t held[kHold ? R / kStep : 1][S::kMw][2][4], next[kHold ? R / kStep : 1][4][2];
-  int b = b0 + warp % S::kAcross;
-  if (kHold && has) {
-#pragma unroll
-    for (int k = 0; k < R / kStep; ++k) {
-#pragma unroll
-      for (int m = 0; m < S::kMw; ++m)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) load_h(m, k * kStep, p, held[k][m][p]);
-      if (b < b1) load_w(b, k * kStep, next[k]);
-    }
-  }
-  for (int i = 0; b < b1; b += S::kAcross, ++i) {
-    const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
-    float acc[S::kMw][4][4];
-    if (has) {
-      auto multiply = [&](uint32_t (*w)[2], auto h, bool start) {
-#pragma unroll
-        for (int m = 0; m < S::kMw; ++m)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (F32) {
-              uint32_t h0, l0, h1, l1;
-              lr_split(__uint_as_float(w[j][0]), h0, l0);
-              lr_split(__uint_as_float(w[j][1]), h1, l1);
-              lr_mma8(acc[m][j], h(m, 1), h0, h1, start);
-              lr_mma8(acc[m][j], h(m, 0), l0, l1);
-              lr_mma8(acc[m][j], h(m, 0), h0, h1);
-            } else {
-              lr_mma16<T>(acc[m][j], h(m, 1), w[j][0], w[j][1], start);
-              lr_mma16<T>(acc[m][j], h(m, 0), w[j][0], w[j][1]);
-            }
+            for (int j = 0; j < 4; ++j) { w[k][j][0] = next[k][j][0]; w[k][j][1] = next[k][j][1]; }
+            if (b + kLrWarps < b1) w2.load(b + kLrWarps, k * kStep, next[k]);
           }
-      };
-      if constexpr (kHold) {
-        uint32_t w[R / kStep][4][2];
 #pragma unroll
-        for (int k = 0; k < R / kStep; ++k) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { w[k][j][0] = next[k][j][0]; w[k][j][1] = next[k][j][1]; }
-          if (b + S::kAcross < b1) load_w(b + S::kAcross, k * kStep, next[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < R / kStep; ++k) multiply(w[k], [&](int m, int p) -> const uint32_t* { return held[k][m][p]; }, k == 0);
-      } else {
+          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[k], k == 0);
+        } else {
 #pragma unroll 2
-        for (int k = 0; k < R; k += kStep) {
-          if (k >= a.rank) break;
-          uint32_t w[4][2], hv[S::kMw][2][4];
-          load_w(b, k, w);
-#pragma unroll
-          for (int m = 0; m < S::kMw; ++m)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) load_h(m, k, p, hv[m][p]);
-          multiply(w, [&](int m, int p) -> const uint32_t* { return hv[m][p]; }, k == 0);
+          for (int k = 0; k < R; k += kStep) {
+            if (k >= a.rank) break;
+            uint32_t w[4][2], hi[4], lo[4];
+            w2.load(b, k, w);
+            load_h(k, 0, hi);
+            load_h(k, 1, lo);
+            lr_multiply<T>(acc, hi, lo, w, k == 0);
+          }
         }
       }
-    }
-    if (!BACK) lr_wait<L::kDepth - 1>();
-    const uint4* here = ahead + i % L::kDepth * L::kPieces * 32;
-#pragma unroll
-    for (int m = 0; m < S::kMw; ++m)
+      if (!BACK) lr_wait<L::kDepth - 1>();
+      const uint4* here = ahead + i % L::kDepth * L::kPieces * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!live[m][h] || left <= 0) continue;
+        if (row_of[h] < 0 || left <= 0) continue;
         float v[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = 0.0f;
@@ -702,38 +738,187 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 2 : 1) lr_rows_kernel(co
           if (a.vec_y) {
             __align__(16) T e[8];
 #pragma unroll
-            for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(e)[q] = here[((m * 2 + h) * ((int)sizeof(T) / 2) + q) * 32];
+            for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(e)[q] = here[(h * ((int)sizeof(T) / 2) + q) * 32];
             lr_load8<T, true>(e, 8, v);
           } else {
-            lr_load8<T, false>((const T*)a.base + at_base[m][h] + col, left, v);
+            lr_load8<T, false>((const T*)a.base + row_of[h] * a.ld_base + col, left, v);
           }
         }
         if (has) {
-#pragma unroll
-          for (int q = 0; q < 8; q += 2) {
-            float* d = &acc[m][q >> 1][2 * h];
-            lr_fma2(d, scaled[m][h], v + q);
-            v[q] = d[0]; v[q + 1] = d[1];
-          }
-          if (BACK && a.drop_y) {
-            const uint4 words = dropout_words((unsigned)col >> 3, rows[me + m * 16 + h * 8 + g], key);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = dropout_keeps(words, q, a.drop.limit) ? v[q] : 0.0f;
-          }
+          uint4 words;
+          if (BACK && a.drop_y) words = dropout_words((unsigned)col >> 3, row_of[h], key);
+          lr_finish(v, acc, h, scaled[h], BACK && a.drop_y ? &words : nullptr, a.drop.limit);
         } else if (tile.group > a.groups.adapters) {
 #pragma unroll
           for (int q = 0; q < 8; ++q) v[q] = __uint_as_float(0x7fc00000u);
         }
-        T* p = (T*)a.y + at_y[m][h] + col;
+        T* p = (T*)a.y + row_of[h] * a.ldy + col;
         if (a.vec_y) lr_store8<T, true>(p, 8, v);
         else lr_store8<T, false>(p, left, v);
       }
-    request(i + L::kDepth);
-    if (!BACK) lr_commit();
+      request(i + L::kDepth);
+      if (!BACK) lr_commit();
+    }
+    lr_wait<0>();
   }
-  lr_wait<0>();
   __syncwarp();
   if (has) lr_meet();
+}
+
+// ---- the second product of many rows ---------------------------------------------------------------------------------------------------------
+// y = base + s W2 h, h by place.  A warp takes 16 rows of one adapter and walks over blocks of columns, its own lanes' pieces of base two blocks ahead in shared
+// memory; warps do not wait for one another.
+template <typename T, int R, bool BACK> struct LrExpand {
+  static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4, kCols = 32 * kGroups;         // of a block of columns
+  static constexpr int kStages = 2, kPieces = 8, kBytes = BACK ? 0 : kLrWarps * kStages * kPieces * 512;
+  static constexpr bool kHold = R <= 32;
+  static constexpr int kBlocks = R == 16 && sizeof(T) == 2 ? 3 : 2;                    // on an SM
+};
+
+template <typename T, int R, bool BACK>
+__global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_expand_kernel(const __grid_constant__ LrRowsArgs a, int tiles, int row_blocks, int per) {
+  using X = LrExpand<T, R, BACK>;
+  constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value, BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kStep = LrStep<T>::kStep, kEach = LrStep<T>::kEach, kSize = (int)sizeof(T) / 2;
+  extern __shared__ __align__(16) unsigned char lr_dynamic[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int index = blockIdx.x % row_blocks * kLrWarps + warp;
+  if (index >= tiles) return;
+  int group = 0, place = index * 16, count = a.groups.n - place;
+  if (a.groups.mode == LR_PLAN) {
+    const int4 tile = a.groups.tiles[index];
+    group = tile.x; place = tile.y; count = tile.z;
+    if (group < 0) return;
+  }
+  const bool has = group < a.groups.adapters;
+  const int blocks = (a.cols + X::kCols - 1) / X::kCols, c0 = blockIdx.x / row_blocks * per, c1 = c0 + per < blocks ? c0 + per : blocks;
+  int row_of[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = g + 8 * h;
+    row_of[h] = r < count ? (a.groups.mode == LR_PLAN ? a.groups.order[place + r] : place + r) : -1;
+  }
+  const bool fetched = !BACK && a.base != nullptr && a.vec_y;
+  const T* from[2] = {(const T*)a.base + (row_of[0] < 0 ? 0 : row_of[0]) * a.ld_base + 8 * t, (const T*)a.base + (row_of[1] < 0 ? 0 : row_of[1]) * a.ld_base + 8 * t};
+  T* to[2] = {(T*)a.y + (row_of[0] < 0 ? 0 : row_of[0]) * a.ldy + 8 * t, (T*)a.y + (row_of[1] < 0 ? 0 : row_of[1]) * a.ldy + 8 * t};
+  uint4* ring = reinterpret_cast<uint4*>(lr_dynamic) + warp * X::kStages * X::kPieces * 32 + lane;
+  auto request = [&](int c, int stage) {
+    if constexpr (!BACK) {
+      if (fetched && c < c1) {
+#pragma unroll
+        for (int q = 0; q < X::kGroups; ++q)
+          if (c * X::kCols + q * 32 + 8 * t < a.cols) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int v = 0; v < kSize; ++v)
+                if (row_of[h] >= 0) lr_copy16(ring + ((stage * X::kGroups + q) * 2 * kSize + h * kSize + v) * 32, from[h] + c * X::kCols + q * 32 + v * (8 / kSize));
+          }
+      }
+      lr_commit();
+    }
+  };
+  request(c0, 0);
+  request(c0 + 1, 1);
+  const uint2 key = a.drop_y ? philox_key(a.drop) : make_uint2(0, 0);
+  const LrFactor<T, BACK> w2((const T*)a.w2 + (has ? (long long)group * a.cols * a.rank : 0), a.cols, a.rank, a.vec_w2, g, t);
+  // two parts of the rank values; rows behind the last have those of the first one, which go nowhere
+  const long long at[2] = {(long long)(place + (g < count ? g : 0)) * R + kEach * t, (long long)(place + (g + 8 < count ? g + 8 : 0)) * R + kEach * t};
+  auto load_h = [&](int k, uint32_t* hi, uint32_t* lo) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 f = *reinterpret_cast<const float2*>((const float*)a.kept.values + at[h] + k);
+        lr_split(f.x, hi[h], lo[h]);
+        lr_split(f.y, hi[2 + h], lo[2 + h]);
+      }
+    } else {
+      const T* p = BF16 ? (const T*)a.kept.values : (const T*)a.kept.parts;
+      const long long second = (long long)a.groups.n * R;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p + at[h] + k), v = *reinterpret_cast<const uint2*>(p + second + at[h] + k);
+        hi[h] = u.x; hi[2 + h] = u.y;
+        lo[h] = v.x; lo[2 + h] = v.y;
+      }
+    }
+  };
+  float scaled[2];
+  {
+    const float by = (a.scales != nullptr ? (has ? a.scales[group] : 0.0f) : a.scale) * (a.drop_y ? a.drop.share : 1.0f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) scaled[h] = F16 && has ? by * a.kept.factors[place + (g + 8 * h < count ? g + 8 * h : 0)] : by;
+  }
+  constexpr int kSteps = X::kHold ? R / kStep : 1;
+  uint32_t held[kSteps][2][4], next[kSteps][4][2];
+  if (X::kHold && has) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      load_h(k * kStep, held[k][0], held[k][1]);
+      w2.load(c0 * X::kGroups, k * kStep, next[k]);
+    }
+  }
+  for (int c = c0, stage = 0; c < c1; ++c, stage ^= 1) {
+    if (!BACK) lr_wait<1>();
+#pragma unroll
+    for (int q = 0; q < X::kGroups; ++q) {
+      const int b = c * X::kGroups + q, col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
+      float acc[4][4];
+      if (has) {
+        if constexpr (X::kHold) {
+          uint32_t w[kSteps][4][2];
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { w[k][j][0] = next[k][j][0]; w[k][j][1] = next[k][j][1]; }
+            if (q + 1 < X::kGroups || c + 1 < c1) w2.load(b + 1, k * kStep, next[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[k], k == 0);
+        } else {
+#pragma unroll 2
+          for (int k = 0; k < R; k += kStep) {
+            if (k >= a.rank) break;
+            uint32_t w[4][2], hi[4], lo[4];
+            w2.load(b, k, w);
+            load_h(k, hi, lo);
+            lr_multiply<T>(acc, hi, lo, w, k == 0);
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (row_of[h] < 0 || left <= 0) continue;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (!BACK && a.base != nullptr) {
+          if (a.vec_y) {
+            __align__(16) T e[8];
+#pragma unroll
+            for (int i = 0; i < kSize; ++i) reinterpret_cast<uint4*>(e)[i] = ring[((stage * X::kGroups + q) * 2 * kSize + h * kSize + i) * 32];
+            lr_load8<T, true>(e, 8, v);
+          } else {
+            lr_load8<T, false>(from[h] + b * 32, left, v);
+          }
+        }
+        if (has) {
+          uint4 words;
+          if (BACK && a.drop_y) words = dropout_words((unsigned)col >> 3, row_of[h], key);
+          lr_finish(v, acc, h, scaled[h], BACK && a.drop_y ? &words : nullptr, a.drop.limit);
+        } else if (group > a.groups.adapters) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
+        }
+        if (a.vec_y) lr_store8<T, true>(to[h] + b * 32, 8, v);
+        else lr_store8<T, false>(to[h] + b * 32, left, v);
+      }
+    }
+    request(c + 2, stage);
+  }
+  if (!BACK) lr_wait<0>();
 }
 
 // ---- the factors' gradients --------------------------------------------------------------------------------------------------------------
@@ -963,12 +1148,13 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------------------------
-template <typename Kern, typename Args>
-static cudaError_t lr_launch(Kern kernel, int clusters, int ranks, int smem, cudaStream_t st, const Args& args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename Kern, typename... Args>
+static cudaError_t lr_launch(Kern kernel, long long clusters, int ranks, int smem, cudaStream_t st, const Args&... args) {
+  if (clusters * ranks >= 1ll << 31) return cudaErrorInvalidValue;
+  cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)clusters * ranks);
+  cfg.gridDim = dim3((unsigned)(clusters * ranks));
   cfg.blockDim = dim3(kLrThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -980,7 +1166,7 @@ static cudaError_t lr_launch(Kern kernel, int clusters, int ranks, int smem, cud
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, args);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // Blocks of a cluster: as many, in powers of two, as bring the grid near two blocks an SM, and no more than `most` have work.
@@ -989,30 +1175,45 @@ inline int lr_ranks_for(long long clusters, long long most) {
   while (ranks < 8 && 2 * ranks <= most && clusters * ranks < 148 * 2) ranks *= 2;
   return ranks;
 }
+// Tiles of M rows, the empty ones among them.
+inline long long lr_slots(const LrGroups& g, int M) { return g.mode == LR_ONE ? (g.n + M - 1) / M : g.mode == LR_SELF ? g.n : g.n / M + g.adapters + 2; }
 
-
-template <typename T, int R, int M, bool BACK>
-static cudaError_t lr_rows_as(LrRowsArgs a, cudaStream_t st) {
-  using L = LrSmem<T, R, M, BACK>;
+template <typename T, int R, int M, bool BACK, bool SPLIT>
+static cudaError_t lr_rows_as(const LrRowsArgs& a, cudaStream_t st) {
+  using L = LrSmem<T, R, M, BACK, SPLIT>;
+  static_assert(L::kBytes <= kLrSmemMost, "shared memory");
   const LrGroups& g = a.groups;
-  const long long slots = g.mode == LR_ONE ? (g.n + M - 1) / M : g.mode == LR_SELF ? g.n : g.n / M + g.adapters + 2;
-  const long long busy = g.mode == LR_ONE ? slots : g.n / M + (g.n < g.adapters ? g.n : g.adapters);
+  const long long slots = lr_slots(g, M), busy = g.mode == LR_ONE ? slots : g.n / M + (g.n < g.adapters ? g.n : g.adapters);
   const int chunks = (a.k + L::kChunk - 1) / L::kChunk;
-  const int ranks = lr_ranks_for(busy < 1 ? 1 : busy, chunks > 1 ? chunks : 1);
-  if (slots * ranks >= 1ll << 31) return cudaErrorInvalidValue;
-  return lr_launch(lr_rows_kernel<T, R, M, BACK>, (int)slots, ranks, L::kBytes, st, a);
+  return lr_launch(lr_rows_kernel<T, R, M, BACK, SPLIT>, slots, lr_ranks_for(busy < 1 ? 1 : busy, chunks), L::kBytes, st, a);
+}
+
+template <typename T, int R, bool BACK>
+static cudaError_t lr_expand_as(const LrRowsArgs& a, cudaStream_t st) {
+  using X = LrExpand<T, R, BACK>;
+  const int tiles = (int)lr_slots(a.groups, 16), row_blocks = (tiles + kLrWarps - 1) / kLrWarps, blocks = (a.cols + X::kCols - 1) / X::kCols;
+  // blocks of columns for a block: what leaves the last wave fullest, where a block's start costs about as much as one of them
+  const int resident = 148 * X::kBlocks;
+  int per = 1;
+  double least = 1e30;
+  for (int p = 1; p <= 16 && p <= blocks; ++p) {
+    const long long grid = (long long)row_blocks * ((blocks + p - 1) / p);
+    const double cost = (double)((grid + resident - 1) / resident) * (p + 1);
+    if (cost < least) { least = cost; per = p; }
+  }
+  const long long grid = (long long)row_blocks * ((blocks + per - 1) / per);
+  return lr_launch(lr_expand_kernel<T, R, BACK>, grid, 1, X::kBytes, st, a, tiles, row_blocks, per);
 }
 
 template <typename T, int R, bool BACK>
 static cudaError_t lr_rows_r(const LrRowsArgs& a, cudaStream_t st) {
   const LrGroups& g = a.groups;
+  if (g.n < kLrSplit) return lr_rows_as<T, R, 16, BACK, false>(a, st);
   // Tiles of 64 rows where adapters fill them; 16 rows keep more clusters busy and waste less of the tiles
-  const long long each = g.mode == LR_ONE ? g.n : g.n / (g.adapters > 0 ? g.adapters : 1);
-  static_assert(LrSmem<T, R, 16, BACK>::kBytes <= kLrSmemMost, "shared memory");
-  if constexpr (LrSmem<T, R, 64, BACK>::kBytes <= kLrSmemMost) {       // f32 of rank above 64 has too large ones
-    if (g.mode != LR_SELF && each >= 48 && g.n >= 1024) return lr_rows_as<T, R, 64, BACK>(a, st);
-  }
-  return lr_rows_as<T, R, 16, BACK>(a, st);
+  cudaError_t e;
+  if (g.n / g.adapters >= 48) e = lr_rows_as<T, R, 64, BACK, true>(a, st);
+  else e = lr_rows_as<T, R, 16, BACK, true>(a, st);
+  return e == cudaSuccess && a.y != nullptr ? lr_expand_as<T, R, BACK>(a, st) : e;
 }
 
 template <typename T, int R>

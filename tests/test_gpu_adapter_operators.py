@@ -205,6 +205,11 @@ def test_update_gradient_by_differences():
         assert abs(ends[0] - ends[1] - float((grad.double() * way).sum())) <= 2.0 ** -20 * 40 * 32 * 24
 
 
+def test_rows_that_are_grouped_without_a_plan():
+    from oxibonsai_b200.ops import train_ops
+    assert train_ops._LR_SELF_ROWS == train_ops._lib().bonsai_lr_self_rows()
+
+
 def test_update_no_rows():
     x, base, dy, a, b, scales, ids = update_inputs(4, 16, 8, 2, 3, torch.float32, DEV)
     got = run_update(x[:0], base[:0], dy[:0], a, b, scales, ids[:0])
