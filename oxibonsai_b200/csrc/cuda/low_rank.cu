@@ -189,8 +189,6 @@ int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long l
     o.vec[0] = lr_vec(x, ldx, d, size);
     o.vec[1] = lr_vec(dy, lddy, out, size);
     o.rank = rank;
-    o.scales = scales;
-    o.scale = scale;
     o.drop = rule;
     o.drop_x = steps < 65536;
     e = type == 0 ? lr_outer<float>(o, st) : type == 1 ? lr_outer<__half>(o, st) : lr_outer<__nv_bfloat16>(o, st);

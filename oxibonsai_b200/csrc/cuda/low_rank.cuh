@@ -27,7 +27,7 @@ namespace bonsai {
 constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
 // From so many rows on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.
 constexpr int kLrSplit = 1024;
-constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024;        // dynamic shared memory of a block, of each of two on an SM
+constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024, kLrSmemThird = 74 * 1024;        // dynamic shared memory of a block, of each of two or three on an SM
 constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
 enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
 
@@ -41,7 +41,7 @@ struct LrGroups {            // which rows have which adapter
   int n, adapters;
 };
 
-// The rank values of a forward or a backward pass, by place in the order: f32 [n][R] (R: the padded rank), of bf16 two parts [2][n][R].  f16 for the second
+// The rank values of a forward or a backward pass, times the adapter's scale, by place in the order: f32 [n][R] (R: the padded rank), of bf16 two parts [2][n][R].  f16 for the second
 // product: two parts over a power of two for each row, and that power.
 struct LrValues {
   void* values;
@@ -72,8 +72,6 @@ struct LrOuterArgs {
   void* out[2];
   int width[2], blocks[2], vec[2];       // columns, blocks of columns
   int rank;
-  const float* scales;
-  float scale;
   DropoutRule drop;
   int drop_x;
 };
@@ -103,13 +101,6 @@ template <> __device__ __forceinline__ uint32_t lr_two<__nv_bfloat16>(float a, f
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// a * s + c of two values at once
-__device__ __forceinline__ void lr_fma2(float* a, float s, const float* c) {
-  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %2};\nmov.b64 z, {%3, %4};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
-      : "+f"(a[0]), "+f"(a[1])
-      : "f"(s), "f"(c[0]), "f"(c[1]));
-}
-
 // eight neighbouring values
 template <typename T, bool VEC>
 __device__ __forceinline__ void lr_load8(const T* p, int n, float* v) {
@@ -161,24 +152,22 @@ __device__ __forceinline__ void lr_ldm4(uint32_t* r, const void* p) {
 __device__ __forceinline__ void lr_ldm4t(uint32_t* r, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(lr_smem(p)) : "memory");
 }
-// d = a b + d, or a b
-#define LR_MMA(name, shape, types)                                                                                                     \
-  __device__ __forceinline__ void name(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool start) {                                  \
-    const float c0 = start ? 0.0f : d[0], c1 = start ? 0.0f : d[1], c2 = start ? 0.0f : d[2], c3 = start ? 0.0f : d[3];                      \
-    asm volatile("mma.sync.aligned." shape ".row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"            \
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                                            \
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));                        \
+// d = a b + d
+#define LR_MMA(name, shape, types)                                                                                                           \
+  __device__ __forceinline__ void name(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {                                              \
+    asm volatile("mma.sync.aligned." shape ".row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                \
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                                            \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                                            \
   }
 LR_MMA(lr_mma_f16, "m16n8k16", "f16.f16")
 LR_MMA(lr_mma_bf16, "m16n8k16", "bf16.bf16")
-LR_MMA(lr_mma_tf32, "m16n8k8", "tf32.tf32")
+LR_MMA(lr_mma8, "m16n8k8", "tf32.tf32")
 #undef LR_MMA
 template <typename T>
-__device__ __forceinline__ void lr_mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool start = false) {
-  if constexpr (std::is_same<T, __half>::value) lr_mma_f16(d, a, b0, b1, start);
-  else lr_mma_bf16(d, a, b0, b1, start);
+__device__ __forceinline__ void lr_mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) lr_mma_f16(d, a, b0, b1);
+  else lr_mma_bf16(d, a, b0, b1);
 }
-__device__ __forceinline__ void lr_mma8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, bool start = false) { lr_mma_tf32(d, a, b0, b1, start); }
 __device__ __forceinline__ uint32_t lr_tf32(float v) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
@@ -376,35 +365,45 @@ struct LrFactor {              // w2 of one adapter: forward [cols][rank], backw
 
 // acc += the rank values of 16 rows (two parts) times the factors of 32 columns
 template <typename T>
-__device__ __forceinline__ void lr_multiply(float (*acc)[4], const uint32_t* hi, const uint32_t* lo, const uint32_t (*w)[2], bool start) {
+__device__ __forceinline__ void lr_multiply(float (*acc)[4], const uint32_t* hi, const uint32_t* lo, const uint32_t (*w)[2]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if constexpr (sizeof(T) == 4) {
       uint32_t h0, l0, h1, l1;
       lr_split(__uint_as_float(w[j][0]), h0, l0);
       lr_split(__uint_as_float(w[j][1]), h1, l1);
-      lr_mma8(acc[j], lo, h0, h1, start);
+      lr_mma8(acc[j], lo, h0, h1);
       lr_mma8(acc[j], hi, l0, l1);
       lr_mma8(acc[j], hi, h0, h1);
     } else {
-      lr_mma16<T>(acc[j], lo, w[j][0], w[j][1], start);
+      lr_mma16<T>(acc[j], lo, w[j][0], w[j][1]);
       lr_mma16<T>(acc[j], hi, w[j][0], w[j][1]);
     }
   }
 }
 
-// v (base, or zeros) + the eight sums of row g + 8 h, dropped where asked
-__device__ __forceinline__ void lr_finish(float* v, float (*acc)[4], int h, float scale, const uint4* words, unsigned limit) {
+// What the sums of a block start from.  bf16: base itself, so that the matrix instructions add it; a last bit of f32 that they cut off is far below bf16's.
+// f32 would lose that bit, f16 has its rows over a power of two: zeros, and base is added behind.
+template <typename T> struct LrStart {
+  static constexpr bool kBase = std::is_same<T, __nv_bfloat16>::value;
+};
+// the eight values of row g + 8 h that a thread has in the sums
+template <typename T>
+__device__ __forceinline__ void lr_set(float (*acc)[4], int h, const float* v) {
 #pragma unroll
-  for (int q = 0; q < 8; q += 2) {
-    float* d = &acc[q >> 1][2 * h];
-    lr_fma2(d, scale, v + q);
-    v[q] = d[0]; v[q + 1] = d[1];
-  }
-  if (words != nullptr) {
+  for (int q = 0; q < 8; ++q) acc[q >> 1][2 * h + (q & 1)] = v[q];
+}
+template <typename T>
+__device__ __forceinline__ void lr_get(float (*acc)[4], int h, float up, const float* base, float* v) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = dropout_keeps(*words, q, limit) ? v[q] : 0.0f;
+  for (int q = 0; q < 8; ++q) {
+    const float d = acc[q >> 1][2 * h + (q & 1)];
+    v[q] = LrStart<T>::kBase ? d : std::is_same<T, __half>::value ? fmaf(d, up, base[q]) : d + base[q];
   }
+}
+__device__ __forceinline__ void lr_drop(float* v, const uint4& words, unsigned limit) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = dropout_keeps(words, q, limit) ? v[q] : 0.0f;
 }
 
 // f16: the power of two that brings a row's largest rank value between 2^13 and 2^14, and one over it; 1 for zeros, infinities and what is next to them
@@ -425,25 +424,25 @@ __device__ __forceinline__ void lr_parts(const float* f, T* hi, T* lo) {
 }
 
 // ---- the rows ------------------------------------------------------------------------------------------------------------------------------
-template <int M> struct LrShape {
+template <typename T, int M> struct LrShape {
   static constexpr int kM16 = M / 16, kParts = kLrWarps / kM16;       // warps over rows, and over the long axis
-  static constexpr int kChunk = M == 64 ? 64 : 128, kWarpK = kChunk / kParts;
+  static constexpr int kChunk = M == 64 && sizeof(T) == 4 ? 64 : 128, kWarpK = kChunk / kParts;
 };
 
 // SPLIT: the rank values are all that is made.  Else they wait for the second product in two parts, each of the inputs' 16-bit type (f16 over a power of two for
 // each row, so that neither large nor small ones are lost) or TF32, and tiles have 16 rows.
 template <typename T, int R, int M, bool BACK, bool SPLIT> struct LrSmem {
   static constexpr int kPad = 16 / sizeof(T);
-  static constexpr int kChunk = LrShape<M>::kChunk;
+  static constexpr int kChunk = LrShape<T, M>::kChunk;
   static constexpr int kPitchX = kChunk + kPad, kPitchW = BACK ? R + 8 : kChunk + kPad, kRowsW = BACK ? kChunk : R;
   static constexpr int kStage = (M * kPitchX + kRowsW * kPitchW) * (int)sizeof(T);
-  static constexpr int kJoin = LrShape<M>::kParts * M * R * 4;         // the warps' parts, over the stages
+  static constexpr int kJoin = LrShape<T, M>::kParts * M * R * 4;         // the warps' parts, over the stages
   static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = SPLIT ? 0 : 2 * M * kPitchH * (int)sizeof(T);
   // what of base is on its way: each lane's own 16 bytes, `kDepth` steps of a warp
   static constexpr int kDepth = sizeof(T) == 4 ? 2 : 4, kPieces = (int)sizeof(T);
   static constexpr int kBase = BACK || SPLIT ? 0 : kLrWarps * kDepth * kPieces * 512;
-  // as many stages as leave room for two blocks on an SM, or one where the rank is large
-  static constexpr int kMost = R <= 32 ? kLrSmemHalf : kLrSmemMost;
+  // as many stages as leave room for two blocks on an SM (three that make rank values of 16-bit types), or one where the rank is large
+  static constexpr int kMost = SPLIT && R == 16 && sizeof(T) == 2 ? kLrSmemThird : R <= 32 ? kLrSmemHalf : kLrSmemMost;
   static constexpr int ring(int stages) { return stages * kStage > kJoin ? stages * kStage : kJoin; }
   static constexpr int bytes(int stages) { return ring(stages) + kPart + kH + kBase; }
   static constexpr int kStages = bytes(4) <= kMost ? 4 : bytes(3) <= kMost ? 3 : 2, kRing = ring(kStages), kBytes = bytes(kStages);
@@ -451,7 +450,7 @@ template <typename T, int R, int M, bool BACK, bool SPLIT> struct LrSmem {
 
 template <typename T, int R, int M, bool BACK, bool SPLIT>
 __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2 ? 3 : R <= 32 ? 2 : 1) lr_rows_kernel(const __grid_constant__ LrRowsArgs a) {
-  using S = LrShape<M>;
+  using S = LrShape<T, M>;
   using L = LrSmem<T, R, M, BACK, SPLIT>;
   static_assert(SPLIT || M == 16, "tiles of 16 rows");
   constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value, BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -618,7 +617,7 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
     }
     lr_arrive();
     lr_meet();
-    const float share = a.drop_x ? a.drop.share : 1.0f;
+    const float by = (a.scales != nullptr ? a.scales[tile.group] : a.scale) * (a.drop_x || a.drop_y ? a.drop.share : 1.0f);
     constexpr int kUnits = M * R / 4, kLanes = R / 4;              // of a row: neighbouring lanes
 #pragma unroll 1
     for (int u = threadIdx.x; u < kUnits; u += kLrThreads) {       // a multiple of 32: whole warps
@@ -629,7 +628,7 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
       }
       const int row = u / kLanes, col = u % kLanes * 4;
       // behind the rank there is nothing, also beside an infinity, whose product with the zeros there is none
-      float f[4] = {col < a.rank ? v.x * share : 0.0f, col + 1 < a.rank ? v.y * share : 0.0f, col + 2 < a.rank ? v.z * share : 0.0f, col + 3 < a.rank ? v.w * share : 0.0f};
+      float f[4] = {col < a.rank ? v.x * by : 0.0f, col + 1 < a.rank ? v.y * by : 0.0f, col + 2 < a.rank ? v.z * by : 0.0f, col + 3 < a.rank ? v.w * by : 0.0f};
       const bool keeps = a.kept.values != nullptr && rank == 0 && row < tile.count;
       const long long place = (long long)(tile.place + row) * R + col, second = (long long)a.groups.n * R;
       if (!BF16 && keeps) *reinterpret_cast<float4*>((float*)a.kept.values + place) = make_float4(f[0], f[1], f[2], f[3]);
@@ -686,8 +685,7 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
       const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(p + 8 * L::kPitchH);
       h[0] = u.x; h[1] = v.x; h[2] = u.y; h[3] = v.y;
     };
-    const float by = (a.scales != nullptr ? (has ? a.scales[tile.group] : 0.0f) : a.scale) * (a.drop_y ? a.drop.share : 1.0f);
-    const float scaled[2] = {F16 && has ? by * factors[g] : by, F16 && has ? by * factors[g + 8] : by};
+    const float up[2] = {F16 && has ? factors[g] : 1.0f, F16 && has ? factors[g + 8] : 1.0f};
     constexpr bool kHold = R == 16;                                  // the rank values and the next factors stay in registers
     constexpr int kSteps = kHold ? R / kStep : 1;
     uint32_t held[kSteps][2][4], next[kSteps][4][2];
@@ -702,7 +700,26 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
     }
     for (int i = 0; b < b1; b += kLrWarps, ++i) {
       const int col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
-      float acc[4][4];
+      float acc[4][4], from[2][8];
+      if (!BACK) lr_wait<L::kDepth - 1>();
+      const uint4* here = ahead + i % L::kDepth * L::kPieces * 32;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) from[h][q] = 0.0f;
+        if (!BACK && a.base != nullptr && row_of[h] >= 0 && left > 0) {
+          if (a.vec_y) {
+            __align__(16) T e[8];
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(e)[q] = here[(h * ((int)sizeof(T) / 2) + q) * 32];
+            lr_load8<T, true>(e, 8, from[h]);
+          } else {
+            lr_load8<T, false>((const T*)a.base + row_of[h] * a.ld_base + col, left, from[h]);
+          }
+        }
+        const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        lr_set<T>(acc, h, LrStart<T>::kBase ? from[h] : zeros);
+      }
       if (has) {
         if constexpr (kHold) {
           uint32_t w[kSteps][4][2];
@@ -713,7 +730,7 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
             if (b + kLrWarps < b1) w2.load(b + kLrWarps, k * kStep, next[k]);
           }
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[k], k == 0);
+          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[k]);
         } else {
 #pragma unroll 2
           for (int k = 0; k < R; k += kStep) {
@@ -722,33 +739,17 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
             w2.load(b, k, w);
             load_h(k, 0, hi);
             load_h(k, 1, lo);
-            lr_multiply<T>(acc, hi, lo, w, k == 0);
+            lr_multiply<T>(acc, hi, lo, w);
           }
         }
       }
-      if (!BACK) lr_wait<L::kDepth - 1>();
-      const uint4* here = ahead + i % L::kDepth * L::kPieces * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (row_of[h] < 0 || left <= 0) continue;
         float v[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
-        if (!BACK && a.base != nullptr) {
-          if (a.vec_y) {
-            __align__(16) T e[8];
-#pragma unroll
-            for (int q = 0; q < (int)sizeof(T) / 2; ++q) reinterpret_cast<uint4*>(e)[q] = here[(h * ((int)sizeof(T) / 2) + q) * 32];
-            lr_load8<T, true>(e, 8, v);
-          } else {
-            lr_load8<T, false>((const T*)a.base + row_of[h] * a.ld_base + col, left, v);
-          }
-        }
-        if (has) {
-          uint4 words;
-          if (BACK && a.drop_y) words = dropout_words((unsigned)col >> 3, row_of[h], key);
-          lr_finish(v, acc, h, scaled[h], BACK && a.drop_y ? &words : nullptr, a.drop.limit);
-        } else if (tile.group > a.groups.adapters) {
+        lr_get<T>(acc, h, up[h], from[h], v);
+        if (BACK && a.drop_y && has) lr_drop(v, dropout_words((unsigned)col >> 3, row_of[h], key), a.drop.limit);
+        if (tile.group > a.groups.adapters) {
 #pragma unroll
           for (int q = 0; q < 8; ++q) v[q] = __uint_as_float(0x7fc00000u);
         }
@@ -845,84 +846,88 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
       }
     }
   };
-  float scaled[2];
-  {
-    const float by = (a.scales != nullptr ? (has ? a.scales[group] : 0.0f) : a.scale) * (a.drop_y ? a.drop.share : 1.0f);
+  float up[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) scaled[h] = F16 && has ? by * a.kept.factors[place + (g + 8 * h < count ? g + 8 * h : 0)] : by;
-  }
+  for (int h = 0; h < 2; ++h) up[h] = F16 && has ? a.kept.factors[place + (g + 8 * h < count ? g + 8 * h : 0)] : 1.0f;
   constexpr int kSteps = X::kHold ? R / kStep : 1;
-  uint32_t held[kSteps][2][4], next[kSteps][4][2];
+  uint32_t held[kSteps][2][4], w[2][kSteps][4][2];         // the factors of a group of columns and of the next one
   if (X::kHold && has) {
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       load_h(k * kStep, held[k][0], held[k][1]);
-      w2.load(c0 * X::kGroups, k * kStep, next[k]);
+      w2.load(c0 * X::kGroups, k * kStep, w[0][k]);
     }
   }
-  for (int c = c0, stage = 0; c < c1; ++c, stage ^= 1) {
-    if (!BACK) lr_wait<1>();
+  // WHOLE: all 16 rows are there, and so are all columns of the block, in whole accesses
+  auto block = [&](auto whole, int c, int stage) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int q = 0; q < X::kGroups; ++q) {
-      const int b = c * X::kGroups + q, col = b * 32 + 8 * t, left = a.cols - col;         // may be negative
-      float acc[4][4];
-      if (has) {
+      const int b = c * X::kGroups + q, left = a.cols - b * 32 - 8 * t;         // may be negative
+      float acc[4][4], base[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) base[h][i] = 0.0f;
+        if (!BACK && (WHOLE || (a.base != nullptr && row_of[h] >= 0 && left > 0))) {
+          if (WHOLE || a.vec_y) {
+            __align__(16) T e[8];
+#pragma unroll
+            for (int i = 0; i < kSize; ++i) reinterpret_cast<uint4*>(e)[i] = ring[((stage * X::kGroups + q) * 2 * kSize + h * kSize + i) * 32];
+            lr_load8<T, true>(e, 8, base[h]);
+          } else {
+            lr_load8<T, false>(from[h] + b * 32, left, base[h]);
+          }
+        }
+        const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        lr_set<T>(acc, h, LrStart<T>::kBase ? base[h] : zeros);
+      }
+      if (WHOLE || has) {
         if constexpr (X::kHold) {
-          uint32_t w[kSteps][4][2];
+          if (q + 1 < X::kGroups || c + 1 < c1) {
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { w[k][j][0] = next[k][j][0]; w[k][j][1] = next[k][j][1]; }
-            if (q + 1 < X::kGroups || c + 1 < c1) w2.load(b + 1, k * kStep, next[k]);
+            for (int k = 0; k < kSteps; ++k) w2.load(b + 1, k * kStep, w[(q + 1) & 1][k]);
           }
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[k], k == 0);
+          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[q & 1][k]);
         } else {
 #pragma unroll 2
           for (int k = 0; k < R; k += kStep) {
             if (k >= a.rank) break;
-            uint32_t w[4][2], hi[4], lo[4];
-            w2.load(b, k, w);
+            uint32_t wk[4][2], hi[4], lo[4];
+            w2.load(b, k, wk);
             load_h(k, hi, lo);
-            lr_multiply<T>(acc, hi, lo, w, k == 0);
+            lr_multiply<T>(acc, hi, lo, wk);
           }
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (row_of[h] < 0 || left <= 0) continue;
+        if (!WHOLE && (row_of[h] < 0 || left <= 0)) continue;
         float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        if (!BACK && a.base != nullptr) {
-          if (a.vec_y) {
-            __align__(16) T e[8];
-#pragma unroll
-            for (int i = 0; i < kSize; ++i) reinterpret_cast<uint4*>(e)[i] = ring[((stage * X::kGroups + q) * 2 * kSize + h * kSize + i) * 32];
-            lr_load8<T, true>(e, 8, v);
-          } else {
-            lr_load8<T, false>(from[h] + b * 32, left, v);
-          }
-        }
-        if (has) {
-          uint4 words;
-          if (BACK && a.drop_y) words = dropout_words((unsigned)col >> 3, row_of[h], key);
-          lr_finish(v, acc, h, scaled[h], BACK && a.drop_y ? &words : nullptr, a.drop.limit);
-        } else if (group > a.groups.adapters) {
+        lr_get<T>(acc, h, up[h], base[h], v);
+        if (BACK && a.drop_y && has) lr_drop(v, dropout_words((unsigned)(b * 32 + 8 * t) >> 3, row_of[h], key), a.drop.limit);
+        if (!WHOLE && group > a.groups.adapters) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
         }
-        if (a.vec_y) lr_store8<T, true>(to[h] + b * 32, 8, v);
+        if (WHOLE || a.vec_y) lr_store8<T, true>(to[h] + b * 32, 8, v);
         else lr_store8<T, false>(to[h] + b * 32, left, v);
       }
     }
+  };
+  const bool whole = has && count == 16 && a.vec_y && (BACK || a.base != nullptr);
+  for (int c = c0, stage = 0; c < c1; ++c, stage ^= 1) {
+    if (!BACK) lr_wait<1>();
+    if (whole && (c + 1) * X::kCols <= a.cols) block(std::true_type(), c, stage);
+    else block(std::false_type(), c, stage);
     request(c + 2, stage);
   }
   if (!BACK) lr_wait<0>();
 }
 
 // ---- the factors' gradients --------------------------------------------------------------------------------------------------------------
-// out[r][c] (or [c][r]) = s sum over the adapter's rows of p[row][r] q[row][c].  A cluster takes 128 columns of one adapter and one product, its blocks
+// out[r][c] (or [c][r]) = sum over the adapter's rows of p[row][r] q[row][c]; the rank values p have the scales in them.  A cluster takes 128 columns of one adapter and one product, its blocks
 // split the rows.  bf16: the rank values' two parts times q, both as ldmatrix turns them.  f16 and f32: TF32, where f16 is exact (its range would lose small rank
 // values); the two rows 2 t and 2 t + 1 of every eight are then what a thread has of a matrix instruction's axis of eight, which is how
 // ldmatrix hands out 16-bit values of q; p follows.
@@ -968,15 +973,17 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
     const int* list = rows[s % 4];
     const int from = first + s * kLrOuterRows;
     lr_fill<T, kLrOuterCols>(qs(slot), L::kPitchQ, kLrOuterRows, col0, width, a.vec[which], q, [&](int r) { return list[r] < 0 ? (const T*)nullptr : q + list[r] * a.ldq[which]; });
-    if constexpr (BF16) {
+    // rank values: eights of the rows side by side, of bf16 both parts
+    using P = typename std::conditional<BF16, T, float>::type;
+    constexpr int kOne = kLrOuterRows * (R / 8), kAll = BF16 ? 2 * kOne : kOne;
+    const P* p = (const P*)a.p[which] + (long long)from * R;
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const T* p = (const T*)a.p[which] + part * (long long)a.groups.n * R;
-        lr_fill<T, R>((T*)(ps(slot) + part * L::kP), L::kPitchP, kLrOuterRows, 0, R, true, p, [&](int r) { return from + r < last ? p + (long long)(from + r) * R : (const T*)nullptr; });
-      }
-    } else {
-      const float* p = (const float*)a.p[which];
-      lr_fill<float, R>((float*)ps(slot), L::kPitchP, kLrOuterRows, 0, R, true, p, [&](int r) { return from + r < last ? p + (long long)(from + r) * R : (const float*)nullptr; });
+    for (int u0 = 0; u0 < kAll; u0 += kLrThreads) {
+      const int u = u0 + threadIdx.x;
+      if (kAll % kLrThreads != 0 && u >= kAll) break;
+      const int part = u / kOne, r = u % kOne / (R / 8), c = u % (R / 8) * 8;
+      const P* src = p + part * (long long)a.groups.n * R + r * R + c;
+      lr_copy8<P>((P*)(ps(slot) + part * L::kP) + r * L::kPitchP + c, src, from + r < last ? 8 : 0, true, (const P*)a.p[which]);
     }
   };
   float acc[R / 16][2][4];
@@ -1126,7 +1133,6 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
     }
   lr_arrive();
   lr_meet();
-  const float by = (a.scales != nullptr ? a.scales[adapter] : a.scale) * (drop ? a.drop.share : 1.0f);
   T* out = (T*)a.out[which] + (long long)adapter * a.rank * width;
   // each block adds and writes its share of the tile: along the rank for dB, whose rank values lie side by side
   for (int u = threadIdx.x + rank * kLrThreads; u < R * kLrOuterCols / 4; u += kLrThreads * ranks) {
@@ -1137,7 +1143,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
       const float4 w = lr_remote4(part + 4 * u, k);
       v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
-    const float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+    const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (col0 + c + i < width) out[which ? (long long)(col0 + c + i) * a.rank + r : (long long)r * width + col0 + c + i] = lr_round<T>(f[i]);
