@@ -280,17 +280,6 @@ __device__ __forceinline__ void lr_copy8(T* dst, const T* src, int left, bool ve
   }
 }
 
-// Eights of rows into shared memory: rows r < nrows of `from(r)` (null: zeros), columns c0 .. c0 + C - 1 of `width`; to: rows of `pitch` values.  any: a
-// readable address for copies of nothing.
-template <typename T, int C, typename From>
-__device__ __forceinline__ void lr_fill(T* to, int pitch, int nrows, int c0, int width, bool vec, const T* any, From from) {
-  for (int u = threadIdx.x; u < nrows * (C / 8); u += kLrThreads) {
-    const int r = u / (C / 8), c = u % (C / 8) * 8;
-    const T* src = from(r);
-    lr_copy8<T>(to + r * pitch + c, src + c0 + c, src != nullptr ? width - c0 - c : 0, vec, any);
-  }
-}
-
 // ---- the second product ------------------------------------------------------------------------------------------------------------------------
 // A warp takes 16 rows and 32 columns at a time, four matrix instructions wide.  Column 8 (c / 2) + 2 j + c % 2 is column c of the j-th, so that the eight
 // values that a thread has of a row lie side by side.  Of the rank values a thread has 4 t .. 4 t + 3 of every sixteen (f32: 2 t and 2 t + 1 of
@@ -306,7 +295,45 @@ struct LrFactor {              // w2 of one adapter: forward [cols][rank], backw
   __device__ __forceinline__ LrFactor(const T* w2, int cols, int rank, int vec, int g, int t)
       : p(BACK ? w2 + (long long)(LrStep<T>::kEach * t) * cols + 8 * (g >> 1) : w2 + (long long)(8 * (g >> 1) + (g & 1)) * rank + LrStep<T>::kEach * t),
         cols(cols), rank(rank), vec(vec), g(g), t(t) {}
-  // columns 32 b and on, rank values k and on
+  // columns 32 b and on, rank values k and on; `at`: first + k of the first (forward), all columns and words there, RANK the rank
+  template <int RANK>
+  __device__ __forceinline__ static void whole(const T* at, long long cols, int k, int g, int t, uint32_t (*w)[2]) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int kEach = LrStep<T>::kEach;
+    const bool there = RANK % LrStep<T>::kStep == 0 || k + kEach * t < RANK;
+    if (BACK) {
+      uint32_t v[kEach][F32 ? 8 : 4];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+          const uint4 u = there ? reinterpret_cast<const uint4*>(at + i * cols)[h] : make_uint4(0, 0, 0, 0);
+          v[i][4 * h] = u.x; v[i][4 * h + 1] = u.y; v[i][4 * h + 2] = u.z; v[i][4 * h + 3] = u.w;
+        }
+      pick(v, g, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint2 u = there ? *reinterpret_cast<const uint2*>(at + 2 * j * RANK) : make_uint2(0, 0);
+        w[j][0] = u.x; w[j][1] = u.y;
+      }
+    }
+  }
+  template <typename V>
+  __device__ __forceinline__ static void pick(const V& v, int g, uint32_t (*w)[2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        w[j][0] = g & 1 ? v[0][2 * j + 1] : v[0][2 * j];
+        w[j][1] = g & 1 ? v[1][2 * j + 1] : v[1][2 * j];
+      } else {
+        const unsigned half = g & 1 ? 0x7632u : 0x5410u;        // the upper or the lower halves of two words
+        w[j][0] = __byte_perm(v[0][j], v[1][j], half);
+        w[j][1] = __byte_perm(v[LrStep<T>::kEach - 2][j], v[LrStep<T>::kEach - 1][j], half);
+      }
+    }
+  }
+  // as they are, with everything checked
   __device__ __forceinline__ void load(int b, int k, uint32_t (*w)[2]) const {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int kEach = LrStep<T>::kEach;
@@ -331,17 +358,7 @@ struct LrFactor {              // w2 of one adapter: forward [cols][rank], backw
           for (int h = 0; h < (F32 ? 8 : 4); ++h) v[i][h] = reinterpret_cast<const uint32_t*>(e)[h];
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (F32) {
-          w[j][0] = g & 1 ? v[0][2 * j + 1] : v[0][2 * j];
-          w[j][1] = g & 1 ? v[1][2 * j + 1] : v[1][2 * j];
-        } else {
-          const unsigned pick = g & 1 ? 0x7632u : 0x5410u;        // the upper or the lower halves of two words
-          w[j][0] = __byte_perm(v[0][j], v[1][j], pick);
-          w[j][1] = __byte_perm(v[kEach - 2][j], v[kEach - 1][j], pick);
-        }
-      }
+      pick(v, g, w);
     } else {
       const T* first = p + (long long)b * 32 * rank + k;
 #pragma unroll
@@ -787,7 +804,7 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int index = blockIdx.x % row_blocks * kLrWarps + warp;
   if (index >= tiles) return;
-  int group = 0, place = index * 16, count = a.groups.n - place;
+  int group = 0, place = index * 16, count = a.groups.n - place < 16 ? a.groups.n - place : 16;
   if (a.groups.mode == LR_PLAN) {
     const int4 tile = a.groups.tiles[index];
     group = tile.x; place = tile.y; count = tile.z;
@@ -801,14 +818,22 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
     const int r = g + 8 * h;
     row_of[h] = r < count ? (a.groups.mode == LR_PLAN ? a.groups.order[place + r] : place + r) : -1;
   }
-  const bool fetched = !BACK && a.base != nullptr && a.vec_y;
+  const bool fetched = !BACK && a.base != nullptr && a.vec_y, full = fetched && count == 16;
   const T* from[2] = {(const T*)a.base + (row_of[0] < 0 ? 0 : row_of[0]) * a.ld_base + 8 * t, (const T*)a.base + (row_of[1] < 0 ? 0 : row_of[1]) * a.ld_base + 8 * t};
   T* to[2] = {(T*)a.y + (row_of[0] < 0 ? 0 : row_of[0]) * a.ldy + 8 * t, (T*)a.y + (row_of[1] < 0 ? 0 : row_of[1]) * a.ldy + 8 * t};
   uint4* ring = reinterpret_cast<uint4*>(lr_dynamic) + warp * X::kStages * X::kPieces * 32 + lane;
   auto request = [&](int c, int stage) {
     if constexpr (!BACK) {
-      if (fetched && c < c1) {
+      if (full && c < c1 && (c + 1) * X::kCols <= a.cols) {
 #pragma unroll
+        for (int q = 0; q < X::kGroups; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int v = 0; v < kSize; ++v)
+              lr_copy16(ring + ((stage * X::kGroups + q) * 2 * kSize + h * kSize + v) * 32, from[h] + c * X::kCols + q * 32 + v * (8 / kSize));
+      } else if (fetched && c < c1) {
+#pragma unroll 1
         for (int q = 0; q < X::kGroups; ++q)
           if (c * X::kCols + q * 32 + 8 * t < a.cols) {
 #pragma unroll
@@ -850,18 +875,71 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
 #pragma unroll
   for (int h = 0; h < 2; ++h) up[h] = F16 && has ? a.kept.factors[place + (g + 8 * h < count ? g + 8 * h : 0)] : 1.0f;
   constexpr int kSteps = X::kHold ? R / kStep : 1;
-  uint32_t held[kSteps][2][4], w[2][kSteps][4][2];         // the factors of a group of columns and of the next one
+  uint32_t held[kSteps][2][4];
   if (X::kHold && has) {
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      load_h(k * kStep, held[k][0], held[k][1]);
-      w2.load(c0 * X::kGroups, k * kStep, w[0][k]);
+    for (int k = 0; k < kSteps; ++k) load_h(k * kStep, held[k][0], held[k][1]);
+  }
+  int c = c0, stage = 0;
+  // Whole blocks: 16 rows, all columns and their factors in whole accesses, the rank known.  Nothing is checked, and the next factors are on their way.
+  auto walk = [&](auto known) {
+    constexpr int RANK = decltype(known)::value;
+    const long long step = BACK ? 32 : 32 * RANK;
+    const T* at = w2.p + c * X::kGroups * step;
+    uint32_t w[2][kSteps][4][2];                    // the factors of a group of columns and of the next one
+    const int last = c1 < a.cols / X::kCols ? c1 : a.cols / X::kCols;
+    if (c >= last) return;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) LrFactor<T, BACK>::template whole<RANK>(at + k * kStep * (BACK ? a.cols : 1), a.cols, k * kStep, g, t, w[0][k]);
+    T* y[2] = {to[0] + c * X::kCols, to[1] + c * X::kCols};
+    for (; c < last; ++c, stage ^= 1) {
+      if (!BACK) lr_wait<1>();
+      const uint4* here = ring + stage * X::kPieces * 32;
+#pragma unroll
+      for (int q = 0; q < X::kGroups; ++q) {
+        float acc[4][4], base[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) base[h][i] = 0.0f;
+          if (!BACK) {
+            __align__(16) T e[8];
+#pragma unroll
+            for (int i = 0; i < kSize; ++i) reinterpret_cast<uint4*>(e)[i] = here[(q * 2 * kSize + h * kSize + i) * 32];
+            lr_load8<T, true>(e, 8, base[h]);
+          }
+          const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          lr_set<T>(acc, h, LrStart<T>::kBase ? base[h] : zeros);
+        }
+        at += step;
+        if (q + 1 < X::kGroups || c + 1 < last) {
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) LrFactor<T, BACK>::template whole<RANK>(at + k * kStep * (BACK ? a.cols : 1), a.cols, k * kStep, g, t, w[(q + 1) & 1][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[q & 1][k]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[8];
+          lr_get<T>(acc, h, up[h], base[h], v);
+          if (BACK && a.drop_y) lr_drop(v, dropout_words((unsigned)((c * X::kGroups + q) * 32 + 8 * t) >> 3, row_of[h], key), a.drop.limit);
+          lr_store8<T, true>(y[h] + q * 32, 8, v);
+        }
+      }
+      y[0] += X::kCols;
+      y[1] += X::kCols;
+      request(c + 2, stage);
+    }
+  };
+  if constexpr (X::kHold) {
+    if (has && count == 16 && a.vec_y && a.vec_w2 && (BACK || a.base != nullptr)) {
+      if (a.rank == R) walk(std::integral_constant<int, R>());
+      else if (R == 16 && a.rank == 8) walk(std::integral_constant<int, 8>());
     }
   }
-  // WHOLE: all 16 rows are there, and so are all columns of the block, in whole accesses
-  auto block = [&](auto whole, int c, int stage) {
-    constexpr bool WHOLE = decltype(whole)::value;
-#pragma unroll
+  for (; c < c1; ++c, stage ^= 1) {                 // anything else
+    if (!BACK) lr_wait<1>();
+#pragma unroll 1
     for (int q = 0; q < X::kGroups; ++q) {
       const int b = c * X::kGroups + q, left = a.cols - b * 32 - 8 * t;         // may be negative
       float acc[4][4], base[2][8];
@@ -869,8 +947,8 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) base[h][i] = 0.0f;
-        if (!BACK && (WHOLE || (a.base != nullptr && row_of[h] >= 0 && left > 0))) {
-          if (WHOLE || a.vec_y) {
+        if (!BACK && a.base != nullptr && row_of[h] >= 0 && left > 0) {
+          if (a.vec_y) {
             __align__(16) T e[8];
 #pragma unroll
             for (int i = 0; i < kSize; ++i) reinterpret_cast<uint4*>(e)[i] = ring[((stage * X::kGroups + q) * 2 * kSize + h * kSize + i) * 32];
@@ -882,45 +960,39 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
         const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         lr_set<T>(acc, h, LrStart<T>::kBase ? base[h] : zeros);
       }
-      if (WHOLE || has) {
+      if (has) {
         if constexpr (X::kHold) {
-          if (q + 1 < X::kGroups || c + 1 < c1) {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) w2.load(b + 1, k * kStep, w[(q + 1) & 1][k]);
+          for (int k = 0; k < kSteps; ++k) {
+            uint32_t w[4][2];
+            w2.load(b, k * kStep, w);
+            lr_multiply<T>(acc, held[k][0], held[k][1], w);
           }
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[q & 1][k]);
         } else {
 #pragma unroll 2
           for (int k = 0; k < R; k += kStep) {
             if (k >= a.rank) break;
-            uint32_t wk[4][2], hi[4], lo[4];
-            w2.load(b, k, wk);
+            uint32_t w[4][2], hi[4], lo[4];
+            w2.load(b, k, w);
             load_h(k, hi, lo);
-            lr_multiply<T>(acc, hi, lo, wk);
+            lr_multiply<T>(acc, hi, lo, w);
           }
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!WHOLE && (row_of[h] < 0 || left <= 0)) continue;
+        if (row_of[h] < 0 || left <= 0) continue;
         float v[8];
         lr_get<T>(acc, h, up[h], base[h], v);
         if (BACK && a.drop_y && has) lr_drop(v, dropout_words((unsigned)(b * 32 + 8 * t) >> 3, row_of[h], key), a.drop.limit);
-        if (!WHOLE && group > a.groups.adapters) {
+        if (group > a.groups.adapters) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
         }
-        if (WHOLE || a.vec_y) lr_store8<T, true>(to[h] + b * 32, 8, v);
+        if (a.vec_y) lr_store8<T, true>(to[h] + b * 32, 8, v);
         else lr_store8<T, false>(to[h] + b * 32, left, v);
       }
     }
-  };
-  const bool whole = has && count == 16 && a.vec_y && (BACK || a.base != nullptr);
-  for (int c = c0, stage = 0; c < c1; ++c, stage ^= 1) {
-    if (!BACK) lr_wait<1>();
-    if (whole && (c + 1) * X::kCols <= a.cols) block(std::true_type(), c, stage);
-    else block(std::false_type(), c, stage);
     request(c + 2, stage);
   }
   if (!BACK) lr_wait<0>();
@@ -948,6 +1020,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
   constexpr bool F32 = sizeof(T) == 4, BF16 = L::kBf16;
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
   __shared__ int rows[4][kLrOuterRows];
+  __shared__ long long places[4][kLrOuterRows];          // of the rows in q
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t rank = lr_rank(), ranks = lr_ranks();
@@ -959,20 +1032,35 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
   const int s0 = (int)((long long)steps * rank / ranks), s1 = (int)((long long)steps * (rank + 1) / ranks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const T* q = (const T*)a.q[which];
-  const bool drop = which == 0 && a.drop_x;
+  const bool drop = which == 0 && a.drop_x, inside = a.vec[which] && col0 + kLrOuterCols <= width;
   const uint2 key = drop ? philox_key(a.drop) : make_uint2(0, 0);
   auto list = [&](int s) {          // row numbers of a step, four steps side by side
     if (threadIdx.x < kLrOuterRows) {
       const int place = first + s * kLrOuterRows + threadIdx.x;
-      rows[s % 4][threadIdx.x] = place < last ? (a.groups.mode == LR_PLAN ? a.groups.order[place] : place) : -1;
+      const int row = place < last ? (a.groups.mode == LR_PLAN ? a.groups.order[place] : place) : -1;
+      rows[s % 4][threadIdx.x] = row;
+      places[s % 4][threadIdx.x] = (row < 0 ? 0 : row) * a.ldq[which];
     }
   };
   auto qs = [&](int i) { return reinterpret_cast<T*>(lr_dynamic + i * L::kStage); };
   auto ps = [&](int i) { return lr_dynamic + i * L::kStage + kLrOuterRows * L::kPitchQ * sizeof(T); };
   auto fetch = [&](int s, int slot) {
-    const int* list = rows[s % 4];
     const int from = first + s * kLrOuterRows;
-    lr_fill<T, kLrOuterCols>(qs(slot), L::kPitchQ, kLrOuterRows, col0, width, a.vec[which], q, [&](int r) { return list[r] < 0 ? (const T*)nullptr : q + list[r] * a.ldq[which]; });
+    constexpr int kAcross = kLrOuterCols / 8, kRows = kLrThreads / kAcross;
+    const int r0 = threadIdx.x / kAcross, c0 = threadIdx.x % kAcross * 8;
+    T* to = qs(slot) + r0 * L::kPitchQ + c0;
+    if (inside && from + kLrOuterRows <= last) {
+#pragma unroll
+      for (int r = 0; r < kLrOuterRows; r += kRows) {
+        const T* src = q + places[s % 4][r0 + r] + col0 + c0;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(to + r * L::kPitchQ + i * (16 / sizeof(T)), src + i * (16 / sizeof(T)));
+      }
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < kLrOuterRows; r += kRows)
+        lr_copy8<T>(to + r * L::kPitchQ, q + places[s % 4][r0 + r] + col0 + c0, from + r0 + r < last ? width - col0 - c0 : 0, a.vec[which], q);
+    }
     // rank values: eights of the rows side by side, of bf16 both parts
     using P = typename std::conditional<BF16, T, float>::type;
     constexpr int kOne = kLrOuterRows * (R / 8), kAll = BF16 ? 2 * kOne : kOne;
@@ -1006,6 +1094,7 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
     lr_wait<kAhead - 1>();
     if (drop) {                     // the eights that this thread copied
       const int* list = rows[s % 4];
+#pragma unroll 2
       for (int u = threadIdx.x; u < kLrOuterRows * (kLrOuterCols / 8); u += kLrThreads) {
         const int r = u / (kLrOuterCols / 8), c = u % (kLrOuterCols / 8) * 8;
         if (list[r] >= 0) lr_drop8<T>(qs(slot) + r * L::kPitchQ + c, dropout_words((unsigned)(col0 + c) >> 3, list[r], key), a.drop.limit);
