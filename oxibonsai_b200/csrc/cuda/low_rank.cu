@@ -7,8 +7,9 @@ constexpr int kPlanThreads = 512, kPlanEach = 8;
 
 // order: the rows by adapter, in their own order within each; start[e]: where adapter e's begin.  A block makes one adapter's list on its own: it counts
 // the ids below its own, which is where the list begins, and goes through the ids once more.  Nothing is shared between blocks, no atomics.
-// tiles (may be null): of 16 rows, those of adapter e in places start[e] / 16 + e to start[e + 1] / 16 + e, which are enough for all and lie apart.
-__global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* order, int* start, int4* tiles) {
+// tiles and their rows (may be null): of 16 rows, those of adapter e in places start[e] / 16 + e to start[e + 1] / 16 + e, which are enough for all and lie
+// apart.
+__global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* order, int* start, int4* tiles, int* tile_rows) {
   __shared__ int warps[kPlanThreads / 32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -32,9 +33,22 @@ __global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* 
     }
     return before + up - v;
   };
-  int below = 0;
-  for (long long row = t; row < g.n; row += kPlanThreads) below += lr_group(g, (int)row) < e;
-  int place;
+  // bit i: the thread's i-th id of the sweep is this adapter's; below: how many are smaller ones
+  auto sweep = [&](long long first, int& below) {
+    const long long row = first + (long long)t * kPlanEach;
+    unsigned mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i)
+      if (row + i < g.n) {
+        const int of = lr_group(g, (int)(row + i));
+        mine |= (of == e ? 1u : 0u) << i;
+        below += of < e;
+      }
+    return mine;
+  };
+  int below = 0, place, skip = 0;
+  unsigned mine = sweep(0, below);
+  for (long long first = per; first < g.n; first += per) sweep(first, below);
   block_scan(below, place);
   if (t == 0) {
     start[e] = place;
@@ -42,20 +56,21 @@ __global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* 
   }
   const int begin = place;
   for (long long first = 0; first < g.n; first += per) {
-    const long long row = first + (long long)t * kPlanEach;
-    unsigned mine = 0;
-#pragma unroll
-    for (int i = 0; i < kPlanEach; ++i)
-      if (row + i < g.n && lr_group(g, (int)(row + i)) == e) mine |= 1u << i;
+    if (first > 0) mine = sweep(first, skip);
     int all;
     int at = place + block_scan(__popc(mine), all);
-    for (unsigned m = mine; m != 0; m &= m - 1) order[at++] = (int)row + __ffs(m) - 1;
+    for (unsigned m = mine; m != 0; m &= m - 1, ++at) {
+      const int row = (int)(first + (long long)t * kPlanEach) + __ffs(m) - 1;
+      order[at] = row;
+      if (tiles != nullptr) tile_rows[(begin / 16 + e) * 16ll + at - begin] = row;
+    }
     place += all;
   }
   if (tiles != nullptr)
     for (int i = t; i <= place / 16 - begin / 16; i += kPlanThreads) {
       const int at = begin + 16 * i, left = place - at;
       tiles[begin / 16 + e + i] = left > 0 ? make_int4(e, at, left < 16 ? left : 16, 0) : make_int4(-1, 0, 0, 0);
+      for (int r = left > 0 ? left : 0; r < 16; ++r) tile_rows[(begin / 16 + e + i) * 16ll + r] = -1;
     }
 }
 
@@ -71,7 +86,7 @@ static int lr_vec(const void* p, long long ld, long long width, int size) { retu
 // kernel of its own), the order of rows, where each adapter's rows begin in it, the tiles of 16 rows.
 struct LrRoom {
   bool values, grouped, split;
-  long long parts, factors, order, start, tiles, bytes;
+  long long parts, factors, order, start, tiles, tile_rows, bytes;
 };
 static LrRoom lr_room(int n, int rank, int adapters, int type, bool grouped, bool values) {
   LrRoom k;
@@ -85,7 +100,9 @@ static LrRoom lr_room(int n, int rank, int adapters, int type, bool grouped, boo
   k.order = k.factors + (k.split && type == 1 ? up(4ll * n) : 0);
   k.start = k.order + (grouped ? up(4ll * n) : 0);
   k.tiles = k.start + (grouped ? up(4ll * (adapters + 3)) : 0);
-  k.bytes = k.tiles + (grouped && k.split ? 16ll * (n / 16 + adapters + 2) : 0);
+  const long long slots = grouped && k.split ? n / 16 + adapters + 2 : 0;
+  k.tile_rows = k.tiles + 16 * slots;
+  k.bytes = k.tile_rows + 64 * slots;
   return k;
 }
 static LrValues lr_values(void* room, const LrRoom& k) {
@@ -99,6 +116,7 @@ static void lr_grouped(LrGroups& g, void* room, const LrRoom& k) {
   g.order = (const int*)(p + k.order);
   g.start = (const int*)(p + k.start);
   g.tiles = k.split ? (const int4*)(p + k.tiles) : nullptr;
+  g.tile_rows = k.split ? (const int*)(p + k.tile_rows) : nullptr;
 }
 
 template <typename Args>
@@ -133,13 +151,13 @@ int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b
   const bool self = ids != nullptr && kept == nullptr && !values && n <= kLrSelf;
   const LrRoom at = lr_room(n, rank, adapters, type, ids != nullptr, values);
   if (!self && at.bytes > 0 && (kept == nullptr || kept_bytes < at.bytes)) return BONSAI_CUDA_BAD_ARG;
-  LrGroups g = {LR_ONE, ids, ids_wide, nullptr, nullptr, nullptr, n, adapters};
+  LrGroups g = {LR_ONE, ids, ids_wide, nullptr, nullptr, nullptr, nullptr, n, adapters};
   cudaError_t e = cudaSuccess;
   if (ids != nullptr) {
     g.mode = LR_SELF;
     if (!self) {
       lr_grouped(g, kept, at);
-      e = launch_pdl(lr_plan_kernel, dim3(adapters + 2), dim3(kPlanThreads), 0, st, g, (int*)g.order, (int*)g.start, (int4*)g.tiles);
+      e = launch_pdl(lr_plan_kernel, dim3(adapters + 2), dim3(kPlanThreads), 0, st, g, (int*)g.order, (int*)g.start, (int4*)g.tiles, (int*)g.tile_rows);
     }
   }
   if (e != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
@@ -167,7 +185,7 @@ int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long l
   const bool rows = dx != nullptr || da != nullptr;
   const LrRoom at = lr_room(n, rank, adapters, type, grouped, values), of = lr_room(n, rank, adapters, type, false, true);
   if ((at.bytes > 0 && (kept == nullptr || kept_bytes < at.bytes)) || (rows && (ws == nullptr || ws_bytes < of.bytes))) return BONSAI_CUDA_BAD_ARG;
-  LrGroups g = {LR_ONE, nullptr, 0, nullptr, nullptr, nullptr, n, adapters};
+  LrGroups g = {LR_ONE, nullptr, 0, nullptr, nullptr, nullptr, nullptr, n, adapters};
   if (grouped) lr_grouped(g, (void*)kept, at);
   const int size = type == 0 ? 4 : 2;
   const DropoutRule rule = dropout_rule(seed, seed_dev, steps);

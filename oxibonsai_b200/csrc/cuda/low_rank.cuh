@@ -37,7 +37,8 @@ struct LrGroups {            // which rows have which adapter
   int ids_wide;              // int64, else int32
   const int* order;          // LR_PLAN: rows by adapter; behind them those without one, and those whose id names none
   const int* start;          // [adapters + 3]: where each adapter's rows begin in it
-  const int4* tiles;         // LR_PLAN of kLrSplit rows and more: tiles of 16 rows: group (-1: none), place, rows
+  const int4* tiles;         // LR_PLAN of kLrSplit rows and more: tiles of 16 rows: group (-1: none), place, number of rows
+  const int* tile_rows;      // and their rows, -1 behind the last
   int n, adapters;
 };
 
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
     static_assert(M * kAcrossX % kLrThreads == 0 && kLrThreads % kAcrossX == 0 && kLrThreads % kAcrossW == 0, "whole rows of threads");
     const int xr = threadIdx.x / kAcrossX, xc = threadIdx.x % kAcrossX * 8, wr = threadIdx.x / kAcrossW, wc = threadIdx.x % kAcrossW * 8;
     const T* from[kX];
-    int from_row[kX];
+    int from_row[kX];             // -1: none
 #pragma unroll
     for (int i = 0; i < kX; ++i) {
       from_row[i] = rows[xr + i * kRowStep];
@@ -530,9 +531,29 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
       T* xs = stage(slot);
       T* ws = xs + M * L::kPitchX;
       const int k0 = c * S::kChunk;
+      if (a.vec_x && k0 + S::kChunk <= a.k) {
 #pragma unroll
-      for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i] + k0, a.k - k0 - xc, a.vec_x, (const T*)a.x);
+        for (int i = 0; i < kX; ++i)
 #pragma unroll
+          for (int v = 0; v < (int)sizeof(T) / 2; ++v)
+            lr_copy16(xs + (xr + i * kRowStep) * L::kPitchX + xc + v * (16 / (int)sizeof(T)), from[i] + k0 + v * (16 / (int)sizeof(T)));
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i] + k0, a.k - k0 - xc, a.vec_x, (const T*)a.x);
+      }
+      if (a.vec_w1 && a.rank == R && k0 + S::kChunk <= a.k) {
+        const T* src = BACK ? w1 + (long long)(k0 + wr) * R + wc : w1 + (long long)wr * a.k + k0 + wc;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+          const int r = wr + i * kStepW;
+          if (kUnitsW % kLrThreads != 0 && r >= L::kRowsW) break;
+#pragma unroll
+          for (int v = 0; v < (int)sizeof(T) / 2; ++v)
+            lr_copy16(ws + r * L::kPitchW + wc + v * (16 / (int)sizeof(T)), src + (BACK ? i * kStepW * R : (long long)i * kStepW * a.k) + v * (16 / (int)sizeof(T)));
+        }
+        return;
+      }
+#pragma unroll 1
       for (int i = 0; i < kW; ++i) {
         const int r = wr + i * kStepW;
         if (kUnitsW % kLrThreads != 0 && r >= L::kRowsW) break;
@@ -790,7 +811,10 @@ template <typename T, int R, bool BACK> struct LrExpand {
   static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4, kCols = 32 * kGroups;         // of a block of columns
   static constexpr int kStages = 2, kPieces = 8, kBytes = BACK ? 0 : kLrWarps * kStages * kPieces * 512;
   static constexpr bool kHold = R <= 32;
-  static constexpr int kBlocks = R == 16 && sizeof(T) == 2 ? 3 : 2;                    // on an SM
+  // groups of factors in registers: without base on its way, the factors are what is waited for
+  static constexpr int kWays = BACK && R == 16 && sizeof(T) == 2 ? 4 : 2;
+  static_assert(kWays - 1 <= kGroups && kGroups % kWays == 0, "a block's groups take turns");
+  static constexpr int kBlocks = R == 16 && sizeof(T) == 2 && !BACK ? 3 : 2;            // on an SM
 };
 
 template <typename T, int R, bool BACK>
@@ -799,25 +823,21 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
   constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value, BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kStep = LrStep<T>::kStep, kEach = LrStep<T>::kEach, kSize = (int)sizeof(T) / 2;
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int index = blockIdx.x % row_blocks * kLrWarps + warp;
   if (index >= tiles) return;
   int group = 0, place = index * 16, count = a.groups.n - place < 16 ? a.groups.n - place : 16;
+  int row_of[2] = {g < count ? place + g : -1, g + 8 < count ? place + g + 8 : -1};
   if (a.groups.mode == LR_PLAN) {
     const int4 tile = a.groups.tiles[index];
+    row_of[0] = a.groups.tile_rows[index * 16ll + g];
+    row_of[1] = a.groups.tile_rows[index * 16ll + g + 8];
     group = tile.x; place = tile.y; count = tile.z;
     if (group < 0) return;
   }
   const bool has = group < a.groups.adapters;
   const int blocks = (a.cols + X::kCols - 1) / X::kCols, c0 = blockIdx.x / row_blocks * per, c1 = c0 + per < blocks ? c0 + per : blocks;
-  int row_of[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = g + 8 * h;
-    row_of[h] = r < count ? (a.groups.mode == LR_PLAN ? a.groups.order[place + r] : place + r) : -1;
-  }
   const bool fetched = !BACK && a.base != nullptr && a.vec_y, full = fetched && count == 16;
   const T* from[2] = {(const T*)a.base + (row_of[0] < 0 ? 0 : row_of[0]) * a.ld_base + 8 * t, (const T*)a.base + (row_of[1] < 0 ? 0 : row_of[1]) * a.ld_base + 8 * t};
   T* to[2] = {(T*)a.y + (row_of[0] < 0 ? 0 : row_of[0]) * a.ldy + 8 * t, (T*)a.y + (row_of[1] < 0 ? 0 : row_of[1]) * a.ldy + 8 * t};
@@ -886,11 +906,16 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
     constexpr int RANK = decltype(known)::value;
     const long long step = BACK ? 32 : 32 * RANK;
     const T* at = w2.p + c * X::kGroups * step;
-    uint32_t w[2][kSteps][4][2];                    // the factors of a group of columns and of the next one
+    uint32_t w[X::kWays][kSteps][4][2];             // the factors of a group of columns and of the next ones
     const int last = c1 < a.cols / X::kCols ? c1 : a.cols / X::kCols;
     if (c >= last) return;
+    auto ask = [&](int q) {                         // of the group at `at`
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) LrFactor<T, BACK>::template whole<RANK>(at + k * kStep * (BACK ? a.cols : 1), a.cols, k * kStep, g, t, w[0][k]);
+      for (int k = 0; k < kSteps; ++k) LrFactor<T, BACK>::template whole<RANK>(at + k * kStep * (BACK ? a.cols : 1), a.cols, k * kStep, g, t, w[q % X::kWays][k]);
+      at += step;
+    };
+#pragma unroll
+    for (int q = 0; q < X::kWays - 1; ++q) ask(q);  // a block has as many groups
     T* y[2] = {to[0] + c * X::kCols, to[1] + c * X::kCols};
     for (; c < last; ++c, stage ^= 1) {
       if (!BACK) lr_wait<1>();
@@ -911,13 +936,9 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
           const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
           lr_set<T>(acc, h, LrStart<T>::kBase ? base[h] : zeros);
         }
-        at += step;
-        if (q + 1 < X::kGroups || c + 1 < last) {
+        if (q + X::kWays - 1 < X::kGroups || c + 1 < last) ask(q + X::kWays - 1);
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) LrFactor<T, BACK>::template whole<RANK>(at + k * kStep * (BACK ? a.cols : 1), a.cols, k * kStep, g, t, w[(q + 1) & 1][k]);
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[q & 1][k]);
+        for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[q % X::kWays][k]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
@@ -1021,7 +1042,6 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
   extern __shared__ __align__(16) unsigned char lr_dynamic[];
   __shared__ int rows[4][kLrOuterRows];
   __shared__ long long places[4][kLrOuterRows];          // of the rows in q
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t rank = lr_rank(), ranks = lr_ranks();
   const int cluster = blockIdx.x / ranks, per = a.blocks[0] + a.blocks[1], adapter = cluster / per, within = cluster % per;
@@ -1264,11 +1284,16 @@ static cudaError_t lr_launch(Kern kernel, long long clusters, int ranks, int sme
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Blocks of a cluster: as many, in powers of two, as bring the grid near two blocks an SM, and no more than `most` have work.
-inline int lr_ranks_for(long long clusters, long long most) {
-  int ranks = 1;
-  while (ranks < 8 && 2 * ranks <= most && clusters * ranks < 148 * 2) ranks *= 2;
-  return ranks;
+// Blocks of a cluster that divide `units` of work among them: what ends first where `resident` blocks run at once and a block's start and end cost as
+// much as `ends` units.
+inline int lr_ranks_for(long long clusters, long long units, int resident, int ends) {
+  int best = 1;
+  double least = 1e300;
+  for (int r = 1; r <= 8 && r <= units; ++r) {
+    const double cost = (double)((clusters * r + resident - 1) / resident) * ((double)units / r + ends);
+    if (cost < least * 0.999) { least = cost; best = r; }
+  }
+  return best;
 }
 // Tiles of M rows, the empty ones among them.
 inline long long lr_slots(const LrGroups& g, int M) { return g.mode == LR_ONE ? (g.n + M - 1) / M : g.mode == LR_SELF ? g.n : g.n / M + g.adapters + 2; }
@@ -1280,7 +1305,8 @@ static cudaError_t lr_rows_as(const LrRowsArgs& a, cudaStream_t st) {
   const LrGroups& g = a.groups;
   const long long slots = lr_slots(g, M), busy = g.mode == LR_ONE ? slots : g.n / M + (g.n < g.adapters ? g.n : g.adapters);
   const int chunks = (a.k + L::kChunk - 1) / L::kChunk;
-  return lr_launch(lr_rows_kernel<T, R, M, BACK, SPLIT>, slots, lr_ranks_for(busy < 1 ? 1 : busy, chunks), L::kBytes, st, a);
+  const int resident = 148 * (SPLIT && R == 16 && sizeof(T) == 2 ? 3 : R <= 32 ? 2 : 1);
+  return lr_launch(lr_rows_kernel<T, R, M, BACK, SPLIT>, slots, lr_ranks_for(busy < 1 ? 1 : busy, chunks, resident, 4), L::kBytes, st, a);
 }
 
 template <typename T, int R, bool BACK>
@@ -1316,9 +1342,9 @@ static cudaError_t lr_outer_r(const LrOuterArgs& a, cudaStream_t st) {
   using L = LrOuterSmem<T, R>;
   const long long clusters = (long long)(a.blocks[0] + a.blocks[1]) * a.groups.adapters;
   const long long steps = (a.groups.n / a.groups.adapters + kLrOuterRows - 1) / kLrOuterRows;
-  const int ranks = lr_ranks_for(clusters / 2, steps > 1 ? steps : 1);          // four blocks an SM: they are short
-  if (clusters * ranks >= 1ll << 31) return cudaErrorInvalidValue;
-  return lr_launch(lr_outer_kernel<T, R>, (int)clusters, ranks, L::kBytes, st, a);
+  // Columns that are dropped take twice the others' time: many short blocks then even out
+  const int ranks = a.drop_x && a.blocks[0] > 0 && a.blocks[1] > 0 && steps >= 32 ? 8 : lr_ranks_for(clusters, steps, 148 * (R <= 32 ? (L::kBytes <= kLrSmemThird ? 3 : 2) : 1), 4);
+  return lr_launch(lr_outer_kernel<T, R>, clusters, ranks, L::kBytes, st, a);
 }
 
 inline int lr_padded(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
