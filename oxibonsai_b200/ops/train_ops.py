@@ -201,9 +201,9 @@ def _lr_room(n: int, rank: int, adapters: int, grouped: bool, values: bool, like
 def low_rank_forward(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: torch.Tensor | None, ids: torch.Tensor | None, scale: float | torch.Tensor,
                      steps: int, seed: Seed, out: torch.Tensor | None = None, train: bool = False,
                      values: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """x [n, d], a [e, r, d], b [e, out, r] (dense), base [n, out] or None (unit strides along rows), ids [n] or None -> the result [n, out] and what a
+    """x [n, d], a [e, r, d], b [e, out, r] (dense, or of one adapter without e), base [n, out] or None (unit strides along rows), ids [n] or None -> the result [n, out] and what a
     backward pass takes (``train``; ``values``: that of ``b`` too)."""
-    (n, d), (e, r, _), cols, device = x.shape, a.shape, b.shape[1], x.device
+    (n, d), (cols, r), e, device = x.shape, b.shape[-2:], 1 if b.dim() == 2 else b.shape[0], x.device
     with _on(device):
         y = x.new_empty((n, cols)) if out is None else out
         grouped = ids is not None
@@ -215,17 +215,16 @@ def low_rank_forward(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: to
 
 
 def low_rank_backward(x: torch.Tensor | None, dy: torch.Tensor, a: torch.Tensor | None, b: torch.Tensor, d: int, kept: torch.Tensor | None, grouped: bool,
-                      values: bool, scale: float | torch.Tensor, steps: int, seed: Seed, want_x: bool, want_a: bool,
-                      want_b: bool) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
-    """Gradients of :func:`low_rank_forward` by x (needs ``a``), a (needs ``x``) and b (needs a pass with ``values``)."""
-    (n, cols), (e, _, r), device, dtype = dy.shape, b.shape, dy.device, dy.dtype
+                      scale: float | torch.Tensor, steps: int, seed: Seed, want_x: bool, want_a: bool, want_b: bool) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of :func:`low_rank_forward` by x (needs ``a``), a (needs ``x``) and b (needs a pass with ``values``, and only that)."""
+    (n, cols), r, e, one, device, dtype = dy.shape, b.shape[-1], 1 if b.dim() == 2 else b.shape[0], b.dim() == 2, dy.device, dy.dtype
     with _on(device):
         dx = dy.new_empty((n, d)) if want_x else None
-        da = dy.new_empty((e, r, d)) if want_a else None
-        db = dy.new_empty((e, cols, r)) if want_b else None
+        da = dy.new_empty((r, d) if one else (e, r, d)) if want_a else None
+        db = dy.new_empty(b.shape) if want_b else None
         ws = _lr_room(n, r, e, False, True, dy) if want_x or want_a else None
         K.check(_lib().bonsai_lr_backward(K.ptr(x), 0 if x is None else _ld(x), dy.data_ptr(), _ld(dy), K.ptr(a), b.data_ptr(), K.ptr(dx), K.ptr(da), K.ptr(db),
-                                          *_scale(scale), n, d, cols, r, e, TYPE_CODES[dtype], grouped, K.ptr(kept), 0 if kept is None else kept.numel(), values,
+                                          *_scale(scale), n, d, cols, r, e, TYPE_CODES[dtype], grouped, K.ptr(kept), 0 if kept is None else kept.numel(), want_b,
                                           K.ptr(ws), 0 if ws is None else ws.numel(), *_seed(seed), steps, _stream(device)), "low_rank_backward")
     return dx, da, db
 

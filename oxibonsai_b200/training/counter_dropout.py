@@ -61,6 +61,11 @@ def rows_of(x: torch.Tensor) -> torch.Tensor:
     return flat if flat.is_contiguous() or flat.stride(1) == 1 or flat.shape[1] == 1 and flat.stride(0) >= 1 else flat.contiguous()
 
 
+def _cuda(x, steps, seed):
+    y = train_ops.dropout(rows_of(x), steps, seed)
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, steps, seed):
@@ -68,7 +73,7 @@ class _Dropout(torch.autograd.Function):
         if ctx.seed is None:
             ctx.save_for_backward(seed)
         if x.is_cuda:
-            return train_ops.dropout(rows_of(x), steps, seed).view(x.shape)
+            return _cuda(x, steps, seed)
         kind = torch.float64 if x.dtype == torch.float64 else torch.float32
         share = 65536.0 / steps if steps else 0.0
         mask = kept(x.numel() // x.shape[-1], x.shape[-1], steps, seed).view(x.shape)
@@ -78,7 +83,7 @@ class _Dropout(torch.autograd.Function):
     def backward(ctx, up):
         seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
         if up.is_cuda and not torch.is_grad_enabled():
-            return train_ops.dropout(rows_of(up), ctx.steps, seed).view(up.shape), None, None
+            return _cuda(up, ctx.steps, seed), None, None
         return _Dropout.apply(up, ctx.steps, seed), None, None
 
 
@@ -104,4 +109,6 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = N
     steps = keep_steps(p)
     if not training or steps == 65536 or x.numel() == 0:
         return x
+    if x.is_cuda and not (x.requires_grad and torch.is_grad_enabled()):
+        return _cuda(x, steps, seed)
     return _Dropout.apply(x, steps, seed)

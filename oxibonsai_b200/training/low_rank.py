@@ -23,19 +23,21 @@ MAX_RANK = 128
 
 
 def _cpu_parts(x, a, ids, scale, steps, seed):
-    """What both passes on the CPU need: the type of the sums, rows as they enter the adapters, a row's scale, its adapter's rows."""
+    """What both passes on the CPU need: the type of the sums, the mask and its scale, the adapters' scales and rows."""
     kind = torch.float64 if x.dtype == torch.float64 else torch.float32
     keep = kept(*x.shape, steps, seed) if steps < 65536 else None
     share = 1.0 if keep is None else 65536.0 / steps if steps else 0.0
-    scales = scale.to(kind) if isinstance(scale, torch.Tensor) else torch.full((len(a),), scale, dtype=kind)
-    rows = [torch.arange(len(x))] if ids is None else [(ids == e).nonzero().flatten() for e in range(len(a))]
-    return kind, keep, share, scales, rows
+    count = 1 if a.dim() == 2 else len(a)
+    scales = scale.to(kind) if isinstance(scale, torch.Tensor) else torch.full((count,), scale, dtype=kind)
+    rows = [torch.arange(len(x))] if ids is None else [(ids.reshape(-1) == e).nonzero().flatten() for e in range(count)]
+    return kind, keep, share, scales.reshape(-1), rows
 
 
 def _cpu_forward(x, a, b, base, ids, scale, steps, seed):
     kind, keep, share, scales, rows = _cpu_parts(x, a, ids, scale, steps, seed)
     xs = x.to(kind) if keep is None else torch.where(keep, x.to(kind) * share, 0.0)
-    y = torch.zeros(len(x), b.shape[1], dtype=kind) if base is None else base.to(kind).clone()
+    y = torch.zeros(len(x), b.shape[-2], dtype=kind) if base is None else base.to(kind).clone()
+    a, b = a.view(-1, *a.shape[-2:]), b.view(-1, *b.shape[-2:])
     for e, at in enumerate(rows):
         if len(at):
             y[at] += (xs[at] @ a[e].to(kind).T) @ b[e].to(kind).T * scales[e]
@@ -45,6 +47,7 @@ def _cpu_forward(x, a, b, base, ids, scale, steps, seed):
 def _cpu_backward(x, a, b, ids, scale, steps, seed, up):
     kind, keep, share, scales, rows = _cpu_parts(x, a, ids, scale, steps, seed)
     xs = x.to(kind) if keep is None else torch.where(keep, x.to(kind) * share, 0.0)
+    shapes, a, b = (a.shape, b.shape), a.view(-1, *a.shape[-2:]), b.view(-1, *b.shape[-2:])
     dx, da, db = torch.zeros_like(xs), torch.zeros(a.shape, dtype=kind), torch.zeros(b.shape, dtype=kind)
     for e, at in enumerate(rows):
         if len(at):
@@ -53,23 +56,23 @@ def _cpu_backward(x, a, b, ids, scale, steps, seed, up):
             dx[at], da[e], db[e] = g @ ae, g.T @ xs[at], u.T @ (xs[at] @ ae.T)
     if keep is not None:
         dx = torch.where(keep, dx * share, 0.0)
-    return dx.to(x.dtype), da.to(a.dtype), db.to(b.dtype)
+    return dx.to(x.dtype), da.to(a.dtype).view(shapes[0]), db.to(b.dtype).view(shapes[1])
 
 
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, a, b, base, ids, scale, steps, seed):
-        ctx.scale, ctx.steps, ctx.seed = (None if isinstance(v, torch.Tensor) else v for v in (scale, steps, seed))
+    def forward(ctx, x, a, b, base, how):
+        ids, scale, steps, seed = how
         held = [v for v in (scale, seed) if isinstance(v, torch.Tensor)]
+        ctx.how = ids is not None, None if isinstance(scale, torch.Tensor) else scale, steps, None if isinstance(seed, torch.Tensor) else seed, a.dim()
         if not x.is_cuda:
-            ids = None if ids is None else ids.reshape(-1)
             ctx.save_for_backward(x, a, b, ids, *held)
             return _cpu_forward(x, a, b, base, ids, scale, steps, seed)
         want_x, want_a, want_b = ctx.needs_input_grad[:3]
         y, kept = train_ops.low_rank_forward(x, a, b, base, ids, scale, steps, seed, train=True, values=want_b)
         # x is for the gradient of a, a for that of x
         ctx.save_for_backward(x if want_a else None, a if want_x else None, b, kept, *held)
-        ctx.width, ctx.grouped = x.shape[1], ids is not None
+        ctx.width = x.shape[1]
         return y
 
     @staticmethod
@@ -77,15 +80,19 @@ class _LowRankUpdate(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("low_rank_update: its gradients cannot be differentiated again (create_graph=True)")
         x, a, b, more, *held = ctx.saved_tensors
-        scale = held.pop(0) if ctx.scale is None else ctx.scale
-        seed = held.pop(0) if ctx.seed is None else ctx.seed
+        grouped, scale, steps, seed, _ = ctx.how
+        if scale is None:
+            scale = held.pop(0)
+        if seed is None:
+            seed = held.pop(0)
         want_x, want_a, want_b, want_base = ctx.needs_input_grad[:4]
         dx = da = db = None
         if not up.is_cuda:
-            dx, da, db = _cpu_backward(x, a, b, more, scale, ctx.steps, seed, up)
+            dx, da, db = _cpu_backward(x, a, b, more, scale, steps, seed, up)
+            dx, da, db = dx if want_x else None, da if want_a else None, db if want_b else None
         elif want_x or want_a or want_b:
-            dx, da, db = train_ops.low_rank_backward(x, rows_of(up), a, b, ctx.width, more, ctx.grouped, want_b, scale, ctx.steps, seed, want_x, want_a, want_b)
-        return dx if want_x else None, da if want_a else None, db if want_b else None, up if want_base else None, None, None, None, None
+            dx, da, db = train_ops.low_rank_backward(x, rows_of(up), a, b, ctx.width, more, grouped, scale, steps, seed, want_x, want_a, want_b)
+        return dx, da, db, up if want_base else None, None
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -172,10 +179,8 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     wants_grad = torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or (base is not None and base.requires_grad))
     if out is not None:
         _check_out(out, (*rows, cols), x, [t for t in (x, a, b, ids, scale, seed) if isinstance(t, torch.Tensor)], base, wants_grad)
-    if single:
-        a, b = a[None], b[None]
     if n == 0:
-        y = x @ a[0].T @ b[0].T                     # zero gradients
+        y = (x @ a.T @ b.T) if single else x @ a[0].T @ b[0].T                     # zero gradients
         return out if out is not None else y if base is None else base + y
     flat, base2 = rows_of(x), None if base is None else rows_of(base)
     a, b = a.contiguous(), b.contiguous()
@@ -184,10 +189,10 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
         if not x.is_cuda and bool((ids >= count).any()):
             raise IndexError(f"{what}: an id names none of {count} adapters")
     if wants_grad:
-        y = _LowRankUpdate.apply(flat, a, b, base2, ids, scale, steps, seed)
+        y = _LowRankUpdate.apply(flat, a, b, base2, (ids, scale, steps, seed))
         return y if len(xs) == 2 else y.reshape((*rows, cols))
     if not x.is_cuda:
-        y = _cpu_forward(flat, a, b, base2, None if ids is None else ids.reshape(-1), scale, steps, seed).reshape((*rows, cols))
+        y = _cpu_forward(flat, a, b, base2, ids, scale, steps, seed).reshape((*rows, cols))
         return y if out is None else out.copy_(y)
     y, _ = train_ops.low_rank_forward(flat, a, b, base2, ids, scale, steps, seed, out=None if out is None else out if out.dim() == 2 else out.view(-1, cols))
     if out is None:

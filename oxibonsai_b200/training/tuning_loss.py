@@ -57,11 +57,10 @@ def _rows(t):
 # ---- preference pairs --------------------------------------------------------------------------------------------------------------------
 class _Preference(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logps, ref, mask, beta, kind, smoothing, average, reduction, keep):
-        loss, rewards, kept = train_ops.preference_forward(logps, ref, mask, beta, kind, smoothing, average, reduction, keep)
-        if keep:
-            ctx.save_for_backward(kept, mask)
-            ctx.shape, ctx.dtype = logps.shape, logps.dtype
+    def forward(ctx, logps, how):
+        loss, rewards, kept = train_ops.preference_forward(logps, *how, True)
+        ctx.save_for_backward(kept, how[1])
+        ctx.shape, ctx.dtype = logps.shape, logps.dtype
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
@@ -71,9 +70,9 @@ class _Preference(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("preference_loss: its gradients cannot be differentiated again (create_graph=True)")
         if up is None:
-            return (None,) * 9
+            return None, None
         kept, mask = ctx.saved_tensors
-        return (train_ops.tune_scale(kept, False, up.contiguous(), mask, ctx.shape, ctx.dtype),) + (None,) * 8
+        return train_ops.tune_scale(kept, False, up.contiguous(), mask, ctx.shape, ctx.dtype), None
 
 
 def _preference_cpu(logps, ref, mask, beta, kind, smoothing, average, reduction):
@@ -126,19 +125,21 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
         raise ValueError(f"{what}: label_smoothing is between 0 and 1 and for the sigmoid loss, got {label_smoothing} for {kind}")
     if not logps.is_cuda or logps.numel() == 0:
         return _preference_cpu(logps, ref_logps, mask, float(beta), kind, float(label_smoothing), average, reduction)
-    keep = torch.is_grad_enabled() and logps.requires_grad
-    loss, rewards = _Preference.apply(rows_of(logps), _rows(ref_logps), _rows(mask), float(beta), kind, float(label_smoothing), bool(average), reduction, keep)
+    how = _rows(ref_logps), _rows(mask), float(beta), kind, float(label_smoothing), bool(average), reduction
+    if torch.is_grad_enabled() and logps.requires_grad:
+        loss, rewards = _Preference.apply(rows_of(logps), how)
+    else:
+        loss, rewards, _ = train_ops.preference_forward(rows_of(logps), *how, False)
     return PreferenceLoss(loss, *rewards.chunk(2))
 
 
 # ---- clipped policy ratio ----------------------------------------------------------------------------------------------------------------
 class _Policy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logps, old, ref, mask, gain, clip, kl_weight, reduction, keep):
-        loss, stats, kept = train_ops.policy_forward(logps, old, ref, mask, gain, clip, kl_weight, reduction, keep)
-        if keep:
-            ctx.save_for_backward(kept)
-            ctx.shape, ctx.dtype = logps.shape, logps.dtype
+    def forward(ctx, logps, how):
+        loss, stats, kept = train_ops.policy_forward(logps, *how, True)
+        ctx.save_for_backward(kept)
+        ctx.shape, ctx.dtype = logps.shape, logps.dtype
         ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
         return loss, stats
@@ -148,8 +149,8 @@ class _Policy(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("policy_loss: its gradients cannot be differentiated again (create_graph=True)")
         if up is None:
-            return (None,) * 9
-        return (train_ops.tune_scale(ctx.saved_tensors[0], True, up.contiguous(), None, ctx.shape, ctx.dtype),) + (None,) * 8
+            return None, None
+        return train_ops.tune_scale(ctx.saved_tensors[0], True, up.contiguous(), None, ctx.shape, ctx.dtype), None
 
 
 def _policy_cpu(logps, old, ref, mask, gain, clip, kl_weight, reduction):
@@ -214,6 +215,9 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     if not logps.is_cuda or logps.numel() == 0:
         return _policy_cpu(logps, old_logps, ref_logps, mask, advantages, clip, float(kl_weight), reduction)
     gain = _rows(advantages.float()) if advantages.dim() == 2 else advantages.detach().float()
-    keep = torch.is_grad_enabled() and logps.requires_grad
-    loss, stats = _Policy.apply(rows_of(logps), _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction, keep)
+    how = _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction
+    if torch.is_grad_enabled() and logps.requires_grad:
+        loss, stats = _Policy.apply(rows_of(logps), how)
+    else:
+        loss, stats, _ = train_ops.policy_forward(rows_of(logps), *how, False)
     return PolicyLoss(loss, *stats.unbind())
