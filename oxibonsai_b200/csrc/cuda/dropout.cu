@@ -78,7 +78,6 @@ struct DropPlace {
 template <typename T, bool WHOLE, int U>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ y, long long rows, unsigned d,
                                                                unsigned groups, long long step_rows, unsigned step_groups, DropoutRule rule) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint2 key = philox_key(rule);
   const long long first = (long long)blockIdx.x * kDropThreads + threadIdx.x;

@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <math.h>
+
 #include "common.cuh"
 
 namespace bonsai {
@@ -87,18 +89,26 @@ __device__ __forceinline__ void tune_store4(T* p, int n, const float* v) {
   }
 }
 
-// Sum over a block of `blockDim.x` threads (whole warps), in thread 0, in one order.
-template <typename S>
-__device__ __forceinline__ S tune_block_sum(S v, S* s) {
+// Sums over a block of `blockDim.x` threads (whole warps), in thread 0, in one order; room for N of each warp.
+template <int N>
+__device__ __forceinline__ void tune_block_sums(double* v, double (*room)[N]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) room[threadIdx.x >> 5][i] = v[i];
+  }
   __syncthreads();
-  S t = S(0);
-  if (threadIdx.x == 0)
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += s[i];
-  return t;
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = room[0][i];
+      for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v[i] += room[w][i];
+    }
+  }
 }
 
 struct TuneRows {            // rows of tokens: an address and the distance of rows
@@ -125,6 +135,23 @@ __device__ __forceinline__ void tune_quads(const TuneShape& sh, int chunk, Body 
   }
 }
 
+// exp(x) - x - 1, and exp(x) - 1.  Up to 1/2 by the series x^2 / 2! + x^3 / 3! + ..., whose ninth term is below 2^-24 of the first; from there on
+// no more than two bits cancel.
+__device__ __forceinline__ float tune_excess(float x, float* grown) {
+  float p = 1.0f / 362880.0f;
+  p = fmaf(p, x, 1.0f / 40320.0f);
+  p = fmaf(p, x, 1.0f / 5040.0f);
+  p = fmaf(p, x, 1.0f / 720.0f);
+  p = fmaf(p, x, 1.0f / 120.0f);
+  p = fmaf(p, x, 1.0f / 24.0f);
+  p = fmaf(p, x, 1.0f / 6.0f);
+  p = fmaf(p, x, 0.5f);
+  const float small = p * x * x, large = expf(x) - 1.0f;
+  const bool near = fabsf(x) <= 0.5f;
+  *grown = near ? small + x : large;
+  return near ? small : large - x;
+}
+
 struct PolicyArgs {
   TuneShape shape;
   TuneRows logps, old, ref, mask;       // old, ref and mask may be absent
@@ -132,6 +159,7 @@ struct PolicyArgs {
   long long gain_ld;
   int gain_per_token;
   double log_low, log_high;             // of the borders 1 - lo and 1 + hi
+  float low_below, low_above, high_below, high_above;      // f32 next to them, or they themselves
   float low, high, kl_weight;
   float* slope;                         // [rows][length], absent where no gradient is wanted
   float* each;                          // [rows][length], absent where the loss is added up
@@ -140,8 +168,7 @@ struct PolicyArgs {
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kTuneThreads) policy_kernel(PolicyArgs a) {
-  __shared__ double sd[kTuneThreads / 32];
-  __shared__ int si[kTuneThreads / 32];
+  __shared__ double room[kTuneThreads / 32][4];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long row = blockIdx.x / a.shape.chunks;
@@ -152,8 +179,7 @@ __global__ void __launch_bounds__(kTuneThreads) policy_kernel(PolicyArgs a) {
   const unsigned char* mask = a.mask.p != nullptr ? (const unsigned char*)a.mask.p + row * a.mask.ld : nullptr;
   const float* gain = a.gain + row * a.gain_ld;
   const float row_gain = a.gain_per_token ? 0.0f : *gain;
-  double loss = 0.0, kls = 0.0;
-  int live = 0, cut = 0;
+  double v[4] = {0.0, 0.0, 0.0, 0.0};          // loss, divergence, live tokens, clipped ones
   tune_quads(a.shape, chunk, [&](int at, int n) {
     float l[4], o[4], r[4], g[4] = {row_gain, row_gain, row_gain, row_gain}, e[4], s[4];
     const unsigned m = tune_mask4<WIDE>(mask == nullptr ? nullptr : mask + at, n);
@@ -161,92 +187,110 @@ __global__ void __launch_bounds__(kTuneThreads) policy_kernel(PolicyArgs a) {
     if (old != nullptr) tune_load4<WIDE>(old + at, n, o);
     if (ref != nullptr) tune_load4<WIDE>(ref + at, n, r);
     if (a.gain_per_token) tune_load4<WIDE>(gain + at, n, g);
+    // Rounding keeps order: a step above the f32 behind a border is above the border, and only one between its neighbours needs l - old itself
+    float step[4];
+    unsigned over = 0, under = 0, near = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double step = old != nullptr ? (double)l[i] - (double)o[i] : (double)l[i] - (double)l[i];
-      const bool clipped = (g[i] > 0.0f && step > a.log_high) || (g[i] < 0.0f && step < a.log_low);
-      const float q = expf((float)step);
-      // a gain of 0 leaves 0, also where the ratio is infinite
-      const float gained = g[i] == 0.0f ? 0.0f : q * g[i];
-      float v = clipped ? -(g[i] > 0.0f ? a.high : a.low) * g[i] : -gained, d = clipped ? 0.0f : -gained, kl = 0.0f;
-      if (ref != nullptr) {
-        const float back = r[i] - l[i], grown = expm1f(back);
-        kl = grown - back;
-        if (a.kl_weight != 0.0f) {
-          v = fmaf(a.kl_weight, kl, v);
-          d = fmaf(-a.kl_weight, grown, d);
-        }
-      }
-      const bool on = m >> i & 1u;
-      e[i] = on ? v : 0.0f;
-      s[i] = on ? d : 0.0f;
-      loss += (double)e[i];
-      kls += on ? (double)kl : 0.0;
-      live += on;
-      cut += on && clipped;
+      step[i] = old != nullptr ? l[i] - o[i] : l[i] - l[i];
+      over |= (step[i] > a.high_above ? 1u : 0u) << i;
+      under |= (step[i] < a.low_below ? 1u : 0u) << i;
+      near |= (step[i] >= a.high_below && step[i] <= a.high_above) || (step[i] >= a.low_below && step[i] <= a.low_above) ? 1u : 0u;
     }
+    if (near && old != nullptr) {
+      over = under = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double exact = (double)l[i] - (double)o[i];
+        over |= (exact > a.log_high ? 1u : 0u) << i;
+        under |= (exact < a.log_low ? 1u : 0u) << i;
+      }
+    }
+    unsigned cut = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // a gain of 0 leaves 0, also where the ratio is infinite
+      const float gained = g[i] == 0.0f ? 0.0f : expf(step[i]) * g[i];
+      const unsigned clipped = (g[i] > 0.0f ? over : g[i] < 0.0f ? under : 0u) >> i & 1u;
+      cut |= clipped << i;
+      e[i] = clipped ? (g[i] > 0.0f ? -a.high : -a.low) * g[i] : -gained;
+      s[i] = clipped ? 0.0f : -gained;
+    }
+    float loss = 0.0f, kls = 0.0f;             // of four tokens
+    if (ref != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float grown;
+        const float kl = tune_excess(r[i] - l[i], &grown);
+        if (a.kl_weight != 0.0f) {
+          e[i] = fmaf(a.kl_weight, kl, e[i]);
+          s[i] = fmaf(-a.kl_weight, grown, s[i]);
+        }
+        kls += m >> i & 1u ? kl : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = m >> i & 1u ? e[i] : 0.0f;
+      s[i] = m >> i & 1u ? s[i] : 0.0f;
+      loss += e[i];
+    }
+    v[0] += (double)loss;
+    v[1] += (double)kls;
+    v[2] += (double)__popc(m);
+    v[3] += (double)__popc(cut & m);
     if (a.slope != nullptr) tune_store4<WIDE>(a.slope + row * a.shape.length + at, n, s);
     if (a.each != nullptr) tune_store4<WIDE>(a.each + row * a.shape.length + at, n, e);
   });
-  loss = tune_block_sum(loss, sd);
-  kls = tune_block_sum(kls, sd);
-  live = tune_block_sum(live, si);
-  cut = tune_block_sum(cut, si);
-  if (threadIdx.x == 0) a.part[blockIdx.x] = {loss, kls, live, cut};
+  tune_block_sums<4>(v, room);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = {v[0], v[1], (int)v[2], (int)v[3]};
 }
 
 enum TuneReduction { TUNE_TOKENS = 0, TUNE_SEQUENCES = 1, TUNE_SUM = 2, TUNE_NONE = 3 };
 
 // Adds the chunks up; weight[row] is what a token's loss counts in the whole.  One block.
 __global__ void __launch_bounds__(kTuneFinish) policy_finish_kernel(TuneShape sh, const TunePart* part, int reduction, float* loss, float* stats, float* weight) {
-  __shared__ double sd[kTuneFinish / 32];
-  __shared__ long long sl[kTuneFinish / 32];
-  __shared__ long long counts[2];
+  __shared__ double room[kTuneFinish / 32][6];
+  __shared__ double counts[2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  double sum = 0.0, kls = 0.0, means = 0.0;
-  long long live = 0, cut = 0, filled = 0;
+  double v[6] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};        // loss, divergence, live, clipped, rows with live tokens, means of rows
   for (long long row = threadIdx.x; row < sh.rows; row += kTuneFinish) {
-    double s = 0.0;
-    long long n = 0;
+    double s = 0.0, n = 0.0;
+#pragma unroll 4
     for (int c = 0; c < sh.chunks; ++c) {
       const TunePart p = part[row * sh.chunks + c];
       s += p.loss;
-      kls += p.kl;
-      n += p.live;
-      cut += p.clipped;
+      v[1] += p.kl;
+      n += (double)p.live;
+      v[3] += (double)p.clipped;
     }
-    sum += s;
-    live += n;
-    filled += n > 0;
-    means += n > 0 ? s / (double)n : 0.0;
+    v[0] += s;
+    v[2] += n;
+    v[4] += n > 0.0 ? 1.0 : 0.0;
+    if (reduction == TUNE_SEQUENCES) v[5] += n > 0.0 ? s / n : 0.0;
   }
-  sum = tune_block_sum(sum, sd);
-  kls = tune_block_sum(kls, sd);
-  means = tune_block_sum(means, sd);
-  live = tune_block_sum(live, sl);
-  cut = tune_block_sum(cut, sl);
-  filled = tune_block_sum(filled, sl);
+  tune_block_sums<6>(v, room);
   if (threadIdx.x == 0) {
-    const double n = (double)live;              // 0 / 0 is NaN: the mean of no tokens
-    if (loss != nullptr) *loss = (float)(reduction == TUNE_TOKENS ? sum / n : reduction == TUNE_SEQUENCES ? means / (double)filled : sum);
-    stats[0] = (float)(kls / n);
-    stats[1] = (float)((double)cut / n);
-    counts[0] = live;
-    counts[1] = filled;
+    const double one = 1.0 / v[2];              // 0 / 0 is NaN: the mean of no tokens
+    if (loss != nullptr) *loss = (float)(reduction == TUNE_TOKENS ? v[0] * one : reduction == TUNE_SEQUENCES ? v[5] / v[4] : v[0]);
+    stats[0] = (float)(v[1] * one);
+    stats[1] = (float)(v[3] * one);
+    counts[0] = v[2];
+    counts[1] = v[4];
   }
   if (weight == nullptr) return;
   __syncthreads();
   for (long long row = threadIdx.x; row < sh.rows; row += kTuneFinish) {
-    long long n = 1;
+    double n = 1.0;
     if (reduction == TUNE_TOKENS) {
       n = counts[0];
     } else if (reduction == TUNE_SEQUENCES) {
-      n = 0;
-      for (int c = 0; c < sh.chunks; ++c) n += part[row * sh.chunks + c].live;
+      n = 0.0;
+      for (int c = 0; c < sh.chunks; ++c) n += (double)part[row * sh.chunks + c].live;
       n *= counts[1];
     }
-    weight[row] = n > 0 ? (float)(1.0 / (double)n) : 0.0f;
+    weight[row] = n > 0.0 ? (float)(1.0 / n) : 0.0f;
   }
 }
 
@@ -291,8 +335,7 @@ struct PreferenceArgs {
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kTuneThreads) preference_kernel(PreferenceArgs a) {
-  __shared__ double sd[kTuneThreads / 32];
-  __shared__ int si[kTuneThreads / 32];
+  __shared__ double room[kTuneThreads / 32][2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long row = blockIdx.x / a.shape.chunks;
@@ -300,23 +343,18 @@ __global__ void __launch_bounds__(kTuneThreads) preference_kernel(PreferenceArgs
   const T* logps = (const T*)a.logps.p + row * a.logps.ld;
   const T* ref = a.ref.p != nullptr ? (const T*)a.ref.p + row * a.ref.ld : nullptr;
   const unsigned char* mask = a.mask.p != nullptr ? (const unsigned char*)a.mask.p + row * a.mask.ld : nullptr;
-  double sum = 0.0;
-  int live = 0;
+  double v[2] = {0.0, 0.0};             // differences, live tokens
   tune_quads(a.shape, chunk, [&](int at, int n) {
     float l[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const unsigned m = tune_mask4<WIDE>(mask == nullptr ? nullptr : mask + at, n);
     tune_load4<WIDE>(logps + at, n, l);
     if (ref != nullptr) tune_load4<WIDE>(ref + at, n, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool on = m >> i & 1u;
-      sum += on ? (double)(l[i] - r[i]) : 0.0;
-      live += on;
-    }
+    for (int i = 0; i < 4; ++i) v[0] += m >> i & 1u ? (double)(l[i] - r[i]) : 0.0;
+    v[1] += (double)__popc(m);
   });
-  sum = tune_block_sum(sum, sd);
-  live = tune_block_sum(live, si);
-  if (threadIdx.x == 0) a.part[blockIdx.x] = {sum, 0.0, live, 0};
+  tune_block_sums<2>(v, room);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = {v[0], 0.0, (int)v[1], 0};
 }
 
 enum PreferenceKind { PREF_SIGMOID = 0, PREF_HINGE = 1, PREF_IPO = 2 };
@@ -336,10 +374,10 @@ __device__ __forceinline__ double preference_row(const TunePart* part, int chunk
 
 __global__ void __launch_bounds__(kTuneFinish) preference_finish_kernel(long long pairs, int chunks, const TunePart* part, PreferenceRule rule, float* loss,
                                                                         float* chosen, float* rejected, float* slope) {
-  __shared__ double sd[kTuneFinish / 32];
+  __shared__ double room[kTuneFinish / 32][1];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  double sum = 0.0;
+  double sum[1] = {0.0};
   for (long long p = threadIdx.x; p < pairs; p += kTuneFinish) {
     double tc, tr;
     const double sc = preference_row(part + p * chunks, chunks, rule.average, &tc), sr = preference_row(part + (pairs + p) * chunks, chunks, rule.average, &tr);
@@ -360,7 +398,7 @@ __global__ void __launch_bounds__(kTuneFinish) preference_finish_kernel(long lon
       d = 2.0 * t;
     }
     if (rule.reduction == 2) loss[p] = (float)v;
-    sum += v;
+    sum[0] += v;
     chosen[p] = (float)(rule.beta * sc);
     rejected[p] = (float)(rule.beta * sr);
     if (slope != nullptr) {
@@ -369,8 +407,8 @@ __global__ void __launch_bounds__(kTuneFinish) preference_finish_kernel(long lon
       slope[pairs + p] = (float)(-d * tr);
     }
   }
-  sum = tune_block_sum(sum, sd);
-  if (threadIdx.x == 0 && rule.reduction != 2) *loss = (float)(rule.reduction == 0 ? sum / (double)pairs : sum);
+  tune_block_sums<1>(sum, room);
+  if (threadIdx.x == 0 && rule.reduction != 2) *loss = (float)(rule.reduction == 0 ? sum[0] / (double)pairs : sum[0]);
 }
 
 // Threads of a block: rows that fit a few warps take no more.
@@ -394,6 +432,16 @@ static TuneKept tune_kept(long long rows, long long length, int slopes) {
   k.slope = k.weight + (slopes == 2 ? (rows * 4 + 15) / 16 * 16 : 0);
   k.bytes = k.slope + (slopes == 2 ? rows * length * 4 : slopes == 1 ? rows * 4 : 0);
   return k;
+}
+
+// The largest f32 at most v, and the smallest at least v.
+static float tune_below(double v) {
+  const float f = (float)v;
+  return (double)f <= v ? f : nextafterf(f, -INFINITY);
+}
+static float tune_above(double v) {
+  const float f = (float)v;
+  return (double)f >= v ? f : nextafterf(f, INFINITY);
 }
 
 // Whether four neighbouring tokens of every row are one aligned access; an absent array does not matter.
@@ -426,8 +474,9 @@ int bonsai_policy_loss(const void* logps, long long ld_logps, const void* old, l
   float* weight = gradient ? (float*)((char*)kept + at.weight) : nullptr;
   const TuneShape sh = tune_shape(rows, length);
   const int size = type == 0 ? 4 : 2, threads = tune_threads(length);
-  PolicyArgs a = {sh, {logps, ld_logps}, {old, ld_old}, {ref, ld_ref}, {mask, ld_mask}, gain, ld_gain, gain_per_token, log1p(-low), log1p(high),
-                  (float)(1.0 - low), (float)(1.0 + high), (float)kl_weight, slope, reduction == TUNE_NONE ? loss : nullptr, (TunePart*)kept};
+  const double log_low = log1p(-low), log_high = log1p(high);
+  PolicyArgs a = {sh, {logps, ld_logps}, {old, ld_old}, {ref, ld_ref}, {mask, ld_mask}, gain, ld_gain, gain_per_token, log_low, log_high, tune_below(log_low), tune_above(log_low), tune_below(log_high),
+                  tune_above(log_high), (float)(1.0 - low), (float)(1.0 + high), (float)kl_weight, slope, reduction == TUNE_NONE ? loss : nullptr, (TunePart*)kept};
   const bool wide = length % 4 == 0 && tune_wide(logps, ld_logps, size) && tune_wide(old, ld_old, size) && tune_wide(ref, ld_ref, size) &&
                     tune_wide(mask, ld_mask, 1) && (!gain_per_token || tune_wide(gain, ld_gain, 4)) && tune_wide(slope, length, 4) &&
                     tune_wide(a.each, length, 4);
