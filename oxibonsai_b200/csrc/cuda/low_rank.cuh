@@ -17,7 +17,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <map>
+#include <mutex>
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "philox.cuh"
@@ -27,6 +30,7 @@ namespace bonsai {
 constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
 // From so many rows on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.
 constexpr int kLrSplit = 1024;
+static_assert(kLrSplit > kLrSelf, "rows without a plan have no rank values to keep");
 constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024, kLrSmemThird = 74 * 1024;        // dynamic shared memory of a block, of each of two or three on an SM
 constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
 enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
@@ -301,7 +305,7 @@ struct LrFactor {              // w2 of one adapter: forward [cols][rank], backw
   __device__ __forceinline__ static void whole(const T* at, long long cols, int k, int g, int t, uint32_t (*w)[2]) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int kEach = LrStep<T>::kEach;
-    const bool there = RANK % LrStep<T>::kStep == 0 || k + kEach * t < RANK;
+    const bool there = RANK % LrStep<T>::kStep == 0 ? k < RANK : k + kEach * t < RANK;         // behind the rank lies what is not this adapter's
     if (BACK) {
       uint32_t v[kEach][F32 ? 8 : 4];
 #pragma unroll
@@ -1266,8 +1270,20 @@ __global__ void __launch_bounds__(kLrThreads, R <= 32 ? 3 : 1) lr_outer_kernel(c
 template <typename Kern, typename... Args>
 static cudaError_t lr_launch(Kern kernel, long long clusters, int ranks, int smem, cudaStream_t st, const Args&... args) {
   if (clusters * ranks >= 1ll << 31) return cudaErrorInvalidValue;
-  cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
-  if (e != cudaSuccess) return e;
+  if (smem > 48 * 1024) {          // once for each kernel and device: it costs the host a microsecond
+    static std::mutex guard;
+    static std::map<std::pair<const void*, int>, int> allowed;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> hold(guard);
+    int& have = allowed[{(const void*)kernel, device}];
+    if (have < smem) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+      have = smem;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * ranks));
   cfg.blockDim = dim3(kLrThreads);

@@ -49,7 +49,8 @@ def test_update_sizes(n, d, out, rank, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("spread", ["mixed", "runs"])
-@pytest.mark.parametrize("n, adapters, rank", [(1, 3, 4), (16, 1, 16), (33, 40, 8), (255, 2, 5), (256, 7, 16), (257, 7, 16), (600, 64, 20), (1300, 3, 40), (2050, 30, 128)])
+@pytest.mark.parametrize("n, adapters, rank", [(1, 3, 4), (16, 1, 16), (33, 40, 8), (255, 2, 5), (256, 7, 16), (257, 7, 16), (600, 64, 20), (1300, 3, 40), (2050, 30, 128),
+                                               (1100, 40, 16), (1030, 200, 8)])
 def test_update_groups(n, adapters, rank, spread, dtype):
     args, got = check_update(n, 88, 104, rank, adapters, dtype, seed=n, bare=0.2, spread=spread)
     ids = args[6]
@@ -171,6 +172,22 @@ def test_update_strides_orders_and_out(dtype):
         assert got is out and torch.equal(block, whole)              # in place, and nothing beside it
     fresh = torch.full((40, 24), float("nan"), device=DEV, dtype=dtype)
     assert torch.equal(TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=fresh), want[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, rank", [(3, 8), (3, 5), (300, 8), (1100, 8), (1100, 4), (1100, 16), (1100, 24), (1100, 40)])
+def test_update_reads_its_own_factors(n, rank, dtype):
+    """NaN before and behind the factors, the rows and the base: nothing of it is read into a result."""
+    x, base, dy, a, b, scales, _ = update_inputs(n, 256, 192, rank, 0, dtype, DEV, seed=n)
+    want = run_update(x, base, dy, a, b, scales, None)
+
+    def fenced(t):
+        room = torch.full((t.numel() + 2 * 65536,), float("nan"), dtype=dtype, device=DEV)
+        room[65536:65536 + t.numel()] = t.flatten()
+        return room[65536:65536 + t.numel()].view(t.shape)
+
+    got = run_update(*(fenced(t) for t in (x, base, dy, a, b)), scales, None)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -416,7 +433,7 @@ def test_losses_without_parts(dtype):
         r = TR.policy_loss(logps, old, gain, mask=nothing, reduction=reduction)
         assert r.loss.isnan() and r.clipped.isnan() and not torch.autograd.grad(r.loss, logps)[0].any()
     r = TR.preference_loss(logps, ref, nothing)
-    assert abs(float(r.loss) - 0.6931472) < 1e-6 and not torch.autograd.grad(r.loss, logps)[0].any()
+    assert abs(float(r.loss.detach()) - 0.6931472) < 1e-6 and not torch.autograd.grad(r.loss, logps)[0].any()
     with torch.no_grad():
         assert not TR.policy_loss(logps, old, gain).loss.requires_grad and not TR.preference_loss(logps, ref).loss.requires_grad
 
