@@ -85,25 +85,27 @@ static int lr_vec(const void* p, long long ld, long long width, int size) { retu
 // What a forward pass leaves for the backward one, and what the backward pass works with: the rank values (and their two f16 parts where the second product is a
 // kernel of its own), the order of rows, where each adapter's rows begin in it, the tiles of 16 rows.
 struct LrRoom {
-  bool values, grouped, split;
+  bool values;
   long long parts, factors, order, start, tiles, tile_rows, bytes;
 };
-static LrRoom lr_room(int n, int rank, int adapters, int type, bool grouped, bool values) {
+static LrRoom lr_room(int n, int rank, int adapters, int type, bool grouped, bool values, bool split, bool tiles) {
   LrRoom k;
-  k.split = n >= kLrSplit;
-  k.values = values || k.split;
-  k.grouped = grouped;
+  k.values = values || split;
   auto up = [](long long b) { return (b + 15) / 16 * 16; };
-  const long long all = 4ll * n * lr_padded(rank);
+  const long long all = 4ll * n * lr_padded(rank), slots = grouped && tiles ? n / 16 + adapters + 2 : 0;
   k.parts = k.values ? all : 0;
-  k.factors = k.parts + (k.split && type == 1 ? all : 0);
-  k.order = k.factors + (k.split && type == 1 ? up(4ll * n) : 0);
+  k.factors = k.parts + (split && type == 1 ? all : 0);
+  k.order = k.factors + (split && type == 1 ? up(4ll * n) : 0);
   k.start = k.order + (grouped ? up(4ll * n) : 0);
   k.tiles = k.start + (grouped ? up(4ll * (adapters + 3)) : 0);
-  const long long slots = grouped && k.split ? n / 16 + adapters + 2 : 0;
   k.tile_rows = k.tiles + 16 * slots;
   k.bytes = k.tile_rows + 64 * slots;
   return k;
+}
+// Of a forward pass (tiles are for its own second product or that of the backward one), and the workspace of the backward one.
+static LrRoom lr_room_of(int n, int d, int out, int rank, int adapters, int type, bool grouped, bool values, bool back) {
+  return back ? lr_room(n, rank, adapters, type, false, true, lr_split_at(n, d), false)
+              : lr_room(n, rank, adapters, type, grouped, values, lr_split_at(n, out), lr_split_at(n, out) || lr_split_at(n, d));
 }
 static LrValues lr_values(void* room, const LrRoom& k) {
   char* p = (char*)room;
@@ -115,8 +117,9 @@ static void lr_grouped(LrGroups& g, void* room, const LrRoom& k) {
   g.mode = LR_PLAN;
   g.order = (const int*)(p + k.order);
   g.start = (const int*)(p + k.start);
-  g.tiles = k.split ? (const int4*)(p + k.tiles) : nullptr;
-  g.tile_rows = k.split ? (const int*)(p + k.tile_rows) : nullptr;
+  const bool tiles = k.tile_rows > k.tiles;
+  g.tiles = tiles ? (const int4*)(p + k.tiles) : nullptr;
+  g.tile_rows = tiles ? (const int*)(p + k.tile_rows) : nullptr;
 }
 
 template <typename Args>
@@ -131,11 +134,11 @@ extern "C" {
 // Rows of ids that a forward pass groups without `kept`, where no backward pass follows.
 int bonsai_lr_self_rows() { return bonsai::kLrSelf; }
 
-// Bytes of `kept` for a forward pass (values: the rank values are wanted behind it; grouped: ids are given), and of the workspace of the backward pass
-// (values, not grouped).  0: none is needed.  Negative for sizes that are refused.
-long long bonsai_lr_bytes(int n, int rank, int adapters, int type, int grouped, int values) {
+// Bytes of `kept` for a forward pass (values: the rank values are wanted behind it; grouped: ids are given), or of the workspace of the backward pass (back).
+// 0: none is needed.  Negative for sizes that are refused.
+long long bonsai_lr_bytes(int n, int d, int out, int rank, int adapters, int type, int grouped, int values, int back) {
   using namespace bonsai;
-  return lr_good(n, 1, 1, rank, adapters, type) ? lr_room(n, rank, adapters, type, grouped, values).bytes : BONSAI_CUDA_BAD_ARG;
+  return lr_good(n, d, out, rank, adapters, type) ? lr_room_of(n, d, out, rank, adapters, type, grouped, values, back).bytes : BONSAI_CUDA_BAD_ARG;
 }
 
 // y [n][out] = base + s b (a x) by rows: a [adapters][rank][d], b [adapters][out][rank], rows of x, base and y at distances of their ld; base may be null, or y
@@ -149,7 +152,7 @@ int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b
       (ids == nullptr && adapters != 1))
     return BONSAI_CUDA_BAD_ARG;
   const bool self = ids != nullptr && kept == nullptr && !values && n <= kLrSelf;
-  const LrRoom at = lr_room(n, rank, adapters, type, ids != nullptr, values);
+  const LrRoom at = lr_room_of(n, d, out, rank, adapters, type, ids != nullptr, values, false);
   if (!self && at.bytes > 0 && (kept == nullptr || kept_bytes < at.bytes)) return BONSAI_CUDA_BAD_ARG;
   LrGroups g = {LR_ONE, ids, ids_wide, nullptr, nullptr, nullptr, nullptr, n, adapters};
   cudaError_t e = cudaSuccess;
@@ -162,7 +165,7 @@ int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b
   }
   if (e != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
   const int size = type == 0 ? 4 : 2;
-  LrRowsArgs r = {g, x, ldx, a, b, base, ld_base, y, ldy, self ? LrValues{} : lr_values(kept, at), scales, scale, d, out, rank};
+  LrRowsArgs r = {g, x, ldx, a, b, base, ld_base, y, ldy, self ? LrValues{} : lr_values(kept, at), scales, scale, d, out, rank, lr_split_at(n, out)};
   r.vec_x = lr_vec(x, ldx, d, size);
   r.vec_w1 = lr_vec(a, d, d, size);
   r.vec_w2 = rank % (8 / size) == 0 && (uintptr_t)b % 8 == 0;         // rank values of a column as words of 8 bytes
@@ -173,7 +176,7 @@ int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b
 }
 
 // Gradients of bonsai_lr_forward: dx [n][d], da, db (like a and b; zeros of adapters without rows), each may be null.  kept: of the forward pass, with the
-// values where db is wanted (values, grouped: as there).  ws: bonsai_lr_bytes(n, rank, adapters, type, 0, 1) where dx or da is wanted.
+// values where db is wanted (values, grouped: as there).  ws: bonsai_lr_bytes of the backward pass where dx or da is wanted.
 int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long lddy, const void* a, const void* b, void* dx, void* da, void* db,
                        const float* scales, float scale, int n, int d, int out, int rank, int adapters, int type, int grouped, const void* kept,
                        long long kept_bytes, int values, void* ws, long long ws_bytes, unsigned long long seed, const long long* seed_dev, int steps,
@@ -183,7 +186,7 @@ int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long l
       (dx != nullptr && a == nullptr) || (da != nullptr && x == nullptr) || (db != nullptr && !values))
     return BONSAI_CUDA_BAD_ARG;
   const bool rows = dx != nullptr || da != nullptr;
-  const LrRoom at = lr_room(n, rank, adapters, type, grouped, values), of = lr_room(n, rank, adapters, type, false, true);
+  const LrRoom at = lr_room_of(n, d, out, rank, adapters, type, grouped, values, false), of = lr_room_of(n, d, out, rank, adapters, type, grouped, values, true);
   if ((at.bytes > 0 && (kept == nullptr || kept_bytes < at.bytes)) || (rows && (ws == nullptr || ws_bytes < of.bytes))) return BONSAI_CUDA_BAD_ARG;
   LrGroups g = {LR_ONE, nullptr, 0, nullptr, nullptr, nullptr, nullptr, n, adapters};
   if (grouped) lr_grouped(g, (void*)kept, at);
@@ -191,7 +194,7 @@ int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long l
   const DropoutRule rule = dropout_rule(seed, seed_dev, steps);
   cudaError_t e = cudaSuccess;
   if (rows) {
-    LrRowsArgs r = {g, dy, lddy, b, a, nullptr, 0, dx, d, lr_values(ws, of), scales, scale, out, d, rank};
+    LrRowsArgs r = {g, dy, lddy, b, a, nullptr, 0, dx, d, lr_values(ws, of), scales, scale, out, d, rank, lr_split_at(n, d)};
     r.vec_x = lr_vec(dy, lddy, out, size);
     r.vec_w1 = lr_vec(b, rank, rank, size);
     r.vec_w2 = lr_vec(a, d, d, size);

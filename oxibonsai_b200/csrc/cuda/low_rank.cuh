@@ -28,9 +28,11 @@
 namespace bonsai {
 
 constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
-// From so many rows on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.
+// From so many rows and results on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.  bf16, rank 16,
+// us in one kernel and in two: 2000 rows 4096 to 4096 19 and 23, 4000 rows 34 and 37, 2000 rows 4096 to 12288 38 and 34, 8000 rows 4096 to 4096 67 and 49,
+// to 12288 143 and 94.
 constexpr int kLrSplit = 1024;
-static_assert(kLrSplit > kLrSelf, "rows without a plan have no rank values to keep");
+inline bool lr_split_at(int n, int cols) { return n >= kLrSplit && (long long)n * cols >= 1 << 24; }
 constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024, kLrSmemThird = 74 * 1024;        // dynamic shared memory of a block, of each of two or three on an SM
 constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
 enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
@@ -41,7 +43,7 @@ struct LrGroups {            // which rows have which adapter
   int ids_wide;              // int64, else int32
   const int* order;          // LR_PLAN: rows by adapter; behind them those without one, and those whose id names none
   const int* start;          // [adapters + 3]: where each adapter's rows begin in it
-  const int4* tiles;         // LR_PLAN of kLrSplit rows and more: tiles of 16 rows: group (-1: none), place, number of rows
+  const int4* tiles;         // LR_PLAN where a product is split: tiles of 16 rows: group (-1: none), place, number of rows
   const int* tile_rows;      // and their rows, -1 behind the last
   int n, adapters;
 };
@@ -64,6 +66,7 @@ struct LrRowsArgs {
   const float* scales;                   // of the adapters, or null: scale
   float scale;
   int k, cols, rank;
+  int split;                             // two kernels: lr_split_at
   int vec_x, vec_w1, vec_w2, vec_y;      // rows that 16-byte (w2 of the forward pass: 8-byte) accesses may take
   DropoutRule drop;
   int drop_x, drop_y;                    // forward: the rows of x; backward: those of dx
@@ -1345,7 +1348,7 @@ static cudaError_t lr_expand_as(const LrRowsArgs& a, cudaStream_t st) {
 template <typename T, int R, bool BACK>
 static cudaError_t lr_rows_r(const LrRowsArgs& a, cudaStream_t st) {
   const LrGroups& g = a.groups;
-  if (g.n < kLrSplit) return lr_rows_as<T, R, 16, BACK, false>(a, st);
+  if (!a.split) return lr_rows_as<T, R, 16, BACK, false>(a, st);
   // Tiles of 64 rows where adapters fill them; 16 rows keep more clusters busy and waste less of the tiles
   cudaError_t e;
   if (g.n / g.adapters >= 48) e = lr_rows_as<T, R, 64, BACK, true>(a, st);
@@ -1358,8 +1361,10 @@ static cudaError_t lr_outer_r(const LrOuterArgs& a, cudaStream_t st) {
   using L = LrOuterSmem<T, R>;
   const long long clusters = (long long)(a.blocks[0] + a.blocks[1]) * a.groups.adapters;
   const long long steps = (a.groups.n / a.groups.adapters + kLrOuterRows - 1) / kLrOuterRows;
-  // Columns that are dropped take twice the others' time: many short blocks then even out
-  const int ranks = a.drop_x && a.blocks[0] > 0 && a.blocks[1] > 0 && steps >= 32 ? 8 : lr_ranks_for(clusters, steps, 148 * (R <= 32 ? (L::kBytes <= kLrSmemThird ? 3 : 2) : 1), 4);
+  // How the rows are split goes by both products, wanted or not: a gradient has the same bits alone and beside the other.  Columns that are dropped take twice
+  // the others' time: many short blocks then even out.
+  const long long both = ((a.width[0] + kLrOuterCols - 1) / kLrOuterCols + (a.width[1] + kLrOuterCols - 1) / kLrOuterCols) * (long long)a.groups.adapters;
+  const int ranks = a.drop_x && steps >= 32 ? 8 : lr_ranks_for(both, steps, 148 * (R <= 32 ? (L::kBytes <= kLrSmemThird ? 3 : 2) : 1), 4);
   return lr_launch(lr_outer_kernel<T, R>, clusters, ranks, L::kBytes, st, a);
 }
 

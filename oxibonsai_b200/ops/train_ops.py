@@ -26,7 +26,7 @@ _SIG = {
     "bonsai_mt_adam": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _d, _vp, _d, _d, _d, _d, _i, _vp, _d, _vp, _vp, _vp],
     "bonsai_dropout": [_vp, _ll, _vp, _ll, _ll, _i, _u64, _vp, _i, _vp],
     "bonsai_lr_self_rows": [],
-    "bonsai_lr_bytes": [_i, _i, _i, _i, _i, _i],
+    "bonsai_lr_bytes": [_i, _i, _i, _i, _i, _i, _i, _i, _i],
     "bonsai_lr_forward": [_vp, _ll, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _f, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _ll, _i, _u64, _vp, _i, _vp],
     "bonsai_lr_backward": [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _vp, _ll, _i, _vp, _ll, _u64, _vp, _i, _vp],
     "bonsai_tune_bytes": [_ll, _ll, _i],
@@ -192,8 +192,8 @@ def _scale(scale: float | torch.Tensor) -> tuple[int | None, float]:
     return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
 
 
-def _lr_room(n: int, rank: int, adapters: int, grouped: bool, values: bool, like: torch.Tensor) -> torch.Tensor | None:
-    size = int(_lib().bonsai_lr_bytes(n, rank, adapters, TYPE_CODES[like.dtype], grouped, values))
+def _lr_room(n: int, d: int, out: int, rank: int, adapters: int, grouped: bool, values: bool, back: bool, like: torch.Tensor) -> torch.Tensor | None:
+    size = int(_lib().bonsai_lr_bytes(n, d, out, rank, adapters, TYPE_CODES[like.dtype], grouped, values, back))
     K.check(min(0, size), "low_rank_bytes")
     return like.new_empty(size, dtype=torch.uint8) if size else None
 
@@ -207,7 +207,7 @@ def low_rank_forward(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: to
     with _on(device):
         y = x.new_empty((n, cols)) if out is None else out
         grouped = ids is not None
-        kept = None if not train and n <= _LR_SELF_ROWS else _lr_room(n, r, e, grouped, values, x)
+        kept = None if not train and n <= _LR_SELF_ROWS else _lr_room(n, d, cols, r, e, grouped, values, False, x)
         K.check(_lib().bonsai_lr_forward(x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), K.ptr(base), 0 if base is None else _ld(base), y.data_ptr(), _ld(y),
                                          *_scale(scale), n, d, cols, r, e, TYPE_CODES[x.dtype], K.ptr(ids), grouped and ids.dtype == torch.int64,
                                          K.ptr(kept), 0 if kept is None else kept.numel(), values, *_seed(seed), steps, _stream(device)), "low_rank_forward")
@@ -222,7 +222,7 @@ def low_rank_backward(x: torch.Tensor | None, dy: torch.Tensor, a: torch.Tensor 
         dx = dy.new_empty((n, d)) if want_x else None
         da = dy.new_empty((r, d) if one else (e, r, d)) if want_a else None
         db = dy.new_empty(b.shape) if want_b else None
-        ws = _lr_room(n, r, e, False, True, dy) if want_x or want_a else None
+        ws = _lr_room(n, d, cols, r, e, grouped, want_b, True, dy) if want_x or want_a else None
         K.check(_lib().bonsai_lr_backward(K.ptr(x), 0 if x is None else _ld(x), dy.data_ptr(), _ld(dy), K.ptr(a), b.data_ptr(), K.ptr(dx), K.ptr(da), K.ptr(db),
                                           *_scale(scale), n, d, cols, r, e, TYPE_CODES[dtype], grouped, K.ptr(kept), 0 if kept is None else kept.numel(), want_b,
                                           K.ptr(ws), 0 if ws is None else ws.numel(), *_seed(seed), steps, _stream(device)), "low_rank_backward")
