@@ -817,9 +817,8 @@ __global__ void __launch_bounds__(kLrThreads, SPLIT && R == 16 && sizeof(T) == 2
 template <typename T, int R, bool BACK> struct LrExpand {
   static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4, kCols = 32 * kGroups;         // of a block of columns
   static constexpr int kStages = 2, kPieces = 8, kBytes = BACK ? 0 : kLrWarps * kStages * kPieces * 512;
-  static constexpr bool kHold = R <= 32;
-  // groups of factors in registers: without base on its way, the factors are what is waited for
-  static constexpr int kWays = BACK && R == 16 && sizeof(T) == 2 ? 4 : 2;
+  static constexpr bool kHold = R <= 32 || (R == 64 && sizeof(T) == 2);
+  static constexpr int kWays = R == 64 ? 1 : 2;                                          // groups of factors in registers
   static_assert(kWays - 1 <= kGroups && kGroups % kWays == 0, "a block's groups take turns");
   static constexpr int kBlocks = R == 16 && sizeof(T) == 2 && !BACK ? 3 : 2;            // on an SM
 };
@@ -959,10 +958,87 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
       request(c + 2, stage);
     }
   };
+  // The backward factors lie by rank value: 64 columns at a time, column 8 n + j for column n of the j-th of eight instructions, so that all of a thread's
+  // 16 bytes of a rank value's row are its own; of a row it has 16 neighbouring results.  (32 columns as above use half of what they load: 52 us of
+  // 8192 rows to 4096 values at rank 32.)
+  auto walk_back = [&](auto known) {
+    constexpr int RANK = decltype(known)::value;
+    const int last = c1 < a.cols / X::kCols ? c1 : a.cols / X::kCols;
+    if (c >= last) return;
+    const T* at = (const T*)a.w2 + (long long)group * a.cols * a.rank + (long long)(4 * t) * a.cols + 8 * g + c * X::kCols;
+    constexpr int kNext = kSteps <= 2 ? kSteps : 1;
+    uint4 next[kNext][4];
+    auto ask = [&](int k, uint4* v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = 16 * k + 4 * t < RANK ? *reinterpret_cast<const uint4*>(at + (long long)(16 * k + i) * a.cols) : make_uint4(0, 0, 0, 0);
+    };
+    if constexpr (kSteps <= 2) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) ask(k, next[k]);
+    }
+    T* y[2] = {to[0] + c * X::kCols + 8 * t, to[1] + c * X::kCols + 8 * t};       // 16 t: `to` has 8 t
+    for (int b = 2 * c; b < 2 * last; ++b) {
+      float acc[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+      auto multiply = [&](int k, const uint4* v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned half = j & 1 ? 0x7632u : 0x5410u;
+          auto word = [&](int i) { return j < 2 ? v[i].x : j < 4 ? v[i].y : j < 6 ? v[i].z : v[i].w; };
+          const uint32_t w0 = __byte_perm(word(0), word(1), half), w1 = __byte_perm(word(2), word(3), half);
+          lr_mma16<T>(acc[j], held[k][1], w0, w1);
+          lr_mma16<T>(acc[j], held[k][0], w0, w1);
+        }
+      };
+      if constexpr (kSteps <= 2) {
+        uint4 now[kNext][4];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) now[k][i] = next[k][i];
+        at += 64;
+        if (b + 1 < 2 * last) {
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) ask(k, next[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) multiply(k, now[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          uint4 now[4];
+          ask(k, now);
+          multiply(k, now);
+        }
+        at += 64;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = F16 ? acc[j][2 * h + i] * up[h] : acc[j][2 * h + i];
+          if (a.drop_y) lr_drop(v, dropout_words((unsigned)(8 * b + 2 * t + i), row_of[h], key), a.drop.limit);
+          lr_store8<T, true>(y[h] + 8 * i, 8, v);
+        }
+      y[0] += 64;
+      y[1] += 64;
+    }
+    c = last;
+  };
   if constexpr (X::kHold) {
     if (has && count == 16 && a.vec_y && a.vec_w2 && (BACK || a.base != nullptr)) {
-      if (a.rank == R) walk(std::integral_constant<int, R>());
-      else if (R == 16 && a.rank == 8) walk(std::integral_constant<int, 8>());
+      if constexpr (BACK && !F32) {
+        if (a.rank == R) walk_back(std::integral_constant<int, R>());
+        else if (R == 16 && a.rank == 8) walk_back(std::integral_constant<int, 8>());
+      } else {
+        if (a.rank == R) walk(std::integral_constant<int, R>());
+        else if (R == 16 && a.rank == 8) walk(std::integral_constant<int, 8>());
+      }
     }
   }
   for (; c < c1; ++c, stage ^= 1) {                 // anything else
