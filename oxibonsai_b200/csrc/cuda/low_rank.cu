@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kPlanThreads) lr_plan_kernel(LrGroups g, int* 
 
 static bool lr_good(int n, int k, int cols, int rank, int adapters, int type) {
   constexpr int kMost = 1 << 30;
-  return n >= 1 && n < kMost && k >= 1 && k < kMost && cols >= 1 && cols < kMost && rank >= 1 && rank <= 128 && adapters >= 1 && adapters <= 65536 && type >= 0 &&
+  return n >= 1 && n < kMost && k >= 1 && k < kMost && cols >= 1 && cols < kMost && rank >= 1 && rank <= 128 && adapters >= 1 && adapters <= 4096 && type >= 0 &&
          type <= 2;
 }
 // rows of `width` values at distances of ld that begin at multiples of 16 bytes and hold whole eights

@@ -1,4 +1,4 @@
-#include "low_rank.cuh"
+#include "low_rank_launch.cuh"
 
 namespace bonsai {
 template <> cudaError_t lr_rows<__nv_bfloat16>(const LrRowsArgs& a, bool back, cudaStream_t st) { return lr_rows_of<__nv_bfloat16>(a, back, st); }

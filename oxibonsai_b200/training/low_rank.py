@@ -19,7 +19,7 @@ from .counter_dropout import check_p, check_seed, keep_steps, kept, rows_of
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _CPU_TYPES = _TYPES + (torch.float64,)
-MAX_RANK = 128
+MAX_RANK, MAX_ADAPTERS = 128, 4096
 
 
 def _cpu_parts(x, a, ids, scale, steps, seed):
@@ -127,10 +127,12 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     ``a`` [count, rank, in], ``b`` [count, out, rank] and ``ids`` [...] (int32 or int64) with each row's adapter, in any order.  A negative id
     is a row without one, whose result is ``base`` as it is.  An id of ``count`` or more raises IndexError on the CPU; on the GPU, where nothing waits,
     the results of that row and the gradient of its ``x`` are NaN, and no adapter's gradient has it.  ``scale``: a number, or float32 [count].  All
-    tensors have one type (float32, float16 or bfloat16; float64 on the CPU); ranks go up to 128, adapters to 65536, all sizes stay below 2^30.  ``dropout``
+    tensors have one type (float32, float16 or bfloat16; float64 on the CPU); ranks go up to 128, adapters to 4096, all sizes stay below 2^30.  ``dropout``
     zeroes values of ``x`` on their way in, as :func:`dropout` of ``x`` (as rows) with the same ``seed`` does.
 
-    Sums are float32 whatever the inputs, the rank values keep 22 bits or more, results and gradients are rounded once.  ``out`` takes the result of a call
+    Sums are float32 whatever the inputs, the rank values keep 22 bits (16 of bfloat16), results and gradients are rounded once.  How sums are split goes by the
+    sizes of the call: a row's last bits may differ between batches of different sizes, within a batch they do not depend on its place or the other rows.  A
+    row with an infinity has results that are not finite; other rows are as without it.  ``out`` takes the result of a call
     without gradients; it may be ``base`` itself.  Between the passes the rank values are kept (4 bytes each, the rank rounded up to 16, 32, 64 or 128), and
     ``x``, ``a`` and ``b`` as every product keeps them.  On the GPU nothing is read back and all memory comes from torch's allocator; a pass and its
     gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives are refused."""
@@ -142,8 +144,8 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
                          f"{tuple(xs)}, {tuple(sa)} and {tuple(sb)}")
     rows, d, rank, cols, count = xs[:-1], sa[-1], sa[-2], sb[-2], 1 if single else sa[0]
     n = math.prod(rows)
-    if not 1 <= rank <= MAX_RANK or not 1 <= count <= 65536 or d < 1 or cols < 1 or max(d, cols, n) >= 2 ** 30:
-        raise ValueError(f"{what}: 1 to 65536 adapters of rank 1 to {MAX_RANK}, widths of at least 1 and sizes below 2^30 are wanted, got {count} of rank {rank}, "
+    if not 1 <= rank <= MAX_RANK or not 1 <= count <= MAX_ADAPTERS or d < 1 or cols < 1 or max(d, cols, n) >= 2 ** 30:
+        raise ValueError(f"{what}: 1 to {MAX_ADAPTERS} adapters of rank 1 to {MAX_RANK}, widths of at least 1 and sizes below 2^30 are wanted, got {count} of rank {rank}, "
                          f"widths {d} and {cols}, {n} rows")
     if base is not None:
         if base.shape[:-1] != rows or base.shape[-1] != cols or base.dim() != len(xs):
@@ -212,8 +214,8 @@ class AdapterBank:
     """
 
     def __init__(self, in_features: int, out_features: int, rank: int, count: int, dtype: torch.dtype = torch.bfloat16, device="cuda"):
-        if not 1 <= rank <= MAX_RANK or not 1 <= count <= 65536 or min(in_features, out_features) < 1:
-            raise ValueError(f"AdapterBank: 1 to 65536 adapters of rank 1 to {MAX_RANK} are wanted, got {count} of rank {rank}, {in_features} to {out_features}")
+        if not 1 <= rank <= MAX_RANK or not 1 <= count <= MAX_ADAPTERS or min(in_features, out_features) < 1:
+            raise ValueError(f"AdapterBank: 1 to {MAX_ADAPTERS} adapters of rank 1 to {MAX_RANK} are wanted, got {count} of rank {rank}, {in_features} to {out_features}")
         self.a = torch.zeros(count, rank, in_features, dtype=dtype, device=device)
         self.b = torch.zeros(count, out_features, rank, dtype=dtype, device=device)
         self.scales = torch.zeros(count, dtype=torch.float32, device=device)
