@@ -10,9 +10,14 @@
 // gradients (lr_outer_kernel) are sums over an adapter's rows, split over a cluster and joined the same way.
 //
 // All are bound by memory: 2 rank operations for each value that is read.  So the matrix instructions are mma.sync, whose operands are gathered rows
-// from shared memory; tcgen05 would want tiles of 128 rows and does not pay at one operation a byte.  The long product of 16-bit types multiplies them as they are
-// (f32 sums); everything that meets the rank values keeps these in two TF32 parts, 22 bits, beside 16-bit operands that TF32 holds exactly.  f32 operands are
-// two TF32 parts too, three products of them, added to f32 registers every few steps because the matrix instructions' own sums truncate.
+// from shared memory; tcgen05 would want tiles of 128 rows of one adapter and does not pay at a few operations a byte.  The long product of 16-bit types
+// multiplies them as they are (f32 sums).  The rank values are kept in two parts, so that nothing is rounded to 16 bits between the products: two bf16
+// parts hold 16 bits, far below the result's 8; two f16 parts 22, over a power of two for each row in the second product, since f16's range would lose small
+// gradients; f16 in the sums over rows and f32 everywhere have two TF32 parts, 22 bits (f16 itself is exact in TF32).  f32 operands are two TF32 parts too,
+// three products of them, added to f32 registers every few steps because the matrix instructions' own sums truncate.
+//
+// Measured on one B200, rank 16, bf16, in a graph (copy rate 6.54 TB/s): 1 row 4096 to 4096 6.3 us, 64 rows over 48 adapters 4096 to 12288 15 us (f16); 8192 rows 4096 to
+// 12288 without dropout 95 us forward (470 MB: 4.9 TB/s), 80 us for dx (268 MB), 61 us for both factors' gradients (270 MB: 4.4 TB/s); dropout adds 12, 4 and 14.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,7 +35,8 @@ constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: ro
 // to 12288 143 and 94.
 constexpr int kLrSplit = 1024;
 inline bool lr_split_at(int n, int cols) { return n >= kLrSplit && (long long)n * cols >= 1 << 24; }
-constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024, kLrSmemThird = 74 * 1024;        // dynamic shared memory of a block, of each of two or three on an SM
+// dynamic shared memory of a block, of each of two or three on an SM
+constexpr int kLrSmemMost = 227 * 1024 - 2048, kLrSmemHalf = 112 * 1024, kLrSmemThird = 74 * 1024;
 constexpr int kLrOuterCols = 128, kLrOuterRows = 64;
 enum LrGrouping { LR_ONE = 0, LR_SELF = 1, LR_PLAN = 2 };
 
@@ -45,8 +51,8 @@ struct LrGroups {            // which rows have which adapter
   int n, adapters;
 };
 
-// The rank values of a forward or a backward pass, times the adapter's scale, by place in the order: f32 [n][R] (R: the padded rank), of bf16 two parts [2][n][R].  f16 for the second
-// product: two parts over a power of two for each row, and that power.
+// The rank values of a forward or a backward pass, times the adapter's scale, by place in the order: f32 [n][R] (R: the padded rank), of bf16 two parts
+// [2][n][R].  f16 for the second product: two parts over a power of two for each row, and that power.
 struct LrValues {
   void* values;
   __half* parts;

@@ -130,7 +130,8 @@ def test_update_refusals():
     bad = [dict(x=x[:, :7]), dict(a=a[0]), dict(b=b[:3]), dict(base=base[:, :4]), dict(ids=None), dict(ids=ids[:5]), dict(scale=scales[:2]),
            dict(scale=scales.double()), dict(scale=scales.clone().requires_grad_()), dict(dropout=1.1), dict(dropout=0.5, seed=-4), dict(out=base[:5]),
            dict(out=base.double()), dict(out=base.T.contiguous().T), dict(out=torch.empty(5).expand(6, 5)), dict(x=x[0, 0]),
-           dict(a=torch.zeros(4, 129, 8), b=torch.zeros(4, 5, 129)), dict(a=a[:, :0], b=b[:, :, :0]), dict(a=a[:0], b=b[:0], scale=scales[:0])]
+           dict(a=torch.zeros(4, 129, 8), b=torch.zeros(4, 5, 129)), dict(a=a[:, :0], b=b[:, :, :0]), dict(a=a[:0], b=b[:0], scale=scales[:0]),
+           dict(a=torch.zeros(4097, 1, 8), b=torch.zeros(4097, 5, 1), scale=1.0)]
     for change in bad:
         with pytest.raises(ValueError):
             TR.low_rank_update(**{**ok, **change})
