@@ -4,6 +4,10 @@
 //
 // The backward pass is the same kernel over the gradient.  A thread takes eight neighbouring values, one counter, and walks on by the
 // grid; its place (row, group of eight) is advanced by a quotient and a remainder from the host, without a division.
+//
+// Some 90 instructions go into eight values (ten rounds of two wide multiplications), about as long as 16-bit values take from memory: 8192 x 4096 bf16 (134 MB)
+// in 26.5 us, 5.1 TB/s.  Eight blocks an SM of which six fit are faster than six (30 us): the last ones fill in where others end.  The next kernel is not let
+// in early: its blocks would take places of this one's (333 x 2049 f32, there and back: 21 us, 11 without).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
