@@ -166,10 +166,11 @@ int bonsai_lr_forward(const void* x, long long ldx, const void* a, const void* b
   if (e != cudaSuccess) return BONSAI_CUDA_LAUNCH_FAILED;
   const int size = type == 0 ? 4 : 2;
   LrRowsArgs r = {g, x, ldx, a, b, base, ld_base, y, ldy, self ? LrValues{} : lr_values(kept, at), scales, scale, d, out, rank, lr_split_at(n, out)};
-  r.vec_x = lr_vec(x, ldx, d, size);
+  // a single row may have any stride
+  r.vec_x = lr_vec(x, n > 1 ? ldx : 0, d, size);
   r.vec_w1 = lr_vec(a, d, d, size);
   r.vec_w2 = rank % (8 / size) == 0 && (uintptr_t)b % 8 == 0;         // rank values of a column as words of 8 bytes
-  r.vec_y = lr_vec(y, ldy, out, size) && (base == nullptr || lr_vec(base, ld_base, out, size));
+  r.vec_y = lr_vec(y, n > 1 ? ldy : 0, out, size) && (base == nullptr || lr_vec(base, n > 1 ? ld_base : 0, out, size));
   r.drop = dropout_rule(seed, seed_dev, steps);
   r.drop_x = steps < 65536;
   return lr_rows_by(type, r, false, st) == cudaSuccess ? BONSAI_CUDA_OK : BONSAI_CUDA_LAUNCH_FAILED;
@@ -195,7 +196,7 @@ int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long l
   cudaError_t e = cudaSuccess;
   if (rows) {
     LrRowsArgs r = {g, dy, lddy, b, a, nullptr, 0, dx, d, lr_values(ws, of), scales, scale, out, d, rank, lr_split_at(n, d)};
-    r.vec_x = lr_vec(dy, lddy, out, size);
+    r.vec_x = lr_vec(dy, n > 1 ? lddy : 0, out, size);
     r.vec_w1 = lr_vec(b, rank, rank, size);
     r.vec_w2 = lr_vec(a, d, d, size);
     r.vec_y = lr_vec(dx, d, d, size);
@@ -207,8 +208,8 @@ int bonsai_lr_backward(const void* x, long long ldx, const void* dy, long long l
     LrOuterArgs o = {g, {x, dy}, {ldx, lddy}, {ws, kept}, {da, db}, {d, out}};
     o.blocks[0] = da != nullptr ? (d + kLrOuterCols - 1) / kLrOuterCols : 0;
     o.blocks[1] = db != nullptr ? (out + kLrOuterCols - 1) / kLrOuterCols : 0;
-    o.vec[0] = lr_vec(x, ldx, d, size);
-    o.vec[1] = lr_vec(dy, lddy, out, size);
+    o.vec[0] = lr_vec(x, n > 1 ? ldx : 0, d, size);
+    o.vec[1] = lr_vec(dy, n > 1 ? lddy : 0, out, size);
     o.rank = rank;
     o.drop = rule;
     o.drop_x = steps < 65536;

@@ -54,27 +54,25 @@ def _rows(t):
     return None if t is None else rows_of(t.detach() if t.requires_grad else t)
 
 
-# ---- preference pairs --------------------------------------------------------------------------------------------------------------------
-class _Preference(torch.autograd.Function):
+class _Loss(torch.autograd.Function):
+    """A loss that its kernels have made already: what it kept, and the gradient of the log-probabilities from that."""
+
     @staticmethod
-    def forward(ctx, logps, how):
-        loss, rewards, kept = train_ops.preference_forward(logps, *how, True)
-        ctx.save_for_backward(kept, how[1])
+    def forward(ctx, logps, made):
+        loss, kept, mask, ctx.tokens, ctx.what = made
+        ctx.save_for_backward(kept, mask)
         ctx.shape, ctx.dtype = logps.shape, logps.dtype
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
+        return loss
 
     @staticmethod
-    def backward(ctx, up, _):
+    def backward(ctx, up):
         if torch.is_grad_enabled():
-            raise RuntimeError("preference_loss: its gradients cannot be differentiated again (create_graph=True)")
-        if up is None:
-            return None, None
+            raise RuntimeError(f"{ctx.what}: its gradients cannot be differentiated again (create_graph=True)")
         kept, mask = ctx.saved_tensors
-        return train_ops.tune_scale(kept, False, up.contiguous(), mask, ctx.shape, ctx.dtype), None
+        return train_ops.tune_scale(kept, ctx.tokens, up.contiguous(), mask, ctx.shape, ctx.dtype), None
 
 
+# ---- preference pairs --------------------------------------------------------------------------------------------------------------------
 def _preference_cpu(logps, ref, mask, beta, kind, smoothing, average, reduction):
     wide = logps.double()
     d = wide if ref is None else wide - ref.double()
@@ -125,34 +123,13 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
         raise ValueError(f"{what}: label_smoothing is between 0 and 1 and for the sigmoid loss, got {label_smoothing} for {kind}")
     if not logps.is_cuda or logps.numel() == 0:
         return _preference_cpu(logps, ref_logps, mask, float(beta), kind, float(label_smoothing), average, reduction)
-    how = _rows(ref_logps), _rows(mask), float(beta), kind, float(label_smoothing), bool(average), reduction
-    if torch.is_grad_enabled() and logps.requires_grad:
-        loss, rewards = _Preference.apply(rows_of(logps), how)
-    else:
-        loss, rewards, _ = train_ops.preference_forward(rows_of(logps), *how, False)
-    return PreferenceLoss(loss, *rewards.chunk(2))
+    wants_grad = torch.is_grad_enabled() and logps.requires_grad
+    rows, mask = rows_of(logps), _rows(mask)
+    loss, rewards, kept = train_ops.preference_forward(rows, _rows(ref_logps), mask, float(beta), kind, float(label_smoothing), bool(average), reduction, wants_grad)
+    return PreferenceLoss(_Loss.apply(rows, (loss, kept, mask, False, what)) if wants_grad else loss, *rewards.chunk(2))
 
 
 # ---- clipped policy ratio ----------------------------------------------------------------------------------------------------------------
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logps, how):
-        loss, stats, kept = train_ops.policy_forward(logps, *how, True)
-        ctx.save_for_backward(kept)
-        ctx.shape, ctx.dtype = logps.shape, logps.dtype
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
-        return loss, stats
-
-    @staticmethod
-    def backward(ctx, up, _):
-        if torch.is_grad_enabled():
-            raise RuntimeError("policy_loss: its gradients cannot be differentiated again (create_graph=True)")
-        if up is None:
-            return None, None
-        return train_ops.tune_scale(ctx.saved_tensors[0], True, up.contiguous(), None, ctx.shape, ctx.dtype), None
-
-
 def _policy_cpu(logps, old, ref, mask, gain, clip, kl_weight, reduction):
     kind = torch.float64 if logps.dtype == torch.float64 else torch.float32
     live = torch.ones_like(logps, dtype=torch.bool) if mask is None else mask
@@ -215,9 +192,7 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     if not logps.is_cuda or logps.numel() == 0:
         return _policy_cpu(logps, old_logps, ref_logps, mask, advantages, clip, float(kl_weight), reduction)
     gain = _rows(advantages.float()) if advantages.dim() == 2 else advantages.detach().float()
-    how = _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction
-    if torch.is_grad_enabled() and logps.requires_grad:
-        loss, stats = _Policy.apply(rows_of(logps), how)
-    else:
-        loss, stats, _ = train_ops.policy_forward(rows_of(logps), *how, False)
-    return PolicyLoss(loss, *stats.unbind())
+    wants_grad = torch.is_grad_enabled() and logps.requires_grad
+    rows = rows_of(logps)
+    loss, stats, kept = train_ops.policy_forward(rows, _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction, wants_grad)
+    return PolicyLoss(_Loss.apply(rows, (loss, kept, None, True, what)) if wants_grad else loss, *stats.unbind())

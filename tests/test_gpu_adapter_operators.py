@@ -315,6 +315,34 @@ def test_update_streams_and_graphs():
             assert all(torch.equal(g, w) for g, w in zip(held, want))
 
 
+@pytest.mark.parametrize("n", [1, 7, 256, 300])
+def test_a_bank_in_a_graph(n):
+    """Served rows captured and replayed with other rows, ids and adapters, in place; beside an eager call on another stream."""
+    x, base, _, a, b, scales, ids = update_inputs(n, 264, 136, 12, 5, torch.float16, DEV, seed=n, bare=0.2)
+    bank = TR.AdapterBank(264, 136, rank=12, count=5, dtype=torch.float16, device=DEV)
+    bank.a.copy_(a), bank.b.copy_(b), bank.scales.copy_(scales)
+    sx, sbase, sids = x.clone(), base.clone(), ids.clone()
+    bank(sx, sbase, sids)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = bank(sx, sbase, sids)
+        bank(sx, y, sids, out=y)                     # a second time on top
+    other = torch.cuda.Stream()
+    for k in range(3):
+        sids.copy_(ids.roll(k))
+        sx.copy_(x.roll(k, 1))
+        bank.a.copy_(a.roll(k, 0))
+        other.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(other):
+            z = bank(sx, sbase, sids)
+            z = bank(sx, z, sids)
+        torch.cuda.synchronize()
+        assert torch.equal(y, z)
+        want, bound = update_by_formula(sx, sbase, base, bank.a, bank.b, scales, sids)
+        within(bank(sx, sbase, sids), want[0], bound[0], "y")
+
+
 def test_update_places_past_32_bits():
     """Rows whose places in x, base and the result pass 2^31 values."""
     n, cols = 70000, 32768
