@@ -155,6 +155,9 @@ __device__ __forceinline__ void lr_copy16(void* dst, const void* src, bool there
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(lr_smem(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void lr_copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(lr_smem(dst)), "l"(src) : "memory"); }
+__device__ __forceinline__ void lr_copy4(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(lr_smem(dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void lr_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void lr_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void lr_ldm4(uint32_t* r, const void* p) {
@@ -288,6 +291,31 @@ __device__ __forceinline__ void lr_copy8(T* dst, const T* src, int left, bool ve
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) dst[i] = i < left ? src[i] : lr_round<T>(0.0f);
+  }
+}
+
+// Rows at odd addresses into shared memory: C columns of rows r < ROWS from `from(r)` (null: zeros), `left` of them there (`any`: an address that is).  A warp takes
+// a row at a time, so that neighbouring lanes take neighbouring values; only those of f32 are wide enough for cp.async.  8000 rows 4095 to 4097 values, bf16, rank 16:
+// with eights to a thread 286 us forward and 348 backward, with this and the rows of lr_expand_kernel 183 and 244 (of 4096 values 62 and 99).
+template <typename T, int ROWS, int C, typename From>
+__device__ __forceinline__ void lr_copy_rows(T* to, int pitch, int left, const T* any, From from) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 2
+  for (int r = warp; r < ROWS; r += kLrWarps) {
+    const T* src = from(r);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < C / 32; ++i) {
+        const bool there = src != nullptr && i * 32 + lane < left;
+        lr_copy4(to + r * pitch + i * 32 + lane, there ? src + i * 32 + lane : any, there);
+      }
+    } else {
+      T v[C / 32];
+#pragma unroll
+      for (int i = 0; i < C / 32; ++i) v[i] = src != nullptr && i * 32 + lane < left ? src[i * 32 + lane] : lr_round<T>(0.0f);
+#pragma unroll
+      for (int i = 0; i < C / 32; ++i) to[r * pitch + i * 32 + lane] = v[i];
+    }
   }
 }
 

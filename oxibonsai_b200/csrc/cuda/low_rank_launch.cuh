@@ -10,7 +10,7 @@ namespace bonsai {
 template <auto KERNEL, typename... Args>
 static cudaError_t lr_launch(long long clusters, int ranks, int smem, cudaStream_t st, const Args&... args) {
   if (clusters * ranks >= 1ll << 31) return cudaErrorInvalidValue;
-  if (smem > 48 * 1024) {          // allowed once for each kernel and device: it costs the host a microsecond.  A kernel's size is always the same
+  if (smem > 48 * 1024) {          // allowed once for each kernel and device: it costs the host a microsecond.  A kernel's size above 48 KB is always the same
     static std::atomic<unsigned long long> allowed{0};
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -76,7 +76,7 @@ static cudaError_t lr_expand_as(const LrRowsArgs& a, cudaStream_t st) {
     if (cost < least) { least = cost; per = p; }
   }
   const long long grid = (long long)row_blocks * ((blocks + per - 1) / per);
-  return lr_launch<lr_expand_kernel<T, R, BACK>>(grid, 1, X::kBytes, st, a, tiles, row_blocks, per);
+  return lr_launch<lr_expand_kernel<T, R, BACK>>(grid, 1, X::bytes(a.vec_y), st, a, tiles, row_blocks, per);
 }
 
 template <typename T, int R, bool BACK>

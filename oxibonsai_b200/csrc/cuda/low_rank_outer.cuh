@@ -63,10 +63,12 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) lr_copy16(to + r * L::kPitchQ + i * (16 / sizeof(T)), src + i * (16 / sizeof(T)));
       }
-    } else {
+    } else if (a.vec[which]) {
 #pragma unroll 1
       for (int r = 0; r < kLrOuterRows; r += kRows)
-        lr_copy8<T>(to + r * L::kPitchQ, q + places[s % 4][r0 + r] + col0 + c0, from + r0 + r < last ? width - col0 - c0 : 0, a.vec[which], q);
+        lr_copy8<T>(to + r * L::kPitchQ, q + places[s % 4][r0 + r] + col0 + c0, from + r0 + r < last ? width - col0 - c0 : 0, true, q);
+    } else {
+      lr_copy_rows<T, kLrOuterRows, kLrOuterCols>(qs(slot), L::kPitchQ, width - col0, q, [&](int r) { return from + r < last ? q + places[s % 4][r] + col0 : (const T*)nullptr; });
     }
     // rank values: eights of the rows side by side, of bf16 both parts
     using P = typename std::conditional<BF16, T, float>::type;
@@ -101,6 +103,7 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
     lr_wait<kAhead - 1>();
     if (drop) {                     // the eights that this thread copied
       const int* list = rows[s % 4];
+      if (!a.vec[which]) __syncthreads();          // others have copied them
 #pragma unroll 2
       for (int u = threadIdx.x; u < kLrOuterRows * (kLrOuterCols / 8); u += kLrThreads) {
         const int r = u / (kLrOuterCols / 8), c = u % (kLrOuterCols / 8) * 8;

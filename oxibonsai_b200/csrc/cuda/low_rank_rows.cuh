@@ -261,9 +261,11 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
 #pragma unroll
           for (int v = 0; v < (int)sizeof(T) / 2; ++v)
             lr_copy16(xs + (xr + i * kRowStep) * L::kPitchX + xc + v * (16 / (int)sizeof(T)), from[i] + k0 + v * (16 / (int)sizeof(T)));
-      } else {
+      } else if (a.vec_x) {
 #pragma unroll
-        for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i] + k0, a.k - k0 - xc, a.vec_x, (const T*)a.x);
+        for (int i = 0; i < kX; ++i) lr_copy8<T>(xs + (xr + i * kRowStep) * L::kPitchX + xc, from[i] + k0, a.k - k0 - xc, true, (const T*)a.x);
+      } else {
+        lr_copy_rows<T, M, S::kChunk>(xs, L::kPitchX, a.k - k0, (const T*)a.x, [&](int r) { return rows[r] < 0 ? (const T*)nullptr : (const T*)a.x + rows[r] * a.ldx + k0; });
       }
       if (a.vec_w1 && a.rank == R && k0 + S::kChunk <= a.k) {
         const T* src = BACK ? w1 + (long long)(k0 + wr) * R + wc : w1 + (long long)wr * a.k + k0 + wc;
@@ -275,6 +277,10 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
           for (int v = 0; v < (int)sizeof(T) / 2; ++v)
             lr_copy16(ws + r * L::kPitchW + wc + v * (16 / (int)sizeof(T)), src + (BACK ? i * kStepW * R : (long long)i * kStepW * a.k) + v * (16 / (int)sizeof(T)));
         }
+        return;
+      }
+      if (!BACK && !a.vec_w1) {
+        lr_copy_rows<T, R, S::kChunk>(ws, L::kPitchW, a.k - k0, w1, [&](int r) { return r < a.rank ? w1 + (long long)r * a.k + k0 : (const T*)nullptr; });
         return;
       }
 #pragma unroll 1
@@ -304,6 +310,7 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
       lr_wait<L::kStages - 2>();
       T* xs = stage(slot);
       if (a.drop_x) {
+        if (!a.vec_x) __syncthreads();                 // others have copied this thread's eights
 #pragma unroll
         for (int i = 0; i < kX; ++i)
           if (from_row[i] >= 0)
@@ -535,7 +542,11 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
 // 8192 rows: 327 us, 289 without).
 template <typename T, int R, bool BACK> struct LrExpand {
   static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4, kCols = 32 * kGroups;         // of a block of columns
-  static constexpr int kStages = 2, kPieces = 8, kBytes = BACK ? 0 : kLrWarps * kStages * kPieces * 512;
+  static constexpr int kStages = 2, kPieces = 8, kRing = BACK ? 0 : kLrWarps * kStages * kPieces * 512;
+  // results of rows at odd addresses pass through shared memory, 16 rows of a block, so that lanes write neighbouring values (f32, 8000 rows 4095 to 4097 values,
+  // rank 16: 255 us forward and 446 backward with eights to a lane, 198 and 353 so)
+  static constexpr int kPitch = kCols + 16 / (int)sizeof(T), kTile = 16 * kPitch * (int)sizeof(T);
+  static constexpr int bytes(bool vec) { return vec ? kRing : kRing > kLrWarps * kTile ? kRing : kLrWarps * kTile; }
   static constexpr bool kHold = R <= 32 || (R == 64 && sizeof(T) == 2);
   static constexpr int kWays = R == 64 ? 1 : 2;                                          // groups of factors in registers
   static_assert(kWays - 1 <= kGroups && kGroups % kWays == 0, "a block's groups take turns");
@@ -760,6 +771,7 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
       }
     }
   }
+  T* tile = reinterpret_cast<T*>(lr_dynamic + warp * X::kTile);
   for (; c < c1; ++c, stage ^= 1) {                 // anything else
     if (!BACK) lr_wait<1>();
 #pragma unroll 1
@@ -812,9 +824,21 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
         }
-        if (a.vec_y) lr_store8<T, true>(to[h] + b * 32, 8, v);
-        else lr_store8<T, false>(to[h] + b * 32, left, v);
+        lr_store8<T, true>(a.vec_y ? to[h] + b * 32 : tile + (g + 8 * h) * X::kPitch + q * 32 + 8 * t, 8, v);
       }
+    }
+    if (!a.vec_y) {
+      __syncwarp();
+      T* p = (T*)a.y + c * X::kCols + lane;
+#pragma unroll 2
+      for (int r = 0; r < 16; ++r) {
+        const int row = __shfl_sync(0xffffffffu, r < 8 ? row_of[0] : row_of[1], (r & 7) * 4);
+        if (row < 0) continue;
+#pragma unroll
+        for (int q = 0; q < X::kGroups; ++q)
+          if (c * X::kCols + q * 32 + lane < a.cols) p[row * a.ldy + q * 32] = tile[r * X::kPitch + q * 32 + lane];
+      }
+      __syncwarp();
     }
     request(c + 2, stage);
   }
