@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kTuneThreads) policy_kernel(PolicyArgs a) {
       e[i] = clipped ? (g[i] > 0.0f ? -a.high : -a.low) * g[i] : -gained;
       s[i] = clipped ? 0.0f : -gained;
     }
-    float loss = 0.0f, kls = 0.0f;             // of four tokens
+    float loss = 0.0f, kls = 0.0f;             // of four tokens: no more rounding than each of them has, and a quarter of the conversions
     if (ref != nullptr) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -23,7 +23,7 @@ def keep_steps(p: float) -> int:
 def check_seed(seed, device: torch.device, what: str) -> train_ops.Seed:
     """``None`` draws one from torch's CPU generator; a tensor is read when the kernel runs."""
     if seed is None:
-        return int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64))
+        return int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64, device="cpu"))
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise ValueError(f"{what}: a seed tensor holds one int64 on {device}, got {seed.dtype} of shape {tuple(seed.shape)} on {seed.device}")
@@ -43,8 +43,8 @@ def kept(rows: int, d: int, steps: int, seed: train_ops.Seed) -> torch.Tensor:
     """The mask [rows, d] on the CPU: what stays."""
     seed = int(seed) & (2 ** 64 - 1)
     groups = -(-d // 8)
-    c0 = torch.arange(groups, dtype=torch.int64).expand(rows, groups)
-    c1, r = torch.zeros_like(c0), torch.arange(rows, dtype=torch.int64)[:, None].expand(rows, groups)
+    c0 = torch.arange(groups, dtype=torch.int64, device="cpu").expand(rows, groups)
+    c1, r = torch.zeros_like(c0), torch.arange(rows, dtype=torch.int64, device="cpu")[:, None].expand(rows, groups)
     c2, c3 = r & _LOW, r >> 32
     k0, k1 = seed & _LOW, seed >> 32
     for _ in range(10):

@@ -28,15 +28,15 @@ def _cpu_parts(x, a, ids, scale, steps, seed):
     keep = kept(*x.shape, steps, seed) if steps < 65536 else None
     share = 1.0 if keep is None else 65536.0 / steps if steps else 0.0
     count = 1 if a.dim() == 2 else len(a)
-    scales = scale.to(kind) if isinstance(scale, torch.Tensor) else torch.full((count,), scale, dtype=kind)
-    rows = [torch.arange(len(x))] if ids is None else [(ids.reshape(-1) == e).nonzero().flatten() for e in range(count)]
+    scales = scale.to(kind) if isinstance(scale, torch.Tensor) else torch.full((count,), scale, dtype=kind, device=x.device)
+    rows = [torch.arange(len(x), device=x.device)] if ids is None else [(ids.reshape(-1) == e).nonzero().flatten() for e in range(count)]
     return kind, keep, share, scales.reshape(-1), rows
 
 
 def _cpu_forward(x, a, b, base, ids, scale, steps, seed):
     kind, keep, share, scales, rows = _cpu_parts(x, a, ids, scale, steps, seed)
     xs = x.to(kind) if keep is None else torch.where(keep, x.to(kind) * share, 0.0)
-    y = torch.zeros(len(x), b.shape[-2], dtype=kind) if base is None else base.to(kind).clone()
+    y = x.new_zeros(len(x), b.shape[-2], dtype=kind) if base is None else base.to(kind).clone()
     a, b = a.view(-1, *a.shape[-2:]), b.view(-1, *b.shape[-2:])
     for e, at in enumerate(rows):
         if len(at):
@@ -48,7 +48,7 @@ def _cpu_backward(x, a, b, ids, scale, steps, seed, up):
     kind, keep, share, scales, rows = _cpu_parts(x, a, ids, scale, steps, seed)
     xs = x.to(kind) if keep is None else torch.where(keep, x.to(kind) * share, 0.0)
     shapes, a, b = (a.shape, b.shape), a.view(-1, *a.shape[-2:]), b.view(-1, *b.shape[-2:])
-    dx, da, db = torch.zeros_like(xs), torch.zeros(a.shape, dtype=kind), torch.zeros(b.shape, dtype=kind)
+    dx, da, db = torch.zeros_like(xs), a.new_zeros(a.shape, dtype=kind), b.new_zeros(b.shape, dtype=kind)
     for e, at in enumerate(rows):
         if len(at):
             u, ae, be = up[at].to(kind) * scales[e], a[e].to(kind), b[e].to(kind)

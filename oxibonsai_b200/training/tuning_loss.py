@@ -147,7 +147,7 @@ def _policy_cpu(logps, old, ref, mask, gain, clip, kl_weight, reduction):
         kl = torch.expm1(back) - back
         if kl_weight:
             each = each + kl_weight * kl
-    per = torch.zeros(logps.shape, dtype=kind).index_put(at, each)
+    per = logps.new_zeros(logps.shape, dtype=kind).index_put(at, each)
     size = live.sum(1)
     if reduction == "none":
         loss = per
@@ -173,8 +173,8 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     ``reduction``: "tokens" is the mean over all live tokens, "sequences" the mean over the sequences that have live tokens of each one's mean, "sum", or "none"
     (a loss of the shape of ``logps``, 0 at masked tokens); means of nothing are NaN, with a gradient of 0.  A clipped token has no gradient but the penalty's;
     whether it is clipped is decided on ``logps - old_logps`` in float64.  An advantage of 0 leaves the penalty alone, also where the ratio is infinite.  Returns
-    the loss, the mean of ``exp(gap) - gap - 1`` and the share of clipped tokens.  Sums are float64, losses float32 (float64 of float64, on the CPU), the gradient
-    has the type of ``logps``.  Between the passes four bytes for every token are kept.  Nothing is read back; second derivatives are refused on the GPU."""
+    the loss, the mean of ``exp(gap) - gap - 1`` and the share of clipped tokens.  Sums are float64 (on the GPU over fours that are added in
+    float32), losses float32 (float64 of float64, on the CPU), the gradient has the type of ``logps``.  Between the passes four bytes for every token are kept.  Nothing is read back; second derivatives are refused on the GPU."""
     what = "policy_loss"
     _check(what, logps, {"old_logps": old_logps, "ref_logps": ref_logps}, mask)
     if advantages.shape not in (logps.shape[:1], logps.shape) or advantages.device != logps.device or not advantages.is_floating_point():

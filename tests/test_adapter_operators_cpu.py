@@ -254,3 +254,22 @@ def test_loss_refusals():
                    dict(clip=(0.1,)), dict(kl_weight=0.1, ref_logps=None), dict(kl_weight=float("nan")), dict(reduction="mean"), dict(mask=mask.int())):
         with pytest.raises(ValueError):
             TR.policy_loss(**{**dict(logps=logps, old_logps=old, advantages=gain, mask=mask, ref_logps=ref), **change})
+
+
+def test_operators_beside_a_default_device():
+    """What the operators make themselves lies where their inputs do, whatever device a program has made the default."""
+    x, base, dy, a, b, scales, ids = update_inputs(9, 12, 10, 3, 2, torch.float32, "cpu", seed=1, bare=0.2)
+    one = a[:1].clone(), b[:1].clone()
+
+    def run():
+        logps = torch.ones_like(x).requires_grad_()
+        loss = TR.policy_loss(logps, None, x[:, 0]).loss
+        return [TR.dropout(x, 0.5, seed=3), *run_update(x, base, dy, a, b, scales, ids, dropout=0.5, seed=3), *run_update(x, None, dy, *one, 0.5, None), loss.detach(),
+                *torch.autograd.grad(loss, logps)]
+
+    torch.manual_seed(5)
+    drawn, want = TR.dropout(x, 0.5), run()
+    torch.manual_seed(5)
+    with torch.device("meta"):
+        again, got = TR.dropout(x, 0.5), run()
+    assert torch.equal(drawn, again) and all(torch.equal(g, w) for g, w in zip(got, want))

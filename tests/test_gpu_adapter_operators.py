@@ -1,4 +1,6 @@
 """The adapter operators' kernels against their formulas in 64 bits: sizes that no tile divides, groups of rows, masks, strides, streams, graphs."""
+import math
+
 import pytest
 import torch
 from adapter_operators import (loss_inputs, mask_by_formula, policy_by_formula, preference_by_formula, update_by_formula, update_inputs)
@@ -522,6 +524,21 @@ def test_losses_without_parts(dtype):
     assert abs(float(r.loss.detach()) - 0.6931472) < 1e-6 and not torch.autograd.grad(r.loss, logps)[0].any()
     with torch.no_grad():
         assert not TR.policy_loss(logps, old, gain).loss.requires_grad and not TR.preference_loss(logps, ref).loss.requires_grad
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (4, 0)])
+def test_losses_of_nothing(shape):
+    logps = torch.zeros(shape, device=DEV, requires_grad=True)
+    for reduction in ("tokens", "sequences", "sum", "none"):
+        got = TR.policy_loss(logps, None, torch.zeros(shape[0], device=DEV), ref_logps=torch.zeros(shape, device=DEV), kl_weight=0.1, reduction=reduction)
+        assert all(t.device.type == "cuda" for t in got) and got.kl.isnan() and got.clipped.isnan()
+        assert got.loss.shape == (shape if reduction == "none" else ())
+        assert (got.loss == 0).all() if reduction in ("sum", "none") else got.loss.isnan()
+        assert torch.autograd.grad(got.loss.sum(), logps)[0].shape == shape
+    got = TR.preference_loss(logps, torch.zeros(shape, device=DEV), reduction="none")
+    assert all(t.device.type == "cuda" and t.shape == (shape[0] // 2,) for t in got)
+    torch.testing.assert_close(got.loss.cpu(), torch.full((shape[0] // 2,), math.log(2.0)))
+    assert torch.autograd.grad(got.loss.sum(), logps)[0].shape == shape
 
 
 def test_losses_at_their_borders():
