@@ -273,3 +273,17 @@ def test_operators_beside_a_default_device():
     with torch.device("meta"):
         again, got = TR.dropout(x, 0.5), run()
     assert torch.equal(drawn, again) and all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_seeded_dropout_in_a_segment_that_runs_again():
+    x, _, _, a, b, scales, _ = update_inputs(6, 16, 12, 4, 0, torch.float64, "cpu", seed=2, bare=0.0)
+
+    def segment(v):
+        return TR.dropout(TR.low_rank_update(v, a, b, scale=scales, dropout=0.5, seed=7).tanh(), 0.25, seed=8)
+
+    grads = []
+    for run in (segment, lambda v: TR.checkpoint(segment, v)):
+        v = x.clone().requires_grad_()
+        y = run(v)
+        grads.append(torch.autograd.grad(y.square().sum(), v)[0])
+    assert grads[0].any() and torch.equal(*grads)
