@@ -82,7 +82,7 @@ static bool lr_good(int n, int k, int cols, int rank, int adapters, int type) {
 // rows of `width` values at distances of ld that begin at multiples of 16 bytes and hold whole eights
 static int lr_vec(const void* p, long long ld, long long width, int size) { return width % 8 == 0 && ((uintptr_t)p | (uintptr_t)(ld * size)) % 16 == 0; }
 
-// What a forward pass leaves for the backward one, and what the backward pass works with: the rank values (and their two f16 parts where the second product is a
+// What a forward pass leaves for the backward one, and what the backward pass works with: the rank values (of bf16 three parts; of f16 also their two parts where the second product is a
 // kernel of its own), the order of rows, where each adapter's rows begin in it, the tiles of 16 rows.
 struct LrRoom {
   bool values;
@@ -92,7 +92,7 @@ static LrRoom lr_room(int n, int rank, int adapters, int type, bool grouped, boo
   LrRoom k;
   k.values = values || split;
   auto up = [](long long b) { return (b + 15) / 16 * 16; };
-  const long long all = 4ll * n * lr_padded(rank), slots = grouped && tiles ? n / 16 + adapters + 2 : 0;
+  const long long all = (type == 2 ? 6ll : 4ll) * n * lr_padded(rank), slots = grouped && tiles ? n / 16 + adapters + 2 : 0;
   k.parts = k.values ? all : 0;
   k.factors = k.parts + (split && type == 1 ? all : 0);
   k.order = k.factors + (split && type == 1 ? up(4ll * n) : 0);

@@ -11,13 +11,14 @@
 //
 // All are bound by memory: 2 rank operations for each value that is read.  So the matrix instructions are mma.sync, whose operands are gathered rows
 // from shared memory; tcgen05 would want tiles of 128 rows of one adapter and does not pay at a few operations a byte.  The long product of 16-bit types
-// multiplies them as they are (f32 sums).  The rank values are kept in two parts, so that nothing is rounded to 16 bits between the products: two bf16
-// parts hold 16 bits, far below the result's 8; two f16 parts 22, over a power of two for each row in the second product, since f16's range would lose small
-// gradients; f16 in the sums over rows and f32 everywhere have two TF32 parts, 22 bits (f16 itself is exact in TF32).  f32 operands are two TF32 parts too,
-// three products of them, added to f32 registers every few steps because the matrix instructions' own sums truncate.
+// multiplies them as they are (f32 sums).  The rank values are kept in parts, so that nothing is rounded to 16 bits between the products: three bf16
+// parts hold the 24 bits of f32 (two would hold 16: one result in 256 then rounds to the other neighbour than f32's); two f16 parts 22, over a power of two for each
+// row in the second product, since f16's range would lose small gradients; f16 in the sums over rows and f32 everywhere have two TF32 parts, 22 bits (f16 itself
+// is exact in TF32).  f32 operands are two TF32 parts too, three products of them, added to f32 registers every few steps because the matrix instructions' own
+// sums truncate.
 //
 // Measured on one B200, rank 16, bf16, in a graph (copy rate 6.54 TB/s): 1 row 4096 to 4096 6.3 us, 64 rows over 48 adapters 4096 to 12288 15 us (f16); 8192 rows 4096 to
-// 12288 without dropout 95 us forward (470 MB: 4.9 TB/s), 80 us for dx (268 MB), 61 us for both factors' gradients (270 MB: 4.4 TB/s); dropout adds 12, 4 and 14.
+// 12288 without dropout 96 us forward (470 MB: 4.9 TB/s), 83 us for dx (268 MB), 70 us for both factors' gradients (270 MB: 3.9 TB/s); dropout adds 13, 7 and 14.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,8 +52,8 @@ struct LrGroups {            // which rows have which adapter
   int n, adapters;
 };
 
-// The rank values of a forward or a backward pass, times the adapter's scale, by place in the order: f32 [n][R] (R: the padded rank), of bf16 two parts
-// [2][n][R].  f16 for the second product: two parts over a power of two for each row, and that power.
+// The rank values of a forward or a backward pass, times the adapter's scale, by place in the order: f32 [n][R] (R: the padded rank), of bf16 three parts
+// [3][n][R].  f16 for the second product: two parts over a power of two for each row, and that power.
 struct LrValues {
   void* values;
   __half* parts;
@@ -85,6 +86,11 @@ struct LrOuterArgs {
   int rank;
   DropoutRule drop;
   int drop_x;
+};
+
+// Parts of a rank value in the products.
+template <typename T> struct LrParts {
+  static constexpr int kCount = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
 };
 
 // ---- values ------------------------------------------------------------------------------------------------------------------------------

@@ -6,17 +6,19 @@ namespace bonsai {
 
 // ---- the factors' gradients --------------------------------------------------------------------------------------------------------------
 // out[r][c] (or [c][r]) = sum over the adapter's rows of p[row][r] q[row][c]; the rank values p have the scales in them.  A cluster takes 128 columns of one adapter and one product, its blocks
-// split the rows.  bf16: the rank values' two parts times q, both as ldmatrix turns them.  f16 and f32: TF32, where f16 is exact (its range would lose small rank
+// split the rows.  bf16: the rank values' three parts times q, both as ldmatrix turns them.  f16 and f32: TF32, where f16 is exact (its range would lose small rank
 // values); the two rows 2 t and 2 t + 1 of every eight are then what a thread has of a matrix instruction's axis of eight, which is how
-// ldmatrix hands out 16-bit values of q; p follows.  8192 rows, 4096 and 12288 columns, rank 16, bf16: 270 MB in 61 us, 4.4 TB/s (the copies alone 48), with dropout of
-// the 4096 columns 75.
+// ldmatrix hands out 16-bit values of q; p follows.  8192 rows, 4096 and 12288 columns, rank 16, bf16: 270 MB in 70 us, 3.9 TB/s (with two parts 63), with dropout of
+// the 4096 columns 84.
 template <typename T, int R> struct LrOuterSmem {
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  static constexpr int kPitchQ = kLrOuterCols + (sizeof(T) == 4 ? 4 : 8), kPitchP = kBf16 ? R + 8 : R + 4;
-  static constexpr int kSizeP = kBf16 ? 2 : 4, kP = kLrOuterRows * kPitchP * kSizeP;            // one part
-  static constexpr int kStage = kLrOuterRows * kPitchQ * (int)sizeof(T) + 2 * kP;
+  // bf16: a row's three parts side by side, whose pitch spreads eight rows over all banks; else the first parts and, kP bytes on, the second ones
+  static constexpr int kPitchQ = kLrOuterCols + (sizeof(T) == 4 ? 4 : 8), kPitchP = kBf16 ? 3 * R + 8 : R + 4;
+  static constexpr int kP = kLrOuterRows * kPitchP * (kBf16 ? 2 : 4);
+  static constexpr int kStage = kLrOuterRows * kPitchQ * (int)sizeof(T) + (kBf16 ? 1 : 2) * kP;
   static constexpr int kSum = R * kLrOuterCols * 4;
-  static constexpr int kStages = 3 * kStage <= kLrSmemMost ? 3 : 2;
+  // bf16 of rank 64 takes two stages, which leave room for a second block: 8192 rows to 12288 columns in 180 us, with three stages and one block 217
+  static constexpr int kStages = 3 * kStage <= (kBf16 && R == 64 ? kLrSmemHalf : kLrSmemMost) ? 3 : 2;
   static constexpr int kBytes = kStages * kStage > kSum ? kStages * kStage : kSum;
   static constexpr int kBlocks = kBytes <= kLrSmemThird && R <= 32 ? 3 : kBytes <= kLrSmemHalf && R <= 64 ? 2 : 1;            // on an SM
   static_assert(kBytes <= kLrSmemMost, "shared memory");
@@ -70,9 +72,9 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
     } else {
       lr_copy_rows<T, kLrOuterRows, kLrOuterCols>(qs(slot), L::kPitchQ, width - col0, q, [&](int r) { return from + r < last ? q + places[s % 4][r] + col0 : (const T*)nullptr; });
     }
-    // rank values: eights of the rows side by side, of bf16 both parts
+    // rank values: eights of the rows side by side, of bf16 all parts
     using P = typename std::conditional<BF16, T, float>::type;
-    constexpr int kOne = kLrOuterRows * (R / 8), kAll = BF16 ? 2 * kOne : kOne;
+    constexpr int kOne = kLrOuterRows * (R / 8), kAll = BF16 ? 3 * kOne : kOne;
     const P* p = (const P*)a.p[which] + (long long)from * R;
 #pragma unroll
     for (int u0 = 0; u0 < kAll; u0 += kLrThreads) {
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
       if (kAll % kLrThreads != 0 && u >= kAll) break;
       const int part = u / kOne, r = u % kOne / (R / 8), c = u % (R / 8) * 8;
       const P* src = p + part * (long long)a.groups.n * R + r * R + c;
-      lr_copy8<P>((P*)(ps(slot) + part * L::kP) + r * L::kPitchP + c, src, from + r < last ? 8 : 0, true, (const P*)a.p[which]);
+      lr_copy8<P>((P*)ps(slot) + r * L::kPitchP + part * R + c, src, from + r < last ? 8 : 0, true, (const P*)a.p[which]);
     }
   };
   float acc[R / 16][2][4];
@@ -140,14 +142,13 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
         lr_ldm4t(w, qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
 #pragma unroll
         for (int i = 0; i < R / 16; ++i) {
-          uint32_t hi[4], lo[4];
           const T* p = pp + (k + (lane & 7) + (lane >> 4) * 8) * L::kPitchP + i * 16 + (lane >> 3 & 1) * 8;
-          lr_ldm4t(lo, p + L::kP / 2);
-          lr_ldm4t(hi, p);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            lr_mma16<T>(acc[i][j], lo, w[2 * j], w[2 * j + 1]);
-            lr_mma16<T>(acc[i][j], hi, w[2 * j], w[2 * j + 1]);
+          for (int part = 2; part >= 0; --part) {
+            uint32_t v[4];
+            lr_ldm4t(v, p + part * R);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) lr_mma16<T>(acc[i][j], v, w[2 * j], w[2 * j + 1]);
           }
         }
       }

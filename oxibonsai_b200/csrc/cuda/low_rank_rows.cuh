@@ -104,21 +104,21 @@ struct LrFactor {              // w2 of one adapter: forward [cols][rank], backw
   }
 };
 
-// acc += the rank values of 16 rows (two parts) times the factors of 32 columns
+// acc += the rank values of 16 rows (their parts, the largest first) times the factors of 32 columns
 template <typename T>
-__device__ __forceinline__ void lr_multiply(float (*acc)[4], const uint32_t* hi, const uint32_t* lo, const uint32_t (*w)[2]) {
+__device__ __forceinline__ void lr_multiply(float (*acc)[4], const uint32_t (*h)[4], const uint32_t (*w)[2]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if constexpr (sizeof(T) == 4) {
       uint32_t h0, l0, h1, l1;
       lr_split(__uint_as_float(w[j][0]), h0, l0);
       lr_split(__uint_as_float(w[j][1]), h1, l1);
-      lr_mma8(acc[j], lo, h0, h1);
-      lr_mma8(acc[j], hi, l0, l1);
-      lr_mma8(acc[j], hi, h0, h1);
+      lr_mma8(acc[j], h[1], h0, h1);
+      lr_mma8(acc[j], h[0], l0, l1);
+      lr_mma8(acc[j], h[0], h0, h1);
     } else {
-      lr_mma16<T>(acc[j], lo, w[j][0], w[j][1]);
-      lr_mma16<T>(acc[j], hi, w[j][0], w[j][1]);
+#pragma unroll
+      for (int p = LrParts<T>::kCount - 1; p >= 0; --p) lr_mma16<T>(acc[j], h[p], w[j][0], w[j][1]);
     }
   }
 }
@@ -155,12 +155,16 @@ __device__ __forceinline__ float lr_power(float top, float& down) {
   return scaled ? __uint_as_float((unsigned)(127 + e) << 23) : 1.0f;
 }
 template <typename T>
-__device__ __forceinline__ void lr_parts(const float* f, T* hi, T* lo) {
+__device__ __forceinline__ void lr_parts(const float* f, T (*part)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    hi[i] = lr_round<T>(f[i]);
-    const float h = lr_float<T>(hi[i]);
-    lo[i] = lr_round<T>(fabsf(h) <= 3.4028234e38f ? f[i] - h : 0.0f);
+    float left = f[i];
+#pragma unroll
+    for (int p = 0; p < LrParts<T>::kCount; ++p) {
+      part[p][i] = lr_round<T>(left);
+      const float h = lr_float<T>(part[p][i]);
+      left = fabsf(h) <= 3.4028234e38f ? left - h : 0.0f;          // an infinity has no other parts
+    }
   }
 }
 
@@ -170,15 +174,15 @@ template <typename T, int M> struct LrShape {
   static constexpr int kChunk = M == 64 && sizeof(T) == 4 ? 64 : 128, kWarpK = kChunk / kParts;
 };
 
-// SPLIT: the rank values are all that is made.  Else they wait for the second product in two parts, each of the inputs' 16-bit type (f16 over a power of two for
-// each row, so that neither large nor small ones are lost) or TF32, and tiles have 16 rows.
+// SPLIT: the rank values are all that is made.  Else they wait for the second product in their parts, each of the inputs' 16-bit type (f16 over a power of two
+// for each row, so that neither large nor small ones are lost) or TF32, and tiles have 16 rows.
 template <typename T, int R, int M, bool BACK, bool SPLIT> struct LrSmem {
   static constexpr int kPad = 16 / sizeof(T);
   static constexpr int kChunk = LrShape<T, M>::kChunk;
   static constexpr int kPitchX = kChunk + kPad, kPitchW = BACK ? R + 8 : kChunk + kPad, kRowsW = BACK ? kChunk : R;
   static constexpr int kStage = (M * kPitchX + kRowsW * kPitchW) * (int)sizeof(T);
   static constexpr int kJoin = LrShape<T, M>::kParts * M * R * 4;         // the warps' parts, over the stages
-  static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = SPLIT ? 0 : 2 * M * kPitchH * (int)sizeof(T);
+  static constexpr int kPart = M * R * 4, kPitchH = R + 8, kH = SPLIT ? 0 : LrParts<T>::kCount * M * kPitchH * (int)sizeof(T);
   // what of base is on its way: each lane's own 16 bytes, `kDepth` steps of a warp
   static constexpr int kDepth = sizeof(T) == 4 ? 2 : 4, kPieces = (int)sizeof(T);
   static constexpr int kBase = BACK || SPLIT ? 0 : kLrWarps * kDepth * kPieces * 512;
@@ -206,7 +210,7 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
   unsigned char* behind = lr_dynamic + L::kRing;
   float* join = reinterpret_cast<float*>(lr_dynamic);
   float* part = reinterpret_cast<float*>(behind);
-  T* hs = reinterpret_cast<T*>(behind + L::kPart);                   // first parts, then second parts
+  T* hs = reinterpret_cast<T*>(behind + L::kPart);                   // first parts, then second ones, then third ones
   const uint32_t rank = lr_rank(), ranks = lr_ranks();
   const LrTile tile = lr_tile<M>(a.groups, blockIdx.x / ranks, rows, scratch);
   if (tile.count == 0) return;                        // the whole cluster
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
       // behind the rank there is nothing, also beside an infinity, whose product with the zeros there is none
       float f[4] = {col < a.rank ? v.x * by : 0.0f, col + 1 < a.rank ? v.y * by : 0.0f, col + 2 < a.rank ? v.z * by : 0.0f, col + 3 < a.rank ? v.w * by : 0.0f};
       const bool keeps = a.kept.values != nullptr && rank == 0 && row < tile.count;
-      const long long place = (long long)(tile.place + row) * R + col, second = (long long)a.groups.n * R;
+      const long long place = (long long)(tile.place + row) * R + col, next = (long long)a.groups.n * R;
       if (!BF16 && keeps) *reinterpret_cast<float4*>((float*)a.kept.values + place) = make_float4(f[0], f[1], f[2], f[3]);
       if constexpr (F16) {
         float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))), down;
@@ -424,16 +428,14 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
           *reinterpret_cast<uint4*>(hs + (M + row) * L::kPitchH + col) = lo;
         }
       } else {
-        __align__(8) T hi[4], lo[4];
-        lr_parts<T>(f, hi, lo);
-        if constexpr (!SPLIT) {
-          *reinterpret_cast<uint2*>(hs + row * L::kPitchH + col) = *reinterpret_cast<const uint2*>(hi);
-          *reinterpret_cast<uint2*>(hs + (M + row) * L::kPitchH + col) = *reinterpret_cast<const uint2*>(lo);
-        }
+        __align__(8) T part_of[LrParts<T>::kCount][4];
+        lr_parts<T>(f, part_of);
         T* to = BF16 ? (T*)a.kept.values : (T*)a.kept.parts;
-        if (keeps && to != nullptr) {
-          *reinterpret_cast<uint2*>(to + place) = *reinterpret_cast<const uint2*>(hi);
-          *reinterpret_cast<uint2*>(to + second + place) = *reinterpret_cast<const uint2*>(lo);
+#pragma unroll
+        for (int p = 0; p < LrParts<T>::kCount; ++p) {
+          const uint2 four = *reinterpret_cast<const uint2*>(part_of[p]);
+          if constexpr (!SPLIT) *reinterpret_cast<uint2*>(hs + (p * M + row) * L::kPitchH + col) = four;
+          if (keeps && to != nullptr) *reinterpret_cast<uint2*>(to + p * next + place) = four;
         }
       }
     }
@@ -457,13 +459,13 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
     const float up[2] = {F16 && has ? factors[g] : 1.0f, F16 && has ? factors[g + 8] : 1.0f};
     constexpr bool kHold = R == 16;                                  // the rank values and the next factors stay in registers
     constexpr int kSteps = kHold ? R / kStep : 1;
-    uint32_t held[kSteps][2][4], next[kSteps][4][2];
+    uint32_t held[kSteps][LrParts<T>::kCount][4], next[kSteps][4][2];
     int b = b0 + warp;
     if (kHold && has) {
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        load_h(k * kStep, 0, held[k][0]);
-        load_h(k * kStep, 1, held[k][1]);
+#pragma unroll
+        for (int p = 0; p < LrParts<T>::kCount; ++p) load_h(k * kStep, p, held[k][p]);
         if (b < b1) w2.load(b, k * kStep, next[k]);
       }
     }
@@ -499,16 +501,16 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
             if (b + kLrWarps < b1) w2.load(b + kLrWarps, k * kStep, next[k]);
           }
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[k]);
+          for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k], w[k]);
         } else {
 #pragma unroll 2
           for (int k = 0; k < R; k += kStep) {
             if (k >= a.rank) break;
-            uint32_t w[4][2], hi[4], lo[4];
+            uint32_t w[4][2], h[LrParts<T>::kCount][4];
             w2.load(b, k, w);
-            load_h(k, 0, hi);
-            load_h(k, 1, lo);
-            lr_multiply<T>(acc, hi, lo, w);
+#pragma unroll
+            for (int p = 0; p < LrParts<T>::kCount; ++p) load_h(k, p, h[p]);
+            lr_multiply<T>(acc, h, w);
           }
         }
       }
@@ -606,35 +608,36 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
   request(c0 + 1, 1);
   const uint2 key = a.drop_y ? philox_key(a.drop) : make_uint2(0, 0);
   const LrFactor<T, BACK> w2((const T*)a.w2 + (has ? (long long)group * a.cols * a.rank : 0), a.cols, a.rank, a.vec_w2, g, t);
-  // two parts of the rank values; rows behind the last have those of the first one, which go nowhere
+  // the rank values' parts; rows behind the last have those of the first one, which go nowhere
   const long long at[2] = {(long long)(place + (g < count ? g : 0)) * R + kEach * t, (long long)(place + (g + 8 < count ? g + 8 : 0)) * R + kEach * t};
-  auto load_h = [&](int k, uint32_t* hi, uint32_t* lo) {
+  auto load_h = [&](int k, uint32_t (*part)[4]) {
     if constexpr (F32) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float2 f = *reinterpret_cast<const float2*>((const float*)a.kept.values + at[h] + k);
-        lr_split(f.x, hi[h], lo[h]);
-        lr_split(f.y, hi[2 + h], lo[2 + h]);
+        lr_split(f.x, part[0][h], part[1][h]);
+        lr_split(f.y, part[0][2 + h], part[1][2 + h]);
       }
     } else {
       const T* p = BF16 ? (const T*)a.kept.values : (const T*)a.kept.parts;
-      const long long second = (long long)a.groups.n * R;
+      const long long next = (long long)a.groups.n * R;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p + at[h] + k), v = *reinterpret_cast<const uint2*>(p + second + at[h] + k);
-        hi[h] = u.x; hi[2 + h] = u.y;
-        lo[h] = v.x; lo[2 + h] = v.y;
-      }
+      for (int i = 0; i < LrParts<T>::kCount; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 u = *reinterpret_cast<const uint2*>(p + i * next + at[h] + k);
+          part[i][h] = u.x; part[i][2 + h] = u.y;
+        }
     }
   };
   float up[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) up[h] = F16 && has ? a.kept.factors[place + (g + 8 * h < count ? g + 8 * h : 0)] : 1.0f;
   constexpr int kSteps = X::kHold ? R / kStep : 1;
-  uint32_t held[kSteps][2][4];
+  uint32_t held[kSteps][LrParts<T>::kCount][4];
   if (X::kHold && has) {
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) load_h(k * kStep, held[k][0], held[k][1]);
+    for (int k = 0; k < kSteps; ++k) load_h(k * kStep, held[k]);
   }
   int c = c0, stage = 0;
   // Whole blocks: 16 rows, all columns and their factors in whole accesses, the rank known.  Nothing is checked, and the next factors are on their way.
@@ -674,7 +677,7 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
         }
         if (q + X::kWays - 1 < X::kGroups || c + 1 < last) ask(q + X::kWays - 1);
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k][0], held[k][1], w[q % X::kWays][k]);
+        for (int k = 0; k < kSteps; ++k) lr_multiply<T>(acc, held[k], w[q % X::kWays][k]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
@@ -719,8 +722,8 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
           const unsigned half = j & 1 ? 0x7632u : 0x5410u;
           auto word = [&](int i) { return j < 2 ? v[i].x : j < 4 ? v[i].y : j < 6 ? v[i].z : v[i].w; };
           const uint32_t w0 = __byte_perm(word(0), word(1), half), w1 = __byte_perm(word(2), word(3), half);
-          lr_mma16<T>(acc[j], held[k][1], w0, w1);
-          lr_mma16<T>(acc[j], held[k][0], w0, w1);
+#pragma unroll
+          for (int p = LrParts<T>::kCount - 1; p >= 0; --p) lr_mma16<T>(acc[j], held[k][p], w0, w1);
         }
       };
       if constexpr (kSteps <= 2) {
@@ -801,16 +804,16 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
           for (int k = 0; k < kSteps; ++k) {
             uint32_t w[4][2];
             w2.load(b, k * kStep, w);
-            lr_multiply<T>(acc, held[k][0], held[k][1], w);
+            lr_multiply<T>(acc, held[k], w);
           }
         } else {
 #pragma unroll 2
           for (int k = 0; k < R; k += kStep) {
             if (k >= a.rank) break;
-            uint32_t w[4][2], hi[4], lo[4];
+            uint32_t w[4][2], h[LrParts<T>::kCount][4];
             w2.load(b, k, w);
-            load_h(k, hi, lo);
-            lr_multiply<T>(acc, hi, lo, w);
+            load_h(k, h);
+            lr_multiply<T>(acc, h, w);
           }
         }
       }

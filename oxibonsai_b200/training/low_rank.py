@@ -130,10 +130,10 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     tensors have one type (float32, float16 or bfloat16; float64 on the CPU); ranks go up to 128, adapters to 4096, all sizes stay below 2^30.  ``dropout``
     zeroes values of ``x`` on their way in, as :func:`dropout` of ``x`` (as rows) with the same ``seed`` does.
 
-    Sums are float32 whatever the inputs, the rank values keep 22 bits (16 of bfloat16), results and gradients are rounded once.  How sums are split goes by the
+    Sums are float32 whatever the inputs, the rank values keep 22 bits (24 of bfloat16), results and gradients are rounded once.  How sums are split goes by the
     sizes of the call: a row's last bits may differ between batches of different sizes, within a batch they do not depend on its place or the other rows.  A
     row with an infinity has results that are not finite; other rows are as without it.  ``out`` takes the result of a call
-    without gradients; it may be ``base`` itself.  Between the passes the rank values are kept (4 bytes each, the rank rounded up to 16, 32, 64 or 128), and
+    without gradients; it may be ``base`` itself.  Between the passes the rank values are kept (4 bytes each, 6 of bfloat16, the rank rounded up to 16, 32, 64 or 128), and
     ``x``, ``a`` and ``b`` as every product keeps them.  On the GPU nothing is read back and all memory comes from torch's allocator; a pass and its
     gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives are refused."""
     what = "low_rank_update"

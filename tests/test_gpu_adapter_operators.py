@@ -690,3 +690,56 @@ def _planar(codes):
         word |= nib << 4 * i
     word = torch.where(word >= 2 ** 31, word - 2 ** 32, word).to(torch.int32)
     return word.to(DEV), torch.full((n, k // 128), 0.05, dtype=torch.float16, device=DEV)
+
+
+# ---- what the entry points promise at their edges ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rank", [2, 16, 64, 128])
+@pytest.mark.parametrize("n, d, out", [(2, 200, 200), (1100, 200, 15360), (1100, 15360, 200)])
+def test_update_rank_values_of_21_bits(n, d, out, rank, dtype):
+    """Two rank values of 21 bits (sums of 200 products of 64 to 127) that differ by one term: their difference comes out as it is, in both
+    passes and in the sums over rows.  All sums are whole numbers below 2^24, exact in float32, and the results below 2^7 in every type."""
+    g = torch.Generator().manual_seed(rank)
+    m, j, p, q = 200, 77, n // 3, n - 1
+    whole = lambda *shape: torch.randint(64, 128, shape, generator=g).to(DEV, dtype)  # noqa: E731
+    zeros = lambda *shape: torch.zeros(shape, dtype=dtype, device=DEV)  # noqa: E731
+    base = zeros(n, out)
+
+    def pair(t):                       # along the first axis: a row and the same less one at j
+        row = whole(m)
+        t[0, ..., :m] = row
+        t[1, ..., :m] = row
+        t[1, ..., j] -= 1
+
+    x, a, b = zeros(n, d), zeros(1, rank, d), zeros(1, out, rank)
+    x[:, :m] = whole(n, m)
+    pair(a[0])
+    b[0, :, 0], b[0, :, 1] = 1, -1
+    for with_base in (base, None):
+        y, = run_update(x, with_base, None, a, b, 1.0, None, want="")
+        assert torch.equal(y, x[:, j:j + 1].expand(n, out))
+
+    dy, a, b = zeros(n, out), zeros(1, rank, d), zeros(1, out, rank)
+    dy[:, :m] = whole(n, m)
+    pair(b[0].T)
+    a[0, 0], a[0, 1] = 1, -1
+    _, dx = run_update(x, base, dy, a, b, 1.0, None, want="x")
+    assert torch.equal(dx, dy[:, j:j + 1].expand(n, d))
+
+    x, dy, b = zeros(n, d), zeros(n, out), zeros(1, out, rank)
+    x[p], x[q] = 1, -1
+    two = zeros(2, out)
+    pair(two)
+    dy[p], dy[q] = two
+    b[0, :m, 0] = whole(m)
+    _, da = run_update(x, base, dy, a, b, 1.0, None, want="a")
+    assert torch.equal(da[0, 0], b[0, j, 0].expand(d)) and not da[0, 1:].any()
+
+    x, dy, a = zeros(n, d), zeros(n, out), zeros(1, rank, d)
+    dy[p], dy[q] = 1, -1
+    two = zeros(2, d)
+    pair(two)
+    x[p], x[q] = two
+    a[0, 0, :m] = whole(m)
+    _, db = run_update(x, base, dy, a, b, 1.0, None, want="b")
+    assert torch.equal(db[0, :, 0], a[0, 0, j].expand(out)) and not db[0, :, 1:].any()
