@@ -11,14 +11,15 @@
 //
 // All are bound by memory: 2 rank operations for each value that is read.  So the matrix instructions are mma.sync, whose operands are gathered rows
 // from shared memory; tcgen05 would want tiles of 128 rows of one adapter and does not pay at a few operations a byte.  The long product of 16-bit types
-// multiplies them as they are (f32 sums).  The rank values are kept in parts, so that nothing is rounded to 16 bits between the products: three bf16
+// multiplies them as they are.  The rank values are kept in parts, so that nothing is rounded to 16 bits between the products: three bf16
 // parts hold the 24 bits of f32 (two would hold 16: one result in 256 then rounds to the other neighbour than f32's); two f16 parts 22, over a power of two for each
 // row in the second product, since f16's range would lose small gradients; f16 in the sums over rows and f32 everywhere have two TF32 parts, 22 bits (f16 itself
-// is exact in TF32).  f32 operands are two TF32 parts too, three products of them, added to f32 registers every few steps because the matrix instructions' own
-// sums truncate.
+// is exact in TF32).  f32 operands are two TF32 parts too, three products of them.  Matrix instructions cut their sums off instead of rounding them: the long
+// product and the sums over rows start from zero for each 16 to 64 terms and are added to f32 registers (8192 rows, bf16: one value in 4000 of the factors'
+// gradients is not the exact one rounded, one in 800 of f32 products by a library).
 //
 // Measured on one B200, rank 16, bf16, in a graph (copy rate 6.54 TB/s): 1 row 4096 to 4096 6.3 us, 64 rows over 48 adapters 4096 to 12288 15 us (f16); 8192 rows 4096 to
-// 12288 without dropout 96 us forward (470 MB: 4.9 TB/s), 83 us for dx (268 MB), 70 us for both factors' gradients (270 MB: 3.9 TB/s); dropout adds 13, 7 and 14.
+// 12288 without dropout 96 us forward (470 MB: 4.9 TB/s), 82 us for dx (268 MB), 68 us for both factors' gradients (270 MB: 4.0 TB/s); dropout adds 15, 7 and 20.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

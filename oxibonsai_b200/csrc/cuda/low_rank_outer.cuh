@@ -8,8 +8,8 @@ namespace bonsai {
 // out[r][c] (or [c][r]) = sum over the adapter's rows of p[row][r] q[row][c]; the rank values p have the scales in them.  A cluster takes 128 columns of one adapter and one product, its blocks
 // split the rows.  bf16: the rank values' three parts times q, both as ldmatrix turns them.  f16 and f32: TF32, where f16 is exact (its range would lose small rank
 // values); the two rows 2 t and 2 t + 1 of every eight are then what a thread has of a matrix instruction's axis of eight, which is how
-// ldmatrix hands out 16-bit values of q; p follows.  8192 rows, 4096 and 12288 columns, rank 16, bf16: 270 MB in 70 us, 3.9 TB/s (with two parts 63), with dropout of
-// the 4096 columns 84.
+// ldmatrix hands out 16-bit values of q; p follows.  8192 rows, 4096 and 12288 columns, rank 16, bf16: 270 MB in 68 us, 4.0 TB/s, with dropout of
+// the 4096 columns 88.
 template <typename T, int R> struct LrOuterSmem {
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   // bf16: a row's three parts side by side, whose pitch spreads eight rows over all banks; else the first parts and, kP bytes on, the second ones
@@ -136,33 +136,37 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
     const T* qp = qs(slot) + warp * 16;
     if constexpr (BF16) {
       const T* pp = (const T*)ps(slot);
+      uint32_t w[kLrOuterRows / 16][4];
 #pragma unroll
-      for (int k = 0; k < kLrOuterRows; k += 16) {
-        uint32_t w[4];
-        lr_ldm4t(w, qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
+      for (int k = 0; k < kLrOuterRows; k += 16) lr_ldm4t(w[k / 16], qp + (k + (lane & 15)) * L::kPitchQ + (lane >> 4) * 8);
 #pragma unroll
-        for (int i = 0; i < R / 16; ++i) {
+      for (int i = 0; i < R / 16; ++i) {
+        float sum[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < kLrOuterRows; k += 16) {
           const T* p = pp + (k + (lane & 7) + (lane >> 4) * 8) * L::kPitchP + i * 16 + (lane >> 3 & 1) * 8;
 #pragma unroll
           for (int part = 2; part >= 0; --part) {
             uint32_t v[4];
             lr_ldm4t(v, p + part * R);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) lr_mma16<T>(acc[i][j], v, w[2 * j], w[2 * j + 1]);
+            for (int j = 0; j < 2; ++j) lr_mma16<T>(sum[j], v, w[k / 16][2 * j], w[k / 16][2 * j + 1]);
           }
         }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[j][k];
       }
     } else {
       const uint32_t* pp = (const uint32_t*)ps(slot);
       float sum[R / 16][2][4];
-      if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < R / 16; ++i)
+      for (int i = 0; i < R / 16; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum[i][j][k] = 0.0f;
-      }
+          for (int k = 0; k < 4; ++k) sum[i][j][k] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kLrOuterRows; k += 16) {
         float v[2][2][2];             // of the first and the second eight rows: product j, rows 2 t and 2 t + 1
@@ -202,22 +206,19 @@ __global__ void __launch_bounds__(kLrThreads, LrOuterSmem<T, R>::kBlocks) lr_out
             const uint32_t lo[4] = {p[0], p[8], p[L::kPitchP], p[L::kPitchP + 8]};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float* d = F32 ? sum[i][j] : acc[i][j];
-              lr_mma8(d, lo, vh[j][0], vh[j][1]);
-              if constexpr (F32) lr_mma8(d, hi, vl[j][0], vl[j][1]);
-              lr_mma8(d, hi, vh[j][0], vh[j][1]);
+              lr_mma8(sum[i][j], lo, vh[j][0], vh[j][1]);
+              if constexpr (F32) lr_mma8(sum[i][j], hi, vl[j][0], vl[j][1]);
+              lr_mma8(sum[i][j], hi, vh[j][0], vh[j][1]);
             }
           }
         }
       }
-      if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < R / 16; ++i)
+      for (int i = 0; i < R / 16; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[i][j][k];
-      }
+          for (int k = 0; k < 4; ++k) acc[i][j][k] += sum[i][j][k];
     }
   }
   lr_wait<0>();

@@ -325,17 +325,24 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
       lr_commit();
       const T* ws = xs + M * L::kPitchX;
       if constexpr (!F32) {
+        uint32_t x[S::kWarpK / 16][4];
 #pragma unroll
-        for (int k = 0; k < S::kWarpK; k += 16) {
-          uint32_t x[4];
-          lr_ldm4(x, xs + (m0 + (lane & 15)) * L::kPitchX + kp + k + (lane >> 4) * 8);
+        for (int k = 0; k < S::kWarpK; k += 16) lr_ldm4(x[k / 16], xs + (m0 + (lane & 15)) * L::kPitchX + kp + k + (lane >> 4) * 8);
 #pragma unroll
-          for (int j = 0; j < R / 16; ++j) {
+        for (int j = 0; j < R / 16; ++j) {
+          float sum[2][4] = {};
+#pragma unroll
+          for (int k = 0; k < S::kWarpK; k += 16) {
             uint32_t w[4];
             if (BACK) lr_ldm4t(w, ws + (kp + k + (lane & 15)) * L::kPitchW + j * 16 + (lane >> 4) * 8);
             else lr_ldm4(w, ws + (j * 16 + (lane & 7) + (lane >> 4) * 8) * L::kPitchW + kp + k + (lane >> 3 & 1) * 8);
-            lr_mma16<T>(acc[2 * j], x, w[0], w[1]);
-            lr_mma16<T>(acc[2 * j + 1], x, w[2], w[3]);
+            lr_mma16<T>(sum[0], x[k / 16], w[0], w[1]);
+            lr_mma16<T>(sum[1], x[k / 16], w[2], w[3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[2 * j][i] += sum[0][i];
+            acc[2 * j + 1][i] += sum[1][i];
           }
         }
       } else {

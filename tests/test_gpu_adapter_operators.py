@@ -743,3 +743,65 @@ def test_update_rank_values_of_21_bits(n, d, out, rank, dtype):
     a[0, 0, :m] = whole(m)
     _, db = run_update(x, base, dy, a, b, 1.0, None, want="b")
     assert torch.equal(db[0, :, 0], a[0, 0, j].expand(out)) and not db[0, :, 1:].any()
+
+
+
+def _groups_that_cancel(groups, total, make, seed):
+    """[2 groups + 1, 16, ...] of `make` (groups of 16 whole numbers whose sum is a multiple of 256), the same ones negative in another order, and one that
+    leaves ``total``."""
+    g = torch.Generator().manual_seed(seed)
+    first = make(g, groups)
+    return torch.cat([first, -first[torch.randperm(groups, generator=g)], total]).flatten(0, 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, groups, cols, adapters", [(2, 8192, 40, 0), (1100, 1000, 15360, 0), (1100, 1000, 15360, 40)])
+def test_update_long_products_are_not_cut_off(n, groups, cols, adapters, dtype):
+    """Sums of products of up to 2^16 that pass 2^24 on their way and come back to 768.  What matrix instructions add between two additions in float32 stays below
+    2^24, and every group of 16 of them is a multiple of 256: such sums are exact in float32 to 2^32, in any order of groups."""
+    def make(g, count):
+        x, a = torch.randint(0, 256, (count, 16), generator=g), torch.randint(0, 128, (count, 16), generator=g) * 2 + 1
+        inverse = torch.tensor([pow(v, -1, 256) for v in a[:, 15].tolist()])
+        x[:, 15] = -(x[:, :15] * a[:, :15]).sum(1) * inverse % 256
+        return torch.stack([x, a], 2)
+
+    left = torch.zeros(1, 16, 2, dtype=torch.int64)
+    left[0, :3] = 16
+    both = _groups_that_cancel(groups, left, make, n)
+    x, a = both.unbind(1)
+    a = a.abs()
+    assert int((x * a).sum()) == 768 and int((x * a).cumsum(0).max()) > 2 ** 27
+    k, e = len(x), max(1, adapters)
+    x, a = x.to(DEV, dtype).expand(n, k).contiguous(), a.to(DEV, dtype).expand(e, 1, k).contiguous()
+    b = torch.ones(e, cols, 1, dtype=dtype, device=DEV)
+    ids = torch.arange(n, device=DEV) % e if adapters else None
+    base = torch.zeros(n, cols, dtype=dtype, device=DEV)
+    y, = run_update(x, base, None, a, b, 1.0, ids, want="")
+    assert (y == 768).all()
+    # the gradient of the rows is the same product: dy as x, b as a
+    _, dx = run_update(base, torch.zeros_like(x), x, b.transpose(1, 2).contiguous(), a.transpose(1, 2).contiguous(), 1.0, ids, want="x")
+    assert (dx == 768).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rank", [3, 64])
+def test_update_sums_over_rows_are_not_cut_off(rank, dtype):
+    """As above, over 16 400 rows whose rank values have 17 bits."""
+    def make(g, count):
+        parts = torch.randint(0, 256, (count, 16, 3), generator=g)
+        parts[:, 15, 0] = -parts[:, :15, 0].sum(1) % 256
+        return parts
+
+    left = torch.zeros(1, 16, 3, dtype=torch.int64)
+    left[0, 4, 1] = 3
+    rows = _groups_that_cancel(512, left, make, rank).to(DEV, dtype)
+    n = len(rows)
+    weight = torch.tensor([1, 256, 256], device=DEV, dtype=dtype)
+    assert float((rows.double() @ weight.double()).sum()) == 768 and float((rows.double() @ weight.double()).cumsum(0).max()) > 2 ** 28
+    ones = torch.ones(n, 40, dtype=dtype, device=DEV)
+    b = torch.zeros(1, 3, rank, dtype=dtype, device=DEV)
+    b[0, :, 1] = weight
+    _, da = run_update(ones, None, rows, torch.zeros(1, rank, 40, dtype=dtype, device=DEV), b, 1.0, None, want="a")
+    assert (da[0, 1] == 768).all() and not da[0, 2:].any()
+    _, db = run_update(rows, None, ones, b.transpose(1, 2).contiguous(), torch.zeros(1, 40, rank, dtype=dtype, device=DEV), 1.0, None, want="b")
+    assert (db[0, :, 1] == 768).all() and not db[0, :, 2:].any()
