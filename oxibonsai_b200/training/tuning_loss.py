@@ -83,8 +83,8 @@ def _preference_cpu(logps, ref, mask, beta, kind, smoothing, average, reduction)
     chosen, rejected = s.chunk(2)
     z = chosen - rejected
     if kind == "sigmoid":
-        soft = torch.nn.functional.softplus
-        each = (1 - smoothing) * soft(-beta * z, threshold=1e9) + (smoothing * soft(beta * z, threshold=1e9) if smoothing else 0.0)
+        log = torch.nn.functional.logsigmoid
+        each = (smoothing - 1) * log(beta * z) - (smoothing * log(-beta * z) if smoothing else 0.0)
     elif kind == "hinge":
         each = (1.0 - beta * z).clamp(min=0.0)
     else:

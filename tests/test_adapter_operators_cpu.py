@@ -287,3 +287,12 @@ def test_seeded_dropout_in_a_segment_that_runs_again():
         y = run(v)
         grads.append(torch.autograd.grad(y.square().sum(), v)[0])
     assert grads[0].any() and torch.equal(*grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_preference_margins_that_overflow_an_exponential(dtype):
+    x = torch.tensor([[5000.0], [-5000.0], [0.0], [0.0]], dtype=dtype, requires_grad=True)
+    for smoothing, loss, slopes in ((0.0, [0.0, 5000.0], [0.0, -1.0]), (0.25, [1250.0, 3750.0], [0.25, -0.75])):
+        got = TR.preference_loss(x, None, beta=1.0, label_smoothing=smoothing, reduction="none")
+        grad, = torch.autograd.grad(got.loss, x, torch.ones(2, dtype=dtype))
+        assert got.loss.tolist() == loss and grad.flatten().tolist() == [*slopes, *(-s for s in slopes)]
