@@ -139,7 +139,7 @@ def _policy_cpu(logps, old, ref, mask, gain, clip, kl_weight, reduction):
     far = l.detach().double() - (l.detach().double() if old is None else old[at].double())
     high, low = (g > 0) & (far > math.log1p(clip[1])), (g < 0) & (far < (math.log1p(-clip[0]) if clip[0] < 1 else -math.inf))
     cut = high | low
-    gained = torch.where(g == 0, 0.0, torch.where(cut, 0.0, step).exp() * g)
+    gained = torch.where(cut | (g == 0), 0.0, step).exp() * g         # an exponential that overflows enters neither pass
     each = -torch.where(cut, torch.where(high, 1 + clip[1] if math.isfinite(clip[1]) else 1.0, 1 - clip[0]) * g, gained)
     kl = torch.zeros_like(l)
     if ref is not None:

@@ -296,3 +296,12 @@ def test_preference_margins_that_overflow_an_exponential(dtype):
         got = TR.preference_loss(x, None, beta=1.0, label_smoothing=smoothing, reduction="none")
         grad, = torch.autograd.grad(got.loss, x, torch.ones(2, dtype=dtype))
         assert got.loss.tolist() == loss and grad.flatten().tolist() == [*slopes, *(-s for s in slopes)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("weight", [0.0, 0.5])
+def test_policy_advantages_of_zero_beside_infinite_ratios(dtype, weight):
+    x = torch.tensor([[800.0, 800.0, 800.0, -800.0]], dtype=dtype, requires_grad=True)
+    got = TR.policy_loss(x, torch.zeros_like(x), torch.tensor([[0.0, 1.0, -1.0, -1.0]]), ref_logps=x.detach(), kl_weight=weight, reduction="none")
+    grad, = torch.autograd.grad(got.loss, x, torch.ones_like(x))
+    assert got.loss.tolist() == [[0.0, pytest.approx(-1.2), float("inf"), pytest.approx(0.8)]] and grad.tolist() == [[0.0, 0.0, float("inf"), 0.0]]
