@@ -86,7 +86,7 @@ def _preference_cpu(logps, ref, mask, beta, kind, smoothing, average, reduction)
         log = torch.nn.functional.logsigmoid
         each = (smoothing - 1) * log(beta * z) - (smoothing * log(-beta * z) if smoothing else 0.0)
     elif kind == "hinge":
-        each = (1.0 - beta * z).clamp(min=0.0)
+        each = torch.where(beta * z >= 1.0, 0.0, 1.0 - beta * z)              # flat from the corner on, NaN of NaN
     else:
         each = (z - 0.5 / beta) ** 2
     loss = each.mean() if reduction == "mean" else each.sum() if reduction == "sum" else each
@@ -103,7 +103,7 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
     ``s`` the sum of ``logps - ref_logps`` over an answer (``average``: its mean, 0 of an answer without tokens) and ``z = s_chosen - s_rejected``, ``kind`` is
 
     * "sigmoid": ``(1 - label_smoothing) * -log sigmoid(beta z) + label_smoothing * -log sigmoid(-beta z)``,
-    * "hinge": ``max(0, 1 - beta z)``,
+    * "hinge": ``max(0, 1 - beta z)``, whose gradient is 0 at ``beta z = 1``,
     * "ipo": ``(z - 1 / (2 beta))^2``,
 
     and ``reduction`` is "mean" over the pairs, "sum" or "none".  Returns the loss and the rewards ``beta s`` of the chosen and of the rejected answers.  Sums

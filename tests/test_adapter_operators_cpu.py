@@ -305,3 +305,12 @@ def test_policy_advantages_of_zero_beside_infinite_ratios(dtype, weight):
     got = TR.policy_loss(x, torch.zeros_like(x), torch.tensor([[0.0, 1.0, -1.0, -1.0]]), ref_logps=x.detach(), kl_weight=weight, reduction="none")
     grad, = torch.autograd.grad(got.loss, x, torch.ones_like(x))
     assert got.loss.tolist() == [[0.0, pytest.approx(-1.2), float("inf"), pytest.approx(0.8)]] and grad.tolist() == [[0.0, 0.0, float("inf"), 0.0]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_hinge_at_its_corner(dtype):
+    for margin, slope in ((1.0, 0.0), (1.0 - 2.0 ** -24, -0.5), (1.5, 0.0)):
+        x = torch.tensor([[2 * margin], [0.0]], dtype=dtype, requires_grad=True)
+        r = TR.preference_loss(x, None, beta=0.5, kind="hinge")
+        assert float(r.loss.detach()) == max(0.0, 1.0 - margin) and torch.autograd.grad(r.loss, x)[0].flatten().tolist() == [slope, -slope]
+    assert TR.preference_loss(torch.tensor([[float("nan")], [0.0]], dtype=dtype), None, kind="hinge").loss.isnan()

@@ -805,3 +805,10 @@ def test_update_sums_over_rows_are_not_cut_off(rank, dtype):
     assert (da[0, 1] == 768).all() and not da[0, 2:].any()
     _, db = run_update(rows, None, ones, b.transpose(1, 2).contiguous(), torch.zeros(1, 40, rank, dtype=dtype, device=DEV), 1.0, None, want="b")
     assert (db[0, :, 1] == 768).all() and not db[0, :, 2:].any()
+
+
+def test_hinge_at_its_corner():
+    for kind, margin, slope in ((torch.float32, 1.0, 0.0), (torch.bfloat16, 1.0, 0.0), (torch.float32, 1.0 - 2.0 ** -24, -0.5)):
+        x = torch.tensor([[2 * margin], [0.0]], device=DEV).to(kind).requires_grad_()
+        r = TR.preference_loss(x, None, beta=0.5, kind="hinge")
+        assert float(r.loss.detach()) == 1.0 - margin and torch.autograd.grad(r.loss, x)[0].flatten().tolist() == [slope, -slope]
