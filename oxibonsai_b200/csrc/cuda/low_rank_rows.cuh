@@ -134,12 +134,13 @@ __device__ __forceinline__ void lr_set(float (*acc)[4], int h, const float* v) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) acc[q >> 1][2 * h + (q & 1)] = v[q];
 }
+// `has`: the row has an adapter; without one it is base as it is, where an addition of zeros would lose the sign of -0
 template <typename T>
-__device__ __forceinline__ void lr_get(float (*acc)[4], int h, float up, const float* base, float* v) {
+__device__ __forceinline__ void lr_get(float (*acc)[4], int h, float up, const float* base, bool has, float* v) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const float d = acc[q >> 1][2 * h + (q & 1)];
-    v[q] = LrStart<T>::kBase ? d : std::is_same<T, __half>::value ? fmaf(d, up, base[q]) : d + base[q];
+    v[q] = LrStart<T>::kBase ? d : !has ? base[q] : std::is_same<T, __half>::value ? fmaf(d, up, base[q]) : d + base[q];
   }
 }
 __device__ __forceinline__ void lr_drop(float* v, const uint4& words, unsigned limit) {
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
       for (int h = 0; h < 2; ++h) {
         if (row_of[h] < 0 || left <= 0) continue;
         float v[8];
-        lr_get<T>(acc, h, up[h], from[h], v);
+        lr_get<T>(acc, h, up[h], from[h], has, v);
         if (BACK && a.drop_y && has) lr_drop(v, dropout_words((unsigned)col >> 3, row_of[h], key), a.drop.limit);
         if (tile.group > a.groups.adapters) {
 #pragma unroll
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[8];
-          lr_get<T>(acc, h, up[h], base[h], v);
+          lr_get<T>(acc, h, up[h], base[h], true, v);
           if (BACK && a.drop_y) lr_drop(v, dropout_words((unsigned)((c * X::kGroups + q) * 32 + 8 * t) >> 3, row_of[h], key), a.drop.limit);
           lr_store8<T, true>(y[h] + q * 32, 8, v);
         }
@@ -828,7 +829,7 @@ __global__ void __launch_bounds__(kLrThreads, LrExpand<T, R, BACK>::kBlocks) lr_
       for (int h = 0; h < 2; ++h) {
         if (row_of[h] < 0 || left <= 0) continue;
         float v[8];
-        lr_get<T>(acc, h, up[h], base[h], v);
+        lr_get<T>(acc, h, up[h], base[h], has, v);
         if (BACK && a.drop_y && has) lr_drop(v, dropout_words((unsigned)(b * 32 + 8 * t) >> 3, row_of[h], key), a.drop.limit);
         if (group > a.groups.adapters) {
 #pragma unroll

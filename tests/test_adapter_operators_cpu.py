@@ -314,3 +314,10 @@ def test_hinge_at_its_corner(dtype):
         r = TR.preference_loss(x, None, beta=0.5, kind="hinge")
         assert float(r.loss.detach()) == max(0.0, 1.0 - margin) and torch.autograd.grad(r.loss, x)[0].flatten().tolist() == [slope, -slope]
     assert TR.preference_loss(torch.tensor([[float("nan")], [0.0]], dtype=dtype), None, kind="hinge").loss.isnan()
+
+
+def test_update_leaves_the_sign_of_zeros_in_rows_without_an_adapter():
+    x, base, _, a, b, scales, ids = update_inputs(9, 16, 10, 4, 3, torch.float32, "cpu", bare=0.4)
+    ids[::2], base[:, ::2] = -1, -0.0
+    y = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
+    assert torch.equal(y[ids < 0].view(torch.int32), base[ids < 0].view(torch.int32))

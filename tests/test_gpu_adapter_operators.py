@@ -812,3 +812,14 @@ def test_hinge_at_its_corner():
         x = torch.tensor([[2 * margin], [0.0]], device=DEV).to(kind).requires_grad_()
         r = TR.preference_loss(x, None, beta=0.5, kind="hinge")
         assert float(r.loss.detach()) == 1.0 - margin and torch.autograd.grad(r.loss, x)[0].flatten().tolist() == [slope, -slope]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, out", [(5, 64), (5, 33), (300, 40), (1100, 15360), (1100, 15361)])
+def test_update_leaves_the_sign_of_zeros_in_rows_without_an_adapter(n, out, dtype):
+    x, base, _, a, b, scales, ids = update_inputs(n, 16, out, 4, 3, dtype, DEV, seed=n, bare=0.4)
+    ids[::2] = -1                                  # tiles of such rows alone, and rows beside others
+    base[:, ::2] = -0.0
+    y = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
+    kind = torch.int32 if dtype == torch.float32 else torch.int16
+    assert torch.equal(y[ids < 0].view(kind), base[ids < 0].view(kind))
