@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kTuneThreads) preference_kernel(PreferenceArgs
     tune_load4<WIDE>(logps + at, n, l);
     if (ref != nullptr) tune_load4<WIDE>(ref + at, n, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[0] += m >> i & 1u ? (double)(l[i] - r[i]) : 0.0;
+    for (int i = 0; i < 4; ++i) v[0] += m >> i & 1u ? (double)l[i] - (double)r[i] : 0.0;
     v[1] += (double)__popc(m);
   });
   tune_block_sums<2>(v, room);

@@ -106,8 +106,8 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
     * "hinge": ``max(0, 1 - beta z)``, whose gradient is 0 at ``beta z = 1``,
     * "ipo": ``(z - 1 / (2 beta))^2``,
 
-    and ``reduction`` is "mean" over the pairs, "sum" or "none".  Returns the loss and the rewards ``beta s`` of the chosen and of the rejected answers.  Sums
-    are float64, the loss is float32 (float64 of float64, on the CPU), the gradient has the type of ``logps`` and is 0 at masked tokens.  Nothing is read back;
+    and ``reduction`` is "mean" over the pairs, "sum" or "none".  Returns the loss and the rewards ``beta s`` of the chosen and of the rejected answers.  Differences
+    and sums are float64, the loss is float32 (float64 of float64, on the CPU), the gradient has the type of ``logps`` and is 0 at masked tokens.  Nothing is read back;
     second derivatives are refused on the GPU."""
     what = "preference_loss"
     _check(what, logps, {"ref_logps": ref_logps}, mask)

@@ -321,3 +321,10 @@ def test_update_leaves_the_sign_of_zeros_in_rows_without_an_adapter():
     ids[::2], base[:, ::2] = -1, -0.0
     y = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
     assert torch.equal(y[ids < 0].view(torch.int32), base[ids < 0].view(torch.int32))
+
+
+def test_preference_differences_are_not_rounded():
+    logps, ref = torch.full((2, 1025), -1.0), torch.full((2, 1025), -2.0 ** -30)
+    logps[:, 0], ref[:, 0] = 1024, 0
+    logps[1], ref[1] = 0, 0
+    assert float(TR.preference_loss(logps, ref, beta=1.0).chosen_rewards[0]) == 2.0 ** -20

@@ -823,3 +823,14 @@ def test_update_leaves_the_sign_of_zeros_in_rows_without_an_adapter(n, out, dtyp
     y = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
     kind = torch.int32 if dtype == torch.float32 else torch.int16
     assert torch.equal(y[ids < 0].view(kind), base[ids < 0].view(kind))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_preference_differences_are_not_rounded(dtype):
+    """l - ref of -1 + 2^-30 a thousand times, and 1024: what is left, 2^-20, is lost where each difference is rounded to float32."""
+    logps, ref = torch.full((2, 1025), -1.0, device=DEV).to(dtype), torch.full((2, 1025), -2.0 ** -20 if dtype == torch.float16 else -2.0 ** -30, device=DEV).to(dtype)
+    logps[:, 0], ref[:, 0] = 1024, 0
+    logps[1], ref[1] = 0, 0
+    r = TR.preference_loss(logps, ref, beta=1.0)
+    step = 2.0 ** -10 if dtype == torch.float16 else 2.0 ** -20
+    assert float(r.chosen_rewards[0]) == step
