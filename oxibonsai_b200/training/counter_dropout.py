@@ -8,6 +8,7 @@ torch, so that a mask does not depend on where it is made.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ..ops import train_ops
 
@@ -61,6 +62,11 @@ def rows_of(x: torch.Tensor) -> torch.Tensor:
     return flat if flat.is_contiguous() or flat.stride(1) == 1 or flat.shape[1] == 1 and flat.stride(0) >= 1 else flat.contiguous()
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether forward-mode differentiation goes through one of these (None is none): a kernel sees their values alone."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _cuda(x, steps, seed):
     y = train_ops.dropout(rows_of(x), steps, seed)
     return y if x.dim() == 2 else y.view(x.shape)
@@ -82,7 +88,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, up):
         seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
-        if up.is_cuda and not torch.is_grad_enabled():
+        if up.is_cuda and not torch.is_grad_enabled() and not has_tangent(up):
             return _cuda(up, ctx.steps, seed), None, None
         return _Dropout.apply(up, ctx.steps, seed), None, None
 
@@ -96,7 +102,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = N
     Without a seed one is drawn from torch's CPU generator; a graph captured that way drops the same values every time, and a segment
     under :func:`checkpoint`, which is run again, needs a seed to drop the same ones.  The same seed, shape
     and ``p`` give the same mask on any device, and in :func:`low_rank_update`.  Nothing is kept between the passes but the seed.  Types are
-    float32, float16 and bfloat16 (float64 on the CPU); the result is dense, rounded once."""
+    float32, float16 and bfloat16 (float64 on the CPU); the result is dense, rounded once.  Forward-mode derivatives are refused."""
     check_p(p, "dropout")
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError("dropout: a tensor of at least one dimension is wanted")
@@ -110,6 +116,6 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = N
     steps = keep_steps(p)
     if not training or steps == 65536 or x.numel() == 0:
         return x
-    if x.is_cuda and not (x.requires_grad and torch.is_grad_enabled()):
+    if x.is_cuda and not (x.requires_grad and torch.is_grad_enabled()) and not has_tangent(x):
         return _cuda(x, steps, seed)
     return _Dropout.apply(x, steps, seed)

@@ -15,7 +15,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from ..ops import train_ops
-from .counter_dropout import check_p, check_seed, keep_steps, kept, rows_of
+from .counter_dropout import check_p, check_seed, has_tangent, keep_steps, kept, rows_of
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _CPU_TYPES = _TYPES + (torch.float64,)
@@ -77,8 +77,8 @@ class _LowRankUpdate(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, up):
-        if torch.is_grad_enabled():
-            raise RuntimeError("low_rank_update: its gradients cannot be differentiated again (create_graph=True)")
+        if torch.is_grad_enabled() or (up.is_cuda and has_tangent(up)):
+            raise RuntimeError("low_rank_update: its gradients cannot be differentiated again (create_graph=True, or a tangent of the gradient)")
         x, a, b, more, *held = ctx.saved_tensors
         grouped, scale, steps, seed, _ = ctx.how
         if scale is None:
@@ -101,7 +101,7 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 
 def _check_out(out, shape, x, others, base, wants_grad) -> None:
-    if wants_grad:
+    if wants_grad or has_tangent(out):
         raise ValueError("low_rank_update: out is for calls without gradients")
     if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"low_rank_update: out is {tuple(shape)} of {x.dtype} on {x.device}, got {tuple(out.shape)} of {out.dtype} on {out.device}")
@@ -135,7 +135,7 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     row with an infinity has results that are not finite; other rows are as without it.  ``out`` takes the result of a call
     without gradients; it may be ``base`` itself.  Between the passes the rank values are kept (4 bytes each, 6 of bfloat16, the rank rounded up to 16, 32, 64 or 128), and
     ``x``, ``a`` and ``b`` as every product keeps them.  On the GPU nothing is read back and all memory comes from torch's allocator; a pass and its
-    gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives are refused."""
+    gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives and, on the GPU, forward-mode ones are refused."""
     what = "low_rank_update"
     xs, sa, sb, device, dtype = x.shape, a.shape, b.shape, x.device, x.dtype
     single = len(sa) == 2
@@ -162,7 +162,7 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     if isinstance(scale, torch.Tensor):
         if scale.dtype != torch.float32 or scale.numel() != count or scale.dim() > 1:
             raise ValueError(f"{what}: a scale for each adapter is float32 [{count}], got {scale.dtype} of shape {tuple(scale.shape)}")
-        if scale.requires_grad and torch.is_grad_enabled():
+        if (scale.requires_grad and torch.is_grad_enabled()) or has_tangent(scale):
             raise ValueError(f"{what}: the scale has no gradient")
         if scale.device != device:
             raise ValueError(f"{what}: tensors of one device are wanted, got a scale on {scale.device} and x on {device}")
@@ -179,6 +179,7 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     steps = 65536 if dropout == 0.0 else keep_steps(check_p(dropout, what))
     seed = 0 if seed is None and steps == 65536 else check_seed(seed, device, what)
     wants_grad = torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or (base is not None and base.requires_grad))
+    wants_grad = wants_grad or (x.is_cuda and has_tangent(x, a, b, base))                # which autograd refuses
     if out is not None:
         _check_out(out, (*rows, cols), x, [t for t in (x, a, b, ids, scale, seed) if isinstance(t, torch.Tensor)], base, wants_grad)
     if n == 0:

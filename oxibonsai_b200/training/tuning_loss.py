@@ -12,7 +12,7 @@ from typing import NamedTuple
 import torch
 
 from ..ops import train_ops
-from .counter_dropout import rows_of
+from .counter_dropout import has_tangent, rows_of
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -42,7 +42,7 @@ def _check(what, logps, others, mask) -> None:
         if t.shape != logps.shape or t.dtype != logps.dtype or t.device != logps.device:
             raise ValueError(f"{what}: {name} of the shape, type and device of logps ({tuple(logps.shape)}, {logps.dtype}, {logps.device}) is wanted, got "
                              f"{tuple(t.shape)}, {t.dtype}, {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if (t.requires_grad and torch.is_grad_enabled()) or has_tangent(t):
             raise ValueError(f"{what}: {name} has no gradient: detach it")
     if mask is not None and (mask.shape != logps.shape or mask.dtype != torch.bool or mask.device != logps.device):
         raise ValueError(f"{what}: a bool mask of shape {tuple(logps.shape)} on {logps.device} is wanted, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
@@ -66,8 +66,8 @@ class _Loss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, up):
-        if torch.is_grad_enabled():
-            raise RuntimeError(f"{ctx.what}: its gradients cannot be differentiated again (create_graph=True)")
+        if torch.is_grad_enabled() or has_tangent(up):
+            raise RuntimeError(f"{ctx.what}: its gradients cannot be differentiated again (create_graph=True, or a tangent of the gradient)")
         kept, mask = ctx.saved_tensors
         return train_ops.tune_scale(kept, ctx.tokens, up.contiguous(), mask, ctx.shape, ctx.dtype), None
 
@@ -108,7 +108,7 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
 
     and ``reduction`` is "mean" over the pairs, "sum" or "none".  Returns the loss and the rewards ``beta s`` of the chosen and of the rejected answers.  Differences
     and sums are float64, the loss is float32 (float64 of float64, on the CPU), the gradient has the type of ``logps`` and is 0 at masked tokens.  Nothing is read back;
-    second derivatives are refused on the GPU."""
+    second and forward-mode derivatives are refused on the GPU."""
     what = "preference_loss"
     _check(what, logps, {"ref_logps": ref_logps}, mask)
     if logps.shape[0] % 2:
@@ -123,7 +123,7 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor | None, mask: t
         raise ValueError(f"{what}: label_smoothing is between 0 and 1 and for the sigmoid loss, got {label_smoothing} for {kind}")
     if not logps.is_cuda or logps.numel() == 0:
         return _preference_cpu(logps, ref_logps, mask, float(beta), kind, float(label_smoothing), average, reduction)
-    wants_grad = torch.is_grad_enabled() and logps.requires_grad
+    wants_grad = (torch.is_grad_enabled() and logps.requires_grad) or has_tangent(logps)
     rows, mask = rows_of(logps), _rows(mask)
     loss, rewards, kept = train_ops.preference_forward(rows, _rows(ref_logps), mask, float(beta), kind, float(label_smoothing), bool(average), reduction, wants_grad)
     return PreferenceLoss(_Loss.apply(rows, (loss, kept, mask, False, what)) if wants_grad else loss, *rewards.chunk(2))
@@ -174,13 +174,13 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     (a loss of the shape of ``logps``, 0 at masked tokens); means of nothing are NaN, with a gradient of 0.  A clipped token has no gradient but the penalty's;
     whether it is clipped is decided on ``logps - old_logps`` in float64.  An advantage of 0 leaves the penalty alone, also where the ratio is infinite.  Returns
     the loss, the mean of ``exp(gap) - gap - 1`` and the share of clipped tokens.  Sums are float64 (on the GPU over fours that are added in
-    float32), losses float32 (float64 of float64, on the CPU), the gradient has the type of ``logps``.  Between the passes four bytes for every token are kept.  Nothing is read back; second derivatives are refused on the GPU."""
+    float32), losses float32 (float64 of float64, on the CPU), the gradient has the type of ``logps``.  Between the passes four bytes for every token are kept.  Nothing is read back; second and forward-mode derivatives are refused on the GPU."""
     what = "policy_loss"
     _check(what, logps, {"old_logps": old_logps, "ref_logps": ref_logps}, mask)
     if advantages.shape not in (logps.shape[:1], logps.shape) or advantages.device != logps.device or not advantages.is_floating_point():
         raise ValueError(f"{what}: floating advantages of shape {tuple(logps.shape[:1])} or {tuple(logps.shape)} on {logps.device} are wanted, got "
                          f"{advantages.dtype} {tuple(advantages.shape)} on {advantages.device}")
-    if advantages.requires_grad and torch.is_grad_enabled():
+    if (advantages.requires_grad and torch.is_grad_enabled()) or has_tangent(advantages):
         raise ValueError(f"{what}: advantages have no gradient: detach them")
     if len(clip) != 2 or not 0.0 <= clip[0] <= 1.0 or not clip[1] >= 0.0:
         raise ValueError(f"{what}: clip is (low, high) with low from 0 to 1 and high from 0 on, got {clip}")
@@ -192,7 +192,7 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages:
     if not logps.is_cuda or logps.numel() == 0:
         return _policy_cpu(logps, old_logps, ref_logps, mask, advantages, clip, float(kl_weight), reduction)
     gain = _rows(advantages.float()) if advantages.dim() == 2 else advantages.detach().float()
-    wants_grad = torch.is_grad_enabled() and logps.requires_grad
+    wants_grad = (torch.is_grad_enabled() and logps.requires_grad) or has_tangent(logps)
     rows = rows_of(logps)
     loss, stats, kept = train_ops.policy_forward(rows, _rows(old_logps), _rows(ref_logps), _rows(mask), gain, clip, float(kl_weight), reduction, wants_grad)
     return PolicyLoss(_Loss.apply(rows, (loss, kept, None, True, what)) if wants_grad else loss, *stats.unbind())

@@ -328,3 +328,26 @@ def test_preference_differences_are_not_rounded():
     logps[:, 0], ref[:, 0] = 1024, 0
     logps[1], ref[1] = 0, 0
     assert float(TR.preference_loss(logps, ref, beta=1.0).chosen_rewards[0]) == 2.0 ** -20
+
+
+def test_forward_mode():
+    """Tangents are right or refused, and those of what has no gradient are refused."""
+    import torch.autograd.forward_ad as fw
+    x, base, _, a, b, scales, ids = update_inputs(4, 16, 8, 2, 3, torch.float64, "cpu")
+    logps, old, ref, mask, gain = loss_inputs(4, 6, torch.float64, "cpu")
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        y = TR.low_rank_update(dual(x), a, b, base=base, ids=ids, scale=scales)
+        tangent = TR.low_rank_update(torch.ones_like(x), a, b, ids=ids, scale=scales)
+        assert torch.allclose(fw.unpack_dual(y).tangent, tangent)
+        for loss in (lambda v: TR.preference_loss(v, ref, mask).loss, lambda v: TR.policy_loss(v, old, gain, mask=mask, ref_logps=ref, kl_weight=0.1).loss):
+            v = logps.clone().requires_grad_()
+            grad, = torch.autograd.grad(loss(v), v)
+            assert torch.allclose(fw.unpack_dual(loss(dual(logps))).tangent, grad.sum())
+        with pytest.raises(NotImplementedError):
+            TR.dropout(dual(x), 0.5, seed=1)
+        for call in (lambda: TR.low_rank_update(x, a, b, ids=ids, scale=dual(scales)), lambda: TR.preference_loss(logps, dual(ref), mask),
+                     lambda: TR.policy_loss(logps, dual(old), gain), lambda: TR.policy_loss(logps, old, dual(gain)), lambda: TR.policy_loss(logps, old, gain, ref_logps=dual(ref)),
+                     lambda: TR.low_rank_update(x, a, b, ids=ids, scale=scales, out=dual(torch.empty_like(base)))):
+            with pytest.raises(ValueError):
+                call()

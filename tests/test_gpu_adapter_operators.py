@@ -834,3 +834,35 @@ def test_preference_differences_are_not_rounded(dtype):
     r = TR.preference_loss(logps, ref, beta=1.0)
     step = 2.0 ** -10 if dtype == torch.float16 else 2.0 ** -20
     assert float(r.chosen_rewards[0]) == step
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor needs no requires_grad: the kernels, which would drop its tangent, refuse it wherever it comes in."""
+    import torch.autograd.forward_ad as fw
+    x, base, dy, a, b, scales, ids = update_inputs(4, 16, 8, 2, 3, torch.float32, DEV)
+    logps, old, ref, mask, gain = loss_inputs(4, 6, torch.float32, DEV)
+    update = dict(x=x, a=a, b=b, base=base, ids=ids, scale=scales)
+    policy = dict(logps=logps, old_logps=old, advantages=gain, mask=mask, ref_logps=ref, kl_weight=0.1)
+    bank = TR.AdapterBank(16, 8, rank=2, count=3, dtype=torch.float32, device=DEV)
+    v, w = x.clone().requires_grad_(), logps.clone().requires_grad_()
+    y, z, loss = TR.dropout(v, 0.5, seed=1), TR.low_rank_update(**{**update, "x": v}), TR.preference_loss(w, ref, mask).loss
+    want = TR.low_rank_update(**update), TR.policy_loss(**policy).loss, TR.dropout(x, 0.5, seed=1)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in [lambda: TR.dropout(dual(x), 0.5, seed=1), lambda: TR.preference_loss(dual(logps), ref, mask), lambda: bank(dual(x), base, ids),
+                     *(lambda k=k: TR.low_rank_update(**{**update, k: dual(update[k])}) for k in ("x", "a", "b", "base")),
+                     lambda: TR.policy_loss(**{**policy, "logps": dual(logps)})]:
+            with pytest.raises(NotImplementedError):
+                call()
+        for call in [lambda: TR.low_rank_update(**{**update, "scale": dual(scales)}), lambda: TR.preference_loss(logps, dual(ref), mask),
+                     lambda: TR.low_rank_update(**update, out=dual(torch.empty_like(base))), lambda: TR.low_rank_update(**{**update, "x": dual(x)}, out=torch.empty_like(base)),
+                     *(lambda k=k: TR.policy_loss(**{**policy, k: dual(policy[k])}) for k in ("old_logps", "advantages", "ref_logps"))]:
+            with pytest.raises(ValueError):
+                call()
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y, v, dual(x))
+        for out, leaf, up in ((z, v, dy), (loss, w, torch.ones_like(loss))):
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                torch.autograd.grad(out, leaf, dual(up))
+        got = TR.low_rank_update(**update), TR.policy_loss(**policy).loss, TR.dropout(x, 0.5, seed=1)          # others pass
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
