@@ -103,6 +103,8 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 def _check_out(out, shape, x, others, base, wants_grad) -> None:
     if wants_grad or has_tangent(out):
         raise ValueError("low_rank_update: out is for calls without gradients")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("low_rank_update: out has a gradient or a history of its own, which a result written into it would not change: detach it")
     if out.shape != shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"low_rank_update: out is {tuple(shape)} of {x.dtype} on {x.device}, got {tuple(out.shape)} of {out.dtype} on {out.device}")
     if out.numel() == 0:
@@ -133,7 +135,7 @@ def low_rank_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: tor
     Sums are float32 whatever the inputs, the rank values keep 22 bits (24 of bfloat16), results and gradients are rounded once.  How sums are split goes by the
     sizes of the call: a row's last bits may differ between batches of different sizes, within a batch they do not depend on its place or the other rows.  A
     row with an infinity has results that are not finite; other rows are as without it.  ``out`` takes the result of a call
-    without gradients; it may be ``base`` itself.  Between the passes the rank values are kept (4 bytes each, 6 of bfloat16, the rank rounded up to 16, 32, 64 or 128), and
+    without gradients and has none itself; it may be ``base``.  Between the passes the rank values are kept (4 bytes each, 6 of bfloat16, the rank rounded up to 16, 32, 64 or 128), and
     ``x``, ``a`` and ``b`` as every product keeps them.  On the GPU nothing is read back and all memory comes from torch's allocator; a pass and its
     gradients can be captured into a CUDA graph as those of :func:`linear_cross_entropy` can.  Second derivatives and, on the GPU, forward-mode ones are refused."""
     what = "low_rank_update"

@@ -351,3 +351,15 @@ def test_forward_mode():
                      lambda: TR.low_rank_update(x, a, b, ids=ids, scale=scales, out=dual(torch.empty_like(base)))):
             with pytest.raises(ValueError):
                 call()
+
+
+def test_update_out_with_a_history_is_refused():
+    x, base, _, a, b, scales, ids = update_inputs(5, 12, 7, 4, 2, torch.float32, "cpu")
+    w = torch.ones(5, 7, requires_grad=True)
+    for out in (w, w * 2, w[:]):
+        with pytest.raises(ValueError):
+            TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=out)
+    assert torch.equal(w.detach(), torch.ones_like(w))
+    want = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
+    with torch.no_grad():
+        assert torch.equal(TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=w), want)

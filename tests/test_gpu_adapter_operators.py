@@ -866,3 +866,15 @@ def test_forward_mode_is_refused():
                 torch.autograd.grad(out, leaf, dual(up))
         got = TR.low_rank_update(**update), TR.policy_loss(**policy).loss, TR.dropout(x, 0.5, seed=1)          # others pass
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_update_out_with_a_history_is_refused_on_the_gpu():
+    x, base, _, a, b, scales, ids = update_inputs(5, 12, 7, 4, 2, torch.float32, DEV)
+    w = torch.ones(5, 7, device=DEV, requires_grad=True)
+    for out in (w, w * 2, w[:], (w * 2).T.contiguous().T[:, :]):
+        with pytest.raises(ValueError):
+            TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=out)
+    assert torch.equal(w.detach(), torch.ones_like(w))
+    want = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
+    with torch.no_grad():
+        assert torch.equal(TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=w), want)
