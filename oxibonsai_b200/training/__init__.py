@@ -44,7 +44,11 @@ class LoraConfig:
 
 
 class LoraAdapter(torch.nn.Module):
-    """``delta(x) = scale * B (A x)`` with A ~ N(0, 1/r) and B = 0, so a fresh adapter is a no-op."""
+    """``delta(x) = scale * B (A x)`` with A ~ N(0, 1/r) and B = 0, so a fresh adapter is a no-op.
+
+    ``seed`` of a call names its dropout mask as that of :func:`dropout` does: an integer, or an int64 tensor on the device of ``x``, which a captured graph reads at
+    each replay.  Without one a mask is drawn for each call, by ``fused`` adapters from torch's CPU generator, so that a graph that is captured without a seed
+    drops the same values in every replay; by others from the generator of the device.  Give different adapters different seeds."""
 
     def __init__(self, in_features: int, out_features: int, config: LoraConfig, seed: int = 0):
         super().__init__()
@@ -53,18 +57,20 @@ class LoraAdapter(torch.nn.Module):
         self.A = torch.nn.Parameter(torch.randn(config.rank, in_features, generator=g) / math.sqrt(config.rank))
         self.B = torch.nn.Parameter(torch.zeros(out_features, config.rank))
 
-    def _fused(self, x: torch.Tensor, base_out: torch.Tensor | None) -> torch.Tensor:
-        return low_rank_update(x, self.A, self.B, base=base_out, scale=self.config.scale, dropout=self.config.dropout if self.training else 0.0)
+    def _fused(self, x: torch.Tensor, base_out: torch.Tensor | None, seed: int | torch.Tensor | None) -> torch.Tensor:
+        return low_rank_update(x, self.A, self.B, base=base_out, scale=self.config.scale, dropout=self.config.dropout if self.training else 0.0, seed=seed)
 
-    def apply_delta(self, x: torch.Tensor) -> torch.Tensor:
+    def apply_delta(self, x: torch.Tensor, seed: int | torch.Tensor | None = None) -> torch.Tensor:
         if self.config.fused:
-            return self._fused(x, None)
+            return self._fused(x, None, seed)
         if self.training and self.config.dropout > 0:
-            x = F.dropout(x, self.config.dropout)
+            x = F.dropout(x, self.config.dropout) if seed is None else dropout(x, self.config.dropout, seed=seed)
         return (x @ self.A.T) @ self.B.T * self.config.scale
 
-    def forward(self, x: torch.Tensor, base_out: torch.Tensor) -> torch.Tensor:
-        return self._fused(x, base_out) if self.config.fused else base_out + self.apply_delta(x)
+    def forward(self, x: torch.Tensor, base_out: torch.Tensor, seed: int | torch.Tensor | None = None) -> torch.Tensor:
+        if self.config.fused:
+            return self._fused(x, base_out, seed)
+        return base_out + (self.apply_delta(x) if seed is None else self.apply_delta(x, seed))
 
     def param_count(self) -> int:
         return self.A.numel() + self.B.numel()
@@ -93,9 +99,9 @@ class LoraRegistry:
     def get(self, module: str) -> LoraAdapter | None:
         return self.adapters.get(module)
 
-    def apply_adapter(self, module: str, x: torch.Tensor, base_out: torch.Tensor) -> torch.Tensor:
+    def apply_adapter(self, module: str, x: torch.Tensor, base_out: torch.Tensor, seed: int | torch.Tensor | None = None) -> torch.Tensor:
         a = self.adapters.get(module)
-        return base_out if a is None else a(x, base_out)
+        return base_out if a is None else a(x, base_out) if seed is None else a(x, base_out, seed=seed)
 
     def adapter_count(self) -> int:
         return len(self.adapters)

@@ -363,3 +363,21 @@ def test_update_out_with_a_history_is_refused():
     want = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
     with torch.no_grad():
         assert torch.equal(TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=w), want)
+
+
+def test_adapter_takes_a_seed():
+    config = dict(rank=4, alpha=6.0, dropout=0.5)
+    fused, plain = (TR.LoraAdapter(12, 7, TR.LoraConfig(**config, fused=f)).double() for f in (True, False))
+    torch.nn.init.normal_(fused.B)
+    plain.load_state_dict(fused.state_dict())
+    x, base = torch.randn(5, 12, dtype=torch.float64), torch.randn(5, 7, dtype=torch.float64)
+    want = TR.low_rank_update(TR.dropout(x, 0.5, seed=9), fused.A, fused.B, base=base, scale=1.5)
+    for adapter in (fused, plain):
+        registry = TR.LoraRegistry()
+        registry.adapters["attn_q"] = adapter
+        for seed in (9, torch.tensor(9)):
+            assert torch.allclose(adapter(x, base, seed=seed), want) and torch.allclose(base + adapter.apply_delta(x, seed=seed), want)
+            assert torch.allclose(registry.apply_adapter("attn_q", x, base, seed=seed), want)
+        assert not torch.allclose(adapter(x, base, seed=10), want)
+        adapter.eval()
+        assert torch.allclose(adapter(x, base, seed=9), adapter(x, base))

@@ -878,3 +878,32 @@ def test_update_out_with_a_history_is_refused_on_the_gpu():
     want = TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales)
     with torch.no_grad():
         assert torch.equal(TR.low_rank_update(x, a, b, base=base, ids=ids, scale=scales, out=w), want)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_adapter_with_a_seed_in_a_graph(fused):
+    adapter = TR.LoraAdapter(64, 48, TR.LoraConfig(rank=4, fused=fused, dropout=0.5)).to(DEV)
+    torch.nn.init.normal_(adapter.B)
+    x, base, seed = torch.randn(33, 64, device=DEV), torch.zeros(33, 48, device=DEV), torch.tensor(1, device=DEV)
+
+    def call(v):
+        y = adapter(v, base, seed=seed)
+        return y.detach(), torch.autograd.grad(y.sum(), v)[0]
+
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        call(x.clone().requires_grad_())
+    torch.cuda.current_stream().wait_stream(warm)
+    v = x.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call(v)
+    seen = []
+    for k in (1, 9):
+        seed.fill_(k)
+        graph.replay()
+        seen.append(held[0].clone())
+        want = call(x.clone().requires_grad_())
+        assert all(torch.equal(p, q) for p, q in zip(held, want))
+    assert not torch.equal(*seen)
