@@ -15,6 +15,7 @@ ratios) run kernels of their own there.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass, field
 from typing import Callable, Iterable, Sequence
@@ -470,10 +471,30 @@ class LoraTrainer:
 
 
 # ---- gradient checkpointing ----------------------------------------------------------------------------------------------------------------
+class _Generators:
+    """torch's generators as they stand now, of the CPU and of a tensor's device; ``again()`` puts them there for a segment that runs a second time, and
+    back behind it.  While a graph is captured the device's cannot be read or set, and stays out."""
+
+    def __init__(self, x: torch.Tensor):
+        self.cpu = torch.get_rng_state()
+        self.device = x.device if x.is_cuda and not torch.cuda.is_current_stream_capturing() else None
+        self.cuda = None if self.device is None else torch.cuda.get_rng_state(self.device)
+
+    @contextlib.contextmanager
+    def again(self):
+        cuda = self.cuda is not None and not torch.cuda.is_current_stream_capturing()
+        with torch.random.fork_rng(devices=[self.device] if cuda else []):
+            torch.set_rng_state(self.cpu)
+            if cuda:
+                torch.cuda.set_rng_state(self.cuda, self.device)
+            yield
+
+
 class _CheckpointFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, fn, x):
         ctx.fn = fn
+        ctx.drawn = _Generators(x)
         ctx.save_for_backward(x)
         with torch.no_grad():
             return fn(x)
@@ -482,7 +503,7 @@ class _CheckpointFn(torch.autograd.Function):
     def backward(ctx, grad_out):
         (x,) = ctx.saved_tensors
         x = x.detach().requires_grad_(True)
-        with torch.enable_grad():
+        with torch.enable_grad(), ctx.drawn.again():
             y = ctx.fn(x)
         params = [p for p in getattr(ctx.fn, "parameters", lambda: [])() if p.requires_grad]
         grads = torch.autograd.grad(y, [x] + params, grad_out, allow_unused=True)
@@ -493,7 +514,9 @@ class _CheckpointFn(torch.autograd.Function):
 
 
 def checkpoint(fn, x: torch.Tensor) -> torch.Tensor:
-    """Runs ``fn(x)`` keeping only ``x``; the segment is recomputed during the backward pass."""
+    """Runs ``fn(x)`` keeping only ``x``; the segment is recomputed during the backward pass, with torch's generators (the CPU's, and that of the device of
+    ``x``) as they stood before it: what it draws, a dropout mask say, it draws again.  In a captured graph that holds for what is drawn from the CPU's
+    generator and for masks with a seed."""
     return _CheckpointFn.apply(fn, x)
 
 

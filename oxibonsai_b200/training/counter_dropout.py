@@ -99,9 +99,8 @@ def dropout(x: torch.Tensor, p: float = 0.5, seed: int | torch.Tensor | None = N
 
     ``seed``: an integer, or an int64 tensor on the device of ``x``, which is read when the kernel runs: a captured graph takes a new mask
     in each replay if the program changes the tensor in between (not between a pass and its backward pass, where autograd reports the change).
-    Without a seed one is drawn from torch's CPU generator; a graph captured that way drops the same values every time, and a segment
-    under :func:`checkpoint`, which is run again, needs a seed to drop the same ones.  The same seed, shape
-    and ``p`` give the same mask on any device, and in :func:`low_rank_update`.  Nothing is kept between the passes but the seed.  Types are
+    Without a seed one is drawn from torch's CPU generator; a graph captured that way drops the same values every time.  A segment
+    under :func:`checkpoint`, which is run again, draws the same one again.  The same seed, shape and ``p`` give the same mask on any device, and in :func:`low_rank_update`.  Nothing is kept between the passes but the seed.  Types are
     float32, float16 and bfloat16 (float64 on the CPU); the result is dense, rounded once.  Forward-mode derivatives are refused."""
     check_p(p, "dropout")
     if not isinstance(x, torch.Tensor) or x.dim() < 1:

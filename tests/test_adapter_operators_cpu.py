@@ -381,3 +381,33 @@ def test_adapter_takes_a_seed():
         assert not torch.allclose(adapter(x, base, seed=10), want)
         adapter.eval()
         assert torch.allclose(adapter(x, base, seed=9), adapter(x, base))
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_adapter_in_a_segment_that_runs_again(fused):
+    """The update is linear in x: the product of x and its gradient is the sum of the results, with the same mask in both passes alone."""
+    adapter = TR.LoraAdapter(12, 7, TR.LoraConfig(rank=4, fused=fused, dropout=0.5)).double()
+    torch.nn.init.normal_(adapter.B)
+    x, base = torch.rand(5, 12, dtype=torch.float64) + 0.5, torch.zeros(5, 7, dtype=torch.float64)
+
+    class Segment(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.adapter = adapter
+
+        def forward(self, t):
+            return self.adapter(t, base)
+
+    for run in (*(lambda v, s=s: TR.checkpoint(lambda t: adapter(t, base, seed=s), v) for s in (None, 5, torch.tensor(6))), TR.CheckpointedPipeline([Segment()])):
+        v = x.clone().requires_grad_()
+        y = run(v)
+        drawn = torch.get_rng_state()
+        grad, = torch.autograd.grad(y.sum(), v)
+        assert torch.equal(drawn, torch.get_rng_state())                  # the second run draws nothing new
+        assert abs(float(y.detach().sum() - (grad * x).sum())) <= 1e-9
+    with_parameters = TR.CheckpointedPipeline([Segment()])
+    v = x.clone().requires_grad_()
+    y = with_parameters(v)
+    adapter.zero_grad()
+    y.sum().backward()
+    assert abs(float((adapter.B.grad * adapter.B).sum().detach() - y.detach().sum())) <= 1e-9

@@ -907,3 +907,49 @@ def test_adapter_with_a_seed_in_a_graph(fused):
         want = call(x.clone().requires_grad_())
         assert all(torch.equal(p, q) for p, q in zip(held, want))
     assert not torch.equal(*seen)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_adapter_in_a_segment_that_runs_again_on_the_gpu(fused):
+    """The update is linear in x: the product of x and its gradient is the sum of the results, with the same mask in both passes alone."""
+    adapter = TR.LoraAdapter(64, 48, TR.LoraConfig(rank=4, fused=fused, dropout=0.5)).to(DEV)
+    torch.nn.init.normal_(adapter.B)
+    x, base = torch.rand(33, 64, device=DEV) + 0.5, torch.zeros(33, 48, device=DEV)
+    for seed in (None, 5, torch.tensor(6, device=DEV)):
+        v = x.clone().requires_grad_()
+        y = TR.checkpoint(lambda t: adapter(t, base, seed=seed), v)
+        drawn = torch.cuda.get_rng_state(), torch.get_rng_state()
+        grad, = torch.autograd.grad(y.sum(), v)
+        assert all(torch.equal(p, q) for p, q in zip(drawn, (torch.cuda.get_rng_state(), torch.get_rng_state())))
+        size = float(((x @ adapter.A.T).abs() @ adapter.B.abs().T).sum())
+        assert abs(float(y.detach().sum() - (grad * x).sum())) <= 2.0 ** -16 * size           # 2^12 sums of 64 values in float32
+
+
+def test_a_segment_that_runs_again_in_a_graph():
+    """Captured: a fused adapter draws its seed from the CPU's generator, which both runs see alike; one with a seed in a tensor follows the tensor."""
+    adapter = TR.LoraAdapter(64, 48, TR.LoraConfig(rank=4, fused=True, dropout=0.5)).to(DEV)
+    torch.nn.init.normal_(adapter.B)
+    x, base, seed = torch.rand(33, 64, device=DEV) + 0.5, torch.zeros(33, 48, device=DEV), torch.tensor(1, device=DEV)
+
+    def call(v, s):
+        y = TR.checkpoint(lambda t: adapter(t, base, seed=s), v)
+        return y.detach(), torch.autograd.grad(y.sum(), v)[0]
+
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        call(x.clone().requires_grad_(), None)
+    torch.cuda.current_stream().wait_stream(warm)
+    size = float(((x @ adapter.A.T).abs() @ adapter.B.abs().T).sum())
+    for s in (None, seed):
+        v = x.clone().requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, grad = call(v, s)
+        seen = []
+        for k in (1, 9):
+            seed.fill_(k)
+            graph.replay()
+            assert abs(float(y.sum() - (grad * x).sum())) <= 2.0 ** -16 * size
+            seen.append(y.clone())
+        assert torch.equal(*seen) == (s is None)
