@@ -148,16 +148,16 @@ def _policy_cpu(logps, old, ref, mask, gain, clip, kl_weight, reduction):
         if kl_weight:
             each = each + kl_weight * kl
     per = logps.new_zeros(logps.shape, dtype=kind).index_put(at, each)
-    size = live.sum(1)
+    size, total = live.sum(1), per.sum(1, dtype=torch.float64)
     if reduction == "none":
         loss = per
     elif reduction == "sum":
-        loss = per.sum()
+        loss = total.sum()
     elif reduction == "tokens":
-        loss = per.sum() / size.sum()
+        loss = total.sum() / size.sum()
     else:
-        loss = (per.sum(1) / size.clamp(min=1)).sum() / (size > 0).sum()
-    return PolicyLoss(loss, kl.detach().sum() / size.sum(), cut.to(kind).sum() / size.sum())
+        loss = (total / size.clamp(min=1)).sum() / (size > 0).sum()
+    return PolicyLoss(loss.to(kind), (kl.detach().sum(dtype=torch.float64) / size.sum()).to(kind), (cut.sum(dtype=torch.float64) / size.sum()).to(kind))
 
 
 def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor | None, advantages: torch.Tensor, mask: torch.Tensor | None = None,

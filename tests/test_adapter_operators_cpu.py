@@ -411,3 +411,14 @@ def test_adapter_in_a_segment_that_runs_again(fused):
     adapter.zero_grad()
     y.sum().backward()
     assert abs(float((adapter.B.grad * adapter.B).sum().detach() - y.detach().sum())) <= 1e-9
+
+
+@pytest.mark.parametrize("reduction", ["tokens", "sequences", "sum"])
+def test_policy_sums_are_float64(reduction):
+    """Losses of 2^27, 1 and -2^27: the 1 is lost where they are added in float32.  Gradients are rounded three times, by 2^-24 each."""
+    logps = torch.zeros(2, 3, requires_grad=True)
+    gain = torch.tensor([[-2.0 ** 27, -1.0, 2.0 ** 27]] * 2)
+    loss = TR.policy_loss(logps, None, gain, reduction=reduction).loss
+    each = 1.0 if reduction == "sum" else 1 / 6
+    assert loss.dtype == torch.float32 and float(loss.detach()) == float(torch.tensor(2 * each, dtype=torch.float32))
+    assert torch.allclose(torch.autograd.grad(loss, logps)[0], -gain * each, rtol=2.0 ** -22, atol=0.0)
