@@ -19,7 +19,7 @@
 // gradients is not the exact one rounded, one in 800 of f32 products by a library).
 //
 // Measured on one B200, rank 16, bf16, in a graph (copy rate 6.54 TB/s): 1 row 4096 to 4096 6.3 us, 64 rows over 48 adapters 4096 to 12288 15 us (f16); 8192 rows 4096 to
-// 12288 without dropout 96 us forward (470 MB: 4.9 TB/s), 82 us for dx (268 MB), 68 us for both factors' gradients (270 MB: 4.0 TB/s); dropout adds 15, 7 and 20.
+// 12288 without dropout 96 us forward (470 MB: 4.9 TB/s), 82 us for dx (268 MB), 68 us for both factors' gradients (270 MB: 4.0 TB/s); dropout adds 15, 5 and 21.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

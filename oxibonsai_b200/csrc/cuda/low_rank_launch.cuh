@@ -95,10 +95,11 @@ static cudaError_t lr_outer_r(const LrOuterArgs& a, cudaStream_t st) {
   using L = LrOuterSmem<T, R>;
   const long long clusters = (long long)(a.blocks[0] + a.blocks[1]) * a.groups.adapters;
   const long long steps = (a.groups.n / a.groups.adapters + kLrOuterRows - 1) / kLrOuterRows;
-  // How the rows are split goes by both products, wanted or not: a gradient has the same bits alone and beside the other.  Columns that are dropped take twice
-  // the others' time: many short blocks then even out.
+  // How the rows are split goes by both products, wanted or not: a gradient has the same bits alone and beside the other.  Dropped columns, which take longer, have no
+  // rule of their own: clusters of eight from 2048 rows on, which was one, took 176 us where this takes 179 (all gradients of 8192 rows, 4096 to 12288,
+  // rank 16, bf16), but 101 and 95 of 4096 rows, 220 and 206 of three adapters, 721 and 578 of three in f32.
   const long long both = ((a.width[0] + kLrOuterCols - 1) / kLrOuterCols + (a.width[1] + kLrOuterCols - 1) / kLrOuterCols) * (long long)a.groups.adapters;
-  const int ranks = a.drop_x && steps >= 32 ? 8 : lr_ranks_for(both, steps, 148 * L::kBlocks, 4);
+  const int ranks = lr_ranks_for(both, steps, 148 * L::kBlocks, 4);
   return lr_launch<lr_outer_kernel<T, R>>(clusters, ranks, L::kBytes, st, a);
 }
 

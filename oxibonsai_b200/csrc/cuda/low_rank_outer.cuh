@@ -9,7 +9,7 @@ namespace bonsai {
 // split the rows.  bf16: the rank values' three parts times q, both as ldmatrix turns them.  f16 and f32: TF32, where f16 is exact (its range would lose small rank
 // values); the two rows 2 t and 2 t + 1 of every eight are then what a thread has of a matrix instruction's axis of eight, which is how
 // ldmatrix hands out 16-bit values of q; p follows.  8192 rows, 4096 and 12288 columns, rank 16, bf16: 270 MB in 68 us, 4.0 TB/s, with dropout of
-// the 4096 columns 88.
+// the 4096 columns 89.
 template <typename T, int R> struct LrOuterSmem {
   static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   // bf16: a row's three parts side by side, whose pitch spreads eight rows over all banks; else the first parts and, kP bytes on, the second ones
