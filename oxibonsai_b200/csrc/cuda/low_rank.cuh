@@ -32,9 +32,16 @@
 namespace bonsai {
 
 constexpr int kLrThreads = 256, kLrWarps = 8, kLrSelf = 256;      // kLrSelf: rows that blocks group by themselves
-// From so many rows and results on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.  bf16, rank 16,
-// us in one kernel and in two: 2000 rows 4096 to 4096 19 and 23, 4000 rows 34 and 37, 2000 rows 4096 to 12288 38 and 34, 8000 rows 4096 to 4096 67 and 49,
-// to 12288 143 and 94.
+// From so many rows and results on the two products are kernels of their own: each is then a stream over memory with as many blocks as it likes.  Forward, us in
+// one kernel and in two, of rows with 4096 values:
+//                  1100 to 4096   2000 to 4096   4000 to 4096   2000 to 12288   8000 to 4096
+//   bf16 rank 16      12    16       17    20       32    34       37    32        66    48
+//   f16 rank 16       13    16       17    20       33    34       38    32        66    49
+//   bf16 rank 64      22    31       38    37       74    51       82    66       136    91
+//   bf16 rank 128     42    64       76    72      157   133      199   174       287   252
+//   f32 rank 16       27    33       45    42       85    78       86    80       162   143
+//   f32 rank 128     129   162      260   203      520   391      559   404       904   767
+// The border, 2^24 results, is that of 16-bit types at rank 16; larger ranks and f32 would have theirs at 2^23.
 constexpr int kLrSplit = 1024;
 inline bool lr_split_at(int n, int cols) { return n >= kLrSplit && (long long)n * cols >= 1 << 24; }
 // dynamic shared memory of a block, of each of two or three on an SM
@@ -303,7 +310,8 @@ __device__ __forceinline__ void lr_copy8(T* dst, const T* src, int left, bool ve
 
 // Rows at odd addresses into shared memory: C columns of rows r < ROWS from `from(r)` (null: zeros), `left` of them there (`any`: an address that is).  A warp takes
 // a row at a time, so that neighbouring lanes take neighbouring values; only those of f32 are wide enough for cp.async.  8000 rows 4095 to 4097 values, bf16, rank 16:
-// with eights to a thread 286 us forward and 348 backward, with this and the rows of lr_expand_kernel 183 and 244 (of 4096 values 62 and 99).
+// with eights to a thread 286 us forward and 348 backward, with this and the rows of lr_expand_kernel 183 and 244, calls timed one behind another; in a graph 156 and 229 (of
+// 4096 values 48 and 92).
 template <typename T, int ROWS, int C, typename From>
 __device__ __forceinline__ void lr_copy_rows(T* to, int pitch, int left, const T* any, From from) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

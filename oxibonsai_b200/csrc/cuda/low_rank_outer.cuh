@@ -17,7 +17,7 @@ template <typename T, int R> struct LrOuterSmem {
   static constexpr int kP = kLrOuterRows * kPitchP * (kBf16 ? 2 : 4);
   static constexpr int kStage = kLrOuterRows * kPitchQ * (int)sizeof(T) + (kBf16 ? 1 : 2) * kP;
   static constexpr int kSum = R * kLrOuterCols * 4;
-  // bf16 of rank 64 takes two stages, which leave room for a second block: 8192 rows to 12288 columns in 180 us, with three stages and one block 217
+  // bf16 of rank 64 takes two stages, which leave room for a second block: 8192 rows to 12288 columns in 198 us, with three stages and one block 221
   static constexpr int kStages = 3 * kStage <= (kBf16 && R == 64 ? kLrSmemHalf : kLrSmemMost) ? 3 : 2;
   static constexpr int kBytes = kStages * kStage > kSum ? kStages * kStage : kSum;
   static constexpr int kBlocks = kBytes <= kLrSmemThird && R <= 32 ? 3 : kBytes <= kLrSmemHalf && R <= 64 ? 2 : 1;            // on an SM

@@ -547,8 +547,8 @@ __global__ void __launch_bounds__(kLrThreads, LrSmem<T, R, M, BACK, SPLIT>::kBlo
 
 // ---- the second product of many rows ---------------------------------------------------------------------------------------------------------
 // y = base + s W2 h, h by place.  A warp takes 16 rows of one adapter and walks over blocks of columns, its own lanes' pieces of base two blocks ahead in shared
-// memory; warps do not wait for one another.  8192 rows to 12288 values, rank 16, bf16: 402 MB in 74 us, 5.4 TB/s, 18 % of the issue slots (41 M
-// instructions with everything checked took 95 us, 12.5 M in whole blocks of known rank 74).  The next kernel is not let in early, as in dropout.cu (a training step of
+// memory; warps do not wait for one another.  8192 rows to 12288 values, rank 16, bf16: 402 MB in 79 us, 5.1 TB/s, 19 % of the issue slots (41 M
+// instructions with everything checked took 95 us, 12.5 M in whole blocks of known rank 74, 13.6 M with the third part of the rank values 79).  The next kernel is not let in early, as in dropout.cu (a training step of
 // 8192 rows: 327 us, 289 without).
 template <typename T, int R, bool BACK> struct LrExpand {
   static constexpr int kGroups = sizeof(T) == 4 ? 2 : 4, kCols = 32 * kGroups;         // of a block of columns

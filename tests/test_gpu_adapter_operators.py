@@ -921,7 +921,7 @@ def test_adapter_in_a_segment_that_runs_again_on_the_gpu(fused):
         drawn = torch.cuda.get_rng_state(), torch.get_rng_state()
         grad, = torch.autograd.grad(y.sum(), v)
         assert all(torch.equal(p, q) for p, q in zip(drawn, (torch.cuda.get_rng_state(), torch.get_rng_state())))
-        size = float(((x @ adapter.A.T).abs() @ adapter.B.abs().T).sum())
+        size = float(((x @ adapter.A.T).abs() @ adapter.B.abs().T).sum().detach())
         assert abs(float(y.detach().sum() - (grad * x).sum())) <= 2.0 ** -16 * size           # 2^12 sums of 64 values in float32
 
 
@@ -940,7 +940,7 @@ def test_a_segment_that_runs_again_in_a_graph():
     with torch.cuda.stream(warm):
         call(x.clone().requires_grad_(), None)
     torch.cuda.current_stream().wait_stream(warm)
-    size = float(((x @ adapter.A.T).abs() @ adapter.B.abs().T).sum())
+    size = float(((x @ adapter.A.T).abs() @ adapter.B.abs().T).sum().detach())
     for s in (None, seed):
         v = x.clone().requires_grad_()
         graph = torch.cuda.CUDAGraph()
